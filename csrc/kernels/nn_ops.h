@@ -140,6 +140,65 @@ int geeps_bn_forward_noalloc(const void* x, void* y, const float* gamma, const f
                              float* running_mean, float* running_var, long long P, int C, long long ldx,
                              long long ldy, float eps, float momentum, int relu, void* stream);
 
+// ---- norms over the channels of a row, before and after a residual block (no counterpart in the reference) ----
+// One row = one pixel or token.  kind: 0 none, 1 LayerNorm, 2 RMSNorm.  weight / bias: C floats or NULL (1 / 0).  stats:
+// {mean, rstd} of every row, written forward (or NULL there) and read backward.  dweight / dbias: C floats or NULL.
+typedef struct GeepsNorm {
+  const float* weight;
+  const float* bias;
+  float* stats;
+  float* dweight;
+  float* dbias;
+  float eps;
+  int kind;
+} GeepsNorm;
+// Forward:  out = res + scale * g * post(x), y = pre(out); without x: y = pre(res).  g = gate or its sigmoid, one row a pixel
+// (gate_rows = rows) or one for rows / gate_rows neighbouring pixels (an image); no gate: 1.
+// Backward: dres = dout + pre'(dy) (dout may be NULL with pre), dx, dgate and the parameters' gradients (each or NULL) of
+// the join; without x, out holds the norm's input.  Pitches in elements.  stream_fp32: res, out, dout and dres are fp32,
+// else bf16; block_fp32 (with stream_fp32 only): x, y, gate, dy, dx and dgate.  An output may be the very same rows as an
+// input of its size; any other overlap of an output with another operand is refused.  Rows are any number (none: the
+// parameters' gradients are zeros), C is 1 to 16384, every address and pitch will do.  work: geeps_residual_work() floats,
+// private to the call while it runs.  mode: 1 for a norm alone (no x), 2 for a join, 3 for a join with a norm behind it.
+#define GEEPS_ERR_NORM_CHANNELS (-10)
+#define GEEPS_ERR_NORM_GATE (-11)
+#define GEEPS_ERR_NORM_OVERLAP (-12)
+typedef struct GeepsResidual {
+  const void *x, *res, *gate;
+  void *out, *y;
+  const void *dout, *dy;
+  void *dx, *dres, *dgate;
+  const float* scale;
+  float* dscale;
+  float* work;
+  GeepsNorm post, pre;
+  long long rows, gate_rows;
+  long long ldx, ldres, ldgate, ldout, ldy, lddout, lddy, lddx, lddres, lddgate;
+  int C, mode, stream_fp32, block_fp32, sigmoid;
+} GeepsResidual;
+long long geeps_residual_work(long long rows, long long gate_rows, int C, int mode);
+int geeps_residual_forward(const GeepsResidual* p, void* stream);
+int geeps_residual_backward(const GeepsResidual* p, void* stream);
+// launch shape (host arithmetic only): vectors a thread, threads a row, rows a block at a time, blocks
+int geeps_norm_shape(long long rows, int C, int* out);
+
+// ---- clipping of gradients by their global norm (the reference's solver had it in its absent Caffe application) ----
+// norm = sqrt(sum over all tensors of g^2), c = norm > max_norm ? max_norm / norm : 1, dst = c * g; dst NULL: in place, and
+// then nothing is written while c is 1.  result: {norm, c}.  Tensors are dense, fp32 or bf16 each; dst[i] has src[i]'s
+// count and shares no memory with any src but src[i] itself, type and all.  The squares are added in 64 bits, in an order that
+// depends on the counts alone.  work: geeps_clip_work() doubles, private to the call while it runs.
+#define GEEPS_ERR_CLIP_OVERLAP (-13)
+typedef struct GeepsTensors {
+  long long n;
+  void* const* ptr;
+  const long long* count;
+  const unsigned char* fp32;
+  const long long* order;       // the tensors' numbers by ascending address
+} GeepsTensors;
+long long geeps_clip_work(const GeepsTensors* src);
+int geeps_clip_gradients(const GeepsTensors* src, const GeepsTensors* dst, double max_norm, float* result, double* work,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

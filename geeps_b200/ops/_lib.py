@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -127,6 +128,20 @@ class U8Transform(C.Structure):
                 ("B", "C", "Hin", "Win", "H", "W", "S", "Hs", "Ws", "Cpad")] + [("mean", C.c_float * 4), ("scale", C.c_float)]
 
 
+# GeepsResidual (csrc/kernels/nn_ops.h) as packed bytes: x, res, gate, out, y, dout, dy, dx, dres, dgate, scale, dscale, work;
+# two norms of weight, bias, stats, dweight, dbias, eps, kind; rows, gate_rows, ten pitches; C, mode, stream_fp32, block_fp32, sigmoid
+RESIDUAL = struct.Struct("@13P 5Pfi 5Pfi 12q 5i4x")
+
+
+class Tensors(C.Structure):
+    """Mirror of GeepsTensors (csrc/kernels/nn_ops.h)."""
+    _fields_ = [("n", C.c_longlong), ("ptr", C.c_void_p), ("count", C.c_void_p), ("fp32", C.c_void_p), ("order", C.c_void_p)]
+
+
+# what the argument checks of native calls answer besides CUDA's error codes
+REFUSALS = {-10: "a row has 1 to 16384 channels", -11: "the gate's rows do not divide the rows",
+            -12: "an output overlaps another operand", -13: "tensors overlap"}
+
 _lib = None
 _launches = 0
 
@@ -135,6 +150,7 @@ def lib() -> C.CDLL:
     global _lib
     if _lib is None:
         _lib = _native.load()
+        _lib.geeps_residual_work.restype = _lib.geeps_clip_work.restype = C.c_longlong
     return _lib
 
 
@@ -161,6 +177,8 @@ def ptr(t) -> C.c_void_p:
 
 def check(err: int, what: str) -> None:
     global _launches
+    if err in REFUSALS:
+        raise ValueError(f"{what}: {REFUSALS[err]}")
     _launches += 1
     if err != 0:
         raise RuntimeError(f"{what}: CUDA launch error {err}")
@@ -265,10 +283,11 @@ def stop_recording() -> Tape:
 
 
 def launch(fn, label: str, *args) -> None:
-    """Call a native launcher; record it when a tape is being recorded."""
-    if _tape is not None:
+    """Call a native launcher; record it when a tape is being recorded (a call that it refuses is not)."""
+    err = fn(*args)
+    if _tape is not None and err not in REFUSALS:
         _tape.ops.append((fn, args, label))
-    check(fn(*args), label)
+    check(err, label)
 
 
 def hold(t):

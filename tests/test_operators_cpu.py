@@ -1,0 +1,134 @@
+"""Host side of the norm and clipping kernels: launch shapes, workspaces and refusals, which need no GPU."""
+import ctypes as C
+
+import pytest
+
+from geeps_b200.ops import _lib as L
+
+
+def shape(rows, c):
+    out = (C.c_int * 4)()
+    assert L.lib().geeps_norm_shape(C.c_longlong(rows), c, out) == 0
+    return list(out)
+
+
+@pytest.mark.parametrize("c", [1, 7, 8, 9, 64, 72, 255, 256, 257, 576, 1000, 1024, 4095, 4096, 4097, 8192, 8193, 16383, 16384])
+@pytest.mark.parametrize("rows", [1, 2, 5, 300, 50176, 10_000_000])
+def test_shapes_cover_the_rows_within_the_launch_limits(rows, c):
+    vectors, slot, slots, blocks = shape(rows, c)
+    assert vectors * slot * 8 >= c and slot * slots <= 512 and slots >= 1
+    assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
+    assert slot <= 32 or slots <= 15                    # a named barrier for each slot
+    assert 1 <= blocks <= 10_000 and (blocks - 1) * slots < rows
+    assert (slot * slots) % 32 == 0                     # whole warps: their lanes meet in shuffles
+
+
+def pack(**kw):
+    names = ["x", "res", "gate", "out", "y", "dout", "dy", "dx", "dres", "dgate", "scale", "dscale", "work"]
+    v = [kw.get(n, 0) for n in names]
+    for n in ("post", "pre"):
+        v += list(kw.get(n, (0, 0, 0, 0, 0, 0.0, 0)))
+    mode = kw.get("mode", (2 if "x" in kw else 0) | (1 if "pre" in kw else 0))
+    v += [kw["rows"], kw.get("gate_rows", 0)] + [kw.get("ld", kw["c"])] * 10 + [kw["c"], mode, kw.get("stream_fp32", 0), kw.get("block_fp32", 0), 0]
+    return L.RESIDUAL.pack(*v)         # the structure ends on a multiple of eight bytes
+
+
+def test_packed_arguments_have_the_structures_size():
+    class Norm(C.Structure):
+        _fields_ = [(n, C.c_void_p) for n in ("weight", "bias", "stats", "dweight", "dbias")] + [("eps", C.c_float), ("kind", C.c_int)]
+
+    class Residual(C.Structure):
+        _fields_ = ([(f"p{i}", C.c_void_p) for i in range(13)] + [("post", Norm), ("pre", Norm)]
+                    + [(f"n{i}", C.c_longlong) for i in range(12)] + [(f"i{i}", C.c_int) for i in range(5)])
+    assert C.sizeof(Residual) == L.RESIDUAL.size
+    r = Residual.from_buffer_copy(pack(rows=5, c=8, x=4096, pre=(0, 0, 64, 0, 0, 0.5, 2), gate_rows=3))
+    assert (r.p0, r.pre.stats, r.pre.eps, r.pre.kind, r.n0, r.n1, r.n2, r.i0) == (4096, 64, 0.5, 2, 5, 3, 8, 8)
+
+
+LAYER = (0, 0, 1 << 30, 0, 0, 1e-5, 1)
+A, B, D = 1 << 32, 1 << 33, 1 << 34        # addresses that are never touched: every call here is refused
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(res=A, y=B, pre=LAYER, rows=4, c=0), -10),
+    (dict(res=A, y=B, pre=LAYER, rows=4, c=16385), -10),
+    (dict(x=A, res=B, out=D, gate=D + (1 << 20), gate_rows=3, rows=4, c=8), -11),
+    (dict(x=A, res=B, out=D, gate=D + (1 << 20), gate_rows=8, rows=4, c=8), -11),
+    (dict(x=A, res=B, out=D, gate=D + (1 << 20), gate_rows=0, rows=4, c=8), -11),
+    (dict(x=A, res=B, out=A + 16, rows=4, c=8), -12),
+    (dict(x=A, res=B, out=D, y=D, pre=LAYER, rows=4, c=8), -12),
+    (dict(x=A, res=B, out=A, rows=4, c=8, stream_fp32=1), -12),
+    (dict(x=A, res=B, out=B + 8, rows=4, c=8, ld=12), -12),
+    (dict(x=A, res=B, rows=4, c=8), 1),
+    (dict(res=A, pre=LAYER, rows=4, c=8), 1),
+    (dict(res=A, y=B, rows=4, c=8), 1),
+    (dict(x=A, res=B, out=D, rows=-1, c=8), 1),
+    (dict(x=A, res=B, out=D, rows=4, c=8, mode=3), 1),
+    (dict(x=A, res=B, out=D, rows=4, c=8, mode=0), 1),
+    (dict(res=B, out=D, rows=4, c=8, mode=2), 1),
+    (dict(x=A, res=B, out=D, rows=4, c=8, ld=7), 1),
+    (dict(x=A, res=B, out=D, rows=4, c=8, block_fp32=1), 1),
+])
+def test_refused_forward_calls(kw, code):
+    assert L.lib().geeps_residual_forward(pack(**kw), None) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(out=A, dy=B, dres=D, pre=(0, 0, 0, 0, 0, 1e-5, 1), rows=4, c=8), 1),
+    (dict(x=A, dout=B, dx=D, dres=D, rows=4, c=8), -12),
+    (dict(x=A, dout=B, dx=D, rows=4, c=8), 1),
+    (dict(x=A, dx=B, dres=D, rows=4, c=8), 1),
+    (dict(x=A, dout=B, dx=D, dres=D + (1 << 20), rows=1 << 20, c=8), -12),
+    (dict(x=A, dout=B, dx=D, dres=D + (1 << 30), rows=1 << 20, c=8), 1),        # no workspace
+])
+def test_refused_backward_calls(kw, code):
+    assert L.lib().geeps_residual_backward(pack(**kw), None) == code
+
+
+def test_ranges_of_columns_of_one_matrix_do_not_overlap():
+    # refused only for the missing output behind the overlap check
+    for x, out in ((A, A + 16), (A + 16, A), (A, A + 16 + 32 * 2)):
+        assert L.lib().geeps_residual_forward(pack(x=x, out=out, rows=4, c=8, ld=16), None) == 1
+    for x, out in ((A, A + 14), (A + 18, A), (A, A + 16 + 32 * 2 + 2)):
+        assert L.lib().geeps_residual_forward(pack(x=x, out=out, rows=4, c=8, ld=16), None) == -12
+
+
+def test_workspaces():
+    work = L.lib().geeps_residual_work
+    assert work(C.c_longlong(0), C.c_longlong(0), 64, 1) == 0 and work(C.c_longlong(1), C.c_longlong(0), 64, 3) == 0
+    vectors, slot, slots, blocks = shape(50176, 1024)
+    assert work(C.c_longlong(50176), C.c_longlong(0), 1024, 1) == blocks * 2 * 1024
+    assert work(C.c_longlong(50176), C.c_longlong(256), 1024, 3) == (blocks * 4 + blocks + 256) * 1024
+    assert work(C.c_longlong(50176), C.c_longlong(50176), 1024, 2) == blocks * 2 * 1024
+    assert work(C.c_longlong(1 << 22), C.c_longlong(1 << 21), 4096, 2) > 1 << 32
+
+
+def tensors(ranges, fp32=1):
+    n = len(ranges)
+    order = sorted(range(n), key=lambda i: ranges[i])
+    arrays = ((C.c_void_p * n)(*[r[0] for r in ranges]), (C.c_longlong * n)(*[r[1] for r in ranges]), (C.c_ubyte * n)(*[fp32] * n),
+              (C.c_longlong * n)(*order))
+    return L.Tensors(n, *(C.addressof(a) for a in arrays)), arrays
+
+
+@pytest.mark.parametrize("src,dst,code", [
+    ([(A, 10), (A + 36, 10)], None, -13),
+    ([(A, 10)], [(A + 4, 10)], -13),
+    ([(A, 10), (A + 40, 10)], [(A + 40, 10), (A, 10)], -13),
+    ([(A, 10), (B, 5)], [(D, 10), (A + 20, 5)], -13),
+    ([(A, 10), (B, 5)], [(D, 10), (D + 36, 5)], -13),
+    ([(A, 10)], [(A, 9)], 1),
+    ([(A, 10)], [(A, 10), (B, 10)], 1),
+    ([(0, 10)], None, 1),
+    ([(A, -1)], None, 1),
+])
+def test_refused_clipping_calls(src, dst, code):
+    s, hold = tensors(src)
+    d, hold2 = tensors(dst) if dst is not None else (None, None)
+    assert L.lib().geeps_clip_gradients(C.byref(s), C.byref(d) if d is not None else None, C.c_double(1.0), C.c_void_p(A), C.c_void_p(B), None) == code
+
+
+@pytest.mark.parametrize("bound", [-1.0, float("nan")])
+def test_a_bound_that_is_no_norm_is_refused(bound):
+    s, hold = tensors([(A, 10)])
+    assert L.lib().geeps_clip_gradients(C.byref(s), None, C.c_double(bound), C.c_void_p(A), C.c_void_p(B), None) == 1
