@@ -157,8 +157,8 @@ typedef struct GeepsNorm {
 // Backward: dres = dout + pre'(dy) (dout may be NULL with pre), dx, dgate and the parameters' gradients (each or NULL) of
 // the join; without x, out holds the norm's input.  Pitches in elements.  stream_fp32: res, out, dout and dres are fp32,
 // else bf16; block_fp32 (with stream_fp32 only): x, y, gate, dy, dx and dgate.  An output may be the very same rows as an
-// input of its size; any other overlap of an output with another operand is refused.  Rows are any number (none: the
-// parameters' gradients are zeros), C is 1 to 16384, every address and pitch will do.  work: geeps_residual_work() floats,
+// input of its size; any other overlap of an output with another operand is refused.  Rows are
+// less than 2^31 - 256, pitches than 2^29 (no rows: the parameters' gradients are zeros), C is 1 to 16384, every address will do.  work: geeps_residual_work() floats,
 // private to the call while it runs.  mode: 1 for a norm alone (no x), 2 for a join, 3 for a join with a norm behind it.
 #define GEEPS_ERR_NORM_CHANNELS (-10)
 #define GEEPS_ERR_NORM_GATE (-11)
@@ -180,7 +180,7 @@ long long geeps_residual_work(long long rows, long long gate_rows, int C, int mo
 int geeps_residual_forward(const GeepsResidual* p, void* stream);
 int geeps_residual_backward(const GeepsResidual* p, void* stream);
 // launch shape (host arithmetic only): vectors a thread, threads a row, rows a block at a time, blocks
-int geeps_norm_shape(long long rows, int C, int* out);
+int geeps_norm_shape(long long rows, int C, int backward, int mode, int* out);
 
 // ---- clipping of gradients by their global norm (the reference's solver had it in its absent Caffe application) ----
 // norm = sqrt(sum over all tensors of g^2), c = norm > max_norm ? max_norm / norm : 1, dst = c * g; dst NULL: in place, and

@@ -6,16 +6,19 @@ import pytest
 from geeps_b200.ops import _lib as L
 
 
-def shape(rows, c):
+def shape(rows, c, backward=True, mode=3):
     out = (C.c_int * 4)()
-    assert L.lib().geeps_norm_shape(C.c_longlong(rows), c, out) == 0
+    assert L.lib().geeps_norm_shape(C.c_longlong(rows), c, int(backward), mode, out) == 0
     return list(out)
 
 
 @pytest.mark.parametrize("c", [1, 7, 8, 9, 64, 72, 255, 256, 257, 576, 1000, 1024, 4095, 4096, 4097, 8192, 8193, 16383, 16384])
 @pytest.mark.parametrize("rows", [1, 2, 5, 300, 50176, 10_000_000])
-def test_shapes_cover_the_rows_within_the_launch_limits(rows, c):
-    vectors, slot, slots, blocks = shape(rows, c)
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("mode", [1, 3])
+def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode):
+    vectors, slot, slots, blocks = shape(rows, c, backward, mode)
+    assert slot * slots <= (256 if vectors == 1 and not backward else 512)
     assert vectors * slot * 8 >= c and slot * slots <= 512 and slots >= 1
     assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
     assert slot <= 32 or slots <= 15                    # a named barrier for each slot
@@ -98,7 +101,7 @@ def test_workspaces():
     assert work(C.c_longlong(0), C.c_longlong(0), 64, 1) == 0 and work(C.c_longlong(1), C.c_longlong(0), 64, 3) == 0
     vectors, slot, slots, blocks = shape(50176, 1024)
     assert work(C.c_longlong(50176), C.c_longlong(0), 1024, 1) == blocks * 2 * 1024
-    assert work(C.c_longlong(50176), C.c_longlong(256), 1024, 3) == (blocks * 4 + blocks + 256) * 1024
+    assert work(C.c_longlong(50176), C.c_longlong(256), 1024, 3) == (blocks * 4 + blocks * slots + 256) * 1024
     assert work(C.c_longlong(50176), C.c_longlong(50176), 1024, 2) == blocks * 2 * 1024
     assert work(C.c_longlong(1 << 22), C.c_longlong(1 << 21), 4096, 2) > 1 << 32
 
