@@ -21,19 +21,20 @@ struct Shape {
   int blocks, per_sm;
   int threads() const { return slot * slots; }
 };
-// K vectors a thread: as few as 512 threads allow, since what a thread keeps for its columns is in registers.  A block of the
-// backward pass has up to 512 threads and an SM to itself, so that few blocks leave column sums behind; forward several
-// blocks of half the size share an SM.
+// K vectors a thread: as few as the threads of a block allow, since what a thread keeps for its columns is in registers.  A
+// block of the backward pass has up to 384 (rows of up to 384 vectors, but of more than 16) or 512 threads and an SM to itself,
+// so that few blocks leave column sums behind; forward several blocks of 256 share an SM.
 inline Shape plan(long long rows, int C, bool backward, int mode) {
   Shape s;
-  const int vec = (C + kVec - 1) / kVec, most = backward ? 512 : 256;
-  s.vectors = vec <= most ? 1 : vec <= 1024 ? 2 : 4;
-  const int need = (vec + s.vectors - 1) / s.vectors;
+  const int vec = (C + kVec - 1) / kVec;
+  const int narrow = vec <= 16, one = backward ? 384 : 256;
+  s.vectors = vec <= one ? 1 : vec <= 1024 ? 2 : 4;
+  const int need = (vec + s.vectors - 1) / s.vectors, most = s.vectors > 1 ? 512 : backward ? narrow ? 512 : 384 : 256;
   s.slot = 1;
   if (need <= 32) while (s.slot < need) s.slot <<= 1;
   else s.slot = (need + 31) / 32 * 32;
-  s.slots = s.slot >= most ? 1 : most / s.slot;
-  s.per_sm = backward || s.vectors > 1 ? 1 : mode == MODE_NORM ? 4 : 2;
+  s.slots = s.slot > most / 2 ? 1 : most / s.slot;
+  s.per_sm = backward || s.vectors > 1 ? 1 : mode == MODE_NORM ? 3 : 2;
   const long long room = (long long)geeps_sm_count() * s.per_sm, want = (rows + s.slots - 1) / s.slots;
   s.blocks = (int)(want < room ? want : room);
   return s;
@@ -58,6 +59,7 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 // until at most depth - 1 of this thread's groups are under way
 __device__ __forceinline__ void copy_wait(int depth) {
   if (depth == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (depth == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
   else if (depth == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
   else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -170,6 +172,14 @@ struct Columns {
         f[i] = make_float2(there && on(2 * i) ? (float)row[at(2 * i)] : 0.f, there && on(2 * i + 1) ? (float)row[at(2 * i + 1)] : 0.f);
     }
   }
+  // zeros in the place of a row that the slot does not have
+  template <typename T>
+  __device__ __forceinline__ void no_row(uint32_t to) const {
+    if (!VEC) return;
+#pragma unroll
+    for (int q = 0; q < K * 8 * (int)sizeof(T) / 16; ++q)
+      asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(to + q * THREADS * 16), "r"(0) : "memory");
+  }
   // a row from the ring if there is one; zeros where the slot has no such row
   template <typename T>
   __device__ __forceinline__ void load(const Rows<T>& rows, int row, bool active, bool there, uint32_t from, float2 (&f)[N]) const {
@@ -181,7 +191,7 @@ struct Columns {
       for (int k = 0; k < K; ++k)
 #pragma unroll
         for (int q = 0; q < Q; ++q)
-          unpack<T>(active ? ld_shared16(from + (k * Q + q) * THREADS * 16) : make_uint4(0u, 0u, 0u, 0u), f + 4 * k + q * (4 / Q));
+          unpack<T>(ld_shared16(from + (k * Q + q) * THREADS * 16), f + 4 * k + q * (4 / Q));
     } else {
       const uint32_t r = from + (threadIdx.x / slot) * pieces<T>() + (uint32_t)((uintptr_t)rows.at(row) & 15);
       const bool any = active && there;
@@ -220,20 +230,19 @@ struct Columns {
     for (int i = 0; i < N; ++i)
       f[i] = make_float2(!on(2 * i) ? 0.f : p ? p[at(2 * i)] : other, !on(2 * i + 1) ? 0.f : p ? p[at(2 * i + 1)] : other);
   }
-  // (f - mean) * rstd, zero where there is no column
-  __device__ __forceinline__ void centre(float2 (&f)[N], float mean, float rstd) const {
+  // f - mean, zero where there is no column
+  __device__ __forceinline__ void subtract(float2 (&f)[N], float mean) const {
     if (VEC) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const bool live = on(8 * k);
-        const float2 m = both(live ? -mean : 0.f), r = both(rstd);
+        const float2 m = both(on(8 * k) ? -mean : 0.f);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[4 * k + e] = mul2(add2(f[4 * k + e], m), r);
+        for (int e = 0; e < 4; ++e) f[4 * k + e] = add2(f[4 * k + e], m);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float2 v = mul2(add2(f[i], both(-mean)), both(rstd));
+        const float2 v = add2(f[i], both(-mean));
         f[i] = make_float2(on(2 * i) ? v.x : 0.f, on(2 * i + 1) ? v.y : 0.f);
       }
     }
@@ -242,7 +251,7 @@ struct Columns {
 
 struct Slot {
   int id, t, size;
-  float* red;        // 64 floats of shared memory: two turns of 32, zero where no warp writes
+  float* red;        // 128 floats of shared memory: two turns of 64, zero where no warp writes
   int turn;
   __device__ __forceinline__ void sync() const {
     if (size > 32) asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(size) : "memory");
@@ -250,50 +259,58 @@ struct Slot {
   }
 };
 
-// Sums of one or two values over the threads of a slot, the same in each.  Slots of several warps meet at their named barrier;
-// the two turns of `red` alternate, so the next sum may be written while this one is still being read.
-template <bool WIDE>
-__device__ __forceinline__ float slot_sum(float v, Slot& s) {
+// Sums of M values (1, 2 or 4) over the threads of a slot, the same in each.  In a warp each step halves the values a lane
+// goes on with, until it is one: four sums take six shuffles.  Warps meet in shared memory at the slot's named barrier; the two
+// turns of `red` alternate, so the next sums may be written while these are still being read.
+template <bool WIDE, int M>
+__device__ __forceinline__ void slot_sum(float (&v)[M], Slot& s) {
   if (!WIDE) {
-    for (int o = s.size >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int o = s.size >> 1; o; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < M; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    }
+    return;
+  }
+  float one;
+  if (M == 4) {
+    const bool a = threadIdx.x & 16, b = threadIdx.x & 8;
+    float x = a ? v[2 % M] : v[0], y = a ? v[3 % M] : v[1 % M];
+    x += __shfl_xor_sync(0xffffffffu, a ? v[0] : v[2 % M], 16);
+    y += __shfl_xor_sync(0xffffffffu, a ? v[1 % M] : v[3 % M], 16);
+    one = b ? y : x;
+    one += __shfl_xor_sync(0xffffffffu, b ? x : y, 8);
+  } else if (M == 2) {
+    const bool a = threadIdx.x & 16;
+    one = a ? v[1 % M] : v[0];
+    one += __shfl_xor_sync(0xffffffffu, a ? v[0] : v[1 % M], 16);
+    one += __shfl_xor_sync(0xffffffffu, one, 8);
+  } else {
+    one = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
+    one += __shfl_xor_sync(0xffffffffu, one, 8);
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (s.size == 32) return v;
+  for (int o = 4; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
   float* r = s.red + s.turn;
-  s.turn ^= 32;
-  if ((s.t & 31) == 0) r[s.t >> 5] = v;
+  s.turn ^= 64;
+  constexpr int L = 32 / M;           // lanes that hold the same sum
+  if (s.t % L == 0) r[s.t / L] = one;
   s.sync();
-  float4 q = ld_f4(r);
-  v = (q.x + q.y) + (q.z + q.w);
-  for (int w = 128; w < s.size; w += 128) { q = ld_f4(r + (w >> 5)); v += (q.x + q.y) + (q.z + q.w); }
-  return v;
-}
-template <bool WIDE>
-__device__ __forceinline__ float2 slot_sum(float2 v, Slot& s) {
-  if (!WIDE) {
-    for (int o = s.size >> 1; o; o >>= 1) { v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o); }
-    return v;
-  }
-  // the lower half of the warp goes on with x, the upper with y
-  const bool upper = threadIdx.x & 16;
-  float one = upper ? v.y : v.x;
-  one += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+  // four values at a time, values of more warps than four (M = 4), eight or sixteen in a loop
+  constexpr int Q = M == 4 ? 4 : M == 2 ? 2 : 1;
 #pragma unroll
-  for (int o = 8; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
-  if (s.size == 32) {
-    const float other = __shfl_xor_sync(0xffffffffu, one, 16);
-    return upper ? make_float2(other, one) : make_float2(one, other);
+  for (int i = 0; i < M; ++i) v[i] = 0.f;
+  auto add = [&](int w) {
+    const float4 q = ld_f4(r + 4 * w);
+    if (M == 4) { v[0] += q.x; v[1 % M] += q.y; v[2 % M] += q.z; v[3 % M] += q.w; }
+    else if (M == 2) { v[0] += q.x + q.z; v[1 % M] += q.y + q.w; }
+    else v[0] += (q.x + q.y) + (q.z + q.w);
+  };
+#pragma unroll
+  for (int w = 0; w < Q; ++w) add(w);
+  for (int w = 4; w < s.size >> 5; w += 4) {
+#pragma unroll
+    for (int u = 0; u < Q; ++u) add(w * Q / 4 + u);
   }
-  float* r = s.red + s.turn;
-  s.turn ^= 32;
-  if ((s.t & 15) == 0) r[s.t >> 4] = one;
-  s.sync();
-  const float4 q = ld_f4(r), u = ld_f4(r + 4);
-  v = make_float2((q.x + q.z) + (u.x + u.z), (q.y + q.w) + (u.y + u.w));
-  for (int w = 128; w < s.size; w += 64) { const float4 e = ld_f4(r + (w >> 4)); v.x += e.x + e.z; v.y += e.y + e.w; }
-  return v;
 }
 template <int N>
 __device__ __forceinline__ float total(const float2 (&f)[N]) {
@@ -302,37 +319,63 @@ __device__ __forceinline__ float total(const float2 (&f)[N]) {
   for (int i = 1; i < N; ++i) v = add2(v, f[i]);
   return v.x + v.y;
 }
-
-// n = (f - mean) * rstd in place; mean and rstd go to stats
-template <bool WIDE, int K, bool VEC, int THREADS>
-__device__ __forceinline__ void normalise(const Columns<K, VEC, THREADS>& cols, Slot& s, const GeepsNorm& norm, int row, bool active,
-                                          float inv_c, float2 (&f)[4 * K]) {
-  float mean = 0.f;
-  if (norm.kind == NORM_LAYER) {
-    mean = slot_sum<WIDE>(total(f), s) * inv_c;
-    cols.centre(f, mean, 1.f);
-  }
-  float2 q = mul2(f[0], f[0]);
+template <int N>
+__device__ __forceinline__ float dot(const float2 (&f)[N], const float2 (&g)[N]) {
+  float2 v = mul2(f[0], g[0]);
 #pragma unroll
-  for (int i = 1; i < 4 * K; ++i) q = fma2(f[i], f[i], q);
-  const float rstd = 1.f / sqrtf(fmaf(slot_sum<WIDE>(q.x + q.y, s), inv_c, norm.eps));
-#pragma unroll
-  for (int i = 0; i < 4 * K; ++i) f[i] = mul2(f[i], both(rstd));
-  if (norm.stats && active && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * row) = make_float2(mean, rstd);
+  for (int i = 1; i < N; ++i) v = fma2(f[i], g[i], v);
+  return v.x + v.y;
 }
 
-// gradient of n * w + b by its input, a = dz * w in place: rstd * (a - mean a - n mean(a n))
-template <bool WIDE, int K>
-__device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, float inv_c, const float2 (&n)[4 * K], float2 (&a)[4 * K]) {
-  float2 q = mul2(a[0], n[0]);
+// n = (f - mean) * rstd of R rows in place; mean and rstd go to stats
+template <bool WIDE, int R, int K, bool VEC, int THREADS>
+__device__ __forceinline__ void normalise(const Columns<K, VEC, THREADS>& cols, Slot& s, const GeepsNorm& norm, int row, int end,
+                                          float inv_c, float2 (&f)[R][4 * K]) {
+  float mean[R], v[R];
 #pragma unroll
-  for (int i = 1; i < 4 * K; ++i) q = fma2(a[i], n[i], q);
-  float2 m = make_float2(0.f, q.x + q.y);
-  if (kind == NORM_LAYER) { m.x = total(a); m = slot_sum<WIDE>(m, s); }
-  else m.y = slot_sum<WIDE>(m.y, s);
-  const float2 m0 = both(-m.x * inv_c * rstd), m1 = both(-m.y * inv_c * rstd), r = both(rstd);
+  for (int r = 0; r < R; ++r) mean[r] = 0.f;
+  if (norm.kind == NORM_LAYER) {
 #pragma unroll
-  for (int i = 0; i < 4 * K; ++i) a[i] = fma2(n[i], m1, fma2(a[i], r, m0));
+    for (int r = 0; r < R; ++r) mean[r] = total(f[r]);
+    slot_sum<WIDE>(mean, s);
+#pragma unroll
+    for (int r = 0; r < R; ++r) { mean[r] *= inv_c; cols.subtract(f[r], mean[r]); }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = dot(f[r], f[r]);
+  slot_sum<WIDE>(v, s);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float rstd = 1.f / sqrtf(fmaf(v[r], inv_c, norm.eps));
+#pragma unroll
+    for (int i = 0; i < 4 * K; ++i) f[r][i] = mul2(f[r][i], both(rstd));
+    if (norm.stats && row + r < end && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * (row + r)) = make_float2(mean[r], rstd);
+  }
+}
+
+// n = (f - mean) * rstd with the statistics at hand.  Not zero where there is no column, but whatever it meets there is.
+template <int N>
+__device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
+  const float2 r = both(st.y), m = both(-st.x * st.y);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = fma2(f[i], r, m);
+}
+
+// Gradients of R rows n * w + b by their inputs, for a = dz * w: rstd * (a - mean a - n mean(a n)), added to `to`
+template <bool WIDE, int R, int N>
+__device__ __forceinline__ void norm_gradient(Slot& s, int kind, const float2 (&st)[R], float inv_c, const float2 (&n)[R][N],
+                                              const float2 (&a)[R][N], float2 (&to)[R][N]) {
+  float v[2 * R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) { v[2 * r] = total(a[r]); v[2 * r + 1] = dot(a[r], n[r]); }
+  slot_sum<WIDE>(v, s);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float scale = -inv_c * st[r].y;
+    const float2 m0 = both(kind == NORM_LAYER ? v[2 * r] * scale : 0.f), m1 = both(v[2 * r + 1] * scale), rs = both(st[r].y);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[r][i] = fma2(n[r][i], m1, fma2(a[r][i], rs, add2(to[r][i], m0)));
+  }
 }
 
 __device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
@@ -353,30 +396,39 @@ __device__ __forceinline__ void clear_ring(unsigned char* ring, int bytes) {
   __syncthreads();
 }
 
-// The rows of a slot and its place in the ring.  Slots that share a warp take the same number of turns, since its lanes meet in
-// sums: some have no row in the last.
+// The rows of a slot, R a turn.  Slots that share a warp take the same number of turns, since its lanes meet in sums: some have
+// no row in the last.
 struct Walk {
   int lo, hi, turns;
-  __device__ __forceinline__ Walk(const GeepsResidual& p, int slots, int id, bool wide) {
+  __device__ __forceinline__ Walk(const GeepsResidual& p, int slots, int id, bool wide, int R) {
     const int rows = (int)p.rows, all = gridDim.x * slots, me = blockIdx.x * slots + id;
     lo = first_row(rows, all, me); hi = first_row(rows, all, me + 1);
-    turns = wide ? hi - lo : rows / all + (rows % all ? 1 : 0);
+    turns = wide ? (hi - lo + R - 1) / R : rows / all + (rows % all ? 1 : 0);
   }
+};
+
+// What kernels of K vectors a thread are like.  Two rows a turn where a turn's overhead counts most and registers allow: bf16
+// rows of up to 384 vectors; blocks have 384 threads then backward (168 registers a thread).
+template <typename TB, int K, bool VEC, bool WIDE>
+struct Form {
+  static constexpr int R = WIDE && K == 1 && VEC && sizeof(TB) == 2 ? 2 : 1;
+  static constexpr int forward_threads = K == 1 ? 256 : 512;
+  static constexpr int backward_threads = K == 1 && WIDE ? 384 : 512;
 };
 
 // WIDE: a slot is whole warps.  PIXEL: a gate for every row.
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(K == 1 ? 256 : 512, K == 1 ? MODE == MODE_NORM ? 4 : 2 : 1)
+__global__ void __launch_bounds__(Form<TB, K, VEC, WIDE>::forward_threads, K == 1 ? MODE == MODE_NORM ? 3 : 2 : 1)
 residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ __align__(16) float red[16][64];
-  constexpr int N = 4 * K;
-  for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
+  __shared__ __align__(16) float red[16][128];
+  constexpr int N = 4 * K, R = Form<TB, K, VEC, WIDE>::R;
+  for (int i = threadIdx.x; i < 16 * 128; i += blockDim.x) red[0][i] = 0.f;
   __syncthreads();
   Slot s;
-  s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[slot > 32 ? s.id : 0]; s.turn = 0;
-  const Columns<K, VEC, K == 1 ? 256 : 512> cols = {s.t, slot, p.C, slots};
+  s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
+  const Columns<K, VEC, Form<TB, K, VEC, WIDE>::forward_threads> cols = {s.t, slot, p.C, slots};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
   float2 sw[N], sb[N], w2[N], b2[N];           // scale * weight and scale * bias, times the gate where an image has one
@@ -388,68 +440,84 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
   };
   if ((MODE & MODE_JOIN) && !by_image) join_params();
   if (MODE & MODE_NORM) { cols.param(p.pre.weight, 1.f, w2); cols.param(p.pre.bias, 0.f, b2); }
-  const Walk w(p, slots, s.id, WIDE);
+  const Walk w(p, slots, s.id, WIDE, R);
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
-  int left = 0;                          // rows to go with the gate at hand
+  int left = 0;                                // rows to go with the gate at hand
 
   const bool live = !VEC || cols.on(0);        // K = 1: a thread has its one vector or nothing
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring) + (VEC ? threadIdx.x * 16 : 0);
   const int at_x = cols.template stage<TR>(), at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
-  const int stage = at_g + (PIXEL ? cols.template stage<TB>() : 0);
+  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * R * one;
   const Rows<TR> res(p.res, p.ldres, cols.first()), h_out(p.out, p.ldout, cols.first());
   const Rows<TB> x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first()), y_out(p.y, p.ldy, cols.first());
-  auto copy = [&](int turn) {               // depth is a power of two
-    const int row = w.lo + turn;
-    if (row < w.hi && live) {
-      const uint32_t to = base + (turn & (depth - 1)) * stage;
-      cols.copy(res.at(row), to);
-      if (MODE & MODE_JOIN) cols.copy(x.at(row), to + at_x);
-      if (PIXEL) cols.copy(gate.at(row), to + at_g);
+  int ahead = w.lo, in = 0, out = 0;           // the row that is copied next, stages that are filled and read next
+  auto copy = [&]() {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = ahead + r;
+      if (row < w.hi && live) {
+        const uint32_t to = base + in + r * one;
+        cols.copy(res.at(row), to);
+        if (MODE & MODE_JOIN) cols.copy(x.at(row), to + at_x);
+        if (PIXEL) cols.copy(gate.at(row), to + at_g);
+      }
     }
+    ahead += R;
+    in = in == last ? 0 : in + R * one;
     copy_commit();
   };
   if (cols.RING) {
-    clear_ring(ring, depth * stage);
-    for (int i = 0; i < depth - 1; ++i) copy(i);
+    clear_ring(ring, depth * R * one);
+    for (int i = 0; i < depth - 1; ++i) copy();
   }
   for (int i = 0; i < w.turns; ++i) {
-    const int row = w.lo + i;
-    const bool active = WIDE || row < w.hi;
+    const int row = w.lo + i * R;
     if (cols.RING) {
-      copy(i + depth - 1);
+      if (!VEC) s.sync();
+      copy();
       copy_wait(depth);
       if (!VEC) s.sync();
     }
-    const uint32_t from = base + (i & (depth - 1)) * stage;
-    float2 h[N];
-    cols.load(res, row, active, true, from, h);
+    const uint32_t from = base + out;
+    if (cols.RING) out = out == last ? 0 : out + R * one;
+    float2 h[R][N];
+#pragma unroll
+    for (int r = 0; r < R; ++r) cols.load(res, row + r, row + r < w.hi, true, from + r * one, h[r]);
     if (MODE & MODE_JOIN) {
-      float2 z[N], g[N];
-      cols.load(x, row, active, true, from + at_x, z);
-      if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_factor(p.sigmoid, g); }
-      if (!VEC && cols.RING) s.sync();
-      if (by_image && left-- == 0 && active) {
-        const int image = row / per_gate;
-        left = (image + 1) * per_gate - row - 1;
-        cols.fetch(gate.at(image), true, g);
-        gate_factor(p.sigmoid, g);
-        join_params();
+      float2 z[R][N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) { sw[j] = mul2(sw[j], g[j]); sb[j] = mul2(sb[j], g[j]); }
-      }
-      if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, active, inv_c, z);
+      for (int r = 0; r < R; ++r) cols.load(x, row + r, row + r < w.hi, true, from + r * one + at_x, z[r]);
+      if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, w.hi, inv_c, z);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (PIXEL) h[j] = fma2(fma2(z[j], sw[j], sb[j]), g[j], h[j]);
-        else h[j] = add2(h[j], fma2(z[j], sw[j], sb[j]));
+      for (int r = 0; r < R; ++r) {
+        float2 g[N];
+        const bool active = row + r < w.hi;
+        if (by_image && left-- == 0 && active) {
+          const int image = (row + r) / per_gate;
+          left = (image + 1) * per_gate - (row + r) - 1;
+          cols.fetch(gate.at(image), true, g);
+          gate_factor(p.sigmoid, g);
+          join_params();
+#pragma unroll
+          for (int j = 0; j < N; ++j) { sw[j] = mul2(sw[j], g[j]); sb[j] = mul2(sb[j], g[j]); }
+        }
+        if (PIXEL) { cols.load(gate, row + r, active, true, from + r * one + at_g, g); gate_factor(p.sigmoid, g); }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (PIXEL) h[r][j] = fma2(fma2(z[r][j], sw[j], sb[j]), g[j], h[r][j]);
+          else h[r][j] = add2(h[r][j], fma2(z[r][j], sw[j], sb[j]));
+        }
+        cols.store(h_out.at(row + r), active, h[r]);
       }
-      cols.store(h_out.at(row), active, h);
-    } else if (!VEC && cols.RING) s.sync();
+    }
     if (MODE & MODE_NORM) {
-      normalise<WIDE>(cols, s, p.pre, row, active, inv_c, h);
+      normalise<WIDE>(cols, s, p.pre, row, w.hi, inv_c, h);
 #pragma unroll
-      for (int j = 0; j < N; ++j) h[j] = fma2(h[j], w2[j], b2[j]);
-      cols.store(y_out.at(row), active, h);
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[r][j] = fma2(h[r][j], w2[j], b2[j]);
+        cols.store(y_out.at(row + r), row + r < w.hi, h[r]);
+      }
     }
   }
 }
@@ -474,17 +542,17 @@ __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int
 }
 
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(Form<TB, K, VEC, WIDE>::backward_threads)
 residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ __align__(16) float red[16][64];
-  constexpr int N = 4 * K;
-  for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
+  __shared__ __align__(16) float red[16][128];
+  constexpr int N = 4 * K, R = Form<TB, K, VEC, WIDE>::R;
+  for (int i = threadIdx.x; i < 16 * 128; i += blockDim.x) red[0][i] = 0.f;
   __syncthreads();
   Slot s;
-  s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[slot > 32 ? s.id : 0]; s.turn = 0;
-  const Columns<K, VEC, 512> cols = {s.t, slot, p.C, slots};
+  s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
+  const Columns<K, VEC, Form<TB, K, VEC, WIDE>::backward_threads> cols = {s.t, slot, p.C, slots};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
   float2 sw[N], sb[N], w2[N], a0[N], a1[N], n0[N], n1[N];     // sw: scale * weight, times the gate where an image has one
@@ -505,33 +573,46 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
 #pragma unroll
     for (int i = 0; i < N; ++i) n0[i] = n1[i] = both(0.f);
   }
-  const Walk w(p, slots, s.id, WIDE);
+  const Walk w(p, slots, s.id, WIDE, R);
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
-  int image = 0, left = 0;
+  int image = -1, left = 0;
 
   const bool live = !VEC || cols.on(0);        // K = 1: a thread has its one vector or nothing
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring) + (VEC ? threadIdx.x * 16 : 0);
   const int at_o = cols.template stage<TR>(), at_y = at_o + (MODE & MODE_NORM ? cols.template stage<TR>() : 0);
   const int at_x = at_y + (MODE & MODE_NORM ? cols.template stage<TB>() : 0);
   const int at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
-  const int stage = at_g + (PIXEL ? cols.template stage<TB>() : 0);
+  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * R * one;
   const Rows<TR> dout(p.dout, p.lddout, cols.first()), h(p.out, p.ldout, cols.first()), dres(p.dres, p.lddres, cols.first());
   const Rows<TB> dy(p.dy, p.lddy, cols.first()), x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first());
   const Rows<TB> dx(p.dx, p.lddx, cols.first()), dgate(p.dgate, p.lddgate, cols.first());
   const bool has_dout = p.dout != nullptr;
-  auto copy = [&](int turn) {
-    const int row = w.lo + turn;
-    if (row < w.hi && live) {
-      const uint32_t to = base + (turn & (depth - 1)) * stage;
-      if (has_dout) cols.copy(dout.at(row), to);
-      if (MODE & MODE_NORM) { cols.copy(h.at(row), to + at_o); cols.copy(dy.at(row), to + at_y); }
-      if (MODE & MODE_JOIN) cols.copy(x.at(row), to + at_x);
-      if (PIXEL) cols.copy(gate.at(row), to + at_g);
+  int ahead = w.lo, in = 0, out = 0;
+  auto copy = [&]() {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = ahead + r;
+      const uint32_t to = base + in + r * one;
+      if (row < w.hi) {
+        if (live) {
+          if (has_dout) cols.copy(dout.at(row), to);
+          if (MODE & MODE_NORM) { cols.copy(h.at(row), to + at_o); cols.copy(dy.at(row), to + at_y); }
+          if (MODE & MODE_JOIN) cols.copy(x.at(row), to + at_x);
+          if (PIXEL) cols.copy(gate.at(row), to + at_g);
+        }
+      } else if (R > 1 || !WIDE) {             // rows that are read and are none: they add nothing to the sums
+        cols.template no_row<TR>(to);
+        if (MODE & MODE_NORM) { cols.template no_row<TR>(to + at_o); cols.template no_row<TB>(to + at_y); }
+        if (MODE & MODE_JOIN) cols.template no_row<TB>(to + at_x);
+        if (PIXEL) cols.template no_row<TB>(to + at_g);
+      }
     }
+    ahead += R;
+    in = in == last ? 0 : in + R * one;
     copy_commit();
   };
   // with a gate per image a0 and a1 are the sums u and v of the image at hand; A and B of all images are kept behind the ring
-  float* all_images = reinterpret_cast<float*>(ring + depth * stage) + threadIdx.x;
+  float* all_images = reinterpret_cast<float*>(ring + depth * R * one) + threadIdx.x;
   auto kept = [&](int i) -> float& { return all_images[i * slot * slots]; };
   if (by_image) {
     for (int i = 0; i < 4 * N; ++i) kept(i) = 0.f;
@@ -561,76 +642,115 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
   };
   if (cols.RING) {
-    clear_ring(ring, depth * stage);
-    for (int i = 0; i < depth - 1; ++i) copy(i);
+    clear_ring(ring, depth * R * one);
+    for (int i = 0; i < depth - 1; ++i) copy();
   }
-  float2 st1 = both(0.f), st2 = both(0.f);
-  if (w.lo < w.hi) {
-    if ((MODE & MODE_JOIN) && p.post.kind) st1 = stats_of(p.post, w.lo);
-    if (MODE & MODE_NORM) st2 = stats_of(p.pre, w.lo);
-  }
+  // the statistics of a turn's rows come a turn before
+  float2 st1[R], st2[R];
+  auto statistics = [&](int row) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int q = row + r < w.hi ? row + r : w.hi - 1;
+      st1[r] = st2[r] = both(0.f);
+      if (!WIDE && w.lo == w.hi) continue;
+      if ((MODE & MODE_JOIN) && p.post.kind) st1[r] = stats_of(p.post, q);
+      if (MODE & MODE_NORM) st2[r] = stats_of(p.pre, q);
+    }
+  };
+  if (w.turns) statistics(w.lo);
   for (int i = 0; i < w.turns; ++i) {
-    const int row = w.lo + i;
-    const bool active = WIDE || row < w.hi;
+    const int row = w.lo + i * R;
     if (cols.RING) {
-      copy(i + depth - 1);
+      if (!VEC) s.sync();
+      copy();
       copy_wait(depth);
       if (!VEC) s.sync();
     }
-    const uint32_t from = base + (i & (depth - 1)) * stage;
-    // everything of the row is read before its first output is written
-    float2 dh[N], z[N], n[N], a[N], g[N];
-    cols.load(dout, row, active, has_dout, from, dh);
-    if (MODE & MODE_NORM) { cols.load(h, row, active, true, from + at_o, n); cols.load(dy, row, active, true, from + at_y, a); }
-    if (MODE & MODE_JOIN) cols.load(x, row, active, true, from + at_x, z);
-    if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_factor(p.sigmoid, g); }
-    if (!VEC && cols.RING) s.sync();
-    if (by_image && left == 0 && active) {
-      image = row / per_gate;
-      left = (image + 1) * per_gate - row;
-      cols.fetch(gate.at(image), true, g);
-      gate_factor(p.sigmoid, g);
-      scaled(p.post.weight, 1.f, sw);
+    const uint32_t from = base + out;
+    if (cols.RING) out = out == last ? 0 : out + R * one;
+    float2 now1[R], now2[R];
 #pragma unroll
-      for (int j = 0; j < N; ++j) sw[j] = mul2(sw[j], g[j]);
-    }
-    const float2 now1 = st1, now2 = st2;
-    const int ahead = row + 1 < w.hi ? row + 1 : w.hi - 1;
-    if (WIDE || w.lo < w.hi) {
-      if ((MODE & MODE_JOIN) && p.post.kind) st1 = stats_of(p.post, ahead);
-      if (MODE & MODE_NORM) st2 = stats_of(p.pre, ahead);
-    }
+    for (int r = 0; r < R; ++r) { now1[r] = st1[r]; now2[r] = st2[r]; }
+    statistics(row + R);
+    // an output may lie where an operand does: without a ring everything of the row is read before its first output is written
+    float2 dh[R][N], z[R][N], g[R][N];
+    auto load_branch = [&]() {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool active = WIDE && R == 1 || row + r < w.hi;
+        if (MODE & MODE_JOIN) cols.load(x, row + r, active, true, from + r * one + at_x, z[r]);
+        if (PIXEL) { cols.load(gate, row + r, active, true, from + r * one + at_g, g[r]); gate_factor(p.sigmoid, g[r]); }
+      }
+    };
+    if (!cols.RING) load_branch();
+#pragma unroll
+    for (int r = 0; r < R; ++r) cols.load(dout, row + r, WIDE && R == 1 || row + r < w.hi, has_dout, from + r * one, dh[r]);
     if (MODE & MODE_NORM) {
-      cols.centre(n, now2.x, now2.y);
+      float2 n[R][N], a[R][N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        n0[j] = fma2(a[j], n[j], n0[j]); n1[j] = add2(n1[j], a[j]);
-        a[j] = mul2(a[j], w2[j]);
-      }
-      norm_gradient<WIDE, K>(s, p.pre.kind, now2.y, inv_c, n, a);
+      for (int r = 0; r < R; ++r) {
+        const bool active = WIDE && R == 1 || row + r < w.hi;
+        cols.load(h, row + r, active, true, from + r * one + at_o, n[r]);
+        cols.load(dy, row + r, active, true, from + r * one + at_y, a[r]);
+        normalised(n[r], now2[r]);
 #pragma unroll
-      for (int j = 0; j < N; ++j) dh[j] = add2(dh[j], a[j]);
-    }
-    cols.store(dres.at(row), active, dh);
-    if (MODE & MODE_JOIN) {
-      float2 e[N];
-      if (p.post.kind) cols.centre(z, now1.x, now1.y);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float2 d = dh[j];
-        if (PIXEL) {
-          n[j] = mul2(mul2(d, fma2(sw[j], z[j], sb[j])), gate_slope(p.sigmoid, g[j]));
-          d = mul2(d, g[j]);
+        for (int j = 0; j < N; ++j) {
+          n0[j] = fma2(a[r][j], n[r][j], n0[j]); n1[j] = add2(n1[j], a[r][j]);
+          a[r][j] = mul2(a[r][j], w2[j]);
         }
-        a0[j] = fma2(d, z[j], a0[j]); a1[j] = add2(a1[j], d);
-        e[j] = mul2(d, sw[j]);
       }
-      if (PIXEL && p.dgate) cols.store(dgate.at(row), active, n);
-      if (p.post.kind) norm_gradient<WIDE, K>(s, p.post.kind, now1.y, inv_c, z, e);
-      cols.store(dx.at(row), active, e);
-      if (by_image && active && (--left == 0 || row + 1 == w.hi)) image_done();
+      norm_gradient<WIDE>(s, p.pre.kind, now2, inv_c, n, a, dh);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) cols.store(dres.at(row + r), WIDE && R == 1 || row + r < w.hi, dh[r]);
+    if (MODE & MODE_JOIN) {
+      if (cols.RING) load_branch();
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool active = WIDE && R == 1 || row + r < w.hi;
+        if (by_image && left == 0 && active) {
+          if (image >= 0) image_done();
+          image = (row + r) / per_gate;
+          left = (image + 1) * per_gate - (row + r);
+          float2 factor[N];
+          cols.fetch(gate.at(image), true, factor);
+          gate_factor(p.sigmoid, factor);
+          scaled(p.post.weight, 1.f, sw);
+#pragma unroll
+          for (int j = 0; j < N; ++j) sw[j] = mul2(sw[j], factor[j]);
+        }
+        --left;
+        if (p.post.kind) normalised(z[r], now1[r]);
+        float2 dg[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          float2 d = dh[r][j];
+          if (PIXEL) {
+            dg[j] = mul2(mul2(d, fma2(sw[j], z[r][j], sb[j])), gate_slope(p.sigmoid, g[r][j]));
+            d = mul2(d, g[r][j]);
+          }
+          a0[j] = fma2(d, z[r][j], a0[j]); a1[j] = add2(a1[j], d);
+          dh[r][j] = mul2(d, sw[j]);
+        }
+        if (PIXEL && p.dgate) cols.store(dgate.at(row + r), active, dg);
+      }
+      if (p.post.kind) {
+        float2 e[R][N];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+          for (int j = 0; j < N; ++j) e[r][j] = both(0.f);
+        }
+        norm_gradient<WIDE>(s, p.post.kind, now1, inv_c, z, dh, e);
+#pragma unroll
+        for (int r = 0; r < R; ++r) cols.store(dx.at(row + r), WIDE && R == 1 || row + r < w.hi, e[r]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r) cols.store(dx.at(row + r), WIDE && R == 1 || row + r < w.hi, dh[r]);
+      }
     }
   }
+  if (by_image && image >= 0) image_done();
   // the slots' sums, in slot order, in the threads of slot 0
   if (by_image) {
 #pragma unroll
@@ -707,16 +827,17 @@ residual_sums_kernel(const __grid_constant__ GeepsResidual p, int mode, int bloc
 }
 
 // ---- launches ----
-// stages of the ring: what fits, a power of two up to four (kRingBytes holds one of every kind of call with a ring)
-template <typename TR, typename TB, int K, bool VEC>
+// stages of the ring: what fits, up to four (kRingBytes holds one of every kind of call with a ring)
+template <typename TR, typename TB, int K, bool VEC, bool WIDE>
 int ring_depth(const GeepsResidual& p, const Shape& s, bool backward, size_t* bytes) {
+  typedef Form<TB, K, VEC, WIDE> F;
   const bool norm = p.mode & MODE_NORM, join = p.mode & MODE_JOIN, by_pixel = p.gate && p.gate_rows == p.rows, by_image = p.gate && !by_pixel;
   const int r = backward ? (norm ? 2 : 1) : 1, b = (backward && norm ? 1 : 0) + (join ? 1 : 0) + (by_pixel ? 1 : 0);
-  const size_t threads = backward || K > 1 ? 512 : 256;
-  auto stage = [&](int size) { return VEC ? K * 8 * size * threads : (size_t)((p.C * size + 15) / 16 + 1) * 16 * s.slots; };
+  const size_t threads = backward ? F::backward_threads : F::forward_threads;
+  auto stage = [&](int size) { return F::R * (VEC ? K * 8 * size * threads : (size_t)((p.C * size + 15) / 16 + 1) * 16 * s.slots); };
   const size_t one = r * stage(sizeof(TR)) + b * stage(sizeof(TB)), kept = backward && by_image ? (size_t)s.threads() * 16 * K * sizeof(float) : 0;
   const size_t room = kRingBytes / s.per_sm - kept;
-  const int depth = !Columns<K, VEC, 512>::RING ? 0 : one * 4 <= room ? 4 : one * 2 <= room ? 2 : 1;
+  const int depth = !Columns<K, VEC, 512>::RING ? 0 : one * 4 <= room ? 4 : (int)(room / one);
   *bytes = depth * one + kept;
   return depth;
 }
@@ -735,7 +856,7 @@ template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool P
 void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
   static bool forward_done[64] = {false}, backward_done[64] = {false};
   size_t smem = 0;
-  const int depth = ring_depth<TR, TB, K, VEC>(p, s, backward, &smem);
+  const int depth = ring_depth<TR, TB, K, VEC, WIDE>(p, s, backward, &smem);
   if (backward) {
     const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0;
     if (smem < meet) smem = meet;

@@ -516,86 +516,103 @@ class Norm:
     __slots__ = ("kind", "weight", "bias", "stats", "eps", "dweight", "dbias")
 
     def __init__(self, kind: str = "layer", weight=None, bias=None, stats=None, eps: float = 1e-5, dweight=None, dbias=None):
-        _need(kind in NORM_KINDS, f"unknown norm {kind!r}; one of {', '.join(NORM_KINDS)}")
-        _need(eps >= 0, "a norm's eps must not be negative")
+        if kind not in NORM_KINDS:
+            raise ValueError(f"unknown norm {kind!r}; one of {', '.join(NORM_KINDS)}")
+        if not eps >= 0:
+            raise ValueError("a norm's eps must not be negative")
         self.kind, self.weight, self.bias, self.stats, self.eps, self.dweight, self.dbias = kind, weight, bias, stats, eps, dweight, dbias
 
     def _pack(self, dev, rows, cols, backward):
         st = self.stats
-        _need(st is not None or not backward, "a norm's backward pass needs its stats")
-        _need(st is None or (st.dtype is torch.float32 and st.shape == (rows, 2) and st.is_contiguous() and st.get_device() == dev),
-              f"stats: need contiguous fp32 [{rows}, 2] on the same device")
-        return (_column(self.weight, dev, cols, "weight"), _column(self.bias, dev, cols, "bias"), 0 if st is None else st.data_ptr(),
-                _column(self.dweight, dev, cols, "dweight"), _column(self.dbias, dev, cols, "dbias"), self.eps, NORM_KINDS[self.kind])
+        if st is not None:
+            _need(st.dtype is torch.float32 and st.shape == (rows, 2) and st.is_contiguous() and st.get_device() == dev,
+                  "stats: need contiguous fp32 [rows, 2] on the same device")
+            at = st.data_ptr()
+        else:
+            _need(not backward, "a norm's backward pass needs its stats")
+            at = 0
+        w, b, dw, db = self.weight, self.bias, self.dweight, self.dbias
+        return (0 if w is None else _column(w, dev, cols), 0 if b is None else _column(b, dev, cols), at,
+                0 if dw is None or not backward else _column(dw, dev, cols), 0 if db is None or not backward else _column(db, dev, cols),
+                self.eps, NORM_KINDS[self.kind])
 
 
-def _column(t, dev, cols, what) -> int:
+def _column(t, dev, cols) -> int:
     """Address of an fp32 vector of one value a channel."""
-    if t is None:
-        return 0
-    _need(t.dtype is torch.float32 and t.numel() == cols and t.is_contiguous() and t.get_device() == dev,
-          f"{what}: need {cols} contiguous fp32 values on the same device")
-    return t.data_ptr()
+    if t.dtype is torch.float32 and t.numel() == cols and t.is_contiguous() and t.get_device() == dev:
+        return t.data_ptr()
+    raise ValueError(f"a norm's weight, bias and their gradients and the scale need {cols} contiguous fp32 values on cuda:{dev}, "
+                     f"got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _operand(t, dev, rows, cols, dtype, what):
-    """Address and pitch of a matrix of rows; rows are contiguous and may be a slice of wider ones."""
-    if t is None:
-        return 0, 0
-    _need(t.dim() == 2 and t.shape[0] == rows and t.shape[1] == cols, f"{what}: need [{rows}, {cols}], got {list(t.shape)}")
-    _need(t.dtype is dtype, f"{what}: need {dtype}, got {t.dtype}")
-    _need(t.get_device() == dev, f"{what}: need device cuda:{dev}, got {t.device}")
-    _need(cols == 1 or rows == 0 or t.stride(1) == 1, f"{what}: channels must be contiguous")
-    return t.data_ptr(), (t.stride(0) if rows > 1 else cols)
+def _operand(t, dev, shape, dtype, what, ld):
+    """Address of a matrix of rows, whose pitch goes to `ld`; rows are contiguous and may be a slice of wider ones."""
+    if t.shape == shape and t.dtype is dtype and t.get_device() == dev:
+        s = t.stride()
+        if s[1] == 1 or shape[1] == 1 or shape[0] == 0:
+            ld.append(s[0] if shape[0] > 1 else shape[1])
+            return t.data_ptr()
+        raise ValueError(f"{what}: channels must be contiguous, got strides {s}")
+    raise ValueError(f"{what}: need {dtype} [{shape[0]}, {shape[1]}] on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _residual(backward, x, res, out, y, dout, dy, dx, dres, post, pre, scale, dscale, gate, dgate, sigmoid, work, label):
-    L.require_cuda()
-    stream = dres if backward else res
-    _need(stream.dim() == 2, f"need [rows, channels], got {list(stream.shape)}")
-    rows, cols = stream.shape
-    dev = stream.get_device()
-    _need(dev == torch._C._cuda_getDevice(), f"{label}: tensors are on {stream.device}, the current device is cuda:{torch.cuda.current_device()}")
-    rt = stream.dtype
-    bt = (x if x is not None else dy if backward else y).dtype
-    _need((rt, bt) in ((bf16, bf16), (torch.float32, bf16), (torch.float32, torch.float32)),
-          f"{label}: types must be bf16, fp32, or fp32 along the residual connection and bf16 inside the block; got {rt}, {bt}")
-    gate_rows = 0
+def _residual(label, backward, tensors, post, pre, scale, dscale, sigmoid, work):
+    """One call of the native residual_forward / residual_backward.  tensors: x, res, gate, out, y, dout, dy, dx, dres, dgate."""
+    x, gate, stream = tensors[0], tensors[2], tensors[8 if backward else 1]
+    block = x if x is not None else tensors[6 if backward else 4]
+    shape, dev, rt, bt = stream.shape, stream.get_device(), stream.dtype, block.dtype
+    if len(shape) != 2:
+        raise ValueError(f"{label}: need [rows, channels], got {list(shape)}")
+    if dev != torch._C._cuda_getDevice() or dev < 0:
+        L.require_cuda()
+        raise ValueError(f"{label}: tensors are on {stream.device}, the current device is cuda:{torch.cuda.current_device()}")
+    f32 = torch.float32
+    if not ((rt is bf16 or rt is f32) and (bt is bf16 or (bt is f32 and rt is f32))):
+        raise ValueError(f"{label}: types must be bf16, fp32, or fp32 along the residual connection and bf16 inside the block; got {rt}, {bt}")
+    rows, cols = shape
+    gate_rows, gate_shape, ld, v = 0, None, [], []
     if gate is not None:
         gate_rows = gate.shape[0]
-    ops = (_operand(x, dev, rows, cols, bt, "x"), _operand(res, dev, rows, cols, rt, "res"),
-           _operand(gate, dev, gate_rows, cols, bt, "gate"), _operand(out, dev, rows, cols, rt, "out"),
-           _operand(y, dev, rows, cols, bt, "y"), _operand(dout, dev, rows, cols, rt, "dout"),
-           _operand(dy, dev, rows, cols, bt, "dy"), _operand(dx, dev, rows, cols, bt, "dx"),
-           _operand(dres, dev, rows, cols, rt, "dres"), _operand(dgate, dev, gate_rows, cols, bt, "dgate"))
+        gate_shape = (gate_rows, cols)
+    for t, what, of_stream, of_gate in zip(tensors, _NAMES, _STREAM, _GATE):
+        if t is None:
+            v.append(0)
+            ld.append(0)
+        else:
+            v.append(_operand(t, dev, gate_shape if of_gate else shape, rt if of_stream else bt, what, ld))
     mode = (2 if x is not None else 0) | (1 if pre is not None else 0)
+    at = 0
     if backward:
         n = lib().geeps_residual_work(C.c_longlong(rows), C.c_longlong(gate_rows), cols, mode)
-        if work is None and n:
-            work = L.hold(torch.empty(n, dtype=torch.float32, device=stream.device))
-        _need(not n or (work.dtype is torch.float32 and work.is_contiguous() and work.numel() >= n and work.get_device() == dev),
-              f"{label}: work needs {n} contiguous fp32 values")
-    p = [o[0] for o in ops]
-    p += [_column(scale, dev, cols, "scale"), _column(dscale, dev, cols, "dscale"), 0 if work is None else work.data_ptr()]
-    p += post._pack(dev, rows, cols, backward) if post is not None else _NO_NORM
-    p += pre._pack(dev, rows, cols, backward) if pre is not None else _NO_NORM
-    ld = [o[1] for o in ops]
-    f32 = torch.float32
-    packed = L.RESIDUAL.pack(*p, rows, gate_rows, ld[0], ld[1], ld[2], ld[3], ld[4], ld[5], ld[6], ld[7], ld[8], ld[9], cols,
-                             mode, rt is f32, bt is f32, bool(sigmoid))
-    launch(lib().geeps_residual_backward if backward else lib().geeps_residual_forward, label, packed, stream_ptr())
+        if n:
+            if work is None:
+                work = L.hold(torch.empty(n, dtype=f32, device=stream.device))
+            elif not (work.dtype is f32 and work.is_contiguous() and work.numel() >= n and work.get_device() == dev):
+                raise ValueError(f"{label}: work needs {n} contiguous fp32 values on cuda:{dev}")
+            at = work.data_ptr()
+    launch(lib().geeps_residual_backward if backward else lib().geeps_residual_forward, label,
+           L.RESIDUAL.pack(*v, 0 if scale is None else _column(scale, dev, cols), 0 if dscale is None else _column(dscale, dev, cols), at,
+                           *(_NO_NORM if post is None else post._pack(dev, rows, cols, backward)),
+                           *(_NO_NORM if pre is None else pre._pack(dev, rows, cols, backward)),
+                           rows, gate_rows, *ld, cols, mode, rt is f32, bt is f32, bool(sigmoid)),
+           C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+
+
+_NAMES = ("x", "res", "gate", "out", "y", "dout", "dy", "dx", "dres", "dgate")
+_STREAM = tuple(n in ("res", "out", "dout", "dres") for n in _NAMES)
+_GATE = tuple(n in ("gate", "dgate") for n in _NAMES)
 
 
 def norm_forward(x, y, norm: Norm) -> None:
     """y = norm(x) over the channels of every row.  x: [rows, C] bf16 or fp32; y: the same, or bf16 beside fp32 x.  Any C up to
     16384, any pitch, rows of a wider matrix; y may be x itself."""
-    _residual(False, None, x, None, y, None, None, None, None, None, norm, None, None, None, None, False, None, "norm_forward")
+    _residual("norm_forward", False, (None, x, None, None, y, None, None, None, None, None), None, norm, None, None, False, None)
 
 
 def norm_backward(x, dy, dx, norm: Norm, dres=None, work=None) -> None:
     """dx = gradient of norm_forward()'s input for dy, plus dres: what reaches x on its way round the block.  Types as there, dx and
     dres like x.  work: norm_work() floats to use instead of memory taken from the allocator for the call."""
-    _residual(True, None, None, x, None, dres, dy, None, dx, None, norm, None, None, None, None, False, work, "norm_backward")
+    _residual("norm_backward", True, (None, None, None, x, None, dres, dy, None, dx, None), None, norm, None, None, False, work)
 
 
 def residual_forward(x, res, out, *, post: Norm | None = None, scale=None, gate=None, sigmoid: bool = False, y=None,
@@ -604,8 +621,9 @@ def residual_forward(x, res, out, *, post: Norm | None = None, scale=None, gate=
     `pre`, y = pre(out).  scale: fp32 [C]; g: gate, or its sigmoid, a row a pixel or one for each group of rows / gate rows
     neighbouring pixels (an image's).  Types: all bf16, all fp32, or res and out fp32 with bf16 x, gate and y.
     y is taken of out before it is rounded to its type."""
-    _need(x is not None and (y is None) == (pre is None), "residual_forward: need x, and y exactly with pre")
-    _residual(False, x, res, out, y, None, None, None, None, post, pre, scale, None, gate, None, sigmoid, None, "residual_forward")
+    if x is None or (y is None) != (pre is None):
+        raise ValueError("residual_forward: need x, and y exactly with pre")
+    _residual("residual_forward", False, (x, res, gate, out, y, None, None, None, None, None), post, pre, scale, None, sigmoid, None)
 
 
 def residual_backward(x, dout, dx, dres, *, post: Norm | None = None, scale=None, dscale=None, gate=None, dgate=None,
@@ -616,7 +634,7 @@ def residual_backward(x, dout, dx, dres, *, post: Norm | None = None, scale=None
     _need(x is not None and (dy is None) == (pre is None) and (out is not None or pre is None) and (dout is not None or pre is not None),
           "residual_backward: need x, dy and out with pre, dout without")
     _need(dgate is None or gate is not None, "residual_backward: dgate without a gate")
-    _residual(True, x, None, out, None, dout, dy, dx, dres, post, pre, scale, dscale, gate, dgate, sigmoid, work, "residual_backward")
+    _residual("residual_backward", True, (x, None, gate, out, None, dout, dy, dx, dres, dgate), post, pre, scale, dscale, sigmoid, work)
 
 
 def norm_work(rows: int, cols: int, gate_rows: int = 0, join: bool = False, pre: bool = True) -> int:
@@ -657,18 +675,19 @@ def clip_gradients(grads, max_norm: float, result: torch.Tensor, out=None) -> No
     has grads[i]'s count).  result: fp32 [2] on the device, receives N and the coefficient (1 where nothing is clipped).
     Without `out` nothing is written to the gradients where nothing is clipped; max_norm = inf only measures.  A norm that is
     infinite gives the coefficient 0 and one that is not a number 1: the gradients then carry it on."""
-    L.require_cuda()
     grads = grads if isinstance(grads, GradList) else GradList(grads)
     out = out if out is None or isinstance(out, GradList) else GradList(out)
-    _need(max_norm >= 0, f"clip_gradients: max_norm must be a number from 0 up, got {max_norm}")
+    if not max_norm >= 0:
+        raise ValueError(f"clip_gradients: max_norm must be a number from 0 up, got {max_norm}")
     _need(out is None or out.numel == grads.numel, "clip_gradients: out and grads differ in their counts")
     _need(result.dtype is torch.float32 and result.numel() == 2 and result.is_contiguous() and result.is_cuda,
           "clip_gradients: result needs two contiguous fp32 values on the device")
     dev = result.get_device()
-    _need(dev == torch._C._cuda_getDevice(), f"clip_gradients: result is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"clip_gradients: result is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     for t in (grads, out):
         _need(t is None or not t.tensors or t.device.index == dev, "clip_gradients: need every tensor on the current device")
     work = L.hold(torch.empty(lib().geeps_clip_work(C.byref(grads.native)), dtype=torch.float64, device=result.device))
     L.hold((grads, out))
     launch(lib().geeps_clip_gradients, "clip_gradients", C.byref(grads.native), None if out is None else C.byref(out.native),
-           C.c_double(max_norm), ptr(result), ptr(work), stream_ptr())
+           C.c_double(max_norm), ptr(result), ptr(work), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))

@@ -18,7 +18,7 @@ def shape(rows, c, backward=True, mode=3):
 @pytest.mark.parametrize("mode", [1, 3])
 def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode):
     vectors, slot, slots, blocks = shape(rows, c, backward, mode)
-    assert slot * slots <= (256 if vectors == 1 and not backward else 512)
+    assert slot * slots <= (512 if vectors > 1 or (backward and slot < 32) else 384 if backward else 256)
     assert vectors * slot * 8 >= c and slot * slots <= 512 and slots >= 1
     assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
     assert slot <= 32 or slots <= 15                    # a named barrier for each slot
