@@ -158,7 +158,7 @@ typedef struct GeepsNorm {
 // the join; without x, out holds the norm's input.  Pitches in elements.  stream_fp32: res, out, dout and dres are fp32,
 // else bf16; block_fp32 (with stream_fp32 only): x, y, gate, dy, dx and dgate.  An output may be the very same rows as an
 // input of its size; any other overlap of an output with another operand is refused.  Rows are
-// less than 2^31 - 256, pitches than 2^29 (no rows: the parameters' gradients are zeros), C is 1 to 16384, every address will do.  work: geeps_residual_work() floats,
+// at most 2^30, pitches less than 2^29 (no rows: the parameters' gradients are zeros), C is 1 to 16384, every address will do.  work: geeps_residual_work() floats,
 // private to the call while it runs.  mode: 1 for a norm alone (no x), 2 for a join, 3 for a join with a norm behind it.
 #define GEEPS_ERR_NORM_CHANNELS (-10)
 #define GEEPS_ERR_NORM_GATE (-11)

@@ -49,7 +49,7 @@ bool clash(const Use& a, const Use& b, int C) {
 
 int check(const GeepsResidual& p, bool backward, int mode, bool* vec) {
   if (p.C < 1 || p.C > kMaxChannels) return GEEPS_ERR_NORM_CHANNELS;
-  if (p.rows < 0 || p.rows > 0x7fffff00LL) return (int)cudaErrorInvalidValue;
+  if (p.rows < 0 || p.rows > 1LL << 30) return (int)cudaErrorInvalidValue;
   if (p.gate && (p.gate_rows < 1 || p.gate_rows > p.rows || p.rows % p.gate_rows)) return p.rows ? GEEPS_ERR_NORM_GATE : 0;
   if (p.stream_fp32 == 0 && p.block_fp32) return (int)cudaErrorInvalidValue;
   const int r = p.stream_fp32 ? 4 : 2, b = p.block_fp32 ? 4 : 2;

@@ -9,7 +9,7 @@ namespace rownorm {
 
 constexpr int kMaxChannels = 16384;
 constexpr int kVec = 8;                 // channels a vector
-constexpr int kRingBytes = 196 * 1024;  // shared memory of an SM for rows on their way
+constexpr int kRingBytes = 200 * 1024;  // shared memory of an SM for rows on their way
 enum { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 enum { MODE_NORM = 1, MODE_JOIN = 2, MODE_BOTH = 3 };     // the next norm alone, a join alone, a join and the norm behind it
 
@@ -119,6 +119,7 @@ struct Columns {
   static constexpr bool RING = K <= 2;
   int t, slot, C, slots;
   __device__ __forceinline__ int first() const { return VEC ? at(0) : 0; }
+  __device__ __forceinline__ static constexpr int threads() { return THREADS; }
   __device__ __forceinline__ int at(int j) const { return VEC ? (t + (j >> 3) * slot) * 8 + (j & 7) : t + j * slot; }
   __device__ __forceinline__ bool on(int j) const { return at(VEC ? j & ~7 : j) < C; }
 
@@ -388,7 +389,6 @@ __device__ __forceinline__ void gate_factor(int through_sigmoid, float2 (&g)[N])
 __device__ __forceinline__ float2 gate_slope(int through_sigmoid, float2 g) {       // of the factor g by the gate
   return through_sigmoid ? make_float2(g.x * (1.f - g.x), g.y * (1.f - g.y)) : both(1.f);
 }
-__device__ __forceinline__ float2 stats_of(const GeepsNorm& norm, int row) { return *reinterpret_cast<const float2*>(norm.stats + 2LL * row); }
 
 // zeros to the ring, before any copy
 __device__ __forceinline__ void clear_ring(unsigned char* ring, int bytes) {
@@ -399,11 +399,14 @@ __device__ __forceinline__ void clear_ring(unsigned char* ring, int bytes) {
 // The rows of a slot, R a turn.  Slots that share a warp take the same number of turns, since its lanes meet in sums: some have
 // no row in the last.
 struct Walk {
-  int lo, hi, turns;
-  __device__ __forceinline__ Walk(const GeepsResidual& p, int slots, int id, bool wide, int R) {
+  int lo, hi, step, turns;
+  __device__ __forceinline__ Walk(const GeepsResidual& p, int slots, int id, bool wide, int R, bool ranges) {
     const int rows = (int)p.rows, all = gridDim.x * slots, me = blockIdx.x * slots + id;
-    lo = first_row(rows, all, me); hi = first_row(rows, all, me + 1);
-    turns = wide ? (hi - lo + R - 1) / R : rows / all + (rows % all ? 1 : 0);
+    lo = ranges ? first_row(rows, all, me) : me * R;
+    hi = ranges ? first_row(rows, all, me + 1) : rows;
+    step = ranges ? R : all * R;
+    const int most = ranges ? (rows + all - 1) / all : (rows + step - 1) / step;
+    turns = !wide ? most : lo < hi ? (hi - lo + step - 1) / step : 0;
   }
 };
 
@@ -440,7 +443,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
   };
   if ((MODE & MODE_JOIN) && !by_image) join_params();
   if (MODE & MODE_NORM) { cols.param(p.pre.weight, 1.f, w2); cols.param(p.pre.bias, 0.f, b2); }
-  const Walk w(p, slots, s.id, WIDE, R);
+  const Walk w(p, slots, s.id, WIDE, R, by_image);
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
   int left = 0;                                // rows to go with the gate at hand
 
@@ -462,7 +465,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
         if (PIXEL) cols.copy(gate.at(row), to + at_g);
       }
     }
-    ahead += R;
+    ahead += w.step;
     in = in == last ? 0 : in + R * one;
     copy_commit();
   };
@@ -471,7 +474,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
     for (int i = 0; i < depth - 1; ++i) copy();
   }
   for (int i = 0; i < w.turns; ++i) {
-    const int row = w.lo + i * R;
+    const int row = w.lo + i * w.step;
     if (cols.RING) {
       if (!VEC) s.sync();
       copy();
@@ -546,9 +549,11 @@ __global__ void __launch_bounds__(Form<TB, K, VEC, WIDE>::backward_threads)
 residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float2 stats[2][512];
   __shared__ __align__(16) float red[16][128];
   constexpr int N = 4 * K, R = Form<TB, K, VEC, WIDE>::R;
   for (int i = threadIdx.x; i < 16 * 128; i += blockDim.x) red[0][i] = 0.f;
+  for (int i = threadIdx.x; i < 2 * 512; i += blockDim.x) stats[0][i] = both(0.f);
   __syncthreads();
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
@@ -573,7 +578,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
 #pragma unroll
     for (int i = 0; i < N; ++i) n0[i] = n1[i] = both(0.f);
   }
-  const Walk w(p, slots, s.id, WIDE, R);
+  const Walk w(p, slots, s.id, WIDE, R, by_image);
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
   int image = -1, left = 0;
 
@@ -607,7 +612,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         if (PIXEL) cols.template no_row<TB>(to + at_g);
       }
     }
-    ahead += R;
+    ahead += w.step;
     in = in == last ? 0 : in + R * one;
     copy_commit();
   };
@@ -645,21 +650,8 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     clear_ring(ring, depth * R * one);
     for (int i = 0; i < depth - 1; ++i) copy();
   }
-  // the statistics of a turn's rows come a turn before
-  float2 st1[R], st2[R];
-  auto statistics = [&](int row) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int q = row + r < w.hi ? row + r : w.hi - 1;
-      st1[r] = st2[r] = both(0.f);
-      if (!WIDE && w.lo == w.hi) continue;
-      if ((MODE & MODE_JOIN) && p.post.kind) st1[r] = stats_of(p.post, q);
-      if (MODE & MODE_NORM) st2[r] = stats_of(p.pre, q);
-    }
-  };
-  if (w.turns) statistics(w.lo);
   for (int i = 0; i < w.turns; ++i) {
-    const int row = w.lo + i * R;
+    const int row = w.lo + i * w.step;
     if (cols.RING) {
       if (!VEC) s.sync();
       copy();
@@ -668,10 +660,25 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
     const uint32_t from = base + out;
     if (cols.RING) out = out == last ? 0 : out + R * one;
+    // Statistics of the rows of several turns at a time, a row a lane: a load for every turn was waited for in the turn that
+    // issued it, with the loads from shared memory that share its scoreboard (50176 x 576: 36 % of the time).
+    const int chunk = WIDE ? 32 : slot, k = i * R & (chunk - 1);
+    if (k == 0) {
+      const int turn = i + (s.t & (chunk - 1)) / R, q = w.lo + turn * w.step + (s.t & (R - 1));
+      __syncwarp();
+      if (turn < w.turns && q < w.hi) {
+        if ((MODE & MODE_JOIN) && p.post.kind) stats[0][threadIdx.x] = *reinterpret_cast<const float2*>(p.post.stats + 2LL * q);
+        if (MODE & MODE_NORM) stats[1][threadIdx.x] = *reinterpret_cast<const float2*>(p.pre.stats + 2LL * q);
+      }
+      __syncwarp();
+    }
     float2 now1[R], now2[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) { now1[r] = st1[r]; now2[r] = st2[r]; }
-    statistics(row + R);
+    for (int r = 0; r < R; ++r) {
+      const int lane = (threadIdx.x & ~(chunk - 1)) + k + r;
+      now1[r] = MODE & MODE_JOIN ? stats[0][lane] : both(0.f);
+      now2[r] = MODE & MODE_NORM ? stats[1][lane] : both(0.f);
+    }
     // an output may lie where an operand does: without a ring everything of the row is read before its first output is written
     float2 dh[R][N], z[R][N], g[R][N];
     auto load_branch = [&]() {
@@ -845,10 +852,10 @@ int ring_depth(const GeepsResidual& p, const Shape& s, bool backward, size_t* by
 // done: one a kernel
 template <typename F>
 void allow_shared(F kernel, size_t bytes, bool (&done)[64]) {
-  if (bytes <= 32 * 1024) return;             // the default limit, 48 KB, less what the kernels have statically
+  if (bytes <= 24 * 1024) return;             // the default limit, 48 KB, less what the kernels have statically
   int dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 && done[dev]) return;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 212 * 1024) == cudaSuccess && dev >= 0 && dev < 64)
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024) == cudaSuccess && dev >= 0 && dev < 64)
     done[dev] = true;
 }
 
