@@ -179,8 +179,10 @@ typedef struct GeepsResidual {
 long long geeps_residual_work(long long rows, long long gate_rows, int C, int mode);
 int geeps_residual_forward(const GeepsResidual* p, void* stream);
 int geeps_residual_backward(const GeepsResidual* p, void* stream);
-// launch shape (host arithmetic only): vectors a thread, threads a row, rows a block at a time, blocks
-int geeps_norm_shape(long long rows, int C, int backward, int mode, int* out);
+// launch shape (host arithmetic only), eight values: vectors a thread, threads a row, rows a block at a time, blocks, blocks an
+// SM, stages of the ring, bytes of shared memory, rows read where they lie; vec: rows of whole, aligned vectors
+int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int backward, int vec, int stream_fp32, int block_fp32,
+                     int* out);
 
 // ---- clipping of gradients by their global norm (the reference's solver had it in its absent Caffe application) ----
 // norm = sqrt(sum over all tensors of g^2), c = norm > max_norm ? max_norm / norm : 1, dst = c * g; dst NULL: in place, and

@@ -107,17 +107,27 @@ int residual(const GeepsResidual* q, bool backward, void* stream) {
 
 }  // namespace
 
+// The most that any layout and types of these sizes take
 extern "C" long long geeps_residual_work(long long rows, long long gate_rows, int C, int mode) {
-  if (rows <= 0 || C < 1 || C > kMaxChannels) return 0;
-  const Shape s = plan(rows, C, true, mode);
+  if (rows <= 0 || C < 1 || C > kMaxChannels || mode < MODE_NORM || mode > MODE_BOTH) return 0;
   const bool by_image = gate_rows > 0 && gate_rows < rows;
-  if (s.blocks == 1 && !by_image) return 0;
-  return ((long long)s.blocks * sums_of(mode) + (by_image ? (long long)s.blocks * s.slots + gate_rows : 0)) * C;
+  long long most = 0;
+  for (int form = 0; form < 6; ++form) {
+    const Call c = {true, form < 3, gate_rows == rows, by_image, mode, form % 3 ? 4 : 2, form % 3 == 2 ? 4 : 2};
+    const Shape s = plan(rows, C, c);
+    if (s.blocks == 1 && !by_image) continue;
+    const long long n = work_floats(s, C, mode, by_image ? gate_rows : 0);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 extern "C" int geeps_residual_forward(const GeepsResidual* p, void* stream) { return residual(p, false, stream); }
 extern "C" int geeps_residual_backward(const GeepsResidual* p, void* stream) { return residual(p, true, stream); }
-extern "C" int geeps_norm_shape(long long rows, int C, int backward, int mode, int* out) {
-  const Shape s = plan(rows, C, backward != 0, mode);
-  out[0] = s.vectors; out[1] = s.slot; out[2] = s.slots; out[3] = s.blocks;
+extern "C" int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int backward, int vec, int stream_fp32, int block_fp32,
+                                int* out) {
+  const bool by_image = gate_rows > 0 && gate_rows < rows;
+  const Shape s = plan(rows, C, {backward != 0, vec != 0, gate_rows == rows, by_image, mode, stream_fp32 ? 4 : 2, block_fp32 ? 4 : 2});
+  const int v[8] = {s.vectors, s.slot, s.slots, s.blocks, s.per_sm, s.depth, (int)s.smem, s.large};
+  for (int i = 0; i < 8; ++i) out[i] = v[i];
   return 0;
 }

@@ -14,30 +14,73 @@ enum { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 enum { MODE_NORM = 1, MODE_JOIN = 2, MODE_BOTH = 3 };     // the next norm alone, a join alone, a join and the norm behind it
 
 // ---- launch shape ----
+// VEC: rows of whole, aligned vectors.  LARGE: rows that registers and shared memory do not hold.
 struct Shape {
   int vectors;       // vectors a thread
   int slot;          // threads a row: a power of two up to 32, or whole warps
   int slots;         // rows a block works on at a time
-  int blocks, per_sm;
+  int blocks, per_sm, depth;
+  bool large;
+  size_t smem;
   int threads() const { return slot * slots; }
 };
-// K vectors a thread: as few as the threads of a block allow, since what a thread keeps for its columns is in registers.  A
-// block of the backward pass has up to 384 (rows of up to 384 vectors, but of more than 16) or 512 threads and an SM to itself,
-// so that few blocks leave column sums behind; forward several blocks of 256 share an SM.
-inline Shape plan(long long rows, int C, bool backward, int mode) {
-  Shape s;
-  const int vec = (C + kVec - 1) / kVec;
-  const int narrow = vec <= 16, one = backward ? 384 : 256;
-  s.vectors = vec <= one ? 1 : vec <= 1024 ? 2 : 4;
-  const int need = (vec + s.vectors - 1) / s.vectors, most = s.vectors > 1 ? 512 : backward ? narrow ? 512 : 384 : 256;
-  s.slot = 1;
-  if (need <= 32) while (s.slot < need) s.slot <<= 1;
-  else s.slot = (need + 31) / 32 * 32;
-  s.slots = s.slot > most / 2 ? 1 : most / s.slot;
-  s.per_sm = backward || s.vectors > 1 ? 1 : mode == MODE_NORM ? 3 : 2;
-  const long long room = (long long)geeps_sm_count() * s.per_sm, want = (rows + s.slots - 1) / s.slots;
-  s.blocks = (int)(want < room ? want : room);
-  return s;
+// Blocks of the backward pass have up to 384 threads (168 registers each) and an SM to themselves, so that few blocks leave
+// column sums behind; forward several blocks of 256 share an SM.
+constexpr int kForwardThreads = 256, kBackwardThreads = 384, kLargeThreads = 512;
+constexpr int block_threads(bool backward, bool large) { return large ? kLargeThreads : backward ? kBackwardThreads : kForwardThreads; }
+
+// What a call keeps in shared memory: parameters of the columns (one vector a thread keeps them in registers), with a gate per
+// image its factors, and the ring.
+struct Call {
+  bool backward, vec, by_pixel, by_image;
+  int mode, stream, block;                 // sizes of the two types
+};
+inline size_t fixed_bytes(const Call& c, const Shape& s) {
+  const bool norm = c.mode & 1, join = c.mode & 2;
+  const int params = c.backward ? (norm ? 1 : 0) + (join ? c.by_pixel ? 2 : 1 : 0) : (norm ? 2 : 0) + (join ? 2 : 0);
+  const size_t thread = (size_t)8 * s.vectors * sizeof(float);         // a value for each of a thread's columns
+  return (s.large || s.vectors == 1 ? 0 : params * thread * s.slot) +
+         (c.by_image && !s.large ? thread * block_threads(c.backward, s.large) : 0);
+}
+inline size_t stage_bytes(const Call& c, const Shape& s, int C) {
+  const bool norm = c.mode & 1, join = c.mode & 2;
+  const int r = c.backward ? (norm ? 2 : 1) : 1, b = (c.backward && norm ? 1 : 0) + (join ? 1 : 0) + (c.by_pixel ? 1 : 0);
+  auto stage = [&](int size) {
+    return c.vec ? (size_t)s.vectors * 8 * size * block_threads(c.backward, false) : (size_t)((C * size + 15) / 16 + 1) * 16 * s.slots;
+  };
+  return r * stage(c.stream) + b * stage(c.block);
+}
+// How many vectors a thread has: more save what every thread does once a row, up to the registers (backward the column sums of
+// a join and of a norm behind it leave room for two), fewer leave no lane without work.  The costs are instructions a row.
+// Eight threads a row at least, where there is so much: a row's pieces in a warp's access are then whole lines.
+inline Shape plan(long long rows, int C, const Call& c) {
+  Shape best;
+  const int vec = (C + kVec - 1) / kVec, most = c.vec ? c.backward && c.mode != 1 ? 2 : 4 : 2;
+  long long least = -1;
+  for (int k = 1; k <= most + 1; ++k) {
+    Shape s;
+    s.large = k > most;
+    s.vectors = s.large ? 4 : k;
+    const int need = (vec + s.vectors - 1) / s.vectors, limit = block_threads(c.backward, s.large);
+    if (need > limit || (s.large && least >= 0)) continue;
+    s.slot = 1;
+    while (s.slot < 32 && (s.slot < need || (s.slot < 8 && s.slot < vec))) s.slot <<= 1;
+    if (need > 32 || s.large) s.slot = (need + 31) / 32 * 32;
+    if (s.slot >= 32 && s.vectors == 1 && c.vec) continue;
+    if (s.slot < 32 && s.vectors == 2 && !c.vec) continue;
+    s.slots = limit / s.slot;
+    s.per_sm = c.backward || s.large ? 1 : c.mode == 1 ? 4 : 2;
+    s.smem = fixed_bytes(c, s);
+    const size_t room = kRingBytes / s.per_sm, stage = stage_bytes(c, s, C);
+    s.depth = s.large || s.smem > room ? 0 : s.smem + 4 * stage <= room ? 4 : (int)((room - s.smem) / stage);
+    if (!s.large && s.depth < 1) continue;
+    s.smem += s.depth * stage;
+    const long long cost = (long long)s.slot * (100 + 45 * s.vectors + (s.slot > 32 ? 60 : 0));
+    if (least < 0 || (cost < least && c.vec)) { least = cost; best = s; }       // single columns cost the same for any k
+  }
+  const long long room = (long long)geeps_sm_count() * best.per_sm, want = (rows + best.slots - 1) / best.slots;
+  best.blocks = (int)(want < room ? want : room);
+  return best;
 }
 // rows [first_row(i), first_row(i + 1)) are slot i's, of all slots of all blocks; rows are less than 2^31
 __host__ __device__ inline int first_row(int rows, int slots, int i) {
@@ -104,22 +147,20 @@ __device__ __forceinline__ float ld_shared1(uint32_t a) {
 }
 
 // ---- a thread's columns ----
-// Eight a vector, held as pairs.  VEC: vectors t, t + slot, ...: 16- or 32-byte accesses.  Otherwise (odd widths, pitches or
+// K vectors of eight, held as pairs.  VEC: vectors t, t + slot, ...: 16- or 32-byte accesses.  Otherwise (odd widths, pitches or
 // addresses) single columns t, t + slot, ...: neighbouring threads on neighbouring columns.  A thread without a column at some
 // place has zeros there.
 // Rows come through a ring of `depth` stages in shared memory, so that what is on its way takes no registers.  With VEC a thread
 // copies what it reads itself and nobody waits for anybody; otherwise the slot copies the 16-byte pieces that hold the row (up
 // to 15 bytes before and behind it in the same pieces come along) and meets before and after reading them.  The ring starts as
-// zeros, so what has no column or no operand is read from it like the rest.  Rows of more than two vectors a thread do not
-// fit and are read where they lie.
-// THREADS: as many as a block may have; a thread's places in the ring are then the same for every launch.
-template <int K, bool VEC, int THREADS>
+// zeros, so what has no column or no operand is read from it like the rest.  Rows that do not fit (RING = false) are read where
+// they lie.  THREADS: as many as a block may have; a thread's places in the ring are then the same for every launch.
+template <int K, bool VEC, bool RING_, int THREADS>
 struct Columns {
   static constexpr int N = 4 * K;      // pairs
-  static constexpr bool RING = K <= 2;
+  static constexpr bool RING = RING_;
   int t, slot, C, slots;
   __device__ __forceinline__ int first() const { return VEC ? at(0) : 0; }
-  __device__ __forceinline__ static constexpr int threads() { return THREADS; }
   __device__ __forceinline__ int at(int j) const { return VEC ? (t + (j >> 3) * slot) * 8 + (j & 7) : t + j * slot; }
   __device__ __forceinline__ bool on(int j) const { return at(VEC ? j & ~7 : j) < C; }
 
@@ -135,7 +176,7 @@ struct Columns {
       constexpr int Q = 8 * sizeof(T) / 16;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        if (K > 1 && !on(8 * k)) continue;         // K = 1: the caller has asked
+        if (!on(8 * k)) continue;
 #pragma unroll
         for (int q = 0; q < Q; ++q) copy16(to + (k * Q + q) * THREADS * 16, from + k * slot * 8 + q * (8 / Q));
       }
@@ -196,10 +237,11 @@ struct Columns {
     } else {
       const uint32_t r = from + (threadIdx.x / slot) * pieces<T>() + (uint32_t)((uintptr_t)rows.at(row) & 15);
       const bool any = active && there;
+      float v[2 * N];              // without branches: beyond the row the last column is read and dropped
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        f[i] = make_float2(any && on(2 * i) ? ld_shared1<T>(r + at(2 * i) * (int)sizeof(T)) : 0.f,
-                           any && on(2 * i + 1) ? ld_shared1<T>(r + at(2 * i + 1) * (int)sizeof(T)) : 0.f);
+      for (int j = 0; j < 2 * N; ++j) v[j] = ld_shared1<T>(r + (on(j) ? at(j) : C - 1) * (int)sizeof(T));
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = make_float2(any && on(2 * i) ? v[2 * i] : 0.f, any && on(2 * i + 1) ? v[2 * i + 1] : 0.f);
     }
   }
   template <typename T>
@@ -225,12 +267,6 @@ struct Columns {
       for (int j = 0; j < 2 * N; ++j) if (on(j)) row[at(j)] = (T)(j & 1 ? f[j >> 1].y : f[j >> 1].x);
     }
   }
-  // a parameter of every column; `other` where there is none
-  __device__ __forceinline__ void param(const float* p, float other, float2 (&f)[N]) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      f[i] = make_float2(!on(2 * i) ? 0.f : p ? p[at(2 * i)] : other, !on(2 * i + 1) ? 0.f : p ? p[at(2 * i + 1)] : other);
-  }
   // f - mean, zero where there is no column
   __device__ __forceinline__ void subtract(float2 (&f)[N], float mean) const {
     if (VEC) {
@@ -250,9 +286,90 @@ struct Columns {
   }
 };
 
+// A parameter of every column: one, times another, or `other` where there is none.  In registers for one vector a thread, else
+// in shared memory (16 bytes of a vector's half beside those of the next thread), read for every row; rows that do not fit read
+// it where it lies.
+template <typename C_, int K, bool VEC>
+struct Param {
+  static constexpr bool REG = K == 1 && C_::RING, SHARED = K > 1 && C_::RING;
+  float2 reg[REG ? 4 * K : 1];
+  uint32_t at;
+  const float *one, *two;
+  float other;
+  __device__ __forceinline__ float value(int c) const { return (one ? one[c] : other) * (two ? two[c] : 1.f); }
+  // `area` moves on behind what is taken; the block meets before the first get()
+  __device__ __forceinline__ void set(const C_& cols, const float* a, float b, const float* c, unsigned char*& area) {
+    one = a; two = c; other = b;
+    if (REG) {
+#pragma unroll
+      for (int i = 0; i < C_::N; ++i)
+        reg[REG ? i : 0] = make_float2(cols.on(2 * i) ? value(cols.at(2 * i)) : 0.f, cols.on(2 * i + 1) ? value(cols.at(2 * i + 1)) : 0.f);
+    } else if (SHARED) {
+      float* to = reinterpret_cast<float*>(area);
+      for (int i = threadIdx.x; i < 8 * K * cols.slot; i += blockDim.x) {
+        int col = i;
+        if (VEC) {         // [k][half][thread][4]
+          const int e = i & 3, q = i >> 2, t = q % cols.slot, h = q / cols.slot;
+          col = (t + (h >> 1) * cols.slot) * 8 + (h & 1) * 4 + e;
+        }
+        to[i] = col < cols.C ? value(col) : 0.f;
+      }
+      at = (uint32_t)__cvta_generic_to_shared(area) + cols.t * (VEC ? 16 : 4);
+      area += 8 * K * cols.slot * sizeof(float);
+    }
+  }
+  // pairs 4 k to 4 k + 3
+  __device__ __forceinline__ void get(const C_& cols, int k, float2 (&f)[4]) const {
+    if (REG) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = reg[REG ? 4 * k + e : 0];
+    } else if (SHARED && VEC) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 v = ld_shared16(at + (2 * k + h) * cols.slot * 16);
+        f[2 * h] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+        f[2 * h + 1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+      }
+    } else if (SHARED) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f[e] = make_float2(ld_shared1<float>(at + (8 * k + 2 * e) * cols.slot * 4), ld_shared1<float>(at + (8 * k + 2 * e + 1) * cols.slot * 4));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = 8 * k + 2 * e;
+        f[e] = make_float2(cols.on(j) ? value(cols.at(j)) : 0.f, cols.on(j + 1) ? value(cols.at(j + 1)) : 0.f);
+      }
+    }
+  }
+};
+// A thread's own values of its columns in shared memory: 16 bytes beside those of the next thread
+template <int K, int THREADS>
+struct Own {
+  uint32_t at;
+  __device__ __forceinline__ void set(unsigned char*& area) {
+    at = (uint32_t)__cvta_generic_to_shared(area) + threadIdx.x * 16;
+    area += 8 * K * THREADS * sizeof(float);
+  }
+  __device__ __forceinline__ void get(int k, float2 (&f)[4]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 v = ld_shared16(at + (2 * k + h) * THREADS * 16);
+      f[2 * h] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+      f[2 * h + 1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+    }
+  }
+  __device__ __forceinline__ void put(int k, const float2 (&f)[4]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(at + (2 * k + h) * THREADS * 16), "f"(f[2 * h].x), "f"(f[2 * h].y),
+                   "f"(f[2 * h + 1].x), "f"(f[2 * h + 1].y) : "memory");
+  }
+};
+
 struct Slot {
   int id, t, size;
-  float* red;        // 128 floats of shared memory: two turns of 64, zero where no warp writes
+  float* red;        // 64 floats of shared memory: two turns of 32, zero where no warp writes
   int turn;
   __device__ __forceinline__ void sync() const {
     if (size > 32) asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(size) : "memory");
@@ -260,58 +377,55 @@ struct Slot {
   }
 };
 
-// Sums of M values (1, 2 or 4) over the threads of a slot, the same in each.  In a warp each step halves the values a lane
-// goes on with, until it is one: four sums take six shuffles.  Warps meet in shared memory at the slot's named barrier; the two
-// turns of `red` alternate, so the next sums may be written while these are still being read.
-template <bool WIDE, int M>
-__device__ __forceinline__ void slot_sum(float (&v)[M], Slot& s) {
+// Sums of one or two values over the threads of a slot, the same in each.  Of two, a half of the warp goes on with each after
+// the first step.  Warps meet in shared memory at the slot's named barrier; the two turns of `red` alternate, so the next sums
+// may be written while these are still being read.
+template <bool WIDE>
+__device__ __forceinline__ float slot_sum(float v, Slot& s) {
   if (!WIDE) {
-    for (int o = s.size >> 1; o; o >>= 1) {
-#pragma unroll
-      for (int i = 0; i < M; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-    }
-    return;
-  }
-  float one;
-  if (M == 4) {
-    const bool a = threadIdx.x & 16, b = threadIdx.x & 8;
-    float x = a ? v[2 % M] : v[0], y = a ? v[3 % M] : v[1 % M];
-    x += __shfl_xor_sync(0xffffffffu, a ? v[0] : v[2 % M], 16);
-    y += __shfl_xor_sync(0xffffffffu, a ? v[1 % M] : v[3 % M], 16);
-    one = b ? y : x;
-    one += __shfl_xor_sync(0xffffffffu, b ? x : y, 8);
-  } else if (M == 2) {
-    const bool a = threadIdx.x & 16;
-    one = a ? v[1 % M] : v[0];
-    one += __shfl_xor_sync(0xffffffffu, a ? v[0] : v[1 % M], 16);
-    one += __shfl_xor_sync(0xffffffffu, one, 8);
-  } else {
-    one = v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
-    one += __shfl_xor_sync(0xffffffffu, one, 8);
+    for (int o = s.size >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
   }
 #pragma unroll
-  for (int o = 4; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (s.size == 32) return v;
   float* r = s.red + s.turn;
-  s.turn ^= 64;
-  constexpr int L = 32 / M;           // lanes that hold the same sum
-  if (s.t % L == 0) r[s.t / L] = one;
+  s.turn ^= 32;
+  if ((s.t & 31) == 0) r[s.t >> 5] = v;
   s.sync();
-  // four values at a time, values of more warps than four (M = 4), eight or sixteen in a loop
-  constexpr int Q = M == 4 ? 4 : M == 2 ? 2 : 1;
-#pragma unroll
-  for (int i = 0; i < M; ++i) v[i] = 0.f;
-  auto add = [&](int w) {
-    const float4 q = ld_f4(r + 4 * w);
-    if (M == 4) { v[0] += q.x; v[1 % M] += q.y; v[2 % M] += q.z; v[3 % M] += q.w; }
-    else if (M == 2) { v[0] += q.x + q.z; v[1 % M] += q.y + q.w; }
-    else v[0] += (q.x + q.y) + (q.z + q.w);
-  };
-#pragma unroll
-  for (int w = 0; w < Q; ++w) add(w);
-  for (int w = 4; w < s.size >> 5; w += 4) {
-#pragma unroll
-    for (int u = 0; u < Q; ++u) add(w * Q / 4 + u);
+  float4 q = ld_f4(r);
+  v = (q.x + q.y) + (q.z + q.w);
+  for (int w = 128; w < s.size; w += 128) { q = ld_f4(r + (w >> 5)); v += (q.x + q.y) + (q.z + q.w); }
+  return v;
+}
+template <bool WIDE>
+__device__ __forceinline__ float2 slot_sum(float2 v, Slot& s) {
+  if (!WIDE) {
+    for (int o = s.size >> 1; o; o >>= 1) { v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o); }
+    return v;
   }
+  const bool upper = threadIdx.x & 16;
+  float one = upper ? v.y : v.x;
+  one += __shfl_xor_sync(0xffffffffu, upper ? v.x : v.y, 16);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+  if (s.size == 32) {
+    const float other = __shfl_xor_sync(0xffffffffu, one, 16);
+    return upper ? make_float2(other, one) : make_float2(one, other);
+  }
+  float* r = s.red + s.turn;
+  s.turn ^= 32;
+  if ((s.t & 15) == 0) r[s.t >> 4] = one;
+  s.sync();
+  float4 q = ld_f4(r);
+  v = make_float2(q.x + q.z, q.y + q.w);
+  for (int w = 64; w < s.size; w += 64) { q = ld_f4(r + (w >> 4)); v.x += q.x + q.z; v.y += q.y + q.w; }
+  return v;
+}
+// 1 / sqrt(v): the approximation and a step of Newton's, which leaves it within two roundings
+__device__ __forceinline__ float inverse_root(float v) {
+  const float y = rsqrtf(v);
+  return v > 0.f && v < 3e38f ? fmaf(y * fmaf(-v * y, y, 1.f), 0.5f, y) : y;
 }
 template <int N>
 __device__ __forceinline__ float total(const float2 (&f)[N]) {
@@ -328,32 +442,19 @@ __device__ __forceinline__ float dot(const float2 (&f)[N], const float2 (&g)[N])
   return v.x + v.y;
 }
 
-// n = (f - mean) * rstd of R rows in place; mean and rstd go to stats
-template <bool WIDE, int R, int K, bool VEC, int THREADS>
-__device__ __forceinline__ void normalise(const Columns<K, VEC, THREADS>& cols, Slot& s, const GeepsNorm& norm, int row, int end,
-                                          float inv_c, float2 (&f)[R][4 * K]) {
-  float mean[R], v[R];
-#pragma unroll
-  for (int r = 0; r < R; ++r) mean[r] = 0.f;
+// n = (f - mean) * rstd in place; mean and rstd go to stats
+template <bool WIDE, typename C_, int N>
+__device__ __forceinline__ void normalise(const C_& cols, Slot& s, const GeepsNorm& norm, int row, bool active, float inv_c, float2 (&f)[N]) {
+  float mean = 0.f;
   if (norm.kind == NORM_LAYER) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) mean[r] = total(f[r]);
-    slot_sum<WIDE>(mean, s);
-#pragma unroll
-    for (int r = 0; r < R; ++r) { mean[r] *= inv_c; cols.subtract(f[r], mean[r]); }
+    mean = slot_sum<WIDE>(total(f), s) * inv_c;
+    cols.subtract(f, mean);
   }
+  const float rstd = inverse_root(fmaf(slot_sum<WIDE>(dot(f, f), s), inv_c, norm.eps));
 #pragma unroll
-  for (int r = 0; r < R; ++r) v[r] = dot(f[r], f[r]);
-  slot_sum<WIDE>(v, s);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float rstd = 1.f / sqrtf(fmaf(v[r], inv_c, norm.eps));
-#pragma unroll
-    for (int i = 0; i < 4 * K; ++i) f[r][i] = mul2(f[r][i], both(rstd));
-    if (norm.stats && row + r < end && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * (row + r)) = make_float2(mean[r], rstd);
-  }
+  for (int i = 0; i < N; ++i) f[i] = mul2(f[i], both(rstd));
+  if (norm.stats && active && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * row) = make_float2(mean, rstd);
 }
-
 // n = (f - mean) * rstd with the statistics at hand.  Not zero where there is no column, but whatever it meets there is.
 template <int N>
 __device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
@@ -361,22 +462,14 @@ __device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
 #pragma unroll
   for (int i = 0; i < N; ++i) f[i] = fma2(f[i], r, m);
 }
-
-// Gradients of R rows n * w + b by their inputs, for a = dz * w: rstd * (a - mean a - n mean(a n)), added to `to`
-template <bool WIDE, int R, int N>
-__device__ __forceinline__ void norm_gradient(Slot& s, int kind, const float2 (&st)[R], float inv_c, const float2 (&n)[R][N],
-                                              const float2 (&a)[R][N], float2 (&to)[R][N]) {
-  float v[2 * R];
+// Gradient of n * w + b by its input, for a = dz * w in place: rstd * (a - mean a - n mean(a n))
+template <bool WIDE, int N>
+__device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, float inv_c, const float2 (&n)[N], float2 (&a)[N]) {
+  const float2 v = slot_sum<WIDE>(make_float2(total(a), dot(a, n)), s);
+  const float scale = -inv_c * rstd;
+  const float2 m0 = both(kind == NORM_LAYER ? v.x * scale : 0.f), m1 = both(v.y * scale), r = both(rstd);
 #pragma unroll
-  for (int r = 0; r < R; ++r) { v[2 * r] = total(a[r]); v[2 * r + 1] = dot(a[r], n[r]); }
-  slot_sum<WIDE>(v, s);
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const float scale = -inv_c * st[r].y;
-    const float2 m0 = both(kind == NORM_LAYER ? v[2 * r] * scale : 0.f), m1 = both(v[2 * r + 1] * scale), rs = both(st[r].y);
-#pragma unroll
-    for (int i = 0; i < N; ++i) to[r][i] = fma2(n[r][i], m1, fma2(a[r][i], rs, add2(to[r][i], m0)));
-  }
+  for (int i = 0; i < N; ++i) a[i] = fma2(n[i], m1, fma2(a[i], r, m0));
 }
 
 __device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
@@ -396,85 +489,68 @@ __device__ __forceinline__ void clear_ring(unsigned char* ring, int bytes) {
   __syncthreads();
 }
 
-// The rows of a slot, R a turn.  Slots that share a warp take the same number of turns, since its lanes meet in sums: some have
-// no row in the last.
+// The rows of a slot: a range of its own with a gate per image, else every `step`-th of all.  Slots that share a warp take the
+// same number of turns, since its lanes meet in sums: some have no row in the last.
 struct Walk {
   int lo, hi, step, turns;
-  __device__ __forceinline__ Walk(const GeepsResidual& p, int slots, int id, bool wide, int R, bool ranges) {
+  __device__ __forceinline__ Walk(const GeepsResidual& p, int slots, int id, bool wide, bool ranges) {
     const int rows = (int)p.rows, all = gridDim.x * slots, me = blockIdx.x * slots + id;
-    lo = ranges ? first_row(rows, all, me) : me * R;
+    lo = ranges ? first_row(rows, all, me) : me;
     hi = ranges ? first_row(rows, all, me + 1) : rows;
-    step = ranges ? R : all * R;
-    const int most = ranges ? (rows + all - 1) / all : (rows + step - 1) / step;
-    turns = !wide ? most : lo < hi ? (hi - lo + step - 1) / step : 0;
+    step = ranges ? 1 : all;
+    turns = !wide ? (rows + all - 1) / all : lo < hi ? (hi - lo + step - 1) / step : 0;
   }
 };
 
-// What kernels of K vectors a thread are like.  Two rows a turn where a turn's overhead counts most and registers allow: bf16
-// rows of up to 384 vectors; blocks have 384 threads then backward (168 registers a thread).
-template <typename TB, int K, bool VEC, bool WIDE>
-struct Form {
-  static constexpr int R = WIDE && K == 1 && VEC && sizeof(TB) == 2 ? 2 : 1;
-  static constexpr int forward_threads = K == 1 ? 256 : 512;
-  static constexpr int backward_threads = K == 1 && WIDE ? 384 : 512;
-};
-
 // WIDE: a slot is whole warps.  PIXEL: a gate for every row.
-template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(Form<TB, K, VEC, WIDE>::forward_threads, K == 1 ? MODE == MODE_NORM ? 3 : 2 : 1)
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
+__global__ void __launch_bounds__(block_threads(false, LARGE), LARGE ? 1 : MODE == MODE_NORM ? 4 : 2)
 residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
   geeps_pdl_enter();
-  extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ __align__(16) float red[16][128];
-  constexpr int N = 4 * K, R = Form<TB, K, VEC, WIDE>::R;
-  for (int i = threadIdx.x; i < 16 * 128; i += blockDim.x) red[0][i] = 0.f;
-  __syncthreads();
+  extern __shared__ __align__(16) unsigned char shared[];
+  __shared__ __align__(16) float red[16][64];
+  constexpr int N = 4 * K, THREADS = block_threads(false, LARGE);
+  typedef Columns<K, VEC, !LARGE, THREADS> Cols;
+  for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
-  const Columns<K, VEC, Form<TB, K, VEC, WIDE>::forward_threads> cols = {s.t, slot, p.C, slots};
+  const Cols cols = {s.t, slot, p.C, slots};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
-  float2 sw[N], sb[N], w2[N], b2[N];           // scale * weight and scale * bias, times the gate where an image has one
-  auto join_params = [&]() {
-    float2 sc[N];
-    cols.param(p.scale, 1.f, sc); cols.param(p.post.weight, 1.f, sw); cols.param(p.post.bias, 0.f, sb);
-#pragma unroll
-    for (int i = 0; i < N; ++i) { sw[i] = mul2(sw[i], sc[i]); sb[i] = mul2(sb[i], sc[i]); }
-  };
-  if ((MODE & MODE_JOIN) && !by_image) join_params();
-  if (MODE & MODE_NORM) { cols.param(p.pre.weight, 1.f, w2); cols.param(p.pre.bias, 0.f, b2); }
-  const Walk w(p, slots, s.id, WIDE, R, by_image);
+  unsigned char* area = shared;
+  Param<Cols, K, VEC> sw, sb, w2, b2;          // scale * weight and scale * bias of the join, weight and bias of the next norm
+  Own<K, THREADS> factor;                      // the gate of the image at hand
+  if (MODE & MODE_JOIN) { sw.set(cols, p.post.weight, 1.f, p.scale, area); sb.set(cols, p.post.bias, 0.f, p.scale, area); }
+  if (MODE & MODE_NORM) { w2.set(cols, p.pre.weight, 1.f, nullptr, area); b2.set(cols, p.pre.bias, 0.f, nullptr, area); }
+  if (by_image && !LARGE) factor.set(area);
+  const Walk w(p, slots, s.id, WIDE, by_image);
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
-  int left = 0;                                // rows to go with the gate at hand
+  int image = 0, left = 0;                     // rows to go with the gate at hand
 
-  const bool live = !VEC || cols.on(0);        // K = 1: a thread has its one vector or nothing
-  const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring) + (VEC ? threadIdx.x * 16 : 0);
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(area) + (VEC ? threadIdx.x * 16 : 0);
   const int at_x = cols.template stage<TR>(), at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
-  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * R * one;
+  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * one;
   const Rows<TR> res(p.res, p.ldres, cols.first()), h_out(p.out, p.ldout, cols.first());
   const Rows<TB> x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first()), y_out(p.y, p.ldy, cols.first());
   int ahead = w.lo, in = 0, out = 0;           // the row that is copied next, stages that are filled and read next
   auto copy = [&]() {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = ahead + r;
-      if (row < w.hi && live) {
-        const uint32_t to = base + in + r * one;
-        cols.copy(res.at(row), to);
-        if (MODE & MODE_JOIN) cols.copy(x.at(row), to + at_x);
-        if (PIXEL) cols.copy(gate.at(row), to + at_g);
-      }
+    if (ahead < w.hi) {
+      const uint32_t to = base + in;
+      cols.copy(res.at(ahead), to);
+      if (MODE & MODE_JOIN) cols.copy(x.at(ahead), to + at_x);
+      if (PIXEL) cols.copy(gate.at(ahead), to + at_g);
     }
     ahead += w.step;
-    in = in == last ? 0 : in + R * one;
+    in = in == last ? 0 : in + one;
     copy_commit();
   };
   if (cols.RING) {
-    clear_ring(ring, depth * R * one);
+    clear_ring(area, depth * one);
     for (int i = 0; i < depth - 1; ++i) copy();
   }
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
+    const bool active = WIDE || row < w.hi;
     if (cols.RING) {
       if (!VEC) s.sync();
       copy();
@@ -482,52 +558,79 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
       if (!VEC) s.sync();
     }
     const uint32_t from = base + out;
-    if (cols.RING) out = out == last ? 0 : out + R * one;
-    float2 h[R][N];
-#pragma unroll
-    for (int r = 0; r < R; ++r) cols.load(res, row + r, row + r < w.hi, true, from + r * one, h[r]);
+    if (cols.RING) out = out == last ? 0 : out + one;
+    float2 h[N];
     if (MODE & MODE_JOIN) {
-      float2 z[R][N];
-#pragma unroll
-      for (int r = 0; r < R; ++r) cols.load(x, row + r, row + r < w.hi, true, from + r * one + at_x, z[r]);
-      if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, w.hi, inv_c, z);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float2 g[N];
-        const bool active = row + r < w.hi;
-        if (by_image && left-- == 0 && active) {
-          const int image = (row + r) / per_gate;
-          left = (image + 1) * per_gate - (row + r) - 1;
+      float2 z[N];
+      cols.load(x, row, active, true, from + at_x, z);
+      if (by_image && left-- == 0 && active) {
+        image = row / per_gate;
+        left = (image + 1) * per_gate - row - 1;
+        if (!LARGE) {
+          float2 g[N];
           cols.fetch(gate.at(image), true, g);
           gate_factor(p.sigmoid, g);
-          join_params();
 #pragma unroll
-          for (int j = 0; j < N; ++j) { sw[j] = mul2(sw[j], g[j]); sb[j] = mul2(sb[j], g[j]); }
+          for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(g[4 * k]));
         }
-        if (PIXEL) { cols.load(gate, row + r, active, true, from + r * one + at_g, g); gate_factor(p.sigmoid, g); }
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if (PIXEL) h[r][j] = fma2(fma2(z[r][j], sw[j], sb[j]), g[j], h[r][j]);
-          else h[r][j] = add2(h[r][j], fma2(z[r][j], sw[j], sb[j]));
-        }
-        cols.store(h_out.at(row + r), active, h[r]);
       }
+      if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, active, inv_c, z);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float2 a[4], b[4];
+        sw.get(cols, k, a); sb.get(cols, k, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[4 * k + e] = fma2(z[4 * k + e], a[e], b[e]);
+      }
+      if (by_image && !LARGE) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          float2 g[4];
+          factor.get(k, g);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[4 * k + e] = mul2(z[4 * k + e], g[e]);
+        }
+      } else if (PIXEL || (by_image && LARGE)) {
+        float2 g[N];
+        if (PIXEL) cols.load(gate, row, active, true, from + at_g, g); else cols.fetch(gate.at(image), active, g);
+        gate_factor(p.sigmoid, g);
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = mul2(z[j], g[j]);
+      }
+      cols.load(res, row, active, true, from, h);
+#pragma unroll
+      for (int j = 0; j < N; ++j) h[j] = add2(h[j], z[j]);
+      cols.store(h_out.at(row), active, h);
+    } else {
+      cols.load(res, row, active, true, from, h);
     }
     if (MODE & MODE_NORM) {
-      normalise<WIDE>(cols, s, p.pre, row, w.hi, inv_c, h);
+      normalise<WIDE>(cols, s, p.pre, row, active, inv_c, h);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
+      for (int k = 0; k < K; ++k) {
+        float2 a[4], b[4];
+        w2.get(cols, k, a); b2.get(cols, k, b);
 #pragma unroll
-        for (int j = 0; j < N; ++j) h[r][j] = fma2(h[r][j], w2[j], b2[j]);
-        cols.store(y_out.at(row + r), row + r < w.hi, h[r]);
+        for (int e = 0; e < 4; ++e) h[4 * k + e] = fma2(h[4 * k + e], a[e], b[e]);
       }
+      cols.store(y_out.at(row), active, h);
     }
   }
 }
 
-// Sums kept per block in the workspace: [block][sums][C], A and B of the join, then dweight and dbias of the next norm;
-// behind them a row of the gate's gradient for each (slot, image) pair that shares rows, number slot + image.
+// The workspace: sums of every block, [block][sums][C], A and B of the join, then dweight and dbias of the next norm; with a
+// gate per image {A, B} of every slot's images, [slot][C][2], and a row of the gate's gradient for each (slot, image) pair that
+// shares rows, number slot + image.
 __host__ __device__ inline int sums_of(int mode) { return mode == MODE_BOTH ? 4 : 2; }
+inline long long work_floats(const Shape& s, int C, int mode, long long images) {
+  return ((long long)s.blocks * sums_of(mode) + (images ? 3LL * s.blocks * s.slots + images : 0)) * C;
+}
+__device__ __forceinline__ float* sums_of_images(const GeepsResidual& p, int mode, long long slot) {
+  return p.work + ((long long)gridDim.x * sums_of(mode) + 2 * slot) * p.C;
+}
+__device__ __forceinline__ float* image_share(const GeepsResidual& p, int mode, int blocks, long long all, long long slot, int image) {
+  return p.work + (blocks * sums_of(mode) + 2 * all + slot + image) * p.C;
+}
 
 // dw, db, dscale from a column's sums
 __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int c, const float* v) {
@@ -544,101 +647,104 @@ __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int
   }
 }
 
-template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(Form<TB, K, VEC, WIDE>::backward_threads)
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
+__global__ void __launch_bounds__(block_threads(true, LARGE))
 residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
   geeps_pdl_enter();
-  extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float2 stats[2][512];
-  __shared__ __align__(16) float red[16][128];
-  constexpr int N = 4 * K, R = Form<TB, K, VEC, WIDE>::R;
-  for (int i = threadIdx.x; i < 16 * 128; i += blockDim.x) red[0][i] = 0.f;
-  for (int i = threadIdx.x; i < 2 * 512; i += blockDim.x) stats[0][i] = both(0.f);
-  __syncthreads();
+  extern __shared__ __align__(16) unsigned char shared[];
+  constexpr int N = 4 * K, THREADS = block_threads(true, LARGE);
+  typedef Columns<K, VEC, !LARGE, THREADS> Cols;
+  __shared__ float2 stats[2][THREADS];
+  __shared__ __align__(16) float red[16][64];
+  for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
-  const Columns<K, VEC, Form<TB, K, VEC, WIDE>::backward_threads> cols = {s.t, slot, p.C, slots};
+  stats[0][threadIdx.x] = stats[1][threadIdx.x] = both(0.f);
+  const Cols cols = {s.t, slot, p.C, slots};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
-  float2 sw[N], sb[N], w2[N], a0[N], a1[N], n0[N], n1[N];     // sw: scale * weight, times the gate where an image has one
-  auto scaled = [&](const float* of, float other, float2 (&f)[N]) {
-    float2 sc[N];
-    cols.param(p.scale, 1.f, sc); cols.param(of, other, f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = mul2(f[i], sc[i]);
-  };
+  unsigned char* area = shared;
+  Param<Cols, K, VEC> sw, sb, w2;              // scale * weight, scale * bias (for a gate's gradient), the next norm's weight
+  Own<K, THREADS> factor;                      // the gate of the image at hand
   if (MODE & MODE_JOIN) {
-    scaled(p.post.weight, 1.f, sw);
-    if (PIXEL) scaled(p.post.bias, 0.f, sb);
-#pragma unroll
-    for (int i = 0; i < N; ++i) a0[i] = a1[i] = both(0.f);
+    sw.set(cols, p.post.weight, 1.f, p.scale, area);
+    if (PIXEL) sb.set(cols, p.post.bias, 0.f, p.scale, area);
   }
-  if (MODE & MODE_NORM) {
-    cols.param(p.pre.weight, 1.f, w2);
+  if (MODE & MODE_NORM) w2.set(cols, p.pre.weight, 1.f, nullptr, area);
+  if (by_image && !LARGE) factor.set(area);
+  float2 a0[N], a1[N], n0[N], n1[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) n0[i] = n1[i] = both(0.f);
-  }
-  const Walk w(p, slots, s.id, WIDE, R, by_image);
+  for (int i = 0; i < N; ++i) a0[i] = a1[i] = n0[i] = n1[i] = both(0.f);
+  const Walk w(p, slots, s.id, WIDE, by_image);
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
   int image = -1, left = 0;
 
-  const bool live = !VEC || cols.on(0);        // K = 1: a thread has its one vector or nothing
-  const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring) + (VEC ? threadIdx.x * 16 : 0);
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(area) + (VEC ? threadIdx.x * 16 : 0);
   const int at_o = cols.template stage<TR>(), at_y = at_o + (MODE & MODE_NORM ? cols.template stage<TR>() : 0);
   const int at_x = at_y + (MODE & MODE_NORM ? cols.template stage<TB>() : 0);
   const int at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
-  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * R * one;
+  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * one;
   const Rows<TR> dout(p.dout, p.lddout, cols.first()), h(p.out, p.ldout, cols.first()), dres(p.dres, p.lddres, cols.first());
   const Rows<TB> dy(p.dy, p.lddy, cols.first()), x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first());
   const Rows<TB> dx(p.dx, p.lddx, cols.first()), dgate(p.dgate, p.lddgate, cols.first());
   const bool has_dout = p.dout != nullptr;
   int ahead = w.lo, in = 0, out = 0;
   auto copy = [&]() {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int row = ahead + r;
-      const uint32_t to = base + in + r * one;
-      if (row < w.hi) {
-        if (live) {
-          if (has_dout) cols.copy(dout.at(row), to);
-          if (MODE & MODE_NORM) { cols.copy(h.at(row), to + at_o); cols.copy(dy.at(row), to + at_y); }
-          if (MODE & MODE_JOIN) cols.copy(x.at(row), to + at_x);
-          if (PIXEL) cols.copy(gate.at(row), to + at_g);
-        }
-      } else if (R > 1 || !WIDE) {             // rows that are read and are none: they add nothing to the sums
-        cols.template no_row<TR>(to);
-        if (MODE & MODE_NORM) { cols.template no_row<TR>(to + at_o); cols.template no_row<TB>(to + at_y); }
-        if (MODE & MODE_JOIN) cols.template no_row<TB>(to + at_x);
-        if (PIXEL) cols.template no_row<TB>(to + at_g);
-      }
+    const uint32_t to = base + in;
+    if (ahead < w.hi) {
+      if (has_dout) cols.copy(dout.at(ahead), to);
+      if (MODE & MODE_NORM) { cols.copy(h.at(ahead), to + at_o); cols.copy(dy.at(ahead), to + at_y); }
+      if (MODE & MODE_JOIN) cols.copy(x.at(ahead), to + at_x);
+      if (PIXEL) cols.copy(gate.at(ahead), to + at_g);
+    } else if (!WIDE) {                        // rows that are read and are none: they add nothing to the sums
+      cols.template no_row<TR>(to);
+      if (MODE & MODE_NORM) { cols.template no_row<TR>(to + at_o); cols.template no_row<TB>(to + at_y); }
+      if (MODE & MODE_JOIN) cols.template no_row<TB>(to + at_x);
+      if (PIXEL) cols.template no_row<TB>(to + at_g);
     }
     ahead += w.step;
-    in = in == last ? 0 : in + R * one;
+    in = in == last ? 0 : in + one;
     copy_commit();
   };
-  // with a gate per image a0 and a1 are the sums u and v of the image at hand; A and B of all images are kept behind the ring
-  float* all_images = reinterpret_cast<float*>(ring + depth * R * one) + threadIdx.x;
-  auto kept = [&](int i) -> float& { return all_images[i * slot * slots]; };
-  if (by_image) {
-    for (int i = 0; i < 4 * N; ++i) kept(i) = 0.f;
-  }
-  // the rows of an image that this slot has are done: its part of the gate's gradient, all of it if no other slot has any
+  // The rows of an image that this slot has are done: its part of the gate's gradient, all of it if no other slot has any.  With
+  // a gate per image a0 and a1 are the sums u and v of the image at hand; A and B of the images before it are in the workspace,
+  // every thread its own columns.
+  float2* before = by_image ? reinterpret_cast<float2*>(sums_of_images(p, MODE, blockIdx.x * slots + s.id)) : nullptr;
+  bool none_before = true;
   auto image_done = [&]() {
-    float2 g[N], d[N], b[N];
+    float2 g[N], d[N];
     cols.fetch(gate.at(image), true, g);
     gate_factor(p.sigmoid, g);
-    scaled(p.post.weight, 1.f, d); scaled(p.post.bias, 0.f, b);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      d[i] = mul2(fma2(d[i], a0[i], mul2(b[i], a1[i])), gate_slope(p.sigmoid, g[i]));
-      kept(4 * i) = fmaf(g[i].x, a0[i].x, kept(4 * i)); kept(4 * i + 1) = fmaf(g[i].y, a0[i].y, kept(4 * i + 1));
-      kept(4 * i + 2) = fmaf(g[i].x, a1[i].x, kept(4 * i + 2)); kept(4 * i + 3) = fmaf(g[i].y, a1[i].y, kept(4 * i + 3));
-      a0[i] = a1[i] = both(0.f);
+    for (int k = 0; k < K; ++k) {
+      float2 m[4];
+      sw.get(cols, k, m);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * k + e, c = cols.at(2 * i), c1 = cols.at(2 * i + 1);
+        float2 bias = both(0.f);
+        if (p.post.bias) {
+          if (cols.on(2 * i)) bias.x = p.post.bias[c] * (p.scale ? p.scale[c] : 1.f);
+          if (cols.on(2 * i + 1)) bias.y = p.post.bias[c1] * (p.scale ? p.scale[c1] : 1.f);
+        }
+        d[i] = mul2(fma2(m[e], a0[i], mul2(bias, a1[i])), gate_slope(p.sigmoid, g[i]));
+        float2 sum = mul2(g[i], a0[i]), sum1 = mul2(g[i], a1[i]);
+        if (cols.on(2 * i)) {                    // [column]{A, B}
+          if (!none_before) { sum.x += before[c].x; sum1.x += before[c].y; }
+          before[c] = make_float2(sum.x, sum1.x);
+        }
+        if (cols.on(2 * i + 1)) {
+          if (!none_before) { sum.y += before[c1].x; sum1.y += before[c1].y; }
+          before[c1] = make_float2(sum.y, sum1.y);
+        }
+        a0[i] = a1[i] = both(0.f);
+      }
     }
+    none_before = false;
     if (!p.dgate) return;
     if (image * per_gate >= w.lo && (image + 1) * per_gate <= w.hi) cols.store(dgate.at(image), true, d);
     else {
-      float* to = p.work + ((long long)gridDim.x * sums_of(MODE) + (long long)blockIdx.x * slots + s.id + image) * p.C;
+      float* to = image_share(p, MODE, gridDim.x, (long long)gridDim.x * slots, blockIdx.x * slots + s.id, image);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (cols.on(2 * i)) to[cols.at(2 * i)] = d[i].x;
@@ -647,11 +753,12 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
   };
   if (cols.RING) {
-    clear_ring(ring, depth * R * one);
+    clear_ring(area, depth * one);
     for (int i = 0; i < depth - 1; ++i) copy();
-  }
+  } else __syncthreads();
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
+    const bool active = WIDE || row < w.hi;
     if (cols.RING) {
       if (!VEC) s.sync();
       copy();
@@ -659,12 +766,12 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       if (!VEC) s.sync();
     }
     const uint32_t from = base + out;
-    if (cols.RING) out = out == last ? 0 : out + R * one;
+    if (cols.RING) out = out == last ? 0 : out + one;
     // Statistics of the rows of several turns at a time, a row a lane: a load for every turn was waited for in the turn that
     // issued it, with the loads from shared memory that share its scoreboard (50176 x 576: 36 % of the time).
-    const int chunk = WIDE ? 32 : slot, k = i * R & (chunk - 1);
-    if (k == 0) {
-      const int turn = i + (s.t & (chunk - 1)) / R, q = w.lo + turn * w.step + (s.t & (R - 1));
+    const int chunk = WIDE ? 32 : slot, k0 = i & (chunk - 1);
+    if (k0 == 0) {
+      const int turn = i + (s.t & (chunk - 1)), q = w.lo + turn * w.step;
       __syncwarp();
       if (turn < w.turns && q < w.hi) {
         if ((MODE & MODE_JOIN) && p.post.kind) stats[0][threadIdx.x] = *reinterpret_cast<const float2*>(p.post.stats + 2LL * q);
@@ -672,99 +779,94 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       }
       __syncwarp();
     }
-    float2 now1[R], now2[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int lane = (threadIdx.x & ~(chunk - 1)) + k + r;
-      now1[r] = MODE & MODE_JOIN ? stats[0][lane] : both(0.f);
-      now2[r] = MODE & MODE_NORM ? stats[1][lane] : both(0.f);
-    }
+    const int lane = (threadIdx.x & ~(chunk - 1)) + k0;
+    const float2 st1 = stats[0][lane], st2 = stats[1][lane];
     // an output may lie where an operand does: without a ring everything of the row is read before its first output is written
-    float2 dh[R][N], z[R][N], g[R][N];
+    float2 dh[N], z[N], g[N];
     auto load_branch = [&]() {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool active = WIDE && R == 1 || row + r < w.hi;
-        if (MODE & MODE_JOIN) cols.load(x, row + r, active, true, from + r * one + at_x, z[r]);
-        if (PIXEL) { cols.load(gate, row + r, active, true, from + r * one + at_g, g[r]); gate_factor(p.sigmoid, g[r]); }
-      }
+      if (MODE & MODE_JOIN) cols.load(x, row, active, true, from + at_x, z);
+      if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_factor(p.sigmoid, g); }
     };
-    if (!cols.RING) load_branch();
-#pragma unroll
-    for (int r = 0; r < R; ++r) cols.load(dout, row + r, WIDE && R == 1 || row + r < w.hi, has_dout, from + r * one, dh[r]);
+    if (!cols.RING) { load_branch(); cols.load(dout, row, active, has_dout, from, dh); }
     if (MODE & MODE_NORM) {
-      float2 n[R][N], a[R][N];
+      float2 n[N], a[N];
+      cols.load(h, row, active, true, from + at_o, n);
+      cols.load(dy, row, active, true, from + at_y, a);
+      normalised(n, st2);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool active = WIDE && R == 1 || row + r < w.hi;
-        cols.load(h, row + r, active, true, from + r * one + at_o, n[r]);
-        cols.load(dy, row + r, active, true, from + r * one + at_y, a[r]);
-        normalised(n[r], now2[r]);
+      for (int k = 0; k < K; ++k) {
+        float2 m[4];
+        w2.get(cols, k, m);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          n0[j] = fma2(a[r][j], n[r][j], n0[j]); n1[j] = add2(n1[j], a[r][j]);
-          a[r][j] = mul2(a[r][j], w2[j]);
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * k + e;
+          n0[j] = fma2(a[j], n[j], n0[j]); n1[j] = add2(n1[j], a[j]);
+          a[j] = mul2(a[j], m[e]);
         }
       }
-      norm_gradient<WIDE>(s, p.pre.kind, now2, inv_c, n, a, dh);
-    }
+      norm_gradient<WIDE>(s, p.pre.kind, st2.y, inv_c, n, a);
+      if (cols.RING) cols.load(dout, row, active, has_dout, from, dh);
 #pragma unroll
-    for (int r = 0; r < R; ++r) cols.store(dres.at(row + r), WIDE && R == 1 || row + r < w.hi, dh[r]);
+      for (int j = 0; j < N; ++j) dh[j] = add2(dh[j], a[j]);
+    } else if (cols.RING) {
+      cols.load(dout, row, active, has_dout, from, dh);
+    }
+    cols.store(dres.at(row), active, dh);
     if (MODE & MODE_JOIN) {
       if (cols.RING) load_branch();
+      if (by_image && left == 0 && active) {
+        if (image >= 0) image_done();
+        image = row / per_gate;
+        left = (image + 1) * per_gate - row;
+        if (!LARGE) {
+          float2 f[N];
+          cols.fetch(gate.at(image), true, f);
+          gate_factor(p.sigmoid, f);
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool active = WIDE && R == 1 || row + r < w.hi;
-        if (by_image && left == 0 && active) {
-          if (image >= 0) image_done();
-          image = (row + r) / per_gate;
-          left = (image + 1) * per_gate - (row + r);
-          float2 factor[N];
-          cols.fetch(gate.at(image), true, factor);
-          gate_factor(p.sigmoid, factor);
-          scaled(p.post.weight, 1.f, sw);
-#pragma unroll
-          for (int j = 0; j < N; ++j) sw[j] = mul2(sw[j], factor[j]);
+          for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(f[4 * k]));
         }
-        --left;
-        if (p.post.kind) normalised(z[r], now1[r]);
-        float2 dg[N];
+      }
+      --left;
+      if (by_image && LARGE) { cols.fetch(gate.at(image), true, g); gate_factor(p.sigmoid, g); }
+      if (p.post.kind) normalised(z, st1);
+      float2 dg[N];
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          float2 d = dh[r][j];
+      for (int k = 0; k < K; ++k) {
+        float2 m[4], f[4], b[4];
+        sw.get(cols, k, m);
+        if (PIXEL) sb.get(cols, k, b);
+        if (by_image && !LARGE) factor.get(k, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 4 * k + e;
+          float2 d = dh[j];
           if (PIXEL) {
-            dg[j] = mul2(mul2(d, fma2(sw[j], z[r][j], sb[j])), gate_slope(p.sigmoid, g[r][j]));
-            d = mul2(d, g[r][j]);
+            dg[j] = mul2(mul2(d, fma2(m[e], z[j], b[e])), gate_slope(p.sigmoid, g[j]));
+            d = mul2(d, g[j]);
           }
-          a0[j] = fma2(d, z[r][j], a0[j]); a1[j] = add2(a1[j], d);
-          dh[r][j] = mul2(d, sw[j]);
+          a0[j] = fma2(d, z[j], a0[j]); a1[j] = add2(a1[j], d);
+          if (by_image) d = mul2(d, LARGE ? g[j] : f[e]);
+          dh[j] = mul2(d, m[e]);
         }
-        if (PIXEL && p.dgate) cols.store(dgate.at(row + r), active, dg);
       }
-      if (p.post.kind) {
-        float2 e[R][N];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-#pragma unroll
-          for (int j = 0; j < N; ++j) e[r][j] = both(0.f);
-        }
-        norm_gradient<WIDE>(s, p.post.kind, now1, inv_c, z, dh, e);
-#pragma unroll
-        for (int r = 0; r < R; ++r) cols.store(dx.at(row + r), WIDE && R == 1 || row + r < w.hi, e[r]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < R; ++r) cols.store(dx.at(row + r), WIDE && R == 1 || row + r < w.hi, dh[r]);
-      }
+      if (PIXEL && p.dgate) cols.store(dgate.at(row), active, dg);
+      if (p.post.kind) norm_gradient<WIDE>(s, p.post.kind, st1.y, inv_c, z, dh);
+      cols.store(dx.at(row), active, dh);
     }
   }
   if (by_image && image >= 0) image_done();
   // the slots' sums, in slot order, in the threads of slot 0
   if (by_image) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) { a0[i] = make_float2(kept(4 * i), kept(4 * i + 1)); a1[i] = make_float2(kept(4 * i + 2), kept(4 * i + 3)); }
+    for (int i = 0; i < N; ++i) {
+      a0[i] = a1[i] = both(0.f);
+      if (none_before) continue;
+      if (cols.on(2 * i)) { const float2 v = before[cols.at(2 * i)]; a0[i].x = v.x; a1[i].x = v.y; }
+      if (cols.on(2 * i + 1)) { const float2 v = before[cols.at(2 * i + 1)]; a0[i].y = v.x; a1[i].y = v.y; }
+    }
   }
   __syncthreads();
-  float2* meet = reinterpret_cast<float2*>(ring);
+  float2* meet = reinterpret_cast<float2*>(shared);
   auto over_slots = [&](float2 (&v)[N]) {
     if (slots == 1) return;
 #pragma unroll
@@ -795,60 +897,89 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   }
 }
 
-// Second launch: the blocks' sums in block order (blockIdx.y = 0), and the gate's gradient of the images whose rows several
-// slots had: blockIdx.y - 1, by gridDim.y - 1, goes through the slots that begin inside of an image and are its first cut.
+// The slot whose rows have row i
+__device__ __forceinline__ int slot_of(int rows, int slots, int i) {
+  const int base = rows / slots, longer = rows % slots, split = longer * (base + 1);
+  return i < split ? i / (base + 1) : longer + (i - split) / base;
+}
+// Second launch: the blocks' sums, and the gate's gradient of the images whose rows several slots had, each in the order of the
+// blocks or slots.  A block has 32 columns at the most and 32 shares: blockIdx.y 0 to 3 a quarter of the columns each and every
+// 32nd block's sums a share; then 32 / `parts` images, or, where there are more images than slots, slots that begin inside of
+// one and are its first cut.
+constexpr int kSumsThreads = 256;
 template <typename TB>
-__global__ void __launch_bounds__(256)
-residual_sums_kernel(const __grid_constant__ GeepsResidual p, int mode, int blocks, int slots) {
+__global__ void __launch_bounds__(kSumsThreads)
+residual_sums_kernel(const __grid_constant__ GeepsResidual p, int mode, int blocks, int slots, int parts) {
   geeps_pdl_enter();
-  const int lane = threadIdx.x & 7, part = threadIdx.x >> 3, c = blockIdx.x * 8 + lane, sums = sums_of(mode);
-  if (blockIdx.y == 0) {
-    if (blocks == 1) return;
-    __shared__ float sh[32][4][8];
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+  __shared__ float sh[32][4][8];
+  const int lane = threadIdx.x & 7, share = threadIdx.x >> 3, sums = sums_of(mode);
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (blockIdx.y < 4) {
+    const int c = blockIdx.x * 32 + blockIdx.y * 8 + lane;
+    if (blocks == 1 || c - lane >= p.C) return;
     if (c < p.C) {
-      for (int b = part; b < blocks; b += 32)
-        for (int i = 0; i < sums; ++i) v[i] += p.work[((long long)b * sums + i) * p.C + c];
+#pragma unroll 5
+      for (int b = share; b < blocks; b += 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (i < sums) v[i] += p.work[((long long)b * sums + i) * p.C + c];
+      }
     }
-    for (int i = 0; i < 4; ++i) sh[part][i][lane] = v[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] += __shfl_xor_sync(0xffffffffu, v[i], 8);
+      v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+      if ((threadIdx.x & 24) == 0) sh[threadIdx.x >> 5][i][lane] = v[i];
+    }
     __syncthreads();
-    if (part != 0 || c >= p.C) return;
-    for (int i = 0; i < sums; ++i) { v[i] = 0.f; for (int q = 0; q < 32; ++q) v[i] += sh[q][i][lane]; }
+    if (share != 0 || c >= p.C) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) v[i] += sh[w][i][lane];
+    }
     write_sums(p, mode, c, v);
     return;
   }
-  if (c >= p.C) return;
-  const int rows = (int)p.rows, per_gate = (int)(p.rows / p.gate_rows);
-  const int all = blocks * slots;
-  const float* w = p.work + (long long)blocks * sums * p.C;
-  for (int b = 1 + (blockIdx.y - 1) * 32 + part; b < all; b += (gridDim.y - 1) * 32) {
-    const int cut = first_row(rows, all, b);
-    if (cut >= rows) break;
-    const int image = cut / per_gate, start = image * per_gate;
-    if (cut == start || first_row(rows, all, b - 1) > start) continue;
-    float v = 0.f;
-    for (int q = b - 1; q < all && first_row(rows, all, q) - start < per_gate && first_row(rows, all, q) < rows; ++q)
-      v += w[((long long)q + image) * p.C + c];
-    ((TB*)p.dgate)[image * p.lddgate + c] = (TB)v;
+  const int rows = (int)p.rows, images = (int)p.gate_rows, per_gate = rows / images, all = blocks * slots;
+  const int item = (blockIdx.y - 4) * (32 / parts) + share / parts, part = share % parts;
+  int image = item, first = 0, end = 0;               // slots [first, end) have rows of the image
+  if (images <= all) {
+    if (item < images) {
+      first = slot_of(rows, all, item * per_gate);
+      end = slot_of(rows, all, (item + 1) * per_gate - 1) + 1;
+    }
+  } else if (item + 1 < all && first_row(rows, all, item + 1) < rows) {
+    const int cut = first_row(rows, all, item + 1), start = cut / per_gate * per_gate;
+    image = cut / per_gate;
+    if (cut != start && first_row(rows, all, item) <= start) {
+      first = item;
+      end = slot_of(rows, all, start + per_gate - 1) + 1;
+    }
+  }
+  if (end - first < 2) end = first;                   // one slot had it all
+#pragma unroll 4
+  for (int q = first + part; q < end; q += parts) {
+    const float* w = image_share(p, mode, blocks, all, q, image);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = blockIdx.x * 32 + u * 8 + lane;
+      if (c < p.C) v[u] += w[c];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) sh[share][u][lane] = v[u];
+  __syncthreads();
+  if (part != 0 || end == first) return;
+  for (int u = 0; u < 4; ++u) {
+    const int c = blockIdx.x * 32 + u * 8 + lane;
+    float t = 0.f;
+    for (int q = 0; q < parts; ++q) t += sh[share + q][u][lane];
+    if (c < p.C) ((TB*)p.dgate)[image * p.lddgate + c] = (TB)t;
   }
 }
 
 // ---- launches ----
-// stages of the ring: what fits, up to four (kRingBytes holds one of every kind of call with a ring)
-template <typename TR, typename TB, int K, bool VEC, bool WIDE>
-int ring_depth(const GeepsResidual& p, const Shape& s, bool backward, size_t* bytes) {
-  typedef Form<TB, K, VEC, WIDE> F;
-  const bool norm = p.mode & MODE_NORM, join = p.mode & MODE_JOIN, by_pixel = p.gate && p.gate_rows == p.rows, by_image = p.gate && !by_pixel;
-  const int r = backward ? (norm ? 2 : 1) : 1, b = (backward && norm ? 1 : 0) + (join ? 1 : 0) + (by_pixel ? 1 : 0);
-  const size_t threads = backward ? F::backward_threads : F::forward_threads;
-  auto stage = [&](int size) { return F::R * (VEC ? K * 8 * size * threads : (size_t)((p.C * size + 15) / 16 + 1) * 16 * s.slots); };
-  const size_t one = r * stage(sizeof(TR)) + b * stage(sizeof(TB)), kept = backward && by_image ? (size_t)s.threads() * 16 * K * sizeof(float) : 0;
-  const size_t room = kRingBytes / s.per_sm - kept;
-  const int depth = !Columns<K, VEC, 512>::RING ? 0 : one * 4 <= room ? 4 : (int)(room / one);
-  *bytes = depth * one + kept;
-  return depth;
-}
-
 // done: one a kernel
 template <typename F>
 void allow_shared(F kernel, size_t bytes, bool (&done)[64]) {
@@ -859,48 +990,64 @@ void allow_shared(F kernel, size_t bytes, bool (&done)[64]) {
     done[dev] = true;
 }
 
-template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
 void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
   static bool forward_done[64] = {false}, backward_done[64] = {false};
-  size_t smem = 0;
-  const int depth = ring_depth<TR, TB, K, VEC, WIDE>(p, s, backward, &smem);
   if (backward) {
-    const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0;
-    if (smem < meet) smem = meet;
-    const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, MODE, PIXEL>;
-    allow_shared(kernel, smem, backward_done);
-    geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, depth);
+    if constexpr (LARGE || K <= 2 || MODE == MODE_NORM) {         // plan() gives no others
+      const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0, smem = s.smem < meet ? meet : s.smem;
+      const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
+      allow_shared(kernel, smem, backward_done);
+      geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth);
+    }
   } else {
-    const auto kernel = residual_forward_kernel<TR, TB, K, VEC, WIDE, MODE, PIXEL>;
-    allow_shared(kernel, smem, forward_done);
-    geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, depth);
+    const auto kernel = residual_forward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
+    allow_shared(kernel, s.smem, forward_done);
+    geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), s.smem, st, p, s.slot, s.slots, s.depth);
   }
 }
-template <typename TR, typename TB, int K, bool VEC, bool WIDE>
-void launch(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
-  const bool by_pixel = p.gate && p.gate_rows == p.rows;
-  if (p.mode == MODE_NORM) launch_kernel<TR, TB, K, VEC, WIDE, MODE_NORM, false>(p, s, backward, st);
-  else if (p.mode == MODE_JOIN && by_pixel) launch_kernel<TR, TB, K, VEC, WIDE, MODE_JOIN, true>(p, s, backward, st);
-  else if (p.mode == MODE_JOIN) launch_kernel<TR, TB, K, VEC, WIDE, MODE_JOIN, false>(p, s, backward, st);
-  else if (by_pixel) launch_kernel<TR, TB, K, VEC, WIDE, MODE_BOTH, true>(p, s, backward, st);
-  else launch_kernel<TR, TB, K, VEC, WIDE, MODE_BOTH, false>(p, s, backward, st);
+template <typename TR, typename TB, int MODE, bool PIXEL>
+void launch(const GeepsResidual& p, const Shape& s, bool backward, bool vec, cudaStream_t st) {
+  const bool wide = s.slot >= 32;
+  if (!vec) {
+    if (s.large) launch_kernel<TR, TB, 4, false, true, true, MODE, PIXEL>(p, s, backward, st);
+    else if (s.vectors == 2) launch_kernel<TR, TB, 2, false, true, false, MODE, PIXEL>(p, s, backward, st);
+    else if (wide) launch_kernel<TR, TB, 1, false, true, false, MODE, PIXEL>(p, s, backward, st);
+    else launch_kernel<TR, TB, 1, false, false, false, MODE, PIXEL>(p, s, backward, st);
+    return;
+  }
+  if (s.large) launch_kernel<TR, TB, 4, true, true, true, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 1) launch_kernel<TR, TB, 1, true, false, false, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 2 && wide) launch_kernel<TR, TB, 2, true, true, false, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 2) launch_kernel<TR, TB, 2, true, false, false, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 3 && wide) launch_kernel<TR, TB, 3, true, true, false, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 3) launch_kernel<TR, TB, 3, true, false, false, MODE, PIXEL>(p, s, backward, st);
+  else if (wide) launch_kernel<TR, TB, 4, true, true, false, MODE, PIXEL>(p, s, backward, st);
+  else launch_kernel<TR, TB, 4, true, false, false, MODE, PIXEL>(p, s, backward, st);
 }
-template <typename TR, typename TB, bool VEC>
-void run_vec(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
-  if (s.slot < 32) launch<TR, TB, 1, VEC, false>(p, s, backward, st);
-  else if (s.vectors == 1) launch<TR, TB, 1, VEC, true>(p, s, backward, st);
-  else if (s.vectors == 2) launch<TR, TB, 2, VEC, true>(p, s, backward, st);
-  else launch<TR, TB, 4, VEC, true>(p, s, backward, st);
+inline Call call_of(const GeepsResidual& p, bool backward, bool vec) {
+  const bool by_pixel = p.gate && p.gate_rows == p.rows;
+  return {backward, vec, by_pixel, p.gate && !by_pixel, p.mode, p.stream_fp32 ? 4 : 2, p.block_fp32 ? 4 : 2};
 }
 template <typename TR, typename TB>
 void run(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) {
-  const Shape s = plan(p.rows, p.C, backward, p.mode);
-  (vec ? run_vec<TR, TB, true> : run_vec<TR, TB, false>)(p, s, backward, st);
+  const Call c = call_of(p, backward, vec);
+  const Shape s = plan(p.rows, p.C, c);
+  if (p.mode == MODE_NORM) launch<TR, TB, MODE_NORM, false>(p, s, backward, vec, st);
+  else if (p.mode == MODE_JOIN && c.by_pixel) launch<TR, TB, MODE_JOIN, true>(p, s, backward, vec, st);
+  else if (p.mode == MODE_JOIN) launch<TR, TB, MODE_JOIN, false>(p, s, backward, vec, st);
+  else if (c.by_pixel) launch<TR, TB, MODE_BOTH, true>(p, s, backward, vec, st);
+  else launch<TR, TB, MODE_BOTH, false>(p, s, backward, vec, st);
   const bool cuts = p.gate && p.gate_rows < p.rows && p.dgate;
   if (!backward || (s.blocks == 1 && !(cuts && s.slots > 1))) return;
-  int y = cuts ? (s.blocks * s.slots + 31) / 32 : 0;
-  if (y > 64) y = 64;
-  geeps_launch(residual_sums_kernel<TB>, dim3((p.C + 7) / 8, 1 + y), dim3(256), 0, st, p, p.mode, s.blocks, s.slots);
+  int y = 4, parts = 1;
+  if (cuts) {
+    const long long all = (long long)s.blocks * s.slots, per_image = all / p.gate_rows + 2;      // slots that an image may meet
+    while (parts < 32 && parts < per_image) parts <<= 1;
+    const long long items = p.gate_rows <= all ? p.gate_rows : all - 1;
+    y += (int)((items + 32 / parts - 1) / (32 / parts));
+  }
+  geeps_launch(residual_sums_kernel<TB>, dim3((p.C + 31) / 32, y), dim3(kSumsThreads), 0, st, p, p.mode, s.blocks, s.slots, parts);
 }
 
 void run_bf16(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);

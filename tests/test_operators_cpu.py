@@ -6,24 +6,33 @@ import pytest
 from geeps_b200.ops import _lib as L
 
 
-def shape(rows, c, backward=True, mode=3):
-    out = (C.c_int * 4)()
-    assert L.lib().geeps_norm_shape(C.c_longlong(rows), c, int(backward), mode, out) == 0
+def shape(rows, c, backward=True, mode=3, gate_rows=0, vec=True, types=(0, 0)):
+    out = (C.c_int * 8)()
+    assert L.lib().geeps_norm_shape(C.c_longlong(rows), C.c_longlong(gate_rows), c, mode, int(backward), int(vec), *types, out) == 0
     return list(out)
 
 
-@pytest.mark.parametrize("c", [1, 7, 8, 9, 64, 72, 255, 256, 257, 576, 1000, 1024, 4095, 4096, 4097, 8192, 8193, 16383, 16384])
-@pytest.mark.parametrize("rows", [1, 2, 5, 300, 50176, 10_000_000])
+@pytest.mark.parametrize("c", [1, 7, 8, 9, 64, 72, 96, 136, 255, 256, 257, 576, 1000, 1024, 2048, 4095, 4096, 4097, 6144, 6152, 8192, 8193, 12296, 16383,
+                               16384])
+@pytest.mark.parametrize("rows", [1, 5, 300, 50176, 10_000_000])
 @pytest.mark.parametrize("backward", [False, True])
-@pytest.mark.parametrize("mode", [1, 3])
+@pytest.mark.parametrize("mode", [1, 2, 3])
 def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode):
-    vectors, slot, slots, blocks = shape(rows, c, backward, mode)
-    assert slot * slots <= (512 if vectors > 1 or (backward and slot < 32) else 384 if backward else 256)
-    assert vectors * slot * 8 >= c and slot * slots <= 512 and slots >= 1
-    assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
-    assert slot <= 32 or slots <= 15                    # a named barrier for each slot
-    assert 1 <= blocks <= 10_000 and (blocks - 1) * slots < rows
-    assert (slot * slots) % 32 == 0                     # whole warps: their lanes meet in shuffles
+    for types in ((0, 0), (1, 0), (1, 1)):
+        for vec in ((True, False) if c % 8 == 0 else (False,)):
+            for gate in ((0, rows, max(1, rows // 5 if rows % 5 == 0 else 1)) if mode > 1 else (0,)):
+                vectors, slot, slots, blocks, per_sm, depth, smem, large = shape(rows, c, backward, mode, gate, vec, types)
+                assert vectors * slot * 8 >= c and slot * slots <= (512 if large else 384 if backward else 256) and slots >= 1
+                assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
+                assert slot < 32 or slots <= 15                     # a named barrier for each slot of several warps
+                assert 1 <= blocks <= 148 * per_sm and (blocks - 1) * slots < rows
+                assert (slot * slots) % 32 == 0                     # whole warps: their lanes meet in shuffles
+                assert depth == 0 if large else 1 <= depth <= 4
+                # dynamic and static shared memory of all blocks of an SM (1 KB of each is the system's)
+                fixed = 16 * 64 * 4 + (2 * 8 * (512 if large else 384) if backward else 0) + 1024
+                assert per_sm * (smem + fixed) <= 228 * 1024 and smem <= 208 * 1024
+                ring = not large
+                assert not ring or vectors <= (4 if mode == 1 or not backward else 2)
 
 
 def pack(**kw):
@@ -97,13 +106,17 @@ def test_ranges_of_columns_of_one_matrix_do_not_overlap():
 
 
 def test_workspaces():
-    work = L.lib().geeps_residual_work
-    assert work(C.c_longlong(0), C.c_longlong(0), 64, 1) == 0 and work(C.c_longlong(1), C.c_longlong(0), 64, 3) == 0
-    vectors, slot, slots, blocks = shape(50176, 1024)
-    assert work(C.c_longlong(50176), C.c_longlong(0), 1024, 1) == blocks * 2 * 1024
-    assert work(C.c_longlong(50176), C.c_longlong(256), 1024, 3) == (blocks * 4 + blocks * slots + 256) * 1024
-    assert work(C.c_longlong(50176), C.c_longlong(50176), 1024, 2) == blocks * 2 * 1024
-    assert work(C.c_longlong(1 << 22), C.c_longlong(1 << 21), 4096, 2) > 1 << 32
+    def work(rows, gate_rows, c, mode):
+        return L.lib().geeps_residual_work(C.c_longlong(rows), C.c_longlong(gate_rows), c, mode)
+    assert work(0, 0, 64, 1) == 0 and work(1, 0, 64, 3) == 0
+    assert work(1 << 22, 1 << 21, 4096, 2) > 1 << 32
+    for rows, gate, c, mode in ((50176, 0, 1024, 1), (50176, 256, 1024, 3), (50176, 50176, 1024, 2), (7, 7, 16, 3), (40, 4, 8192, 3), (999, 3, 77, 2)):
+        for types in ((0, 0), (1, 0), (1, 1)):
+            for vec in (True, False):
+                _, _, slots, blocks, *_ = shape(rows, c, True, mode, gate, vec, types)
+                by_image = 0 < gate < rows
+                need = (blocks * (4 if mode == 3 else 2) + (3 * blocks * slots + gate if by_image else 0)) * c
+                assert work(rows, gate, c, mode) >= (need if blocks > 1 or by_image else 0)
 
 
 def tensors(ranges, fp32=1):
