@@ -21,7 +21,7 @@ struct Shape {
   int slots;         // rows a block works on at a time
   int blocks, per_sm, depth;
   bool large;
-  size_t smem;
+  size_t ring, smem;      // bytes before the ring, and of all
   int threads() const { return slot * slots; }
 };
 // Blocks of the backward pass have up to 384 threads (168 registers each) and an SM to themselves, so that few blocks leave
@@ -46,7 +46,7 @@ inline size_t stage_bytes(const Call& c, const Shape& s, int C) {
   const bool norm = c.mode & 1, join = c.mode & 2;
   const int r = c.backward ? (norm ? 2 : 1) : 1, b = (c.backward && norm ? 1 : 0) + (join ? 1 : 0) + (c.by_pixel ? 1 : 0);
   auto stage = [&](int size) {
-    return c.vec ? (size_t)s.vectors * 8 * size * block_threads(c.backward, false) : (size_t)((C * size + 15) / 16 + 1) * 16 * s.slots;
+    return c.vec ? (size_t)s.vectors * 8 * size * block_threads(c.backward, false) : (size_t)(8 * s.vectors * s.slot * size + 16) * s.slots;
   };
   return r * stage(c.stream) + b * stage(c.block);
 }
@@ -70,7 +70,7 @@ inline Shape plan(long long rows, int C, const Call& c) {
     if (s.slot < 32 && s.vectors == 2 && !c.vec) continue;
     s.slots = limit / s.slot;
     s.per_sm = c.backward || s.large ? 1 : c.mode == 1 ? 4 : 2;
-    s.smem = fixed_bytes(c, s);
+    s.ring = s.smem = fixed_bytes(c, s);
     const size_t room = kRingBytes / s.per_sm, stage = stage_bytes(c, s, C);
     s.depth = s.large || s.smem > room ? 0 : s.smem + 4 * stage <= room ? 4 : (int)((room - s.smem) / stage);
     if (!s.large && s.depth < 1) continue;
@@ -153,7 +153,7 @@ __device__ __forceinline__ float ld_shared1(uint32_t a) {
 // Rows come through a ring of `depth` stages in shared memory, so that what is on its way takes no registers.  With VEC a thread
 // copies what it reads itself and nobody waits for anybody; otherwise the slot copies the 16-byte pieces that hold the row (up
 // to 15 bytes before and behind it in the same pieces come along) and meets before and after reading them.  The ring starts as
-// zeros, so what has no column or no operand is read from it like the rest.  Rows that do not fit (RING = false) are read where
+// zeros where no copy goes, so what has no column or no operand is read from it like the rest.  Rows that do not fit (RING = false) are read where
 // they lie.  THREADS: as many as a block may have; a thread's places in the ring are then the same for every launch.
 template <int K, bool VEC, bool RING_, int THREADS>
 struct Columns {
@@ -166,7 +166,7 @@ struct Columns {
 
   // bytes of a row of a slot without VEC, and of a stage for one stream of T
   template <typename T>
-  __device__ __forceinline__ int pieces() const { return ((C * (int)sizeof(T) + 15) / 16 + 1) * 16; }
+  __device__ __forceinline__ int pieces() const { return 8 * K * slot * (int)sizeof(T) + 16; }
   template <typename T>
   __device__ __forceinline__ int stage() const { return VEC ? K * 8 * (int)sizeof(T) * THREADS : pieces<T>() * slots; }
   // `from` is what Rows::at() gives; `to` has the thread's 16 * threadIdx.x with VEC, the slot's share without
@@ -214,13 +214,18 @@ struct Columns {
         f[i] = make_float2(there && on(2 * i) ? (float)row[at(2 * i)] : 0.f, there && on(2 * i + 1) ? (float)row[at(2 * i + 1)] : 0.f);
     }
   }
-  // zeros in the place of a row that the slot does not have
+  // zeros in the place of what no copy fills: vectors behind the row, or all of a row that is not there
   template <typename T>
-  __device__ __forceinline__ void no_row(uint32_t to) const {
+  __device__ __forceinline__ void no_copy(uint32_t to, bool all) const {
     if (!VEC) return;
+    constexpr int Q = 8 * sizeof(T) / 16;
 #pragma unroll
-    for (int q = 0; q < K * 8 * (int)sizeof(T) / 16; ++q)
-      asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(to + q * THREADS * 16), "r"(0) : "memory");
+    for (int k = 0; k < K; ++k) {
+      if (!all && on(8 * k)) continue;
+#pragma unroll
+      for (int q = 0; q < Q; ++q)
+        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(to + (k * Q + q) * THREADS * 16), "r"(0) : "memory");
+    }
   }
   // a row from the ring if there is one; zeros where the slot has no such row
   template <typename T>
@@ -237,9 +242,9 @@ struct Columns {
     } else {
       const uint32_t r = from + (threadIdx.x / slot) * pieces<T>() + (uint32_t)((uintptr_t)rows.at(row) & 15);
       const bool any = active && there;
-      float v[2 * N];              // without branches: beyond the row the last column is read and dropped
+      float v[2 * N];              // without branches: what lies behind the row is read and dropped
 #pragma unroll
-      for (int j = 0; j < 2 * N; ++j) v[j] = ld_shared1<T>(r + (on(j) ? at(j) : C - 1) * (int)sizeof(T));
+      for (int j = 0; j < 2 * N; ++j) v[j] = ld_shared1<T>(r + at(j) * (int)sizeof(T));
 #pragma unroll
       for (int i = 0; i < N; ++i) f[i] = make_float2(any && on(2 * i) ? v[2 * i] : 0.f, any && on(2 * i + 1) ? v[2 * i + 1] : 0.f);
     }
@@ -305,14 +310,25 @@ struct Param {
       for (int i = 0; i < C_::N; ++i)
         reg[REG ? i : 0] = make_float2(cols.on(2 * i) ? value(cols.at(2 * i)) : 0.f, cols.on(2 * i + 1) ? value(cols.at(2 * i + 1)) : 0.f);
     } else if (SHARED) {
+      // eight loads are under way at a time: one after the other they were a fifth of a short call
       float* to = reinterpret_cast<float*>(area);
-      for (int i = threadIdx.x; i < 8 * K * cols.slot; i += blockDim.x) {
-        int col = i;
-        if (VEC) {         // [k][half][thread][4]
-          const int e = i & 3, q = i >> 2, t = q % cols.slot, h = q / cols.slot;
-          col = (t + (h >> 1) * cols.slot) * 8 + (h & 1) * 4 + e;
+      const int all = 8 * K * cols.slot, step = blockDim.x;
+      for (int i0 = threadIdx.x; i0 < all; i0 += 8 * step) {
+        float v[8], w[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int i = i0 + u * step;
+          int col = i;
+          if (VEC) {       // [k][half][thread][4]
+            const int e = i & 3, q = i >> 2, t = q % cols.slot, h = q / cols.slot;
+            col = (t + (h >> 1) * cols.slot) * 8 + (h & 1) * 4 + e;
+          }
+          const bool there = i < all && col < cols.C;
+          v[u] = !there ? 0.f : one ? one[col] : other;
+          w[u] = there && two ? two[col] : 1.f;
         }
-        to[i] = col < cols.C ? value(col) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) if (i0 + u * step < all) to[i0 + u * step] = v[u] * w[u];
       }
       at = (uint32_t)__cvta_generic_to_shared(area) + cols.t * (VEC ? 16 : 4);
       area += 8 * K * cols.slot * sizeof(float);
@@ -427,30 +443,47 @@ __device__ __forceinline__ float inverse_root(float v) {
   const float y = rsqrtf(v);
   return v > 0.f && v < 3e38f ? fmaf(y * fmaf(-v * y, y, 1.f), 0.5f, y) : y;
 }
+// Sums over a thread's pairs, in up to four chains: few warps share a scheduler
 template <int N>
 __device__ __forceinline__ float total(const float2 (&f)[N]) {
-  float2 v = f[0];
+  constexpr int W = N >= 16 ? 4 : N >= 8 ? 2 : 1;
+  float2 v[W];
 #pragma unroll
-  for (int i = 1; i < N; ++i) v = add2(v, f[i]);
-  return v.x + v.y;
+  for (int i = 0; i < N; ++i) v[i % W] = i < W ? f[i] : add2(v[i % W], f[i]);
+#pragma unroll
+  for (int i = W >> 1; i; i >>= 1)
+#pragma unroll
+    for (int u = 0; u < i; ++u) v[u] = add2(v[u], v[u + i]);
+  return v[0].x + v[0].y;
 }
 template <int N>
 __device__ __forceinline__ float dot(const float2 (&f)[N], const float2 (&g)[N]) {
-  float2 v = mul2(f[0], g[0]);
+  constexpr int W = N >= 16 ? 4 : N >= 8 ? 2 : 1;
+  float2 v[W];
 #pragma unroll
-  for (int i = 1; i < N; ++i) v = fma2(f[i], g[i], v);
-  return v.x + v.y;
+  for (int i = 0; i < N; ++i) v[i % W] = i < W ? mul2(f[i], g[i]) : fma2(f[i], g[i], v[i % W]);
+#pragma unroll
+  for (int i = W >> 1; i; i >>= 1)
+#pragma unroll
+    for (int u = 0; u < i; ++u) v[u] = add2(v[u], v[u + i]);
+  return v[0].x + v[0].y;
 }
 
-// n = (f - mean) * rstd in place; mean and rstd go to stats
-template <bool WIDE, typename C_, int N>
-__device__ __forceinline__ void normalise(const C_& cols, Slot& s, const GeepsNorm& norm, int row, bool active, float inv_c, float2 (&f)[N]) {
-  float mean = 0.f;
+// n = (f - mean) * rstd in place; mean and rstd go to stats.  used(): called when the first sum of f is there
+template <bool WIDE, typename C_, int N, typename U_>
+__device__ __forceinline__ void normalise(const C_& cols, Slot& s, const GeepsNorm& norm, int row, bool active, float inv_c, float2 (&f)[N],
+                                          U_ used) {
+  float mean = 0.f, squares;
   if (norm.kind == NORM_LAYER) {
     mean = slot_sum<WIDE>(total(f), s) * inv_c;
+    used();
     cols.subtract(f, mean);
+    squares = slot_sum<WIDE>(dot(f, f), s);
+  } else {
+    squares = slot_sum<WIDE>(dot(f, f), s);
+    used();
   }
-  const float rstd = inverse_root(fmaf(slot_sum<WIDE>(dot(f, f), s), inv_c, norm.eps));
+  const float rstd = inverse_root(fmaf(squares, inv_c, norm.eps));
 #pragma unroll
   for (int i = 0; i < N; ++i) f[i] = mul2(f[i], both(rstd));
   if (norm.stats && active && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * row) = make_float2(mean, rstd);
@@ -472,7 +505,7 @@ __device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, flo
   for (int i = 0; i < N; ++i) a[i] = fma2(n[i], m1, fma2(a[i], r, m0));
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + expf(-g)); }      // 0 from exp(-g) = 2^126 on
 template <int N>
 __device__ __forceinline__ void gate_factor(int through_sigmoid, float2 (&g)[N]) {
   if (!through_sigmoid) return;
@@ -481,12 +514,6 @@ __device__ __forceinline__ void gate_factor(int through_sigmoid, float2 (&g)[N])
 }
 __device__ __forceinline__ float2 gate_slope(int through_sigmoid, float2 g) {       // of the factor g by the gate
   return through_sigmoid ? make_float2(g.x * (1.f - g.x), g.y * (1.f - g.y)) : both(1.f);
-}
-
-// zeros to the ring, before any copy
-__device__ __forceinline__ void clear_ring(unsigned char* ring, int bytes) {
-  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
-  __syncthreads();
 }
 
 // The rows of a slot: a range of its own with a gate per image, else every `step`-th of all.  Slots that share a warp take the
@@ -505,7 +532,7 @@ struct Walk {
 // WIDE: a slot is whole warps.  PIXEL: a gate for every row.
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
 __global__ void __launch_bounds__(block_threads(false, LARGE), LARGE ? 1 : MODE == MODE_NORM ? 4 : 2)
-residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
+residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ __align__(16) float red[16][64];
@@ -517,48 +544,55 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
   const Cols cols = {s.t, slot, p.C, slots};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
+  const Walk w(p, slots, s.id, WIDE, by_image);
+  const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
+  int image = 0, left = 0;                     // rows to go with the gate at hand
+
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(shared + ring) + (VEC ? threadIdx.x * 16 : 0);
+  const int at_x = cols.template stage<TR>(), at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
+  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * one;
+  const Rows<TR> res(p.res, p.ldres, cols.first()), h_out(p.out, p.ldout, cols.first());
+  const Rows<TB> x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first()), y_out(p.y, p.ldy, cols.first());
+  // The row that is copied next and the stage that is read and then filled with it: a row's copies start when what lay there is
+  // in registers, so a ring of one stage has a row on its way for most of a turn, too.
+  int ahead = w.lo, now = 0;
+  auto copy = [&]() {
+    if (!cols.RING) return;
+    if (!VEC) s.sync();
+    if (ahead < w.hi) {
+      const uint32_t to = base + now;
+      cols.copy(res.at(ahead), to);
+      if (MODE & MODE_JOIN) cols.copy(x.at(ahead), to + at_x);
+      if (PIXEL) cols.copy(gate.at(ahead), to + at_g);
+    }
+    ahead += w.step;
+    now = now == last ? 0 : now + one;
+    copy_commit();
+  };
+  if (cols.RING) {
+    for (int i = 0; i < depth; ++i) {
+      const uint32_t to = base + i * one;
+      cols.template no_copy<TR>(to, false);
+      if (MODE & MODE_JOIN) cols.template no_copy<TB>(to + at_x, false);
+      if (PIXEL) cols.template no_copy<TB>(to + at_g, false);
+      copy();
+    }
+  }
   unsigned char* area = shared;
   Param<Cols, K, VEC> sw, sb, w2, b2;          // scale * weight and scale * bias of the join, weight and bias of the next norm
   Own<K, THREADS> factor;                      // the gate of the image at hand
   if (MODE & MODE_JOIN) { sw.set(cols, p.post.weight, 1.f, p.scale, area); sb.set(cols, p.post.bias, 0.f, p.scale, area); }
   if (MODE & MODE_NORM) { w2.set(cols, p.pre.weight, 1.f, nullptr, area); b2.set(cols, p.pre.bias, 0.f, nullptr, area); }
   if (by_image && !LARGE) factor.set(area);
-  const Walk w(p, slots, s.id, WIDE, by_image);
-  const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
-  int image = 0, left = 0;                     // rows to go with the gate at hand
-
-  const uint32_t base = (uint32_t)__cvta_generic_to_shared(area) + (VEC ? threadIdx.x * 16 : 0);
-  const int at_x = cols.template stage<TR>(), at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
-  const int one = at_g + (PIXEL ? cols.template stage<TB>() : 0), last = (depth - 1) * one;
-  const Rows<TR> res(p.res, p.ldres, cols.first()), h_out(p.out, p.ldout, cols.first());
-  const Rows<TB> x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first()), y_out(p.y, p.ldy, cols.first());
-  int ahead = w.lo, in = 0, out = 0;           // the row that is copied next, stages that are filled and read next
-  auto copy = [&]() {
-    if (ahead < w.hi) {
-      const uint32_t to = base + in;
-      cols.copy(res.at(ahead), to);
-      if (MODE & MODE_JOIN) cols.copy(x.at(ahead), to + at_x);
-      if (PIXEL) cols.copy(gate.at(ahead), to + at_g);
-    }
-    ahead += w.step;
-    in = in == last ? 0 : in + one;
-    copy_commit();
-  };
-  if (cols.RING) {
-    clear_ring(area, depth * one);
-    for (int i = 0; i < depth - 1; ++i) copy();
-  }
+  __syncthreads();
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
     const bool active = WIDE || row < w.hi;
     if (cols.RING) {
-      if (!VEC) s.sync();
-      copy();
       copy_wait(depth);
       if (!VEC) s.sync();
     }
-    const uint32_t from = base + out;
-    if (cols.RING) out = out == last ? 0 : out + one;
+    const uint32_t from = base + now;
     float2 h[N];
     if (MODE & MODE_JOIN) {
       float2 z[N];
@@ -574,7 +608,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
           for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(g[4 * k]));
         }
       }
-      if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, active, inv_c, z);
+      if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, active, inv_c, z, [] {});
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float2 a[4], b[4];
@@ -600,12 +634,13 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
       cols.load(res, row, active, true, from, h);
 #pragma unroll
       for (int j = 0; j < N; ++j) h[j] = add2(h[j], z[j]);
+      copy();
       cols.store(h_out.at(row), active, h);
     } else {
       cols.load(res, row, active, true, from, h);
     }
     if (MODE & MODE_NORM) {
-      normalise<WIDE>(cols, s, p.pre, row, active, inv_c, h);
+      normalise<WIDE>(cols, s, p.pre, row, active, inv_c, h, [&] { if (!(MODE & MODE_JOIN)) copy(); });
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float2 a[4], b[4];
@@ -649,7 +684,7 @@ __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int
 
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
 __global__ void __launch_bounds__(block_threads(true, LARGE))
-residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth) {
+residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
   constexpr int N = 4 * K, THREADS = block_threads(true, LARGE);
@@ -663,15 +698,8 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   const Cols cols = {s.t, slot, p.C, slots};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
-  unsigned char* area = shared;
   Param<Cols, K, VEC> sw, sb, w2;              // scale * weight, scale * bias (for a gate's gradient), the next norm's weight
   Own<K, THREADS> factor;                      // the gate of the image at hand
-  if (MODE & MODE_JOIN) {
-    sw.set(cols, p.post.weight, 1.f, p.scale, area);
-    if (PIXEL) sb.set(cols, p.post.bias, 0.f, p.scale, area);
-  }
-  if (MODE & MODE_NORM) w2.set(cols, p.pre.weight, 1.f, nullptr, area);
-  if (by_image && !LARGE) factor.set(area);
   float2 a0[N], a1[N], n0[N], n1[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) a0[i] = a1[i] = n0[i] = n1[i] = both(0.f);
@@ -679,7 +707,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   const int per_gate = by_image ? (int)(p.rows / p.gate_rows) : 1;
   int image = -1, left = 0;
 
-  const uint32_t base = (uint32_t)__cvta_generic_to_shared(area) + (VEC ? threadIdx.x * 16 : 0);
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(shared + ring) + (VEC ? threadIdx.x * 16 : 0);
   const int at_o = cols.template stage<TR>(), at_y = at_o + (MODE & MODE_NORM ? cols.template stage<TR>() : 0);
   const int at_x = at_y + (MODE & MODE_NORM ? cols.template stage<TB>() : 0);
   const int at_g = at_x + (MODE & MODE_JOIN ? cols.template stage<TB>() : 0);
@@ -688,22 +716,32 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   const Rows<TB> dy(p.dy, p.lddy, cols.first()), x(p.x, p.ldx, cols.first()), gate(p.gate, p.ldgate, cols.first());
   const Rows<TB> dx(p.dx, p.lddx, cols.first()), dgate(p.dgate, p.lddgate, cols.first());
   const bool has_dout = p.dout != nullptr;
-  int ahead = w.lo, in = 0, out = 0;
-  auto copy = [&]() {
-    const uint32_t to = base + in;
+  int ahead = w.lo, now = 0;                   // as in the forward pass, the branch's share of a row later than the rest
+  auto copy_stream = [&]() {
+    if (!cols.RING) return;
+    if (!VEC) s.sync();
+    const uint32_t to = base + now;
     if (ahead < w.hi) {
       if (has_dout) cols.copy(dout.at(ahead), to);
       if (MODE & MODE_NORM) { cols.copy(h.at(ahead), to + at_o); cols.copy(dy.at(ahead), to + at_y); }
+    } else if (!WIDE) {                        // rows that are read and are none: they add nothing to the sums
+      cols.template no_copy<TR>(to, true);
+      if (MODE & MODE_NORM) { cols.template no_copy<TR>(to + at_o, true); cols.template no_copy<TB>(to + at_y, true); }
+    }
+  };
+  auto copy_branch = [&]() {
+    if (!cols.RING) return;
+    if (!VEC && (MODE & MODE_JOIN)) s.sync();
+    const uint32_t to = base + now;
+    if (ahead < w.hi) {
       if (MODE & MODE_JOIN) cols.copy(x.at(ahead), to + at_x);
       if (PIXEL) cols.copy(gate.at(ahead), to + at_g);
-    } else if (!WIDE) {                        // rows that are read and are none: they add nothing to the sums
-      cols.template no_row<TR>(to);
-      if (MODE & MODE_NORM) { cols.template no_row<TR>(to + at_o); cols.template no_row<TB>(to + at_y); }
-      if (MODE & MODE_JOIN) cols.template no_row<TB>(to + at_x);
-      if (PIXEL) cols.template no_row<TB>(to + at_g);
+    } else if (!WIDE) {
+      if (MODE & MODE_JOIN) cols.template no_copy<TB>(to + at_x, true);
+      if (PIXEL) cols.template no_copy<TB>(to + at_g, true);
     }
     ahead += w.step;
-    in = in == last ? 0 : in + one;
+    now = now == last ? 0 : now + one;
     copy_commit();
   };
   // The rows of an image that this slot has are done: its part of the gate's gradient, all of it if no other slot has any.  With
@@ -753,20 +791,32 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
   };
   if (cols.RING) {
-    clear_ring(area, depth * one);
-    for (int i = 0; i < depth - 1; ++i) copy();
-  } else __syncthreads();
+    for (int i = 0; i < depth; ++i) {
+      const uint32_t to = base + i * one;
+      cols.template no_copy<TR>(to, !has_dout);
+      if (MODE & MODE_NORM) { cols.template no_copy<TR>(to + at_o, false); cols.template no_copy<TB>(to + at_y, false); }
+      if (MODE & MODE_JOIN) cols.template no_copy<TB>(to + at_x, false);
+      if (PIXEL) cols.template no_copy<TB>(to + at_g, false);
+      copy_stream();
+      copy_branch();
+    }
+  }
+  unsigned char* area = shared;
+  if (MODE & MODE_JOIN) {
+    sw.set(cols, p.post.weight, 1.f, p.scale, area);
+    if (PIXEL) sb.set(cols, p.post.bias, 0.f, p.scale, area);
+  }
+  if (MODE & MODE_NORM) w2.set(cols, p.pre.weight, 1.f, nullptr, area);
+  if (by_image && !LARGE) factor.set(area);
+  __syncthreads();
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
     const bool active = WIDE || row < w.hi;
     if (cols.RING) {
-      if (!VEC) s.sync();
-      copy();
       copy_wait(depth);
       if (!VEC) s.sync();
     }
-    const uint32_t from = base + out;
-    if (cols.RING) out = out == last ? 0 : out + one;
+    const uint32_t from = base + now;
     // Statistics of the rows of several turns at a time, a row a lane: a load for every turn was waited for in the turn that
     // issued it, with the loads from shared memory that share its scoreboard (50176 x 576: 36 % of the time).
     const int chunk = WIDE ? 32 : slot, k0 = i & (chunk - 1);
@@ -811,6 +861,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     } else if (cols.RING) {
       cols.load(dout, row, active, has_dout, from, dh);
     }
+    if (MODE & MODE_NORM) copy_stream();       // what it overwrites has gone into sums that are there
     cols.store(dres.at(row), active, dh);
     if (MODE & MODE_JOIN) {
       if (cols.RING) load_branch();
@@ -851,8 +902,10 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       }
       if (PIXEL && p.dgate) cols.store(dgate.at(row), active, dg);
       if (p.post.kind) norm_gradient<WIDE>(s, p.post.kind, st1.y, inv_c, z, dh);
+      if (!(MODE & MODE_NORM)) copy_stream();
+      copy_branch();
       cols.store(dx.at(row), active, dh);
-    }
+    } else copy_branch();
   }
   if (by_image && image >= 0) image_done();
   // the slots' sums, in slot order, in the threads of slot 0
@@ -998,12 +1051,12 @@ void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaSt
       const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0, smem = s.smem < meet ? meet : s.smem;
       const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
       allow_shared(kernel, smem, backward_done);
-      geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth);
+      geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
     }
   } else {
     const auto kernel = residual_forward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
     allow_shared(kernel, s.smem, forward_done);
-    geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), s.smem, st, p, s.slot, s.slots, s.depth);
+    geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), s.smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
   }
 }
 template <typename TR, typename TB, int MODE, bool PIXEL>
