@@ -28,7 +28,8 @@ namespace {
 struct Use { const void* p; long long ld, rows; int size; bool out; };
 bool vectors_ok(const Use& u, int C) {
   if (!u.p) return true;
-  return ((uintptr_t)u.p & 15) == 0 && (u.rows <= 1 || (u.ld * u.size & 15) == 0) && C % kVec == 0;
+  const uintptr_t line = kVec * u.size - 1;
+  return ((uintptr_t)u.p & line) == 0 && (u.rows <= 1 || ((uintptr_t)(u.ld * u.size) & line) == 0) && C % kVec == 0;
 }
 // Do two operands share memory in a way that rows of one would be overwritten before the other is read?  The very same rows
 // are fine (every thread reads its columns of a row before it writes them), and so are two ranges of columns of one matrix.

@@ -24,57 +24,65 @@ struct Shape {
   size_t ring, smem;      // bytes before the ring, and of all
   int threads() const { return slot * slots; }
 };
-// Blocks of the backward pass have up to 384 threads (168 registers each) and an SM to themselves, so that few blocks leave
-// column sums behind; forward several blocks of 256 share an SM.
-constexpr int kForwardThreads = 256, kBackwardThreads = 384, kLargeThreads = 512;
-constexpr int block_threads(bool backward, bool large) { return large ? kLargeThreads : backward ? kBackwardThreads : kForwardThreads; }
+// Threads of a block.  Backward a block has an SM to itself, so that few blocks leave column sums behind, and as many threads as
+// their column sums leave registers for; forward several blocks of 256 share an SM.
+__host__ __device__ constexpr int block_threads(bool backward, bool vec, bool large, int vectors, int mode) {
+  return large ? 512 : !backward ? 256 : !vec ? 512 : vectors > 2 && mode != MODE_NORM ? 256 : 384;
+}
+// ... and blocks an SM that registers allow forward
+__host__ __device__ constexpr int blocks_forward(bool large, int mode) { return large ? 1 : mode == MODE_NORM ? 4 : 2; }
 
 // What a call keeps in shared memory: parameters of the columns (one vector a thread keeps them in registers), with a gate per
 // image its factors, and the ring.
 struct Call {
   bool backward, vec, by_pixel, by_image;
   int mode, stream, block;                 // sizes of the two types
+  int threads(const Shape& s) const { return block_threads(backward, vec, s.large, s.vectors, mode); }
 };
 inline size_t fixed_bytes(const Call& c, const Shape& s) {
-  const bool norm = c.mode & 1, join = c.mode & 2;
-  const int params = c.backward ? (norm ? 1 : 0) + (join ? c.by_pixel ? 2 : 1 : 0) : (norm ? 2 : 0) + (join ? 2 : 0);
+  const bool norm = c.mode & MODE_NORM, join = c.mode & MODE_JOIN;
+  const int params = c.backward ? (norm ? 1 : 0) + (join ? c.by_pixel || c.by_image ? 2 : 1 : 0) : (norm ? 2 : 0) + (join ? 2 : 0);
   const size_t thread = (size_t)8 * s.vectors * sizeof(float);         // a value for each of a thread's columns
-  return (s.large || s.vectors == 1 ? 0 : params * thread * s.slot) +
-         (c.by_image && !s.large ? thread * block_threads(c.backward, s.large) : 0);
+  return (s.large || s.vectors == 1 ? 0 : params * thread * s.slot) + (c.by_image ? thread * c.threads(s) : 0);
 }
-inline size_t stage_bytes(const Call& c, const Shape& s, int C) {
-  const bool norm = c.mode & 1, join = c.mode & 2;
+inline size_t stage_bytes(const Call& c, const Shape& s) {
+  const bool norm = c.mode & MODE_NORM, join = c.mode & MODE_JOIN;
   const int r = c.backward ? (norm ? 2 : 1) : 1, b = (c.backward && norm ? 1 : 0) + (join ? 1 : 0) + (c.by_pixel ? 1 : 0);
   auto stage = [&](int size) {
-    return c.vec ? (size_t)s.vectors * 8 * size * block_threads(c.backward, false) : (size_t)(8 * s.vectors * s.slot * size + 16) * s.slots;
+    return c.vec ? (size_t)s.vectors * 8 * size * c.threads(s) : (size_t)(8 * s.vectors * s.slot * size + 16) * s.slots;
   };
   return r * stage(c.stream) + b * stage(c.block);
 }
-// How many vectors a thread has: more save what every thread does once a row, up to the registers (backward the column sums of
-// a join and of a norm behind it leave room for two), fewer leave no lane without work.  The costs are instructions a row.
-// Eight threads a row at least, where there is so much: a row's pieces in a warp's access are then whole lines.
+// How many vectors a thread has: more save what every thread does once a row, fewer leave no lane without work.  The costs are
+// instructions a row.  Eight threads a row at least, where there is so much: pieces of rows in a warp's access are whole lines then
+// (50176 x 64 backward 12 us, 21 with four).  A join with a norm behind it has four column sums: two vectors while they do
+// (50176 x 1024 backward 110 us, four vectors by half the threads 180).
 inline Shape plan(long long rows, int C, const Call& c) {
   Shape best;
-  const int vec = (C + kVec - 1) / kVec, most = c.vec ? c.backward && c.mode != 1 ? 2 : 4 : 2;
+  const int vec = (C + kVec - 1) / kVec, most = c.vec ? 4 : 2;
   long long least = -1;
   for (int k = 1; k <= most + 1; ++k) {
     Shape s;
     s.large = k > most;
     s.vectors = s.large ? 4 : k;
-    const int need = (vec + s.vectors - 1) / s.vectors, limit = block_threads(c.backward, s.large);
-    if (need > limit || (s.large && least >= 0)) continue;
+    const int need = (vec + s.vectors - 1) / s.vectors, limit = c.threads(s);
+    if (need > limit || ((s.large || (c.backward && c.mode == MODE_BOTH && k > 2)) && least >= 0)) continue;
     s.slot = 1;
     while (s.slot < 32 && (s.slot < need || (s.slot < 8 && s.slot < vec))) s.slot <<= 1;
     if (need > 32 || s.large) s.slot = (need + 31) / 32 * 32;
     if (s.slot >= 32 && s.vectors == 1 && c.vec) continue;
     if (s.slot < 32 && s.vectors == 2 && !c.vec) continue;
     s.slots = limit / s.slot;
-    s.per_sm = c.backward || s.large ? 1 : c.mode == 1 ? 4 : 2;
-    s.ring = s.smem = fixed_bytes(c, s);
-    const size_t room = kRingBytes / s.per_sm, stage = stage_bytes(c, s, C);
-    s.depth = s.large || s.smem > room ? 0 : s.smem + 4 * stage <= room ? 4 : (int)((room - s.smem) / stage);
+    s.ring = fixed_bytes(c, s);
+    const size_t stage = stage_bytes(c, s);
+    s.depth = 0;
+    for (s.per_sm = c.backward ? 1 : blocks_forward(s.large, c.mode); s.per_sm >= 1 && s.depth < 1; --s.per_sm) {
+      const size_t room = kRingBytes / s.per_sm;
+      s.depth = s.ring > room ? 0 : s.ring + 4 * stage <= room ? 4 : (int)((room - s.ring) / stage);
+    }
+    ++s.per_sm;
     if (!s.large && s.depth < 1) continue;
-    s.smem += s.depth * stage;
+    s.smem = s.ring + s.depth * stage;
     const long long cost = (long long)s.slot * (100 + 45 * s.vectors + (s.slot > 32 ? 60 : 0));
     if (least < 0 || (cost < least && c.vec)) { least = cost; best = s; }       // single columns cost the same for any k
   }
@@ -97,6 +105,14 @@ struct Rows {
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// ... a piece whose other half of a 32-byte sector comes with another copy
+__device__ __forceinline__ void copy16_half(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void st_f8(float* p, float2 a, float2 b, float2 c, float2 d) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y),
+               "f"(d.x), "f"(d.y) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // until at most depth - 1 of this thread's groups are under way
@@ -153,13 +169,13 @@ __device__ __forceinline__ float ld_shared1(uint32_t a) {
 // Rows come through a ring of `depth` stages in shared memory, so that what is on its way takes no registers.  With VEC a thread
 // copies what it reads itself and nobody waits for anybody; otherwise the slot copies the 16-byte pieces that hold the row (up
 // to 15 bytes before and behind it in the same pieces come along) and meets before and after reading them.  The ring starts as
-// zeros where no copy goes, so what has no column or no operand is read from it like the rest.  Rows that do not fit (RING = false) are read where
-// they lie.  THREADS: as many as a block may have; a thread's places in the ring are then the same for every launch.
-template <int K, bool VEC, bool RING_, int THREADS>
+// zeros where no copy goes, so what has no column or no operand is read from it like the rest.  LARGE rows take more threads, leave
+// no room for parameters, and are read where they lie if they do not fit the ring.  THREADS: as many as a block may have; a thread's places in the ring are then the same for every launch.
+template <int K, bool VEC, bool LARGE, int THREADS>
 struct Columns {
   static constexpr int N = 4 * K;      // pairs
-  static constexpr bool RING = RING_;
   int t, slot, C, slots;
+  bool ring;
   __device__ __forceinline__ int first() const { return VEC ? at(0) : 0; }
   __device__ __forceinline__ int at(int j) const { return VEC ? (t + (j >> 3) * slot) * 8 + (j & 7) : t + j * slot; }
   __device__ __forceinline__ bool on(int j) const { return at(VEC ? j & ~7 : j) < C; }
@@ -178,7 +194,10 @@ struct Columns {
       for (int k = 0; k < K; ++k) {
         if (!on(8 * k)) continue;
 #pragma unroll
-        for (int q = 0; q < Q; ++q) copy16(to + (k * Q + q) * THREADS * 16, from + k * slot * 8 + q * (8 / Q));
+        for (int q = 0; q < Q; ++q) {
+          if (Q == 1) copy16(to + k * THREADS * 16, from + k * slot * 8);
+          else copy16_half(to + (k * Q + q) * THREADS * 16, from + k * slot * 8 + q * (8 / Q));
+        }
       }
     } else {
       const uintptr_t start = (uintptr_t)from & ~(uintptr_t)15, end = (uintptr_t)(from + C);
@@ -230,7 +249,7 @@ struct Columns {
   // a row from the ring if there is one; zeros where the slot has no such row
   template <typename T>
   __device__ __forceinline__ void load(const Rows<T>& rows, int row, bool active, bool there, uint32_t from, float2 (&f)[N]) const {
-    if (!RING) {
+    if (LARGE && !ring) {
       fetch(rows.at(row), active && there, f);
     } else if (VEC) {
       constexpr int Q = 8 * sizeof(T) / 16;
@@ -262,9 +281,7 @@ struct Columns {
           *reinterpret_cast<uint4*>(row + c) = make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y),
                                                           pack_bf16x2(v[2].x, v[2].y), pack_bf16x2(v[3].x, v[3].y));
         } else {
-          float* r = reinterpret_cast<float*>(row) + c;
-          st_f4(r, make_float4(v[0].x, v[0].y, v[1].x, v[1].y));
-          st_f4(r + 4, make_float4(v[2].x, v[2].y, v[3].x, v[3].y));
+          st_f8(reinterpret_cast<float*>(row) + c, v[0], v[1], v[2], v[3]);
         }
       }
     } else {
@@ -294,9 +311,9 @@ struct Columns {
 // A parameter of every column: one, times another, or `other` where there is none.  In registers for one vector a thread, else
 // in shared memory (16 bytes of a vector's half beside those of the next thread), read for every row; rows that do not fit read
 // it where it lies.
-template <typename C_, int K, bool VEC>
+template <typename C_, int K, bool VEC, bool LARGE>
 struct Param {
-  static constexpr bool REG = K == 1 && C_::RING, SHARED = K > 1 && C_::RING;
+  static constexpr bool REG = K == 1, SHARED = K > 1 && !LARGE;
   float2 reg[REG ? 4 * K : 1];
   uint32_t at;
   const float *one, *two;
@@ -351,10 +368,25 @@ struct Param {
       for (int e = 0; e < 4; ++e)
         f[e] = make_float2(ld_shared1<float>(at + (8 * k + 2 * e) * cols.slot * 4), ld_shared1<float>(at + (8 * k + 2 * e + 1) * cols.slot * 4));
     } else {
+      const int c = cols.at(8 * k);
+      if (VEC && (((uintptr_t)one | (uintptr_t)two) & 15) == 0) {
+        float v[8], w[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = 8 * k + 2 * e;
-        f[e] = make_float2(cols.on(j) ? value(cols.at(j)) : 0.f, cols.on(j + 1) ? value(cols.at(j + 1)) : 0.f);
+        for (int h = 0; h < 2; ++h) {
+          const bool on = cols.on(8 * k);
+          const float4 a = on && one ? ld_f4(one + c + 4 * h) : make_float4(on ? other : 0.f, on ? other : 0.f, on ? other : 0.f, on ? other : 0.f);
+          const float4 b = on && two ? ld_f4(two + c + 4 * h) : make_float4(1.f, 1.f, 1.f, 1.f);
+          v[4 * h] = a.x; v[4 * h + 1] = a.y; v[4 * h + 2] = a.z; v[4 * h + 3] = a.w;
+          w[4 * h] = b.x; w[4 * h + 1] = b.y; w[4 * h + 2] = b.z; w[4 * h + 3] = b.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = make_float2(v[2 * e] * w[2 * e], v[2 * e + 1] * w[2 * e + 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 8 * k + 2 * e;
+          f[e] = make_float2(cols.on(j) ? value(cols.at(j)) : 0.f, cols.on(j + 1) ? value(cols.at(j + 1)) : 0.f);
+        }
       }
     }
   }
@@ -531,17 +563,17 @@ struct Walk {
 
 // WIDE: a slot is whole warps.  PIXEL: a gate for every row.
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(block_threads(false, LARGE), LARGE ? 1 : MODE == MODE_NORM ? 4 : 2)
+__global__ void __launch_bounds__(block_threads(false, VEC, LARGE, K, MODE), blocks_forward(LARGE, MODE))
 residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ __align__(16) float red[16][64];
-  constexpr int N = 4 * K, THREADS = block_threads(false, LARGE);
-  typedef Columns<K, VEC, !LARGE, THREADS> Cols;
+  constexpr int N = 4 * K, THREADS = block_threads(false, VEC, LARGE, K, MODE);
+  typedef Columns<K, VEC, LARGE, THREADS> Cols;
   for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
-  const Cols cols = {s.t, slot, p.C, slots};
+  const Cols cols = {s.t, slot, p.C, slots, !LARGE || depth > 0};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
   const Walk w(p, slots, s.id, WIDE, by_image);
@@ -557,7 +589,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
   // in registers, so a ring of one stage has a row on its way for most of a turn, too.
   int ahead = w.lo, now = 0;
   auto copy = [&]() {
-    if (!cols.RING) return;
+    if (!cols.ring) return;
     if (!VEC) s.sync();
     if (ahead < w.hi) {
       const uint32_t to = base + now;
@@ -569,7 +601,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
     now = now == last ? 0 : now + one;
     copy_commit();
   };
-  if (cols.RING) {
+  if (cols.ring) {
     for (int i = 0; i < depth; ++i) {
       const uint32_t to = base + i * one;
       cols.template no_copy<TR>(to, false);
@@ -579,16 +611,16 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
     }
   }
   unsigned char* area = shared;
-  Param<Cols, K, VEC> sw, sb, w2, b2;          // scale * weight and scale * bias of the join, weight and bias of the next norm
+  Param<Cols, K, VEC, LARGE> sw, sb, w2, b2;          // scale * weight and scale * bias of the join, weight and bias of the next norm
   Own<K, THREADS> factor;                      // the gate of the image at hand
   if (MODE & MODE_JOIN) { sw.set(cols, p.post.weight, 1.f, p.scale, area); sb.set(cols, p.post.bias, 0.f, p.scale, area); }
   if (MODE & MODE_NORM) { w2.set(cols, p.pre.weight, 1.f, nullptr, area); b2.set(cols, p.pre.bias, 0.f, nullptr, area); }
-  if (by_image && !LARGE) factor.set(area);
+  if (by_image) factor.set(area);
   __syncthreads();
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
     const bool active = WIDE || row < w.hi;
-    if (cols.RING) {
+    if (cols.ring) {
       copy_wait(depth);
       if (!VEC) s.sync();
     }
@@ -600,13 +632,11 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
       if (by_image && left-- == 0 && active) {
         image = row / per_gate;
         left = (image + 1) * per_gate - row - 1;
-        if (!LARGE) {
-          float2 g[N];
-          cols.fetch(gate.at(image), true, g);
-          gate_factor(p.sigmoid, g);
+        float2 g[N];
+        cols.fetch(gate.at(image), true, g);
+        gate_factor(p.sigmoid, g);
 #pragma unroll
-          for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(g[4 * k]));
-        }
+        for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(g[4 * k]));
       }
       if (p.post.kind) normalise<WIDE>(cols, s, p.post, row, active, inv_c, z, [] {});
 #pragma unroll
@@ -616,7 +646,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[4 * k + e] = fma2(z[4 * k + e], a[e], b[e]);
       }
-      if (by_image && !LARGE) {
+      if (by_image) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           float2 g[4];
@@ -624,9 +654,9 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
 #pragma unroll
           for (int e = 0; e < 4; ++e) z[4 * k + e] = mul2(z[4 * k + e], g[e]);
         }
-      } else if (PIXEL || (by_image && LARGE)) {
+      } else if (PIXEL) {
         float2 g[N];
-        if (PIXEL) cols.load(gate, row, active, true, from + at_g, g); else cols.fetch(gate.at(image), active, g);
+        cols.load(gate, row, active, true, from + at_g, g);
         gate_factor(p.sigmoid, g);
 #pragma unroll
         for (int j = 0; j < N; ++j) z[j] = mul2(z[j], g[j]);
@@ -683,22 +713,22 @@ __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int
 }
 
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(block_threads(true, LARGE))
+__global__ void __launch_bounds__(block_threads(true, VEC, LARGE, K, MODE))
 residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
-  constexpr int N = 4 * K, THREADS = block_threads(true, LARGE);
-  typedef Columns<K, VEC, !LARGE, THREADS> Cols;
+  constexpr int N = 4 * K, THREADS = block_threads(true, VEC, LARGE, K, MODE);
+  typedef Columns<K, VEC, LARGE, THREADS> Cols;
   __shared__ float2 stats[2][THREADS];
   __shared__ __align__(16) float red[16][64];
   for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
   stats[0][threadIdx.x] = stats[1][threadIdx.x] = both(0.f);
-  const Cols cols = {s.t, slot, p.C, slots};
+  const Cols cols = {s.t, slot, p.C, slots, !LARGE || depth > 0};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
-  Param<Cols, K, VEC> sw, sb, w2;              // scale * weight, scale * bias (for a gate's gradient), the next norm's weight
+  Param<Cols, K, VEC, LARGE> sw, sb, w2;              // scale * weight, scale * bias (for a gate's gradient), the next norm's weight
   Own<K, THREADS> factor;                      // the gate of the image at hand
   float2 a0[N], a1[N], n0[N], n1[N];
 #pragma unroll
@@ -718,7 +748,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   const bool has_dout = p.dout != nullptr;
   int ahead = w.lo, now = 0;                   // as in the forward pass, the branch's share of a row later than the rest
   auto copy_stream = [&]() {
-    if (!cols.RING) return;
+    if (!cols.ring) return;
     if (!VEC) s.sync();
     const uint32_t to = base + now;
     if (ahead < w.hi) {
@@ -730,7 +760,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
   };
   auto copy_branch = [&]() {
-    if (!cols.RING) return;
+    if (!cols.ring) return;
     if (!VEC && (MODE & MODE_JOIN)) s.sync();
     const uint32_t to = base + now;
     if (ahead < w.hi) {
@@ -749,33 +779,25 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   // every thread its own columns.
   float2* before = by_image ? reinterpret_cast<float2*>(sums_of_images(p, MODE, blockIdx.x * slots + s.id)) : nullptr;
   bool none_before = true;
-  auto image_done = [&]() {
-    float2 g[N], d[N];
-    cols.fetch(gate.at(image), true, g);
-    gate_factor(p.sigmoid, g);
+  auto image_done = [&](bool end) {
+    float2 d[N];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float2 m[4];
-      sw.get(cols, k, m);
+      float2 m[4], b[4], g[4];
+      sw.get(cols, k, m); sb.get(cols, k, b); factor.get(k, g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int i = 4 * k + e, c = cols.at(2 * i), c1 = cols.at(2 * i + 1);
-        float2 bias = both(0.f);
-        if (p.post.bias) {
-          if (cols.on(2 * i)) bias.x = p.post.bias[c] * (p.scale ? p.scale[c] : 1.f);
-          if (cols.on(2 * i + 1)) bias.y = p.post.bias[c1] * (p.scale ? p.scale[c1] : 1.f);
+        const int i = 4 * k + e;
+        d[i] = mul2(fma2(m[e], a0[i], mul2(b[e], a1[i])), gate_slope(p.sigmoid, g[e]));
+        float2 sum = mul2(g[e], a0[i]), sum1 = mul2(g[e], a1[i]);
+        float2 *x = before + cols.at(2 * i), *y = before + cols.at(2 * i + 1);           // [column]{A, B}
+        if (!none_before) {
+          const float2 v = cols.on(2 * i) ? *x : both(0.f), u = cols.on(2 * i + 1) ? *y : both(0.f);
+          sum = add2(sum, make_float2(v.x, u.x)); sum1 = add2(sum1, make_float2(v.y, u.y));
         }
-        d[i] = mul2(fma2(m[e], a0[i], mul2(bias, a1[i])), gate_slope(p.sigmoid, g[i]));
-        float2 sum = mul2(g[i], a0[i]), sum1 = mul2(g[i], a1[i]);
-        if (cols.on(2 * i)) {                    // [column]{A, B}
-          if (!none_before) { sum.x += before[c].x; sum1.x += before[c].y; }
-          before[c] = make_float2(sum.x, sum1.x);
-        }
-        if (cols.on(2 * i + 1)) {
-          if (!none_before) { sum.y += before[c1].x; sum1.y += before[c1].y; }
-          before[c1] = make_float2(sum.y, sum1.y);
-        }
-        a0[i] = a1[i] = both(0.f);
+        if (!end && cols.on(2 * i)) *x = make_float2(sum.x, sum1.x);
+        if (!end && cols.on(2 * i + 1)) *y = make_float2(sum.y, sum1.y);
+        a0[i] = end ? sum : both(0.f); a1[i] = end ? sum1 : both(0.f);
       }
     }
     none_before = false;
@@ -790,7 +812,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       }
     }
   };
-  if (cols.RING) {
+  if (cols.ring) {
     for (int i = 0; i < depth; ++i) {
       const uint32_t to = base + i * one;
       cols.template no_copy<TR>(to, !has_dout);
@@ -804,15 +826,15 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   unsigned char* area = shared;
   if (MODE & MODE_JOIN) {
     sw.set(cols, p.post.weight, 1.f, p.scale, area);
-    if (PIXEL) sb.set(cols, p.post.bias, 0.f, p.scale, area);
+    if (p.gate) sb.set(cols, p.post.bias, 0.f, p.scale, area);
   }
   if (MODE & MODE_NORM) w2.set(cols, p.pre.weight, 1.f, nullptr, area);
-  if (by_image && !LARGE) factor.set(area);
+  if (by_image) factor.set(area);
   __syncthreads();
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
     const bool active = WIDE || row < w.hi;
-    if (cols.RING) {
+    if (cols.ring) {
       copy_wait(depth);
       if (!VEC) s.sync();
     }
@@ -837,7 +859,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       if (MODE & MODE_JOIN) cols.load(x, row, active, true, from + at_x, z);
       if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_factor(p.sigmoid, g); }
     };
-    if (!cols.RING) { load_branch(); cols.load(dout, row, active, has_dout, from, dh); }
+    if (!cols.ring) { load_branch(); cols.load(dout, row, active, has_dout, from, dh); }
     if (MODE & MODE_NORM) {
       float2 n[N], a[N];
       cols.load(h, row, active, true, from + at_o, n);
@@ -855,30 +877,27 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         }
       }
       norm_gradient<WIDE>(s, p.pre.kind, st2.y, inv_c, n, a);
-      if (cols.RING) cols.load(dout, row, active, has_dout, from, dh);
+      if (cols.ring) cols.load(dout, row, active, has_dout, from, dh);
 #pragma unroll
       for (int j = 0; j < N; ++j) dh[j] = add2(dh[j], a[j]);
-    } else if (cols.RING) {
+    } else if (cols.ring) {
       cols.load(dout, row, active, has_dout, from, dh);
     }
     if (MODE & MODE_NORM) copy_stream();       // what it overwrites has gone into sums that are there
     cols.store(dres.at(row), active, dh);
     if (MODE & MODE_JOIN) {
-      if (cols.RING) load_branch();
+      if (cols.ring) load_branch();
       if (by_image && left == 0 && active) {
-        if (image >= 0) image_done();
+        if (image >= 0) image_done(false);
         image = row / per_gate;
         left = (image + 1) * per_gate - row;
-        if (!LARGE) {
-          float2 f[N];
-          cols.fetch(gate.at(image), true, f);
-          gate_factor(p.sigmoid, f);
+        float2 f[N];
+        cols.fetch(gate.at(image), true, f);
+        gate_factor(p.sigmoid, f);
 #pragma unroll
-          for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(f[4 * k]));
-        }
+        for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(f[4 * k]));
       }
       --left;
-      if (by_image && LARGE) { cols.fetch(gate.at(image), true, g); gate_factor(p.sigmoid, g); }
       if (p.post.kind) normalised(z, st1);
       float2 dg[N];
 #pragma unroll
@@ -886,7 +905,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         float2 m[4], f[4], b[4];
         sw.get(cols, k, m);
         if (PIXEL) sb.get(cols, k, b);
-        if (by_image && !LARGE) factor.get(k, f);
+        if (by_image) factor.get(k, f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int j = 4 * k + e;
@@ -896,7 +915,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
             d = mul2(d, g[j]);
           }
           a0[j] = fma2(d, z[j], a0[j]); a1[j] = add2(a1[j], d);
-          if (by_image) d = mul2(d, LARGE ? g[j] : f[e]);
+          if (by_image) d = mul2(d, f[e]);
           dh[j] = mul2(d, m[e]);
         }
       }
@@ -907,17 +926,8 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       cols.store(dx.at(row), active, dh);
     } else copy_branch();
   }
-  if (by_image && image >= 0) image_done();
+  if (by_image && image >= 0) image_done(true);      // and a0, a1 are A and B
   // the slots' sums, in slot order, in the threads of slot 0
-  if (by_image) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      a0[i] = a1[i] = both(0.f);
-      if (none_before) continue;
-      if (cols.on(2 * i)) { const float2 v = before[cols.at(2 * i)]; a0[i].x = v.x; a1[i].x = v.y; }
-      if (cols.on(2 * i + 1)) { const float2 v = before[cols.at(2 * i + 1)]; a0[i].y = v.x; a1[i].y = v.y; }
-    }
-  }
   __syncthreads();
   float2* meet = reinterpret_cast<float2*>(shared);
   auto over_slots = [&](float2 (&v)[N]) {
@@ -1047,7 +1057,7 @@ template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int 
 void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
   static bool forward_done[64] = {false}, backward_done[64] = {false};
   if (backward) {
-    if constexpr (LARGE || K <= 2 || MODE == MODE_NORM) {         // plan() gives no others
+    {
       const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0, smem = s.smem < meet ? meet : s.smem;
       const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
       allow_shared(kernel, smem, backward_done);

@@ -22,17 +22,16 @@ def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode)
         for vec in ((True, False) if c % 8 == 0 else (False,)):
             for gate in ((0, rows, max(1, rows // 5 if rows % 5 == 0 else 1)) if mode > 1 else (0,)):
                 vectors, slot, slots, blocks, per_sm, depth, smem, large = shape(rows, c, backward, mode, gate, vec, types)
-                assert vectors * slot * 8 >= c and slot * slots <= (512 if large else 384 if backward else 256) and slots >= 1
+                threads = 512 if large else 256 if not backward else 512 if not vec else 256 if vectors > 2 and mode > 1 else 384
+                assert vectors * slot * 8 >= c and slot * slots <= threads and slots >= 1
                 assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
-                assert slot < 32 or slots <= 15                     # a named barrier for each slot of several warps
+                assert slot <= 32 or slots <= 15                    # a named barrier for each slot of several warps
                 assert 1 <= blocks <= 148 * per_sm and (blocks - 1) * slots < rows
                 assert (slot * slots) % 32 == 0                     # whole warps: their lanes meet in shuffles
-                assert depth == 0 if large else 1 <= depth <= 4
+                assert (0 if large else 1) <= depth <= 4
                 # dynamic and static shared memory of all blocks of an SM (1 KB of each is the system's)
-                fixed = 16 * 64 * 4 + (2 * 8 * (512 if large else 384) if backward else 0) + 1024
+                fixed = 16 * 64 * 4 + (2 * 8 * threads if backward else 0) + 1024
                 assert per_sm * (smem + fixed) <= 228 * 1024 and smem <= 208 * 1024
-                ring = not large
-                assert not ring or vectors <= (4 if mode == 1 or not backward else 2)
 
 
 def pack(**kw):
