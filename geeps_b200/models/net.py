@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from ..ops import functional as F
-from ..ops.layers import BF, LRN, BatchNorm, Conv2d, Layer, LRNMaxPool, Pool, SoftmaxLoss
+from ..ops.layers import BF, LRN, BatchNorm, Conv2d, Layer, LRNMaxPool, Norm, Pool, ResidualJoin, SoftmaxLoss
 
 
 _side_streams = {}
@@ -166,6 +166,101 @@ class Concat(Layer):
         return out
 
 
+class Residual(Layer):
+    """A residual block: x + scale * gate(b) * post(b) with b = layers(pre(x)), the layers keeping the shape.
+
+    pre, post: None, "layer" or "rms" (a norm in front of the layers, behind them); scale: None or the initial value of a factor
+    per channel; gate: None or layers from b to a gate for every image ([batch, channels]: Pool("avg", 0, 1), Linear(...), ...)
+    or for every pixel, through a sigmoid unless sigmoid=False.  The join is one pass, and where another Residual follows in a
+    Net, the norm in front of that one is part of it."""
+
+    def __init__(self, name, layers, pre="layer", post=None, scale=None, gate=None, sigmoid=True, eps=1e-5):
+        super().__init__()
+        self.name, self.layers, self.gate = name, list(layers), list(gate or [])
+        self.pre = Norm(name + "_pre", pre, eps) if pre else None
+        self.join = ResidualJoin(name + "_join", post, scale, sigmoid, eps)
+        self.follower = None           # the Residual whose norm the join computes
+
+    def sublayers(self):
+        for l in ([self.pre] if self.pre else []) + self.layers + self.gate + [self.join]:
+            if hasattr(l, "sublayers"):
+                yield from l.sublayers()
+            else:
+                yield l
+
+    def setup(self, in_shape, device):
+        self.in_shape = self.out_shape = s = tuple(in_shape)
+        if self.pre:
+            s = self.pre.setup(s, device)
+        for l in self.layers:
+            s = l.setup(s, device)
+        if tuple(s) != self.in_shape:
+            raise ValueError(f"{self.name}: the layers turn {self.in_shape} into {tuple(s)}; a residual block keeps the shape")
+        g, rows = s, 0
+        for l in self.gate:
+            g = l.setup(g, device)
+            if min(g) < 1:
+                raise ValueError(f"{self.name}: the gate's {type(l).__name__} leaves nothing of its input: {tuple(g)} (global pooling is of square images)")
+        if self.gate:
+            rows = 1
+            for n in g[:-1]:
+                rows *= n
+            if g[-1] != s[-1] or rows not in (s[0], self.out_numel() // s[-1]):
+                raise ValueError(f"{self.name}: the gate is {tuple(g)}; need a row of {s[-1]} channels for every image or pixel")
+        return self.join.setup(s, device, rows)
+
+    def link(self, follower: "Residual") -> None:
+        """Let the join compute the norm in front of `follower`, which comes next."""
+        if follower.pre is not None and not follower.pre.joined:
+            self.follower = follower
+            self.join.follow(follower.pre)
+
+    def bind_output(self, y2d):
+        self.join.bind_output(y2d)
+
+    def set_output(self, flat):
+        self.join.set_output(flat)
+
+    def set_input(self, x):
+        self.x = x.view(self.in_shape)
+        if self.pre is None:
+            self.layers[0].set_input(self.x)
+        elif not self.pre.joined:
+            self.pre.set_input(self.x)
+
+    def forward(self, x):
+        self.x = x if x.dim() == len(self.in_shape) else x.view(self.in_shape)
+        h = self.x
+        if self.pre:
+            h = (self.pre.y if self.pre.joined else self.pre.forward(h)).view(self.in_shape)
+        for l in self.layers:
+            h = l.forward(h)
+        g = None
+        if self.gate:
+            g = h.view(self.in_shape)
+            for l in self.gate:
+                g = l.forward(g)
+            g = g.view(-1, self.in_shape[-1])
+        return self.join.forward(h, self.x, g)
+
+    def backward(self, dy):
+        d, dres, g = self.join.backward(dy, self.follower.pre_grad if self.follower else None)
+        if self.gate:
+            for l in reversed(self.gate):
+                g = l.backward(g)
+            F.add_2d(d, g.view(d.shape))
+        for l in reversed(self.layers):
+            d = l.backward(d)
+        d = d.view(dres.shape)
+        if self.pre is None:
+            F.add_2d(dres, d)
+            return dres
+        if self.pre.joined:            # the join in front takes it together with dres
+            self.pre_grad = d
+            return dres
+        return self.pre.backward(d, dres)
+
+
 class Net:
     """input layer -> layers -> linear logits -> softmax loss."""
 
@@ -177,7 +272,7 @@ class Net:
 
     def all_layers(self):
         for l in self.layers:
-            if isinstance(l, Concat):
+            if hasattr(l, "sublayers"):
                 yield from l.sublayers()
             else:
                 yield l
@@ -205,6 +300,8 @@ class Net:
         # mask to the gradient it hands down and the convolution skips its own masking pass; a max pooling knows the mask from
         # its own maxima
         for a, b in zip(self.layers, self.layers[1:]):
+            if isinstance(a, Residual) and isinstance(b, Residual):
+                a.link(b)
             if isinstance(a, Conv2d) and a.relu and isinstance(b, (LRN, LRNMaxPool)):
                 a.dy_is_masked, b.mask_relu_input = True, True
                 if a.has_bias and b.C % 8 == 0 and b.size in (3, 5, 7):

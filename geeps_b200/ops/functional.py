@@ -669,12 +669,18 @@ class GradList:
         self.native = L.Tensors(n, *(C.addressof(a) for a in self._arrays))
 
 
-def clip_gradients(grads, max_norm: float, result: torch.Tensor, out=None) -> None:
+    def work_size(self) -> int:
+        """fp64 values that clip_gradients() takes as `work` for this list."""
+        return lib().geeps_clip_work(C.byref(self.native))
+
+
+def clip_gradients(grads, max_norm: float, result: torch.Tensor, out=None, work=None) -> None:
     """Scale all gradients by max_norm / N where their global norm N = sqrt(sum of all squares) exceeds max_norm (Caffe's
     clip_gradients), in place or into the tensors of `out`.  grads, out: GradList or a sequence of tensors (fp32 or bf16 each; out[i]
     has grads[i]'s count).  result: fp32 [2] on the device, receives N and the coefficient (1 where nothing is clipped).
     Without `out` nothing is written to the gradients where nothing is clipped; max_norm = inf only measures.  A norm that is
-    infinite gives the coefficient 0 and one that is not a number 1: the gradients then carry it on."""
+    infinite gives the coefficient 0 and one that is not a number 1: the gradients then carry it on.
+    work: GradList.work_size() fp64 values to use instead of memory taken from the allocator for the call."""
     grads = grads if isinstance(grads, GradList) else GradList(grads)
     out = out if out is None or isinstance(out, GradList) else GradList(out)
     if not max_norm >= 0:
@@ -687,7 +693,11 @@ def clip_gradients(grads, max_norm: float, result: torch.Tensor, out=None) -> No
         raise ValueError(f"clip_gradients: result is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     for t in (grads, out):
         _need(t is None or not t.tensors or t.device.index == dev, "clip_gradients: need every tensor on the current device")
-    work = L.hold(torch.empty(lib().geeps_clip_work(C.byref(grads.native)), dtype=torch.float64, device=result.device))
+    n = grads.work_size()
+    if work is None:
+        work = L.hold(torch.empty(n, dtype=torch.float64, device=result.device))
+    elif not (work.dtype is torch.float64 and work.is_contiguous() and work.numel() >= n and work.get_device() == dev):
+        raise ValueError(f"clip_gradients: work needs {n} contiguous fp64 values on cuda:{dev}")
     L.hold((grads, out))
     launch(lib().geeps_clip_gradients, "clip_gradients", C.byref(grads.native), None if out is None else C.byref(out.native),
            C.c_double(max_norm), ptr(result), ptr(work), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))

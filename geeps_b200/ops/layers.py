@@ -545,6 +545,122 @@ class BatchNorm(Layer):
         return self.dx
 
 
+class Norm(Layer):
+    """LayerNorm (kind "layer") or RMSNorm ("rms", without a bias) over the channels of every pixel."""
+
+    def __init__(self, name, kind="layer", eps=1e-5):
+        super().__init__()
+        self.name, self.kind, self.eps = name, kind, eps
+        self.joined = False            # set by Net: the join of the residual block in front computes this norm with its own pass
+
+    def setup(self, in_shape, device):
+        self.in_shape = self.out_shape = tuple(in_shape)
+        self.C = in_shape[-1]
+        self.P = 1
+        for s in in_shape[:-1]:
+            self.P *= s
+        self.y = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.dx = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.stats = torch.empty(self.P, 2, device=device)
+        self.work = torch.empty(F.norm_work(self.P, self.C), device=device)
+        return self.out_shape
+
+    def specs(self, prefix=""):
+        specs = [ParamSpec(prefix + "gamma", (self.C,), "const:1.0", decay=False)]
+        if self.kind == "layer":
+            specs.append(ParamSpec(prefix + "beta", (self.C,), "const:0.0", decay=False))
+        return specs
+
+    def param_specs(self):
+        return [] if self.joined else self.specs()
+
+    def bind_output(self, y2d):
+        self.y = y2d
+
+    def norm(self, p32, g32, prefix="", backward=False):
+        """The arguments of this norm with parameters (and their gradients) from the given views."""
+        w, b = prefix + "gamma", prefix + "beta"
+        return F.Norm(self.kind, p32[w], p32.get(b), self.stats, self.eps, *((g32[w], g32.get(b)) if backward else ()))
+
+    def forward(self, x):
+        self.x = x if x.dim() == 2 else x.view(self.P, self.C)
+        F.norm_forward(self.x, self.y, self.norm(self.p32, self.g32))
+        return self.y
+
+    def backward(self, dy, dres=None):
+        """dres: a gradient that reaches the input on another way, added to dx."""
+        dy = dy if dy.dim() == 2 else dy.view(self.P, self.C)
+        F.norm_backward(self.x, dy, self.dx, self.norm(self.p32, self.g32, backward=True), dres=dres, work=self.work)
+        return self.dx
+
+
+class ResidualJoin(Layer):
+    """The end of a residual block: out = x + scale * gate * norm(branch), with each of norm, scale and gate optional, and, once
+    `follow` has been called, the norm in front of the next block in the same pass."""
+
+    def __init__(self, name, norm=None, scale=None, sigmoid=True, eps=1e-5):
+        """norm: None, "layer" or "rms"; scale: None or the initial value of a factor per channel; sigmoid: of the gate."""
+        super().__init__()
+        self.name, self.scale, self.sigmoid = name, scale, sigmoid
+        self.post = Norm(name + "_norm", norm, eps) if norm else None
+        self.next = None
+
+    def setup(self, in_shape, device, gate_rows=0):
+        self.in_shape = self.out_shape = tuple(in_shape)
+        self.C, self.P = in_shape[-1], 1
+        for s in in_shape[:-1]:
+            self.P *= s
+        self.device, self.gate_rows = device, gate_rows
+        if self.post:
+            self.post.setup(in_shape, device)
+            self.post.y = self.post.dx = None          # the join's own pass has them
+        self.y = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.dx = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.dres = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.dgate = torch.empty(gate_rows, self.C, dtype=BF, device=device) if gate_rows else None
+        self._workspace()
+        return self.out_shape
+
+    def _workspace(self):
+        n = F.norm_work(self.P, self.C, self.gate_rows, join=True, pre=self.next is not None)
+        self.work = torch.empty(n, device=self.device)
+
+    def follow(self, norm: Norm) -> None:
+        """Compute `norm` of the output, too: its parameters become this layer's."""
+        self.next, norm.joined = norm, True
+        norm.dx = None
+        self._workspace()
+
+    def param_specs(self):
+        specs = self.post.specs() if self.post else []
+        if self.scale is not None:
+            specs.append(ParamSpec("scale", (self.C,), f"const:{self.scale}", decay=False))
+        return specs + (self.next.specs("next_") if self.next else [])
+
+    def bind_output(self, y2d):
+        self.y = y2d
+
+    def _norms(self, backward=False):
+        return (self.post.norm(self.p32, self.g32, backward=backward) if self.post else None,
+                self.next.norm(self.p32, self.g32, "next_", backward) if self.next else None)
+
+    def forward(self, branch, x, gate=None):
+        self.x, self.gate = branch.reshape(self.P, self.C), gate
+        post, pre = self._norms()
+        F.residual_forward(self.x, x.view(self.P, self.C), self.y, post=post, scale=self.p32.get("scale"), gate=gate,
+                           sigmoid=self.sigmoid, y=self.next.y if self.next else None, pre=pre)
+        return self.y
+
+    def backward(self, dout, dnext=None):
+        """dout: the gradient of out, dnext: of the norm behind it.  Returns the gradients of the branch, x and the gate."""
+        post, pre = self._norms(backward=True)
+        dout = dout if dout.dim() == 2 else dout.view(self.P, self.C)
+        F.residual_backward(self.x, dout, self.dx, self.dres, post=post, scale=self.p32.get("scale"),
+                            dscale=self.g32.get("scale"), gate=self.gate, dgate=self.dgate, sigmoid=self.sigmoid,
+                            out=self.y if pre else None, dy=dnext.view(self.P, self.C) if pre else None, pre=pre, work=self.work)
+        return self.dx, self.dres, self.dgate
+
+
 class LRN(Layer):
     def __init__(self, size=5, alpha=1e-4, beta=0.75, k=1.0):
         super().__init__()

@@ -50,7 +50,8 @@ class PSModule:
     def __init__(self, net, in_shape, ps_config: GeePsConfig, rank: int = 0, world: int = 1, device="cuda:0",
                  slack: int = 0, seed: int = 0, keep_init: bool = False, trace=None, manage_activations: bool = False,
                  cache_fraction: float | None = None, use_tape: bool = False, bf16_weights_only: bool = False,
-                 use_graph: bool = False, pull_fc: bool = False, uncached=(), resume_from: str | None = None):
+                 use_graph: bool = False, pull_fc: bool = False, uncached=(), resume_from: str | None = None,
+                 clip_gradients: float | None = None):
         """bf16_weights_only: with the NVLINK transport and the bf16 compute cache, weight rows are published to
         the workers' bf16 caches only (the layers never read weights in fp32; biases, BatchNorm scale / shift and
         the shard's master rows stay fp32).  The fp32 views of weights (`params_fp32`) then keep their initial
@@ -69,7 +70,10 @@ class PSModule:
         resume_from: directory of table snapshots (`save_snapshot`): the tables (master rows, momentum, clocks) come
         from its latest snapshot instead of the initial values, and training goes on at the snapshot's clock.  The
         world size may differ from the one that wrote it.  Layer-local state (BatchNorm running statistics) is not
-        part of a table snapshot."""
+        part of a table snapshot.
+        clip_gradients: scale the worker's gradients by clip_gradients / norm where the norm of all of them exceeds it
+        (Caffe's solver parameter; every worker clips its own batch's).  No table is then pushed before the backward pass has
+        ended.  `clip_result` holds the last step's {norm, factor}; inf only measures."""
         self.net, self.rank, self.world, self.slack = net, rank, world, slack
         self.device = torch.device(device)
         self.trace = trace or NullTrace()
@@ -158,6 +162,11 @@ class PSModule:
         self.layer_marks = None
         self.initial_params = {} if keep_init else None
         self.captured = None
+        if clip_gradients is not None and not (clip_gradients >= 0 and self.device.type == "cuda"):
+            raise ValueError(f"clip_gradients needs a bound from 0 up and a GPU, got {clip_gradients} on {self.device}")
+        self.clip_gradients = clip_gradients
+        self.clip_result = None if clip_gradients is None else torch.zeros(2, device=self.device)
+        self._clip_lists, self._clip_work = {}, None
         self._declare()
         if resume_from is not None:
             if not self.ps.load_snapshot(resume_from):
@@ -191,13 +200,39 @@ class PSModule:
                 M[i - 1]["b"] = ps.virtual_local_access(M[i - 1]["rows"], True)
             for t in reversed(tabs):
                 t.h_pre = ps.virtual_pre_update(t.table_id, range(t.rows))
-            for t in reversed(tabs):
-                t.h_post = ps.virtual_post_read(t.h_read)
-                t.h_upd = ps.virtual_update(t.h_pre)
+            if self.clip_gradients is None:
+                self._declare_updates(tabs)
             if i in M:
                 M[i]["pb"] = ps.virtual_post_local_access(M[i]["b"], False)
+        if self.clip_gradients is not None:
+            for _, tabs in reversed(self.groups):
+                self._declare_updates(tabs)
         ps.virtual_clock()
         ps.finish_virtual_iteration()
+
+    def _declare_updates(self, tabs):
+        for t in reversed(tabs):
+            t.h_post = self.ps.virtual_post_read(t.h_read)
+            t.h_upd = self.ps.virtual_update(t.h_pre)
+
+    def _update(self, name, tabs):
+        if tabs:
+            with self.trace.span(f"update:{name}", "ps"):
+                for t in reversed(tabs):
+                    self.ps.post_read(t.h_post)
+                    self.ps.update(t.h_upd)
+
+    def _clip(self):
+        """Clip the gradients where they are, in the tables' update buffers.  Their layout is kept for every set of buffers (the
+        update ring has a few), so that a recorded step finds the same arguments again."""
+        grads = [g for t in self.tables for g in t.layer.g32.values()]
+        key = tuple(g.data_ptr() for g in grads)
+        if key not in self._clip_lists:
+            self._clip_lists[key] = F.GradList(grads)
+        grads = self._clip_lists[key]
+        if self._clip_work is None:
+            self._clip_work = torch.empty(grads.work_size(), dtype=torch.float64, device=self.device)
+        F.clip_gradients(grads, self.clip_gradients, self.clip_result, work=self._clip_work)
 
     def _bootstrap(self, seed):
         # the bootstrap update carries the initial values; updates add up over workers, so only rank 0
@@ -349,14 +384,17 @@ class PSModule:
                 t.layer.g32 = t.views(self.ps.pre_update(t.h_pre))
             with tr.span(f"bwd:{name}", "bwd"):
                 g = l.backward(g)
-            if tabs:
-                with tr.span(f"update:{name}", "ps"):
-                    for t in reversed(tabs):
-                        self.ps.post_read(t.h_post)
-                        self.ps.update(t.h_upd)
+            if self.clip_gradients is None:
+                self._update(name, tabs)
             if i in M:
                 self.ps.post_local_access(M[i]["pb"])
             self._mark("b:" + name)
+        if self.clip_gradients is not None:
+            with tr.span("clip", "bwd"):
+                self._clip()
+            self._mark("clip")
+            for l, tabs in reversed(self.groups):
+                self._update(getattr(l, "name", type(l).__name__), tabs)
         if ev is not None:
             ev[-1][2].record()
         with tr.span("clock", "ps", clock=self.steps):

@@ -116,6 +116,7 @@ def main(argv=None) -> None:
     ap.add_argument("--lr-hold", type=int, default=200)
     ap.add_argument("--momentum", type=float, default=0.9)
     ap.add_argument("--weight-decay", type=float, default=5e-4)
+    ap.add_argument("--clip-gradients", type=float, default=0.0, help="bound of the gradients' norm (Caffe's clip_gradients; 0: none)")
     ap.add_argument("--slack", type=int, default=0)
     ap.add_argument("--display", type=int, default=20)
     ap.add_argument("--snapshot", type=int, default=0)
@@ -170,7 +171,8 @@ def main(argv=None) -> None:
     stream = torch.cuda.Stream(device=dev, priority=-1)
     with torch.cuda.stream(stream):
         mod = PSModule(net, (B,) + image, cfg, rank=rank, world=world, device=dev, slack=args.slack, seed=args.seed,
-                       bf16_weights_only=True, use_graph=not args.no_graph, resume_from=resume)
+                       bf16_weights_only=True, use_graph=not args.no_graph, resume_from=resume,
+                       clip_gradients=args.clip_gradients or None)
         inp = mod.net.input_layer
         inp.set_transform(args.mean, args.scale)
         policy = LrPolicy(args.lr_policy, args.base_lr, args.gamma, args.stepsize, args.stepvalue, args.power, args.max_iter)

@@ -147,3 +147,39 @@ def test_refused_clipping_calls(src, dst, code):
 def test_a_bound_that_is_no_norm_is_refused(bound):
     s, hold = tensors([(A, 10)])
     assert L.lib().geeps_clip_gradients(C.byref(s), None, C.c_double(bound), C.c_void_p(A), C.c_void_p(B), None) == 1
+
+
+def test_the_trainer_hands_the_bound_to_the_module(monkeypatch):
+    import contextlib
+
+    import torch
+
+    import geeps_b200.parallel.ps_module as pm
+    import geeps_b200.train as train
+
+    class Stop(Exception):
+        pass
+
+    seen = []
+
+    def module(*args, **kw):
+        seen.append(kw["clip_gradients"])
+        raise Stop
+    monkeypatch.setattr(pm, "PSModule", module)
+    monkeypatch.setattr(torch.cuda, "set_device", lambda d: None)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda **kw: object())
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+    for args in ([], ["--clip-gradients", "35"]):
+        with pytest.raises(Stop):
+            train.main(["--model", "inception_bn_small", "--batch", "2", "--synthetic-images", "4", "--source-size", "32"] + args)
+    assert seen == [None, 35.0]
+
+
+def test_a_bound_needs_a_gpu():
+    from geeps_b200.models.net import Net
+    from geeps_b200.ops.layers import Input, Linear
+    from geeps_b200.parallel.ps_module import PSModule
+    from geeps_b200.utils.config import GeePsConfig
+    for bound in (1.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="clip_gradients"):
+            PSModule(Net("n", Input(), [Linear("f", 8, fp32_out=True)]), (2, 8, 1, 1), GeePsConfig(tcp_base_port=31990), device="cpu", clip_gradients=bound)
