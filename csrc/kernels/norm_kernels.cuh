@@ -932,11 +932,21 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   float2* meet = reinterpret_cast<float2*>(shared);
   auto over_slots = [&](float2 (&v)[N]) {
     if (slots == 1) return;
+    int shares = slots, share = s.id;
+    if (!WIDE) {                       // slots of a warp first
+      for (int o = slot; o < 32; o <<= 1) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) meet[(s.id * N + j) * slot + s.t] = v[j];
+        for (int j = 0; j < N; ++j) { v[j].x += __shfl_xor_sync(0xffffffffu, v[j].x, o); v[j].y += __shfl_xor_sync(0xffffffffu, v[j].y, o); }
+      }
+      shares = blockDim.x >> 5; share = threadIdx.x >> 5;
+    }
+    if (WIDE || (threadIdx.x & 31) < slot) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) meet[(share * N + j) * slot + s.t] = v[j];
+    }
     __syncthreads();
     if (s.id == 0) {
-      for (int i = 1; i < slots; ++i) {
+      for (int i = 1; i < shares; ++i) {
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] = add2(v[j], meet[(i * N + j) * slot + s.t]);
       }
