@@ -14,30 +14,34 @@ enum { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 enum { MODE_NORM = 1, MODE_JOIN = 2, MODE_BOTH = 3 };     // the next norm alone, a join alone, a join and the norm behind it
 
 // ---- launch shape ----
-// VEC: rows of whole, aligned vectors.  LARGE: rows that registers and shared memory do not hold.
+// VEC: rows of whole, aligned vectors.  large: rows that registers and shared memory do not hold; wide (forward): rows that one
+// block an SM works on, so that the parameters lie there once.
 struct Shape {
   int vectors;       // vectors a thread
   int slot;          // threads a row: a power of two up to 32, or whole warps
   int slots;         // rows a block works on at a time
   int blocks, per_sm, depth;
-  bool large;
+  bool large, wide;
   size_t ring, smem;      // bytes before the ring, and of all
   int threads() const { return slot * slots; }
 };
 // Threads of a block.  Backward a block has an SM to itself, so that few blocks leave column sums behind, and as many threads as
-// their column sums leave registers for; forward several blocks of 256 share an SM.
-__host__ __device__ constexpr int block_threads(bool backward, bool vec, bool large, int vectors, int mode) {
-  return large ? 512 : !backward ? 256 : !vec ? 512 : vectors > 2 && mode != MODE_NORM ? 256 : 384;
+// their column sums leave registers for; forward several blocks of 256 share an SM, and from 4096 channels on blocks of 512
+// (us, blocks of 256 / 512, bf16: 4000 x 6144 norm 40 / 32, join and norm 94 / 62; 16250 x 1536 22.8 / 22.7, 46.5 / 48.3).
+__host__ __device__ constexpr int block_threads(bool backward, bool vec, bool large, bool wide, int vectors, int mode) {
+  return large || wide ? 512 : !backward ? 256 : !vec ? 512 : vectors > 2 && mode != MODE_NORM ? 256 : 384;
 }
 // ... and blocks an SM that registers allow forward
-__host__ __device__ constexpr int blocks_forward(bool large, int mode) { return large ? 1 : mode == MODE_NORM ? 4 : 2; }
+__host__ __device__ constexpr int blocks_forward(bool large, bool wide, int mode) {
+  return large ? 1 : (mode == MODE_NORM ? 4 : 2) / (wide ? 2 : 1);
+}
 
 // What a call keeps in shared memory: parameters of the columns (one vector a thread keeps them in registers), with a gate per
 // image its factors, and the ring.
 struct Call {
   bool backward, vec, by_pixel, by_image;
   int mode, stream, block;                 // sizes of the two types
-  int threads(const Shape& s) const { return block_threads(backward, vec, s.large, s.vectors, mode); }
+  int threads(const Shape& s) const { return block_threads(backward, vec, s.large, s.wide, s.vectors, mode); }
 };
 inline size_t fixed_bytes(const Call& c, const Shape& s) {
   const bool norm = c.mode & MODE_NORM, join = c.mode & MODE_JOIN;
@@ -58,13 +62,16 @@ inline size_t stage_bytes(const Call& c, const Shape& s) {
 // (50176 x 64 backward 12 us, 21 with four).  A join with a norm behind it has four column sums: two vectors while they do
 // (50176 x 1024 backward 110 us, four vectors by half the threads 180).
 inline Shape plan(long long rows, int C, const Call& c) {
-  Shape best;
+  Shape best = {};
   const int vec = (C + kVec - 1) / kVec, most = c.vec ? 4 : 2;
   long long least = -1;
-  for (int k = 1; k <= most + 1; ++k) {
+  const bool wide = !c.backward && c.vec && vec >= 512;
+  for (int k = wide ? 0 : 1; k <= most + 1; ++k) {          // 0: blocks of 512, the rest where these do not fit
     Shape s;
     s.large = k > most;
-    s.vectors = s.large ? 4 : k;
+    s.wide = k == 0;
+    s.vectors = s.wide || s.large ? 4 : k;
+    if (least >= 0 && best.wide) break;
     const int need = (vec + s.vectors - 1) / s.vectors, limit = c.threads(s);
     if (need > limit || ((s.large || (c.backward && c.mode == MODE_BOTH && k > 2)) && least >= 0)) continue;
     s.slot = 1;
@@ -76,7 +83,7 @@ inline Shape plan(long long rows, int C, const Call& c) {
     s.ring = fixed_bytes(c, s);
     const size_t stage = stage_bytes(c, s);
     s.depth = 0;
-    for (s.per_sm = c.backward ? 1 : blocks_forward(s.large, c.mode); s.per_sm >= 1 && s.depth < 1; --s.per_sm) {
+    for (s.per_sm = c.backward ? 1 : blocks_forward(s.large, s.wide, c.mode); s.per_sm >= 1 && s.depth < 1; --s.per_sm) {
       const size_t room = kRingBytes / s.per_sm;
       s.depth = s.ring > room ? 0 : s.ring + 4 * stage <= room ? 4 : (int)((room - s.ring) / stage);
     }
@@ -561,14 +568,14 @@ struct Walk {
   }
 };
 
-// WIDE: a slot is whole warps.  PIXEL: a gate for every row.
-template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(block_threads(false, VEC, LARGE, K, MODE), blocks_forward(LARGE, MODE))
+// WIDE: a slot is whole warps.  BIG: blocks of 512 threads.  PIXEL: a gate for every row.
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, bool BIG, int MODE, bool PIXEL>
+__global__ void __launch_bounds__(block_threads(false, VEC, LARGE, BIG, K, MODE), blocks_forward(LARGE, BIG, MODE))
 residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
   __shared__ __align__(16) float red[16][64];
-  constexpr int N = 4 * K, THREADS = block_threads(false, VEC, LARGE, K, MODE);
+  constexpr int N = 4 * K, THREADS = block_threads(false, VEC, LARGE, BIG, K, MODE);
   typedef Columns<K, VEC, LARGE, THREADS> Cols;
   for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
@@ -713,11 +720,11 @@ __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int
 }
 
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(block_threads(true, VEC, LARGE, K, MODE))
+__global__ void __launch_bounds__(block_threads(true, VEC, LARGE, false, K, MODE))
 residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
-  constexpr int N = 4 * K, THREADS = block_threads(true, VEC, LARGE, K, MODE);
+  constexpr int N = 4 * K, THREADS = block_threads(true, VEC, LARGE, false, K, MODE);
   typedef Columns<K, VEC, LARGE, THREADS> Cols;
   __shared__ float2 stats[2][THREADS];
   __shared__ __align__(16) float red[16][64];
@@ -1063,21 +1070,27 @@ void allow_shared(F kernel, size_t bytes, bool (&done)[64]) {
     done[dev] = true;
 }
 
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, bool BIG, int MODE, bool PIXEL>
+void launch_forward(const GeepsResidual& p, const Shape& s, cudaStream_t st) {
+  static bool done[64] = {false};
+  const auto kernel = residual_forward_kernel<TR, TB, K, VEC, WIDE, LARGE, BIG, MODE, PIXEL>;
+  allow_shared(kernel, s.smem, done);
+  geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), s.smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
+}
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
 void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
-  static bool forward_done[64] = {false}, backward_done[64] = {false};
-  if (backward) {
-    {
-      const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0, smem = s.smem < meet ? meet : s.smem;
-      const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
-      allow_shared(kernel, smem, backward_done);
-      geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
+  if (!backward) {
+    if constexpr (K == 4 && VEC && WIDE && !LARGE) {
+      if (s.wide) { launch_forward<TR, TB, K, VEC, WIDE, LARGE, true, MODE, PIXEL>(p, s, st); return; }
     }
-  } else {
-    const auto kernel = residual_forward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
-    allow_shared(kernel, s.smem, forward_done);
-    geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), s.smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
+    launch_forward<TR, TB, K, VEC, WIDE, LARGE, false, MODE, PIXEL>(p, s, st);
+    return;
   }
+  static bool done[64] = {false};
+  const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0, smem = s.smem < meet ? meet : s.smem;
+  const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
+  allow_shared(kernel, smem, done);
+  geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
 }
 template <typename TR, typename TB, int MODE, bool PIXEL>
 void launch(const GeepsResidual& p, const Shape& s, bool backward, bool vec, cudaStream_t st) {

@@ -22,7 +22,7 @@ def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode)
         for vec in ((True, False) if c % 8 == 0 else (False,)):
             for gate in ((0, rows, max(1, rows // 5 if rows % 5 == 0 else 1)) if mode > 1 else (0,)):
                 vectors, slot, slots, blocks, per_sm, depth, smem, large = shape(rows, c, backward, mode, gate, vec, types)
-                threads = 512 if large else 256 if not backward else 512 if not vec else 256 if vectors > 2 and mode > 1 else 384
+                threads = 512 if large or (vec and not backward and c >= 4089 and vectors == 4) else 256 if not backward else 512 if not vec else 256 if vectors > 2 and mode > 1 else 384
                 assert vectors * slot * 8 >= c and slot * slots <= threads and slots >= 1
                 assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
                 assert slot <= 32 or slots <= 15                    # a named barrier for each slot of several warps
