@@ -6,8 +6,9 @@
 // Two launches over the same ranges: the first adds the squares, in 64 bits (fp32 squares leave the range from 1.8e19 up and
 // from 1e-19 down; the sum of all keeps no rounding that shows in an fp32 norm), the second adds the blocks' sums, in block
 // order in every block, and scales.  The second goes through a block's range backwards and marks what it reads and writes as the
-// first to leave L2, where the end of every range is then still found (268M bf16 315 us without the marks, 289 with).  Up to kOneBlock values take one launch of one block,
-// which keeps them in registers.  The tensors' table travels in the launch arguments, so a call keeps nothing on the device.
+// first to leave L2, where the end of every range is then still found (268M bf16 315 us without the marks, 289 with).
+// Up to kOneBlock values take one launch of one block, which keeps them in registers.  The tensors' table travels in the launch
+// arguments, so a call keeps nothing on the device.
 #include "common.cuh"
 #include "nn_ops.h"
 

@@ -48,6 +48,12 @@ bool clash(const Use& a, const Use& b, int C) {
   return true;
 }
 
+// A parameter, its gradient or statistics: `n` floats
+struct Column { const void* p; long long n; bool out; };
+bool meet(const void* a, uintptr_t na, const void* b, uintptr_t nb) {
+  return a && b && na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 int check(const GeepsResidual& p, bool backward, int mode, bool* vec) {
   if (p.C < 1 || p.C > kMaxChannels) return GEEPS_ERR_NORM_CHANNELS;
   if (p.rows < 0 || p.rows > 1LL << 30) return (int)cudaErrorInvalidValue;
@@ -67,6 +73,18 @@ int check(const GeepsResidual& p, bool backward, int mode, bool* vec) {
     if (u[i].p && u[i].rows > 1 && (u[i].ld < (u[i].out ? p.C : 0) || u[i].ld >= 1LL << 29)) return (int)cudaErrorInvalidValue;
     *vec = *vec && vectors_ok(u[i], p.C);
     for (int j = 0; j < i; ++j) if (clash(u[i], u[j], p.C)) return GEEPS_ERR_NORM_OVERLAP;
+  }
+  if (((uintptr_t)p.post.stats | (uintptr_t)p.pre.stats | (uintptr_t)p.work) & 7) return GEEPS_ERR_NORM_ALIGN;
+  const Column v[] = {{p.post.stats, 2 * n, !backward}, {p.pre.stats, 2 * n, !backward}, {p.scale, p.C, false},
+                      {p.post.weight, p.C, false}, {p.post.bias, p.C, false}, {p.pre.weight, p.C, false}, {p.pre.bias, p.C, false},
+                      {p.dscale, p.C, true}, {p.post.dweight, p.C, true}, {p.post.dbias, p.C, true}, {p.pre.dweight, p.C, true},
+                      {p.pre.dbias, p.C, true}};
+  for (int i = 0; i < (backward ? 12 : 7); ++i) {            // the gradients last: backward only
+    for (int j = 0; j < i; ++j)
+      if ((v[i].out || v[j].out) && meet(v[i].p, 4 * v[i].n, v[j].p, 4 * v[j].n)) return GEEPS_ERR_NORM_OVERLAP;
+    for (int j = 0; j < count; ++j)
+      if ((v[i].out || u[j].out) && u[j].rows &&
+          meet(v[i].p, 4 * v[i].n, u[j].p, ((uintptr_t)(u[j].rows - 1) * u[j].ld + p.C) * u[j].size)) return GEEPS_ERR_NORM_OVERLAP;
   }
   const bool join = mode & MODE_JOIN, norm = mode & MODE_NORM;
   if (norm != (p.pre.kind != NORM_NONE) || (!join && (p.x || p.gate || p.post.kind))) return (int)cudaErrorInvalidValue;

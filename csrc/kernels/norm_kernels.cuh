@@ -9,7 +9,7 @@ namespace rownorm {
 
 constexpr int kMaxChannels = 16384;
 constexpr int kVec = 8;                 // channels a vector
-constexpr int kRingBytes = 200 * 1024;  // shared memory of an SM for rows on their way
+constexpr int kRingBytes = 200 * 1024;  // shared memory of an SM for parameters and rows on their way
 enum { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 enum { MODE_NORM = 1, MODE_JOIN = 2, MODE_BOTH = 3 };     // the next norm alone, a join alone, a join and the norm behind it
 
@@ -27,7 +27,8 @@ struct Shape {
 };
 // Threads of a block.  Backward a block has an SM to itself, so that few blocks leave column sums behind, and as many threads as
 // their column sums leave registers for; forward several blocks of 256 share an SM, and from 4096 channels on blocks of 512
-// (us, blocks of 256 / 512, bf16: 4000 x 6144 norm 40 / 32, join and norm 94 / 62; 16250 x 1536 22.8 / 22.7, 46.5 / 48.3).
+// (us, blocks of 256 / 512, 4000 x 6144: bf16 norm 40 / 32, join and norm without a gate 44 / 37, fp32 84 / 60; 16250 x 1536, bf16:
+// 22.8 / 22.7, 46.5 / 48.3).
 __host__ __device__ constexpr int block_threads(bool backward, bool vec, bool large, bool wide, int vectors, int mode) {
   return large || wide ? 512 : !backward ? 256 : !vec ? 512 : vectors > 2 && mode != MODE_NORM ? 256 : 384;
 }
@@ -97,7 +98,7 @@ inline Shape plan(long long rows, int C, const Call& c) {
   best.blocks = (int)(want < room ? want : room);
   return best;
 }
-// rows [first_row(i), first_row(i + 1)) are slot i's, of all slots of all blocks; rows are less than 2^31
+// rows [first_row(i), first_row(i + 1)) are slot i's, of all slots of all blocks; rows are at most 2^30
 __host__ __device__ inline int first_row(int rows, int slots, int i) {
   return rows / slots * i + (rows % slots < i ? rows % slots : i);
 }
@@ -176,8 +177,9 @@ __device__ __forceinline__ float ld_shared1(uint32_t a) {
 // Rows come through a ring of `depth` stages in shared memory, so that what is on its way takes no registers.  With VEC a thread
 // copies what it reads itself and nobody waits for anybody; otherwise the slot copies the 16-byte pieces that hold the row (up
 // to 15 bytes before and behind it in the same pieces come along) and meets before and after reading them.  The ring starts as
-// zeros where no copy goes, so what has no column or no operand is read from it like the rest.  LARGE rows take more threads, leave
-// no room for parameters, and are read where they lie if they do not fit the ring.  THREADS: as many as a block may have; a thread's places in the ring are then the same for every launch.
+// zeros where no copy goes, so what has no column or no operand is read from it like the rest.  LARGE rows take more threads,
+// leave no room for parameters, and are read where they lie if they do not fit the ring.  THREADS: as many as a block may have; a
+// thread's places in the ring are then the same for every launch.
 template <int K, bool VEC, bool LARGE, int THREADS>
 struct Columns {
   static constexpr int N = 4 * K;      // pairs
@@ -544,15 +546,30 @@ __device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, flo
   for (int i = 0; i < N; ++i) a[i] = fma2(n[i], m1, fma2(a[i], r, m0));
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.f, 1.f + expf(-g)); }      // 0 from exp(-g) = 2^126 on
+// A gate's factor and its slope.  A sigmoid is kept as q = min(f, 1 - f), negative where that is 1 - f: its slope q (1 - q) has
+// then all bits of q.  f (1 - f) lost those that 1 - f has not (84 steps of fp32 at a gate of 5).
+__device__ __forceinline__ float sigmoid(float g) {
+  const float e = expf(-fabsf(g));
+  return copysignf(__fdividef(e, 1.f + e), -g);
+}
+__device__ __forceinline__ float factor_of(float q) { return __float_as_int(q) < 0 ? 1.f + q : q; }
 template <int N>
-__device__ __forceinline__ void gate_factor(int through_sigmoid, float2 (&g)[N]) {
+__device__ __forceinline__ void gate_keep(int through_sigmoid, float2 (&g)[N]) {
   if (!through_sigmoid) return;
 #pragma unroll
   for (int i = 0; i < N; ++i) g[i] = make_float2(sigmoid(g[i].x), sigmoid(g[i].y));
 }
-__device__ __forceinline__ float2 gate_slope(int through_sigmoid, float2 g) {       // of the factor g by the gate
-  return through_sigmoid ? make_float2(g.x * (1.f - g.x), g.y * (1.f - g.y)) : both(1.f);
+__device__ __forceinline__ float2 gate_factor(int through_sigmoid, float2 q) {
+  return through_sigmoid ? make_float2(factor_of(q.x), factor_of(q.y)) : q;
+}
+__device__ __forceinline__ float2 gate_slope(int through_sigmoid, float2 q) {
+  return through_sigmoid ? make_float2(fmaf(-q.x, q.x, fabsf(q.x)), fmaf(-q.y, q.y, fabsf(q.y))) : both(1.f);
+}
+template <int N>
+__device__ __forceinline__ void gate_factor(int through_sigmoid, float2 (&g)[N]) {
+  gate_keep(through_sigmoid, g);
+#pragma unroll
+  for (int i = 0; i < N; ++i) g[i] = gate_factor(through_sigmoid, g[i]);
 }
 
 // The rows of a slot: a range of its own with a gate per image, else every `step`-th of all.  Slots that share a warp take the
@@ -796,6 +813,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       for (int e = 0; e < 4; ++e) {
         const int i = 4 * k + e;
         d[i] = mul2(fma2(m[e], a0[i], mul2(b[e], a1[i])), gate_slope(p.sigmoid, g[e]));
+        g[e] = gate_factor(p.sigmoid, g[e]);
         float2 sum = mul2(g[e], a0[i]), sum1 = mul2(g[e], a1[i]);
         float2 *x = before + cols.at(2 * i), *y = before + cols.at(2 * i + 1);           // [column]{A, B}
         if (!none_before) {
@@ -864,7 +882,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     float2 dh[N], z[N], g[N];
     auto load_branch = [&]() {
       if (MODE & MODE_JOIN) cols.load(x, row, active, true, from + at_x, z);
-      if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_factor(p.sigmoid, g); }
+      if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_keep(p.sigmoid, g); }
     };
     if (!cols.ring) { load_branch(); cols.load(dout, row, active, has_dout, from, dh); }
     if (MODE & MODE_NORM) {
@@ -900,7 +918,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         left = (image + 1) * per_gate - row;
         float2 f[N];
         cols.fetch(gate.at(image), true, f);
-        gate_factor(p.sigmoid, f);
+        gate_keep(p.sigmoid, f);
 #pragma unroll
         for (int k = 0; k < K; ++k) factor.put(k, reinterpret_cast<float2(&)[4]>(f[4 * k]));
       }
@@ -919,10 +937,10 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
           float2 d = dh[j];
           if (PIXEL) {
             dg[j] = mul2(mul2(d, fma2(m[e], z[j], b[e])), gate_slope(p.sigmoid, g[j]));
-            d = mul2(d, g[j]);
+            d = mul2(d, gate_factor(p.sigmoid, g[j]));
           }
           a0[j] = fma2(d, z[j], a0[j]); a1[j] = add2(a1[j], d);
-          if (by_image) d = mul2(d, f[e]);
+          if (by_image) d = mul2(d, gate_factor(p.sigmoid, f[e]));
           dh[j] = mul2(d, m[e]);
         }
       }

@@ -563,7 +563,7 @@ def _residual(label, backward, tensors, post, pre, scale, dscale, sigmoid, work)
     shape, dev, rt, bt = stream.shape, stream.get_device(), stream.dtype, block.dtype
     if len(shape) != 2:
         raise ValueError(f"{label}: need [rows, channels], got {list(shape)}")
-    if dev != torch._C._cuda_getDevice() or dev < 0:
+    if dev < 0 or dev != torch._C._cuda_getDevice():
         L.require_cuda()
         raise ValueError(f"{label}: tensors are on {stream.device}, the current device is cuda:{torch.cuda.current_device()}")
     f32 = torch.float32
@@ -572,7 +572,7 @@ def _residual(label, backward, tensors, post, pre, scale, dscale, sigmoid, work)
     rows, cols = shape
     gate_rows, gate_shape, ld, v = 0, None, [], []
     if gate is not None:
-        gate_rows = gate.shape[0]
+        gate_rows = gate.shape[0] if gate.dim() == 2 else 0
         gate_shape = (gate_rows, cols)
     for t, what, of_stream, of_gate in zip(tensors, _NAMES, _STREAM, _GATE):
         if t is None:
@@ -621,8 +621,8 @@ def residual_forward(x, res, out, *, post: Norm | None = None, scale=None, gate=
     `pre`, y = pre(out).  scale: fp32 [C]; g: gate, or its sigmoid, a row a pixel or one for each group of rows / gate rows
     neighbouring pixels (an image's).  Types: all bf16, all fp32, or res and out fp32 with bf16 x, gate and y.
     y is taken of out before it is rounded to its type."""
-    if x is None or (y is None) != (pre is None):
-        raise ValueError("residual_forward: need x, and y exactly with pre")
+    if x is None or res is None or out is None or (y is None) != (pre is None):
+        raise ValueError("residual_forward: need x, res and out, and y exactly with pre")
     _residual("residual_forward", False, (x, res, gate, out, y, None, None, None, None, None), post, pre, scale, None, sigmoid, None)
 
 
@@ -631,8 +631,9 @@ def residual_backward(x, dout, dx, dres, *, post: Norm | None = None, scale=None
     """Gradients of residual_forward() for dout (the gradient of out; None where only dy reaches it) and, with `pre`, dy: dres (of
     res), dx, and the parameters' (dscale, dgate and those of the norms, each or None).  x, out and the norms' stats are the
     forward pass's.  Parameters' gradients are overwritten and repeat bit for bit.  work: as in norm_backward()."""
-    _need(x is not None and (dy is None) == (pre is None) and (out is not None or pre is None) and (dout is not None or pre is not None),
-          "residual_backward: need x, dy and out with pre, dout without")
+    _need(x is not None and dx is not None and dres is not None and (dy is None) == (pre is None) and (out is not None or pre is None)
+          and (dout is not None or pre is not None),
+          "residual_backward: need x, dx and dres, dy and out with pre, dout without")
     _need(dgate is None or gate is not None, "residual_backward: dgate without a gate")
     _residual("residual_backward", True, (x, None, gate, out, None, dout, dy, dx, dres, dgate), post, pre, scale, dscale, sigmoid, work)
 

@@ -228,6 +228,8 @@ class PSModule:
         grads = [g for t in self.tables for g in t.layer.g32.values()]
         key = tuple(g.data_ptr() for g in grads)
         if key not in self._clip_lists:
+            if len(self._clip_lists) == 64:        # buffers that do not come back are not kept for ever
+                self._clip_lists.clear()
             self._clip_lists[key] = F.GradList(grads)
         grads = self._clip_lists[key]
         if self._clip_work is None:

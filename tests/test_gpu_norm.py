@@ -221,6 +221,29 @@ def test_join_sizes_and_images_cut_by_blocks(rows, c, images, types):
     Join(rows + c, rows, c, "layer", "rms", True, images, True, types).check()
 
 
+# Many rows a slot, so that every ring goes round, for every number of vectors a thread, slots of lanes, warps and several warps,
+# blocks of 512 and rows too wide for a ring; whole vectors and single columns
+TURNS = [(9000, 8), (9001, 24), (14000, 64), (9001, 192), (6000, 256), (9000, 576), (6001, 1024), (3000, 2048), (1500, 4096), (1300, 4104),
+         (900, 6144), (700, 8192), (450, 12288), (450, 16384), (60000, 1), (40000, 3), (9000, 33), (5000, 257), (3001, 1001), (2000, 2050), (900, 4099),
+         (500, 8195), (450, 16383)]
+
+
+@pytest.mark.parametrize("rows,c", TURNS)
+@pytest.mark.parametrize("types", list(TYPES))
+def test_norm_with_many_rows_a_slot(rows, c, types):
+    gen = torch.Generator(device=DEV).manual_seed(rows * 31 + c)
+    check_norm(gen, rows, c, ("layer", "rms")[(rows + c) % 2], types)
+
+
+@pytest.mark.parametrize("rows,c", TURNS)
+@pytest.mark.parametrize("gate", ["pixel", "image", ""])
+def test_join_with_many_rows_a_slot(rows, c, gate):
+    images = next(n for n in (7, 5, 4, 3, 1) if rows % n == 0)
+    g = {"pixel": rows, "image": images, "": 0}[gate]
+    i = (rows + c) % 3
+    Join(rows + c, rows, c, ("layer", "rms", "layer")[i], ("rms", "", "layer")[i], True, g, i != 1, ("bf16", "mixed", "fp32")[(rows // 100 + c) % 3]).check()
+
+
 def test_join_without_dout():
     Join(5, 90, 136, "rms", "layer", True, 9, False, "bf16", dout=False).check()
 
@@ -285,6 +308,14 @@ def test_a_row_that_is_not_finite_stays_alone():
 def test_gates_far_out():
     j = Join(4, 12, 64, "rms", "", False, 12, True, "fp32")
     j.gate[:, ::2], j.gate[:, 1::2] = -2e4, 2e4
+    j.check()
+
+
+@pytest.mark.parametrize("gate", [60, 12])
+@pytest.mark.parametrize("types", ["mixed", "fp32"])
+def test_slope_of_gates_that_are_nearly_open(gate, types):
+    j = Join(8, 60, 200, "layer", "rms", True, gate, True, types)
+    j.gate.copy_(torch.linspace(-24, 24, gate * 200, device=DEV).view(gate, 200))
     j.check()
 
 
@@ -408,3 +439,27 @@ def test_refusals():
         F.norm_forward(x.cpu(), y.cpu(), norm)
     wide = torch.zeros(6, 32, dtype=BF, device=DEV)         # two ranges of columns of one matrix share nothing
     F.norm_forward(wide[:, :16], wide[:, 16:], F.Norm("layer"))
+
+
+def test_refused_statistics_workspaces_and_gradients():
+    x, y = torch.zeros(6, 16, dtype=BF, device=DEV), torch.zeros(6, 16, dtype=BF, device=DEV)
+    st, v = torch.zeros(13, device=DEV), torch.zeros(40, device=DEV)
+    with pytest.raises(ValueError, match="8 bytes"):
+        F.norm_forward(x, y, F.Norm("layer", stats=st[1:].view(6, 2)))
+    good = st[:12].view(6, 2)
+    with pytest.raises(ValueError, match="overlaps"):
+        F.norm_backward(x, y, x.clone(), F.Norm("layer", None, None, good, dweight=v[:16], dbias=v[8:24]))
+    with pytest.raises(ValueError, match="overlaps"):
+        F.norm_backward(x, y, x.clone(), F.Norm("layer", v[4:20], None, good, dweight=v[:16]))
+    rows = torch.zeros(3000, 16, dtype=BF, device=DEV)
+    n = F.norm_work(3000, 16)
+    with pytest.raises(ValueError, match="8 bytes"):
+        F.norm_backward(rows, rows.clone(), rows.clone(), F.Norm("layer", stats=torch.zeros(3000, 2, device=DEV)),
+                        work=torch.zeros(n + 1, device=DEV)[1:])
+    with pytest.raises(ValueError, match="work"):
+        F.norm_backward(rows, rows.clone(), rows.clone(), F.Norm("layer", stats=torch.zeros(3000, 2, device=DEV)),
+                        work=torch.zeros(n - 1, device=DEV))
+    a, b = torch.full((48,), 3.0, device=DEV), torch.randn(6, 16, device=DEV).to(BF)      # gradients side by side in one buffer
+    F.norm_forward(b, y, F.Norm("layer", stats=good))
+    F.norm_backward(b, b, x, F.Norm("layer", stats=good, dweight=a[:16], dbias=a[16:32]))
+    assert (a[32:] == 3.0).all() and torch.isfinite(a).all() and (a[:16] != 3.0).all()

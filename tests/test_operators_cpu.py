@@ -183,3 +183,51 @@ def test_a_bound_needs_a_gpu():
     for bound in (1.0, -1.0, float("nan")):
         with pytest.raises(ValueError, match="clip_gradients"):
             PSModule(Net("n", Input(), [Linear("f", 8, fp32_out=True)]), (2, 8, 1, 1), GeePsConfig(tcp_base_port=31990), device="cpu", clip_gradients=bound)
+
+
+def test_tensors_of_the_host_are_refused():
+    import torch
+
+    from geeps_b200.ops import functional as F
+    x = torch.zeros(4, 8)
+    for call in (lambda: F.norm_forward(x, x, F.Norm("rms")), lambda: F.residual_forward(x, x, x), lambda: F.clip_gradients([x], 1.0, torch.zeros(2))):
+        with pytest.raises((ValueError, RuntimeError), match="CUDA|cpu"):
+            call()
+    with pytest.raises(ValueError, match="need x"):
+        F.residual_forward(x, None, x)
+    with pytest.raises(ValueError, match="need x"):
+        F.residual_backward(x, x, None, x)
+
+
+S = 1 << 30
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(res=A, y=B, pre=(0, 0, S + 4, 0, 0, 1e-5, 1)), -14),
+    (dict(x=A, res=B, out=D, post=(0, 0, S + 12, 0, 0, 1e-5, 2)), -14),
+    (dict(res=A, y=B, pre=(0, 0, B + 56, 0, 0, 1e-5, 1)), -12),                       # statistics in an output
+    (dict(res=A, y=B, pre=(0, 0, A + 56, 0, 0, 1e-5, 1)), -12),                       # ... in an input
+    (dict(res=A, y=B, pre=(B + 60, 0, S, 0, 0, 1e-5, 1)), -12),                       # a parameter in an output
+    (dict(res=A, y=B, pre=(S + 28, 0, S, 0, 0, 1e-5, 1)), -12),                       # ... in statistics
+    (dict(x=A, res=B, out=D, mode=3, pre=(0, 0, S, 0, 0, 1e-5, 1), post=(0, 0, S + 24, 0, 0, 1e-5, 1)), -12),
+    (dict(res=A, mode=1, pre=(A + 60, 0, S, 0, 0, 1e-5, 1)), 1),                      # two inputs may share; the output is missing
+    (dict(res=A, mode=1, pre=(S + 32, S + 32, S, 0, 0, 1e-5, 1)), 1),
+])
+def test_refused_vectors_forward(kw, code):
+    assert L.lib().geeps_residual_forward(pack(**{"rows": 4, "c": 8, **kw}), None) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(pre=(0, 0, S + 4, 0, 0, 1e-5, 1)), -14),
+    (dict(pre=(0, 0, S, 0, 0, 1e-5, 1), work=S + 4), -14),
+    (dict(pre=(0, 0, S, S + 28, 0, 1e-5, 1)), -12),
+    (dict(pre=(0, 0, S, S + 32, S + 60, 1e-5, 1)), -12),
+    (dict(pre=(S + 64, 0, S, S + 68, 0, 1e-5, 1)), -12),
+    (dict(pre=(0, 0, S, B + 60, 0, 1e-5, 1)), -12),
+    (dict(pre=(0, 0, S, A - 28, 0, 1e-5, 1)), -12),
+    (dict(pre=(0, 0, S, 0, D + 60, 1e-5, 1)), -12),
+    (dict(pre=(0, 0, S, S + 32, S + 64, 1e-5, 1), dres=0), 1),                        # side by side; the output is missing
+    (dict(pre=(0, 0, S, B + 64, A - 32, 1e-5, 1), dres=0), 1),
+])
+def test_refused_vectors_backward(kw, code):
+    assert L.lib().geeps_residual_backward(pack(**{"rows": 4, "c": 8, "out": A, "dy": B, "dres": D, **kw}), None) == code
