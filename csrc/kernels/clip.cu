@@ -408,6 +408,10 @@ extern "C" int geeps_clip_gradients(const GeepsTensors* src, const GeepsTensors*
     if (src->count[i] && (!src->ptr[i] || (dst && !dst->ptr[i]))) return (int)cudaErrorInvalidValue;
   }
   if (overlaps_itself(*src) || (dst && (overlaps_itself(*dst) || overlaps(*src, *dst)))) return GEEPS_ERR_CLIP_OVERLAP;
+  const uintptr_t r = (uintptr_t)result, w = (uintptr_t)work, we = w + geeps_clip_work(src) * sizeof(double);
+  auto meets = [&](const Range& q) { return q.from != q.to && ((q.from < r + 8 && r < q.to) || (q.from < we && w < q.to)); };
+  for (long long i = 0; i < src->n; ++i) if (meets(range(*src, i)) || (dst && meets(range(*dst, i)))) return GEEPS_ERR_CLIP_OVERLAP;
+  if (r < we && w < r + 8) return GEEPS_ERR_CLIP_OVERLAP;
   cudaStream_t st = (cudaStream_t)stream;
   long long total = 0;
   for (long long i = 0; i < src->n && total <= kOneBlock; ++i) total += src->count[i];

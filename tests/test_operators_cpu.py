@@ -231,3 +231,10 @@ def test_refused_vectors_forward(kw, code):
 ])
 def test_refused_vectors_backward(kw, code):
     assert L.lib().geeps_residual_backward(pack(**{"rows": 4, "c": 8, "out": A, "dy": B, "dres": D, **kw}), None) == code
+
+
+@pytest.mark.parametrize("result,work", [(A + 36, B), (D + 4, B), (B, A - 8), (B, D + 32), (A - 4, B), (B, B + 8 - 8), (B + 8, B)])
+def test_a_result_or_workspace_in_a_gradient_is_refused(result, work):
+    s, hold = tensors([(A, 10)])
+    d, hold2 = tensors([(D, 10)])
+    assert L.lib().geeps_clip_gradients(C.byref(s), C.byref(d), C.c_double(1.0), C.c_void_p(result), C.c_void_p(work), None) == -13
