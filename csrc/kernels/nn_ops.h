@@ -181,8 +181,9 @@ typedef struct GeepsResidual {
 long long geeps_residual_work(long long rows, long long gate_rows, int C, int mode);
 int geeps_residual_forward(const GeepsResidual* p, void* stream);
 int geeps_residual_backward(const GeepsResidual* p, void* stream);
-// launch shape (host arithmetic only), eight values: vectors a thread, threads a row, rows a block at a time, blocks, blocks an
-// SM, stages of the ring, bytes of shared memory, rows read where they lie; vec: rows of whole, aligned vectors
+// launch shape (host arithmetic only), ten values: vectors a thread, threads a row, rows a block at a time, blocks, blocks an
+// SM, stages of the ring, bytes of shared memory, rows read where they lie, tiles of a row, columns of a tile (the first five and
+// the seventh are of one tile then); vec: rows of whole, aligned vectors
 int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int backward, int vec, int stream_fp32, int block_fp32,
                      int* out);
 

@@ -3,6 +3,8 @@
 #include "common.cuh"
 #include "nn_ops.h"
 
+#include <type_traits>
+
 typedef __nv_bfloat16 bf16;
 
 namespace rownorm {
@@ -14,14 +16,15 @@ enum { NORM_NONE = 0, NORM_LAYER = 1, NORM_RMS = 2 };
 enum { MODE_NORM = 1, MODE_JOIN = 2, MODE_BOTH = 3 };     // the next norm alone, a join alone, a join and the norm behind it
 
 // ---- launch shape ----
-// VEC: rows of whole, aligned vectors.  large: rows that registers and shared memory do not hold; wide (forward): rows that one
-// block an SM works on, so that the parameters lie there once.
+// VEC: rows of whole, aligned vectors.  large (forward): rows that registers and shared memory do not hold; wide (forward): rows
+// that one block an SM works on, so that the parameters lie there once; tiles (backward): rows cut into ranges of `width` columns.
 struct Shape {
   int vectors;       // vectors a thread
   int slot;          // threads a row: a power of two up to 32, or whole warps
   int slots;         // rows a block works on at a time
   int blocks, per_sm, depth;
   bool large, wide;
+  int tiles, width;
   size_t ring, smem;      // bytes before the ring, and of all
   int threads() const { return slot * slots; }
 };
@@ -40,7 +43,7 @@ __host__ __device__ constexpr int blocks_forward(bool large, bool wide, int mode
 // What a call keeps in shared memory: parameters of the columns (one vector a thread keeps them in registers), with a gate per
 // image its factors, and the ring.
 struct Call {
-  bool backward, vec, by_pixel, by_image;
+  bool backward, vec, by_pixel, by_image, tile;
   int mode, stream, block;                 // sizes of the two types
   int threads(const Shape& s) const { return block_threads(backward, vec, s.large, s.wide, s.vectors, mode); }
 };
@@ -58,17 +61,27 @@ inline size_t stage_bytes(const Call& c, const Shape& s) {
   };
   return r * stage(c.stream) + b * stage(c.block);
 }
+// Backward, rows that no thread count holds with their column sums are cut into tiles of columns, with the row's means taken by a
+// launch of its own: it reads once more, but nothing spills (3325 x 8972 bf16, join and norm: 1765 us by one block a row; 2230 x
+// 8968: 147).
+// Rows that fit stay whole (2441 x 4096: 54 us, two tiles 85; 1220 x 8192: 89, 96), but for single columns of a join with a norm
+// behind it and no gate for every pixel, where 16 columns a thread do not fit in 128 registers (2438 x 4101 240 us, 151; 1249 x
+// 8001 169, 158).  A tile is as wide as a block has columns: narrower ones lose (8192 in eight: 184).
+constexpr int tile_columns(bool vec) { return vec ? 2 * kVec * 384 : kVec * 512; }
+constexpr bool spills(bool backward, int mode, bool by_pixel) { return backward && mode == MODE_BOTH && !by_pixel; }
 // How many vectors a thread has: more save what every thread does once a row, fewer leave no lane without work.  The costs are
 // instructions a row.  Eight threads a row at least, where there is so much: pieces of rows in a warp's access are whole lines then
 // (50176 x 64 backward 12 us, 21 with four).  A join with a norm behind it has four column sums: two vectors while they do
 // (50176 x 1024 backward 110 us, four vectors by half the threads 180).
 inline Shape plan(long long rows, int C, const Call& c) {
   Shape best = {};
-  const int vec = (C + kVec - 1) / kVec, most = c.vec ? 4 : 2;
+  best.tiles = 1;
+  best.width = C;
+  const int vec = (C + kVec - 1) / kVec, most = c.tile ? (c.vec ? 2 : 1) : c.vec ? 4 : spills(c.backward, c.mode, c.by_pixel) ? 1 : 2;
   long long least = -1;
   const bool wide = !c.backward && c.vec && vec >= 512;
-  for (int k = wide ? 0 : 1; k <= most + 1; ++k) {          // 0: blocks of 512, the rest where these do not fit
-    Shape s;
+  for (int k = wide ? 0 : c.tile ? most : 1; k <= (c.backward ? most : most + 1); ++k) {   // 0: blocks of 512, the rest where these do not fit
+    Shape s = best;
     s.large = k > most;
     s.wide = k == 0;
     s.vectors = s.wide || s.large ? 4 : k;
@@ -77,7 +90,7 @@ inline Shape plan(long long rows, int C, const Call& c) {
     if (need > limit || ((s.large || (c.backward && c.mode == MODE_BOTH && k > 2)) && least >= 0)) continue;
     s.slot = 1;
     while (s.slot < 32 && (s.slot < need || (s.slot < 8 && s.slot < vec))) s.slot <<= 1;
-    if (need > 32 || s.large) s.slot = (need + 31) / 32 * 32;
+    if (need > 32 || s.large || c.tile) s.slot = (need + 31) / 32 * 32;
     if (s.slot >= 32 && s.vectors == 1 && c.vec) continue;
     if (s.slot < 32 && s.vectors == 2 && !c.vec) continue;
     s.slots = limit / s.slot;
@@ -93,6 +106,14 @@ inline Shape plan(long long rows, int C, const Call& c) {
     s.smem = s.ring + s.depth * stage;
     const long long cost = (long long)s.slot * (100 + 45 * s.vectors + (s.slot > 32 ? 60 : 0));
     if (least < 0 || (cost < least && c.vec)) { least = cost; best = s; }       // single columns cost the same for any k
+  }
+  if (least < 0 && !c.tile) {               // backward only
+    Call t = c;
+    t.tile = true;
+    const int most_columns = tile_columns(c.vec), tiles = (C + most_columns - 1) / most_columns, width = ((C + tiles - 1) / tiles + kVec - 1) / kVec * kVec;
+    best = plan(rows, width, t);
+    best.tiles = tiles;
+    return best;
   }
   const long long room = (long long)geeps_sm_count() * best.per_sm, want = (rows + best.slots - 1) / best.slots;
   best.blocks = (int)(want < room ? want : room);
@@ -537,11 +558,14 @@ __device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
   for (int i = 0; i < N; ++i) f[i] = fma2(f[i], r, m);
 }
 // Gradient of n * w + b by its input, for a = dz * w in place: rstd * (a - mean a - n mean(a n))
-template <bool WIDE, int N>
-__device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, float inv_c, const float2 (&n)[N], float2 (&a)[N]) {
-  const float2 v = slot_sum<WIDE>(make_float2(total(a), dot(a, n)), s);
+__device__ __forceinline__ float2 norm_means(int kind, float rstd, float inv_c, float2 v) {       // of sums of a and a n
   const float scale = -inv_c * rstd;
-  const float2 m0 = both(kind == NORM_LAYER ? v.x * scale : 0.f), m1 = both(v.y * scale), r = both(rstd);
+  return make_float2(kind == NORM_LAYER ? v.x * scale : 0.f, v.y * scale);
+}
+template <bool WIDE, bool TILE, int N>
+__device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, float inv_c, float2 known, const float2 (&n)[N], float2 (&a)[N]) {
+  const float2 m = TILE ? known : norm_means(kind, rstd, inv_c, slot_sum<WIDE>(make_float2(total(a), dot(a, n)), s));
+  const float2 m0 = both(m.x), m1 = both(m.y), r = both(rstd);
 #pragma unroll
   for (int i = 0; i < N; ++i) a[i] = fma2(n[i], m1, fma2(a[i], r, m0));
 }
@@ -736,23 +760,25 @@ __device__ __forceinline__ void write_sums(const GeepsResidual& p, int mode, int
   }
 }
 
-template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
-__global__ void __launch_bounds__(block_threads(true, VEC, LARGE, false, K, MODE))
-residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
+// TILE: the operands are a range of the columns of wider rows, whose means a launch before this one has put into `means`, two pairs
+// a row.
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool TILE, int MODE, bool PIXEL>
+__global__ void __launch_bounds__(block_threads(true, VEC, false, false, K, MODE))
+residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring, const float2* means) {
   geeps_pdl_enter();
   extern __shared__ __align__(16) unsigned char shared[];
-  constexpr int N = 4 * K, THREADS = block_threads(true, VEC, LARGE, false, K, MODE);
-  typedef Columns<K, VEC, LARGE, THREADS> Cols;
-  __shared__ float2 stats[2][THREADS];
+  constexpr int N = 4 * K, THREADS = block_threads(true, VEC, false, false, K, MODE);
+  typedef Columns<K, VEC, false, THREADS> Cols;
+  __shared__ float2 stats[TILE ? 4 : 2][THREADS];      // and the means
   __shared__ __align__(16) float red[16][64];
   for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
   stats[0][threadIdx.x] = stats[1][threadIdx.x] = both(0.f);
-  const Cols cols = {s.t, slot, p.C, slots, !LARGE || depth > 0};
+  const Cols cols = {s.t, slot, p.C, slots, true};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
-  Param<Cols, K, VEC, LARGE> sw, sb, w2;              // scale * weight, scale * bias (for a gate's gradient), the next norm's weight
+  Param<Cols, K, VEC, false> sw, sb, w2;              // scale * weight, scale * bias (for a gate's gradient), the next norm's weight
   Own<K, THREADS> factor;                      // the gate of the image at hand
   float2 a0[N], a1[N], n0[N], n1[N];
 #pragma unroll
@@ -772,7 +798,6 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   const bool has_dout = p.dout != nullptr;
   int ahead = w.lo, now = 0;                   // as in the forward pass, the branch's share of a row later than the rest
   auto copy_stream = [&]() {
-    if (!cols.ring) return;
     if (!VEC) s.sync();
     const uint32_t to = base + now;
     if (ahead < w.hi) {
@@ -784,7 +809,6 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
   };
   auto copy_branch = [&]() {
-    if (!cols.ring) return;
     if (!VEC && (MODE & MODE_JOIN)) s.sync();
     const uint32_t to = base + now;
     if (ahead < w.hi) {
@@ -837,16 +861,14 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       }
     }
   };
-  if (cols.ring) {
-    for (int i = 0; i < depth; ++i) {
-      const uint32_t to = base + i * one;
-      cols.template no_copy<TR>(to, !has_dout);
-      if (MODE & MODE_NORM) { cols.template no_copy<TR>(to + at_o, false); cols.template no_copy<TB>(to + at_y, false); }
-      if (MODE & MODE_JOIN) cols.template no_copy<TB>(to + at_x, false);
-      if (PIXEL) cols.template no_copy<TB>(to + at_g, false);
-      copy_stream();
-      copy_branch();
-    }
+  for (int i = 0; i < depth; ++i) {
+    const uint32_t to = base + i * one;
+    cols.template no_copy<TR>(to, !has_dout);
+    if (MODE & MODE_NORM) { cols.template no_copy<TR>(to + at_o, false); cols.template no_copy<TB>(to + at_y, false); }
+    if (MODE & MODE_JOIN) cols.template no_copy<TB>(to + at_x, false);
+    if (PIXEL) cols.template no_copy<TB>(to + at_g, false);
+    copy_stream();
+    copy_branch();
   }
   unsigned char* area = shared;
   if (MODE & MODE_JOIN) {
@@ -859,10 +881,8 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   for (int i = 0; i < w.turns; ++i) {
     const int row = w.lo + i * w.step;
     const bool active = WIDE || row < w.hi;
-    if (cols.ring) {
-      copy_wait(depth);
-      if (!VEC) s.sync();
-    }
+    copy_wait(depth);
+    if (!VEC) s.sync();
     const uint32_t from = base + now;
     // Statistics of the rows of several turns at a time, a row a lane: a load for every turn was waited for in the turn that
     // issued it, with the loads from shared memory that share its scoreboard (50176 x 576: 36 % of the time).
@@ -873,18 +893,18 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
       if (turn < w.turns && q < w.hi) {
         if ((MODE & MODE_JOIN) && p.post.kind) stats[0][threadIdx.x] = *reinterpret_cast<const float2*>(p.post.stats + 2LL * q);
         if (MODE & MODE_NORM) stats[1][threadIdx.x] = *reinterpret_cast<const float2*>(p.pre.stats + 2LL * q);
+        if (TILE && (MODE & MODE_JOIN) && p.post.kind) stats[TILE ? 2 : 0][threadIdx.x] = means[2LL * q];
+        if (TILE && (MODE & MODE_NORM)) stats[TILE ? 3 : 0][threadIdx.x] = means[2LL * q + 1];
       }
       __syncwarp();
     }
     const int lane = (threadIdx.x & ~(chunk - 1)) + k0;
-    const float2 st1 = stats[0][lane], st2 = stats[1][lane];
-    // an output may lie where an operand does: without a ring everything of the row is read before its first output is written
+    const float2 st1 = stats[0][lane], st2 = stats[1][lane], known1 = stats[TILE ? 2 : 0][lane], known2 = stats[TILE ? 3 : 0][lane];
     float2 dh[N], z[N], g[N];
     auto load_branch = [&]() {
       if (MODE & MODE_JOIN) cols.load(x, row, active, true, from + at_x, z);
       if (PIXEL) { cols.load(gate, row, active, true, from + at_g, g); gate_keep(p.sigmoid, g); }
     };
-    if (!cols.ring) { load_branch(); cols.load(dout, row, active, has_dout, from, dh); }
     if (MODE & MODE_NORM) {
       float2 n[N], a[N];
       cols.load(h, row, active, true, from + at_o, n);
@@ -901,17 +921,17 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
           a[j] = mul2(a[j], m[e]);
         }
       }
-      norm_gradient<WIDE>(s, p.pre.kind, st2.y, inv_c, n, a);
-      if (cols.ring) cols.load(dout, row, active, has_dout, from, dh);
+      norm_gradient<WIDE, TILE>(s, p.pre.kind, st2.y, inv_c, known2, n, a);
+      cols.load(dout, row, active, has_dout, from, dh);
 #pragma unroll
       for (int j = 0; j < N; ++j) dh[j] = add2(dh[j], a[j]);
-    } else if (cols.ring) {
+    } else {
       cols.load(dout, row, active, has_dout, from, dh);
     }
     if (MODE & MODE_NORM) copy_stream();       // what it overwrites has gone into sums that are there
     cols.store(dres.at(row), active, dh);
     if (MODE & MODE_JOIN) {
-      if (cols.ring) load_branch();
+      load_branch();
       if (by_image && left == 0 && active) {
         if (image >= 0) image_done(false);
         image = row / per_gate;
@@ -945,7 +965,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         }
       }
       if (PIXEL && p.dgate) cols.store(dgate.at(row), active, dg);
-      if (p.post.kind) norm_gradient<WIDE>(s, p.post.kind, st1.y, inv_c, z, dh);
+      if (p.post.kind) norm_gradient<WIDE, TILE>(s, p.post.kind, st1.y, inv_c, known1, z, dh);
       if (!(MODE & MODE_NORM)) copy_stream();
       copy_branch();
       cols.store(dx.at(row), active, dh);
@@ -992,6 +1012,113 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     if (MODE & MODE_NORM) { v[k++] = of(n0); v[k++] = of(n1); }
     if (gridDim.x == 1) write_sums(p, MODE, c, v);
     else for (int i = 0; i < sums_of(MODE); ++i) p.work[((long long)blockIdx.x * sums_of(MODE) + i) * p.C + c] = v[i];
+  }
+}
+
+template <int W>
+__device__ __forceinline__ void four(float4 v, float (&f)[W], int e) {
+  if (W >= 4) { f[e] = v.x; f[(e + 1) % W] = v.y; f[(e + 2) % W] = v.z; f[(e + 3) % W] = v.w; }
+}
+// W columns of a row from where they lie
+template <int W, typename T>
+__device__ __forceinline__ void columns(const T* p, float (&f)[W]) {
+  if (W == 1) {
+    f[0] = (float)*p;
+  } else if (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < W; e += 4) four(ld_f4((const float*)p + e), f, e);
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < W; ++e) f[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+  }
+}
+// The means of rows that are worked on in tiles: for each norm {-rstd mean a, -rstd mean (a n)}, what norm_gradient() adds.  A block
+// reads a row twice, the second time from L2: the join's sums are of the gradient that the next norm's means are part of.
+constexpr int kMeansThreads = 256;
+template <typename TR, typename TB, bool VEC, int MODE, bool PIXEL>
+__global__ void __launch_bounds__(kMeansThreads, 4)
+residual_means_kernel(const __grid_constant__ GeepsResidual p, float2* means) {
+  geeps_pdl_enter();
+  constexpr int W = VEC ? kVec : 1, WARPS = kMeansThreads / 32;
+  __shared__ float2 sh[2][WARPS];
+  const float inv_c = 1.f / (float)p.C;
+  const int rows = (int)p.rows, per_gate = p.gate ? (int)(p.rows / p.gate_rows) : 1;
+  int turn = 0;
+  auto block_sum = [&](float2 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) { v.x += __shfl_xor_sync(0xffffffffu, v.x, o); v.y += __shfl_xor_sync(0xffffffffu, v.y, o); }
+    if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) { v.x += sh[turn][w].x; v.y += sh[turn][w].y; }
+    turn ^= 1;
+    return v;
+  };
+  const bool wide = (((uintptr_t)p.pre.weight | (uintptr_t)p.post.weight | (uintptr_t)p.scale) & 15) == 0;
+  auto param = [&](const float* from, int c, float (&v)[W]) {
+    if (!from) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = 1.f;
+    } else if (VEC && wide) {
+#pragma unroll
+      for (int e = 0; e < W; e += 4) four(ld_f4(from + c + e), v, e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; ++e) v[e] = from[c + e];
+    }
+  };
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const TR *h = (const TR*)p.out + row * p.ldout, *dout = (const TR*)p.dout + row * p.lddout;
+    const TB *dy = (const TB*)p.dy + row * p.lddy, *x = (const TB*)p.x + row * p.ldx, *gate = (const TB*)p.gate + row / per_gate * p.ldgate;
+    float2 st1 = both(0.f), st2 = both(0.f), known = both(0.f);
+    if ((MODE & MODE_JOIN) && p.post.kind) st1 = *reinterpret_cast<const float2*>(p.post.stats + 2LL * row);
+    if (MODE & MODE_NORM) {
+      st2 = *reinterpret_cast<const float2*>(p.pre.stats + 2LL * row);
+      float2 v = both(0.f);
+#pragma unroll 2
+      for (int c = threadIdx.x * W; c < p.C; c += kMeansThreads * W) {
+        float n[W], a[W], w[W];
+        columns<W>(h + c, n); columns<W>(dy + c, a); param(p.pre.weight, c, w);
+#pragma unroll
+        for (int e = 0; e < W; ++e) { a[e] *= w[e]; v.x += a[e]; v.y = fmaf(a[e], (n[e] - st2.x) * st2.y, v.y); }
+      }
+      known = norm_means(p.pre.kind, st2.y, inv_c, block_sum(v));
+      if (threadIdx.x == 0) means[2LL * row + 1] = known;
+    }
+    if ((MODE & MODE_JOIN) && p.post.kind) {
+      float2 v = both(0.f);
+#pragma unroll 2
+      for (int c = threadIdx.x * W; c < p.C; c += kMeansThreads * W) {
+        float d[W], z[W], w[W], f[W];
+        columns<W>(x + c, z);
+        if (p.dout) columns<W>(dout + c, d);
+        else {
+#pragma unroll
+          for (int e = 0; e < W; ++e) d[e] = 0.f;
+        }
+        if (MODE & MODE_NORM) {
+          float n[W], a[W];
+          columns<W>(h + c, n); columns<W>(dy + c, a); param(p.pre.weight, c, w);
+#pragma unroll
+          for (int e = 0; e < W; ++e) d[e] += fmaf((n[e] - st2.x) * st2.y, known.y, fmaf(a[e] * w[e], st2.y, known.x));
+        }
+        param(p.post.weight, c, w); param(p.scale, c, f);
+#pragma unroll
+        for (int e = 0; e < W; ++e) d[e] *= w[e] * f[e];
+        if (p.gate) {
+          columns<W>(gate + c, f);
+#pragma unroll
+          for (int e = 0; e < W; ++e) d[e] *= p.sigmoid ? factor_of(sigmoid(f[e])) : f[e];
+        }
+#pragma unroll
+        for (int e = 0; e < W; ++e) { v.x += d[e]; v.y = fmaf(d[e], (z[e] - st1.x) * st1.y, v.y); }
+      }
+      v = block_sum(v);
+      if (threadIdx.x == 0) means[2LL * row] = norm_means(p.post.kind, st1.y, inv_c, v);
+    }
   }
 }
 
@@ -1095,55 +1222,53 @@ void launch_forward(const GeepsResidual& p, const Shape& s, cudaStream_t st) {
   allow_shared(kernel, s.smem, done);
   geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), s.smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
 }
-template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, int MODE, bool PIXEL>
-void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
-  if (!backward) {
-    if constexpr (K == 4 && VEC && WIDE && !LARGE) {
-      if (s.wide) { launch_forward<TR, TB, K, VEC, WIDE, LARGE, true, MODE, PIXEL>(p, s, st); return; }
-    }
-    launch_forward<TR, TB, K, VEC, WIDE, LARGE, false, MODE, PIXEL>(p, s, st);
-    return;
-  }
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool TILE, int MODE, bool PIXEL>
+void launch_backward(const GeepsResidual& p, const Shape& s, const float2* means, cudaStream_t st) {
   static bool done[64] = {false};
   const size_t meet = s.slots > 1 ? (size_t)s.threads() * 8 * K * sizeof(float) : 0, smem = s.smem < meet ? meet : s.smem;
-  const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, LARGE, MODE, PIXEL>;
+  const auto kernel = residual_backward_kernel<TR, TB, K, VEC, WIDE, TILE, MODE, PIXEL>;
   allow_shared(kernel, smem, done);
-  geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth, (int)s.ring);
+  geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth, (int)s.ring, means);
+}
+template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
+void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
+  if (backward) {
+    if constexpr (VEC || K == 1 || !spills(true, MODE, PIXEL)) launch_backward<TR, TB, K, VEC, WIDE, false, MODE, PIXEL>(p, s, nullptr, st);
+    return;
+  }
+  if constexpr (K == 4 && VEC && WIDE) {
+    if (s.wide) { launch_forward<TR, TB, K, VEC, WIDE, false, true, MODE, PIXEL>(p, s, st); return; }
+  }
+  launch_forward<TR, TB, K, VEC, WIDE, false, false, MODE, PIXEL>(p, s, st);
 }
 template <typename TR, typename TB, int MODE, bool PIXEL>
 void launch(const GeepsResidual& p, const Shape& s, bool backward, bool vec, cudaStream_t st) {
   const bool wide = s.slot >= 32;
   if (!vec) {
-    if (s.large) launch_kernel<TR, TB, 4, false, true, true, MODE, PIXEL>(p, s, backward, st);
-    else if (s.vectors == 2) launch_kernel<TR, TB, 2, false, true, false, MODE, PIXEL>(p, s, backward, st);
-    else if (wide) launch_kernel<TR, TB, 1, false, true, false, MODE, PIXEL>(p, s, backward, st);
-    else launch_kernel<TR, TB, 1, false, false, false, MODE, PIXEL>(p, s, backward, st);
+    if (s.large) launch_forward<TR, TB, 4, false, true, true, false, MODE, PIXEL>(p, s, st);
+    else if (s.vectors == 2) launch_kernel<TR, TB, 2, false, true, MODE, PIXEL>(p, s, backward, st);
+    else if (wide) launch_kernel<TR, TB, 1, false, true, MODE, PIXEL>(p, s, backward, st);
+    else launch_kernel<TR, TB, 1, false, false, MODE, PIXEL>(p, s, backward, st);
     return;
   }
-  if (s.large) launch_kernel<TR, TB, 4, true, true, true, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 1) launch_kernel<TR, TB, 1, true, false, false, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 2 && wide) launch_kernel<TR, TB, 2, true, true, false, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 2) launch_kernel<TR, TB, 2, true, false, false, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 3 && wide) launch_kernel<TR, TB, 3, true, true, false, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 3) launch_kernel<TR, TB, 3, true, false, false, MODE, PIXEL>(p, s, backward, st);
-  else if (wide) launch_kernel<TR, TB, 4, true, true, false, MODE, PIXEL>(p, s, backward, st);
-  else launch_kernel<TR, TB, 4, true, false, false, MODE, PIXEL>(p, s, backward, st);
+  if (s.large) launch_forward<TR, TB, 4, true, true, true, false, MODE, PIXEL>(p, s, st);
+  else if (s.vectors == 1) launch_kernel<TR, TB, 1, true, false, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 2 && wide) launch_kernel<TR, TB, 2, true, true, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 2) launch_kernel<TR, TB, 2, true, false, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 3 && wide) launch_kernel<TR, TB, 3, true, true, MODE, PIXEL>(p, s, backward, st);
+  else if (s.vectors == 3) launch_kernel<TR, TB, 3, true, false, MODE, PIXEL>(p, s, backward, st);
+  else if (wide) launch_kernel<TR, TB, 4, true, true, MODE, PIXEL>(p, s, backward, st);
+  else launch_kernel<TR, TB, 4, true, false, MODE, PIXEL>(p, s, backward, st);
 }
 inline Call call_of(const GeepsResidual& p, bool backward, bool vec) {
   const bool by_pixel = p.gate && p.gate_rows == p.rows;
-  return {backward, vec, by_pixel, p.gate && !by_pixel, p.mode, p.stream_fp32 ? 4 : 2, p.block_fp32 ? 4 : 2};
+  return {backward, vec, by_pixel, p.gate && !by_pixel, false, p.mode, p.stream_fp32 ? 4 : 2, p.block_fp32 ? 4 : 2};
 }
-template <typename TR, typename TB>
-void run(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) {
-  const Call c = call_of(p, backward, vec);
-  const Shape s = plan(p.rows, p.C, c);
-  if (p.mode == MODE_NORM) launch<TR, TB, MODE_NORM, false>(p, s, backward, vec, st);
-  else if (p.mode == MODE_JOIN && c.by_pixel) launch<TR, TB, MODE_JOIN, true>(p, s, backward, vec, st);
-  else if (p.mode == MODE_JOIN) launch<TR, TB, MODE_JOIN, false>(p, s, backward, vec, st);
-  else if (c.by_pixel) launch<TR, TB, MODE_BOTH, true>(p, s, backward, vec, st);
-  else launch<TR, TB, MODE_BOTH, false>(p, s, backward, vec, st);
+// The second launch of a backward pass, where blocks or slots share sums
+template <typename TB>
+void join_sums(const GeepsResidual& p, const Shape& s, cudaStream_t st) {
   const bool cuts = p.gate && p.gate_rows < p.rows && p.dgate;
-  if (!backward || (s.blocks == 1 && !(cuts && s.slots > 1))) return;
+  if (s.blocks == 1 && !(cuts && s.slots > 1)) return;
   int y = 4, parts = 1;
   if (cuts) {
     const long long all = (long long)s.blocks * s.slots, per_image = all / p.gate_rows + 2;      // slots that an image may meet
@@ -1152,6 +1277,52 @@ void run(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) {
     y += (int)((items + 32 / parts - 1) / (32 / parts));
   }
   geeps_launch(residual_sums_kernel<TB>, dim3((p.C + 31) / 32, y), dim3(kSumsThreads), 0, st, p, p.mode, s.blocks, s.slots, parts);
+}
+// columns [c, c + width) of the operands
+template <typename TR, typename TB>
+GeepsResidual columns_of(const GeepsResidual& p, int c, int width) {
+  GeepsResidual q = p;
+  auto move = [&](auto& at, size_t size) { if (at) at = (std::remove_reference_t<decltype(at)>)((uintptr_t)at + c * size); };
+  move(q.x, sizeof(TB)); move(q.gate, sizeof(TB)); move(q.dy, sizeof(TB)); move(q.dx, sizeof(TB)); move(q.dgate, sizeof(TB));
+  move(q.out, sizeof(TR)); move(q.dout, sizeof(TR)); move(q.dres, sizeof(TR));
+  move(q.scale, 4); move(q.dscale, 4);
+  for (GeepsNorm* n : {&q.post, &q.pre}) { move(n->weight, 4); move(n->bias, 4); move(n->dweight, 4); move(n->dbias, 4); }
+  q.C = p.C - c < width ? p.C - c : width;
+  return q;
+}
+template <typename TR, typename TB, int MODE, bool PIXEL>
+void run_tiles(const GeepsResidual& p, const Shape& s, Call c, cudaStream_t st) {
+  float2* means = reinterpret_cast<float2*>(p.work);
+  const int room = geeps_sm_count() * 4, grid = p.rows < room ? (int)p.rows : room;
+  if ((MODE & MODE_NORM) || p.post.kind) {
+    if (c.vec) geeps_launch(residual_means_kernel<TR, TB, true, MODE, PIXEL>, dim3(grid), dim3(kMeansThreads), 0, st, p, means);
+    else geeps_launch(residual_means_kernel<TR, TB, false, MODE, PIXEL>, dim3(grid), dim3(kMeansThreads), 0, st, p, means);
+  }
+  c.tile = true;
+  for (int i = 0; i < s.tiles; ++i) {
+    GeepsResidual q = columns_of<TR, TB>(p, i * s.width, s.width);
+    q.work = p.work + 4 * p.rows;
+    const Shape t = plan(p.rows, q.C, c);
+    if (c.vec) launch_backward<TR, TB, 2, true, true, true, MODE, PIXEL>(q, t, means, st);
+    else launch_backward<TR, TB, 1, false, true, true, MODE, PIXEL>(q, t, means, st);
+    join_sums<TB>(q, t, st);
+  }
+}
+template <typename TR, typename TB, int MODE, bool PIXEL>
+void run_mode(const GeepsResidual& p, const Call& c, cudaStream_t st) {
+  const Shape s = plan(p.rows, p.C, c);
+  if (s.tiles > 1) { run_tiles<TR, TB, MODE, PIXEL>(p, s, c, st); return; }
+  launch<TR, TB, MODE, PIXEL>(p, s, c.backward, c.vec, st);
+  if (c.backward) join_sums<TB>(p, s, st);
+}
+template <typename TR, typename TB>
+void run(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) {
+  const Call c = call_of(p, backward, vec);
+  if (p.mode == MODE_NORM) run_mode<TR, TB, MODE_NORM, false>(p, c, st);
+  else if (p.mode == MODE_JOIN && c.by_pixel) run_mode<TR, TB, MODE_JOIN, true>(p, c, st);
+  else if (p.mode == MODE_JOIN) run_mode<TR, TB, MODE_JOIN, false>(p, c, st);
+  else if (c.by_pixel) run_mode<TR, TB, MODE_BOTH, true>(p, c, st);
+  else run_mode<TR, TB, MODE_BOTH, false>(p, c, st);
 }
 
 void run_bf16(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);

@@ -7,12 +7,12 @@ from geeps_b200.ops import _lib as L
 
 
 def shape(rows, c, backward=True, mode=3, gate_rows=0, vec=True, types=(0, 0)):
-    out = (C.c_int * 8)()
+    out = (C.c_int * 10)()
     assert L.lib().geeps_norm_shape(C.c_longlong(rows), C.c_longlong(gate_rows), c, mode, int(backward), int(vec), *types, out) == 0
     return list(out)
 
 
-@pytest.mark.parametrize("c", [1, 7, 8, 9, 64, 72, 96, 136, 255, 256, 257, 576, 1000, 1024, 2048, 4095, 4096, 4097, 6144, 6152, 8192, 8193, 12296, 16383,
+@pytest.mark.parametrize("c", [1, 7, 8, 9, 64, 72, 96, 136, 255, 256, 257, 576, 1000, 1024, 2048, 4095, 4096, 4097, 6144, 6152, 8192, 8193, 12280, 12288, 12296, 16383,
                                16384])
 @pytest.mark.parametrize("rows", [1, 5, 300, 50176, 10_000_000])
 @pytest.mark.parametrize("backward", [False, True])
@@ -21,16 +21,17 @@ def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode)
     for types in ((0, 0), (1, 0), (1, 1)):
         for vec in ((True, False) if c % 8 == 0 else (False,)):
             for gate in ((0, rows, max(1, rows // 5 if rows % 5 == 0 else 1)) if mode > 1 else (0,)):
-                vectors, slot, slots, blocks, per_sm, depth, smem, large = shape(rows, c, backward, mode, gate, vec, types)
+                vectors, slot, slots, blocks, per_sm, depth, smem, large, tiles, width = shape(rows, c, backward, mode, gate, vec, types)
                 threads = 512 if large or (vec and not backward and c >= 4089 and vectors == 4) else 256 if not backward else 512 if not vec else 256 if vectors > 2 and mode > 1 else 384
-                assert vectors * slot * 8 >= c and slot * slots <= threads and slots >= 1
+                assert (tiles - 1) * width < c <= tiles * width and (tiles == 1 or (backward and width % 8 == 0))
+                assert vectors * slot * 8 >= width and slot * slots <= threads and slots >= 1
                 assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
                 assert slot <= 32 or slots <= 15                    # a named barrier for each slot of several warps
                 assert 1 <= blocks <= 148 * per_sm and (blocks - 1) * slots < rows
                 assert (slot * slots) % 32 == 0                     # whole warps: their lanes meet in shuffles
                 assert (0 if large else 1) <= depth <= 4
                 # dynamic and static shared memory of all blocks of an SM (1 KB of each is the system's)
-                fixed = 16 * 64 * 4 + (2 * 8 * threads if backward else 0) + 1024
+                fixed = 16 * 64 * 4 + ((4 if tiles > 1 else 2) * 8 * threads if backward else 0) + 1024
                 assert per_sm * (smem + fixed) <= 228 * 1024 and smem <= 208 * 1024
 
 
@@ -238,3 +239,16 @@ def test_a_result_or_workspace_in_a_gradient_is_refused(result, work):
     s, hold = tensors([(A, 10)])
     d, hold2 = tensors([(D, 10)])
     assert L.lib().geeps_clip_gradients(C.byref(s), C.byref(d), C.c_double(1.0), C.c_void_p(result), C.c_void_p(work), None) == -13
+
+
+@pytest.mark.parametrize("rows,gate,c,mode", [(3325, 0, 8972, 3), (7, 1, 16384, 3), (1, 0, 16384, 1), (450, 50, 12288, 2), (5000, 5000, 16383, 3), (40, 8, 9001, 2)])
+def test_workspaces_of_rows_in_tiles(rows, gate, c, mode):
+    """Four values a row, and the sums of a tile at a time."""
+    for types in ((0, 0), (1, 0), (1, 1)):
+        for vec in (True, False):
+            *_, slots, blocks, _, _, _, _, tiles, width = shape(rows, c, True, mode, gate, vec, types)
+            if tiles == 1:
+                continue
+            by_image = 0 < gate < rows
+            need = (blocks * (4 if mode == 3 else 2) if blocks > 1 or by_image else 0) + (3 * blocks * slots + gate if by_image else 0)
+            assert L.lib().geeps_residual_work(C.c_longlong(rows), C.c_longlong(gate), c, mode) >= 4 * rows + need * width
