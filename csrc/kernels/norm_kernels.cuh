@@ -735,6 +735,9 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
 // gate per image {A, B} of every slot's images, [slot][C][2], and a row of the gate's gradient for each (slot, image) pair that
 // shares rows, number slot + image.
 __host__ __device__ inline int sums_of(int mode) { return mode == MODE_BOTH ? 4 : 2; }
+// How many slots have one share of an image that they alone have rows of: those of a warp, where every slot has rows (125552 x 32 as
+// one image 91 us with a share a slot, 39 with one a warp; 160000 x 8 as four 91, 22)
+__host__ __device__ __forceinline__ int merged_slots(long long rows, long long all, int slot) { return slot < 32 && rows >= all ? 32 / slot : 1; }
 inline long long work_floats(const Shape& s, int C, int mode, long long images) {
   return ((long long)s.blocks * sums_of(mode) + (images ? 3LL * s.blocks * s.slots + images : 0)) * C;
 }
@@ -826,7 +829,11 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
   // a gate per image a0 and a1 are the sums u and v of the image at hand; A and B of the images before it are in the workspace,
   // every thread its own columns.
   float2* before = by_image ? reinterpret_cast<float2*>(sums_of_images(p, MODE, blockIdx.x * slots + s.id)) : nullptr;
-  bool none_before = true;
+  bool none_before = true, merge = false;
+  if (!WIDE && by_image) {
+    const int a = blockIdx.x * slots + s.id & -(32 / slot), all = gridDim.x * slots;
+    merge = merged_slots(p.rows, all, slot) > 1 && first_row((int)p.rows, all, a) / per_gate == (first_row((int)p.rows, all, a + 32 / slot) - 1) / per_gate;
+  }
   auto image_done = [&](bool end) {
     float2 d[N];
 #pragma unroll
@@ -851,6 +858,13 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
     }
     none_before = false;
     if (!p.dgate) return;
+    if (end && merge) {                        // the slots of this warp had rows of this image alone, in the end: one share
+      for (int o = slot; o < 32; o <<= 1) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) { d[i].x += __shfl_xor_sync(0xffffffffu, d[i].x, o); d[i].y += __shfl_xor_sync(0xffffffffu, d[i].y, o); }
+      }
+      if ((threadIdx.x & 31) >= slot) return;
+    }
     if (image * per_gate >= w.lo && (image + 1) * per_gate <= w.hi) cols.store(dgate.at(image), true, d);
     else {
       float* to = image_share(p, MODE, gridDim.x, (long long)gridDim.x * slots, blockIdx.x * slots + s.id, image);
@@ -1132,9 +1146,9 @@ __device__ __forceinline__ int slot_of(int rows, int slots, int i) {
 // 32nd block's sums a share; then 32 / `parts` images, or, where there are more images than slots, slots that begin inside of
 // one and are its first cut.
 constexpr int kSumsThreads = 256;
-template <typename TB>
+template <typename TB, bool MERGED>
 __global__ void __launch_bounds__(kSumsThreads)
-residual_sums_kernel(const __grid_constant__ GeepsResidual p, int mode, int blocks, int slots, int parts) {
+residual_sums_kernel(const __grid_constant__ GeepsResidual p, int mode, int blocks, int slots, int parts, int merged) {
   geeps_pdl_enter();
   __shared__ float sh[32][4][8];
   const int lane = threadIdx.x & 7, share = threadIdx.x >> 3, sums = sums_of(mode);
@@ -1183,14 +1197,28 @@ residual_sums_kernel(const __grid_constant__ GeepsResidual p, int mode, int bloc
     }
   }
   if (end - first < 2) end = first;                   // one slot had it all
+  auto add = [&](int q, int until, int step) {
 #pragma unroll 4
-  for (int q = first + part; q < end; q += parts) {
-    const float* w = image_share(p, mode, blocks, all, q, image);
+    for (q += part * step; q < until; q += parts * step) {
+      const float* w = image_share(p, mode, blocks, all, q, image);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int c = blockIdx.x * 32 + u * 8 + lane;
-      if (c < p.C) v[u] += w[c];
+      for (int u = 0; u < 4; ++u) {
+        const int c = blockIdx.x * 32 + u * 8 + lane;
+        if (c < p.C) v[u] += w[c];
+      }
     }
+  };
+  if (!MERGED) {
+    add(first, end, 1);
+  } else if (end > first) {                  // warps [from, to) have the image alone: one share of each, before and behind them one a slot
+    int from = (first + merged - 1) / merged, to = end / merged;
+    if (from * merged < all && first_row(rows, all, from * merged) < image * per_gate) ++from;
+    if (first_row(rows, all, to * merged) > (image + 1) * per_gate) --to;
+    if (to < from) from = to = (end + merged - 1) / merged;
+    const int head = min(from * merged, end);
+    add(first, head, 1);
+    add(from * merged, to * merged, merged);
+    add(max(to * merged, head), end, 1);
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u) sh[share][u][lane] = v[u];
@@ -1269,14 +1297,17 @@ template <typename TB>
 void join_sums(const GeepsResidual& p, const Shape& s, cudaStream_t st) {
   const bool cuts = p.gate && p.gate_rows < p.rows && p.dgate;
   if (s.blocks == 1 && !(cuts && s.slots > 1)) return;
-  int y = 4, parts = 1;
+  int y = 4, parts = 1, merged = 1;
   if (cuts) {
-    const long long all = (long long)s.blocks * s.slots, per_image = all / p.gate_rows + 2;      // slots that an image may meet
+    merged = merged_slots(p.rows, (long long)s.blocks * s.slots, s.slot);
+    // shares that an image may have
+    const long long all = (long long)s.blocks * s.slots, per_image = all / merged / p.gate_rows + 2 * merged;
     while (parts < 32 && parts < per_image) parts <<= 1;
     const long long items = p.gate_rows <= all ? p.gate_rows : all - 1;
     y += (int)((items + 32 / parts - 1) / (32 / parts));
   }
-  geeps_launch(residual_sums_kernel<TB>, dim3((p.C + 31) / 32, y), dim3(kSumsThreads), 0, st, p, p.mode, s.blocks, s.slots, parts);
+  geeps_launch(merged > 1 ? residual_sums_kernel<TB, true> : residual_sums_kernel<TB, false>, dim3((p.C + 31) / 32, y), dim3(kSumsThreads), 0, st,
+               p, p.mode, s.blocks, s.slots, parts, merged);
 }
 // columns [c, c + width) of the operands
 template <typename TR, typename TB>

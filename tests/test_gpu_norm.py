@@ -244,6 +244,14 @@ def test_join_with_many_rows_a_slot(rows, c, gate):
     Join(rows + c, rows, c, ("layer", "rms", "layer")[i], ("rms", "", "layer")[i], True, g, i != 1, ("bf16", "mixed", "fp32")[(rows // 100 + c) % 3]).check()
 
 
+@pytest.mark.parametrize("images,pixels,c", [(1, 60000, 8), (1, 50001, 24), (2, 20000, 32), (3, 11111, 64), (7, 4000, 5), (1, 9000, 130), (5, 700, 16),
+                                             (900, 40, 8), (2, 37, 16), (11, 333, 100)])
+@pytest.mark.parametrize("types", ["bf16", "fp32"])
+def test_join_with_images_of_many_slots(images, pixels, c, types):
+    Join(images + c, images * pixels, c, "layer", "rms", True, images, True, types).check()
+    Join(images + c, images * pixels, c, "", "", False, images, False, types).check()
+
+
 def test_join_without_dout():
     Join(5, 90, 136, "rms", "layer", True, 9, False, "bf16", dout=False).check()
 
