@@ -31,7 +31,7 @@ struct Shape {
 // Threads of a block.  Backward a block has an SM to itself, so that few blocks leave column sums behind, and as many threads as
 // their column sums leave registers for; forward several blocks of 256 share an SM, and from 4096 channels on blocks of 512
 // (us, blocks of 256 / 512, 4000 x 6144: bf16 norm 40 / 32, join and norm without a gate 44 / 37, fp32 84 / 60; 16250 x 1536, bf16:
-// 22.8 / 22.7, 46.5 / 48.3).
+// 22.8 / 22.7, 46.5 / 48.3; single columns, 3332 x 6001 join 376 / 70).
 __host__ __device__ constexpr int block_threads(bool backward, bool vec, bool large, bool wide, int vectors, int mode) {
   return large || wide ? 512 : !backward ? 256 : !vec ? 512 : vectors > 2 && mode != MODE_NORM ? 256 : 384;
 }
@@ -79,7 +79,7 @@ inline Shape plan(long long rows, int C, const Call& c) {
   best.width = C;
   const int vec = (C + kVec - 1) / kVec, most = c.tile ? (c.vec ? 2 : 1) : c.vec ? 4 : spills(c.backward, c.mode, c.by_pixel) ? 1 : 2;
   long long least = -1;
-  const bool wide = !c.backward && c.vec && vec >= 512;
+  const bool wide = !c.backward && vec >= (c.vec ? 512 : 513);
   for (int k = wide ? 0 : c.tile ? most : 1; k <= (c.backward ? most : most + 1); ++k) {   // 0: blocks of 512, the rest where these do not fit
     Shape s = best;
     s.large = k > most;
@@ -97,12 +97,14 @@ inline Shape plan(long long rows, int C, const Call& c) {
     s.ring = fixed_bytes(c, s);
     const size_t stage = stage_bytes(c, s);
     s.depth = 0;
+    // a row of single columns by a block of 512 is read where it lies if its parameters leave no room for it (2493 x 8021, join and
+    // norm 160 us, 455 with the parameters read again for every row)
     for (s.per_sm = c.backward ? 1 : blocks_forward(s.large, s.wide, c.mode); s.per_sm >= 1 && s.depth < 1; --s.per_sm) {
       const size_t room = kRingBytes / s.per_sm;
       s.depth = s.ring > room ? 0 : s.ring + 4 * stage <= room ? 4 : (int)((room - s.ring) / stage);
     }
     ++s.per_sm;
-    if (!s.large && s.depth < 1) continue;
+    if (!s.large && s.depth < 1 && !(s.wide && !c.vec && s.ring <= kRingBytes)) continue;
     s.smem = s.ring + s.depth * stage;
     const long long cost = (long long)s.slot * (100 + 45 * s.vectors + (s.slot > 32 ? 60 : 0));
     if (least < 0 || (cost < least && c.vec)) { least = cost; best = s; }       // single columns cost the same for any k
@@ -201,7 +203,8 @@ __device__ __forceinline__ float ld_shared1(uint32_t a) {
 // zeros where no copy goes, so what has no column or no operand is read from it like the rest.  LARGE rows take more threads,
 // leave no room for parameters, and are read where they lie if they do not fit the ring.  THREADS: as many as a block may have; a
 // thread's places in the ring are then the same for every launch.
-template <int K, bool VEC, bool LARGE, int THREADS>
+// DIRECT: without a ring, if `ring` says so.
+template <int K, bool VEC, bool DIRECT, int THREADS>
 struct Columns {
   static constexpr int N = 4 * K;      // pairs
   int t, slot, C, slots;
@@ -279,7 +282,7 @@ struct Columns {
   // a row from the ring if there is one; zeros where the slot has no such row
   template <typename T>
   __device__ __forceinline__ void load(const Rows<T>& rows, int row, bool active, bool there, uint32_t from, float2 (&f)[N]) const {
-    if (LARGE && !ring) {
+    if (DIRECT && !ring) {
       fetch(rows.at(row), active && there, f);
     } else if (VEC) {
       constexpr int Q = 8 * sizeof(T) / 16;
@@ -609,7 +612,8 @@ struct Walk {
   }
 };
 
-// WIDE: a slot is whole warps.  BIG: blocks of 512 threads.  PIXEL: a gate for every row.
+// WIDE: a slot is whole warps.  BIG: blocks of 512 threads; with LARGE the parameters leave no room for a ring.  PIXEL: a gate for
+// every row.
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, bool LARGE, bool BIG, int MODE, bool PIXEL>
 __global__ void __launch_bounds__(block_threads(false, VEC, LARGE, BIG, K, MODE), blocks_forward(LARGE, BIG, MODE))
 residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int slots, int depth, int ring) {
@@ -621,7 +625,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
   for (int i = threadIdx.x; i < 16 * 64; i += blockDim.x) red[0][i] = 0.f;
   Slot s;
   s.id = threadIdx.x / slot; s.t = threadIdx.x % slot; s.size = slot; s.red = red[WIDE ? s.id : 0]; s.turn = 0;
-  const Cols cols = {s.t, slot, p.C, slots, !LARGE || depth > 0};
+  const Cols cols = {s.t, slot, p.C, slots, !LARGE || (!BIG && depth > 0)};
   const float inv_c = 1.f / (float)p.C;
   const bool by_image = (MODE & MODE_JOIN) && !PIXEL && p.gate;
   const Walk w(p, slots, s.id, WIDE, by_image);
@@ -659,7 +663,7 @@ residual_forward_kernel(const __grid_constant__ GeepsResidual p, int slot, int s
     }
   }
   unsigned char* area = shared;
-  Param<Cols, K, VEC, LARGE> sw, sb, w2, b2;          // scale * weight and scale * bias of the join, weight and bias of the next norm
+  Param<Cols, K, VEC, LARGE && !BIG> sw, sb, w2, b2;          // scale * weight and scale * bias of the join, weight and bias of the next norm
   Own<K, THREADS> factor;                      // the gate of the image at hand
   if (MODE & MODE_JOIN) { sw.set(cols, p.post.weight, 1.f, p.scale, area); sb.set(cols, p.post.bias, 0.f, p.scale, area); }
   if (MODE & MODE_NORM) { w2.set(cols, p.pre.weight, 1.f, nullptr, area); b2.set(cols, p.pre.bias, 0.f, nullptr, area); }
@@ -1273,14 +1277,22 @@ template <typename TR, typename TB, int MODE, bool PIXEL>
 void launch(const GeepsResidual& p, const Shape& s, bool backward, bool vec, cudaStream_t st) {
   const bool wide = s.slot >= 32;
   if (!vec) {
-    if (s.large) launch_forward<TR, TB, 4, false, true, true, false, MODE, PIXEL>(p, s, st);
+    if constexpr (MODE == MODE_BOTH) {         // the others' two parameters always fit
+      if (s.large) { launch_forward<TR, TB, 4, false, true, true, false, MODE, PIXEL>(p, s, st); return; }
+    }
+    if constexpr (MODE != MODE_NORM) {
+      if (s.wide && s.depth == 0) { launch_forward<TR, TB, 4, false, true, true, true, MODE, PIXEL>(p, s, st); return; }
+    }
+    if (s.wide) launch_forward<TR, TB, 4, false, true, false, true, MODE, PIXEL>(p, s, st);
     else if (s.vectors == 2) launch_kernel<TR, TB, 2, false, true, MODE, PIXEL>(p, s, backward, st);
     else if (wide) launch_kernel<TR, TB, 1, false, true, MODE, PIXEL>(p, s, backward, st);
     else launch_kernel<TR, TB, 1, false, false, MODE, PIXEL>(p, s, backward, st);
     return;
   }
-  if (s.large) launch_forward<TR, TB, 4, true, true, true, false, MODE, PIXEL>(p, s, st);
-  else if (s.vectors == 1) launch_kernel<TR, TB, 1, true, false, MODE, PIXEL>(p, s, backward, st);
+  if constexpr (MODE != MODE_NORM) {
+    if (s.large) { launch_forward<TR, TB, 4, true, true, true, false, MODE, PIXEL>(p, s, st); return; }
+  }
+  if (s.vectors == 1) launch_kernel<TR, TB, 1, true, false, MODE, PIXEL>(p, s, backward, st);
   else if (s.vectors == 2 && wide) launch_kernel<TR, TB, 2, true, true, MODE, PIXEL>(p, s, backward, st);
   else if (s.vectors == 2) launch_kernel<TR, TB, 2, true, false, MODE, PIXEL>(p, s, backward, st);
   else if (s.vectors == 3 && wide) launch_kernel<TR, TB, 3, true, true, MODE, PIXEL>(p, s, backward, st);

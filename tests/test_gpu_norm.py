@@ -288,6 +288,40 @@ def test_outputs_in_the_place_of_inputs(types):
             assert torch.equal(getattr(a, k), getattr(c, k)), k
 
 
+@pytest.mark.parametrize("c", [4101, 8021, 8968, 12289, 16384])
+@pytest.mark.parametrize("types,gate", [("bf16", 20), ("mixed", 160), ("fp32", 160), ("fp32", 0)])
+def test_outputs_in_the_place_of_inputs_of_wide_rows(c, types, gate):
+    a, b = Join(c, 160, c, "layer", "rms", True, gate, True, types), Join(c, 160, c, "layer", "rms", True, gate, True, types)
+    a.forward()
+    a.backward()
+    b.out = b.res
+    b.forward()
+    b.dres, b.dgate, b.dx = b.dout, b.gate, b.dy
+    b.backward()
+    for k in ("out", "y", "dres", "dx", "dgate", "dscale", "dw", "db", "dw2", "db2"):
+        assert (getattr(a, k) is None and getattr(b, k) is None) or torch.equal(getattr(a, k), getattr(b, k)), k
+
+
+@pytest.mark.parametrize("c", [9000, 9001])
+def test_wide_rows_repeat_in_a_captured_graph(c):
+    j = Join(c, 300, c, "layer", "layer", True, 30, True, "bf16")
+    j.forward()
+    j.backward()
+    names = ("out", "y", "dx", "dres", "dgate", "dscale", "dw", "db", "dw2", "db2")
+    first = {k: getattr(j, k).clone() for k in names}
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        j.forward()
+        j.backward()
+    for k in names:
+        getattr(j, k).zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(first[k], getattr(j, k)) for k in names)
+
+
 def test_large_means_small_spreads_and_constant_rows():
     for kind in ("layer", "rms"):
         x = torch.randn(8, 640, device=DEV) * 1e-2 + 100.0

@@ -22,14 +22,14 @@ def test_shapes_cover_the_rows_within_the_launch_limits(rows, c, backward, mode)
         for vec in ((True, False) if c % 8 == 0 else (False,)):
             for gate in ((0, rows, max(1, rows // 5 if rows % 5 == 0 else 1)) if mode > 1 else (0,)):
                 vectors, slot, slots, blocks, per_sm, depth, smem, large, tiles, width = shape(rows, c, backward, mode, gate, vec, types)
-                threads = 512 if large or (vec and not backward and c >= 4089 and vectors == 4) else 256 if not backward else 512 if not vec else 256 if vectors > 2 and mode > 1 else 384
+                threads = 512 if large or (not backward and vectors == 4 and c >= (4089 if vec else 4097)) else 256 if not backward else 512 if not vec else 256 if vectors > 2 and mode > 1 else 384
                 assert (tiles - 1) * width < c <= tiles * width and (tiles == 1 or (backward and width % 8 == 0))
                 assert vectors * slot * 8 >= width and slot * slots <= threads and slots >= 1
                 assert slot in (1, 2, 4, 8, 16, 32) or slot % 32 == 0
                 assert slot <= 32 or slots <= 15                    # a named barrier for each slot of several warps
                 assert 1 <= blocks <= 148 * per_sm and (blocks - 1) * slots < rows
                 assert (slot * slots) % 32 == 0                     # whole warps: their lanes meet in shuffles
-                assert (0 if large else 1) <= depth <= 4
+                assert (0 if large or (threads == 512 and not vec and not backward) else 1) <= depth <= 4
                 # dynamic and static shared memory of all blocks of an SM (1 KB of each is the system's)
                 fixed = 16 * 64 * 4 + ((4 if tiles > 1 else 2) * 8 * threads if backward else 0) + 1024
                 assert per_sm * (smem + fixed) <= 228 * 1024 and smem <= 208 * 1024
