@@ -186,6 +186,9 @@ int geeps_residual_backward(const GeepsResidual* p, void* stream);
 // the seventh are of one tile then); vec: rows of whole, aligned vectors
 int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int backward, int vec, int stream_fp32, int block_fp32,
                      int* out);
+// ... and of the backward pass's second launch, which joins the sums of blocks (of one tile), four values: its grid's x (0: no such
+// launch) and y, threads that share the parts of an image's gate gradient, slots that leave one part of it
+int geeps_norm_sums_shape(long long rows, long long gate_rows, int C, int mode, int vec, int stream_fp32, int block_fp32, int* out);
 
 // ---- clipping of gradients by their global norm (the reference's solver had it in its absent Caffe application) ----
 // norm = sqrt(sum over all tensors of g^2), c = norm > max_norm ? max_norm / norm : 1, dst = c * g; dst NULL: in place, and

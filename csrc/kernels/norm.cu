@@ -158,3 +158,19 @@ extern "C" int geeps_norm_shape(long long rows, long long gate_rows, int C, int 
   for (int i = 0; i < 10; ++i) out[i] = v[i];
   return 0;
 }
+extern "C" int geeps_norm_sums_shape(long long rows, long long gate_rows, int C, int mode, int vec, int stream_fp32, int block_fp32, int* out) {
+  const bool by_image = gate_rows > 0 && gate_rows < rows;
+  const Call c = {true, vec != 0, gate_rows == rows, by_image, false, mode, stream_fp32 ? 4 : 2, block_fp32 ? 4 : 2};
+  Shape s = plan(rows, C, c);
+  int width = C;
+  if (s.tiles > 1) {
+    Call t = c;
+    t.tile = true;
+    width = s.width;
+    s = plan(rows, width, t);
+  }
+  const SumsShape q = plan_sums(rows, gate_rows, width, by_image, s);
+  const int v[4] = {q.x, q.y, q.parts, q.merged};
+  for (int i = 0; i < 4; ++i) out[i] = v[i];
+  return 0;
+}

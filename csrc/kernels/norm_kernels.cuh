@@ -1304,22 +1304,29 @@ inline Call call_of(const GeepsResidual& p, bool backward, bool vec) {
   const bool by_pixel = p.gate && p.gate_rows == p.rows;
   return {backward, vec, by_pixel, p.gate && !by_pixel, false, p.mode, p.stream_fp32 ? 4 : 2, p.block_fp32 ? 4 : 2};
 }
-// The second launch of a backward pass, where blocks or slots share sums
+// The second launch of a backward pass, where blocks or slots share sums: x = 0 if there is none
+struct SumsShape { int x, y, parts, merged; };
+inline SumsShape plan_sums(long long rows, long long images, int C, bool cuts, const Shape& s) {
+  if (s.blocks == 1 && !(cuts && s.slots > 1)) return {0, 0, 1, 1};
+  SumsShape q = {(C + 31) / 32, 4, 1, 1};
+  if (cuts) {
+    q.merged = merged_slots(rows, (long long)s.blocks * s.slots, s.slot);
+    // Shares that an image has: one of each slot, or of each warp between those of its first and its last slots.  With no more
+    // parts than that y stays below 6 / 32 of the slots, 76000 of which are the most: a grid has 65535 blocks along y (with parts for
+    // the merged shares alone 70000 images of two pixels and 4 channels took 70004).
+    const long long all = (long long)s.blocks * s.slots, by_slot = all / images + 2, by_warp = all / q.merged / images + 2 * q.merged;
+    while (q.parts < 32 && q.parts < by_slot && q.parts < by_warp) q.parts <<= 1;
+    const long long items = images <= all ? images : all - 1;
+    q.y += (int)((items + 32 / q.parts - 1) / (32 / q.parts));
+  }
+  return q;
+}
 template <typename TB>
 void join_sums(const GeepsResidual& p, const Shape& s, cudaStream_t st) {
-  const bool cuts = p.gate && p.gate_rows < p.rows && p.dgate;
-  if (s.blocks == 1 && !(cuts && s.slots > 1)) return;
-  int y = 4, parts = 1, merged = 1;
-  if (cuts) {
-    merged = merged_slots(p.rows, (long long)s.blocks * s.slots, s.slot);
-    // shares that an image may have
-    const long long all = (long long)s.blocks * s.slots, per_image = all / merged / p.gate_rows + 2 * merged;
-    while (parts < 32 && parts < per_image) parts <<= 1;
-    const long long items = p.gate_rows <= all ? p.gate_rows : all - 1;
-    y += (int)((items + 32 / parts - 1) / (32 / parts));
-  }
-  geeps_launch(merged > 1 ? residual_sums_kernel<TB, true> : residual_sums_kernel<TB, false>, dim3((p.C + 31) / 32, y), dim3(kSumsThreads), 0, st,
-               p, p.mode, s.blocks, s.slots, parts, merged);
+  const SumsShape q = plan_sums(p.rows, p.gate_rows, p.C, p.gate && p.gate_rows < p.rows && p.dgate, s);
+  if (!q.x) return;
+  geeps_launch(q.merged > 1 ? residual_sums_kernel<TB, true> : residual_sums_kernel<TB, false>, dim3(q.x, q.y), dim3(kSumsThreads), 0, st, p, p.mode,
+               s.blocks, s.slots, q.parts, q.merged);
 }
 // columns [c, c + width) of the operands
 template <typename TR, typename TB>

@@ -1,0 +1,92 @@
+"""Sums of the norms' and joins' backward pass on whole numbers, where fp32 adds without rounding: every sum is compared for
+equality, so a row, a slot's share or an image's share that is lost or counted twice shows in any of them.
+
+Values are whole numbers up to 3, statistics are given as they are (means are whole, 1/std is 1/2, 1 or 2), parameters are powers of two.
+A term of a sum is then a multiple of 1/4 below 2^7 of a random sign: a sum of the 600000 at the most has a standard deviation below
+2^14 and stays a multiple of 1/4 below 2^17 with all of its parts, where fp32 has bits down to 2^-7."""
+import pytest
+import torch
+
+from geeps_b200.ops import functional as F
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+TYPES = {"bf16": (BF, BF), "mixed": (F32, BF), "fp32": (F32, F32)}
+
+
+def whole(gen, shape, dtype, most=3):
+    return torch.randint(-most, most + 1, shape, generator=gen, device=DEV).to(dtype)
+
+
+def power(gen, n):
+    return 2.0 ** torch.randint(-1, 2, (n,), generator=gen, device=DEV).float()
+
+
+def some_stats(gen, rows):
+    return torch.stack([torch.randint(-1, 2, (rows,), generator=gen, device=DEV).float(), power(gen, rows)], 1)
+
+
+def normalised(x, stats):
+    return (x.double() - stats[:, :1].double()) * stats[:, 1:].double()
+
+
+def same(got, want, what):
+    """Equal, where `got` is rounded once to its type."""
+    bad = got != want.to(got.dtype)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} differ, by up to {(got.double() - want).abs().max().item()}"
+
+
+def check_norm(rows, c, types, kind="rms"):
+    gen = torch.Generator(device=DEV).manual_seed(rows * 31 + c)
+    rt, bt = TYPES[types]
+    x, dy, stats = whole(gen, (rows, c), rt), whole(gen, (rows, c), bt), some_stats(gen, rows)
+    dx, dw, db = torch.empty(rows, c, dtype=rt, device=DEV), torch.full((c,), 7.0, device=DEV), torch.full((c,), 7.0, device=DEV)
+    F.norm_backward(x, dy, dx, F.Norm(kind, power(gen, c), None, stats, dweight=dw, dbias=db))
+    same(dw, (dy.double() * normalised(x, stats)).sum(0), "dweight")
+    same(db, dy.double().sum(0), "dbias")
+
+
+def check_join(images, pixels, c, types, gate="image", post="rms", pre="", most=3):
+    """Without `pre` the gradient of the sum is dout itself, so the branch's sums are exact; with it only the sums of the norm
+    behind are.  dgate in bf16 is the exact sum rounded once."""
+    rows = images * pixels
+    gen = torch.Generator(device=DEV).manual_seed(rows * 31 + c)
+    rt, bt = TYPES[types]
+    x, dout = whole(gen, (rows, c), bt, most), whole(gen, (rows, c), rt, most)
+    stats = some_stats(gen, rows)
+    w, s = power(gen, c), power(gen, c)
+    gate = whole(gen, ({"image": images, "pixel": rows}[gate], c), bt, 2) if gate else None
+    e, f = (lambda t, n=rows: torch.full((n, c), 7.0, dtype=t, device=DEV)), (lambda: torch.full((c,), 7.0, device=DEV))
+    dx, dres, dgate = e(bt), e(rt), None if gate is None else e(bt, gate.shape[0])
+    dscale, dw, db, dw2, db2 = f(), f(), f(), f(), f()
+    kw = {}
+    if pre:
+        out, dy, stats2 = whole(gen, (rows, c), rt), whole(gen, (rows, c), bt), some_stats(gen, rows)
+        kw = dict(out=out, dy=dy, pre=F.Norm(pre, power(gen, c), None, stats2, dweight=dw2, dbias=db2))
+    F.residual_backward(x, dout, dx, dres, post=F.Norm(post, w, None, stats, dweight=dw, dbias=db) if post else None, scale=s, dscale=dscale,
+                        gate=gate, dgate=dgate, **kw)
+    if pre:
+        same(dw2, (dy.double() * normalised(out, stats2)).sum(0), "dnext_weight")
+        same(db2, dy.double().sum(0), "dnext_bias")
+        return
+    n = normalised(x, stats) if post else x.double()
+    z = n * w.double() if post else n
+    g = 1.0 if gate is None else gate.double().repeat_interleave(rows // gate.shape[0], 0)
+    dh = dout.double()
+    same(dres, dh, "dres")
+    same(dscale, (dh * g * z).sum(0), "dscale")
+    if post:
+        same(dw, (dh * g * s.double() * n).sum(0), "dweight")
+        same(db, (dh * g * s.double()).sum(0), "dbias")
+    else:
+        same(dx, dh * g * s.double(), "dx")
+    if gate is not None:
+        same(dgate, (dh * s.double() * z).view(gate.shape[0], -1, c).sum(1), "dgate")
+
+
+# more images than slots, and more slots than a grid has blocks along an axis: narrow rows of single columns have 75776 slots
+@pytest.mark.parametrize("images,pixels,c", [(70000, 2, 4), (100000, 2, 3), (75776, 2, 1), (75775, 3, 7), (65532, 5, 5), (200000, 3, 1)])
+@pytest.mark.parametrize("types", list(TYPES))
+def test_gates_of_many_images_of_narrow_rows(images, pixels, c, types):
+    check_join(images, pixels, c, types)
