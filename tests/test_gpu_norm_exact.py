@@ -90,3 +90,32 @@ def check_join(images, pixels, c, types, gate="image", post="rms", pre="", most=
 @pytest.mark.parametrize("types", list(TYPES))
 def test_gates_of_many_images_of_narrow_rows(images, pixels, c, types):
     check_join(images, pixels, c, types)
+
+
+IMAGES = [(1, 60000, 8), (1, 50001, 24), (2, 20000, 32), (3, 11111, 64), (7, 4000, 5), (1, 9000, 130), (5, 700, 16), (900, 40, 8), (2, 37, 16),
+          (11, 333, 100), (512, 8, 64), (3000, 4, 8), (300, 40, 16), (5, 8, 4100), (3, 2, 9000), (2, 2, 16384), (1, 1, 8), (1, 30000, 1), (60, 100, 520)]
+
+
+@pytest.mark.parametrize("images,pixels,c", IMAGES)
+@pytest.mark.parametrize("types", list(TYPES))
+def test_gates_of_images(images, pixels, c, types):
+    check_join(images, pixels, c, types, post="rms" if c % 3 else "")
+
+
+ROWS = [(9000, 8), (9001, 24), (14000, 64), (9001, 192), (6000, 256), (9000, 576), (6001, 1024), (3000, 2048), (1500, 4096), (1300, 4104), (900, 6144), (700, 8192),
+        (450, 12288), (450, 16384), (60000, 1), (40000, 3), (9000, 33), (5000, 257), (3001, 1001), (2000, 2050), (900, 4099), (500, 8195), (450, 16383), (1, 1), (3, 40)]
+
+
+@pytest.mark.parametrize("rows,c", ROWS)
+@pytest.mark.parametrize("types", list(TYPES))
+def test_column_sums(rows, c, types):
+    check_norm(rows, c, types)
+    check_join(rows, 1, c, types, gate="")
+    check_join(rows, 1, c, types, gate="pixel", pre="rms")
+
+
+@pytest.mark.parametrize("rows,c", ROWS[::2])
+def test_column_sums_with_a_gate_for_every_pixel(rows, c):
+    check_join(rows, 1, c, "bf16", gate="pixel")
+    check_join(rows, 1, c, "fp32", gate="pixel", post="layer")
+    check_join(rows, 1, c, "mixed", gate="", pre="layer")
