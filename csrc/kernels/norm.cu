@@ -44,10 +44,9 @@ bool clash(const Use& a, const Use& b, int C) {
   if (a1 <= b0 || b1 <= a0) return false;
   const uintptr_t pa = (uintptr_t)a.ld * a.size, pb = (uintptr_t)b.ld * b.size;
   if (!(a.out && b.out) && a0 == b0 && a.size == b.size && a.rows == b.rows && (pa == pb || a.rows == 1)) return false;
-  if (pa == pb) {
-    const uintptr_t d = a0 < b0 ? (b0 - a0) % pa : pa - 1 - (a0 - b0 - 1) % pa;      // b's first column behind a's
-    const uintptr_t dd = d % pa;
-    if (dd >= wa && dd + wb <= pa) return false;
+  if (pa == pb && pa) {                    // a single row may have a pitch of zero
+    const uintptr_t d = a0 <= b0 ? (b0 - a0) % pa : (pa - (a0 - b0) % pa) % pa;      // bytes from a's first column to b's
+    if (d >= wa && d + wb <= pa) return false;
   }
   return true;
 }

@@ -25,3 +25,41 @@ def test_the_launch_that_joins_the_sums_fits_a_grid(images, pixels, c, mode):
             x, y, parts, merged = sums_shape(images * pixels, images, c, mode, vec, types)
             assert 0 <= x <= 512 and 0 <= y <= 65535, (x, y, parts, merged)
             assert parts in (1, 2, 4, 8, 16, 32) and merged in (1, 2, 4, 8, 16, 32)
+
+
+A, B, D = 1 << 32, 1 << 33, 1 << 34        # addresses that are never touched: every call here is refused
+
+
+def pack(**kw):
+    v = [kw.get(n, 0) for n in ("x", "res", "gate", "out", "y", "dout", "dy", "dx", "dres", "dgate", "scale", "dscale", "work")]
+    for n in ("post", "pre"):
+        v += list(kw.get(n, (0, 0, 0, 0, 0, 0.0, 0)))
+    mode = kw.get("mode", (2 if "x" in kw else 0) | (1 if "pre" in kw else 0))
+    v += [kw["rows"], kw.get("gate_rows", 0)] + [kw.get("ld" + n, kw.get("ld", kw["c"])) for n in
+                                                 ("x", "res", "gate", "out", "y", "dout", "dy", "dx", "dres", "dgate")]
+    return L.RESIDUAL.pack(*v, kw["c"], mode, kw.get("stream_fp32", 0), kw.get("block_fp32", 0), 0)
+
+
+@pytest.mark.parametrize("ld", [8, 9, 12, 16, 20, 24, 25, 31, 32, 40, 48, 1000, 1001])
+def test_two_outputs_on_the_same_rows_are_refused(ld):
+    """Any pitch; without the overlap the missing dout would be what is refused."""
+    lib = L.lib()
+    assert lib.geeps_residual_backward(pack(x=A, dx=D, dres=D, rows=4, c=8, ld=ld), None) == -12
+    assert lib.geeps_residual_backward(pack(x=A, dx=B, dres=D, rows=4, c=8, ld=ld), None) == 1
+    assert lib.geeps_residual_forward(pack(x=A, out=D, y=D, pre=(0, 0, 0, 0, 0, 1e-5, 1), rows=4, c=8, ld=ld), None) == -12
+    # an output and an input of another type at the same address and pitch in bytes
+    assert lib.geeps_residual_forward(pack(x=A, out=A, ldx=2 * ld, ldout=ld, rows=4, c=8, stream_fp32=1), None) == -12
+    assert lib.geeps_residual_forward(pack(x=A, out=A + 2, ldx=2 * ld, ldout=ld, rows=4, c=8, stream_fp32=1), None) == -12
+
+
+@pytest.mark.parametrize("ld", [16, 20, 24, 31, 33])
+def test_ranges_of_columns_side_by_side_are_not(ld):
+    lib = L.lib()
+    for x, out in ((A, A + 16), (A + 2 * (ld - 8), A), (A, A + 2 * ld * 2 + 16), (A + 2 * ld * 2 + 16, A)):
+        assert lib.geeps_residual_forward(pack(x=x, out=out, rows=4, c=8, ld=ld), None) == 1       # res is missing
+    assert lib.geeps_residual_forward(pack(x=A, out=A + 2 * (ld - 7), rows=4, c=8, ld=ld), None) == -12
+
+
+@pytest.mark.parametrize("shift,code", [(0, -12), (2, -12), (14, -12), (-14, -12), (16, 1), (-16, 1)])
+def test_single_rows_without_a_pitch(shift, code):
+    assert L.lib().geeps_residual_backward(pack(x=A, dx=D, dres=D + shift, rows=1, c=8, ld=0), None) == code
