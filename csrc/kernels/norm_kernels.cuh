@@ -553,24 +553,25 @@ __device__ __forceinline__ void normalise(const C_& cols, Slot& s, const GeepsNo
   for (int i = 0; i < N; ++i) f[i] = mul2(f[i], both(rstd));
   if (norm.stats && active && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * row) = make_float2(mean, rstd);
 }
-// n = (f - mean) * rstd with the statistics at hand.  Not zero where there is no column, but whatever it meets there is.
+// n = (f - mean) * rstd with the statistics at hand, the difference first: f * rstd - mean * rstd would be off by the rounding of
+// mean * rstd, however small n is.  Not zero where there is no column, but whatever it meets there is.
 template <int N>
 __device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
-  const float2 r = both(st.y), m = both(-st.x * st.y);
+  const float2 r = both(st.y), m = both(-st.x);
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = fma2(f[i], r, m);
+  for (int i = 0; i < N; ++i) f[i] = mul2(add2(f[i], m), r);
 }
-// Gradient of n * w + b by its input, for a = dz * w in place: rstd * (a - mean a - n mean(a n))
-__device__ __forceinline__ float2 norm_means(int kind, float rstd, float inv_c, float2 v) {       // of sums of a and a n
-  const float scale = -inv_c * rstd;
-  return make_float2(kind == NORM_LAYER ? v.x * scale : 0.f, v.y * scale);
+// Gradient of n * w + b by its input is rstd * (a - mean a - n mean(a n)), for a = dz * w: what stands in the brackets, in place.
+// rstd comes last, so what cancels in there cancels before anything is rounded to rstd's steps.
+__device__ __forceinline__ float2 norm_means(int kind, float inv_c, float2 v) {       // of sums of a and a n, both negative
+  return make_float2(kind == NORM_LAYER ? v.x * -inv_c : 0.f, v.y * -inv_c);
 }
 template <bool WIDE, bool TILE, int N>
-__device__ __forceinline__ void norm_gradient(Slot& s, int kind, float rstd, float inv_c, float2 known, const float2 (&n)[N], float2 (&a)[N]) {
-  const float2 m = TILE ? known : norm_means(kind, rstd, inv_c, slot_sum<WIDE>(make_float2(total(a), dot(a, n)), s));
-  const float2 m0 = both(m.x), m1 = both(m.y), r = both(rstd);
+__device__ __forceinline__ void norm_gradient(Slot& s, int kind, float inv_c, float2 known, const float2 (&n)[N], float2 (&a)[N]) {
+  const float2 m = TILE ? known : norm_means(kind, inv_c, slot_sum<WIDE>(make_float2(total(a), dot(a, n)), s));
+  const float2 m0 = both(m.x), m1 = both(m.y);
 #pragma unroll
-  for (int i = 0; i < N; ++i) a[i] = fma2(n[i], m1, fma2(a[i], r, m0));
+  for (int i = 0; i < N; ++i) a[i] = fma2(n[i], m1, add2(a[i], m0));
 }
 
 // A gate's factor and its slope.  A sigmoid is kept as q = min(f, 1 - f), negative where that is 1 - f: its slope q (1 - q) has
@@ -939,10 +940,10 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
           a[j] = mul2(a[j], m[e]);
         }
       }
-      norm_gradient<WIDE, TILE>(s, p.pre.kind, st2.y, inv_c, known2, n, a);
+      norm_gradient<WIDE, TILE>(s, p.pre.kind, inv_c, known2, n, a);
       cols.load(dout, row, active, has_dout, from, dh);
 #pragma unroll
-      for (int j = 0; j < N; ++j) dh[j] = add2(dh[j], a[j]);
+      for (int j = 0; j < N; ++j) dh[j] = fma2(a[j], both(st2.y), dh[j]);
     } else {
       cols.load(dout, row, active, has_dout, from, dh);
     }
@@ -983,7 +984,11 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         }
       }
       if (PIXEL && p.dgate) cols.store(dgate.at(row), active, dg);
-      if (p.post.kind) norm_gradient<WIDE, TILE>(s, p.post.kind, st1.y, inv_c, known1, z, dh);
+      if (p.post.kind) {
+        norm_gradient<WIDE, TILE>(s, p.post.kind, inv_c, known1, z, dh);
+#pragma unroll
+        for (int j = 0; j < N; ++j) dh[j] = mul2(dh[j], both(st1.y));
+      }
       if (!(MODE & MODE_NORM)) copy_stream();
       copy_branch();
       cols.store(dx.at(row), active, dh);
@@ -1052,7 +1057,7 @@ __device__ __forceinline__ void columns(const T* p, float (&f)[W]) {
     for (int e = 0; e < W; ++e) f[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
   }
 }
-// The means of rows that are worked on in tiles: for each norm {-rstd mean a, -rstd mean (a n)}, what norm_gradient() adds.  A block
+// The means of rows that are worked on in tiles: for each norm {-mean a, -mean (a n)}, what norm_gradient() adds.  A block
 // reads a row twice, the second time from L2: the join's sums are of the gradient that the next norm's means are part of.
 constexpr int kMeansThreads = 256;
 template <typename TR, typename TB, bool VEC, int MODE, bool PIXEL>
@@ -1103,7 +1108,7 @@ residual_means_kernel(const __grid_constant__ GeepsResidual p, float2* means) {
 #pragma unroll
         for (int e = 0; e < W; ++e) { a[e] *= w[e]; v.x += a[e]; v.y = fmaf(a[e], (n[e] - st2.x) * st2.y, v.y); }
       }
-      known = norm_means(p.pre.kind, st2.y, inv_c, block_sum(v));
+      known = norm_means(p.pre.kind, inv_c, block_sum(v));
       if (threadIdx.x == 0) means[2LL * row + 1] = known;
     }
     if ((MODE & MODE_JOIN) && p.post.kind) {
@@ -1121,7 +1126,7 @@ residual_means_kernel(const __grid_constant__ GeepsResidual p, float2* means) {
           float n[W], a[W];
           columns<W>(h + c, n); columns<W>(dy + c, a); param(p.pre.weight, c, w);
 #pragma unroll
-          for (int e = 0; e < W; ++e) d[e] += fmaf((n[e] - st2.x) * st2.y, known.y, fmaf(a[e] * w[e], st2.y, known.x));
+          for (int e = 0; e < W; ++e) d[e] = fmaf(fmaf((n[e] - st2.x) * st2.y, known.y, a[e] * w[e] + known.x), st2.y, d[e]);
         }
         param(p.post.weight, c, w); param(p.scale, c, f);
 #pragma unroll
@@ -1135,7 +1140,7 @@ residual_means_kernel(const __grid_constant__ GeepsResidual p, float2* means) {
         for (int e = 0; e < W; ++e) { v.x += d[e]; v.y = fmaf(d[e], (z[e] - st1.x) * st1.y, v.y); }
       }
       v = block_sum(v);
-      if (threadIdx.x == 0) means[2LL * row] = norm_means(p.post.kind, st1.y, inv_c, v);
+      if (threadIdx.x == 0) means[2LL * row] = norm_means(p.post.kind, inv_c, v);
     }
   }
 }
