@@ -60,7 +60,9 @@ bool meet(const void* a, uintptr_t na, const void* b, uintptr_t nb) {
 int check(const GeepsResidual& p, bool backward, int mode, bool* vec) {
   if (p.C < 1 || p.C > kMaxChannels) return GEEPS_ERR_NORM_CHANNELS;
   if (p.rows < 0 || p.rows > 1LL << 30) return (int)cudaErrorInvalidValue;
-  if (p.gate && (p.gate_rows < 1 || p.gate_rows > p.rows || p.rows % p.gate_rows)) return p.rows ? GEEPS_ERR_NORM_GATE : 0;
+  // without rows any number of images goes: each has none
+  if (p.gate && (p.rows ? p.gate_rows < 1 || p.gate_rows > p.rows || p.rows % p.gate_rows : p.gate_rows < 0)) return GEEPS_ERR_NORM_GATE;
+  if (p.gate && p.gate_rows > 1LL << 30) return (int)cudaErrorInvalidValue;
   if (p.stream_fp32 == 0 && p.block_fp32) return (int)cudaErrorInvalidValue;
   const int r = p.stream_fp32 ? 4 : 2, b = p.block_fp32 ? 4 : 2;
   const long long n = p.rows, gr = p.gate ? p.gate_rows : 0;
@@ -102,11 +104,18 @@ int check(const GeepsResidual& p, bool backward, int mode, bool* vec) {
   return 0;
 }
 
+// Sums over no rows: the parameters' gradients, and the gate's where there are images
 __global__ void clear_sums_kernel(const __grid_constant__ GeepsResidual p) {
   geeps_pdl_enter();
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
+  const long long at = (long long)blockIdx.x * blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < p.C) write_sums(p, p.mode, c, zero);
+  if (at < p.C) write_sums(p, p.mode, (int)at, zero);
+  if (!p.gate || !p.dgate) return;
+  for (long long i = at; i < p.gate_rows * p.C; i += step) {
+    const long long to = i / p.C * p.lddgate + i % p.C;
+    if (p.block_fp32) ((float*)p.dgate)[to] = 0.f;
+    else ((__nv_bfloat16*)p.dgate)[to] = __float2bfloat16(0.f);
+  }
 }
 
 int residual(const GeepsResidual* q, bool backward, void* stream) {
@@ -119,7 +128,8 @@ int residual(const GeepsResidual* q, bool backward, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   if (p.rows == 0) {
     if (!backward) return 0;
-    geeps_launch(clear_sums_kernel, dim3((p.C + 255) / 256), dim3(256), 0, st, p);
+    const long long values = p.gate && p.dgate && p.gate_rows > 1 ? p.gate_rows * p.C : p.C, blocks = (values + 255) / 256;
+    geeps_launch(clear_sums_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, p);
     return (int)cudaGetLastError();
   }
   if (backward && !p.work && geeps_residual_work(p.rows, p.gate ? p.gate_rows : 0, p.C, mode) > 0) return (int)cudaErrorInvalidValue;

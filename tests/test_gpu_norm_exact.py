@@ -119,3 +119,31 @@ def test_column_sums_with_a_gate_for_every_pixel(rows, c):
     check_join(rows, 1, c, "bf16", gate="pixel")
     check_join(rows, 1, c, "fp32", gate="pixel", post="layer")
     check_join(rows, 1, c, "mixed", gate="", pre="layer")
+
+
+def no_rows(types, gate_rows, dgate, c=40):
+    rt, bt = TYPES[types]
+    e = lambda t, n=0: torch.empty(n, c, dtype=t, device=DEV)
+    f = lambda: torch.full((c,), 7.0, device=DEV)
+    gate = torch.ones(gate_rows, c, dtype=bt, device=DEV)
+    sums = [f() for _ in range(5)]
+    stats = torch.empty(0, 2, device=DEV)
+    F.residual_forward(e(bt), e(rt), e(rt), post=F.Norm("layer", stats=stats), gate=gate, y=e(bt), pre=F.Norm("rms", stats=stats))
+    F.residual_backward(e(bt), e(rt), e(bt), e(rt), post=F.Norm("layer", stats=stats, dweight=sums[0], dbias=sums[1]), scale=f(), dscale=sums[2], gate=gate,
+                        dgate=dgate, sigmoid=True, out=e(rt), dy=e(bt), pre=F.Norm("rms", stats=stats, dweight=sums[3], dbias=sums[4]))
+    assert all((s == 0).all() for s in sums)
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("gate_rows", [1, 4, 1000])
+def test_images_without_rows_have_a_gradient_of_zero(types, gate_rows):
+    bt = TYPES[types][1]
+    dgate = torch.full((gate_rows, 40), 7.0, dtype=bt, device=DEV)
+    no_rows(types, gate_rows, dgate)
+    assert (dgate == 0).all()
+    no_rows(types, gate_rows, None)
+    wide = torch.full((gate_rows + 1, 61), 7.0, dtype=bt, device=DEV)      # rows of a wider matrix, and nothing beside them
+    no_rows(types, gate_rows, wide[:gate_rows, 3:43])
+    assert (wide[:gate_rows, 3:43] == 0).all()
+    wide[:gate_rows, 3:43] = 7.0
+    assert (wide == 7.0).all()

@@ -63,3 +63,19 @@ def test_ranges_of_columns_side_by_side_are_not(ld):
 @pytest.mark.parametrize("shift,code", [(0, -12), (2, -12), (14, -12), (-14, -12), (16, 1), (-16, 1)])
 def test_single_rows_without_a_pitch(shift, code):
     assert L.lib().geeps_residual_backward(pack(x=A, dx=D, dres=D + shift, rows=1, c=8, ld=0), None) == code
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(stream_fp32=0, block_fp32=1), 1),
+    (dict(mode=1), 1),
+    (dict(mode=3), 1),
+    (dict(post=(0, 0, 1 << 30 | 4, 0, 0, 1e-5, 1)), -14),
+    (dict(gate_rows=-3), -11),
+    (dict(gate_rows=(1 << 30) + 1), 1),
+    (dict(gate=B, dgate=B + 16, gate_rows=4), -12),
+    (dict(gate=B, dgate=D, gate_rows=4, lddgate=7), 1),
+    (dict(gate=B, dgate=D, gate_rows=4, dscale=D + 60), -12),
+])
+def test_calls_without_rows_are_checked_like_others(kw, code):
+    """A gate without rows to go with was let through whatever else was wrong."""
+    assert L.lib().geeps_residual_backward(pack(**{"x": A, "gate": B, "gate_rows": 4, "rows": 0, "c": 8, **kw}), None) == code
