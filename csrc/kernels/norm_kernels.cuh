@@ -914,6 +914,8 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         if (MODE & MODE_NORM) stats[1][threadIdx.x] = *reinterpret_cast<const float2*>(p.pre.stats + 2LL * q);
         if (TILE && (MODE & MODE_JOIN) && p.post.kind) stats[TILE ? 2 : 0][threadIdx.x] = means[2LL * q];
         if (TILE && (MODE & MODE_NORM)) stats[TILE ? 3 : 0][threadIdx.x] = means[2LL * q + 1];
+      } else if (!WIDE) {                      // a row that is none must not be normalised as one of an image before, which may not be finite
+        stats[0][threadIdx.x] = stats[1][threadIdx.x] = both(0.f);
       }
       __syncwarp();
     }

@@ -147,3 +147,26 @@ def test_images_without_rows_have_a_gradient_of_zero(types, gate_rows):
     assert (wide[:gate_rows, 3:43] == 0).all()
     wide[:gate_rows, 3:43] = 7.0
     assert (wide == 7.0).all()
+
+
+@pytest.mark.parametrize("types", ["bf16", "fp32"])
+@pytest.mark.parametrize("c,images", [(64, 2), (32, 5), (16, 3), (64, 40)])
+def test_a_row_that_is_not_finite_leaves_other_images_alone(types, c, images):
+    """Slots that share a warp take the same number of turns, and some have no row in the last: what they compute there must not
+    come from a row of an image before.  A row without a finite value in every tenth place of all images but the last; only the last's
+    gradient is compared, and all of it."""
+    pixels = 2000
+    for shift in range(0, 8):
+        rows = images * pixels + shift * images
+        per = rows // images
+        gen = torch.Generator(device=DEV).manual_seed(shift)
+        rt, bt = TYPES[types]
+        x, dout, stats, gate = whole(gen, (rows, c), bt), whole(gen, (rows, c), rt), some_stats(gen, rows), whole(gen, (images, c), bt, 2)
+        last = rows - per
+        x[:last:10], stats[:last:10] = float("nan"), float("nan")
+        x[5:last:10], stats[5:last:10] = float("inf"), float("inf")
+        s, dgate = power(gen, c), torch.full((images, c), 7.0, dtype=bt, device=DEV)
+        dx, dres = torch.empty_like(x), torch.empty_like(dout)
+        F.residual_backward(x, dout, dx, dres, post=F.Norm("layer", None, None, stats), scale=s, gate=gate, dgate=dgate)
+        same(dres, dout.double(), "dres")
+        same(dgate[-1], (dout.double() * s.double() * normalised(x, stats))[last:].sum(0), f"dgate of the last image, {rows} rows")
