@@ -19,6 +19,15 @@ def side_streams(device, n: int, kind: str = "branch") -> list:
     return pool[:n]
 
 
+def leaves(layers):
+    """The layers themselves, in the place of containers what these hold, at any depth."""
+    for l in layers:
+        if hasattr(l, "sublayers"):
+            yield from l.sublayers()
+        else:
+            yield l
+
+
 class Concat(Layer):
     """Parallel branches whose outputs are concatenated along channels.  The last layer of each
     branch writes straight into its channel slice of the joint output (no copy); in backward
@@ -39,8 +48,7 @@ class Concat(Layer):
 
     def sublayers(self):
         for br in self.branches:
-            for l in br:
-                yield l
+            yield from leaves(br)
 
     def setup(self, in_shape, device):
         self.in_shape = in_shape
@@ -182,11 +190,7 @@ class Residual(Layer):
         self.follower = None           # the Residual whose norm the join computes
 
     def sublayers(self):
-        for l in ([self.pre] if self.pre else []) + self.layers + self.gate + [self.join]:
-            if hasattr(l, "sublayers"):
-                yield from l.sublayers()
-            else:
-                yield l
+        return leaves(([self.pre] if self.pre else []) + self.layers + self.gate + [self.join])
 
     def setup(self, in_shape, device):
         self.in_shape = self.out_shape = s = tuple(in_shape)
@@ -271,11 +275,7 @@ class Net:
         self.loss_layer = loss or SoftmaxLoss()
 
     def all_layers(self):
-        for l in self.layers:
-            if hasattr(l, "sublayers"):
-                yield from l.sublayers()
-            else:
-                yield l
+        return leaves(self.layers)
 
     def param_layers(self):
         return [l for l in self.all_layers() if l.param_specs()]
