@@ -73,7 +73,8 @@ class PSModule:
         part of a table snapshot.
         clip_gradients: scale the worker's gradients by clip_gradients / norm where the norm of all of them exceeds it
         (Caffe's solver parameter; every worker clips its own batch's).  No table is then pushed before the backward pass has
-        ended.  `clip_result` holds the last step's {norm, factor}; inf only measures."""
+        ended, and the update buffers of all tables are held until then.  `clip_result` holds the last step's {norm, factor};
+        inf only measures."""
         self.net, self.rank, self.world, self.slack = net, rank, world, slack
         self.device = torch.device(device)
         self.trace = trace or NullTrace()
@@ -200,27 +201,27 @@ class PSModule:
                 M[i - 1]["b"] = ps.virtual_local_access(M[i - 1]["rows"], True)
             for t in reversed(tabs):
                 t.h_pre = ps.virtual_pre_update(t.table_id, range(t.rows))
-            if self.clip_gradients is None:
-                self._declare_updates(tabs)
+            for t in reversed(tabs):
+                t.h_post = ps.virtual_post_read(t.h_read)
+                if self.clip_gradients is None:
+                    t.h_upd = ps.virtual_update(t.h_pre)
             if i in M:
                 M[i]["pb"] = ps.virtual_post_local_access(M[i]["b"], False)
-        if self.clip_gradients is not None:
+        if self.clip_gradients is not None:       # only the updates wait for all gradients
             for _, tabs in reversed(self.groups):
-                self._declare_updates(tabs)
+                for t in reversed(tabs):
+                    t.h_upd = ps.virtual_update(t.h_pre)
         ps.virtual_clock()
         ps.finish_virtual_iteration()
 
-    def _declare_updates(self, tabs):
-        for t in reversed(tabs):
-            t.h_post = self.ps.virtual_post_read(t.h_read)
-            t.h_upd = self.ps.virtual_update(t.h_pre)
-
-    def _update(self, name, tabs):
+    def _update(self, name, tabs, post_read, update):
         if tabs:
-            with self.trace.span(f"update:{name}", "ps"):
+            with self.trace.span(f"{'update' if update else 'post_read'}:{name}", "ps"):
                 for t in reversed(tabs):
-                    self.ps.post_read(t.h_post)
-                    self.ps.update(t.h_upd)
+                    if post_read:
+                        self.ps.post_read(t.h_post)
+                    if update:
+                        self.ps.update(t.h_upd)
 
     def _clip(self):
         """Clip the gradients where they are, in the tables' update buffers.  Their layout is kept for every set of buffers (the
@@ -386,8 +387,7 @@ class PSModule:
                 t.layer.g32 = t.views(self.ps.pre_update(t.h_pre))
             with tr.span(f"bwd:{name}", "bwd"):
                 g = l.backward(g)
-            if self.clip_gradients is None:
-                self._update(name, tabs)
+            self._update(name, tabs, post_read=True, update=self.clip_gradients is None)
             if i in M:
                 self.ps.post_local_access(M[i]["pb"])
             self._mark("b:" + name)
@@ -396,7 +396,7 @@ class PSModule:
                 self._clip()
             self._mark("clip")
             for l, tabs in reversed(self.groups):
-                self._update(getattr(l, "name", type(l).__name__), tabs)
+                self._update(getattr(l, "name", type(l).__name__), tabs, post_read=False, update=True)
         if ev is not None:
             ev[-1][2].record()
         with tr.span("clock", "ps", clock=self.steps):
