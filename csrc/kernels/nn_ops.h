@@ -159,9 +159,8 @@ typedef struct GeepsNorm {
 // else bf16; block_fp32 (with stream_fp32 only): x, y, gate, dy, dx and dgate.  An output may be the very same rows as an
 // input of its size; any other overlap of an output, a parameter's gradient or statistics that are written with another operand
 // is refused.  Rows are at most 2^30, pitches less than 2^29, C is 1 to 16384.  Without rows the gradients of the parameters and of
-// the gate are zeros.
-// stats and work are multiples of 8 bytes; every other address will do.  work: geeps_residual_work() floats, private to the
-// call while it runs.  mode: 1 for a norm alone (no x), 2 for a join, 3 for a join with a norm behind it.
+// the gate are zeros.  stats and work are at multiples of 8 bytes, everything else at multiples of a value's size.  work:
+// geeps_residual_work() floats, private to the call while it runs.  mode: 1 for a norm alone (no x), 2 for a join, 3 for a join with a norm behind it.
 #define GEEPS_ERR_NORM_CHANNELS (-10)
 #define GEEPS_ERR_NORM_GATE (-11)
 #define GEEPS_ERR_NORM_OVERLAP (-12)

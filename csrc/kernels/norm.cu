@@ -79,12 +79,17 @@ int check(const GeepsResidual& p, bool backward, int mode, bool* vec) {
     *vec = *vec && vectors_ok(u[i], p.C);
     for (int j = 0; j < i; ++j) if (clash(u[i], u[j], p.C)) return GEEPS_ERR_NORM_OVERLAP;
   }
-  if (((uintptr_t)p.post.stats | (uintptr_t)p.pre.stats | (uintptr_t)p.work) & 7) return GEEPS_ERR_NORM_ALIGN;
+  // the columns' gradients last: backward only
   const Column v[] = {{p.post.stats, 2 * n, !backward}, {p.pre.stats, 2 * n, !backward}, {p.scale, p.C, false},
                       {p.post.weight, p.C, false}, {p.post.bias, p.C, false}, {p.pre.weight, p.C, false}, {p.pre.bias, p.C, false},
                       {p.dscale, p.C, true}, {p.post.dweight, p.C, true}, {p.post.dbias, p.C, true}, {p.pre.dweight, p.C, true},
                       {p.pre.dbias, p.C, true}};
-  for (int i = 0; i < (backward ? 12 : 7); ++i) {            // the gradients last: backward only
+  const int columns = backward ? 12 : 7;
+  uintptr_t off = ((uintptr_t)p.post.stats | (uintptr_t)p.pre.stats | (uintptr_t)p.work) & 7;
+  for (int i = 0; i < count; ++i) off |= (uintptr_t)u[i].p & (u[i].size - 1);
+  for (int i = 0; i < columns; ++i) off |= (uintptr_t)v[i].p & 3;
+  if (off) return GEEPS_ERR_NORM_ALIGN;
+  for (int i = 0; i < columns; ++i) {
     for (int j = 0; j < i; ++j)
       if ((v[i].out || v[j].out) && meet(v[i].p, 4 * v[i].n, v[j].p, 4 * v[j].n)) return GEEPS_ERR_NORM_OVERLAP;
     for (int j = 0; j < count; ++j)
@@ -119,6 +124,7 @@ __global__ void clear_sums_kernel(const __grid_constant__ GeepsResidual p) {
 }
 
 int residual(const GeepsResidual* q, bool backward, void* stream) {
+  if (!q) return (int)cudaErrorInvalidValue;
   const GeepsResidual& p = *q;
   const int mode = p.mode;
   if (mode < MODE_NORM || mode > MODE_BOTH) return (int)cudaErrorInvalidValue;

@@ -79,3 +79,40 @@ def test_single_rows_without_a_pitch(shift, code):
 def test_calls_without_rows_are_checked_like_others(kw, code):
     """A gate without rows to go with was let through whatever else was wrong."""
     assert L.lib().geeps_residual_backward(pack(**{"x": A, "gate": B, "gate_rows": 4, "rows": 0, "c": 8, **kw}), None) == code
+
+
+S = 1 << 30
+NORM = (0, 0, S, 0, 0, 1e-5, 1)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=A + 1), dict(out=D + 1), dict(res=B + 1), dict(y=S + 4097, pre=(0, 0, 0, 0, 0, 1e-5, 1)), dict(gate=S + 4097, gate_rows=4),
+    dict(res=B + 2, stream_fp32=1), dict(out=D + 2, stream_fp32=1), dict(x=A + 2, stream_fp32=1, block_fp32=1),
+    dict(gate=S + 4098, gate_rows=1, stream_fp32=1, block_fp32=1),
+    dict(scale=S + 4098), dict(post=(S + 4098, 0, 0, 0, 0, 1e-5, 1)), dict(post=(0, S + 4097, 0, 0, 0, 1e-5, 1)),
+    dict(y=S + 8192, pre=(S + 4098, 0, 0, 0, 0, 1e-5, 1)), dict(y=S + 8192, pre=(0, S + 4098, 0, 0, 0, 1e-5, 1)),
+])
+def test_addresses_between_values_are_refused_forward(kw):
+    """A value is read at a multiple of its size; a kernel that is given another address faults.  (Without the refusal the missing
+    output or input of each of these calls would be what is refused.)"""
+    kw = {"x": A, "res": B, "out": D, "rows": 4, "c": 8, **kw}
+    kw["out" if kw["out"] == D else "res"] = 0
+    assert L.lib().geeps_residual_forward(pack(**kw), None) == -14
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=A + 1), dict(dout=B + 1), dict(dx=D + 1), dict(gate=S + 4096, gate_rows=4, dgate=S + 8193), dict(dy=S + 4097, out=S + 8192, pre=NORM),
+    dict(dy=S + 4096, out=S + 8193, pre=NORM), dict(dout=B + 2, stream_fp32=1), dict(dx=D + 2, stream_fp32=1, block_fp32=1), dict(dscale=S + 4098),
+    dict(post=(0, 0, S, S + 4098, 0, 1e-5, 1)), dict(post=(0, 0, S, 0, S + 4097, 1e-5, 1)), dict(scale=S + 4098),
+    dict(dy=S + 4096, out=S + 8192, pre=(0, 0, S, S + 16386, 0, 1e-5, 1)), dict(dy=S + 4096, out=S + 8192, pre=(0, 0, S, 0, S + 16387, 1e-5, 1)),
+    dict(rows=0, dscale=S + 4098),
+])
+def test_addresses_between_values_are_refused_backward(kw):
+    assert L.lib().geeps_residual_backward(pack(**{"x": A, "dout": B, "dx": D, "rows": 4, "c": 8, **kw}), None) == -14       # dres is missing
+
+
+def test_dres_between_values_is_refused():
+    assert L.lib().geeps_residual_backward(pack(x=A, dout=B, dres=D + 1, rows=4, c=8), None) == -14       # dx is missing
+    assert L.lib().geeps_residual_backward(pack(x=A, dout=B, dres=D + 2, rows=4, c=8, stream_fp32=1), None) == -14
+    assert L.lib().geeps_residual_backward(pack(x=A, dout=B, dres=D + 2, rows=4, c=8), None) == 1
+    assert L.lib().geeps_residual_backward(pack(x=A + 2, dout=B + 4, dres=D + 4, rows=4, c=8, stream_fp32=1), None) == 1
