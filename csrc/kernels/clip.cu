@@ -407,6 +407,10 @@ extern "C" int geeps_clip_gradients(const GeepsTensors* src, const GeepsTensors*
     if (src->count[i] < 0 || (dst && dst->count[i] != src->count[i])) return (int)cudaErrorInvalidValue;
     if (src->count[i] && (!src->ptr[i] || (dst && !dst->ptr[i]))) return (int)cudaErrorInvalidValue;
   }
+  bool between = ((uintptr_t)result & 3) || ((uintptr_t)work & 7);
+  for (long long i = 0; i < src->n; ++i)
+    if (src->count[i]) between |= ((uintptr_t)src->ptr[i] & (src->fp32[i] ? 3 : 1)) || (dst && ((uintptr_t)dst->ptr[i] & (dst->fp32[i] ? 3 : 1)));
+  if (between) return GEEPS_ERR_CLIP_ALIGN;
   if (overlaps_itself(*src) || (dst && (overlaps_itself(*dst) || overlaps(*src, *dst)))) return GEEPS_ERR_CLIP_OVERLAP;
   const uintptr_t r = (uintptr_t)result, w = (uintptr_t)work, we = w + geeps_clip_work(src) * sizeof(double);
   auto meets = [&](const Range& q) { return q.from != q.to && ((q.from < r + 8 && r < q.to) || (q.from < we && w < q.to)); };

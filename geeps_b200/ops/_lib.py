@@ -141,7 +141,8 @@ class Tensors(C.Structure):
 # what the argument checks of native calls answer besides CUDA's error codes
 REFUSALS = {-10: "a row has 1 to 16384 channels", -11: "the gate's rows do not divide the rows",
             -12: "an output overlaps another operand", -13: "tensors overlap",
-            -14: "stats and work must begin on a multiple of 8 bytes, other operands on one of their size"}
+            -14: "stats and work must begin on a multiple of 8 bytes, other operands on one of their size",
+            -15: "a tensor, the result or the workspace begins between two values"}
 
 _lib = None
 _launches = 0
