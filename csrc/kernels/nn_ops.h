@@ -195,7 +195,8 @@ int geeps_norm_sums_shape(long long rows, long long gate_rows, int C, int mode, 
 // then nothing is written while c is 1.  result: {norm, c}.  Tensors are dense, fp32 or bf16 each; dst[i] has src[i]'s
 // count and shares no memory with any src but src[i] itself, type and all; result and work share none with a tensor.  Every
 // address is a multiple of its values' size (work: of 8 bytes).  The squares are added in 64 bits, in an order that depends on the
-// counts alone.  work: geeps_clip_work() doubles, private to the call while it runs.
+// counts, the types, where each src begins within a line of 32 bytes (bf16: 16) and the GPU's number of SMs.  work:
+// geeps_clip_work() doubles, private to the call while it runs.
 #define GEEPS_ERR_CLIP_OVERLAP (-13)
 #define GEEPS_ERR_CLIP_ALIGN (-15)
 typedef struct GeepsTensors {
