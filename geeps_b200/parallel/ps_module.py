@@ -224,15 +224,13 @@ class PSModule:
                         self.ps.update(t.h_upd)
 
     def _clip(self):
-        """Clip the gradients where they are, in the tables' update buffers.  Their layout is kept for every set of buffers (the
-        update ring has a few), so that a recorded step finds the same arguments again."""
-        grads = [g for t in self.tables for g in t.layer.g32.values()]
-        key = tuple(g.data_ptr() for g in grads)
-        if key not in self._clip_lists:
-            if len(self._clip_lists) == 64:        # buffers that do not come back are not kept for ever
-                self._clip_lists.clear()
-            self._clip_lists[key] = F.GradList(grads)
-        grads = self._clip_lists[key]
+        """Clip the gradients where they are, in the tables' update buffers.  Their layout is made once for each phase of the update
+        ring, so that a recorded step finds the same arguments again, and anew when a phase has other buffers."""
+        buffers = [g for t in self.tables for g in t.layer.g32.values()]
+        phase = self.steps % self._period
+        grads = self._clip_lists.get(phase)
+        if grads is None or [g.data_ptr() for g in grads.tensors] != [g.data_ptr() for g in buffers]:
+            grads = self._clip_lists[phase] = F.GradList(buffers)
         if self._clip_work is None:
             self._clip_work = torch.empty(grads.work_size(), dtype=torch.float64, device=self.device)
         F.clip_gradients(grads, self.clip_gradients, self.clip_result, work=self._clip_work)

@@ -111,3 +111,46 @@ def test_a_clipped_step_trains_under_a_budget():
         return out
     plain = run()
     same_training([plain, run(clip_gradients=float("inf")), run(clip_gradients=float("inf"), cache_fraction=0.9)])
+
+
+def test_layouts_are_kept_for_the_phases_of_the_update_ring_only(monkeypatch):
+    """A step's gradients come in the buffers of its phase of the ring, so a phase's layout serves again (a recorded step finds the same
+    arguments); buffers that do not come back are not held."""
+    import torch
+
+    import geeps_b200.parallel.ps_module as pm
+
+    class List:
+        def __init__(self, tensors):
+            self.tensors = list(tensors)
+
+        def work_size(self):
+            return 4
+    used = []
+    monkeypatch.setattr(pm.F, "GradList", List)
+    monkeypatch.setattr(pm.F, "clip_gradients", lambda grads, bound, result, work: used.append(grads))
+
+    class Layer:
+        pass
+    mod = PSModule.__new__(PSModule)
+    mod.device, mod.clip_gradients, mod.clip_result, mod._clip_lists, mod._clip_work = torch.device("cpu"), 1.0, None, {}, None
+    mod._period, mod.tables = 2, []
+    for i in range(3):
+        t = Table(i, 1)
+        t.layer = Layer()
+        mod.tables.append(t)
+    ring = [[torch.zeros(5) for _ in mod.tables] for _ in range(2)]
+
+    def step(i, buffers):
+        mod.steps = i
+        for t, b in zip(mod.tables, buffers):
+            t.layer.g32 = {"w": b}
+        mod._clip()
+        assert [t.data_ptr() for t in used[-1].tensors] == [b.data_ptr() for b in buffers]
+    for i in range(8):
+        step(i, ring[i % 2])
+    assert len({id(u) for u in used}) == 2 and used[0] is used[2] and used[1] is used[3]
+    other = [[torch.zeros(5) for _ in mod.tables] for _ in range(10)]        # all alive, so all at addresses of their own
+    for i in range(10):
+        step(8 + i, other[i])
+    assert len(mod._clip_lists) == 2
