@@ -183,7 +183,8 @@ int geeps_residual_forward(const GeepsResidual* p, void* stream);
 int geeps_residual_backward(const GeepsResidual* p, void* stream);
 // launch shape (host arithmetic only), ten values: vectors a thread, threads a row, rows a block at a time, blocks, blocks an
 // SM, stages of the ring, bytes of shared memory, rows read where they lie, tiles of a row, columns of a tile (the first five and
-// the seventh are of one tile then); vec: rows of whole, aligned vectors
+// the seventh are of one tile then); vec: rows of whole, aligned vectors.  Not 0: there is no kernel of this shape (the calls' own
+// answer, too; no sizes have it)
 int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int backward, int vec, int stream_fp32, int block_fp32,
                      int* out);
 // ... and of the backward pass's second launch, which joins the sums of blocks (of one tile), four values: its grid's x (0: no such

@@ -139,7 +139,7 @@ int residual(const GeepsResidual* q, bool backward, void* stream) {
     return (int)cudaGetLastError();
   }
   if (backward && !p.work && geeps_residual_work(p.rows, p.gate ? p.gate_rows : 0, p.C, mode) > 0) return (int)cudaErrorInvalidValue;
-  (!p.stream_fp32 ? run_bf16 : !p.block_fp32 ? run_mixed : run_fp32)(p, backward, vec, st);
+  if (!(!p.stream_fp32 ? run_bf16 : !p.block_fp32 ? run_mixed : run_fp32)(p, backward, vec, st)) return (int)cudaErrorNotSupported;
   return (int)cudaGetLastError();
 }
 
@@ -167,11 +167,12 @@ extern "C" int geeps_residual_forward(const GeepsResidual* p, void* stream) { re
 extern "C" int geeps_residual_backward(const GeepsResidual* p, void* stream) { return residual(p, true, stream); }
 extern "C" int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int backward, int vec, int stream_fp32, int block_fp32,
                                 int* out) {
-  const bool by_image = gate_rows > 0 && gate_rows < rows;
-  const Shape s = plan(rows, C, {backward != 0, vec != 0, gate_rows == rows, by_image, false, mode, stream_fp32 ? 4 : 2, block_fp32 ? 4 : 2});
+  const bool by_pixel = gate_rows == rows, by_image = gate_rows > 0 && gate_rows < rows;
+  const Shape s = plan(rows, C, {backward != 0, vec != 0, by_pixel, by_image, false, mode, stream_fp32 ? 4 : 2, block_fp32 ? 4 : 2});
   const int v[10] = {s.vectors, s.slot, s.slots, s.blocks, s.per_sm, s.depth, (int)s.smem, s.large, s.tiles, s.width};
   for (int i = 0; i < 10; ++i) out[i] = v[i];
-  return 0;
+  const bool direct = s.large ? mode == MODE_BOTH || (vec && mode == MODE_JOIN) : !vec && s.wide && s.depth == 0 && mode != MODE_NORM;
+  return s.tiles > 1 || direct || planned(backward, vec, s.slot >= 32, s.wide, s.vectors, mode, by_pixel, block_fp32 ? 4 : 2) ? 0 : (int)cudaErrorNotSupported;
 }
 extern "C" int geeps_norm_sums_shape(long long rows, long long gate_rows, int C, int mode, int vec, int stream_fp32, int block_fp32, int* out) {
   const bool by_image = gate_rows > 0 && gate_rows < rows;

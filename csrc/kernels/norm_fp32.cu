@@ -1,4 +1,4 @@
 // Norms and residual joins: types float, float (along the residual connection, inside a block)
 #include "norm_kernels.cuh"
 
-void rownorm::run_fp32(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) { run<float, float>(p, backward, vec, st); }
+bool rownorm::run_fp32(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) { return run<float, float>(p, backward, vec, st); }

@@ -121,6 +121,17 @@ inline Shape plan(long long rows, int C, const Call& c) {
   best.blocks = (int)(want < room ? want : room);
   return best;
 }
+// The kernels that plan() asks for, besides those for large rows and tiles; no others are built.  `big`: blocks of 512 forward.  Of
+// whole vectors one a thread never fills a warp, and two or three are dearer than four from there on unless four column sums leave
+// no registers for them (then three are not cheapest anywhere).  A gate for every row in fp32 leaves no shared memory for a ring
+// beside four vectors of 512 threads' parameters, nor for rows of four vectors beside four column sums.
+constexpr bool planned(bool backward, bool vec, bool wide, bool big, int vectors, int mode, bool by_pixel, int block) {
+  const bool both = mode == MODE_BOTH, room = !(by_pixel && block == 4);
+  if (!vec) return vectors == 4 ? big && (room || !both) : vectors == 1 || !spills(backward, mode, by_pixel);
+  if (big) return vectors == 4 && room;
+  if (!backward) return vectors > 2 || !wide;
+  return vectors == 1 ? !wide : vectors == 2 ? !wide || both : vectors == 3 ? !both : !both || (wide && room);
+}
 // rows [first_row(i), first_row(i + 1)) are slot i's, of all slots of all blocks; rows are at most 2^30
 __host__ __device__ inline int first_row(int rows, int slots, int i) {
   return rows / slots * i + (rows % slots < i ? rows % slots : i);
@@ -1269,43 +1280,44 @@ void launch_backward(const GeepsResidual& p, const Shape& s, const float2* means
   allow_shared(kernel, smem, done);
   geeps_launch(kernel, dim3(s.blocks), dim3(s.threads()), smem, st, p, s.slot, s.slots, s.depth, (int)s.ring, means);
 }
+// ... false: there is no such kernel
 template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool PIXEL>
-void launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
+bool launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
+  constexpr int B = sizeof(TB);
   if (backward) {
-    if constexpr (VEC || K == 1 || !spills(true, MODE, PIXEL)) launch_backward<TR, TB, K, VEC, WIDE, false, MODE, PIXEL>(p, s, nullptr, st);
-    return;
+    if constexpr (planned(true, VEC, WIDE, false, K, MODE, PIXEL, B)) { launch_backward<TR, TB, K, VEC, WIDE, false, MODE, PIXEL>(p, s, nullptr, st); return true; }
+  } else if (s.wide) {
+    if constexpr (K == 4 && WIDE && planned(false, VEC, WIDE, true, K, MODE, PIXEL, B)) { launch_forward<TR, TB, K, VEC, WIDE, false, true, MODE, PIXEL>(p, s, st); return true; }
+  } else {
+    if constexpr (planned(false, VEC, WIDE, false, K, MODE, PIXEL, B)) { launch_forward<TR, TB, K, VEC, WIDE, false, false, MODE, PIXEL>(p, s, st); return true; }
   }
-  if constexpr (K == 4 && VEC && WIDE) {
-    if (s.wide) { launch_forward<TR, TB, K, VEC, WIDE, false, true, MODE, PIXEL>(p, s, st); return; }
-  }
-  launch_forward<TR, TB, K, VEC, WIDE, false, false, MODE, PIXEL>(p, s, st);
+  return false;
 }
 template <typename TR, typename TB, int MODE, bool PIXEL>
-void launch(const GeepsResidual& p, const Shape& s, bool backward, bool vec, cudaStream_t st) {
+bool launch(const GeepsResidual& p, const Shape& s, bool backward, bool vec, cudaStream_t st) {
   const bool wide = s.slot >= 32;
   if (!vec) {
     if constexpr (MODE == MODE_BOTH) {         // the others' two parameters always fit
-      if (s.large) { launch_forward<TR, TB, 4, false, true, true, false, MODE, PIXEL>(p, s, st); return; }
+      if (s.large) { launch_forward<TR, TB, 4, false, true, true, false, MODE, PIXEL>(p, s, st); return true; }
     }
     if constexpr (MODE != MODE_NORM) {
-      if (s.wide && s.depth == 0) { launch_forward<TR, TB, 4, false, true, true, true, MODE, PIXEL>(p, s, st); return; }
+      if (s.wide && s.depth == 0) { launch_forward<TR, TB, 4, false, true, true, true, MODE, PIXEL>(p, s, st); return true; }
     }
-    if (s.wide) launch_forward<TR, TB, 4, false, true, false, true, MODE, PIXEL>(p, s, st);
-    else if (s.vectors == 2) launch_kernel<TR, TB, 2, false, true, MODE, PIXEL>(p, s, backward, st);
-    else if (wide) launch_kernel<TR, TB, 1, false, true, MODE, PIXEL>(p, s, backward, st);
-    else launch_kernel<TR, TB, 1, false, false, MODE, PIXEL>(p, s, backward, st);
-    return;
+    if (s.wide) return launch_kernel<TR, TB, 4, false, true, MODE, PIXEL>(p, s, backward, st);
+    if (s.vectors == 2) return launch_kernel<TR, TB, 2, false, true, MODE, PIXEL>(p, s, backward, st);
+    if (wide) return launch_kernel<TR, TB, 1, false, true, MODE, PIXEL>(p, s, backward, st);
+    return launch_kernel<TR, TB, 1, false, false, MODE, PIXEL>(p, s, backward, st);
   }
   if constexpr (MODE != MODE_NORM) {
-    if (s.large) { launch_forward<TR, TB, 4, true, true, true, false, MODE, PIXEL>(p, s, st); return; }
+    if (s.large) { launch_forward<TR, TB, 4, true, true, true, false, MODE, PIXEL>(p, s, st); return true; }
   }
-  if (s.vectors == 1) launch_kernel<TR, TB, 1, true, false, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 2 && wide) launch_kernel<TR, TB, 2, true, true, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 2) launch_kernel<TR, TB, 2, true, false, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 3 && wide) launch_kernel<TR, TB, 3, true, true, MODE, PIXEL>(p, s, backward, st);
-  else if (s.vectors == 3) launch_kernel<TR, TB, 3, true, false, MODE, PIXEL>(p, s, backward, st);
-  else if (wide) launch_kernel<TR, TB, 4, true, true, MODE, PIXEL>(p, s, backward, st);
-  else launch_kernel<TR, TB, 4, true, false, MODE, PIXEL>(p, s, backward, st);
+  if (s.vectors == 1) return launch_kernel<TR, TB, 1, true, false, MODE, PIXEL>(p, s, backward, st);
+  if (s.vectors == 2 && wide) return launch_kernel<TR, TB, 2, true, true, MODE, PIXEL>(p, s, backward, st);
+  if (s.vectors == 2) return launch_kernel<TR, TB, 2, true, false, MODE, PIXEL>(p, s, backward, st);
+  if (s.vectors == 3 && wide) return launch_kernel<TR, TB, 3, true, true, MODE, PIXEL>(p, s, backward, st);
+  if (s.vectors == 3) return launch_kernel<TR, TB, 3, true, false, MODE, PIXEL>(p, s, backward, st);
+  if (wide) return launch_kernel<TR, TB, 4, true, true, MODE, PIXEL>(p, s, backward, st);
+  return launch_kernel<TR, TB, 4, true, false, MODE, PIXEL>(p, s, backward, st);
 }
 inline Call call_of(const GeepsResidual& p, bool backward, bool vec) {
   const bool by_pixel = p.gate && p.gate_rows == p.rows;
@@ -1366,24 +1378,23 @@ void run_tiles(const GeepsResidual& p, const Shape& s, Call c, cudaStream_t st) 
   }
 }
 template <typename TR, typename TB, int MODE, bool PIXEL>
-void run_mode(const GeepsResidual& p, const Call& c, cudaStream_t st) {
+bool run_mode(const GeepsResidual& p, const Call& c, cudaStream_t st) {
   const Shape s = plan(p.rows, p.C, c);
-  if (s.tiles > 1) { run_tiles<TR, TB, MODE, PIXEL>(p, s, c, st); return; }
-  launch<TR, TB, MODE, PIXEL>(p, s, c.backward, c.vec, st);
+  if (s.tiles > 1) { run_tiles<TR, TB, MODE, PIXEL>(p, s, c, st); return true; }
+  if (!launch<TR, TB, MODE, PIXEL>(p, s, c.backward, c.vec, st)) return false;
   if (c.backward) join_sums<TB>(p, s, st);
+  return true;
 }
 template <typename TR, typename TB>
-void run(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) {
+bool run(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st) {
   const Call c = call_of(p, backward, vec);
-  if (p.mode == MODE_NORM) run_mode<TR, TB, MODE_NORM, false>(p, c, st);
-  else if (p.mode == MODE_JOIN && c.by_pixel) run_mode<TR, TB, MODE_JOIN, true>(p, c, st);
-  else if (p.mode == MODE_JOIN) run_mode<TR, TB, MODE_JOIN, false>(p, c, st);
-  else if (c.by_pixel) run_mode<TR, TB, MODE_BOTH, true>(p, c, st);
-  else run_mode<TR, TB, MODE_BOTH, false>(p, c, st);
+  if (p.mode == MODE_NORM) return run_mode<TR, TB, MODE_NORM, false>(p, c, st);
+  if (p.mode == MODE_JOIN) return c.by_pixel ? run_mode<TR, TB, MODE_JOIN, true>(p, c, st) : run_mode<TR, TB, MODE_JOIN, false>(p, c, st);
+  return c.by_pixel ? run_mode<TR, TB, MODE_BOTH, true>(p, c, st) : run_mode<TR, TB, MODE_BOTH, false>(p, c, st);
 }
 
-void run_bf16(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);
-void run_mixed(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);
-void run_fp32(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);
+bool run_bf16(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);
+bool run_mixed(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);
+bool run_fp32(const GeepsResidual& p, bool backward, bool vec, cudaStream_t st);
 
 }  // namespace rownorm

@@ -116,3 +116,16 @@ def test_dres_between_values_is_refused():
     assert L.lib().geeps_residual_backward(pack(x=A, dout=B, dres=D + 2, rows=4, c=8, stream_fp32=1), None) == -14
     assert L.lib().geeps_residual_backward(pack(x=A, dout=B, dres=D + 2, rows=4, c=8), None) == 1
     assert L.lib().geeps_residual_backward(pack(x=A + 2, dout=B + 4, dres=D + 4, rows=4, c=8, stream_fp32=1), None) == 1
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+@pytest.mark.parametrize("mode", [1, 2, 3])
+@pytest.mark.parametrize("vec", [1, 0])
+def test_there_is_a_kernel_for_every_width(backward, mode, vec):
+    """Only the kernels that some width asks for are built."""
+    lib, out, rows = L.lib(), (C.c_int * 10)(), 34993
+    for gate in ((0,) if mode == 1 else (0, 7, rows)):
+        for types in TYPES:
+            for c in range(8 if vec else 1, 16385, 8 if vec else 1):
+                if lib.geeps_norm_shape(C.c_longlong(rows), C.c_longlong(gate), c, mode, backward, vec, *types, out) != 0:
+                    raise AssertionError((gate, types, c, list(out)))
