@@ -20,9 +20,11 @@
 // second launch, in a fixed order: results repeat bit for bit.  Sums, statistics and parameters are fp32; an activation is
 // rounded once, when it is stored.  The norm in front of the next block is taken of h before that rounding.
 //
-// What bounds them: whole, aligned rows move at 75 to 90 % of the copy rate (50176 x 1024 bf16 forward 5.4 TB/s, backward 4.9), the
-// rest being issue slots and the meeting of a row's warps with few rows on an SM; odd widths and addresses go column by column and
-// are bound by instructions (29 % backward); calls of a few rows by the launch and one round trip to memory.
+// What bounds them, in parts of the copy rate: whole, aligned rows of 1024 bf16 channels move at 0.81 forward and 0.72 backward (50176
+// rows, 5.3 and 4.7 TB/s), of 576 at 0.66 and 0.76, the rest being issue slots, start and end, and the meeting of a row's warps with
+// few rows on an SM, which leaves 0.43 to 0.20 of 4096 channels and more backward.  Odd widths and addresses go column by column and
+// are bound by instructions (0.28 at 1003 channels backward); narrow rows with one gate for all by the launch that joins its shares
+// (125552 x 32 backward 0.19); calls of a few rows by the launch and one round trip to memory.
 #include "norm_kernels.cuh"
 
 using namespace rownorm;

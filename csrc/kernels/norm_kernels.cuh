@@ -64,15 +64,15 @@ inline size_t stage_bytes(const Call& c, const Shape& s) {
 // Backward, rows that no thread count holds with their column sums are cut into tiles of columns, with the row's means taken by a
 // launch of its own: it reads once more, but nothing spills (3325 x 8972 bf16, join and norm: 1765 us by one block a row; 2230 x
 // 8968: 147).
-// Rows that fit stay whole (2441 x 4096: 54 us, two tiles 85; 1220 x 8192: 89, 96), but for single columns of a join with a norm
-// behind it and no gate for every pixel, where 16 columns a thread do not fit in 128 registers (2438 x 4101 240 us, 151; 1249 x
-// 8001 169, 158).  A tile is as wide as a block has columns: narrower ones lose (8192 in eight: 184).
+// Rows that fit stay whole (2441 x 4096: 55 us, two tiles 85; 1220 x 8192: 89, 96), but for single columns of a join with a norm
+// behind it and no gate for every pixel, where 16 columns a thread do not fit in 128 registers (2438 x 4101 240 us, 149; 1249 x
+// 8001 169, 154).  A tile is as wide as a block has columns: narrower ones lose (8192 in eight: 184).
 constexpr int tile_columns(bool vec) { return vec ? 2 * kVec * 384 : kVec * 512; }
 constexpr bool spills(bool backward, int mode, bool by_pixel) { return backward && mode == MODE_BOTH && !by_pixel; }
 // How many vectors a thread has: more save what every thread does once a row, fewer leave no lane without work.  The costs are
 // instructions a row.  Eight threads a row at least, where there is so much: pieces of rows in a warp's access are whole lines then
 // (50176 x 64 backward 12 us, 21 with four).  A join with a norm behind it has four column sums: two vectors while they do
-// (50176 x 1024 backward 110 us, four vectors by half the threads 180).
+// (50176 x 1024 backward 115 us, four vectors by half the threads 180).
 inline Shape plan(long long rows, int C, const Call& c) {
   Shape best = {};
   best.tiles = 1;
@@ -565,7 +565,7 @@ __device__ __forceinline__ void normalise(const C_& cols, Slot& s, const GeepsNo
   if (norm.stats && active && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * row) = make_float2(mean, rstd);
 }
 // n = (f - mean) * rstd with the statistics at hand, the difference first: f * rstd - mean * rstd would be off by the rounding of
-// mean * rstd, however small n is.  Not zero where there is no column, but whatever it meets there is.
+// mean * rstd, however small n is (and takes an instruction less: a norm of 4882 x 4096 backward 44.5 us, 46.6).  Not zero where there is no column, but whatever it meets there is.
 template <int N>
 __device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
   const float2 r = both(st.y), m = both(-st.x);
