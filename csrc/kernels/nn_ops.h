@@ -142,7 +142,8 @@ int geeps_bn_forward_noalloc(const void* x, void* y, const float* gamma, const f
 
 // ---- norms over the channels of a row, before and after a residual block (no counterpart in the reference) ----
 // One row = one pixel or token.  kind: 0 none, 1 LayerNorm, 2 RMSNorm.  weight / bias: C floats or NULL (1 / 0).  stats:
-// {mean, rstd} of every row, written forward (or NULL there) and read backward.  dweight / dbias: C floats or NULL.
+// {mean, rstd} of every row, written forward (or NULL there) and read backward.  dweight / dbias: C floats or NULL.  Squares are
+// added in fp32: a row whose squares (of x - mean) come to more than 3.4e38 has rstd = 0.
 typedef struct GeepsNorm {
   const float* weight;
   const float* bias;

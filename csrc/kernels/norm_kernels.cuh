@@ -564,8 +564,9 @@ __device__ __forceinline__ void normalise(const C_& cols, Slot& s, const GeepsNo
   for (int i = 0; i < N; ++i) f[i] = mul2(f[i], both(rstd));
   if (norm.stats && active && s.t == 0) *reinterpret_cast<float2*>(norm.stats + 2LL * row) = make_float2(mean, rstd);
 }
-// n = (f - mean) * rstd with the statistics at hand, the difference first: f * rstd - mean * rstd would be off by the rounding of
-// mean * rstd, however small n is (and takes an instruction less: a norm of 4882 x 4096 backward 44.5 us, 46.6).  Not zero where there is no column, but whatever it meets there is.
+// n = (f - mean) * rstd with the statistics at hand, the difference first: f * rstd - mean * rstd takes an instruction less (a norm of
+// 4882 x 4096 backward 44.5 us, 46.6), but is off by the rounding of mean * rstd, however small n is.  Not zero where there is no
+// column, but whatever it meets there is.
 template <int N>
 __device__ __forceinline__ void normalised(float2 (&f)[N], float2 st) {
   const float2 r = both(st.y), m = both(-st.x);
@@ -925,7 +926,7 @@ residual_backward_kernel(const __grid_constant__ GeepsResidual p, int slot, int 
         if (MODE & MODE_NORM) stats[1][threadIdx.x] = *reinterpret_cast<const float2*>(p.pre.stats + 2LL * q);
         if (TILE && (MODE & MODE_JOIN) && p.post.kind) stats[TILE ? 2 : 0][threadIdx.x] = means[2LL * q];
         if (TILE && (MODE & MODE_NORM)) stats[TILE ? 3 : 0][threadIdx.x] = means[2LL * q + 1];
-      } else if (!WIDE) {                      // a row that is none must not be normalised as one of an image before, which may not be finite
+      } else if (!WIDE) {          // a row that is none must not be normalised as one of an image before, which may not be finite
         stats[0][threadIdx.x] = stats[1][threadIdx.x] = both(0.f);
       }
       __syncwarp();
@@ -1285,11 +1286,20 @@ template <typename TR, typename TB, int K, bool VEC, bool WIDE, int MODE, bool P
 bool launch_kernel(const GeepsResidual& p, const Shape& s, bool backward, cudaStream_t st) {
   constexpr int B = sizeof(TB);
   if (backward) {
-    if constexpr (planned(true, VEC, WIDE, false, K, MODE, PIXEL, B)) { launch_backward<TR, TB, K, VEC, WIDE, false, MODE, PIXEL>(p, s, nullptr, st); return true; }
+    if constexpr (planned(true, VEC, WIDE, false, K, MODE, PIXEL, B)) {
+      launch_backward<TR, TB, K, VEC, WIDE, false, MODE, PIXEL>(p, s, nullptr, st);
+      return true;
+    }
   } else if (s.wide) {
-    if constexpr (K == 4 && WIDE && planned(false, VEC, WIDE, true, K, MODE, PIXEL, B)) { launch_forward<TR, TB, K, VEC, WIDE, false, true, MODE, PIXEL>(p, s, st); return true; }
+    if constexpr (K == 4 && WIDE && planned(false, VEC, WIDE, true, K, MODE, PIXEL, B)) {
+      launch_forward<TR, TB, K, VEC, WIDE, false, true, MODE, PIXEL>(p, s, st);
+      return true;
+    }
   } else {
-    if constexpr (planned(false, VEC, WIDE, false, K, MODE, PIXEL, B)) { launch_forward<TR, TB, K, VEC, WIDE, false, false, MODE, PIXEL>(p, s, st); return true; }
+    if constexpr (planned(false, VEC, WIDE, false, K, MODE, PIXEL, B)) {
+      launch_forward<TR, TB, K, VEC, WIDE, false, false, MODE, PIXEL>(p, s, st);
+      return true;
+    }
   }
   return false;
 }
