@@ -148,6 +148,34 @@ int geeps_gemm_pair_supported(const GeepsGemmParams* p);
 // Returns 0 if the tcgen05 path does not accept p.
 typedef struct GeepsGemmPlan { int pair, block_n, split_k, cluster; long long tiles; } GeepsGemmPlan;
 int geeps_gemm_plan(const GeepsGemmParams* p, GeepsGemmPlan* out);
+
+// ---- 8-bit matrices: e4m3 with a scale 2^e for each block of 128 columns of a row (no counterpart in the reference) ----
+// q: rows of `ld` bytes, ld a multiple of 16, begins at a multiple of 16.  scale: E8M0 bytes (e + 127) in atoms of 512 bytes for
+// 128 rows x 4 blocks, [ceil(rows / 128)][ceil(cols / 512)][512], byte (r % 32) * 16 + (r % 128 / 32) * 4 + block % 4, at a multiple of 16.
+// A block with a value that is not finite has the scale 0xff and stands for NaN.
+// Cast of x [rows, cols] (bf16 or fp32, pitch ldx): e is the smallest with no value above 448 in the block, values are rounded to
+// nearest even.  q, scale: x itself; qt, scale_t: x transposed, [cols, rows], with blocks of 128 rows of x; either may be NULL.
+// tile: one scale for 128 x 128 values, for both.  Values behind the last column of a row are written as zeros up to a multiple of 16.
+typedef struct GeepsQuantizeFp8 {
+  const void* x;
+  void *q, *qt;
+  unsigned char *scale, *scale_t;
+  long long rows, cols, ldx, ldq, ldqt;
+  int fp32, tile;
+} GeepsQuantizeFp8;
+int geeps_quantize_fp8(const GeepsQuantizeFp8* p, void* stream);
+// C[M,N] = A[M,K] * B[N,K]^T + bias[n], ReLU; A and B as above, C bf16 or fp32 with any pitch.
+typedef struct GeepsGemmFp8 {
+  const void *A, *B;
+  const unsigned char *scale_a, *scale_b;
+  void* C;
+  const float* bias;
+  int* status;
+  long long M, N, K, lda, ldb, ldc;
+  int out_fp32, relu;
+  int bn, cluster, swap;       // bn 0: chosen.  Tile width (64, 128, 192, or 32 where one tile is enough); CTAs that share K; B's rows on the 128-row side
+} GeepsGemmFp8;
+int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream);
 int geeps_clear_f32(float* c, long long n, void* stream);           // n zeros
 // C[m][n] = beta * C[m][n] (exactly 0 when beta == 0) over an M x N view with pitch ldc
 int geeps_scale_matrix_f32(float* c, long long M, long long N, long long ldc, float beta, void* stream);

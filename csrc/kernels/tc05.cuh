@@ -374,4 +374,47 @@ __device__ __forceinline__ void mma_ktile_warp_pair(uint32_t tmem_d, uint32_t a_
       : "memory");
 }
 
+// ---------------- 8-bit products with block scales (kind::mxf8f6f4) ----------------
+// A row has one E8M0 scale for each MMA of 32 bytes of K.  Scales of 128 rows x 4 K blocks are an atom of 512 bytes, byte
+// (r % 32) * 16 + (r / 32) * 4 + block: in TMEM 4 columns, row r in lane r % 32 (and its three copies) of column r / 32.
+// 512 contiguous bytes from global to shared memory; both addresses and the size are multiples of 16
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+// shared-memory descriptor of an atom: 32 rows of 16 bytes, no swizzle, groups of eight rows 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// an atom from shared memory to 4 columns of TMEM, in all four lane quarters; one thread; before this thread's later MMAs
+__device__ __forceinline__ void scale_copy(uint32_t tmem, uint32_t smem_addr) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(scale_desc(smem_addr)) : "memory");
+}
+// Instruction descriptor: A and B e4m3, both K-major, E8M0 scales, fp32 accumulation.
+//   [4,6) byte of B's scale word  [17,23) N >> 3  [23] scales are E8M0  [27,29) M >> 7  [29,31) byte of A's scale word
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int m, int n) {
+  return ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t idesc_scale_byte(uint32_t b) { return (b << 4) | (b << 29); }
+// One k-tile of 128 bytes: four MMAs by the elected lane of a converged warp, then the commit that frees the stage.
+__device__ __forceinline__ void mma_ktile_e4m3(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc,
+                                               uint32_t sfa, uint32_t sfb, uint32_t accumulate, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred p, q, t;\n\t.reg .b32 a, b;\n\t.reg .b64 da, db;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %7, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %4, [%5], [%6], p;\n\t"
+      "add.u32 a, %1, 2;\n\tadd.u32 b, %2, 2;\n\tmov.b64 da, {a, %3};\n\tmov.b64 db, {b, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %4, [%5], [%6], t;\n\t"
+      "add.u32 a, a, 2;\n\tadd.u32 b, b, 2;\n\tmov.b64 da, {a, %3};\n\tmov.b64 db, {b, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %4, [%5], [%6], t;\n\t"
+      "add.u32 a, a, 2;\n\tadd.u32 b, b, 2;\n\tmov.b64 da, {a, %3};\n\tmov.b64 db, {b, %3};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %4, [%5], [%6], t;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%8];\n\t}"
+      ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(bar)
+      : "memory");
+}
+
 }  // namespace tc05

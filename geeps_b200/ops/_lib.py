@@ -133,6 +133,19 @@ class U8Transform(C.Structure):
 RESIDUAL = struct.Struct("@13P 5Pfi 5Pfi 12q 5i4x")
 
 
+class QuantizeFp8(C.Structure):
+    """Mirror of GeepsQuantizeFp8 (csrc/kernels/kernels.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "q", "qt", "scale", "scale_t")]
+                + [(n, C.c_longlong) for n in ("rows", "cols", "ldx", "ldq", "ldqt")] + [(n, C.c_int) for n in ("fp32", "tile")])
+
+
+class GemmFp8(C.Structure):
+    """Mirror of GeepsGemmFp8 (csrc/kernels/kernels.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("A", "B", "scale_a", "scale_b", "C", "bias", "status")]
+                + [(n, C.c_longlong) for n in ("M", "N", "K", "lda", "ldb", "ldc")]
+                + [(n, C.c_int) for n in ("out_fp32", "relu", "bn", "cluster", "swap")])
+
+
 class Tensors(C.Structure):
     """Mirror of GeepsTensors (csrc/kernels/nn_ops.h)."""
     _fields_ = [("n", C.c_longlong), ("ptr", C.c_void_p), ("count", C.c_void_p), ("fp32", C.c_void_p), ("order", C.c_void_p)]

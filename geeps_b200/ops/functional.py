@@ -702,3 +702,99 @@ def clip_gradients(grads, max_norm: float, result: torch.Tensor, out=None, work=
     L.hold((grads, out))
     launch(lib().geeps_clip_gradients, "clip_gradients", C.byref(grads.native), None if out is None else C.byref(out.native),
            C.c_double(max_norm), ptr(result), ptr(work), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+
+
+# ---- matrices in 8 bits with a scale for each block of 128, and their products ----
+class Fp8Matrix:
+    """A matrix [rows, cols] in e4m3 with a scale 2^e for every 128 columns of a row: `q` (float8_e4m3fn, rows on a pitch of a
+    multiple of 16) and `scale` (E8M0 bytes, 512 for 128 rows x 4 blocks, in the order in which the tensor cores take them).
+    quantize_fp8() fills it, matmul_fp8() multiplies it."""
+    __slots__ = ("rows", "cols", "q", "scale")
+
+    def __init__(self, rows: int, cols: int, device):
+        _need(0 <= rows < 1 << 30 and 0 < cols < 1 << 30, f"Fp8Matrix: need 0 to 2^30 rows and 1 to 2^30 columns, got {rows} x {cols}")
+        self.rows, self.cols = rows, cols
+        self.q = torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
+        self.scale = torch.zeros((rows + 127) // 128, (cols + 511) // 512, 512, dtype=torch.uint8, device=device)
+
+    def exponents(self) -> torch.Tensor:
+        """e + 127 of every block, uint8 [rows, ceil(cols / 128)]; 255 where the block stands for NaN."""
+        a, b = self.scale.shape[:2]
+        return self.scale.view(a, b, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(a * 128, b * 4)[:self.rows, :(self.cols + 127) // 128]
+
+    def dequantize(self) -> torch.Tensor:
+        """What the matrix stands for, in fp32 (for inspection and tests)."""
+        e = self.exponents().to(torch.int32)
+        scale = torch.where(e == 255, float("nan"), torch.exp2(e.double() - 127.0)).float()
+        return self.q.float() * scale.repeat_interleave(128, 1)[:, :self.cols]
+
+
+def _fp8(m, dev, shape, what):
+    _need(isinstance(m, Fp8Matrix) and (m.rows, m.cols) == shape and m.q.get_device() == dev,
+          f"{what}: need an Fp8Matrix {list(shape)} on cuda:{dev}")
+    return m
+
+
+def _rows(t, dev, what) -> int:
+    """Pitch of a bf16 or fp32 matrix on the device whose rows are contiguous."""
+    _need(t.dim() == 2 and t.dtype in (bf16, torch.float32) and t.get_device() == dev, f"{what}: need a bf16 or fp32 matrix on cuda:{dev}")
+    _need(t.stride(1) == 1 or t.shape[1] == 1, f"{what}: columns must be contiguous, got strides {t.stride()}")
+    pitch = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    _need(pitch >= t.shape[1], f"{what}: rows overlap, got strides {t.stride()}")
+    return pitch
+
+
+def _current_device(t, what) -> int:
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        L.require_cuda()
+        raise ValueError(f"{what}: tensors are on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return dev
+
+
+def quantize_fp8(x: torch.Tensor, out: "Fp8Matrix | None" = None, *, transposed: "Fp8Matrix | None" = None, tile: bool = False):
+    """Cast x [rows, cols] (bf16 or fp32, rows of any pitch) into `out` and, or only, x transposed into `transposed` [cols, rows],
+    whose blocks are 128 rows of x.  tile: one scale for 128 x 128 values (for weights, whose transpose then has the same values).
+    A block's scale is the least 2^e with no value above 448; a block with a value that is not finite stands for NaN.  With neither
+    a new `out` is made.  Returns out, or transposed where it is the only one."""
+    dev = _current_device(x, "quantize_fp8")
+    ldx = _rows(x, dev, "quantize_fp8: x")
+    rows, cols = x.shape
+    _need(cols > 0, "quantize_fp8: x has no columns")
+    if out is None and transposed is None:
+        out = L.hold(Fp8Matrix(rows, cols, x.device))
+    p = L.QuantizeFp8()
+    p.x, p.rows, p.cols, p.ldx, p.fp32, p.tile = x.data_ptr(), rows, cols, ldx, x.dtype is torch.float32, bool(tile)
+    if out is not None:
+        _fp8(out, dev, (rows, cols), "quantize_fp8: out")
+        p.q, p.scale, p.ldq = out.q.data_ptr(), out.scale.data_ptr(), (cols + 15) // 16 * 16
+    if transposed is not None and rows:
+        _fp8(transposed, dev, (cols, rows), "quantize_fp8: transposed")
+        p.qt, p.scale_t, p.ldqt = transposed.q.data_ptr(), transposed.scale.data_ptr(), (rows + 15) // 16 * 16
+    launch(lib().geeps_quantize_fp8, "quantize_fp8", C.byref(p), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+    return transposed if out is None else out
+
+
+def matmul_fp8(a: "Fp8Matrix", b: "Fp8Matrix", out: torch.Tensor, *, bias: torch.Tensor | None = None, relu: bool = False,
+               status: torch.Tensor | None = None, plan=(0, 0, 0)) -> torch.Tensor:
+    """out[M,N] = a[M,K] @ b[N,K]^T + bias, ReLU; out bf16 or fp32 with rows of any pitch, bias fp32 [N].  Products are exact and
+    added in fp32.  plan: (tile width, CTAs that share K, operands swapped) instead of the choice by the sizes."""
+    dev = _current_device(out, "matmul_fp8")
+    ldc = _rows(out, dev, "matmul_fp8: out")
+    M, N = out.shape
+    _need(isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix) and a.cols == b.cols, "matmul_fp8: need two Fp8Matrix of as many columns")
+    _fp8(a, dev, (M, a.cols), "matmul_fp8: a")
+    _fp8(b, dev, (N, a.cols), "matmul_fp8: b")
+    p = L.GemmFp8()
+    p.A, p.B, p.scale_a, p.scale_b, p.C = a.q.data_ptr(), b.q.data_ptr(), a.scale.data_ptr(), b.scale.data_ptr(), out.data_ptr()
+    if bias is not None:
+        _need(bias.dtype is torch.float32 and bias.shape == (N,) and bias.is_contiguous() and bias.get_device() == dev,
+              f"matmul_fp8: bias needs {N} contiguous fp32 values on cuda:{dev}")
+        p.bias = bias.data_ptr()
+    p.status = status.data_ptr() if status is not None else None
+    p.M, p.N, p.K, p.ldc = M, N, a.cols, ldc
+    p.lda = p.ldb = (a.cols + 15) // 16 * 16
+    p.out_fp32, p.relu = out.dtype is torch.float32, bool(relu)
+    p.bn, p.cluster, p.swap = plan
+    launch(lib().geeps_gemm_fp8, "matmul_fp8", C.byref(p), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+    return out
