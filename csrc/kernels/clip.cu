@@ -10,7 +10,7 @@
 // Up to kOneBlock values take one launch of one block, which keeps them in registers.  The tensors' table travels in the launch
 // arguments, so a call keeps nothing on the device.
 #include "common.cuh"
-#include "nn_ops.h"
+#include "tensor_list.h"
 
 typedef __nv_bfloat16 bf16;
 
@@ -367,35 +367,6 @@ int clip(const GeepsTensors& src, const GeepsTensors* dst, double max_norm, floa
   return (int)cudaGetLastError();
 }
 
-// Is there a tensor of `a` that shares memory with one of `b` (a itself: with another of its own)?  Both are sorted by address
-// and each without overlaps, so one merge finds it.  dst[i] may be src[i].
-struct Range { uintptr_t from, to; };
-Range range(const GeepsTensors& t, long long i) {
-  const uintptr_t p = (uintptr_t)t.ptr[i];
-  return {p, p + (uintptr_t)t.count[i] * (t.fp32[i] ? 4 : 2)};
-}
-bool overlaps_itself(const GeepsTensors& t) {
-  uintptr_t end = 0;
-  for (long long k = 0; k < t.n; ++k) {
-    const Range r = range(t, t.order[k]);
-    if (r.from == r.to) continue;
-    if (r.from < end) return true;
-    end = r.to;
-  }
-  return false;
-}
-bool overlaps(const GeepsTensors& a, const GeepsTensors& b) {
-  long long i = 0, j = 0;
-  while (i < a.n && j < b.n) {
-    const long long x = a.order[i], y = b.order[j];
-    const Range p = range(a, x), q = range(b, y);
-    const bool same = x == y && p.from == q.from && a.fp32[x] == b.fp32[y];
-    if (p.from < q.to && q.from < p.to && p.from != p.to && q.from != q.to && !same) return true;
-    if (p.to < q.to) ++i; else ++j;
-  }
-  return false;
-}
-
 }  // namespace
 
 extern "C" long long geeps_clip_work(const GeepsTensors* src) { return (pieces(src->n) + 1) * geeps_sm_count() * kSquareBlocks; }
@@ -407,14 +378,11 @@ extern "C" int geeps_clip_gradients(const GeepsTensors* src, const GeepsTensors*
     if (src->count[i] < 0 || (dst && dst->count[i] != src->count[i])) return (int)cudaErrorInvalidValue;
     if (src->count[i] && (!src->ptr[i] || (dst && !dst->ptr[i]))) return (int)cudaErrorInvalidValue;
   }
-  bool between = ((uintptr_t)result & 3) || ((uintptr_t)work & 7);
-  for (long long i = 0; i < src->n; ++i)
-    if (src->count[i]) between |= ((uintptr_t)src->ptr[i] & (src->fp32[i] ? 3 : 1)) || (dst && ((uintptr_t)dst->ptr[i] & (dst->fp32[i] ? 3 : 1)));
-  if (between) return GEEPS_ERR_CLIP_ALIGN;
-  if (overlaps_itself(*src) || (dst && (overlaps_itself(*dst) || overlaps(*src, *dst)))) return GEEPS_ERR_CLIP_OVERLAP;
+  if (((uintptr_t)result & 3) || ((uintptr_t)work & 7) || tensors_between(*src) || (dst && tensors_between(*dst))) return GEEPS_ERR_CLIP_ALIGN;
+  if (tensors_overlap(*src) || (dst && (tensors_overlap(*dst) || tensors_overlap(*src, *dst)))) return GEEPS_ERR_CLIP_OVERLAP;
   const uintptr_t r = (uintptr_t)result, w = (uintptr_t)work, we = w + geeps_clip_work(src) * sizeof(double);
-  auto meets = [&](const Range& q) { return q.from != q.to && ((q.from < r + 8 && r < q.to) || (q.from < we && w < q.to)); };
-  for (long long i = 0; i < src->n; ++i) if (meets(range(*src, i)) || (dst && meets(range(*dst, i)))) return GEEPS_ERR_CLIP_OVERLAP;
+  auto meets = [&](const TensorRange& q) { return q.from != q.to && ((q.from < r + 8 && r < q.to) || (q.from < we && w < q.to)); };
+  for (long long i = 0; i < src->n; ++i) if (meets(tensor_range(*src, i)) || (dst && meets(tensor_range(*dst, i)))) return GEEPS_ERR_CLIP_OVERLAP;
   if (r < we && w < r + 8) return GEEPS_ERR_CLIP_OVERLAP;
   cudaStream_t st = (cudaStream_t)stream;
   long long total = 0;

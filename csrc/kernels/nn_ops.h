@@ -212,6 +212,33 @@ long long geeps_clip_work(const GeepsTensors* src);
 int geeps_clip_gradients(const GeepsTensors* src, const GeepsTensors* dst, double max_norm, float* result, double* work,
                          void* stream);
 
+// ---- AdamW over many tensors (worker-side optimizer; the reference's workers had theirs in the absent Caffe application) ----
+// g = c g; m = beta1 m + (1 - beta1) g; v = beta2 v + (1 - beta2) g^2;
+// change = -lr ((m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay p)
+// with c = norm > max_norm ? max_norm / norm : 1 (norm NULL: 1), weight_decay for tensors with decay[i] only, t = steps[0] + 1.
+// p += change, or out = change with p as it was; out[i] may be grads[i].  States of tensor i begin at value 128 x (sum of
+// ceil(count / 128) of the tensors before it).  bits 32: m and v are fp32.  bits 8: codes (adamw.cu) with two exponent bytes (m's and
+// v's) for 128 values; `blocks` of 128 are there.  stochastic: codes, and parameters in bf16, are rounded at random by the seed;
+// else to nearest even.  lr_ref: the learning rate on the device, instead of lr.  steps: {steps taken, 0}, moved on by the call.
+// Errors as those of clipping: a tensor, state or scalar between two values (m and v: of 16 bytes in 32 bits, of 4 in 8), or one
+// that is written and shares memory with another.
+typedef struct GeepsAdamW {
+  const GeepsTensors *params, *grads, *out;
+  const unsigned char* decay;
+  void *m, *v;
+  unsigned char* exponents;
+  unsigned long long* steps;
+  const float *lr_ref, *norm;
+  double beta1, beta2;
+  unsigned long long seed;
+  long long blocks;
+  float lr, eps, weight_decay, max_norm;
+  int bits, stochastic;
+} GeepsAdamW;
+int geeps_adamw(const GeepsAdamW* k, void* stream);
+// codes of m (second 0) or v (1) as the values they stand for, bf16 (which holds them exactly) or fp32
+int geeps_adamw_moments(const unsigned char* codes, const unsigned char* exponents, void* out, int second, int fp32, long long blocks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

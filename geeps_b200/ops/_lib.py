@@ -151,6 +151,13 @@ class Tensors(C.Structure):
     _fields_ = [("n", C.c_longlong), ("ptr", C.c_void_p), ("count", C.c_void_p), ("fp32", C.c_void_p), ("order", C.c_void_p)]
 
 
+class AdamW(C.Structure):
+    """Mirror of GeepsAdamW (csrc/kernels/nn_ops.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("params", "grads", "out", "decay", "m", "v", "exponents", "steps", "lr_ref", "norm")]
+                + [("beta1", C.c_double), ("beta2", C.c_double), ("seed", C.c_ulonglong), ("blocks", C.c_longlong)]
+                + [(n, C.c_float) for n in ("lr", "eps", "weight_decay", "max_norm")] + [("bits", C.c_int), ("stochastic", C.c_int)])
+
+
 # what the argument checks of native calls answer besides CUDA's error codes
 REFUSALS = {-10: "a row has 1 to 16384 channels", -11: "the gate's rows do not divide the rows",
             -12: "an output overlaps another operand", -13: "tensors overlap",

@@ -704,6 +704,97 @@ def clip_gradients(grads, max_norm: float, result: torch.Tensor, out=None, work=
            C.c_double(max_norm), ptr(result), ptr(work), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
 
 
+# ---- AdamW over many tensors ----
+class AdamWState:
+    """What an AdamW optimizer keeps for a list of parameters (GradList or sequence of fp32 or bf16 tensors): their first and second
+    moments in 32 bits (`m`, `v`: fp32) or 8 (`m`, `v`: codes, `exponents`: two bytes for 128 values; adamw_moments() reads them) and
+    the number of steps taken, on the device (`steps`), so that a captured step can be replayed.  The moments of parameter i are the
+    values offsets[i] to offsets[i] + count of m and v.  decay: whether weight decay applies, for each parameter (None: to all).
+    To save and restore: m, v, exponents and steps."""
+
+    def __init__(self, params, bits: int = 32, decay=None, steps: int = 0):
+        self.params = params if isinstance(params, GradList) else GradList(params)
+        _need(self.params.tensors and bits in (8, 32), f"AdamWState: need at least one parameter and 8 or 32 bits, got {bits}")
+        decay = [True] * len(self.params.tensors) if decay is None else [bool(d) for d in decay]
+        _need(len(decay) == len(self.params.tensors), "AdamWState: decay needs a truth value for each parameter")
+        _need(steps >= 0, "AdamWState: steps must not be negative")
+        self.bits, self.decay, self.offsets, at = bits, decay, [], 0
+        for n in self.params.numel:
+            self.offsets.append(at)
+            at += (n + 127) // 128 * 128
+        self.blocks, dev = at // 128, self.params.device
+        dtype = torch.uint8 if bits == 8 else torch.float32
+        self.m, self.v = torch.zeros(at, dtype=dtype, device=dev), torch.zeros(at, dtype=dtype, device=dev)
+        self.exponents = torch.full((self.blocks, 2), 32, dtype=torch.uint8, device=dev) if bits == 8 else None
+        self.steps = torch.tensor([steps, 0], dtype=torch.int64, device=dev)     # the second is the kernel's own
+        self._decay = (C.c_ubyte * len(decay))(*decay)
+
+    def _check(self):
+        """m, v and the others may have been replaced (a restored run): they must still be what the kernel is told they are."""
+        dev, n = self.params.device, self.blocks * 128
+        dtype = torch.uint8 if self.bits == 8 else torch.float32
+        for t, shape, kind in ((self.m, (n,), dtype), (self.v, (n,), dtype), (self.steps, (2,), torch.int64)) + (
+                ((self.exponents, (self.blocks, 2), torch.uint8),) if self.bits == 8 else ()):
+            _need(t.dtype is kind and t.shape == shape and t.is_contiguous() and t.device == dev,
+                  f"AdamWState: m, v, exponents or steps need {kind} {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def adamw_step(params, grads, state: AdamWState, lr, *, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0, out=None,
+               clip=None, seed: int | None = None) -> None:
+    """One AdamW step of all parameters: g = c g, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2,
+    change = -lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + eps) + weight_decay p), p += change.
+    params, grads, out: GradList or sequence of tensors (fp32 or bf16 each) with equal counts.  out: receives the change, and the
+    parameters stay as they are (what an additive table's update takes); out may be grads.  lr: a number, or an fp32 tensor of one value
+    on the device, which a captured step then reads.  clip: (norm, max_norm) with the result of clip_gradients(grads, inf, norm): c =
+    max_norm / norm where the norm exceeds max_norm.  seed: round 8-bit states and bf16 parameters up or down at random, by bits that
+    are a function of seed, step and place, so that small changes are not lost; None: to the nearest.  A gradient that is not finite makes
+    its parameter's states so, with states in 8 bits those of its neighbours (128 values) useless."""
+    params = params if isinstance(params, GradList) else GradList(params)
+    grads = grads if isinstance(grads, GradList) else GradList(grads)
+    out = out if out is None or isinstance(out, GradList) else GradList(out)
+    dev = _current_device(state.m, "adamw_step")
+    for t in (params, grads, out):
+        _need(t is None or (t.numel == state.params.numel and t.device.index == dev),
+              "adamw_step: params, grads and out need the state's counts, on the current device")
+    state._check()
+    beta1, beta2 = betas
+    _need(0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0 and weight_decay >= 0, "adamw_step: need betas from 0 to below 1, eps and weight_decay from 0 up")
+    k = L.AdamW()
+    k.params, k.grads, k.out = C.addressof(params.native), C.addressof(grads.native), None if out is None else C.addressof(out.native)
+    k.decay, k.m, k.v, k.steps = C.addressof(state._decay), state.m.data_ptr(), state.v.data_ptr(), state.steps.data_ptr()
+    k.exponents = None if state.exponents is None else state.exponents.data_ptr()
+    if isinstance(lr, torch.Tensor):
+        _need(lr.dtype is torch.float32 and lr.numel() == 1 and lr.get_device() == dev, f"adamw_step: lr needs one fp32 value on cuda:{dev}")
+        k.lr_ref = lr.data_ptr()
+    else:
+        k.lr = lr
+    if clip is not None:
+        norm, max_norm = clip
+        _need(norm.dtype is torch.float32 and norm.numel() >= 1 and norm.is_contiguous() and norm.get_device() == dev,
+              f"adamw_step: the norm needs fp32 on cuda:{dev}")
+        _need(max_norm >= 0, f"adamw_step: max_norm must be a number from 0 up, got {max_norm}")
+        k.norm, k.max_norm = norm.data_ptr(), max_norm
+    k.beta1, k.beta2, k.eps, k.weight_decay = beta1, beta2, eps, weight_decay
+    k.blocks, k.bits, k.stochastic, k.seed = state.blocks, state.bits, seed is not None, 0 if seed is None else seed & 0xFFFFFFFFFFFFFFFF
+    L.hold((params, grads, out, state, lr, clip))
+    launch(lib().geeps_adamw, "adamw_step", C.byref(k), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+
+
+def adamw_moments(state: AdamWState, m: torch.Tensor, v: torch.Tensor):
+    """The moments that a state in 8 bits stands for, into m and v (contiguous, bf16, which holds them exactly, or fp32, as many
+    values as state.m).  Returns (m, v)."""
+    _need(state.bits == 8, "adamw_moments: a state in 32 bits has its moments in m and v")
+    dev = _current_device(state.m, "adamw_moments")
+    state._check()
+    for t in (m, v):
+        _need(t.dtype in (bf16, torch.float32) and t.shape == state.m.shape and t.is_contiguous() and t.get_device() == dev,
+              f"adamw_moments: need {state.m.numel()} contiguous bf16 or fp32 values on cuda:{dev}")
+    for i, (codes, t) in enumerate(((state.m, m), (state.v, v))):
+        launch(lib().geeps_adamw_moments, "adamw_moments", ptr(codes), ptr(state.exponents), ptr(t), i, int(t.dtype is torch.float32),
+               C.c_longlong(state.blocks), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+    return m, v
+
+
 # ---- matrices in 8 bits with a scale for each block of 128, and their products ----
 class Fp8Matrix:
     """A matrix [rows, cols] in e4m3 with a scale 2^e for every 128 columns of a row: `q` (float8_e4m3fn, rows on a pitch of a
