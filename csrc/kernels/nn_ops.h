@@ -192,6 +192,30 @@ int geeps_norm_shape(long long rows, long long gate_rows, int C, int mode, int b
 // launch) and y, threads that share the parts of an image's gate gradient, slots that leave one part of it
 int geeps_norm_sums_shape(long long rows, long long gate_rows, int C, int mode, int vec, int stream_fp32, int block_fp32, int* out);
 
+// ---- group norm with its activation, channels last (no counterpart in the reference) ----
+// Rows are the pixels of image after image.  z = ((x - mean) rstd) weight + bias over the pixels x channels of a group of an
+// image, y = act(z); act: 0 none, 1 ReLU, 2 SiLU.  weight / bias: C floats or NULL (1 / 0).  stats: {mean, rstd} [images][groups],
+// written forward (or NULL there) and read backward.  Backward: dx, and dweight / dbias (C floats, or NULL).  x_fp32: x and dx are
+// fp32, else bf16; y_fp32 (with x_fp32 only): y and dy.  work: geeps_group_norm_work() floats at a multiple of 8 bytes, private to the
+// call while it runs.  Pitches in elements.  An output may be the very same rows as an input of its size, or other channels of
+// the same wider rows; any other overlap of what is written is refused.  images x pixels is at most 2^30, C 1 to 16384.
+#define GEEPS_ERR_GROUPS (-16)
+typedef struct GeepsGroupNorm {
+  const void *x, *dy;
+  void *y, *dx;
+  const float *weight, *bias;
+  float *stats, *work, *dweight, *dbias;
+  long long images, pixels, ldx, lddy, ldy, lddx;
+  int C, groups, act, x_fp32, y_fp32;
+  float eps;
+} GeepsGroupNorm;
+long long geeps_group_norm_work(long long images, long long pixels, int C, int groups);
+int geeps_group_norm_forward(const GeepsGroupNorm* p, void* stream);
+int geeps_group_norm_backward(const GeepsGroupNorm* p, void* stream);
+// launch shape (host arithmetic only), eight values: one launch of clusters or two launches, channels of a slice, chunks of an image,
+// pixels of a chunk, pixels that a thread keeps, blocks, bytes of shared memory, threads
+int geeps_group_norm_shape(long long images, long long pixels, int C, int groups, int backward, int vec, int x_fp32, int y_fp32, int* out);
+
 // ---- clipping of gradients by their global norm (the reference's solver had it in its absent Caffe application) ----
 // norm = sqrt(sum over all tensors of g^2), c = norm > max_norm ? max_norm / norm : 1, dst = c * g; dst NULL: in place, and
 // then nothing is written while c is 1.  result: {norm, c}.  Tensors are dense, fp32 or bf16 each; dst[i] has src[i]'s

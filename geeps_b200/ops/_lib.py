@@ -133,6 +133,11 @@ class U8Transform(C.Structure):
 RESIDUAL = struct.Struct("@13P 5Pfi 5Pfi 12q 5i4x")
 
 
+# GeepsGroupNorm (csrc/kernels/nn_ops.h) as packed bytes: x, dy, y, dx, weight, bias, stats, work, dweight, dbias; images, pixels, four
+# pitches (x, dy, y, dx); C, groups, act, x_fp32, y_fp32, eps
+GROUP_NORM = struct.Struct("@10P 6q 5if")
+
+
 class QuantizeFp8(C.Structure):
     """Mirror of GeepsQuantizeFp8 (csrc/kernels/kernels.h)."""
     _fields_ = ([(n, C.c_void_p) for n in ("x", "q", "qt", "scale", "scale_t")]
@@ -162,7 +167,7 @@ class AdamW(C.Structure):
 REFUSALS = {-10: "a row has 1 to 16384 channels", -11: "the gate's rows do not divide the rows",
             -12: "an output overlaps another operand", -13: "tensors overlap",
             -14: "stats and work must begin on a multiple of 8 bytes, other operands on one of their size",
-            -15: "a tensor, the result or the workspace begins between two values"}
+            -15: "a tensor, the result or the workspace begins between two values", -16: "the groups do not divide the channels"}
 
 _lib = None
 _launches = 0
@@ -172,7 +177,7 @@ def lib() -> C.CDLL:
     global _lib
     if _lib is None:
         _lib = _native.load()
-        _lib.geeps_residual_work.restype = _lib.geeps_clip_work.restype = C.c_longlong
+        _lib.geeps_residual_work.restype = _lib.geeps_clip_work.restype = _lib.geeps_group_norm_work.restype = C.c_longlong
     return _lib
 
 

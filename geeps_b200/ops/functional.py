@@ -643,6 +643,78 @@ def norm_work(rows: int, cols: int, gate_rows: int = 0, join: bool = False, pre:
     return lib().geeps_residual_work(C.c_longlong(rows), C.c_longlong(gate_rows), cols, (2 if join else 0) | (1 if pre else 0))
 
 
+# ---- group norm with its activation ----
+GROUP_ACTS = {None: 0, "relu": 1, "silu": 2}
+
+
+class GroupNorm:
+    """Arguments of one group norm: weight / bias fp32 [C] or None (1 / 0), stats fp32 [images, groups, 2] that receives mean and
+    1/std forward (None: not kept) and gives them backward, act None, "relu" or "silu", dweight / dbias fp32 [C] that receive the
+    parameters' gradients backward (None: not wanted)."""
+    __slots__ = ("groups", "weight", "bias", "stats", "eps", "act", "dweight", "dbias")
+
+    def __init__(self, groups: int, weight=None, bias=None, stats=None, eps: float = 1e-5, act: str | None = None, dweight=None, dbias=None):
+        if act not in GROUP_ACTS:
+            raise ValueError(f"unknown activation {act!r}; one of {', '.join(map(str, GROUP_ACTS))}")
+        if not (groups >= 1 and eps >= 0):
+            raise ValueError(f"a group norm needs groups from 1 up and eps from 0 up, got {groups} and {eps}")
+        self.groups, self.weight, self.bias, self.stats, self.eps, self.act, self.dweight, self.dbias = groups, weight, bias, stats, eps, act, dweight, dbias
+
+
+def _group_norm(label, x, y, dy, dx, images, norm, work):
+    if x.dim() != 2:
+        raise ValueError(f"{label}: need [rows, channels], got {list(x.shape)}")
+    dev = _current_device(x, label)
+    rows, cols = x.shape
+    out, f32 = dx if dy is not None else y, torch.float32
+    xt, yt = x.dtype, (dy if dy is not None else y).dtype
+    if not ((xt is bf16 or xt is f32) and (yt is bf16 or (yt is f32 and xt is f32))):
+        raise ValueError(f"{label}: types must be bf16, fp32, or fp32 x and dx with bf16 y and dy; got {xt}, {yt}")
+    if images < 0 or (rows if images == 0 else rows % images):
+        raise ValueError(f"{label}: {rows} rows are no whole pixels of {images} images")
+    ld = []
+    at = (_operand(x, dev, x.shape, xt, "x", ld), 0 if dy is None else _operand(dy, dev, x.shape, yt, "dy", ld),
+          _operand(out, dev, x.shape, yt if dy is None else xt, "y" if dy is None else "dx", ld))
+    st = norm.stats
+    if st is not None:
+        _need(st.dtype is f32 and st.shape == (images, norm.groups, 2) and st.is_contiguous() and st.get_device() == dev,
+              f"{label}: stats: need contiguous fp32 [{images}, {norm.groups}, 2] on cuda:{dev}")
+    else:
+        _need(dy is None, f"{label}: the backward pass needs the stats")
+    pixels = rows // images if images else 0
+    n = lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), cols, norm.groups)
+    if work is None:
+        work = L.hold(torch.empty(n, dtype=f32, device=x.device))
+    elif not (work.dtype is f32 and work.is_contiguous() and work.numel() >= n and work.get_device() == dev):
+        raise ValueError(f"{label}: work needs {n} contiguous fp32 values on cuda:{dev}")
+    w, b, dw, db = (0 if t is None else _column(t, dev, cols) for t in
+                    (norm.weight, norm.bias, norm.dweight if dy is not None else None, norm.dbias if dy is not None else None))
+    pitches = (ld[0], 0, ld[1], 0) if dy is None else (ld[0], ld[1], 0, ld[2])
+    launch(lib().geeps_group_norm_forward if dy is None else lib().geeps_group_norm_backward, label,
+           L.GROUP_NORM.pack(at[0], at[1], at[2] if dy is None else 0, 0 if dy is None else at[2], w, b, 0 if st is None else st.data_ptr(),
+                             work.data_ptr(), dw, db, images, pixels, *pitches, cols, norm.groups, GROUP_ACTS[norm.act], xt is f32,
+                             yt is f32, norm.eps),
+           C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
+
+
+def group_norm_forward(x, y, images: int, norm: GroupNorm, work=None) -> None:
+    """y = act(norm(x)): every group of neighbouring channels is normalised over all pixels of its image.  x: [images * pixels, C], bf16
+    or fp32; y: the same type, or bf16 beside fp32 x.  Any C up to 16384, any pitch; y may be x itself.  work: group_norm_work()
+    floats to use instead of memory taken from the allocator for the call."""
+    _group_norm("group_norm_forward", x, y, None, None, images, norm, work)
+
+
+def group_norm_backward(x, dy, dx, images: int, norm: GroupNorm, work=None) -> None:
+    """dx = gradient of group_norm_forward()'s input x for dy, and norm.dweight and norm.dbias, which are overwritten and repeat bit for
+    bit.  Types as there, dx like x; dx may be x or dy itself."""
+    _group_norm("group_norm_backward", x, None, dy, dx, images, norm, work)
+
+
+def group_norm_work(images: int, pixels: int, cols: int, groups: int) -> int:
+    """fp32 values that group_norm_forward() and group_norm_backward() take as `work`."""
+    return lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), cols, groups)
+
+
 # ---- clipping of gradients by their global norm ----
 class GradList:
     """A list of gradients as clip_gradients() takes it, checked and laid out once: contiguous fp32 or bf16 tensors of one CUDA
