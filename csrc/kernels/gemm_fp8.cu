@@ -12,6 +12,8 @@
 // and the tile is only as wide as A has rows.
 // Every mbarrier wait is bounded; on expiry the CTA records TIMEOUT in `status`, stops issuing work, frees its TMEM and returns.
 #include <cuda.h>
+
+#include <atomic>
 #include <mutex>
 
 #include "kernels.h"
@@ -393,7 +395,13 @@ Plan choose(const GeepsGemmFp8* p, int sms) {
 template <bool CL>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Dev& d, int grid, cudaStream_t st) {
   const size_t smem = (size_t)d.stages * (A_BYTES + d.bn * BK + SCALE_BYTES) + (CL ? 0 : d.slabs * SLAB_BYTES) + sizeof(Ctl) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(gemm_fp8_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  static std::atomic<unsigned long long> ready{0};           // devices on which the kernel may have all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(gemm_fp8_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    ready |= 1ull << (dev & 63);
+  }
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);

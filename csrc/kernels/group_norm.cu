@@ -15,8 +15,11 @@
 // Variance: values less the first of every 32 of a thread's pixels are added and squared, and such parts meet as count, mean and
 // sum of squared differences, so a mean far from zero costs nothing (a part's error is at most 32 x 2^-24 of its variance).
 // The backward pass forms z in the four rounded operations above, so that the border of the ReLU does not depend on how it is compiled.
-#include <stdlib.h>
+#include <string.h>
+
+#include <atomic>
 #include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "nn_ops.h"
@@ -26,9 +29,11 @@ typedef __nv_bfloat16 bf16;
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kMostParts = 256;            // chunks of an image in two launches
 constexpr int kPart = 32;                  // pixels of a part of the variance
-enum Phase { FUSED = 0, SUMS = 1, APPLY = 2 };
+// One launch with the pixels kept in shared memory, or read again; or two launches
+enum Phase { KEPT = 0, TWICE = 1, SUMS = 2, APPLY = 3 };
+constexpr int threads_of(int phase) { return phase == KEPT || phase == TWICE ? 128 : 256; }
 
 // n / d for n below 2^31 by a multiplication (Granlund and Montgomery)
 struct Divide {
@@ -95,6 +100,12 @@ struct Vec<bf16, 8> {
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], zero);
   }
+  __device__ __forceinline__ void mask(const float2 (&z)[4]) {      // zero where z is not above zero
+    uint32_t* w = (uint32_t*)&a;
+    const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] &= __hgt2_mask(__floats2bfloat162_rn(z[i].x, z[i].y), zero);
+  }
 };
 template <>
 struct Vec<float, 8> {
@@ -110,6 +121,11 @@ struct Vec<float, 8> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = f[i] < 0.f ? 0.f : f[i];
   }
+  __device__ __forceinline__ void mask(const float2 (&z)[4]) {
+    float2* f = (float2*)this;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(z[i].x > 0.f ? f[i].x : 0.f, z[i].y > 0.f ? f[i].y : 0.f);
+  }
 };
 template <>
 struct Vec<bf16, 1> {
@@ -119,6 +135,7 @@ struct Vec<bf16, 1> {
   __device__ __forceinline__ void set(const float2 (&f)[1]) { a = __float2bfloat16(f[0].x); }
   __device__ __forceinline__ void store(bf16* p) const { *p = a; }
   __device__ __forceinline__ void relu() { a = __hmax_nan(a, __float2bfloat16(0.f)); }
+  __device__ __forceinline__ void mask(const float2 (&z)[1]) { if (!(z[0].x > 0.f)) a = __float2bfloat16(0.f); }
 };
 template <>
 struct Vec<float, 1> {
@@ -128,6 +145,7 @@ struct Vec<float, 1> {
   __device__ __forceinline__ void set(const float2 (&f)[1]) { a = f[0].x; }
   __device__ __forceinline__ void store(float* p) const { *p = a; }
   __device__ __forceinline__ void relu() { a = a < 0.f ? 0.f : a; }
+  __device__ __forceinline__ void mask(const float2 (&z)[1]) { if (!(z[0].x > 0.f)) a = 0.f; }
 };
 template <int W>
 __device__ __forceinline__ float& value(float2 (&f)[(W + 1) / 2], int i) { return i & 1 ? f[i >> 1].y : f[i >> 1].x; }
@@ -151,6 +169,7 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 // A thread's own rows of vectors in shared memory, 16 bytes of every thread side by side
 template <typename T>
 struct Kept {
+  static constexpr int kThreads = threads_of(KEPT);
   uint8_t* base;
   static constexpr int kPieces = (int)sizeof(T) / 2;        // of 16 bytes
   static constexpr int kBytes = kThreads * 16 * kPieces;    // of a row
@@ -166,24 +185,26 @@ struct Kept {
     for (int i = 0; i < kPieces; ++i) w[i] = *(const uint4*)(base + k * kBytes + i * kThreads * 16 + threadIdx.x * 16);
     return v;
   }
+  __device__ __forceinline__ void put(int k, const Vec<T, 8>& v) const {
+    const uint4* w = (const uint4*)&v;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) *(uint4*)(base + k * kBytes + i * kThreads * 16 + threadIdx.x * 16) = w[i];
+  }
 };
-// Rows of a column as a thread reads them: from its own shared memory (ALL), or the first `keep` from there and the others
-// where they lie
-template <typename T, int W>
+// Rows of a column as a thread reads them: from its own shared memory or where they lie
+template <typename T, int W, bool KEEP>
 struct Rows {
   const T* at;
   long long step;
   Kept<T> kept;
-  int keep;
-  template <bool ALL>
   __device__ __forceinline__ Vec<T, W> get(int k) const {
-    Vec<T, W> v;
-    if constexpr (W == 8) {
-      if (ALL || k < keep) v = kept.get(k); else v.load(at + k * step);
+    if constexpr (KEEP) {
+      return kept.get(k);
     } else {
+      Vec<T, W> v;
       v.load(at + k * step);
+      return v;
     }
-    return v;
   }
 };
 
@@ -227,7 +248,7 @@ __device__ __forceinline__ float lane_sum(float a, int lanes) {
 __device__ __forceinline__ int lanes_for(int n) { return n >= 32 ? 32 : n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 // f(g, lane of the group, whether there is such a group) for every group of the slice, `lanes` lanes of a warp a group; lanes
 // without a group get the last one
-template <typename F>
+template <int kThreads, typename F>
 __device__ __forceinline__ void each_group(int gs, int lanes, F f) {
   const int at = threadIdx.x & (lanes - 1), per = kThreads / lanes;
   for (int g0 = 0; g0 < gs; g0 += per) {
@@ -238,7 +259,7 @@ __device__ __forceinline__ void each_group(int gs, int lanes, F f) {
 
 // finish(c, sum over the R threads of channel c of entry[i][r][v]), c = W v + i, by one thread a channel; entry is overwritten.
 // Every thread of the block calls it; no barrier behind it.
-template <int W, typename F>
+template <int kThreads, int W, typename F>
 __device__ __forceinline__ void column_sums(const Dev& d, float2* entry, F finish) {
   __syncthreads();
   const int all = d.R * d.V;
@@ -254,18 +275,22 @@ __device__ __forceinline__ void column_sums(const Dev& d, float2* entry, F finis
 }
 
 __device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.f + __expf(-z)); }
-
-constexpr int kFlight = 4;                 // rows of a thread in flight
+__device__ __forceinline__ float silu_slope(float z, float dy) {
+  const float g = __fdividef(1.f, 1.f + __expf(-z));
+  return dy * (g * fmaf(z, 1.f - g, 1.f));
+}
 
 template <typename XT, typename YT, bool VEC, int PHASE>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(threads_of(PHASE), PHASE == KEPT ? 6 : PHASE == TWICE ? 4 : 2)
 group_forward_kernel(const __grid_constant__ Dev d) {
-  constexpr int W = VEC ? 8 : 1, H = (W + 1) / 2;
+  constexpr int W = VEC ? 8 : 1, H = (W + 1) / 2, FLIGHT = PHASE == KEPT ? 4 : sizeof(XT) * W > 16 ? 4 : 8;      // FLIGHT: rows of a thread in flight
+  constexpr int kThreads = threads_of(PHASE);
+  constexpr bool KEEP = PHASE == KEPT, ONE = PHASE == KEPT || PHASE == TWICE;
   extern __shared__ __align__(16) uint8_t smem[];
   const Place<W> p(d);
   const int cg = d.by_cg.d, gs = d.slice / cg, chunks = d.by_chunks.d;
   const bool narrow = d.V <= kThreads;                   // one column a thread
-  float* mean_of = (float*)smem;                         // [slice], each: minus the mean, 1/std times weight and bias of a channel
+  float* mean_of = (float*)smem;                         // [slice], each: minus the mean, 1/std times weight, bias of a channel
   float* a_of = mean_of + d.slice;
   float* b_of = a_of + d.slice;
   float2* column = (float2*)smem;                        // [slice], before those: mean and squared differences of a channel
@@ -274,27 +299,26 @@ group_forward_kernel(const __grid_constant__ Dev d) {
   float* base_of = (float*)(stat + gs);                  // [slice], unless a thread has several columns
   float2* entry = (float2*)(base_of + (narrow ? (d.slice + 3) & ~3 : 0));          // [W][R][V]: sums of the threads about a column's base
   const int mine = p.mine();
-  const long long at = (p.pixel + p.r) * d.ldx + p.c0 + p.v * W, step = (long long)d.R * d.ldx;
-  Rows<XT, W> x = {(const XT*)d.x + at, step, {(uint8_t*)entry + d.entries}, 0};
+  const long long at = (p.pixel + p.r) * d.ldx + p.c0 + p.v * W;
+  Rows<XT, W, KEEP> x = {(const XT*)d.x + at, (long long)d.R * d.ldx, {(uint8_t*)entry + d.entries}};
   geeps_pdl_enter();
 
   if (PHASE != APPLY) {
-    if (VEC && PHASE == FUSED) {
-      x.keep = min(d.keep, mine);
+    if constexpr (KEEP) {
       const XT* from = x.at;
-      for (int k = 0; k < x.keep; ++k, from += step) x.kept.fetch(k, from);
+#pragma unroll 4
+      for (int k = 0; k < mine; ++k, from += x.step) x.kept.fetch(k, from);
       copies_done();
     }
     float2 mean[H], m2[H];
-    auto pass = [&](auto all) {
-      constexpr bool ALL = decltype(all)::value;
+    auto pass = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < H; ++i) mean[i] = m2[i] = both(0.f);
       int n = 0;
       for (int k = 0; k < mine;) {
         const int end = min(mine, k + kPart), count = end - k;
         float2 s[H], q[H], base[H];
-        x.template get<ALL>(k).get(base);
+        x.get(k).get(base);
 #pragma unroll
         for (int i = 0; i < H; ++i) {
           s[i] = q[i] = both(0.f);
@@ -311,14 +335,15 @@ group_forward_kernel(const __grid_constant__ Dev d) {
           }
         };
         int j = k + 1;
-        for (; j + kFlight <= end; j += kFlight) {
-          Vec<XT, W> in[kFlight];
+        for (; j + FLIGHT <= end; j += FLIGHT) {
+          Vec<XT, W> in[FLIGHT];
 #pragma unroll
-          for (int u = 0; u < kFlight; ++u) in[u] = x.template get<ALL>(j + u);
+          for (int u = 0; u < FLIGHT; ++u) in[u] = x.get(j + u);
 #pragma unroll
-          for (int u = 0; u < kFlight; ++u) add(in[u]);
+          for (int u = 0; u < FLIGHT; ++u) add(in[u]);
         }
-        for (; j < end; ++j) add(x.template get<ALL>(j));
+#pragma unroll 1
+        for (; j < end; ++j) add(x.get(j));
         const float inv = __frcp_rn((float)count), share = n ? (float)count / (n + count) : 1.f, weight = n * share;
 #pragma unroll
         for (int i = 0; i < H; ++i) {
@@ -332,7 +357,7 @@ group_forward_kernel(const __grid_constant__ Dev d) {
       }
     };
     if (narrow) {
-      if (VEC && PHASE == FUSED && x.keep == mine) pass(std::true_type()); else pass(std::false_type());
+      pass();
       if (p.r == 0) {
 #pragma unroll
         for (int i = 0; i < W; ++i) base_of[p.v * W + i] = value<W>(mean, i);
@@ -341,19 +366,20 @@ group_forward_kernel(const __grid_constant__ Dev d) {
       __syncthreads();
       if (p.works) {
         const float n = (float)mine;
+        float2* to = entry + p.r * d.V + p.v;
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
+        for (int i = 0; i < W; ++i, to += d.R * d.V) {
           const float e = value<W>(mean, i) - base_of[p.v * W + i];
-          entry[(i * d.R + p.r) * d.V + p.v] = mine ? make_float2(n * e, fmaf(n * e, e, value<W>(m2, i))) : both(0.f);
+          *to = mine ? make_float2(n * e, fmaf(n * e, e, value<W>(m2, i))) : both(0.f);
         }
       }
       const float inv = p.rows ? __frcp_rn((float)p.rows) : 0.f;
-      column_sums<W>(d, entry, [&](int c, float2 t) {
+      column_sums<kThreads, W>(d, entry, [&](int c, float2 t) {
         column[c] = make_float2(fmaf(t.x, inv, base_of[c]), fmaxf(t.y - t.x * t.x * inv, 0.f));
       });
     } else {
       for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W) {
-        pass(std::false_type());
+        pass();
 #pragma unroll
         for (int i = 0; i < W; ++i) column[v * W + i] = make_float2(value<W>(mean, i), value<W>(m2, i));
       }
@@ -362,7 +388,7 @@ group_forward_kernel(const __grid_constant__ Dev d) {
     __syncthreads();
     const int lanes = lanes_for(cg);
     const float each = __frcp_rn((float)cg);
-    each_group(gs, lanes, [&](int g, int l, bool mine_g) {
+    each_group<kThreads>(gs, lanes, [&](int g, int l, bool mine_g) {
       const float2* of = column + g * cg;
       float s = 0.f, sq = 0.f;
       for (int c = l; c < cg; c += lanes) s += of[c].x;
@@ -382,29 +408,29 @@ group_forward_kernel(const __grid_constant__ Dev d) {
     return;
   }
   const float total = (float)d.pixels * cg;
-  if (PHASE == FUSED) { if (chunks > 1) tc05::cluster_sync(); else __syncthreads(); }
+  if (ONE) { if (chunks > 1) tc05::cluster_sync(); else __syncthreads(); }
+  constexpr int MOST = ONE ? 1 : kMostParts / 32;       // entries of a lane
   const int lanes = lanes_for(chunks);
-  each_group(gs, lanes, [&](int g, int l, bool) {
+  each_group<kThreads>(gs, lanes, [&](int g, int l, bool) {
     auto get = [&](int i) {
-      if (PHASE == FUSED) return ld_cluster_f2(tc05::map_to_cta(tc05::smem_u32(part + g), i));
+      if (ONE) return ld_cluster_f2(tc05::map_to_cta(tc05::smem_u32(part + g), i));
       return ((const float2*)d.sums)[((long long)p.image * chunks + i) * d.groups + p.slice * gs + g];
     };
     auto n_of = [&](int i) { return (float)max(0, min(d.rows, d.pixels - i * d.rows)) * cg; };
-    float2 first = both(0.f);
-    if (l < chunks) first = get(l);
-    float s = n_of(l) * first.x;
-    for (int i = l + lanes; i < chunks; i += lanes) s = fmaf(n_of(i), get(i).x, s);
+    float2 t[MOST];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) { const int i = l + lanes * u; t[u] = i < chunks ? get(i) : both(0.f); }
+    float s = 0.f, sq = 0.f;
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) s = fmaf(n_of(l + lanes * u), t[u].x, s);
     const float m = lane_sum(s, lanes) / total;
-    float sq = first.y + n_of(l) * (first.x - m) * (first.x - m);
-    for (int i = l + lanes; i < chunks; i += lanes) {
-      const float2 t = get(i);
-      sq += t.y + n_of(i) * (t.x - m) * (t.x - m);
-    }
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) sq += t[u].y + n_of(l + lanes * u) * (t[u].x - m) * (t[u].x - m);
     sq = lane_sum(sq, lanes);
     if (l == 0) stat[g] = make_float2(m, __frcp_rn(__fsqrt_rn(sq / total + d.eps)));
   });
   __syncthreads();
-  if (PHASE == FUSED && chunks > 1) tc05::cluster_arrive();      // nobody leaves while a peer still reads its sums
+  if (ONE && chunks > 1) tc05::cluster_arrive();      // nobody leaves while a peer still reads its sums
   if (d.stats != nullptr && p.chunk == 0)
     for (int g = threadIdx.x; g < gs; g += kThreads) ((float2*)d.stats)[(long long)p.image * d.groups + p.slice * gs + g] = stat[g];
   auto constant = [&](int c, float& mean, float& a, float& b) {
@@ -419,8 +445,8 @@ group_forward_kernel(const __grid_constant__ Dev d) {
   }
   const long long ostep = (long long)d.R * d.ldo;
   YT* y = (YT*)d.out + (p.pixel + p.r) * d.ldo + p.c0 + p.v * W;
-  auto pass = [&](auto all, int v) {
-    constexpr bool ALL = decltype(all)::value;
+  auto pass = [&](int v, auto act) __attribute__((always_inline)) {
+    constexpr int ACT = decltype(act)::value;
     float2 mean[H], a[H], b[H];
     if (narrow) {
       channel_values<W>(mean_of, v, mean);
@@ -437,66 +463,65 @@ group_forward_kernel(const __grid_constant__ Dev d) {
 #pragma unroll
       for (int i = 0; i < H; ++i) {
         f[i] = fma2(add2(f[i], mean[i]), a[i], b[i]);
-        if (d.act == 2) f[i] = make_float2(silu(f[i].x), W > 1 ? silu(f[i].y) : 0.f);
+        if (ACT == 2) f[i] = make_float2(silu(f[i].x), W > 1 ? silu(f[i].y) : 0.f);
       }
       Vec<YT, W> o;
       o.set(f);
-      if (d.act == 1) o.relu();
+      if (ACT == 1) o.relu();
       o.store(to);
       to += ostep;
     };
     int k = 0;
-    for (; k + kFlight <= mine; k += kFlight) {
-      Vec<XT, W> in[kFlight];
+    for (; k + FLIGHT <= mine; k += FLIGHT) {
+      Vec<XT, W> in[FLIGHT];
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u) in[u] = x.template get<ALL>(k + u);
+      for (int u = 0; u < FLIGHT; ++u) in[u] = x.get(k + u);
 #pragma unroll
-      for (int u = 0; u < kFlight; ++u) finish(in[u]);
+      for (int u = 0; u < FLIGHT; ++u) finish(in[u]);
     }
-    for (; k < mine; ++k) finish(x.template get<ALL>(k));
+#pragma unroll 1
+    for (; k < mine; ++k) finish(x.get(k));
+  };
+  auto by_act = [&](int v) __attribute__((always_inline)) {
+    if (d.act == 0) pass(v, std::integral_constant<int, 0>());
+    else if (d.act == 1) pass(v, std::integral_constant<int, 1>());
+    else pass(v, std::integral_constant<int, 2>());
   };
   if (narrow) {
-    if (p.works) { if (VEC && PHASE == FUSED && x.keep == mine) pass(std::true_type(), p.v); else pass(std::false_type(), p.v); }
+    if (p.works) by_act(p.v);
   } else {
-    for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W, y += kThreads * W) pass(std::false_type(), v);
+    for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W, y += kThreads * W) by_act(v);
   }
-  if (PHASE == FUSED && chunks > 1) tc05::cluster_wait();
-}
-
-// act'(z) dy
-__device__ __forceinline__ float slope(float z, float dy, int act) {
-  if (act == 1) return z > 0.f ? dy : (z == z ? 0.f : z);
-  const float g = __fdividef(1.f, 1.f + __expf(-z));
-  return dy * (g * fmaf(z, 1.f - g, 1.f));
+  if (ONE && chunks > 1) tc05::cluster_wait();
 }
 
 template <typename XT, typename YT, bool VEC, int PHASE>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(threads_of(PHASE), PHASE == KEPT && sizeof(XT) == 2 ? 5 : PHASE == KEPT || PHASE == TWICE ? 4 : 2)
 group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
-  constexpr int W = VEC ? 8 : 1, H = (W + 1) / 2;
-  constexpr int FLIGHT = kFlight / 2;
+  constexpr int W = VEC ? 8 : 1, H = (W + 1) / 2, FLIGHT = PHASE == KEPT ? 2 : W == 1 ? 8 : sizeof(XT) > 2 ? 2 : 4;
+  constexpr int kThreads = threads_of(PHASE);
+  constexpr bool KEEP = PHASE == KEPT, ONE = PHASE == KEPT || PHASE == TWICE;
   extern __shared__ __align__(16) uint8_t smem[];
   const Place<W> p(d);
   const int cg = d.by_cg.d, gs = d.slice / cg, chunks = d.by_chunks.d;
   const bool narrow = d.V <= kThreads;
-  float* mean_of = (float*)smem;                         // [slice], each: minus the mean, 1/std, weight and bias of a channel
-  float* rstd_of = mean_of + d.slice;
-  float* w_of = rstd_of + d.slice;
-  float* b_of = w_of + d.slice;
-  float2* column = (float2*)(smem + (narrow ? d.slice * 16 : 0));    // [slice]: sums of dz and dz n of a channel
+  // [slice], each: minus the mean, 1/std, weight and bias of a channel; then the factors of dz and of x - mean in dx, and the rest
+  float* mean_of = (float*)smem;
+  float *rstd_of = mean_of + d.slice, *w_of = rstd_of + d.slice, *b_of = w_of + d.slice, *dz_of = b_of + d.slice, *x_of = dz_of + d.slice, *one_of = x_of + d.slice;
+  float2* column = (float2*)(smem + (narrow ? (d.slice * 28 + 15) & ~15 : 0));     // [slice]: sums of dz and dz n of a channel
   float2* part = column + d.slice;                       // [gs]: sums of dz w and dz w n of the CTA's pixels, then of all
   float2* whole = part + gs;
   float2* entry = (float2*)(((uintptr_t)(whole + gs) + 15) & ~(uintptr_t)15);      // [W][R][V], unless there is one thread a column
   const int mine = p.mine();
   const long long x_at = (p.pixel + p.r) * d.ldx + p.c0 + p.v * W, dy_at = (p.pixel + p.r) * d.lddy + p.c0 + p.v * W;
-  Rows<XT, W> x = {(const XT*)d.x + x_at, (long long)d.R * d.ldx, {(uint8_t*)entry + d.entries}, 0};
-  Rows<YT, W> dy = {(const YT*)d.dy + dy_at, (long long)d.R * d.lddy, {x.kept.base + (size_t)d.keep * Kept<XT>::kBytes}, 0};
+  Rows<XT, W, KEEP> x = {(const XT*)d.x + x_at, (long long)d.R * d.ldx, {(uint8_t*)entry + d.entries}};
+  Rows<YT, W, KEEP> dy = {(const YT*)d.dy + dy_at, (long long)d.R * d.lddy, {x.kept.base + (size_t)d.keep * Kept<XT>::kBytes}};
   geeps_pdl_enter();
-  if (VEC && PHASE == FUSED) {
-    x.keep = dy.keep = min(d.keep, mine);
+  if constexpr (KEEP) {
     const XT* xs = x.at;
     const YT* ds = dy.at;
-    for (int k = 0; k < x.keep; ++k, xs += x.step, ds += dy.step) {
+#pragma unroll 4
+    for (int k = 0; k < mine; ++k, xs += x.step, ds += dy.step) {
       x.kept.fetch(k, xs);
       dy.kept.fetch(k, ds);
     }
@@ -513,77 +538,78 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
     for (int c = threadIdx.x; c < d.slice; c += kThreads) constant(c, mean_of[c], rstd_of[c], w_of[c], b_of[c]);
     __syncthreads();
   }
-  float2 mean[H], rstd[H], w[H], b[H];
-  auto constants = [&](int v) {
-    if (narrow) {
-      channel_values<W>(mean_of, v, mean);
-      channel_values<W>(rstd_of, v, rstd);
-      channel_values<W>(w_of, v, w);
-      channel_values<W>(b_of, v, b);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2 * H; ++i) constant(v * W + (i < W ? i : 0), value<W>(mean, i), value<W>(rstd, i), value<W>(w, i), value<W>(b, i));
-    }
-  };
-  // dz and n of a row
-  auto row = [&](const Vec<XT, W>& xi, const Vec<YT, W>& di, float2 (&dz)[H], float2 (&n)[H]) {
-    xi.get(n);
-    di.get(dz);
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      n[i] = mul2(add2(n[i], mean[i]), rstd[i]);
-      if (d.act) {
-        const float2 z = add2(mul2(n[i], w[i]), b[i]);
-        dz[i] = make_float2(slope(z.x, dz[i].x, d.act), W > 1 ? slope(z.y, dz[i].y, d.act) : 0.f);
-      }
-    }
-  };
-  // f(x, dy) for all rows of a column, FLIGHT of them in flight
-  auto rows = [&](auto all, auto f) {
-    constexpr bool ALL = decltype(all)::value;
+  // f(k, x, dy) for all rows of a column, FLIGHT of them in flight
+  auto rows = [&](auto f) {
     int k = 0;
     for (; k + FLIGHT <= mine; k += FLIGHT) {
       Vec<XT, W> xi[FLIGHT];
       Vec<YT, W> di[FLIGHT];
 #pragma unroll
-      for (int u = 0; u < FLIGHT; ++u) { xi[u] = x.template get<ALL>(k + u); di[u] = dy.template get<ALL>(k + u); }
+      for (int u = 0; u < FLIGHT; ++u) { xi[u] = x.get(k + u); di[u] = dy.get(k + u); }
 #pragma unroll
-      for (int u = 0; u < FLIGHT; ++u) f(xi[u], di[u]);
+      for (int u = 0; u < FLIGHT; ++u) f(k + u, xi[u], di[u]);
     }
-    for (; k < mine; ++k) f(x.template get<ALL>(k), dy.template get<ALL>(k));
+#pragma unroll 1
+    for (; k < mine; ++k) f(k, x.get(k), dy.get(k));
   };
-  const bool all_kept = VEC && PHASE == FUSED && x.keep == mine && narrow;
+  // z, rounded after each operation
+  auto border = [&](const float2& n, const float2& w, const float2& b) { return add2(mul2(n, w), b); };
   if (PHASE != APPLY) {
-    if (VEC && PHASE == FUSED) copies_done();
-    auto pass = [&](auto all, int v) {
-      constants(v);
-      float2 sa[H], sb[H];
+    if constexpr (KEEP) copies_done();
+    auto pass = [&](int v, auto act) __attribute__((always_inline)) {
+      constexpr int ACT = decltype(act)::value;
+      float2 mean[H], rstd[H], w[H], b[H], sa[H], sb[H];
+      if (narrow) {
+        channel_values<W>(mean_of, v, mean);
+        channel_values<W>(rstd_of, v, rstd);
+        if (ACT) { channel_values<W>(w_of, v, w); channel_values<W>(b_of, v, b); }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2 * H; ++i) constant(v * W + (i < W ? i : 0), value<W>(mean, i), value<W>(rstd, i), value<W>(w, i), value<W>(b, i));
+      }
 #pragma unroll
       for (int i = 0; i < H; ++i) sa[i] = sb[i] = both(0.f);
-      rows(all, [&](const Vec<XT, W>& xi, const Vec<YT, W>& di) {
-        float2 dz[H], n[H];
-        row(xi, di, dz, n);
+      rows([&](int k, const Vec<XT, W>& xi, Vec<YT, W> di) {
+        float2 dz[H], n[H], z[H];
+        xi.get(n);
 #pragma unroll
-        for (int i = 0; i < H; ++i) { sa[i] = add2(sa[i], dz[i]); sb[i] = fma2(dz[i], n[i], sb[i]); }
+        for (int i = 0; i < H; ++i) {
+          n[i] = mul2(add2(n[i], mean[i]), rstd[i]);
+          if (ACT) z[i] = border(n[i], w[i], b[i]);
+        }
+        if (ACT == 1) {
+          di.mask(z);
+          if constexpr (KEEP) dy.kept.put(k, di);       // for the second pass, which needs no z then
+        }
+        di.get(dz);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          if (ACT == 2) dz[i] = make_float2(silu_slope(z[i].x, dz[i].x), W > 1 ? silu_slope(z[i].y, dz[i].y) : 0.f);
+          sa[i] = add2(sa[i], dz[i]);
+          sb[i] = fma2(dz[i], n[i], sb[i]);
+        }
       });
+      float2* to = d.R == 1 ? column + v * W : entry + p.r * d.V + v;
+      const int next = d.R == 1 ? 1 : d.R * d.V;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const float2 t = make_float2(value<W>(sa, i), value<W>(sb, i));
-        if (d.R == 1) column[v * W + i] = t;
-        else entry[(i * d.R + p.r) * d.V + v] = t;
-      }
+      for (int i = 0; i < W; ++i, to += next) *to = make_float2(value<W>(sa, i), value<W>(sb, i));
+    };
+    auto by_act = [&](int v) __attribute__((always_inline)) {
+      if (d.act == 0) pass(v, std::integral_constant<int, 0>());
+      else if (d.act == 1) pass(v, std::integral_constant<int, 1>());
+      else pass(v, std::integral_constant<int, 2>());
     };
     if (narrow) {
-      if (p.works) { if (all_kept) pass(std::true_type(), p.v); else pass(std::false_type(), p.v); }
+      if (p.works) by_act(p.v);
     } else {
-      for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W, dy.at += kThreads * W) pass(std::false_type(), v);
+      for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W, dy.at += kThreads * W) by_act(v);
       x.at = (const XT*)d.x + x_at;
       dy.at = (const YT*)d.dy + dy_at;
     }
-    if (d.R > 1) column_sums<W>(d, entry, [&](int c, float2 t) { column[c] = t; });
+    if (d.R > 1) column_sums<kThreads, W>(d, entry, [&](int c, float2 t) { column[c] = t; });
     __syncthreads();
     const int lanes = lanes_for(cg);
-    each_group(gs, lanes, [&](int g, int l, bool mine_g) {
+    each_group<kThreads>(gs, lanes, [&](int g, int l, bool mine_g) {
       float2 s = both(0.f);
       for (int c = l; c < cg; c += lanes) s = fma2(column[g * cg + c], both(narrow ? w_of[g * cg + c] : d.w != nullptr ? __ldg(d.w + p.c0 + g * cg + c) : 1.f), s);
       s.x = lane_sum(s.x, lanes);
@@ -600,12 +626,16 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
     return;
   }
   const float scale = 1.f / ((float)d.pixels * cg);
-  if (PHASE == FUSED) { if (chunks > 1) tc05::cluster_sync(); else __syncthreads(); }
+  if (ONE) { if (chunks > 1) tc05::cluster_sync(); else __syncthreads(); }
+  constexpr int MOST = ONE ? 1 : kMostParts / 32;       // entries of a lane
   const int lanes = lanes_for(chunks);
-  each_group(gs, lanes, [&](int g, int l, bool) {
+  each_group<kThreads>(gs, lanes, [&](int g, int l, bool) {
     float2 s = both(0.f);
-    for (int i = l; i < chunks; i += lanes) {
-      if (PHASE == FUSED) s = add2(s, ld_cluster_f2(tc05::map_to_cta(tc05::smem_u32(part + g), i)));
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+      const int i = l + lanes * u;
+      if (i >= chunks) continue;
+      if (ONE) s = add2(s, ld_cluster_f2(tc05::map_to_cta(tc05::smem_u32(part + g), i)));
       else s = add2(s, ((const float2*)d.sums)[((long long)p.image * chunks + i) * d.groups + p.slice * gs + g]);
     }
     s.x = lane_sum(s.x, lanes);
@@ -613,72 +643,103 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
     if (l == 0) whole[g] = make_float2(-s.x * scale, -s.y * scale);
   });
   // the image's sums of a channel: each CTA joins its share of the slice's
-  if (PHASE == FUSED && channel_sums != nullptr)
+  if (ONE && channel_sums != nullptr)
     for (int c = p.chunk * kThreads + threadIdx.x; c < d.slice; c += chunks * kThreads) {
       float2 s = both(0.f);
       for (int i = 0; i < chunks; ++i) s = add2(s, ld_cluster_f2(tc05::map_to_cta(tc05::smem_u32(column + c), i)));
       ((float2*)channel_sums)[(long long)p.image * d.C + p.c0 + c] = s;
     }
   __syncthreads();
-  if (PHASE == FUSED && chunks > 1) tc05::cluster_arrive();      // nobody leaves while a peer still reads its sums
+  if (ONE && chunks > 1) tc05::cluster_arrive();      // nobody leaves while a peer still reads its sums
+  // dx = dz (w rstd) + (x - mean) (-mean(dz w n) rstd^2) - mean(dz w) rstd
+  auto factors = [&](int c, float w, float rstd, float& dz, float& x, float& one) {
+    const float2 s = whole[d.by_cg(c)];
+    dz = w * rstd;
+    x = s.y * rstd * rstd;
+    one = s.x * rstd;
+  };
+  if (narrow) {
+    for (int c = threadIdx.x; c < d.slice; c += kThreads) factors(c, w_of[c], rstd_of[c], dz_of[c], x_of[c], one_of[c]);
+    __syncthreads();
+  }
   const long long ostep = (long long)d.R * d.ldo;
   XT* dx = (XT*)d.out + (p.pixel + p.r) * d.ldo + p.c0 + p.v * W;
-  auto pass = [&](auto all, int v) {
-    if (PHASE == APPLY || !narrow) constants(v);
-    float2 ca[H], cb[H], wr[H];
+  auto pass = [&](int v, auto act) __attribute__((always_inline)) {
+    constexpr int ACT = decltype(act)::value;
+    constexpr bool AGAIN = ACT == 2 || (ACT == 1 && !KEEP);      // z is needed again
+    float2 mean[H], rstd[H], w[H], b[H], fz[H], fx[H], f1[H];
+    if (narrow) {
+      channel_values<W>(mean_of, v, mean);
+      if (AGAIN) { channel_values<W>(rstd_of, v, rstd); channel_values<W>(w_of, v, w); channel_values<W>(b_of, v, b); }
+      channel_values<W>(dz_of, v, fz);
+      channel_values<W>(x_of, v, fx);
+      channel_values<W>(one_of, v, f1);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2 * H; ++i) {
-      const float2 s = whole[d.by_cg(v * W + (i < W ? i : 0))];
-      value<W>(ca, i) = s.x * value<W>(rstd, i);
-      value<W>(cb, i) = s.y * value<W>(rstd, i);
-      value<W>(wr, i) = value<W>(w, i) * value<W>(rstd, i);
+      for (int i = 0; i < 2 * H; ++i) {
+        const int c = v * W + (i < W ? i : 0);
+        constant(c, value<W>(mean, i), value<W>(rstd, i), value<W>(w, i), value<W>(b, i));
+        factors(c, value<W>(w, i), value<W>(rstd, i), value<W>(fz, i), value<W>(fx, i), value<W>(f1, i));
+      }
     }
     XT* to = dx;
-    rows(all, [&](const Vec<XT, W>& xi, const Vec<YT, W>& di) {
-      float2 dz[H], n[H];
-      row(xi, di, dz, n);
+    rows([&](int, const Vec<XT, W>& xi, Vec<YT, W> di) {
+      float2 dz[H], e[H], z[H];
+      xi.get(e);
 #pragma unroll
-      for (int i = 0; i < H; ++i) dz[i] = fma2(dz[i], wr[i], fma2(n[i], cb[i], ca[i]));
+      for (int i = 0; i < H; ++i) {
+        e[i] = add2(e[i], mean[i]);
+        if (AGAIN) z[i] = border(mul2(e[i], rstd[i]), w[i], b[i]);
+      }
+      if (AGAIN && ACT == 1) di.mask(z);
+      di.get(dz);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        if (ACT == 2) dz[i] = make_float2(silu_slope(z[i].x, dz[i].x), W > 1 ? silu_slope(z[i].y, dz[i].y) : 0.f);
+        dz[i] = fma2(dz[i], fz[i], fma2(e[i], fx[i], f1[i]));
+      }
       Vec<XT, W> o;
       o.set(dz);
       o.store(to);
       to += ostep;
     });
   };
+  auto by_act = [&](int v) __attribute__((always_inline)) {
+    if (d.act == 0) pass(v, std::integral_constant<int, 0>());
+    else if (d.act == 1) pass(v, std::integral_constant<int, 1>());
+    else pass(v, std::integral_constant<int, 2>());
+  };
   if (narrow) {
-    if (p.works) { if (all_kept) pass(std::true_type(), p.v); else pass(std::false_type(), p.v); }
+    if (p.works) by_act(p.v);
   } else {
-    for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W, dy.at += kThreads * W, dx += kThreads * W) pass(std::false_type(), v);
+    for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W, dy.at += kThreads * W, dx += kThreads * W) by_act(v);
   }
-  if (PHASE == FUSED && chunks > 1) tc05::cluster_wait();
+  if (ONE && chunks > 1) tc05::cluster_wait();
 }
 
-// Sums over `parts` rows of {dz, dz n} of the channels: 32 channels a block, its eight warps take every eighth row
+// Sums over `parts` rows of {dz, dz n} of the channels: 8 channels a block, 32 of them in flight for each
 __global__ void __launch_bounds__(256)
 group_parameters_kernel(const float2* __restrict__ sums, long long parts, int C, float* dw, float* db) {
   geeps_pdl_enter();
-  constexpr int WARPS = 8;
-  __shared__ float2 sh[WARPS][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-  float2 s = make_float2(0.f, 0.f);
-  if (c < C)
-    for (long long i = warp; i < parts; i += WARPS) {
-      const float2 t = sums[i * C + c];
-      s.x += t.x;
-      s.y += t.y;
-    }
-  sh[warp][lane] = s;
+  __shared__ float2 sh[32][9];
+  const int i = threadIdx.x >> 3, c = blockIdx.x * 8 + (threadIdx.x & 7);
+  float2 s = both(0.f);
+  if (c < C) {
+#pragma unroll 4
+    for (long long r = i; r < parts; r += 32) s = add2(s, sums[r * C + c]);
+  }
+  sh[i][threadIdx.x & 7] = s;
   __syncthreads();
-  if (warp == 0 && c < C) {
+  if (i == 0 && c < C) {
 #pragma unroll
-    for (int i = 1; i < WARPS; ++i) { s.x += sh[i][lane].x; s.y += sh[i][lane].y; }
+    for (int r = 1; r < 32; ++r) s = add2(s, sh[r][threadIdx.x]);
     if (db != nullptr) db[c] = s.x;
     if (dw != nullptr) dw[c] = s.y;
   }
 }
 
 // ---------------- host side ----------------
-struct Shape { int vec, fused, slice, slices, chunks, rows, keep, blocks, V, R, entries; size_t smem; };
+struct Shape { int vec, threads, fused, slice, slices, chunks, rows, keep, blocks, V, R, entries; size_t smem; };
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -687,59 +748,98 @@ constexpr size_t kSmem = 200 * 1024;
 
 // Shared memory that does not depend on the pixels kept
 size_t fixed_bytes(const Shape& s, int cg, bool backward) {
-  const size_t gs = s.slice / cg, narrow = s.V <= kThreads;
-  if (backward) return (size_t)s.slice * (narrow ? 24 : 8) + gs * 16 + 16;
+  const size_t gs = s.slice / cg, narrow = s.V <= s.threads;
+  if (backward) return (narrow ? (s.slice * 28 + 15) & ~15 : 0) + (size_t)s.slice * 8 + gs * 16 + 16;
   return ((s.slice * (narrow ? 12 : 8) + 15) & ~15) + gs * 16 + (narrow ? ((s.slice + 3) & ~3) * 4 : 0);
 }
 
-Shape choose(int images, int pixels, int C, int groups, bool backward, bool vec, int xsize, int ysize) {
+Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, int xsize, int ysize) {
   Shape s = {};
   const int cg = C / groups, W = vec ? 8 : 1, sms = geeps_sm_count();
   const int unit = cg / gcd(cg, W) * W;          // channels of the narrowest slice
-  const char* kbs = getenv("GN_KB"); const int kb = kbs ? atoi(kbs) : 48; const char* fz = getenv("GN_FUSED"); const char* bl = getenv("GN_BLOCKS"); const char* sl = getenv("GN_SLICE");  // DEV
   s.vec = vec;
-  // slices of 64 channels and more: whole sectors of a pixel
-  const int least = vec ? (sl ? atoi(sl) : 64) : 64;
-  int n = 1;
-  while (unit * n < C && (unit * n < least || C / unit % n)) ++n;
-  s.slice = unit * n;
-  s.slices = C / s.slice;
-  s.V = s.slice / W;
-  s.R = s.V < kThreads ? kThreads / s.V : 1;
-  s.entries = (backward ? s.R > 1 : s.V <= kThreads) ? s.R * s.slice * 8 : 0;
-  s.entries = (s.entries + 15) & ~15;
-  const int row_bytes = kThreads * 16 * (vec ? (xsize / 2 + (backward ? ysize / 2 : 0)) : 0);      // of all threads' kept rows
-  const long long items = (long long)images * s.slices;
-  const long long bytes = (long long)pixels * s.slice * (xsize + (backward ? ysize : 0));
-  int chunks = 1;
-  while (chunks < kMostChunks && bytes / chunks > kb * 1024) ++chunks;
-  while (chunks < kMostChunks && items * chunks < sms && pixels / (chunks * 2) >= s.R) chunks *= 2;
-  if (chunks > kMostChunks) chunks = kMostChunks;
-  s.fused = 1;
-  if (fz ? !atoi(fz) : items * chunks < sms / 2 && pixels > chunks * 4LL * s.R) {
-    // too few items: two launches over as many chunks as fill the machine
-    s.fused = 0;
-    long long want = ((bl ? atoi(bl) : 4LL) * sms + items - 1) / items, most = (pixels + s.R - 1) / s.R;
-    chunks = (int)(want < most ? want : most);
+  s.threads = threads_of(KEPT);
+  const int row_bytes = s.threads * 16 * (vec ? (xsize / 2 + (backward ? ysize / 2 : 0)) : 0);      // of all threads' kept rows
+  // One launch: slices of 32 channels (whole sectors of a pixel) and more, and up to eight CTAs for an item.  The cost is how often the
+  // machine is filled by three CTAs an SM x what one takes, some 6 us and 1 us for 10 KB.
+  auto cut = [&](Shape& t) {
+    t.V = t.slice / W;
+    t.R = t.V < t.threads ? t.threads / t.V : 1;
+    t.entries = (((backward ? t.R > 1 : t.V <= t.threads) ? t.R * t.slice * 8 : 0) + 15) & ~15;
+  };
+  double best = 1e300;
+  int chunks = 0;
+  for (int n = 1; unit * n <= C && (n == 1 || unit * n <= W * s.threads); ++n) {
+    if (C / unit % n || (unit * n < 32 && unit * n < C)) continue;
+    Shape t = s;
+    t.slice = unit * n;
+    t.slices = C / t.slice;
+    cut(t);
+    if (vec && t.V > t.threads) continue;
+    for (int k = 1; k <= kMostChunks; ++k) {
+      const int rows = (pixels + k - 1) / k;
+      const size_t smem = fixed_bytes(t, cg, backward) + t.entries + (size_t)((rows + t.R - 1) / t.R) * row_bytes;
+      if (smem > kSmem || (k > 1 && rows < t.R)) continue;
+      const int fit = (int)(228 * 1024 / (smem + 1024)), most = !vec ? 4 : !backward ? 6 : xsize == 2 ? 5 : 4, resident = fit < most ? fit : most;
+      const double filled = (double)images * t.slices * k / ((double)sms * resident);
+      const double kb = (double)rows * t.slice * (xsize + (backward ? ysize : 0)) / 1024;
+      const double cost = (filled > 1.0 ? filled : 1.0) * (6.0 + kb / (vec ? 10.0 : 1.7) + (k > 1 ? 2.0 : 0.0));
+      if (cost < best) { best = cost; s = t; chunks = k; }
+    }
   }
+  s.fused = chunks > 0;
+  // Two launches: what each SM reads twice from memory or L2, and their beginnings and ends
+  const double twice = 14.0 + (double)images * pixels * C * (xsize + (backward ? ysize : 0)) / 1024 / sms / (vec ? 14.0 : 2.0);
+  if (!s.fused || twice < best) {
+    s.fused = 0;
+    int n = 1;
+    while (unit * n < C && (unit * n < 64 || C / unit % n)) ++n;
+    s.slice = unit * n;
+    s.slices = C / s.slice;
+    s.threads = threads_of(SUMS);
+    cut(s);
+    const long long items = (long long)images * s.slices;
+    const long long want = (2LL * sms + items - 1) / items, most = (pixels + s.R - 1) / s.R;
+    chunks = (int)(want < most ? want : most);
+    if (chunks > kMostParts) chunks = kMostParts;
+  }
+  const long long items = (long long)images * s.slices;
   s.rows = (pixels + chunks - 1) / chunks;
   s.chunks = s.fused ? chunks : (pixels + s.rows - 1) / s.rows;
-  const size_t fixed = fixed_bytes(s, cg, backward) + s.entries;
-  int keep = vec && s.V <= kThreads && s.fused ? (s.rows + s.R - 1) / s.R : 0;
-  while (keep > 0 && fixed + (size_t)keep * row_bytes > kSmem) --keep;
-  s.keep = keep;
-  s.smem = fixed + (size_t)keep * row_bytes;
+  s.keep = vec && s.fused ? (s.rows + s.R - 1) / s.R : 0;
+  s.smem = fixed_bytes(s, cg, backward) + s.entries + (size_t)s.keep * row_bytes;
   s.blocks = items * s.chunks > 0x7fffffffLL ? 0 : (int)(items * s.chunks);
   return s;
 }
 
-template <typename K, typename... A>
-int launch(K kernel, const Shape& s, bool cluster, cudaStream_t st, A&&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+// plan() of the sizes that this thread has met last: a network's layers ask again in every step
+Shape choose(int images, int pixels, int C, int groups, bool backward, bool vec, int xsize, int ysize) {
+  struct Met { int key[8]; Shape s; };
+  static thread_local Met met[64] = {};
+  const int key[8] = {images, pixels, C, groups, geeps_sm_count(), (backward ? 1 : 0) | (vec ? 2 : 0), xsize, ysize};
+  unsigned h = 0;
+  for (int k : key) h = (h ^ (unsigned)k) * 0x9E3779B1u;
+  Met& m = met[h >> 26];
+  if (memcmp(m.key, key, sizeof(key))) {
+    m.s = plan(images, pixels, C, groups, backward, vec, xsize, ysize);
+    memcpy(m.key, key, sizeof(key));
+  }
+  return m.s;
+}
+
+template <auto kernel, typename... A>
+int launch(const Shape& s, bool cluster, cudaStream_t st, A&&... args) {
+  static std::atomic<unsigned long long> ready{0};           // devices on which the kernel may have all shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    ready |= 1ull << (dev & 63);
+  }
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)s.blocks);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(s.threads);
   cfg.dynamicSmemBytes = s.smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -753,24 +853,25 @@ int launch(K kernel, const Shape& s, bool cluster, cudaStream_t st, A&&... args)
 
 template <typename XT, typename YT, bool VEC>
 int run(const GeepsGroupNorm& k, const Shape& s, const Dev& d, bool backward, cudaStream_t st) {
+  constexpr int ONE = VEC ? KEPT : TWICE;
   int e;
   if (!backward) {
-    if (s.fused) return launch(group_forward_kernel<XT, YT, VEC, FUSED>, s, true, st, d);
-    e = launch(group_forward_kernel<XT, YT, VEC, SUMS>, s, false, st, d);
-    return e ? e : launch(group_forward_kernel<XT, YT, VEC, APPLY>, s, false, st, d);
+    if (s.fused) return launch<group_forward_kernel<XT, YT, VEC, ONE>>(s, true, st, d);
+    e = launch<group_forward_kernel<XT, YT, VEC, SUMS>>(s, false, st, d);
+    return e ? e : launch<group_forward_kernel<XT, YT, VEC, APPLY>>(s, false, st, d);
   }
   const bool want = k.dweight != nullptr || k.dbias != nullptr;
   // group sums of the chunks (two launches only), then the channels' sums of the images or chunks
   const long long parts = (long long)k.images * (s.fused ? 1 : s.chunks);
   float* channel = want ? k.work + (s.fused ? 0 : parts * k.groups * 2) : nullptr;
   if (s.fused) {
-    e = launch(group_backward_kernel<XT, YT, VEC, FUSED>, s, true, st, d, channel);
+    e = launch<group_backward_kernel<XT, YT, VEC, ONE>>(s, true, st, d, channel);
   } else {
-    e = launch(group_backward_kernel<XT, YT, VEC, SUMS>, s, false, st, d, channel);
-    if (!e) e = launch(group_backward_kernel<XT, YT, VEC, APPLY>, s, false, st, d, channel);
+    e = launch<group_backward_kernel<XT, YT, VEC, SUMS>>(s, false, st, d, channel);
+    if (!e) e = launch<group_backward_kernel<XT, YT, VEC, APPLY>>(s, false, st, d, channel);
   }
   if (e || !want) return e;
-  geeps_launch(group_parameters_kernel, dim3((unsigned)((k.C + 31) / 32)), dim3(256), 0, st, (const float2*)channel, parts, k.C, k.dweight, k.dbias);
+  geeps_launch(group_parameters_kernel, dim3((unsigned)((k.C + 7) / 8)), dim3(256), 0, st, (const float2*)channel, parts, k.C, k.dweight, k.dbias);
   return (int)cudaGetLastError();
 }
 
@@ -790,7 +891,7 @@ int check(const GeepsGroupNorm* k, bool backward) {
   struct Range { const void* at; long long bytes; bool written; long long pitch; int align; };      // pitch: of rows, in bytes; 0: none
   auto span = [&](long long ld, int size) { return rows ? ((rows - 1) * ld + k->C) * size : 0; };
   if (k->ldx < k->C || (backward ? k->lddy < k->C || k->lddx < k->C : k->ldy < k->C)) return (int)cudaErrorInvalidValue;
-  const long long stats = k->images * k->groups * 8, work = geeps_group_norm_work(k->images, k->pixels, k->C, k->groups) * 4;
+  const long long stats = k->images * k->groups * 8, work = geeps_group_norm_work(k->images, k->pixels, k->C, k->groups, backward) * 4;
   const Range all[] = {
       {k->x, span(k->ldx, xs), false, k->ldx * xs, xs},
       {backward ? k->dy : nullptr, span(k->lddy, ys), false, k->lddy * ys, ys},
@@ -798,7 +899,7 @@ int check(const GeepsGroupNorm* k, bool backward) {
       {k->weight, 4LL * k->C, false, 0, 4}, {k->bias, 4LL * k->C, false, 0, 4},
       {k->stats, stats, !backward, 0, 8}, {k->work, work, true, 0, 8},
       {backward ? k->dweight : nullptr, 4LL * k->C, true, 0, 4}, {backward ? k->dbias : nullptr, 4LL * k->C, true, 0, 4}};
-  if (rows && (!k->x || !(backward ? (const void*)k->dx : k->y) || (backward && (!k->dy || !k->stats)) || !k->work)) return (int)cudaErrorInvalidValue;
+  if (rows && (!k->x || !(backward ? (const void*)k->dx : k->y) || (backward && (!k->dy || !k->stats)) || (work && !k->work))) return (int)cudaErrorInvalidValue;
   for (const auto& r : all) if (r.at && ((uintptr_t)r.at & (r.align - 1))) return GEEPS_ERR_NORM_ALIGN;
   for (const auto& a : all) {
     if (!a.at || !a.written || !a.bytes) continue;
@@ -842,10 +943,19 @@ int call(const GeepsGroupNorm* k, bool backward, void* stream) {
 
 extern "C" {
 
-long long geeps_group_norm_work(long long images, long long pixels, int C, int groups) {
-  // at most 2 SMs' worth of chunks beyond one an image, each with its groups' and channels' sums
-  if (images <= 0 || pixels <= 0 || C <= 0 || groups <= 0) return 2;
-  return (images + 20LL * geeps_sm_count() + 2) * 2 * ((long long)C + groups);
+long long geeps_group_norm_work(long long images, long long pixels, int C, int groups, int backward) {
+  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || images * pixels > (1LL << 30)) return 0;
+  // of two launches for vectors or single values, whichever the addresses will allow, of any type: the chunks' group sums; backward
+  // also the channels' sums of the chunks or images
+  long long most = 0;
+  for (int vec = 0; vec < (C % 8 ? 1 : 2); ++vec)
+    for (int type = 0; type < 3; ++type) {
+      const Shape s = choose((int)images, (int)pixels, C, groups, backward, vec, type ? 4 : 2, type == 2 ? 4 : 2);
+      const long long parts = images * (s.fused ? 1 : s.chunks);
+      const long long n = (s.fused ? 0 : parts * groups * 2) + (backward ? parts * C * 2 : 0);
+      most = n > most ? n : most;
+    }
+  return most;
 }
 
 int geeps_group_norm_forward(const GeepsGroupNorm* p, void* stream) { return call(p, false, stream); }
@@ -854,7 +964,7 @@ int geeps_group_norm_backward(const GeepsGroupNorm* p, void* stream) { return ca
 int geeps_group_norm_shape(long long images, long long pixels, int C, int groups, int backward, int vec, int x_fp32, int y_fp32, int* out) {
   if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || (vec && C % 8)) return (int)cudaErrorInvalidValue;
   const Shape s = choose((int)images, (int)pixels, C, groups, backward, vec, x_fp32 ? 4 : 2, y_fp32 ? 4 : 2);
-  out[0] = s.fused; out[1] = s.slice; out[2] = s.chunks; out[3] = s.rows; out[4] = s.keep; out[5] = s.blocks; out[6] = (int)s.smem; out[7] = kThreads;
+  out[0] = s.fused; out[1] = s.slice; out[2] = s.chunks; out[3] = s.rows; out[4] = s.keep; out[5] = s.blocks; out[6] = (int)s.smem; out[7] = s.threads;
   return 0;
 }
 

@@ -197,7 +197,7 @@ int geeps_norm_sums_shape(long long rows, long long gate_rows, int C, int mode, 
 // image, y = act(z); act: 0 none, 1 ReLU, 2 SiLU.  weight / bias: C floats or NULL (1 / 0).  stats: {mean, rstd} [images][groups],
 // written forward (or NULL there) and read backward.  Backward: dx, and dweight / dbias (C floats, or NULL).  x_fp32: x and dx are
 // fp32, else bf16; y_fp32 (with x_fp32 only): y and dy.  work: geeps_group_norm_work() floats at a multiple of 8 bytes, private to the
-// call while it runs.  Pitches in elements.  An output may be the very same rows as an input of its size, or other channels of
+// call while it runs (NULL where that is 0).  Pitches in elements.  An output may be the very same rows as an input of its size, or other channels of
 // the same wider rows; any other overlap of what is written is refused.  images x pixels is at most 2^30, C 1 to 16384.
 #define GEEPS_ERR_GROUPS (-16)
 typedef struct GeepsGroupNorm {
@@ -209,7 +209,7 @@ typedef struct GeepsGroupNorm {
   int C, groups, act, x_fp32, y_fp32;
   float eps;
 } GeepsGroupNorm;
-long long geeps_group_norm_work(long long images, long long pixels, int C, int groups);
+long long geeps_group_norm_work(long long images, long long pixels, int C, int groups, int backward);
 int geeps_group_norm_forward(const GeepsGroupNorm* p, void* stream);
 int geeps_group_norm_backward(const GeepsGroupNorm* p, void* stream);
 // launch shape (host arithmetic only), eight values: one launch of clusters or two launches, channels of a slice, chunks of an image,

@@ -662,38 +662,44 @@ class GroupNorm:
 
 
 def _group_norm(label, x, y, dy, dx, images, norm, work):
-    if x.dim() != 2:
-        raise ValueError(f"{label}: need [rows, channels], got {list(x.shape)}")
-    dev = _current_device(x, label)
-    rows, cols = x.shape
-    out, f32 = dx if dy is not None else y, torch.float32
-    xt, yt = x.dtype, (dy if dy is not None else y).dtype
+    shape, xt, f32 = x.shape, x.dtype, torch.float32
+    if len(shape) != 2:
+        raise ValueError(f"{label}: need [rows, channels], got {list(shape)}")
+    dev, backward, groups, st = _current_device(x, label), dy is not None, norm.groups, norm.stats
+    rows, cols = shape
+    yt = dy.dtype if backward else y.dtype
     if not ((xt is bf16 or xt is f32) and (yt is bf16 or (yt is f32 and xt is f32))):
         raise ValueError(f"{label}: types must be bf16, fp32, or fp32 x and dx with bf16 y and dy; got {xt}, {yt}")
     if images < 0 or (rows if images == 0 else rows % images):
         raise ValueError(f"{label}: {rows} rows are no whole pixels of {images} images")
     ld = []
-    at = (_operand(x, dev, x.shape, xt, "x", ld), 0 if dy is None else _operand(dy, dev, x.shape, yt, "dy", ld),
-          _operand(out, dev, x.shape, yt if dy is None else xt, "y" if dy is None else "dx", ld))
-    st = norm.stats
-    if st is not None:
-        _need(st.dtype is f32 and st.shape == (images, norm.groups, 2) and st.is_contiguous() and st.get_device() == dev,
-              f"{label}: stats: need contiguous fp32 [{images}, {norm.groups}, 2] on cuda:{dev}")
+    v = [_operand(x, dev, shape, xt, "x", ld)]
+    if backward:
+        v += (_operand(dy, dev, shape, yt, "dy", ld), 0, _operand(dx, dev, shape, xt, "dx", ld))
+        ld.insert(2, 0)
     else:
-        _need(dy is None, f"{label}: the backward pass needs the stats")
+        v += (0, _operand(y, dev, shape, yt, "y", ld), 0)
+        ld = [ld[0], 0, ld[1], 0]
+    if st is None:
+        if backward:
+            raise ValueError(f"{label}: the backward pass needs the stats")
+    elif not (st.dtype is f32 and st.shape == (images, groups, 2) and st.is_contiguous() and st.get_device() == dev):
+        raise ValueError(f"{label}: stats: need contiguous fp32 [{images}, {groups}, 2] on cuda:{dev}")
     pixels = rows // images if images else 0
-    n = lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), cols, norm.groups)
-    if work is None:
+    n, at = lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), cols, groups, backward), 0
+    if work is not None:
+        if not (work.dtype is f32 and work.is_contiguous() and work.numel() >= n and work.get_device() == dev):
+            raise ValueError(f"{label}: work needs {n} contiguous fp32 values on cuda:{dev}")
+        at = work.data_ptr()
+    elif n:
         work = L.hold(torch.empty(n, dtype=f32, device=x.device))
-    elif not (work.dtype is f32 and work.is_contiguous() and work.numel() >= n and work.get_device() == dev):
-        raise ValueError(f"{label}: work needs {n} contiguous fp32 values on cuda:{dev}")
-    w, b, dw, db = (0 if t is None else _column(t, dev, cols) for t in
-                    (norm.weight, norm.bias, norm.dweight if dy is not None else None, norm.dbias if dy is not None else None))
-    pitches = (ld[0], 0, ld[1], 0) if dy is None else (ld[0], ld[1], 0, ld[2])
-    launch(lib().geeps_group_norm_forward if dy is None else lib().geeps_group_norm_backward, label,
-           L.GROUP_NORM.pack(at[0], at[1], at[2] if dy is None else 0, 0 if dy is None else at[2], w, b, 0 if st is None else st.data_ptr(),
-                             work.data_ptr(), dw, db, images, pixels, *pitches, cols, norm.groups, GROUP_ACTS[norm.act], xt is f32,
-                             yt is f32, norm.eps),
+        at = work.data_ptr()
+    w, b, dw, db = norm.weight, norm.bias, norm.dweight, norm.dbias
+    launch(lib().geeps_group_norm_backward if backward else lib().geeps_group_norm_forward, label,
+           L.GROUP_NORM.pack(*v, 0 if w is None else _column(w, dev, cols), 0 if b is None else _column(b, dev, cols),
+                             0 if st is None else st.data_ptr(), at, 0 if dw is None or not backward else _column(dw, dev, cols),
+                             0 if db is None or not backward else _column(db, dev, cols), images, pixels, *ld, cols, groups,
+                             GROUP_ACTS[norm.act], xt is f32, yt is f32, norm.eps),
            C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
 
 
@@ -710,9 +716,9 @@ def group_norm_backward(x, dy, dx, images: int, norm: GroupNorm, work=None) -> N
     _group_norm("group_norm_backward", x, None, dy, dx, images, norm, work)
 
 
-def group_norm_work(images: int, pixels: int, cols: int, groups: int) -> int:
-    """fp32 values that group_norm_forward() and group_norm_backward() take as `work`."""
-    return lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), cols, groups)
+def group_norm_work(images: int, pixels: int, cols: int, groups: int, backward: bool) -> int:
+    """fp32 values that group_norm_forward() (0 where it needs none) or group_norm_backward() takes as `work`."""
+    return lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), cols, groups, int(backward))
 
 
 # ---- clipping of gradients by their global norm ----
@@ -805,10 +811,11 @@ class AdamWState:
         """m, v and the others may have been replaced (a restored run): they must still be what the kernel is told they are."""
         dev, n = self.params.device, self.blocks * 128
         dtype = torch.uint8 if self.bits == 8 else torch.float32
-        for t, shape, kind in ((self.m, (n,), dtype), (self.v, (n,), dtype), (self.steps, (2,), torch.int64)) + (
-                ((self.exponents, (self.blocks, 2), torch.uint8),) if self.bits == 8 else ()):
-            _need(t.dtype is kind and t.shape == shape and t.is_contiguous() and t.device == dev,
-                  f"AdamWState: m, v, exponents or steps need {kind} {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+        for t, shape, kind in ((self.m, (n,), dtype), (self.v, (n,), dtype), (self.steps, (2,), torch.int64),
+                               (self.exponents, (self.blocks, 2), torch.uint8)):
+            if not (t is None and self.bits == 32 and kind is torch.uint8) and not (
+                    t.dtype is kind and t.shape == shape and t.is_contiguous() and t.get_device() == dev.index):
+                raise ValueError(f"AdamWState: m, v, exponents or steps need {kind} {list(shape)} on {dev}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def adamw_step(params, grads, state: AdamWState, lr, *, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0, out=None,
@@ -826,8 +833,8 @@ def adamw_step(params, grads, state: AdamWState, lr, *, betas=(0.9, 0.999), eps:
     out = out if out is None or isinstance(out, GradList) else GradList(out)
     dev = _current_device(state.m, "adamw_step")
     for t in (params, grads, out):
-        _need(t is None or (t.numel == state.params.numel and t.device.index == dev),
-              "adamw_step: params, grads and out need the state's counts, on the current device")
+        if t is not None and (t.numel != state.params.numel or t.device.index != dev):
+            raise ValueError("adamw_step: params, grads and out need the state's counts, on the current device")
     state._check()
     beta1, beta2 = betas
     _need(0 <= beta1 < 1 and 0 <= beta2 < 1 and eps >= 0 and weight_decay >= 0, "adamw_step: need betas from 0 to below 1, eps and weight_decay from 0 up")
@@ -836,15 +843,15 @@ def adamw_step(params, grads, state: AdamWState, lr, *, betas=(0.9, 0.999), eps:
     k.decay, k.m, k.v, k.steps = C.addressof(state._decay), state.m.data_ptr(), state.v.data_ptr(), state.steps.data_ptr()
     k.exponents = None if state.exponents is None else state.exponents.data_ptr()
     if isinstance(lr, torch.Tensor):
-        _need(lr.dtype is torch.float32 and lr.numel() == 1 and lr.get_device() == dev, f"adamw_step: lr needs one fp32 value on cuda:{dev}")
+        if not (lr.dtype is torch.float32 and lr.numel() == 1 and lr.get_device() == dev):
+            raise ValueError(f"adamw_step: lr needs one fp32 value on cuda:{dev}")
         k.lr_ref = lr.data_ptr()
     else:
         k.lr = lr
     if clip is not None:
         norm, max_norm = clip
-        _need(norm.dtype is torch.float32 and norm.numel() >= 1 and norm.is_contiguous() and norm.get_device() == dev,
-              f"adamw_step: the norm needs fp32 on cuda:{dev}")
-        _need(max_norm >= 0, f"adamw_step: max_norm must be a number from 0 up, got {max_norm}")
+        if not (norm.dtype is torch.float32 and norm.numel() >= 1 and norm.is_contiguous() and norm.get_device() == dev and max_norm >= 0):
+            raise ValueError(f"adamw_step: clip needs an fp32 norm on cuda:{dev} and a bound from 0 up, got {max_norm}")
         k.norm, k.max_norm = norm.data_ptr(), max_norm
     k.beta1, k.beta2, k.eps, k.weight_decay = beta1, beta2, eps, weight_decay
     k.blocks, k.bits, k.stochastic, k.seed = state.blocks, state.bits, seed is not None, 0 if seed is None else seed & 0xFFFFFFFFFFFFFFFF
@@ -859,8 +866,8 @@ def adamw_moments(state: AdamWState, m: torch.Tensor, v: torch.Tensor):
     dev = _current_device(state.m, "adamw_moments")
     state._check()
     for t in (m, v):
-        _need(t.dtype in (bf16, torch.float32) and t.shape == state.m.shape and t.is_contiguous() and t.get_device() == dev,
-              f"adamw_moments: need {state.m.numel()} contiguous bf16 or fp32 values on cuda:{dev}")
+        if not (t.dtype in (bf16, torch.float32) and t.shape == state.m.shape and t.is_contiguous() and t.get_device() == dev):
+            raise ValueError(f"adamw_moments: need {state.m.numel()} contiguous bf16 or fp32 values on cuda:{dev}")
     for i, (codes, t) in enumerate(((state.m, m), (state.v, v))):
         launch(lib().geeps_adamw_moments, "adamw_moments", ptr(codes), ptr(state.exponents), ptr(t), i, int(t.dtype is torch.float32),
                C.c_longlong(state.blocks), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
@@ -872,13 +879,14 @@ class Fp8Matrix:
     """A matrix [rows, cols] in e4m3 with a scale 2^e for every 128 columns of a row: `q` (float8_e4m3fn, rows on a pitch of a
     multiple of 16) and `scale` (E8M0 bytes, 512 for 128 rows x 4 blocks, in the order in which the tensor cores take them).
     quantize_fp8() fills it, matmul_fp8() multiplies it."""
-    __slots__ = ("rows", "cols", "q", "scale")
+    __slots__ = ("rows", "cols", "q", "scale", "pitch", "device", "_at")
 
     def __init__(self, rows: int, cols: int, device):
         _need(0 <= rows < 1 << 30 and 0 < cols < 1 << 30, f"Fp8Matrix: need 0 to 2^30 rows and 1 to 2^30 columns, got {rows} x {cols}")
-        self.rows, self.cols = rows, cols
-        self.q = torch.zeros(rows, (cols + 15) // 16 * 16, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
+        self.rows, self.cols, self.pitch = rows, cols, (cols + 15) // 16 * 16
+        self.q = torch.zeros(rows, self.pitch, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
         self.scale = torch.zeros((rows + 127) // 128, (cols + 511) // 512, 512, dtype=torch.uint8, device=device)
+        self.device, self._at = self.q.get_device(), (self.q.data_ptr(), self.scale.data_ptr())
 
     def exponents(self) -> torch.Tensor:
         """e + 127 of every block, uint8 [rows, ceil(cols / 128)]; 255 where the block stands for NaN."""
@@ -892,18 +900,20 @@ class Fp8Matrix:
         return self.q.float() * scale.repeat_interleave(128, 1)[:, :self.cols]
 
 
-def _fp8(m, dev, shape, what):
-    _need(isinstance(m, Fp8Matrix) and (m.rows, m.cols) == shape and m.q.get_device() == dev,
-          f"{what}: need an Fp8Matrix {list(shape)} on cuda:{dev}")
-    return m
+def _fp8(m, dev, rows, cols, what) -> None:
+    if not (isinstance(m, Fp8Matrix) and m.rows == rows and m.cols == cols and m.device == dev):
+        raise ValueError(f"{what}: need an Fp8Matrix [{rows}, {cols}] on cuda:{dev}")
 
 
 def _rows(t, dev, what) -> int:
     """Pitch of a bf16 or fp32 matrix on the device whose rows are contiguous."""
-    _need(t.dim() == 2 and t.dtype in (bf16, torch.float32) and t.get_device() == dev, f"{what}: need a bf16 or fp32 matrix on cuda:{dev}")
-    _need(t.stride(1) == 1 or t.shape[1] == 1, f"{what}: columns must be contiguous, got strides {t.stride()}")
-    pitch = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    _need(pitch >= t.shape[1], f"{what}: rows overlap, got strides {t.stride()}")
+    if t.dim() != 2 or t.dtype not in (bf16, torch.float32) or t.get_device() != dev:
+        raise ValueError(f"{what}: need a bf16 or fp32 matrix on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
+    rows, cols = t.shape
+    s = t.stride()
+    pitch = s[0] if rows > 1 else cols
+    if (s[1] != 1 and cols != 1) or pitch < cols:
+        raise ValueError(f"{what}: columns must be contiguous and rows must not overlap, got strides {s}")
     return pitch
 
 
@@ -923,41 +933,45 @@ def quantize_fp8(x: torch.Tensor, out: "Fp8Matrix | None" = None, *, transposed:
     dev = _current_device(x, "quantize_fp8")
     ldx = _rows(x, dev, "quantize_fp8: x")
     rows, cols = x.shape
-    _need(cols > 0, "quantize_fp8: x has no columns")
+    if cols == 0:
+        raise ValueError("quantize_fp8: x has no columns")
     if out is None and transposed is None:
         out = L.hold(Fp8Matrix(rows, cols, x.device))
     p = L.QuantizeFp8()
     p.x, p.rows, p.cols, p.ldx, p.fp32, p.tile = x.data_ptr(), rows, cols, ldx, x.dtype is torch.float32, bool(tile)
     if out is not None:
-        _fp8(out, dev, (rows, cols), "quantize_fp8: out")
-        p.q, p.scale, p.ldq = out.q.data_ptr(), out.scale.data_ptr(), (cols + 15) // 16 * 16
+        _fp8(out, dev, rows, cols, "quantize_fp8: out")
+        (p.q, p.scale), p.ldq = out._at, out.pitch
     if transposed is not None and rows:
-        _fp8(transposed, dev, (cols, rows), "quantize_fp8: transposed")
-        p.qt, p.scale_t, p.ldqt = transposed.q.data_ptr(), transposed.scale.data_ptr(), (rows + 15) // 16 * 16
+        _fp8(transposed, dev, cols, rows, "quantize_fp8: transposed")
+        (p.qt, p.scale_t), p.ldqt = transposed._at, transposed.pitch
+    L.hold((x, out, transposed))
     launch(lib().geeps_quantize_fp8, "quantize_fp8", C.byref(p), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
     return transposed if out is None else out
 
 
 def matmul_fp8(a: "Fp8Matrix", b: "Fp8Matrix", out: torch.Tensor, *, bias: torch.Tensor | None = None, relu: bool = False,
-               status: torch.Tensor | None = None, plan=(0, 0, 0)) -> torch.Tensor:
+               status: torch.Tensor | None = None, plan=None) -> torch.Tensor:
     """out[M,N] = a[M,K] @ b[N,K]^T + bias, ReLU; out bf16 or fp32 with rows of any pitch, bias fp32 [N].  Products are exact and
     added in fp32.  plan: (tile width, CTAs that share K, operands swapped) instead of the choice by the sizes."""
     dev = _current_device(out, "matmul_fp8")
     ldc = _rows(out, dev, "matmul_fp8: out")
     M, N = out.shape
-    _need(isinstance(a, Fp8Matrix) and isinstance(b, Fp8Matrix) and a.cols == b.cols, "matmul_fp8: need two Fp8Matrix of as many columns")
-    _fp8(a, dev, (M, a.cols), "matmul_fp8: a")
-    _fp8(b, dev, (N, a.cols), "matmul_fp8: b")
+    K = a.cols
+    _fp8(a, dev, M, K, "matmul_fp8: a")
+    _fp8(b, dev, N, K, "matmul_fp8: b")
     p = L.GemmFp8()
-    p.A, p.B, p.scale_a, p.scale_b, p.C = a.q.data_ptr(), b.q.data_ptr(), a.scale.data_ptr(), b.scale.data_ptr(), out.data_ptr()
+    (p.A, p.scale_a), (p.B, p.scale_b), p.C = a._at, b._at, out.data_ptr()
     if bias is not None:
-        _need(bias.dtype is torch.float32 and bias.shape == (N,) and bias.is_contiguous() and bias.get_device() == dev,
-              f"matmul_fp8: bias needs {N} contiguous fp32 values on cuda:{dev}")
+        if not (bias.dtype is torch.float32 and bias.numel() == N and bias.is_contiguous() and bias.get_device() == dev):
+            raise ValueError(f"matmul_fp8: bias needs {N} contiguous fp32 values on cuda:{dev}")
         p.bias = bias.data_ptr()
-    p.status = status.data_ptr() if status is not None else None
-    p.M, p.N, p.K, p.ldc = M, N, a.cols, ldc
-    p.lda = p.ldb = (a.cols + 15) // 16 * 16
-    p.out_fp32, p.relu = out.dtype is torch.float32, bool(relu)
-    p.bn, p.cluster, p.swap = plan
+    if status is not None:
+        p.status = status.data_ptr()
+    p.M, p.N, p.K, p.ldc, p.lda, p.ldb = M, N, K, ldc, a.pitch, b.pitch
+    p.out_fp32, p.relu = out.dtype is torch.float32, relu
+    if plan is not None:
+        p.bn, p.cluster, p.swap = plan
+    L.hold((a, b, out, bias))
     launch(lib().geeps_gemm_fp8, "matmul_fp8", C.byref(p), C.c_void_p(torch._C._cuda_getCurrentRawStream(dev)))
     return out
