@@ -31,14 +31,13 @@ typedef __nv_bfloat16 bf16;
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kBlocks = 1024;                  // blocks a launch, at the most
-constexpr int kUnit = 4;                       // blocks of 128 that a warp has in flight
+constexpr int kUnit = 2;                       // blocks of 128 that a warp has in flight
+constexpr int resident(bool bits8, bool sr) { return bits8 || sr ? 3 : 4; }      // blocks of threads an SM
 
 struct Entry { void* p; const void* g; void* out; long long n; int place, first; };     // place: blocks of 128 before its states; first: units before it
 template <int MAX>
 struct Table {
   Entry e[MAX + 1];                // the last one has the number of units
-  unsigned short start[kBlocks];   // the tensor that block b starts in
   unsigned char type[MAX];         // bit 0: p is fp32, 1: g is, 2: out is, 3: decays, 4: vectors
   int n;
 };
@@ -53,44 +52,64 @@ struct Args {
   int last;                        // the last launch of the step
 };
 __host__ __device__ inline long long units_of(long long n) { return (n + 128 * kUnit - 1) / (128 * kUnit); }
-__host__ __device__ __forceinline__ int share(int units, int blocks, int b) { return (int)((long long)units * b / blocks); }
 
-__device__ __forceinline__ uint64_t mix64(uint64_t z) {
-  z += 0x9E3779B97F4A7C15ull;
+constexpr uint64_t kGamma = 0x9E3779B97F4A7C15ull;
+__device__ __forceinline__ uint64_t mix64_added(uint64_t z) {        // of a z that kGamma has been added to
   z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
   z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
   return z ^ (z >> 31);
 }
+__device__ __forceinline__ uint64_t mix64(uint64_t z) { return mix64_added(z + kGamma); }
 
-struct Step { float c, c1, c2, lr, lr_decay; uint64_t key, key_p; };       // of a launch (lr_decay: of a tensor)
+struct Step { float c, c1, c2, lr, lr_decay; uint64_t key, key_p; };       // of a launch (lr_decay: of a tensor; keys with kGamma added)
 
 // What a lane has of a block of 128: four values
 struct Values { float p[4], g[4], m[4], v[4]; };
 
-// The codes of four values and the exponent of their block.  TOP: the largest code.  r: random bits << 4, + 8, or nearest (even)
+// The codes of four values and the exponent of their block.  TOP: the largest code.  r: random bits << 4, + 8, or nearest (even).
+// The integer pipe bounds a step in 8 bits: sums with limits are one instruction, bytes move by permutations, the multiplications by
+// powers of two are IMADs, and what only zeros need stands behind a branch.
 template <int TOP, bool SR>
 __device__ __forceinline__ uint32_t encode(const float (&f)[4], const uint32_t (&r)[4], uint32_t& exponent) {
-  uint32_t mag[4], code = 0;
+  uint32_t mag[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) mag[j] = min(__float_as_uint(f[j]) & 0x7fffffffu, 0x7FC00000u);
+  for (int j = 0; j < 4; ++j) mag[j] = TOP == 255 ? __float_as_uint(f[j]) : __float_as_uint(f[j]) & 0x7fffffffu;
   const uint32_t top = __reduce_max_sync(0xffffffffu, max(max(mag[0], mag[1]), max(mag[2], mag[3])));
-  exponent = max((top + 0xFFFFFu) >> 23, 32u);
-  const int base = (int)(8 * exponent) - (TOP - 7);
+  exponent = min(max((top + 0xFFFFFu) >> 23, 32u), 255u);
+  const uint32_t base = ((TOP - 7) - 8 * exponent) << 20, up = base + 8u;      // of (bits >> 20) - base, and half of the last random bit
+  int c[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t up = SR ? r[j] : 0x7FFFFu + ((mag[j] >> 20) & 1u);
-    int c = max((int)((mag[j] + up) >> 20) - base, 0);
-    if (TOP == 255) c = mag[j] ? max(c, 1) : c;
-    else if (c && (__float_as_uint(f[j]) >> 31)) c += 128;
-    code |= (uint32_t)c << (8 * j);
+    // the bits as they are added: r holds 16 of them in its lower (m) or upper half (v)
+    const uint32_t add = SR ? (TOP == 255 ? r[j] >> 16 : r[j] & 0xffffu) * 16u + up : 0x7FFFFu + base + ((mag[j] >> 20) & 1u);
+    c[j] = __vimin_s32_relu((int)(mag[j] + add) >> 20, TOP);
   }
-  return code;
+  if (TOP == 255 && __any_sync(0xffffffffu, min(min(c[0], c[1]), min(c[2], c[3])) == 0)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = mag[j] ? max(c[j], 1) : c[j];
+  }
+  const uint32_t codes = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  if (TOP == 255) return codes;
+  const uint32_t high = __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0073),
+                                    __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0073), 0x5410);
+  return codes | (high & 0x80808080u);           // a zero may get a sign
 }
-template <int TOP>
-__device__ __forceinline__ float decode(uint32_t code, uint32_t exponent) {
-  const uint32_t mag = TOP == 255 ? code : code & 127u;
-  const uint32_t f = mag ? (mag + 8 * exponent - (TOP - 7)) << 20 : 0u;
-  return __uint_as_float(TOP == 255 ? f : f | (code & 128u) << 24);
+// WARP: all lanes of a warp call it together
+template <int TOP, bool WARP>
+__device__ __forceinline__ void decode(uint32_t codes, uint32_t exponent, float (&f)[4]) {
+  const uint32_t mags = TOP == 255 ? codes : codes & 0x7f7f7f7fu, base = (8 * exponent - (TOP - 7)) << 20;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t at16 = __byte_perm(mags, 0, 0x4044 | (j << 8));       // the byte at bits 16 to 23
+    uint32_t w = at16 * 16u + base;
+    if (TOP != 255) w |= __byte_perm(codes, 0, 0x0444 | (j << 12)) & 0x80000000u;
+    f[j] = __uint_as_float(w);
+  }
+  const bool zeros = TOP == 255 ? ((codes - 0x01010101u) & ~codes & 0x80808080u) != 0 : ((mags + 0x7f7f7f7fu) & 0x80808080u) != 0x80808080u;
+  if (WARP ? __any_sync(0xffffffffu, zeros) : zeros) {          // by the whole warp: as selections for each lane it would be done always
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = (mags >> (8 * j) & 255u) ? f[j] : 0.f;
+  }
 }
 
 // one value: the new states and the parameter's change
@@ -98,25 +117,27 @@ __device__ __forceinline__ float advance(const Args& a, const Step& s, float p, 
   g = __fmul_rn(g, s.c);
   m = __fadd_rn(__fmul_rn(m, a.b1), __fmul_rn(g, a.a1));
   v = __fadd_rn(__fmul_rn(v, a.b2), __fmul_rn(__fmul_rn(g, g), a.a2));
-  float root;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v * s.c2));       // 1 step of 2^-23 off, as the quotient: a change has 21 bits at least
-  const float q = __fdividef(m * s.c1, root + a.eps);
-  return fmaf(-s.lr, q, -s.lr_decay * p);
+  float root, inverse;
+  // a step or two of 2^-23 off, as the quotient: a change has 20 bits at least.  (A root below 1.1e-19 counts as 0 beside eps.)
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v * s.c2));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(root + a.eps));
+  return fmaf(-s.lr, m * s.c1 * inverse, -s.lr_decay * p);
 }
 // 32 random bits of each of a lane's four values, the first of which has the number i: neighbours, or every 32nd
 template <bool VEC>
 __device__ __forceinline__ void random4(uint64_t key, uint64_t i, uint32_t (&r)[4]) {
+  key += i >> 1;
   if (VEC) {
 #pragma unroll
     for (int j = 0; j < 4; j += 2) {
-      const uint64_t z = mix64(key + ((i + j) >> 1));
+      const uint64_t z = mix64_added(key + (j >> 1));
       r[j] = (uint32_t)z;
       r[j + 1] = (uint32_t)(z >> 32);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint64_t z = mix64(key + ((i + 32 * j) >> 1));
+      const uint64_t z = mix64_added(key + 16 * j);
       r[j] = (uint32_t)(i & 1 ? z >> 32 : z);
     }
   }
@@ -134,9 +155,22 @@ __device__ __forceinline__ void load_vector(const void* p, long long i, float (&
     f[2] = __uint_as_float(w.y << 16); f[3] = __uint_as_float(w.y & 0xffff0000u);
   }
 }
-__device__ __forceinline__ bf16 to_bf16(float f, bool stochastic, uint32_t r) {
-  if (stochastic && (__float_as_uint(f) & 0x7f800000u) != 0x7f800000u) f = __uint_as_float((__float_as_uint(f) + (r & 0xffffu)) & 0xffff0000u);
-  return __float2bfloat16(f);
+// Four values as bf16: to the nearest, or by random bits below the last one that is kept
+template <bool SR>
+__device__ __forceinline__ uint2 to_bf16(const float (&f)[4], const uint32_t (&r)[4]) {
+  if (SR) {
+    const float sum = (f[0] + f[1]) + (f[2] + f[3]);           // not finite if one is not (or if it overflows: then they are looked at)
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(f[j]) + (r[j] & 0xffffu);
+    if (__any_sync(0xffffffffu, (__float_as_uint(sum) & 0x7f800000u) == 0x7f800000u)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if ((__float_as_uint(f[j]) & 0x7f800000u) == 0x7f800000u) w[j] = (__float_as_uint(f[j]) & 0xffff0000u) | (f[j] != f[j] ? 0x400000u : 0u);
+    }
+    return make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+  }
+  return make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
 }
 
 // Blocks [b, b + COUNT) of a tensor by a warp.  VEC: whole blocks, vectors.
@@ -181,25 +215,20 @@ __device__ __forceinline__ void take(const Entry& e, unsigned type, const Args& 
   for (int k = 0; k < COUNT; ++k) {
     Values& y = x[k];
     if (BITS8) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        y.m[j] = decode<127>(mc[k] >> (8 * j) & 255u, ex[k] & 255u);
-        y.v[j] = decode<255>(vc[k] >> (8 * j) & 255u, ex[k] >> 8);
-      }
+      decode<127, true>(mc[k], ex[k] & 255u, y.m);
+      decode<255, true>(vc[k], ex[k] >> 8, y.v);
     }
     float change[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) change[j] = advance(a, s, y.p[j], y.g[j], y.m[j], y.v[j]);
-    uint32_t r[4], rm[4] = {}, rv[4] = {};
+    uint32_t r[4] = {};
     if (BITS8) {
       if (SR) {
         random4<VEC>(s.key, (uint64_t)(state + k * 128), r);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { rm[j] = ((r[j] & 0xffffu) << 4) + 8u; rv[j] = (r[j] >> 16 << 4) + 8u; }
       }
       uint32_t em, ev;
-      mc[k] = encode<127, SR>(y.m, rm, em);
-      vc[k] = encode<255, SR>(y.v, rv, ev);
+      mc[k] = encode<127, SR>(y.m, r, em);
+      vc[k] = encode<255, SR>(y.v, r, ev);
       if (lane == 0) ((unsigned short*)a.exponents)[e.place + b + k] = (unsigned short)(em | ev << 8);
     }
     if (!P32 && SR && e.out == nullptr) random4<VEC>(s.key_p, (uint64_t)(state + k * 128), r);
@@ -218,12 +247,13 @@ __device__ __forceinline__ void take(const Entry& e, unsigned type, const Args& 
       } else if (P32) {
         st_f4((float*)e.p + i, make_float4(y.p[0] + change[0], y.p[1] + change[1], y.p[2] + change[2], y.p[3] + change[3]));
       } else {
-        bf16 h[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = to_bf16(y.p[j] + change[j], SR, r[j]);
-        *(uint2*)((bf16*)e.p + i) = *(const uint2*)h;
+        const float f[4] = {y.p[0] + change[0], y.p[1] + change[1], y.p[2] + change[2], y.p[3] + change[3]};
+        *(uint2*)((bf16*)e.p + i) = to_bf16<SR>(f, r);
       }
     } else {
+      const float f[4] = {y.p[0] + change[0], y.p[1] + change[1], y.p[2] + change[2], y.p[3] + change[3]};
+      uint2 half = make_uint2(0, 0);
+      if (!P32 && e.out == nullptr) half = to_bf16<SR>(f, r);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const long long i = at + k * 128 + 32 * j, si = state + k * 128 + 32 * j;
@@ -238,9 +268,9 @@ __device__ __forceinline__ void take(const Entry& e, unsigned type, const Args& 
           if (e.out != nullptr) {
             if (type & 4) ((float*)e.out)[i] = change[j]; else ((bf16*)e.out)[i] = __float2bfloat16(change[j]);
           } else if (P32) {
-            ((float*)e.p)[i] = y.p[j] + change[j];
+            ((float*)e.p)[i] = f[j];
           } else {
-            ((bf16*)e.p)[i] = to_bf16(y.p[j] + change[j], SR, r[j]);
+            ((unsigned short*)e.p)[i] = (unsigned short)((j < 2 ? half.x : half.y) >> (16 * (j & 1)));
           }
         }
       }
@@ -251,15 +281,17 @@ template <bool BITS8, bool SR, bool P32, bool G32>
 __device__ __forceinline__ void unit(const Entry& e, unsigned type, const Args& a, const Step& s, long long b, int lane) {
   if ((type & 16) && (b + kUnit) * 128 <= e.n) {
     take<BITS8, SR, P32, G32, true, kUnit>(e, type, a, s, b, lane);
+  } else if ((b + kUnit - 1) * 128 < e.n) {
+    take<BITS8, SR, P32, G32, false, kUnit>(e, type, a, s, b, lane);
   } else {
     const long long end = (e.n + 127) >> 7;
 #pragma unroll 1
-    for (int k = 0; k < kUnit && b + k < end; ++k) take<BITS8, SR, P32, G32, false, 1>(e, type, a, s, b + k, lane);
+    for (; b < end; ++b) take<BITS8, SR, P32, G32, false, 1>(e, type, a, s, b, lane);
   }
 }
 
 template <bool BITS8, bool SR, int MAX>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, resident(BITS8, SR))
 adamw_kernel(const __grid_constant__ Table<MAX> t, const __grid_constant__ Args a) {
   geeps_pdl_enter();
   __shared__ float correction[2];
@@ -276,11 +308,14 @@ adamw_kernel(const __grid_constant__ Table<MAX> t, const __grid_constant__ Args 
   s.c1 = correction[0];
   s.c2 = correction[1];
   s.lr = a.lr_ref != nullptr ? *a.lr_ref : a.lr;
-  s.key = mix64(a.seed * 0x100000001B3ull + step);
-  s.key_p = mix64(s.key);
-  const int units = t.e[t.n].first, end = share(units, gridDim.x, blockIdx.x + 1);
-  int i = t.start[blockIdx.x];
-  for (int u = share(units, gridDim.x, blockIdx.x) + warp; u < end; u += kWarps) {
+  const uint64_t key = mix64(a.seed * 0x100000001B3ull + step);
+  s.key = key + kGamma;
+  s.key_p = mix64(key) + kGamma;
+  // all blocks go through the tensors side by side: with a range of its own for each (330 us, 274 for 61M fp32 in 8 bits with the
+  // moments' cast; 134M packed 642, 598) memory has five times as many places open
+  const int units = t.e[t.n].first;
+  int i = 0;
+  for (int u = blockIdx.x * kWarps + warp; u < units; u += gridDim.x * kWarps) {
     while (t.e[i + 1].first <= u) ++i;
     const Entry& e = t.e[i];
     const unsigned type = t.type[i];
@@ -301,28 +336,46 @@ adamw_kernel(const __grid_constant__ Table<MAX> t, const __grid_constant__ Args 
   }
 }
 
+// Two codes (bytes 2 i and 2 i + 1) as a pair of bf16, which hold them exactly: upper halves of what decode() makes
+template <int TOP>
+__device__ __forceinline__ uint32_t decode_pair(uint32_t codes, uint32_t base, int i) {
+  const uint32_t two = __byte_perm(codes, 0, i ? 0x4342 : 0x4140);
+  if (TOP == 255) return two * 16u + base;
+  return ((two & 0x007f007fu) * 16u + base) | (two & 0x00800080u) << 8;
+}
 // What the codes stand for: 16 of them a thread
-template <bool F32>
+template <bool F32, int TOP>
 __global__ void __launch_bounds__(256)
-moments_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exponents, void* __restrict__ out, int second, long long n16) {
+moments_kernel(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ exponents, void* __restrict__ out, long long n16) {
   geeps_pdl_enter();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n16; i += (long long)gridDim.x * 256) {
     const uint4 w = ((const uint4*)codes)[i];
-    const uint32_t c[4] = {w.x, w.y, w.z, w.w}, e = exponents[(i >> 3) * 2 + second];
-    float f[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint32_t b = c[j >> 2] >> (8 * (j & 3)) & 255u;
-      f[j] = second ? decode<255>(b, e) : decode<127>(b, e);
-    }
+    const uint32_t c[4] = {w.x, w.y, w.z, w.w}, e = exponents[(i >> 3) * 2 + (TOP == 255 ? 1 : 0)];
     if (F32) {
 #pragma unroll
-      for (int j = 0; j < 16; j += 4) st_f4((float*)out + i * 16 + j, make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]));
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        decode<TOP, false>(c[j], e, f);
+        st_f4((float*)out + i * 16 + 4 * j, make_float4(f[0], f[1], f[2], f[3]));
+      }
     } else {
+      const uint32_t base = ((8 * e - (TOP - 7)) << 4) * 0x10001u;
+      uint32_t o[8];
+      bool zeros = false;
 #pragma unroll
-      for (int j = 0; j < 16; j += 8)
-        *(uint4*)((bf16*)out + i * 16 + j) = make_uint4(pack_bf16x2(f[j], f[j + 1]), pack_bf16x2(f[j + 2], f[j + 3]),
-                                                        pack_bf16x2(f[j + 4], f[j + 5]), pack_bf16x2(f[j + 6], f[j + 7]));
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t mags = TOP == 255 ? c[j] : c[j] & 0x7f7f7f7fu;
+        zeros |= TOP == 255 ? ((c[j] - 0x01010101u) & ~c[j] & 0x80808080u) != 0 : ((mags + 0x7f7f7f7fu) & 0x80808080u) != 0x80808080u;
+        o[2 * j] = decode_pair<TOP>(c[j], base, 0);
+        o[2 * j + 1] = decode_pair<TOP>(c[j], base, 1);
+      }
+      if (zeros) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (!(c[j >> 2] >> (8 * (j & 3)) & (TOP == 255 ? 255u : 127u))) o[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+      }
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"((uint4*)out + 2 * i), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]),
+                   "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");       // a whole sector
     }
   }
 }
@@ -354,14 +407,8 @@ int run(const GeepsAdamW& k, cudaStream_t st) {
     }
     t.e[t.n].first = (int)units;
     a.last = from + MAX >= p.n;
-    const long long most = (long long)geeps_sm_count() * 4, want = (units + kWarps - 1) / kWarps;
-    int blocks = (int)(want < 1 ? 1 : want < most ? want : most);
-    if (blocks > kBlocks) blocks = kBlocks;
-    for (int b = 0, i = 0; b < blocks; ++b) {
-      const int u = share((int)units, blocks, b);
-      while (i + 1 < t.n && t.e[i + 1].first <= u) ++i;
-      t.start[b] = (unsigned short)i;
-    }
+    const long long most = (long long)geeps_sm_count() * resident(k.bits == 8, k.stochastic), want = (units + kWarps - 1) / kWarps;
+    const int blocks = (int)(want < 1 ? 1 : want < most ? want : most);
     auto kernel = k.bits == 8 ? (k.stochastic ? adamw_kernel<true, true, MAX> : adamw_kernel<true, false, MAX>)
                               : (k.stochastic ? adamw_kernel<false, true, MAX> : adamw_kernel<false, false, MAX>);
     geeps_launch(kernel, dim3(blocks), dim3(kThreads), 0, st, t, a);
@@ -411,10 +458,10 @@ extern "C" int geeps_adamw(const GeepsAdamW* k, void* stream) {
 }
 
 extern "C" int geeps_adamw_moments(const unsigned char* codes, const unsigned char* exponents, void* out, int second, int fp32, long long blocks, void* stream) {
-  if (blocks < 0 || !codes || !exponents || !out || (((uintptr_t)codes | (uintptr_t)out) & 15)) return (int)cudaErrorInvalidValue;
+  if (blocks < 0 || !codes || !exponents || !out || ((uintptr_t)codes & 15) || ((uintptr_t)out & 31)) return (int)cudaErrorInvalidValue;
   if (blocks == 0) return 0;
   const long long n16 = blocks * 8, want = (n16 + 255) / 256, most = (long long)geeps_sm_count() * 8;
-  geeps_launch(fp32 ? moments_kernel<true> : moments_kernel<false>, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, (cudaStream_t)stream,
-               codes, exponents, out, second, n16);
+  auto kernel = second ? (fp32 ? moments_kernel<true, 255> : moments_kernel<false, 255>) : (fp32 ? moments_kernel<true, 127> : moments_kernel<false, 127>);
+  geeps_launch(kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, (cudaStream_t)stream, codes, exponents, out, n16);
   return (int)cudaGetLastError();
 }
