@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
 }
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
 // byte of the 16-byte piece q of row r in a [128][bn] fp32 tile; the XOR keeps a column of rows off a single bank
@@ -65,6 +65,128 @@ __device__ __forceinline__ uint32_t part_off(int r, int q, int bn) { return (uin
 
 __device__ __forceinline__ void store1(const Dev& d, long long i, float v) {
   if (d.out_fp32) ((float*)d.C)[i] = v; else ((__nv_bfloat16*)d.C)[i] = __float2bfloat16(v);
+}
+
+// The epilogue of a group of four warps (group grp of G) for its share of a tile's columns: slabs 128 bytes wide (64 bf16 or 32 fp32
+// columns) leave with one TMA store each, clipped at the matrix edge.  r: the thread's row of the tile
+// TWO: two slabs a group, used in turn
+template <int G, bool TWO>
+__device__ __forceinline__ void store_slabs(const Dev& d, const CUtensorMap& tmC, uint8_t* slabs, uint32_t tacc, int m0, int n0, int grp, int r,
+                                            uint32_t& slab_i) {
+  const int cols = d.out_fp32 ? 32 : 64;
+  const bool issuer = threadIdx.x == 64 + 128 * grp;
+  const uint32_t row_off = (uint32_t)r * 128u, rsw = (uint32_t)(r & 7);
+#pragma unroll 1
+  for (int c = grp * cols; c < d.bn; c += G * cols) {
+    if ((long long)n0 + c >= d.N) break;
+    uint8_t* slab = slabs + (size_t)(TWO ? 2 * grp + (slab_i & 1u) : grp) * SLAB_BYTES;
+    if (issuer) { if (TWO) tc05::bulk_wait_read<1>(); else tc05::bulk_wait_read<0>(); }      // the slab this group stored there has been read out
+    tc05::named_bar_sync(1 + grp, 128);
+    for (int h = 0; h < cols; h += 32) {
+      uint32_t w[32];
+      tc05::tmem_ld_32x32(tacc + (uint32_t)(c + h), w);
+      tc05::tmem_ld_wait();
+      const long long col0 = (long long)n0 + c + h;
+      float v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(w[j]);
+      if (d.bias != nullptr) {
+        if (col0 + 32 <= d.N) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += __ldg(d.bias + col0 + j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] += col0 + j < d.N ? __ldg(d.bias + col0 + j) : 0.f;
+        }
+      }
+      if (d.relu) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];      // not fmaxf: a NaN stays one
+      }
+      if (d.out_fp32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4*>(slab + row_off + (uint32_t)((j ^ rsw) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(slab + row_off + (uint32_t)((((h >> 3) + j) ^ rsw) << 4)) =
+              make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                         pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+      }
+    }
+    tc05::fence_proxy_async_smem();
+    tc05::named_bar_sync(1 + grp, 128);
+    if (issuer) {
+      tc05::tma_store_2d(&tmC, slab, n0 + c, m0);
+      tc05::bulk_commit();
+    }
+    ++slab_i;
+  }
+}
+
+// A warp's 32 rows of an accumulator into the CTA's partial tile
+__device__ __forceinline__ void leave_part(uint8_t* part, uint32_t tacc, int r, int BN) {
+#pragma unroll 1
+  for (int c = 0; c < BN; c += 32) {
+    uint32_t v[32];
+    tc05::tmem_ld_32x32(tacc + (uint32_t)c, v);
+    tc05::tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<uint4*>(part + part_off(r, (c >> 2) + j, BN)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+}
+// Share z of the sums of a tile's partial tiles, which the CTAs of the cluster hold, in the order of their ranks
+__device__ __forceinline__ void finish_slices(const Dev& d, uint32_t part, uint32_t gave_up, int z, int m0, int n0) {
+  const int BN = d.bn, quads = BN >> 2, lane = threadIdx.x & 31;
+  // a CTA that gave up left no partial tile: nobody stores (the status word names it)
+  const bool stop = __any_sync(0xffffffffu, ld_cluster_u32(tc05::map_to_cta(gave_up, lane % d.cluster)) != 0u);
+  const long long ri = d.swap ? 1 : d.ldc, ci = d.swap ? d.ldc : 1;
+  const int items = stop ? 0 : BM * quads, end = (int)((long long)items * (z + 1) / d.cluster);
+  constexpr int U = 4;         // pieces of four columns that a thread has in flight of each slice: the way to another SM takes long
+  for (int i0 = (int)((long long)items * z / d.cluster) + threadIdx.x; i0 < end; i0 += U * blockDim.x) {
+    float4 v[U];
+    uint32_t off[U];
+    long long row[U], col0[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // neighbours in C are neighbouring threads
+      const int i = min(i0 + u * (int)blockDim.x, items - 1), r = d.swap ? i % BM : i / quads, o = d.swap ? i / BM : i % quads;
+      off[u] = part_off(r, o, BN);
+      row[u] = (long long)m0 + r;
+      col0[u] = i0 + u * (int)blockDim.x < end ? (long long)n0 + o * 4 : d.N;
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 2
+    for (int k = 0; k < d.cluster; ++k) {
+      const uint32_t at = tc05::map_to_cta(part, k);
+      float4 a[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) a[u] = i0 + u * (int)blockDim.x < end ? ld_cluster_f4(at + off[u]) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) { v[u].x += a[u].x; v[u].y += a[u].y; v[u].z += a[u].z; v[u].w += a[u].w; }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (row[u] >= d.M || col0[u] >= d.N) continue;
+      const int nc = (int)min((long long)4, d.N - col0[u]);
+      float w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (e < nc) {
+          if (d.bias != nullptr) w[e] += __ldg(d.bias + (d.swap ? row[u] : col0[u] + e));
+          if (d.relu) w[e] = w[e] < 0.f ? 0.f : w[e];
+        }
+      }
+      if (!d.swap && !d.out_fp32 && nc == 4 && (((uintptr_t)((__nv_bfloat16*)d.C + row[u] * d.ldc + col0[u])) & 7) == 0) {
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)d.C + row[u] * d.ldc + col0[u]) = make_uint2(pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) if (e < nc) store1(d, row[u] * ri + (col0[u] + e) * ci, w[e]);
+      }
+    }
+  }
 }
 
 // CL: a cluster of d.cluster CTAs per tile, one slice of K each
@@ -186,67 +308,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const long long row = (long long)m0 + r;
       if (CL) {
         // the commit behind tmem_full covers every MMA of the slice: the operand stages are free to hold the partial tile
-#pragma unroll 1
-        for (int c = 0; c < BN; c += 32) {
-          uint32_t v[32];
-          tc05::tmem_ld_32x32(tacc + (uint32_t)c, v);
-          tc05::tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<uint4*>(tiles + part_off(r, (c >> 2) + j, BN)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
+        leave_part(tiles, tacc, r, BN);
       } else if (d.tma_store) {
-        // slabs 128 bytes wide (64 bf16 or 32 fp32 columns) leave with one TMA store each, clipped at the matrix edge
-        const int cols = d.out_fp32 ? 32 : 64;
-        const bool issuer = threadIdx.x == 64 + 128 * grp;
-        const uint32_t row_off = (uint32_t)r * 128u, rsw = (uint32_t)(r & 7);
-#pragma unroll 1
-        for (int c = grp * cols; c < BN; c += G * cols) {
-          if ((long long)n0 + c >= d.N) break;
-          uint8_t* slab = slabs + (size_t)(2 * grp + (slab_i & 1u)) * SLAB_BYTES;
-          if (issuer) tc05::bulk_wait_read<1>();   // the slab this group stored two slabs ago has been read out
-          tc05::named_bar_sync(1 + grp, 128);
-          for (int h = 0; h < cols; h += 32) {
-            uint32_t w[32];
-            tc05::tmem_ld_32x32(tacc + (uint32_t)(c + h), w);
-            tc05::tmem_ld_wait();
-            const long long col0 = (long long)n0 + c + h;
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(w[j]);
-            if (d.bias != nullptr) {
-              if (col0 + 32 <= d.N) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += __ldg(d.bias + col0 + j);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += col0 + j < d.N ? __ldg(d.bias + col0 + j) : 0.f;
-              }
-            }
-            if (d.relu) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];      // not fmaxf: a NaN stays one
-            }
-            if (d.out_fp32) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<float4*>(slab + row_off + (uint32_t)((j ^ rsw) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint4*>(slab + row_off + (uint32_t)((((h >> 3) + j) ^ rsw) << 4)) =
-                    make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                               pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-            }
-          }
-          tc05::fence_proxy_async_smem();
-          tc05::named_bar_sync(1 + grp, 128);
-          if (issuer) {
-            tc05::tma_store_2d(&tmC, slab, n0 + c, m0);
-            tc05::bulk_commit();
-          }
-          ++slab_i;
-        }
+        store_slabs<G, true>(d, tmC, slabs, tacc, m0, n0, grp, r, slab_i);
       } else {
         // any pitch and alignment; with the operands swapped the lanes of a warp are neighbours in C
         const long long ri = d.swap ? 1 : d.ldc, ci = d.swap ? d.ldc : 1;
@@ -280,42 +344,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (CL) {
     __syncwarp();
     tc05::cluster_sync();
-    // this CTA finishes 128 / cluster rows of the tile, four columns per thread and step
-    const int rank = (int)(blockIdx.x % d.cluster), mn = (int)(blockIdx.x / d.cluster);
-    const int m0 = mn % d.m_tiles * BM, n0 = mn / d.m_tiles * BN;
-    const int rows = BM / d.cluster, quads = BN >> 2;
-    const uint32_t part = tc05::smem_u32(tiles);
-    // a CTA that gave up left no partial tile: nobody stores (the status word names it)
-    const uint32_t gave_up = ld_cluster_u32(tc05::map_to_cta(tc05::smem_u32(&ctl->abort_flag), lane % d.cluster));
-    const int todo = __any_sync(0xffffffffu, gave_up != 0u) ? 0 : rows * quads;
-    const long long ri = d.swap ? 1 : d.ldc, ci = d.swap ? d.ldc : 1;
-    for (int i = threadIdx.x; i < todo; i += blockDim.x) {
-      // neighbours in C are neighbouring threads
-      const int rr = d.swap ? i % rows : i / quads, o = d.swap ? i / rows : i % quads;
-      const int r = rank * rows + rr;
-      const long long row = (long long)m0 + r, col0 = (long long)n0 + o * 4;
-      if (row >= d.M || col0 >= d.N) continue;
-      const uint32_t off = part_off(r, o, BN);
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int z = 0; z < d.cluster; ++z) {
-        const float4 a = ld_cluster_f4(tc05::map_to_cta(part, z) + off);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-      }
-      const int nc = (int)min((long long)4, d.N - col0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (e < nc) {
-          if (d.bias != nullptr) v[e] += __ldg(d.bias + (d.swap ? row : col0 + e));
-          if (d.relu) v[e] = v[e] < 0.f ? 0.f : v[e];
-        }
-      }
-      if (!d.swap && !d.out_fp32 && nc == 4 && (((uintptr_t)((__nv_bfloat16*)d.C + row * d.ldc + col0)) & 7) == 0) {
-        *reinterpret_cast<uint2*>((__nv_bfloat16*)d.C + row * d.ldc + col0) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) if (e < nc) store1(d, row * ri + (col0 + e) * ci, v[e]);
-      }
-    }
+    const int mn = (int)(blockIdx.x / d.cluster);
+    finish_slices(d, tc05::smem_u32(tiles), tc05::smem_u32(&ctl->abort_flag), (int)(blockIdx.x % d.cluster), mn % d.m_tiles * BM, mn / d.m_tiles * BN);
     __syncwarp();
     tc05::cluster_sync();      // nobody leaves while a peer still reads its partial tile
   }
@@ -326,6 +356,132 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (warp == 1) {
     tc05::fence_after_sync();
     tc05::tmem_dealloc(tmem, (uint32_t)d.tmem_cols);
+  }
+}
+
+// Two CTAs compute a tile of 256 rows with MMAs of cta_group::2: each loads its own 128 rows of A and half of B's rows, and the scales
+// of its rows of A and of all of B's.  The leader issues the copies of scales and the MMAs for both; every load signals its barrier.
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(false), 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                     const __grid_constant__ CUtensorMap tmScaleA, const __grid_constant__ CUtensorMap tmScaleB, const Dev d) {
+  extern __shared__ uint8_t smem_raw[];
+  const int BN = d.bn;
+  const int B_BYTES = BN / 2 * BK, STAGE = A_BYTES + B_BYTES + SCALE_BYTES;
+  uint8_t* tiles = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* slabs = tiles + (size_t)d.stages * STAGE;
+  Ctl* ctl = (Ctl*)(slabs + d.slabs * SLAB_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc05::cluster_ctarank();
+  const int S = d.stages, num_tiles = d.m_tiles * d.n_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int b_atoms = (BN + 127) / 128;              // tiles begin at multiples of 64: these hold 64 + 192 rows as well as 192
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) { tc05::mbar_init(&ctl->full[s], 1); tc05::mbar_init(&ctl->empty[s], 1); }
+    for (int a = 0; a < 2; ++a) { tc05::mbar_init(&ctl->tmem_full[a], 1); tc05::mbar_init(&ctl->tmem_empty[a], 16); }
+    ctl->abort_flag = 0;
+    tc05::mbar_fence_init();
+  }
+  if (warp == 1) {
+    tc05::tmem_alloc_pair(&ctl->tmem_base, (uint32_t)d.tmem_cols);
+    tc05::tmem_relinquish_pair();
+  }
+  tc05::fence_before_sync();
+  __syncthreads();
+  tc05::cluster_sync();            // the peer's barriers are initialised before anything signals them
+  tc05::fence_after_sync();
+  const uint32_t tmem = ctl->tmem_base;
+  geeps_pdl_wait();          // everything above touches this CTA's own memory only
+  volatile int* abort_flag = &ctl->abort_flag;
+  const uint32_t tiles_u = tc05::smem_u32(tiles), empty_u = tc05::smem_u32(ctl->empty);
+
+  if (warp == 0) {
+    // ---------------- loads (both CTAs) ----------------
+    const bool leader = tc05::elect_one();
+    if (leader) { tc05::tma_prefetch_desc(&tmA); tc05::tma_prefetch_desc(&tmB); tc05::tma_prefetch_desc(&tmScaleA); tc05::tma_prefetch_desc(&tmScaleB); }
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = first; t < num_tiles && ok; t += step) {
+      const int mt = 2 * (t % d.m_tiles) + (int)rank, n0 = t / d.m_tiles * BN;
+      for (int kt = 0; kt < d.kt; ++kt) {
+        if (!tc05::mbar_wait_warp(&ctl->empty[s], ph ^ 1u, abort_flag, WAIT_BUDGET_NS)) { ok = false; break; }
+        if (leader) {
+          uint8_t* sa = tiles + (size_t)s * STAGE;
+          const bool scales = (kt & 3) == 0;
+          // the leader's barrier counts the bytes of both CTAs
+          if (rank == 0) tc05::mbar_expect_tx(&ctl->full[s], 2u * (uint32_t)(A_BYTES + B_BYTES + (scales ? ATOM * (1 + b_atoms) : 0)));
+          const uint32_t bar = tc05::map_to_cta(tc05::smem_u32(&ctl->full[s]), 0);
+          tc05::tma_load_2d_pair(sa, &tmA, bar, kt * BK, mt * BM);
+          tc05::tma_load_2d_pair(sa + A_BYTES, &tmB, bar, kt * BK, n0 + (int)rank * (BN / 2));
+          if (scales) {
+            // atoms behind the last row arrive as zeros
+            uint8_t* at = sa + A_BYTES + B_BYTES;
+            tc05::tma_load_2d_pair(at, &tmScaleA, bar, 0, mt * d.quads + (kt >> 2));
+            for (int i = 0; i < b_atoms; ++i) tc05::tma_load_2d_pair(at + ATOM * (1 + i), &tmScaleB, bar, 0, ((n0 >> 7) + i) * d.quads + (kt >> 2));
+          }
+        }
+        if (++s == S) { s = 0; ph ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- products (leader) ----------------
+    if (rank == 0) {
+      const bool leader = tc05::elect_one();
+      const uint32_t idesc = tc05::make_idesc_e4m3(2 * BM, BN);
+      uint32_t tile_i = 0, ph = 0, set = 0;
+      int s = 0;
+      bool ok = true;
+      for (int t = first; t < num_tiles && ok; t += step, ++tile_i) {
+        const int n0 = t / d.m_tiles * BN;
+        const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
+        if (!tc05::mbar_wait_warp(&ctl->tmem_empty[acc], acc_ph ^ 1u, abort_flag, WAIT_BUDGET_NS)) { ok = false; break; }
+        tc05::fence_after_sync();
+        const uint32_t tacc = tmem + acc * (uint32_t)BN;
+        uint32_t sf = 0;
+        for (int kt = 0; kt < d.kt; ++kt) {
+          if (!tc05::mbar_wait_warp(&ctl->full[s], ph, abort_flag, WAIT_BUDGET_NS)) { ok = false; break; }
+          tc05::fence_after_sync();
+          const uint32_t sa = tiles_u + (uint32_t)(s * STAGE), sb = sa + A_BYTES;
+          if ((kt & 3) == 0) {
+            sf = tmem + 2u * (uint32_t)BN + 16u * set;
+            if (++set == SCALE_SETS) set = 0;
+            if (leader) {
+              tc05::scale_copy_pair(sf, sb + B_BYTES);
+              for (int i = 0; i < b_atoms; ++i) tc05::scale_copy_pair(sf + 4u + 4u * i, sb + B_BYTES + ATOM * (1 + i));
+            }
+          }
+          tc05::mma_ktile_e4m3_pair(tacc, tc05::desc_lo(sa, 16), tc05::desc_lo(sb, 16), tc05::desc_hi(1024), idesc | tc05::idesc_scale_byte(kt & 3), sf,
+                                    sf + 4u + ((uint32_t)(n0 & 127) >> 5), kt > 0 ? 1u : 0u, empty_u + 8u * (uint32_t)s);
+          if (++s == S) { s = 0; ph ^= 1u; }
+        }
+        if (ok && leader) tc05::mma_commit_pair(&ctl->tmem_full[acc], 3);
+      }
+    }
+  } else {
+    // ---------------- epilogue (both CTAs): own 128 rows ----------------
+    const int q = warp & 3, grp = (warp - 2) >> 2;
+    uint32_t tile_i = 0, slab_i = 0;
+    for (int t = first; t < num_tiles; t += step, ++tile_i) {
+      const int m0 = (2 * (t % d.m_tiles) + (int)rank) * BM, n0 = t / d.m_tiles * BN;
+      const uint32_t acc = tile_i & 1u, acc_ph = (tile_i >> 1) & 1u;
+      if (!tc05::mbar_wait(&ctl->tmem_full[acc], acc_ph, abort_flag, WAIT_BUDGET_NS)) break;
+      tc05::fence_after_sync();
+      const uint32_t tacc = tmem + acc * (uint32_t)BN + ((uint32_t)(q * 32) << 16);
+      if (m0 < d.M) store_slabs<2, false>(d, tmC, slabs, tacc, m0, n0, grp, q * 32 + lane, slab_i);
+      tc05::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc05::mbar_arrive_cluster(tc05::map_to_cta(tc05::smem_u32(&ctl->tmem_empty[acc]), 0));      // the warps of both report
+    }
+  }
+  if (threadIdx.x == 64 || threadIdx.x == 192) tc05::bulk_wait<0>();
+  tc05::fence_before_sync();
+  __syncthreads();
+  if (threadIdx.x == 0 && ctl->abort_flag) geeps_report(d.status, GEEPS_ERR_TIMEOUT, KID_GEMM_FP8, (int)blockIdx.x, 1);
+  // neither CTA may release TMEM or exit while the peer can still signal its barriers or use the pair's TMEM
+  tc05::cluster_sync();
+  if (warp == 1) {
+    tc05::fence_after_sync();
+    tc05::tmem_dealloc_pair(tmem, (uint32_t)d.tmem_cols);
   }
 }
 
@@ -347,17 +503,17 @@ EncodeTiledFn encode_fn() {
 }
 // `outer` lines of `inner` values, `pitch` bytes apart
 bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, long long inner, long long outer, long long pitch,
-              int box_inner, int box_outer) {
+              int box_inner, int box_outer, bool swizzle = true) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
   cuuint64_t strides[1] = {(cuuint64_t)pitch};
   cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer}, one[2] = {1, 1};
-  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-struct Plan { int swap, bn, cluster; };
+struct Plan { int swap, bn, cluster, pair; };        // cluster: CTAs that share K; pair: CTA pairs
 // Tile widths: 64, 128 and 192 (two accumulators and the scales in 512 columns of TMEM), or 32 for a single tile.  The scales of a
 // tile then begin at an even column of TMEM; an MMA whose scales begin at an odd one is a misaligned access.
 bool width_ok(int bn, long long N) { return bn == 64 || bn == 128 || bn == 192 || (bn == 32 && N <= 32); }
@@ -365,44 +521,65 @@ bool width_ok(int bn, long long N) { return bn == 64 || bn == 128 || bn == 192 |
 // Whether an atom's worth of every slice is there
 bool slices_ok(int quads, int cluster) { return (long long)((quads + cluster - 1) / cluster) * (cluster - 1) < quads; }
 
+// The cut with the shortest expected time.  A k tile takes a round trip through the ring of stages (0.25 us, pairs 0.33) or what L2
+// needs for its operands (130 KB/us an SM, 15.5 MB/us in all): seldom the tensor pipe's time (0.2 us for 128 x 192), so wide tiles and
+// pairs win where there are enough of them, and slices of K where there are not.  In a captured chain, us (width / CTAs that share K,
+// p: pairs): 8192 x 16384, K = 4096 407 (192p), 482 (192/1), 588 (128/1); 1024 x 9216, K = 4096 32.2 (192p), 39.1, 39.2; 2048 x 4096,
+// K = 4096 31.8 (192p), 34.9, 36.6; 512 x 4096, K = 4096 11.8 (128/1), 13.9 (192p), 14.0; 256 x 4096, K = 9216 17.8 (128/2), 19.6
+// (64/1), 20.0 (128/1); with B's rows on the tall side 7 x 4096, K = 4096 7 (32/4), 8.3 (32/2), 10.3 (32/1).
 Plan choose(const GeepsGemmFp8* p, int sms) {
   const int quads = (int)((p->K + 511) / 512);
-  Plan best = {0, 64, 1};
-  double best_cost = 1e300;
-  for (int swap = 0; swap < 2; ++swap) {
-    const long long M = swap ? p->N : p->M, N = swap ? p->M : p->N;
-    if (swap && p->M > 128) continue;
-    const long long m_tiles = (M + BM - 1) / BM;
-    for (int bn = 32; bn <= 192; bn += 32) {
-      if (!width_ok(bn, N)) continue;
-      const long long tiles = m_tiles * ((N + bn - 1) / bn);
-      for (int cs = 1; cs <= 8; cs *= 2) {
-        if (cs > 1 && !slices_ok(quads, cs)) continue;
-        // SMs that whole clusters find in GPCs of different sizes
-        const long long slots = cs <= 2 ? sms : cs == 4 ? sms * 9 / 10 / 4 * 4 : sms * 5 / 6 / 8 * 8;
-        const long long rounds = (tiles * cs + slots - 1) / slots;
-        if (cs > 1 && rounds > 1) continue;
-        const double kt = 4.0 * ((quads + cs - 1) / cs);
-        double cost = rounds * (kt * ((M < BM ? M : BM) + bn < 192 ? 192.0 : (double)((M < BM ? M : BM) + bn)) + 1200.0);
-        if (cs > 1) cost += 1200.0 + 8.0 * bn;
-        if (cost < best_cost * 0.98) { best_cost = cost; best = {swap, bn, cs}; }
+  const bool rows16 = ((uintptr_t)p->C & 15) == 0 && p->ldc * (p->out_fp32 ? 4 : 2) % 16 == 0;
+  Plan best = {0, 64, 1, 0};
+  double least = 1e300;
+  for (int pair = 0; pair < 2; ++pair)
+    for (int swap = 0; swap < 2 - pair; ++swap) {
+      const long long M = swap ? p->N : p->M, N = swap ? p->M : p->N;
+      if ((swap && p->M > 128) || (pair && M <= BM)) continue;
+      const int tall = pair ? 2 * BM : BM;
+      for (int bn = 32; bn <= 192; bn += 32) {
+        if (pair ? bn % 64 : !width_ok(bn, N)) continue;
+        const long long tiles = ((M + tall - 1) / tall) * ((N + bn - 1) / bn);
+        for (int cs = 1; cs <= (pair ? 1 : 8); cs *= 2) {
+          if (!slices_ok(quads, cs) || (pair && !rows16)) continue;
+          const int size = pair ? 2 : cs;
+          // CTAs that whole clusters find in GPCs of different sizes
+          const int slots = size <= 2 ? sms : size <= 4 ? sms * 9 / 10 / size * size : sms * 5 / 6 / size * size;
+          const long long rounds = (tiles * size + slots - 1) / slots;
+          if (cs > 1 && rounds > 1) continue;
+          const double active = (double)(tiles * size < slots ? tiles * size : slots), kt = 4.0 * ((quads + cs - 1) / cs);
+          const double kb = 16.0 + (pair ? 0.5 : 1.0) * bn / 8;
+          double each = pair ? 0.33 : 0.25;
+          if (kb / 130.0 > each) each = kb / 130.0;
+          if (active * kb / 15500.0 > each) each = active * kb / 15500.0;
+          // an epilogue of single columns or of rows that TMA does not store is seen behind the products
+          const double over = cs > 1 ? 5.0 + bn / 64.0 : swap || !rows16 ? 2.5 + 0.03 * bn * rounds : 2.5;
+          const double time = rounds * kt * each + over;
+          if (time < least * 0.99) { least = time; best = {swap, bn, cs, pair}; }
+        }
       }
     }
-  }
   return best;
+}
+
+// Lets a kernel have all shared memory of the current device, once
+template <auto kernel>
+int all_shared() {
+  static std::atomic<unsigned long long> ready{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && !(ready >> (dev & 63) & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    ready |= 1ull << (dev & 63);
+  }
+  return (int)e;
 }
 
 template <bool CL>
 int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, const Dev& d, int grid, cudaStream_t st) {
   const size_t smem = (size_t)d.stages * (A_BYTES + d.bn * BK + SCALE_BYTES) + (CL ? 0 : d.slabs * SLAB_BYTES) + sizeof(Ctl) + 1024;
-  static std::atomic<unsigned long long> ready{0};           // devices on which the kernel may have all shared memory
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && !(ready >> (dev & 63) & 1)) {
-    e = cudaFuncSetAttribute(gemm_fp8_kernel<CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    ready |= 1ull << (dev & 63);
-  }
-  if (e != cudaSuccess) return (int)e;
+  const int e = all_shared<gemm_fp8_kernel<CL>>();
+  if (e) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(threads(CL));
@@ -431,12 +608,15 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
       p->lda < p->K || p->ldb < p->K || p->ldc < p->N)
     return (int)cudaErrorInvalidValue;
   const int sms = geeps_sm_count();
-  Plan plan = p->bn ? Plan{p->swap, p->bn, p->cluster} : choose(p, sms);
+  Plan plan = p->bn ? Plan{p->swap, p->bn, p->cluster < 0 ? 1 : p->cluster, p->cluster < 0} : choose(p, sms);
   Dev d = {};
   d.kt = (int)((p->K + BK - 1) / BK);
   d.quads = (d.kt + 3) / 4;
-  if (!width_ok(plan.bn, plan.swap ? p->M : p->N) || plan.cluster < 1 || plan.cluster > 8 || (plan.cluster & (plan.cluster - 1)) ||
-      !slices_ok(d.quads, plan.cluster))
+  const bool pair = plan.pair != 0;
+  const int size = p->out_fp32 ? 4 : 2;
+  const bool rows16 = ((uintptr_t)p->C & 15) == 0 && p->ldc * size % 16 == 0;       // what TMA stores
+  if (plan.cluster < 1 || plan.cluster > 8 || (plan.cluster & (plan.cluster - 1)) || !slices_ok(d.quads, plan.cluster) ||
+      (pair ? plan.swap || !rows16 || (plan.bn != 64 && plan.bn != 128 && plan.bn != 192) : !width_ok(plan.bn, plan.swap ? p->M : p->N)))
     return (int)cudaErrorInvalidValue;
   d.C = p->C; d.bias = p->bias; d.status = p->status;
   d.swap = plan.swap; d.relu = p->relu; d.out_fp32 = p->out_fp32;
@@ -444,29 +624,41 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
   d.scale_a = plan.swap ? p->scale_b : p->scale_a; d.scale_b = plan.swap ? p->scale_a : p->scale_b;
   const void *A = plan.swap ? p->B : p->A, *B = plan.swap ? p->A : p->B;
   const long long lda = plan.swap ? p->ldb : p->lda, ldb = plan.swap ? p->lda : p->ldb;
-  const int size = p->out_fp32 ? 4 : 2;
-  d.tma_store = plan.cluster == 1 && !plan.swap && ((uintptr_t)p->C & 15) == 0 && p->ldc * size % 16 == 0;
+  d.tma_store = plan.cluster == 1 && !plan.swap && rows16;
   d.bn = plan.bn;
   d.cluster = plan.cluster;
-  d.m_tiles = (int)((d.M + BM - 1) / BM);
+  d.m_tiles = (int)((d.M + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM));
   const long long n_tiles = (d.N + d.bn - 1) / d.bn;
   if (n_tiles * d.m_tiles > 0x3fffffffLL) return (int)cudaErrorInvalidValue;
   d.n_tiles = (int)n_tiles;
   d.tmem_cols = 32;
   while (d.tmem_cols < 2 * d.bn + 16 * SCALE_SETS) d.tmem_cols <<= 1;
   CUtensorMap ta, tb, tc;
-  if (!make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, p->K, d.M, lda, BK, BM) || !make_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, p->K, d.N, ldb, BK, d.bn))
+  if (!make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, p->K, d.M, lda, BK, BM) || !make_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, p->K, d.N, ldb, BK, pair ? d.bn / 2 : d.bn))
     return (int)cudaErrorInvalidValue;
   if (d.tma_store && !make_map(&tc, p->out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p->C, p->N, p->M,
                                p->ldc * size, p->out_fp32 ? 32 : 64, BM))
     d.tma_store = 0;
+  if (pair && !d.tma_store) return (int)cudaErrorInvalidValue;
   if (!d.tma_store) tc = ta;   // unused by the kernel
-  d.slabs = d.tma_store ? (d.bn > (p->out_fp32 ? 32 : 64) ? 4 : 2) : 0;
-  const int stage = A_BYTES + d.bn * BK + SCALE_BYTES;
+  d.slabs = d.tma_store ? (pair ? 2 : d.bn > (p->out_fp32 ? 32 : 64) ? 4 : 2) : 0;
+  const int stage = A_BYTES + (pair ? d.bn / 2 : d.bn) * BK + SCALE_BYTES;
   d.stages = (224 * 1024 - d.slabs * SLAB_BYTES) / stage;
   if (d.stages > MAX_STAGES) d.stages = MAX_STAGES;
   const long long tiles = (long long)d.m_tiles * d.n_tiles;
   cudaStream_t st = (cudaStream_t)stream;
+  if (pair) {
+    const long long rows_a = (d.M + 127) / 128 * d.quads, rows_b = (d.N + 127) / 128 * d.quads;
+    CUtensorMap sa, sb;
+    if (!make_map(&sa, CU_TENSOR_MAP_DATA_TYPE_UINT32, d.scale_a, ATOM / 4, rows_a, ATOM, ATOM / 4, 1, false) ||
+        !make_map(&sb, CU_TENSOR_MAP_DATA_TYPE_UINT32, d.scale_b, ATOM / 4, rows_b, ATOM, ATOM / 4, 1, false))
+      return (int)cudaErrorInvalidValue;
+    const int e = all_shared<gemm_fp8_pair_kernel>();
+    if (e) return e;
+    const size_t smem = (size_t)d.stages * stage + d.slabs * SLAB_BYTES + sizeof(Ctl) + 1024;
+    geeps_launch(gemm_fp8_pair_kernel, (int)(tiles < sms / 2 ? tiles : sms / 2) * 2, threads(false), smem, st, ta, tb, tc, sa, sb, d);
+    return (int)cudaGetLastError();
+  }
   if (d.cluster > 1) return launch<true>(ta, tb, tc, d, (int)(tiles * d.cluster), st);
   return launch<false>(ta, tb, tc, d, (int)(tiles < sms ? tiles : sms), st);
 }

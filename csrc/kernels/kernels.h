@@ -173,7 +173,7 @@ typedef struct GeepsGemmFp8 {
   int* status;
   long long M, N, K, lda, ldb, ldc;
   int out_fp32, relu;
-  int bn, cluster, swap;       // bn 0: chosen.  Tile width (64, 128, 192, or 32 where one tile is enough); CTAs that share K; B's rows on the 128-row side
+  int bn, cluster, swap;       // bn 0: chosen.  Tile width (64, 128, 192, or 32 where one tile is enough); CTAs that share K, or -2 for CTA pairs; B's rows on the 128-row side
 } GeepsGemmFp8;
 int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream);
 int geeps_clear_f32(float* c, long long n, void* stream);           // n zeros
