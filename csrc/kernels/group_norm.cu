@@ -762,15 +762,24 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
   const int row_bytes = s.threads * 16 * (vec ? (xsize / 2 + (backward ? ysize / 2 : 0)) : 0);      // of all threads' kept rows
   // One launch: slices of 32 channels (whole sectors of a pixel) and more, and up to eight CTAs for an item.  The cost is how often the
   // machine is filled by three CTAs an SM x what one takes, some 6 us and 1 us for 10 KB.
-  auto cut = [&](Shape& t) {
+  auto cut = [&](Shape& t) {             // what a thread has of a slice
     t.V = t.slice / W;
     t.R = t.V < t.threads ? t.threads / t.V : 1;
     t.entries = (((backward ? t.R > 1 : t.V <= t.threads) ? t.R * t.slice * 8 : 0) + 15) & ~15;
   };
   double best = 1e300;
   int chunks = 0;
-  for (int n = 1; unit * n <= C && (n == 1 || unit * n <= W * s.threads); ++n) {
-    if (C / unit % n || (unit * n < 32 && unit * n < C)) continue;
+  // ... narrower ones only where the channels have no such divisor
+  const int limit = W * s.threads < C ? W * s.threads : C;
+  int least = C < 32 ? 1 : 32;
+  while (least > 1) {
+    int n = (least + unit - 1) / unit;
+    while (unit * n <= limit && C / unit % n) ++n;
+    if (unit * n <= limit || unit >= least) break;
+    least = 1;
+  }
+  for (int n = 1; n == 1 || unit * n <= limit; ++n) {
+    if (C / unit % n || unit * n < least) continue;
     Shape t = s;
     t.slice = unit * n;
     t.slices = C / t.slice;
@@ -794,10 +803,14 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
     s.fused = 0;
     int n = 1;
     while (unit * n < C && (unit * n < 64 || C / unit % n)) ++n;
-    s.slice = unit * n;
-    s.slices = C / s.slice;
     s.threads = threads_of(SUMS);
-    cut(s);
+    for (;; --n) {                             // down to a width that fits (one group does)
+      if (C / unit % n) continue;
+      s.slice = unit * n;
+      s.slices = C / s.slice;
+      cut(s);
+      if (fixed_bytes(s, cg, backward) + s.entries <= kSmem) break;
+    }
     const long long items = (long long)images * s.slices;
     const long long want = (2LL * sms + items - 1) / items, most = (pixels + s.R - 1) / s.R;
     chunks = (int)(want < most ? want : most);

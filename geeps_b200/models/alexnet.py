@@ -6,7 +6,8 @@ from ..ops.layers import LRN, Conv2d, Dropout, Input, Linear, Pool
 from .net import Net
 
 
-def alexnet(num_classes: int = 1000, dropout: float = 0.5) -> Net:
+def alexnet(num_classes: int = 1000, dropout: float = 0.5, fp8: bool = False) -> Net:
+    """fp8: the products of the fully-connected layers run on 8-bit matrices (ops.layers.Linear)."""
     layers = [
         # the input layer emits a space-to-depth(4) layout [B, 57, 57, 48 + 16 zero channels]: the 11 x 11 stride-4
         # convolution becomes a 3 x 3 stride-1 implicit GEMM (taps past 11 and the padding channels are zero
@@ -21,10 +22,10 @@ def alexnet(num_classes: int = 1000, dropout: float = 0.5) -> Net:
         Conv2d("conv4", 384, 3, pad=1, groups=2, relu=True, std=0.01, bias_value=0.1),
         Conv2d("conv5", 256, 3, pad=1, groups=2, relu=True, std=0.01, bias_value=0.1),
         Pool("max", 3, 2),
-        Linear("fc6", 4096, relu=True, std=0.005, bias_value=0.1),
+        Linear("fc6", 4096, relu=True, std=0.005, bias_value=0.1, fp8=fp8),
         Dropout(dropout, seed=61),
-        Linear("fc7", 4096, relu=True, std=0.005, bias_value=0.1),
+        Linear("fc7", 4096, relu=True, std=0.005, bias_value=0.1, fp8=fp8),
         Dropout(dropout, seed=71),
-        Linear("fc8", num_classes, std=0.01, fp32_out=True),
+        Linear("fc8", num_classes, std=0.01, fp32_out=True, fp8=fp8),
     ]
     return Net("alexnet", Input(s2d=4, s2d_k=11, cpad=64), layers)

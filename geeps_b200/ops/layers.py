@@ -397,10 +397,12 @@ class Conv2d(Layer):
 
 
 class Linear(Layer):
-    def __init__(self, name, out_features, relu=False, std=0.01, bias_value=0.0, need_dx=True, fp32_out=False):
+    def __init__(self, name, out_features, relu=False, std=0.01, bias_value=0.0, need_dx=True, fp32_out=False, fp8=False):
+        """fp8: the three products run on e4m3 matrices with a scale for each block of 128 (weights 128 x 128), which are cast from the
+        bf16 values in every step.  Takes no effect on a table whose rows are pulled by the forward product (PSModule(pull_fc=True))."""
         super().__init__()
         self.name, self.out, self.relu, self.std, self.bias_value = name, out_features, relu, std, bias_value
-        self.need_dx, self.fp32_out = need_dx, fp32_out
+        self.need_dx, self.fp32_out, self.fp8 = need_dx, fp32_out, fp8
 
     def setup(self, in_shape, device):
         self.in_shape = in_shape
@@ -415,6 +417,10 @@ class Linear(Layer):
         ybuf = torch.zeros(B, self.out_ld, dtype=torch.float32 if self.fp32_out else BF, device=device)
         self.y = ybuf[:, :self.out]
         self.dx = torch.empty(B, self.k_in, dtype=BF, device=device) if self.need_dx else None
+        if self.fp8:
+            self.xq, self.wq = F.Fp8Matrix(B, self.k_in, device), F.Fp8Matrix(self.out, self.k_in, device)
+            self.xt, self.dyt = F.Fp8Matrix(self.k_in, B, device), F.Fp8Matrix(self.out, B, device)
+            self.wt, self.dyq = (F.Fp8Matrix(self.k_in, self.out, device), F.Fp8Matrix(B, self.out, device)) if self.need_dx else (None, None)
         self.device = device
         self.out_shape = (B, self.out)
         return self.out_shape
@@ -432,6 +438,11 @@ class Linear(Layer):
             shards, n_start = pull
             F.pull_gemm(self.x, shards, n_start, self.y, ldw=self.ld, bias=self.p32["bias"], relu=self.relu,
                         w_local=self.p16["weight"])
+        elif self.fp8:
+            # transposes are for the backward pass: each of x, W and dy is read once for its two products
+            F.quantize_fp8(self.x, self.xq, transposed=self.xt if self.training else None)
+            F.quantize_fp8(self.p16["weight"], self.wq, transposed=self.wt if self.training else None, tile=True)
+            F.matmul_fp8(self.xq, self.wq, self.y, bias=self.p32["bias"], relu=self.relu)
         elif self._split_k():
             # batch-sized M: two or four wide output tiles would leave most SMs idle while the weights stream, so the
             # k range is split over the SMs (partial sums reduce-added in fp32) and a finishing pass converts
@@ -468,6 +479,13 @@ class Linear(Layer):
         else:
             F.colsum(dy, self.g32["bias"])
         # dW[out, in] = dy^T @ x ; dx[B, in] = dy @ W
+        if self.fp8 and not getattr(self, "pull", None):
+            F.quantize_fp8(dy, self.dyq, transposed=self.dyt)
+            F.matmul_fp8(self.dyt, self.xt, self.g32["weight"])
+            if not self.need_dx:
+                return None
+            F.matmul_fp8(self.dyq, self.wt, self.dx)
+            return self.dx.view(self.in_shape)
         F.gemm(dy, self.x, self.g32["weight"], a_mn=True, b_mn=True, split_k=0)
         if self.need_dx:
             if self._split_k():
@@ -591,6 +609,48 @@ class Norm(Layer):
         """dres: a gradient that reaches the input on another way, added to dx."""
         dy = dy if dy.dim() == 2 else dy.view(self.P, self.C)
         F.norm_backward(self.x, dy, self.dx, self.norm(self.p32, self.g32, backward=True), dres=dres, work=self.work)
+        return self.dx
+
+
+class GroupNorm(Layer):
+    """Group norm over the pixels of each image with an activation (None, "relu" or "silu") behind it: no statistics of the batch,
+    so a worker's share of it may have any size and nothing has to be kept for inference."""
+
+    def __init__(self, name, groups=32, act=None, eps=1e-5):
+        super().__init__()
+        self.name, self.groups, self.act, self.eps = name, groups, act, eps
+
+    def setup(self, in_shape, device):
+        self.in_shape = self.out_shape = tuple(in_shape)
+        self.B, self.C, self.P = in_shape[0], in_shape[-1], 1
+        for s in in_shape[:-1]:
+            self.P *= s
+        if self.C % self.groups:
+            raise ValueError(f"{self.name}: {self.groups} groups do not divide {self.C} channels")
+        self.y = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.dx = torch.empty(self.P, self.C, dtype=BF, device=device)
+        self.stats = torch.empty(self.B, self.groups, 2, device=device)
+        pixels = self.P // self.B
+        self.work = torch.empty(max(F.group_norm_work(self.B, pixels, self.C, self.groups, b) for b in (False, True)), device=device)
+        return self.out_shape
+
+    def param_specs(self):
+        return [ParamSpec("gamma", (self.C,), "const:1.0", decay=False), ParamSpec("beta", (self.C,), "const:0.0", decay=False)]
+
+    def bind_output(self, y2d):
+        self.y = y2d
+
+    def _norm(self, dgamma=None, dbeta=None):
+        return F.GroupNorm(self.groups, self.p32["gamma"], self.p32["beta"], self.stats, self.eps, self.act, dgamma, dbeta)
+
+    def forward(self, x):
+        self.x = x if x.dim() == 2 else x.view(self.P, self.C)
+        F.group_norm_forward(self.x, self.y, self.B, self._norm(), work=self.work)
+        return self.y
+
+    def backward(self, dy):
+        dy = dy if dy.dim() == 2 else dy.view(self.P, self.C)
+        F.group_norm_backward(self.x, dy, self.dx, self.B, self._norm(self.g32["gamma"], self.g32["beta"]), work=self.work)
         return self.dx
 
 

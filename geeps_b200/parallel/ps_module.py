@@ -18,7 +18,7 @@ import torch
 from ..ops import _lib as L
 from ..ops import functional as F
 from ..ops.layers import BF
-from ..utils.config import TRANSPORT_NVLINK, GeePsConfig
+from ..utils.config import TABLE_ADDITIVE, TRANSPORT_NVLINK, GeePsConfig
 from ..utils.trace import NullTrace
 from .ps import ROW_FLOATS, GeePs
 
@@ -46,12 +46,52 @@ class _Table:
         return {sp.name: flat[o:o + sp.numel].view(sp.shape) for sp, o in zip(self.specs, self.offsets)}
 
 
+class _AdamW:
+    """The AdamW step of a module's tables: gradients in the update buffers become the updates."""
+
+    def __init__(self, device, world, learning_rate, weight_decay, betas=(0.9, 0.999), eps: float = 1e-8, bits: int = 32, seed: int | None = None):
+        self.betas, self.eps, self.bits, self.seed, self.weight_decay, self.world = betas, eps, bits, seed, weight_decay, world
+        self.lr = torch.tensor([learning_rate / world], device=device)
+        self.state, self._lists = None, {}
+
+    def set(self, learning_rate=None, weight_decay=None) -> bool:
+        """Whether a recorded step carries an old value."""
+        if learning_rate is not None:
+            self.lr.fill_(learning_rate / self.world)
+        changed = weight_decay is not None and weight_decay != self.weight_decay
+        if changed:
+            self.weight_decay = weight_decay
+        return changed
+
+    def step(self, mod) -> None:
+        names = [(t.layer, sp) for t in mod.tables for sp in t.specs]
+        params, grads = [l.p32[sp.name] for l, sp in names], [l.g32[sp.name] for l, sp in names]
+        # laid out once for each phase of the update ring, so that a recorded step finds the same arguments again
+        at = [x.data_ptr() for x in params] + [x.data_ptr() for x in grads]
+        lists = self._lists.get(mod.steps % mod._period)
+        if lists is None or lists[0] != at:
+            lists = self._lists[mod.steps % mod._period] = (at, F.GradList(params), F.GradList(grads))
+        _, params, grads = lists
+        if self.state is None:
+            self.state = F.AdamWState(params, self.bits, [sp.decay for _, sp in names])
+        clip = None
+        if mod.clip_gradients is not None:
+            if mod._clip_work is None:
+                mod._clip_work = torch.empty(grads.work_size(), dtype=torch.float64, device=mod.device)
+            F.clip_gradients(grads, float("inf"), mod.clip_result, work=mod._clip_work)
+            clip = (mod.clip_result, mod.clip_gradients)
+        F.adamw_step(params, grads, self.state, self.lr, betas=self.betas, eps=self.eps, weight_decay=self.weight_decay, out=grads, clip=clip,
+                     seed=self.seed)
+
+
 class PSModule:
+    adamw = None
+
     def __init__(self, net, in_shape, ps_config: GeePsConfig, rank: int = 0, world: int = 1, device="cuda:0",
                  slack: int = 0, seed: int = 0, keep_init: bool = False, trace=None, manage_activations: bool = False,
                  cache_fraction: float | None = None, use_tape: bool = False, bf16_weights_only: bool = False,
                  use_graph: bool = False, pull_fc: bool = False, uncached=(), resume_from: str | None = None,
-                 clip_gradients: float | None = None):
+                 clip_gradients: float | None = None, adamw: dict | None = None):
         """bf16_weights_only: with the NVLINK transport and the bf16 compute cache, weight rows are published to
         the workers' bf16 caches only (the layers never read weights in fp32; biases, BatchNorm scale / shift and
         the shard's master rows stay fp32).  The fp32 views of weights (`params_fp32`) then keep their initial
@@ -74,7 +114,14 @@ class PSModule:
         clip_gradients: scale the worker's gradients by clip_gradients / norm where the norm of all of them exceeds it
         (Caffe's solver parameter; every worker clips its own batch's).  No table is then pushed before the backward pass has
         ended, and the update buffers of all tables are held until then.  `clip_result` holds the last step's {norm, factor};
-        inf only measures."""
+        inf only measures.
+        adamw: the worker computes the updates of all tables with one AdamW step (F.adamw_step) at the end of the backward pass and the
+        shards add them (tables must be TABLE_ADDITIVE): a dict of betas, eps, bits (32, or 8 for states in 8 bits) and seed (of
+        stochastic rounding; None: to the nearest), each optional.  The rate is ps_config.learning_rate (set_hyper_params changes it
+        without a new capture), the decay ps_config.weight_decay, for the parameters that decay.  Of several workers each takes 1 /
+        world of its own step.  With clip_gradients the gradients are scaled on their way into the step and `clip_result` holds {norm, 1}.
+        Parameters are given back when the step has read them.  The states (`adamw.state`) are the worker's own and not part of a
+        table snapshot."""
         self.net, self.rank, self.world, self.slack = net, rank, world, slack
         self.device = torch.device(device)
         self.trace = trace or NullTrace()
@@ -168,6 +215,10 @@ class PSModule:
         self.clip_gradients = clip_gradients
         self.clip_result = None if clip_gradients is None else torch.zeros(2, device=self.device)
         self._clip_lists, self._clip_work = {}, None
+        if adamw is not None:
+            if self.device.type != "cuda" or ps_config.table_mode != TABLE_ADDITIVE or pull_fc or bf16_weights_only:
+                raise ValueError("adamw needs a GPU, additive tables and fp32 parameters of the worker (neither pull_fc nor bf16_weights_only)")
+            self.adamw = _AdamW(self.device, world, ps_config.learning_rate, ps_config.weight_decay, **adamw)
         self._declare()
         if resume_from is not None:
             if not self.ps.load_snapshot(resume_from):
@@ -202,17 +253,23 @@ class PSModule:
             for t in reversed(tabs):
                 t.h_pre = ps.virtual_pre_update(t.table_id, range(t.rows))
             for t in reversed(tabs):
-                t.h_post = ps.virtual_post_read(t.h_read)
-                if self.clip_gradients is None:
+                if self.adamw is None:
+                    t.h_post = ps.virtual_post_read(t.h_read)
+                if not self._updates_late():
                     t.h_upd = ps.virtual_update(t.h_pre)
             if i in M:
                 M[i]["pb"] = ps.virtual_post_local_access(M[i]["b"], False)
-        if self.clip_gradients is not None:       # only the updates wait for all gradients
+        if self._updates_late():       # the updates wait for all gradients, with AdamW the parameters, too
             for _, tabs in reversed(self.groups):
                 for t in reversed(tabs):
+                    if self.adamw is not None:
+                        t.h_post = ps.virtual_post_read(t.h_read)
                     t.h_upd = ps.virtual_update(t.h_pre)
         ps.virtual_clock()
         ps.finish_virtual_iteration()
+
+    def _updates_late(self) -> bool:
+        return self.clip_gradients is not None or self.adamw is not None
 
     def _update(self, name, tabs, post_read, update):
         if tabs:
@@ -385,16 +442,21 @@ class PSModule:
                 t.layer.g32 = t.views(self.ps.pre_update(t.h_pre))
             with tr.span(f"bwd:{name}", "bwd"):
                 g = l.backward(g)
-            self._update(name, tabs, post_read=True, update=self.clip_gradients is None)
+            self._update(name, tabs, post_read=self.adamw is None, update=not self._updates_late())
             if i in M:
                 self.ps.post_local_access(M[i]["pb"])
             self._mark("b:" + name)
-        if self.clip_gradients is not None:
-            with tr.span("clip", "bwd"):
-                self._clip()
-            self._mark("clip")
+        if self._updates_late():
+            if self.adamw is not None:
+                with tr.span("adamw", "bwd"):
+                    self.adamw.step(self)
+                self._mark("adamw")
+            else:
+                with tr.span("clip", "bwd"):
+                    self._clip()
+                self._mark("clip")
             for l, tabs in reversed(self.groups):
-                self._update(getattr(l, "name", type(l).__name__), tabs, post_read=False, update=True)
+                self._update(getattr(l, "name", type(l).__name__), tabs, post_read=self.adamw is not None, update=True)
         if ev is not None:
             ev[-1][2].record()
         with tr.span("clock", "ps", clock=self.steps):
@@ -423,7 +485,14 @@ class PSModule:
     def set_hyper_params(self, learning_rate=None, momentum=None, weight_decay=None) -> None:
         """Change the optimizer's learning rate / momentum / weight decay from the next step on (every rank makes the
         same call before the same step).  Recorded and captured steps carry the old values in their push launches, so
-        they are dropped when a value changes: the next few steps run through the layer code and are captured again."""
+        they are dropped when a value changes: the next few steps run through the layer code and are captured again.
+        With AdamW the rate is read from the device and only another decay drops them; there is no momentum to change."""
+        if self.adamw is not None:
+            if self.adamw.set(learning_rate, weight_decay):
+                if self.use_graph:
+                    torch.cuda.synchronize(self.device)
+                self.invalidate_tapes()
+            return
         old = self.ps.hyper_params()
         self.ps.set_hyper_params(learning_rate, momentum, weight_decay)
         if self.ps.hyper_params() != old:

@@ -117,6 +117,10 @@ def main(argv=None) -> None:
     ap.add_argument("--momentum", type=float, default=0.9)
     ap.add_argument("--weight-decay", type=float, default=5e-4)
     ap.add_argument("--clip-gradients", type=float, default=0.0, help="bound of the gradients' norm (Caffe's clip_gradients; 0: none)")
+    ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw"], help="momentum SGD in the shards, or AdamW in the worker")
+    ap.add_argument("--adam-bits", type=int, default=32, choices=[8, 32], help="bits of AdamW's states")
+    ap.add_argument("--norm", default="batch", choices=["batch", "group"], help="norm of the Inception models")
+    ap.add_argument("--fp8-linear", action="store_true", help="fully-connected layers multiply in 8 bits (alexnet)")
     ap.add_argument("--slack", type=int, default=0)
     ap.add_argument("--display", type=int, default=20)
     ap.add_argument("--snapshot", type=int, default=0)
@@ -133,7 +137,7 @@ def main(argv=None) -> None:
     from .models.inception_bn import inception_bn_22k, inception_bn_small
     from .parallel.ps_module import PSModule
     from .utils.affinity import bind_to_gpu_cores
-    from .utils.config import DEVICE_CUDA, TABLE_SGD_MOMENTUM, TRANSPORT_NVLINK, GeePsConfig
+    from .utils.config import DEVICE_CUDA, TABLE_ADDITIVE, TABLE_SGD_MOMENTUM, TRANSPORT_NVLINK, GeePsConfig
     from .utils.feeder import HostFeeder
     from .utils.solver import LrPolicy, Solver
 
@@ -148,7 +152,9 @@ def main(argv=None) -> None:
 
     image, classes, default_batch = MODELS[args.model]
     B = args.batch or default_batch
-    net = {"alexnet": alexnet, "inception_bn_small": inception_bn_small, "inception_bn_22k": inception_bn_22k}[args.model]()
+    net = alexnet(fp8=args.fp8_linear) if args.model == "alexnet" else \
+        {"inception_bn_small": inception_bn_small, "inception_bn_22k": inception_bn_22k}[args.model](norm=args.norm)
+    adamw = dict(bits=args.adam_bits, seed=args.seed if args.adam_bits == 8 else None) if args.optimizer == "adamw" else None
     if args.data == "synthetic":
         src = args.source_size or image[1] + 29
         images, labels = synthetic_arrays(max(args.synthetic_images, B * world), image, classes, (src, src), args.seed)
@@ -163,7 +169,7 @@ def main(argv=None) -> None:
     base_port = 10000 + (int(os.environ.get("MASTER_PORT", "29500")) % 500) * 40
     cfg = GeePsConfig(host_list=["127.0.0.1"] * world, port_list=[base_port + 10 * r for r in range(world)],
                       device=DEVICE_CUDA, cuda_device=local_rank, transport=TRANSPORT_NVLINK,
-                      table_mode=TABLE_SGD_MOMENTUM, learning_rate=args.base_lr, momentum=args.momentum,
+                      table_mode=TABLE_ADDITIVE if adamw else TABLE_SGD_MOMENTUM, learning_rate=args.base_lr, momentum=args.momentum,
                       weight_decay=args.weight_decay, grad_scale=1.0 / world, bf16_compute_cache=1)
     resume = args.snapshot_dir if args.resume else None
     if args.resume and not (args.snapshot_dir and os.path.exists(os.path.join(args.snapshot_dir, "LATEST"))):
@@ -171,8 +177,8 @@ def main(argv=None) -> None:
     stream = torch.cuda.Stream(device=dev, priority=-1)
     with torch.cuda.stream(stream):
         mod = PSModule(net, (B,) + image, cfg, rank=rank, world=world, device=dev, slack=args.slack, seed=args.seed,
-                       bf16_weights_only=True, use_graph=not args.no_graph, resume_from=resume,
-                       clip_gradients=args.clip_gradients or None)
+                       bf16_weights_only=adamw is None, use_graph=not args.no_graph, resume_from=resume,
+                       clip_gradients=args.clip_gradients or None, adamw=adamw)
         inp = mod.net.input_layer
         inp.set_transform(args.mean, args.scale)
         policy = LrPolicy(args.lr_policy, args.base_lr, args.gamma, args.stepsize, args.stepvalue, args.power, args.max_iter)

@@ -76,3 +76,173 @@ def test_three_steps_follow_the_formulas(sizes, pt, gt, bits, gap):
             off = (params[i].double() - before[i].double() - change).abs()
             half = torch.finfo(pt).eps / 2
             assert (off <= 2.0 ** -19 * change.abs() + (half + 2.0 ** -24) * (before[i].double().abs() + change.abs())).all()
+
+
+def test_out_receives_the_change_and_may_be_the_gradients():
+    from geeps_b200.ops import functional as F
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    sizes = [1000, 7, 4096]
+    params = flat(sizes, torch.float32, gen, 3, 0.1)
+    grads = flat(sizes, torch.float32, gen, 5, 0.01)
+    plain, twin = [p.clone() for p in params], F.AdamWState([p.clone() for p in params])
+    for out in ([torch.empty_like(g) for g in grads], [torch.empty_like(g, dtype=torch.bfloat16) for g in grads], grads):
+        state = F.AdamWState(params)
+        before, g0 = [p.clone() for p in params], [g.clone() for g in grads]
+        F.adamw_step(params, grads, state, LR, weight_decay=WD, out=out)
+        for p, b, g, o in zip(params, before, g0, out):
+            assert torch.equal(p, b)
+            _, _, change = want(b, g, torch.zeros_like(b), torch.zeros_like(b), 1, True)
+            assert ((o.double() - change).abs() <= (2.0 ** -19 + torch.finfo(o.dtype).eps / 2) * change.abs()).all()
+    F.adamw_step(plain, g0, twin, LR, weight_decay=WD)
+    for p, b, o in zip(plain, params, grads):
+        assert torch.equal(p, b + o)                       # what an additive table makes of it
+
+
+def test_a_norm_above_its_bound_scales_the_gradients_on_their_way():
+    from geeps_b200.ops import functional as F
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    grads = flat([5000, 300], torch.bfloat16, gen, 0, 1.0)
+    for ratio in (0.5, 4.0, float("inf")):
+        params = [torch.zeros(5000, device=DEV), torch.zeros(300, device=DEV)]
+        state, norm = F.AdamWState(params), torch.zeros(2, device=DEV)
+        F.clip_gradients(grads, float("inf"), norm)
+        bound = 0.0 if ratio == float("inf") else norm[0].item() / ratio
+        F.adamw_step(params, grads, state, LR, clip=(norm, bound))
+        c = min(1.0, bound / norm[0].item())
+        for o, n, g in zip(state.offsets, state.params.numel, grads):
+            m = (1 - B1) * c * g.double()
+            assert ((state.m[o:o + n].double() - m).abs() <= 4 * 2.0 ** -24 * m.abs()).all()
+    norm.fill_(float("inf"))                                # the factor is 0 then, and what is not finite goes on
+    params[0].fill_(1.0)
+    F.adamw_step(params, grads, state, LR, clip=(norm, 1.0))
+    assert params[0].isfinite().all()
+
+
+@pytest.mark.parametrize("pt", [torch.float32, torch.bfloat16])
+def test_random_rounding_keeps_the_mean_and_depends_on_seed_step_and_place(pt):
+    """States in 8 bits whose mean moves by less than half a code in a step: rounded at random they follow it on average.  The mean of
+    n values that are each up or down with the right odds is off by at most 5 standard deviations of it, d / (2 sqrt(n)) each, where d
+    is the distance of two codes (an eighth of the value)."""
+    from geeps_b200.ops import functional as F
+    n = 1 << 20
+    params, grads = [torch.full((n,), 0.5, dtype=pt, device=DEV)], [torch.full((n,), 0.25, device=DEV)]
+
+    def after(steps, seed):
+        p = [params[0].clone()]
+        state = F.AdamWState(p, bits=8)
+        for _ in range(steps):
+            F.adamw_step(p, grads, state, LR, seed=seed)
+        m, v = F.adamw_moments(state, torch.empty(n, device=DEV), torch.empty(n, device=DEV))
+        return m, v, p[0], state
+    for steps in (1, 7):
+        m, v, p, state = after(steps, 5)
+        wm, wv = 0.25 * (1 - B1 ** steps), 0.0625 * (1 - B2 ** steps)
+        for got, w in ((m, wm), (v, wv)):
+            assert abs(got.double().mean().item() - w) <= 5 * steps * (w / 8) / (2 * math.sqrt(n)) + 2.0 ** -20 * w
+        again = after(steps, 5)
+        assert torch.equal(state.m, again[3].m) and torch.equal(state.v, again[3].v) and torch.equal(p, again[2])
+        other = after(steps, 6)
+        assert not torch.equal(state.m, other[3].m) and not torch.equal(state.v, other[3].v)
+        if pt is torch.bfloat16:                            # a change below half a step of bf16 (0.5: 2^-9)
+            off = p.double().mean().item() - 0.5
+            assert abs(off + LR * steps) <= 5 * steps * 2.0 ** -9 / math.sqrt(n) + 0.1 * LR * steps and len(p.unique()) > 1
+    nearest = after(7, None)
+    assert len(nearest[0].unique()) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_values_that_are_not_finite(bits):
+    from geeps_b200.ops import functional as F
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        p, g = [torch.ones(400, device=DEV)], [torch.full((400,), 0.5, device=DEV)]
+        state = F.AdamWState(p, bits=bits)
+        F.adamw_step(p, g, state, LR, seed=1)
+        g[0][130] = bad
+        F.adamw_step(p, g, state, LR, seed=1)
+        finite = p[0].isfinite()
+        assert not finite[130] and finite[:130].all() and finite[131:].all()
+        g[0][130] = 0.5
+        F.adamw_step(p, g, state, LR, seed=1)
+        assert not p[0][130].isfinite() and p[0][:128].isfinite().all() and p[0][256:].isfinite().all()
+
+
+def test_replayed_steps_count_and_read_the_rate_from_the_device():
+    from geeps_b200.ops import functional as F
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    sizes = [3000, 50]
+    start = flat(sizes, torch.float32, gen, 0, 0.1)
+    grads = flat(sizes, torch.float32, gen, 0, 0.01)
+
+    def run(replay):
+        params = [p.clone() for p in start]
+        state, lr = F.AdamWState(params, bits=8), torch.tensor([LR], device=DEV)
+        args = (F.GradList(params), F.GradList(grads), state, lr)
+        F.adamw_step(*args, weight_decay=WD, seed=2)
+        if replay:
+            stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                F.adamw_step(*args, weight_decay=WD, seed=2)
+            torch.cuda.synchronize()
+        for i in range(4):
+            lr.fill_(LR / (i + 1))
+            if replay:
+                graph.replay()
+            else:
+                F.adamw_step(*args, weight_decay=WD, seed=2)
+        torch.cuda.synchronize()
+        return params, state
+    (p, a), (q, b) = run(False), run(True)
+    assert all(torch.equal(x, y) for x, y in zip(p, q)) and torch.equal(a.m, b.m) and torch.equal(a.v, b.v) and torch.equal(a.exponents, b.exponents)
+    assert a.steps.tolist() == b.steps.tolist() == [5, 0]
+    by_value = [x.clone() for x in start]
+    state = F.AdamWState(by_value, bits=8)
+    for i in range(5):
+        F.adamw_step(by_value, grads, state, LR if i == 0 else torch.tensor(LR / i).item(), weight_decay=WD, seed=2)
+    assert all(((x - y).abs() <= 2.0 ** -20 * (x.abs() + LR)).all() for x, y in zip(p, by_value))
+
+
+def test_states_can_be_saved_and_restored():
+    from geeps_b200.ops import functional as F
+    p, g = [torch.ones(300, device=DEV)], [torch.full((300,), 0.1, device=DEV)]
+    state = F.AdamWState(p, bits=8)
+    F.adamw_step(p, g, state, LR, seed=1)
+    saved = [t.clone() for t in (p[0], state.m, state.v, state.exponents, state.steps)]
+    F.adamw_step(p, g, state, LR, seed=1)
+    again = F.AdamWState([saved[0]], bits=8)
+    again.m, again.v, again.exponents, again.steps = saved[1:]
+    F.adamw_step([saved[0]], g, again, LR, seed=1)
+    assert torch.equal(saved[0], p[0]) and torch.equal(again.m, state.m) and again.steps.tolist() == [2, 0]
+
+
+def test_more_values_than_32_bits_of_bytes():
+    from geeps_b200.ops import functional as F
+    n = (1 << 30) + 12345                                   # fp32: more than 2^32 bytes
+    p, g = torch.zeros(n, device=DEV), torch.zeros(n, dtype=torch.bfloat16, device=DEV)
+    g[0], g[n - 1], g[n // 2] = 1.0, -1.0, 2.0
+    state = F.AdamWState([p], bits=8)
+    F.adamw_step([p], [g], state, LR)
+    hit = p.nonzero().view(-1).tolist()
+    assert hit == [0, n // 2, n - 1]
+    assert abs(p[0].item() + LR) < 1e-8 and abs(p[n - 1].item() - LR) < 1e-8
+
+
+def test_refusals():
+    from geeps_b200.ops import functional as F
+    p, g = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
+    state = F.AdamWState([p])
+    step = lambda **kw: F.adamw_step(kw.pop("params", [p]), kw.pop("grads", [g]), kw.pop("state", state), kw.pop("lr", LR), **kw)
+    for match, call in (
+            ("bits", lambda: F.AdamWState([p], bits=16)), ("parameter", lambda: F.AdamWState([])),
+            ("decay", lambda: F.AdamWState([p], decay=[True, False])), ("steps", lambda: F.AdamWState([p], steps=-1)),
+            ("counts", lambda: step(grads=[g[:50]])), ("counts", lambda: step(params=[p, g])), ("counts", lambda: step(out=[g[:3]])),
+            ("betas", lambda: step(betas=(1.0, 0.9))), ("betas", lambda: step(eps=-1.0)), ("betas", lambda: step(weight_decay=-0.1)),
+            ("lr", lambda: step(lr=torch.zeros(1, dtype=torch.float64, device=DEV))), ("lr", lambda: step(lr=torch.zeros(2, device=DEV))),
+            ("clip", lambda: step(clip=(torch.zeros(2), 1.0))), ("clip", lambda: step(clip=(torch.zeros(2, device=DEV), -1.0))),
+            ("overlap", lambda: step(grads=[p])), ("overlap", lambda: step(out=[p])), ("overlap", lambda: step(clip=(p, 1.0))),
+            ("32 bits", lambda: F.adamw_moments(state, p, g)),
+            ("moments|bf16", lambda: F.adamw_moments(F.AdamWState([p], bits=8), p, g))):
+        with pytest.raises(ValueError, match=match):
+            call()
+    state.m = state.m[:64]
+    with pytest.raises(ValueError, match="AdamWState"):
+        step()

@@ -84,3 +84,134 @@ def test_products_match_64_bits(M, N, K, dtype, plan):
     off = (out.double() - want).abs()
     print("largest error in units of its bound", (off / (sums + half * want.abs() + 1e-30)).max().item(), "of the sum of magnitudes", (off / sums).max().item())
     assert (off <= sums + half * (want.abs() + sums)).all()
+
+
+def test_blocks_that_are_not_finite_are_nan_and_zeros_are_zeros():
+    from geeps_b200.ops import functional as F
+    x = torch.randn(5, 300, device=DEV)
+    x[1, 130] = float("inf")
+    x[2, 299] = float("nan")
+    x[3] = 0.0
+    for kw in (dict(), dict(transposed=F.Fp8Matrix(300, 5, DEV))):
+        q = F.quantize_fp8(x, F.Fp8Matrix(5, 300, DEV), **kw)
+        e = q.exponents()
+        assert (e == 255).nonzero().tolist() == [[1, 1], [2, 2]]
+        d = q.dequantize()
+        assert d[1, 128:256].isnan().all() and d[2, 256:].isnan().all() and (d[3] == 0).all() and d[0].isfinite().all() and d[1, :128].isfinite().all()
+    t = kw["transposed"].dequantize()
+    assert t[130].isnan().all() and t[299].isnan().all() and t[:130].isfinite().all()
+    w = F.quantize_fp8(torch.randn(40, 300, device=DEV))
+    out = torch.zeros(5, 40, device=DEV)
+    F.matmul_fp8(q, w, out, relu=True)
+    assert out[1].isnan().all() and out[2].isnan().all() and (out[3] == 0).all() and out[0].isfinite().all() and (out[0] >= 0).all()
+
+
+def test_extreme_sizes_of_values():
+    """Scales at both ends of their range; the smallest fp32 values are below it and become zeros."""
+    from geeps_b200.ops import functional as F
+    x = torch.tensor([[3.0e38], [1e-30], [2.0 ** -127], [2.0 ** -135], [1e-45], [448.0], [449.0], [448.0 * 2 ** -20]], device=DEV).repeat(1, 128)
+    q = F.quantize_fp8(x)
+    # 3.0e38 = 1.76 x 2^127, so e = 127 - 7; 1e-30 = 1.27 x 2^-100, so e = -100 - 8
+    assert q.exponents().view(-1).tolist() == [127 + 120, 127 - 108, 0, 0, 0, 127, 128, 107]
+    d = q.dequantize().double()
+    assert ((d - x.double()).abs() <= x.double().abs() * 2.0 ** -4 + 2.0 ** -137).all() and d[5, 0] == 448.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_wider_matrices_at_any_address(dtype):
+    """Inputs and outputs whose rows begin anywhere; what lies beside an output stays as it was."""
+    from geeps_b200.ops import functional as F
+    M, N, K = 70, 90, 260
+    big = torch.randn(M, K + 7, device=DEV).to(dtype)
+    w = F.quantize_fp8(torch.randn(N, K, device=DEV))
+    for shift in (0, 1, 3):
+        x = big[:, shift:shift + K]
+        a = F.quantize_fp8(x)
+        same(a, x)
+        t = F.quantize_fp8(x, transposed=F.Fp8Matrix(K, M, DEV))
+        same(t, x.T)
+        out = torch.full((M, N + 5), 9.0, dtype=dtype, device=DEV)
+        F.matmul_fp8(a, w, out[:, shift:shift + N])
+        sums, half = tolerance(a, w, out, K)
+        exact = plain(a, w)
+        assert ((out[:, shift:shift + N].double() - exact).abs() <= sums + half * (exact.abs() + sums)).all()
+        assert (out[:, :shift] == 9.0).all() and (out[:, shift + N:] == 9.0).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 33, 127), (2, 64, 128), (33, 32, 129), (129, 1, 640), (31, 200, 50), (128, 128, 512), (257, 65, 513), (8, 3000, 3000)])
+def test_small_and_odd_sizes(M, N, K):
+    from geeps_b200.ops import functional as F
+    a, b = F.quantize_fp8(torch.randn(M, K, device=DEV)), F.quantize_fp8(torch.randn(N, K, device=DEV).bfloat16(), tile=True)
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
+        F.matmul_fp8(a, b, out)
+        sums, half = tolerance(a, b, out, K)
+        exact = plain(a, b)
+        assert ((out.double() - exact).abs() <= sums + half * (exact.abs() + sums)).all()
+    empty = torch.empty(0, N, device=DEV)
+    F.matmul_fp8(F.quantize_fp8(torch.empty(0, K, device=DEV)), b, empty)
+
+
+def test_gradients_of_a_layer():
+    """Forward and both gradients as a layer forms them, each operand cast once: against the products of what the casts stand for."""
+    from geeps_b200.ops import functional as F
+    M, N, K = 150, 260, 390
+    x, w, dy = torch.randn(M, K, device=DEV).bfloat16(), torch.randn(N, K, device=DEV).bfloat16(), torch.randn(M, N, device=DEV).bfloat16()
+    xq, xt, wq, wt, dq, dt = (F.Fp8Matrix(r, c, DEV) for r, c in ((M, K), (K, M), (N, K), (K, N), (M, N), (N, M)))
+    F.quantize_fp8(x, xq, transposed=xt)
+    F.quantize_fp8(w, wq, transposed=wt, tile=True)
+    F.quantize_fp8(dy, dq, transposed=dt)
+    assert torch.equal(wt.dequantize(), wq.dequantize().T)
+    for a, b, size in ((xq, wq, (M, N)), (dq, wt, (M, K)), (dt, xt, (N, K))):
+        out = torch.empty(size, device=DEV)
+        F.matmul_fp8(a, b, out)
+        sums, half = tolerance(a, b, out, a.cols)
+        exact = plain(a, b)
+        assert ((out.double() - exact).abs() <= sums + half * (exact.abs() + sums)).all()
+    # and the casts are within half a step of what they stand for: 2^-4 of a value, or of the least of e4m3 (2^-9) of the scale
+    for m, t in ((xq, x), (wt, w.T), (dt, dy.T)):
+        step = torch.exp2(m.exponents().double() - 127).repeat_interleave(128, 1)[:, :m.cols] * 2.0 ** -10
+        assert ((m.dequantize().double() - t.double()).abs() <= t.double().abs() * 2.0 ** -4 + step).all()
+
+
+def test_products_repeat_on_other_streams_and_in_graphs():
+    from geeps_b200.ops import functional as F
+    x, w = torch.randn(200, 1500, device=DEV).bfloat16(), F.quantize_fp8(torch.randn(300, 1500, device=DEV), tile=True)
+    q = [F.Fp8Matrix(200, 1500, DEV) for _ in range(3)]
+    outs = [torch.empty(200, 300, dtype=torch.bfloat16, device=DEV) for _ in range(3)]
+
+    def call(i):
+        F.quantize_fp8(x, q[i])
+        F.matmul_fp8(q[i], w, outs[i])
+    call(0)
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for i in (1, 2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(i)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_refusals():
+    from geeps_b200.ops import functional as F
+    x = torch.zeros(10, 40, device=DEV)
+    a, b = F.quantize_fp8(x), F.quantize_fp8(torch.zeros(20, 40, device=DEV))
+    out = torch.zeros(10, 20, device=DEV)
+    for match, call in (
+            ("columns", lambda: F.quantize_fp8(torch.zeros(3, 0, device=DEV))), ("matrix", lambda: F.quantize_fp8(x.half())),
+            ("matrix", lambda: F.quantize_fp8(x.view(-1))), ("contiguous", lambda: F.quantize_fp8(x.t())),
+            ("out", lambda: F.quantize_fp8(x, F.Fp8Matrix(10, 41, DEV))), ("transposed", lambda: F.quantize_fp8(x, transposed=F.Fp8Matrix(10, 40, DEV))),
+            ("out", lambda: F.quantize_fp8(x, x)), ("Fp8Matrix", lambda: F.Fp8Matrix(10, 0, DEV)),
+            ("matmul_fp8: b", lambda: F.matmul_fp8(a, F.quantize_fp8(torch.zeros(20, 41, device=DEV)), out)),
+            ("matmul_fp8: a", lambda: F.matmul_fp8(a, b, out[:9])), ("out", lambda: F.matmul_fp8(a, b, out.double())),
+            ("out", lambda: F.matmul_fp8(a, b, torch.zeros(20, 10, device=DEV).t())), ("bias", lambda: F.matmul_fp8(a, b, out, bias=torch.zeros(19, device=DEV))),
+            ("bias", lambda: F.matmul_fp8(a, b, out, bias=torch.zeros(20, device=DEV).bfloat16()))):
+        with pytest.raises(ValueError, match=match):
+            call()

@@ -125,3 +125,179 @@ def check_backward(x, dy, dx, dw, db, stats, w, b, images, groups, act):
     size = (a + a.mean((1, 3), keepdim=True) + ng * (a * ng).mean((1, 3), keepdim=True)).view_as(n) * rstd
     tol = (adds + 2.0 ** -20) * size.view_as(x) + torch.finfo(dx.dtype).eps / 2 * want.view_as(x).abs() + 1e-30
     assert ((dx.double() - want.view_as(x)).abs() <= tol * 1.01).all()
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("wider,shift", [(8, 0), (3, 0), (5, 3)])
+def test_rows_of_wider_matrices_at_any_address(types, wider, shift):
+    """Pitches and addresses that allow vectors and such that do not; what lies beside the rows stays as it was."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = 3, 50, 64, 8
+    x, dy, w, b = made(images, pixels, c, groups, types, 3)
+
+    def inside(t):
+        full = torch.full((t.shape[0], c + wider + 3), 9.0, dtype=t.dtype, device=DEV).view(-1)
+        full = full[shift:shift + t.shape[0] * (c + wider)].view(t.shape[0], c + wider)
+        full[:, :c] = t
+        return full
+    xf, dyf = inside(x), inside(dy)
+    yf, dxf = inside(torch.zeros_like(dy)), inside(torch.zeros_like(x))
+    stats = torch.empty(images, groups, 2, device=DEV)
+    F.group_norm_forward(xf[:, :c], yf[:, :c], images, F.GroupNorm(groups, w, b, stats, EPS, "silu"))
+    check_forward(x, yf[:, :c], stats, statistics(x, images, groups), w, b, images, groups, "silu")
+    dw, db = torch.empty(c, device=DEV), torch.empty(c, device=DEV)
+    F.group_norm_backward(xf[:, :c], dyf[:, :c], dxf[:, :c], images, F.GroupNorm(groups, w, b, stats, EPS, "relu", dw, db))
+    check_backward(x, dy, dxf[:, :c], dw, db, stats, w, b, images, groups, "relu")
+    for t in (xf, dyf, yf, dxf):
+        assert (t[:, c:] == 9.0).all()
+
+
+def test_in_place_without_parameters_and_into_a_slice_of_the_same_rows():
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = 4, 30, 48, 6
+    x, dy, _, _ = made(images, pixels, c, groups, "bf16", 4)
+    one, zero = torch.ones(c, device=DEV), torch.zeros(c, device=DEV)
+    stats = statistics(x, images, groups).float()
+    y, dx = x.clone(), dy.clone()
+    F.group_norm_forward(y, y, images, F.GroupNorm(groups, act="relu"))
+    check_forward(x, y, stats, statistics(x, images, groups), one, zero, images, groups, "relu")
+    F.group_norm_backward(x, dx, dx, images, F.GroupNorm(groups, stats=stats, act="silu"))
+    dw, db = torch.empty(c, device=DEV), torch.empty(c, device=DEV)
+    other = torch.empty_like(x)
+    F.group_norm_backward(x, dy, other, images, F.GroupNorm(groups, stats=stats, act="silu", dweight=dw, dbias=db))
+    check_backward(x, dy, other, dw, db, stats, one, zero, images, groups, "silu")
+    assert torch.equal(dx, other)
+    wide = torch.cat([x, torch.full_like(x, 5.0)], 1)
+    F.group_norm_forward(wide[:, :c], wide[:, c:], images, F.GroupNorm(groups, act="relu"))
+    assert torch.equal(wide[:, :c], x) and torch.equal(wide[:, c:], y)
+
+
+@pytest.mark.parametrize("size", [(2, 40, 64, 8), (1, 20000, 32, 4), (3, 11, 21, 3)], ids=str)
+def test_a_mean_far_from_zero_and_groups_without_spread(size):
+    """The variance does not lose what the mean has: 1000 standard deviations from zero in fp32 (a value then has 14 bits below the
+    deviation: the bound of check_forward goes by the largest value)."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = size
+    x, _, w, b = made(*size, "fp32", 5)
+    x = x + 1000.0
+    x[:pixels, : c // groups] = 3.25                                   # a group that is all one value
+    y, stats = torch.empty_like(x), torch.empty(images, groups, 2, device=DEV)
+    F.group_norm_forward(x, y, images, F.GroupNorm(groups, w, b, stats, EPS, None))
+    want = statistics(x, images, groups)
+    assert stats[0, 0].tolist() == [3.25, torch.tensor(EPS).rsqrt().item()] or abs(stats[0, 0, 1].item() * EPS ** 0.5 - 1) < 1e-6
+    check_forward(x, y, stats, want, w, b, images, groups, None)
+
+
+def test_values_that_are_not_finite_stay_in_their_group():
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = 2, 9, 32, 4
+    x, dy, w, b = made(images, pixels, c, groups, "bf16", 6)
+    clean, stats = torch.empty_like(x), torch.empty(images, groups, 2, device=DEV)
+    F.group_norm_forward(x, clean, images, F.GroupNorm(groups, w, b, stats, EPS, "relu"))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        z = x.clone()
+        z[pixels + 2, 9] = bad                                           # image 1, group 1
+        y = torch.empty_like(x)
+        F.group_norm_forward(z, y, images, F.GroupNorm(groups, w, b, None, EPS, "relu"))
+        hit = torch.zeros_like(x, dtype=torch.bool)
+        hit[pixels:, 8:16] = True
+        assert y[pixels:, 8:16].isnan().all() and torch.equal(y[~hit], clean[~hit])
+        d = dy.clone()
+        d[pixels + 2, 9] = bad
+        dx = torch.empty_like(x)
+        F.group_norm_backward(x, d, dx, images, F.GroupNorm(groups, w, b, stats, EPS, None))
+        assert not dx[pixels:, 8:16].isfinite().any() and dx[~hit].isfinite().all()
+
+
+def test_repeats_bit_for_bit_on_other_streams_and_in_two_graphs_at_once():
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = 5, 400, 96, 32
+    x, dy, w, b = made(images, pixels, c, groups, "bf16", 7)
+
+    def buffers():
+        return dict(y=torch.empty_like(x), dx=torch.empty_like(x), stats=torch.empty(images, groups, 2, device=DEV), dw=torch.empty(c, device=DEV), db=torch.empty(c, device=DEV))
+
+    def both(o):
+        n = F.GroupNorm(groups, w, b, o["stats"], EPS, "relu", o["dw"], o["db"])
+        F.group_norm_forward(x, o["y"], images, n)
+        F.group_norm_backward(x, dy, o["dx"], images, n)
+    first = buffers()
+    both(first)
+    outs, graphs, streams = [buffers() for _ in range(2)], [], [torch.cuda.Stream() for _ in range(2)]
+    for o in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            both(o)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(o[k], first[k]) for k in first)
+
+
+def test_gradients_match_differences():
+    """Of the sum of dy y, in fp32: a central difference with step h is off by h^2 of a third derivative and 2^-22 / h of the sum."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = 2, 6, 12, 3
+    x, dy, w, b = made(images, pixels, c, groups, "fp32", 8)
+    stats, dx = torch.empty(images, groups, 2, device=DEV), torch.empty_like(x)
+    dw, db = torch.empty(c, device=DEV), torch.empty(c, device=DEV)
+    y = torch.empty_like(x)
+
+    def total(x, w, b):
+        F.group_norm_forward(x, y, images, F.GroupNorm(groups, w, b, stats, EPS, "silu"))
+        return (y.double() * dy.double()).sum().item()
+    total(x, w, b)
+    F.group_norm_backward(x, dy, dx, images, F.GroupNorm(groups, w, b, stats.clone(), EPS, "silu", dw, db))
+    h = 2.0 ** -7
+    size = (y.double().abs() * dy.double().abs()).sum().item()
+    for t, grad in ((x, dx), (w, dw), (b, db)):
+        for i in range(0, t.numel(), 5):
+            v = t.view(-1)[i].item()
+            t.view(-1)[i] = v + h
+            up, high = total(x, w, b), t.view(-1)[i].item()
+            t.view(-1)[i] = v - h
+            down, low = total(x, w, b), t.view(-1)[i].item()
+            t.view(-1)[i] = v
+            assert abs((up - down) / (high - low) - grad.view(-1)[i].item()) <= 40 * h * h + 2.0 ** -22 / h * size
+
+
+def test_without_rows_the_parameters_have_gradients_of_zero():
+    from geeps_b200.ops import functional as F
+    x = torch.empty(0, 16, dtype=BF, device=DEV)
+    dw, db = torch.full((16,), 7.0, device=DEV), torch.full((16,), 7.0, device=DEV)
+    for images in (0, 4):
+        F.group_norm_forward(x, x.clone(), images, F.GroupNorm(4))
+        dw.fill_(7.0), db.fill_(7.0)
+        F.group_norm_backward(x, x.clone(), x.clone(), images, F.GroupNorm(4, stats=torch.empty(images, 4, 2, device=DEV), dweight=dw, dbias=db))
+        assert (dw == 0).all() and (db == 0).all()
+
+
+def test_refusals():
+    from geeps_b200.ops import functional as F
+    x = torch.zeros(12, 16, dtype=BF, device=DEV)
+    stats = torch.zeros(3, 4, 2, device=DEV)
+    ok = F.GroupNorm(4, stats=stats)
+    for match, call in (
+            ("whole pixels", lambda: F.group_norm_forward(x, x.clone(), 5, F.GroupNorm(4))),
+            ("divide", lambda: F.group_norm_forward(x, x.clone(), 3, F.GroupNorm(5))),
+            ("activation", lambda: F.GroupNorm(4, act="tanh")),
+            ("groups", lambda: F.GroupNorm(0)),
+            ("eps", lambda: F.GroupNorm(4, eps=-1.0)),
+            ("types", lambda: F.group_norm_forward(x, x.float(), 3, ok)),
+            ("types", lambda: F.group_norm_forward(x.half(), x.half(), 3, ok)),
+            ("rows, channels", lambda: F.group_norm_forward(x.view(3, 4, 16), x, 3, ok)),
+            ("stats", lambda: F.group_norm_forward(x, x.clone(), 3, F.GroupNorm(4, stats=stats[:2]))),
+            ("stats", lambda: F.group_norm_backward(x, x.clone(), x.clone(), 3, F.GroupNorm(4))),
+            ("fp32", lambda: F.group_norm_forward(x, x.clone(), 3, F.GroupNorm(4, weight=torch.zeros(15, device=DEV)))),
+            ("work", lambda: F.group_norm_backward(x, x.clone(), x.clone(), 3, ok, work=torch.zeros(1, device=DEV))),
+            ("y", lambda: F.group_norm_forward(x, x[:6].clone(), 3, ok)),
+            ("contiguous", lambda: F.group_norm_forward(x.t().contiguous().t(), x.clone(), 3, ok)),
+            ("overlaps", lambda: F.group_norm_forward(x[:9], x[3:], 3, F.GroupNorm(4))),
+            ("on cpu", lambda: F.group_norm_forward(x, x.cpu(), 3, ok))):
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            call()

@@ -1,0 +1,171 @@
+"""Group norms, 8-bit products and AdamW steps as a network's training step uses them together."""
+import pytest
+import torch
+import torch.nn.functional as TF
+
+from geeps_b200.models.inception_bn import inception_bn_small
+from geeps_b200.models.net import Concat, Net
+from geeps_b200.ops.layers import Conv2d, GroupNorm, Input, Linear, Pool
+from geeps_b200.parallel.ps_module import PSModule
+from geeps_b200.utils.config import TABLE_ADDITIVE, TRANSPORT_NVLINK, TRANSPORT_TCP
+from test_gpu_residual import bind, cfg, same_training
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+BF, F64 = torch.bfloat16, torch.float64
+
+
+def test_a_group_norm_layer_has_the_gradients_of_autograd():
+    """Alone and as the end of a branch that writes into a slice of a wider tensor.  bf16 in and out: half a step (2^-8) of the
+    result, and of an fp32 gradient 2^-12 of its terms (some 600 of them, random signs)."""
+    x = torch.randn(3, 7, 5, 48, device=DEV).to(BF)
+    dy = torch.randn(3, 7, 5, 96, device=DEV).to(BF)
+    layers = [GroupNorm("a", 6, act="silu"), GroupNorm("b", 12)]
+    cat = Concat("cat", [[layers[0]], [layers[1]]], concurrent=False)
+    cat.setup(tuple(x.shape), DEV)
+    bind([cat], 3)
+    y = cat.forward(x).view(3, 7, 5, 96)
+    dx = cat.backward(dy.view(-1, 96)).view_as(x)
+    leaf = x.to(F64).requires_grad_(True)
+    p = [{k: v.to(F64).requires_grad_(True) for k, v in l.p32.items()} for l in layers]
+    parts = [TF.group_norm(leaf.permute(0, 3, 1, 2), l.groups, q["gamma"], q["beta"], l.eps).permute(0, 2, 3, 1) for l, q in zip(layers, p)]
+    want = torch.cat([TF.silu(parts[0]), parts[1]], 3)
+    assert ((y.to(F64) - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14).all()
+    grads = torch.autograd.grad(want, [leaf] + [q[k] for q in p for k in ("gamma", "beta")], dy.to(F64))
+    # two branches' gradients, rounded, and their sum
+    size = grads[0].abs().max()
+    assert ((dx.to(F64) - grads[0]).abs() <= 3 * 2.0 ** -8 * size).all()
+    for g, got in zip(grads[1:], [l.g32[k] for l in layers for k in ("gamma", "beta")]):
+        assert ((got.to(F64) - g).abs() <= 2.0 ** -12 * dy.to(F64).abs().sum((0, 1, 2)).max()).all()
+    with pytest.raises(ValueError, match="divide"):
+        GroupNorm("c", 7).setup(tuple(x.shape), DEV)
+
+
+@pytest.mark.parametrize("fp32_out", [False, True])
+def test_an_fp8_layer_is_near_the_bf16_layer(fp32_out):
+    """Each operand is off by half a step of e4m3, 2^-4 of a value at the most and evenly spread, so 2^-4 / sqrt(3) in the mean
+    square; products of two such have sqrt(2) of that, whatever the number of terms: 0.051, with the outputs' own rounding below 0.06."""
+    gen = torch.Generator().manual_seed(1)
+    x, dy = torch.randn(96, 640, generator=gen).to(DEV).to(BF), torch.randn(96, 264, generator=gen).to(DEV).to(BF)
+    got = []
+    for fp8 in (False, True):
+        l = Linear("fc", 264, std=0.05, fp32_out=fp32_out, fp8=fp8)
+        l.setup((96, 640), DEV)
+        bind([l], 2)
+        y = l.forward(x).clone()
+        dx = l.backward(dy).clone()
+        got.append((y, dx, l.g32["weight"], l.g32["bias"]))
+    # column sums of the same 96 rows, in any order: 96 roundings of 2^-24 of the magnitudes on either side
+    assert ((got[0][3] - got[1][3]).abs() <= 96 * 2.0 ** -23 * dy.float().abs().sum(0)).all()
+    for a, b in zip(got[0][:3], got[1][:3]):
+        assert a.dtype == b.dtype and (a.double() - b.double()).norm() <= 0.06 * a.double().norm()
+
+
+def net(fp8=True):
+    return Net("n", Input(cpad=8), [Conv2d("c0", 24, 3, pad=1, bias=False, std=0.2, need_dx=False), GroupNorm("g0", 4, act="relu"),
+                                    Conv2d("c1", 32, 3, pad=1, bias=False, std=0.1), GroupNorm("g1", 8, act="silu"), Pool("avg", 0, 1, ceil_mode=False),
+                                    Linear("f1", 64, relu=True, std=0.2, fp8=fp8), Linear("fc", 10, std=0.3, fp32_out=True, fp8=fp8)])
+
+
+def batch(n=16):
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    return torch.randn(n, 3, 8, 8, generator=gen, device=DEV), torch.randint(0, 10, (n,), generator=gen, device=DEV)
+
+
+def module(transport=TRANSPORT_NVLINK, adamw=None, make=net, shape=(16, 3, 8, 8), **kw):
+    return PSModule(make(), shape, cfg(transport, table_mode=TABLE_ADDITIVE, learning_rate=0.01, weight_decay=0.1), device="cuda:0", seed=4,
+                    adamw=adamw or {}, **kw)
+
+
+@pytest.mark.parametrize("transport", [TRANSPORT_NVLINK, TRANSPORT_TCP])
+@pytest.mark.parametrize("clip", [None, 0.05])
+def test_a_step_moves_the_parameters_by_the_formula(transport, clip):
+    """From the states that the first step leaves: m = (1 - b1) g and v = (1 - b2) g^2, so the change is that of m and v."""
+    mod = module(transport, clip_gradients=clip)
+    x, y = batch()
+    mod.step(x, y, capture=True)
+    before = {k: v.clone() for k, v in mod.captured.items()}
+    state, specs = mod.adamw.state, [(t.layer, sp) for t in mod.tables for sp in t.specs]
+    m = [state.m[o:o + n].double().clone() for o, n in zip(state.offsets, state.params.numel)]
+    v = [state.v[o:o + n].double().clone() for o, n in zip(state.offsets, state.params.numel)]
+    mod.step(x, y, capture=True)
+    after = {k: v.clone() for k, v in mod.captured.items()}
+    assert state.steps[0].item() == 2
+    if clip is not None:
+        assert mod.clip_result[0].item() > clip                # it does clip
+        total = sum((a / 0.1).square().sum().item() for a in m) ** 0.5
+        assert abs(total - clip) <= 1e-5 * clip
+    for (l, sp), a, b in zip(specs, m, v):
+        p = before[f"{l.name}.{sp.name}"].double().view(-1)
+        change = -0.01 * (a / 0.1 / ((b / (1 - 0.999)).sqrt() + 1e-8) + (0.1 * p if sp.decay else 0.0))
+        off = after[f"{l.name}.{sp.name}"].double().view(-1) - p - change
+        # 2^-18 of the change; the sum is a rounding of the parameter, the states one each of m and v
+        assert (off.abs() <= 2.0 ** -18 * change.abs() + 2.0 ** -23 * (p.abs() + change.abs())).all(), (l.name, sp.name)
+    mod.close()
+
+
+@pytest.mark.parametrize("bits,seed", [(32, None), (8, 7)])
+def test_steps_with_graphs_recorded_steps_and_neither_train_alike(bits, seed):
+    x, y = batch()
+    losses = []
+    for kw in (dict(), dict(use_tape=True), dict(use_graph=True)):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            mod = module(adamw=dict(bits=bits, seed=seed), clip_gradients=5.0, **kw)
+            out = [mod.step(x, y).clone() for _ in range(10)]
+            st.synchronize()
+            assert not kw or mod.is_steady(x, y), mod.tape_mismatch
+            assert mod.adamw.state.steps.tolist() == [10, 0] and mod.adamw.state.bits == bits
+            mod.set_hyper_params(learning_rate=0.0, momentum=0.9)             # without a new capture
+            assert not kw or mod.is_steady(x, y)
+            losses.append([v.item() for v in out])
+            mod.close()
+    same_training(losses)
+
+
+def test_a_rate_of_zero_holds_the_parameters():
+    x, y = batch()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        mod = module(use_graph=True)
+
+        def steps(n):
+            for _ in range(n):
+                mod.step(x, y)
+            st.synchronize()
+            return {k: v.clone() for k, v in mod.params_fp32().items()}
+        steps(6)
+        mod.set_hyper_params(learning_rate=0.0)
+        held, later = steps(1), steps(3)
+        assert all(torch.equal(later[k], held[k]) for k in held)
+        mod.set_hyper_params(learning_rate=0.01, weight_decay=0.2)            # another decay: recorded again
+        assert not mod.is_steady(x, y)
+        moved = steps(6)
+        assert mod.is_steady(x, y) and all(not torch.equal(moved[k], held[k]) for k in held)
+        mod.close()
+
+
+def test_an_inception_net_with_group_norms_trains_in_graphs_and_with_managed_activations():
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x, y = torch.randn(8, 3, 32, 32, generator=gen, device=DEV), torch.randint(0, 10, (8,), generator=gen, device=DEV)
+    losses = []
+    for kw in (dict(), dict(use_graph=True), dict(manage_activations=True)):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            mod = module(make=lambda: inception_bn_small(norm="group"), shape=(8, 3, 32, 32), **kw)
+            losses.append([mod.step(x, y).clone() for _ in range(5)])
+            st.synchronize()
+            mod.close()
+    losses = [[v.item() for v in out] for out in losses]
+    assert all(v == v and v < 20 for out in losses for v in out)
+    # one step's loss is a sum in any order; afterwards atomics of the weight gradients, which AdamW's quotient of m and v magnifies
+    # where a gradient is near zero
+    for other in losses[1:]:
+        assert abs(other[0] - losses[0][0]) <= 64 * 2.0 ** -24 * abs(losses[0][0])
+
+
+def test_refusals():
+    with pytest.raises(ValueError, match="additive"):
+        PSModule(net(), (16, 3, 8, 8), cfg(TRANSPORT_NVLINK), device="cuda:0", adamw={})
+    with pytest.raises(ValueError, match="fp32"):
+        module(bf16_weights_only=True)

@@ -1,0 +1,161 @@
+"""Host side of group norm, AdamW steps and 8-bit products: launch shapes, workspaces and refusals, which need no GPU."""
+import ctypes as C
+
+import pytest
+
+from geeps_b200.models.inception_bn import inception_bn_22k, inception_bn_small, norm_groups
+from geeps_b200.ops import _lib as L
+from geeps_b200.ops.layers import BatchNorm, GroupNorm
+
+A, B, D = 1 << 32, 1 << 36, 1 << 40          # addresses that are never touched: every call here is refused
+
+
+def shape(images, pixels, c, groups, backward, vec, types):
+    out = (C.c_int * 8)()
+    assert L.lib().geeps_group_norm_shape(C.c_longlong(images), C.c_longlong(pixels), c, groups, int(backward), int(vec), *types, out) == 0
+    return list(out)
+
+
+def work(images, pixels, c, groups, backward):
+    return L.lib().geeps_group_norm_work(C.c_longlong(images), C.c_longlong(pixels), c, groups, int(backward))
+
+
+@pytest.mark.parametrize("c,groups", [(1, 1), (8, 1), (8, 8), (24, 8), (96, 32), (192, 32), (576, 32), (1003, 17), (1024, 1), (2048, 1), (2056, 1), (4096, 32),
+                                      (16384, 1), (16384, 16384), (16383, 3), (16381, 16381), (16376, 23)])
+@pytest.mark.parametrize("images,pixels", [(1, 1), (1, 7), (3, 196), (256, 196), (32, 3136), (1, 1 << 30), (1 << 16, 4), (2, 50176)])
+def test_group_norm_shapes_cover_the_pixels_within_the_launch_limits(images, pixels, c, groups):
+    for backward in (False, True):
+        for types in ((0, 0), (1, 0), (1, 1)):
+            for vec in ((True, False) if c % 8 == 0 else (False,)):
+                fused, width, chunks, rows, keep, blocks, smem, threads = shape(images, pixels, c, groups, backward, vec, types)
+                assert c % width == 0 and width % (c // groups) == 0 and (not vec or width % 8 == 0)
+                assert chunks * rows >= pixels and blocks == images * (c // width) * chunks < 1 << 31
+                assert 1 <= chunks <= (8 if fused else 256) and smem <= 227 * 1024
+                columns = width // (8 if vec else 1)
+                if fused and vec:
+                    assert columns <= threads and keep == -(-rows // max(1, threads // columns))
+                    # everything kept lies in shared memory
+                    assert keep * threads * 16 * ((2 if types[0] else 1) + ((2 if types[1] else 1) if backward else 0)) < smem
+                else:
+                    assert keep == 0
+                parts = images * (1 if fused else chunks)
+                assert work(images, pixels, c, groups, backward) >= (0 if fused else parts * groups * 2) + (parts * c * 2 if backward else 0)
+
+
+def group_norm(backward=False, **kw):
+    v = dict(x=A, dy=B if backward else 0, y=0 if backward else B, dx=D if backward else 0, weight=0, bias=0, stats=D + (1 << 34), work=D + (1 << 35),
+             dweight=0, dbias=0, images=2, pixels=9, ldx=64, lddy=64, ldy=64, lddx=64, c=64, groups=8, act=1, x_fp32=0, y_fp32=0, eps=1e-5)
+    v.update(kw)
+    fn = L.lib().geeps_group_norm_backward if backward else L.lib().geeps_group_norm_forward
+    return fn(L.GROUP_NORM.pack(*v.values()), None)
+
+
+def test_packed_arguments_have_the_structures_size():
+    class Group(C.Structure):
+        _fields_ = [(f"p{i}", C.c_void_p) for i in range(10)] + [(f"n{i}", C.c_longlong) for i in range(6)] + [(f"i{i}", C.c_int) for i in range(5)] + [("eps", C.c_float)]
+    assert C.sizeof(Group) == L.GROUP_NORM.size
+
+
+REFUSED = (-10, -12, -14, -16)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_group_norm_refusals(backward):
+    call = lambda **kw: group_norm(backward, **kw)
+    out = "dx" if backward else "y"
+    assert call(groups=7) == -16 and call(groups=0) == -16 and call(groups=65) == -16
+    assert call(c=16385, groups=1, ldx=1 << 15, ldy=1 << 15, lddx=1 << 15, lddy=1 << 15) == -10 and call(c=0) == -10
+    assert call(x=A + 1) == -14 and call(x=A + 2, x_fp32=1) == -14 and call(stats=D + (1 << 34) + 4) == -14 and call(weight=B - 2) == -14
+    assert call(work=D + (1 << 35) + 4) == -14
+    assert call(**{out: A + 64}) == -12 and call(**{out: A + 2 * 64 * 17}) == -12          # a shifted overlap
+    assert call(**{out: A + 64 * 2 * 5, "ldx": 200}) == -12
+    assert call(weight=(D if backward else B) + 4) == -12
+    assert call(ldx=63) == 1 and call(eps=-1.0) == 1 and call(act=3) == 1 and call(y_fp32=1) == 1 and call(x=0) == 1 and call(images=-1) == 1
+    assert call(images=1 << 20, pixels=1 << 11) == 1
+    # what is allowed is not refused (without a GPU the launch fails)
+    assert call(**{out: A}) not in REFUSED
+    if not backward:
+        assert group_norm(ldx=200, ldy=200, y=A + 2 * 64) not in REFUSED                        # other channels of the same rows
+        assert group_norm(ldx=200, ldy=200, y=A + 2 * 63) == -12
+    else:
+        assert call(dx=B) not in REFUSED and call(dweight=D + (1 << 34)) == -12 and call(dbias=A) == -12 and call(stats=0) == 1
+
+
+def tensors(ranges, fp32):
+    n = len(ranges)
+    order = sorted(range(n), key=lambda i: ranges[i])
+    arrays = ((C.c_void_p * n)(*[r[0] for r in ranges]), (C.c_longlong * n)(*[r[1] for r in ranges]), (C.c_ubyte * n)(*fp32), (C.c_longlong * n)(*order))
+    return L.Tensors(n, *(C.addressof(a) for a in arrays)), arrays
+
+
+def adamw(params, p32, grads, g32, out=None, o32=None, **kw):
+    p, hold = tensors(params, p32)
+    g, hold2 = tensors(grads, g32)
+    o, hold3 = (None, None) if out is None else tensors(out, o32)
+    decay = (C.c_ubyte * len(params))(*[1] * len(params))
+    k = L.AdamW()
+    k.params, k.grads, k.out, k.decay = C.addressof(p), C.addressof(g), None if o is None else C.addressof(o), C.addressof(decay)
+    k.m, k.v, k.exponents, k.steps = D, D + (1 << 34), D + (1 << 35), D + (1 << 36)
+    k.beta1, k.beta2, k.eps, k.lr, k.bits, k.blocks = 0.9, 0.999, 1e-8, 0.1, 8, 1 << 30
+    for name, v in kw.items():
+        setattr(k, name, v)
+    return L.lib().geeps_adamw(C.byref(k), None)
+
+
+def test_adamw_refusals():
+    one = dict(params=[(A, 1000)], p32=[1], grads=[(B, 1000)], g32=[1])
+    assert adamw([(A + 2, 10)], [1], [(B, 10)], [1]) == -15 and adamw([(A, 10)], [0], [(B + 1, 10)], [0]) == -15
+    assert adamw(**one, out=[(B + (1 << 20) + 2, 1000)], o32=[1]) == -15
+    assert adamw(**one, m=D + 2) == -15 and adamw(**one, bits=32, v=D + (1 << 34) + 8) == -15 and adamw(**one, steps=D + (1 << 36) + 4) == -15
+    assert adamw(**one, lr_ref=D - 2) == -15 and adamw(**one, norm=D - 1) == -15
+    assert adamw([(A, 1000)], [1], [(A + 3996, 1000)], [1]) == -13 and adamw([(A, 1000)], [1], [(A, 1000)], [1]) == -13
+    assert adamw([(A, 10), (A + 36, 10)], [1, 1], [(B, 10), (B + 40, 10)], [1, 1]) == -13
+    assert adamw(**one, out=[(B + 4, 1000)], o32=[1]) == -13 and adamw(**one, out=[(A, 1000)], o32=[1]) == -13
+    assert adamw(**one, out=[(B, 1000)], o32=[0]) == -13                                      # the gradients' place, but another type
+    assert adamw(**one, m=A) == -13 and adamw(**one, v=B) == -13 and adamw(**one, norm=A + 400) == -13 and adamw(**one, v=D + 512) == -13
+    assert adamw(**one, exponents=D + 4) == -13 and adamw(**one, steps=D + 8) == -13 and adamw(**one, lr_ref=D + (1 << 36)) == -13
+    assert adamw(**one, blocks=7) == 1 and adamw(**one, bits=16) == 1 and adamw(**one, beta1=1.0) == 1 and adamw(**one, beta2=-0.1) == 1 and adamw(**one, eps=-1.0) == 1
+    assert adamw([(A, 10)], [1], [(B, 11)], [1]) == 1 and adamw([(0, 10)], [1], [(B, 10)], [1]) == 1
+    # out may be the gradients themselves, and empty tensors may lie anywhere
+    assert adamw(**one, out=[(B, 1000)], o32=[1]) not in (-13, -15)
+    assert adamw([(A, 10), (A + 1, 0)], [1, 1], [(B, 10), (A + 3, 0)], [1, 0]) not in (-13, -15)
+
+
+def test_fp8_refusals():
+    def quantize(**kw):
+        p = L.QuantizeFp8()
+        p.x, p.q, p.scale, p.rows, p.cols, p.ldx, p.ldq = A, B, D, 10, 20, 20, 32
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return L.lib().geeps_quantize_fp8(C.byref(p), None)
+    for kw in (dict(x=A + 1), dict(x=A + 2, fp32=1), dict(ldx=19), dict(q=B + 8), dict(ldq=24), dict(ldq=16), dict(scale=0), dict(rows=-1), dict(cols=1 << 30),
+               dict(qt=B + 16, scale_t=0, ldqt=16), dict(qt=B + 4, scale_t=D, ldqt=16), dict(qt=B, scale_t=D, ldqt=8)):
+        assert quantize(**kw) == 1, kw
+    assert quantize(rows=0) == 0 and quantize(q=0) == 0
+
+    def gemm(**kw):
+        p = L.GemmFp8()
+        p.A, p.B, p.scale_a, p.scale_b, p.C, p.M, p.N, p.K, p.lda, p.ldb, p.ldc = A, B, D, D + 512, D + 4096, 100, 200, 300, 304, 304, 200
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return L.lib().geeps_gemm_fp8(C.byref(p), None)
+    for kw in (dict(A=A + 8), dict(scale_b=D + 8), dict(lda=303), dict(lda=288), dict(ldb=310), dict(ldc=199), dict(K=0), dict(M=-1), dict(N=1 << 30),
+               dict(bn=96, cluster=1), dict(bn=32, cluster=1), dict(bn=256, cluster=1), dict(bn=64, cluster=3), dict(bn=64, cluster=2), dict(bn=64, cluster=16),
+               dict(bn=64, cluster=-2, C=D + 4098), dict(bn=64, cluster=-2, ldc=201), dict(bn=96, cluster=-2), dict(bn=64, cluster=-2, swap=1)):
+        assert gemm(**kw) == 1, kw
+    assert gemm(M=0) == 0 and gemm(N=0) == 0
+
+
+def test_the_inception_models_with_group_norms():
+    for make in (inception_bn_small, inception_bn_22k):
+        batch, group = make(), make(norm="group")
+        b, g = list(batch.all_layers()), list(group.all_layers())
+        assert [type(l) for l in b] == [BatchNorm if isinstance(l, GroupNorm) else type(l) for l in g]
+        assert [l.name for l in b if hasattr(l, "cout")] == [l.name for l in g if hasattr(l, "cout")]
+        convs = {l.name: l.cout for l in g if hasattr(l, "cout")}
+        norms = [l for l in g if isinstance(l, GroupNorm)]
+        assert len(norms) == sum(isinstance(l, BatchNorm) for l in b) == len(convs)
+        assert all(l.act == "relu" and l.groups == norm_groups(convs[l.name[:-3]]) and convs[l.name[:-3]] % l.groups == 0 for l in norms)
+    assert [norm_groups(c) for c in (1, 3, 24, 80, 96, 160, 576)] == [1, 1, 8, 16, 32, 32, 32]
+    with pytest.raises(ValueError, match="norm"):
+        inception_bn_small(norm="layer")
