@@ -552,8 +552,10 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
 #pragma unroll 1
     for (; k < mine; ++k) f(k, x.get(k), dy.get(k));
   };
-  // z, rounded after each operation
-  auto border = [&](const float2& n, const float2& w, const float2& b) { return add2(mul2(n, w), b); };
+  // z, rounded after each operation: not in pairs, which are contracted to fused multiply-adds
+  auto border = [&](const float2& n, const float2& w, const float2& b) {
+    return make_float2(__fadd_rn(__fmul_rn(n.x, w.x), b.x), W > 1 ? __fadd_rn(__fmul_rn(n.y, w.y), b.y) : 0.f);
+  };
   if (PHASE != APPLY) {
     if constexpr (KEEP) copies_done();
     auto pass = [&](int v, auto act) __attribute__((always_inline)) {

@@ -266,6 +266,30 @@ def test_gradients_match_differences():
             assert abs((up - down) / (high - low) - grad.view(-1)[i].item()) <= 40 * h * h + 2.0 ** -22 / h * size
 
 
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("size", [(2, 64, 64, 8), (1, 30000, 64, 8), (2, 50, 21, 3)], ids=str)
+def test_the_border_of_the_relu_is_that_of_rounded_operations(size, types):
+    """A bias that is minus the product to the last bit: z is zero there, and no gradient passes, while a fused multiply-add leaves the
+    product's rounding error, above zero as often as below."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = size
+    x, dy, w, _ = made(*size, types, 9)
+    x = x.view(images, pixels, c)
+    x[:, ::2] = x[:1, :1]                                                # half of the pixels of a channel have one value ...
+    x = x.view(-1, c)
+    stats = statistics(x, images, groups).float()
+    stats[1:] = stats[:1]                                                # ... and z, in all images
+    mean, rstd = (spread(stats[:1, :, i], 1, groups, c)[0] for i in range(2))
+    b = -(((x[:1].float() - mean) * rstd) * w)[0]
+    dx, dw, db = torch.empty_like(x), torch.empty(c, device=DEV), torch.empty(c, device=DEV)
+    F.group_norm_backward(x, dy, dx, images, F.GroupNorm(groups, w, b, stats, EPS, "relu", dw, db))
+    z = ((x.float().view(images, pixels, c) - mean) * rstd) * w + b
+    assert (z[:, ::2] == 0).all()
+    check_backward(x, dy, dx, dw, db, stats, w, b, images, groups, "relu")
+    kept = (dy.float().view(images, pixels, c) * (z > 0)).double().sum((0, 1))
+    assert ((db.double() - kept).abs() <= 2.0 ** -14 * dy.double().abs().sum(0) * 2.0 ** -4).all()
+
+
 def test_without_rows_the_parameters_have_gradients_of_zero():
     from geeps_b200.ops import functional as F
     x = torch.empty(0, 16, dtype=BF, device=DEV)
