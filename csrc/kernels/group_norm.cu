@@ -15,8 +15,10 @@
 // Variance: values less the first of every 32 of a thread's pixels are added and squared, and such parts meet as count, mean and
 // sum of squared differences, so a mean far from zero costs nothing (a part's error is at most 32 x 2^-24 of its variance).
 // The backward pass forms z in the four rounded operations above, so that the border of the ReLU does not depend on how it is compiled.
+#include <math.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -166,29 +168,33 @@ __device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// A thread's own rows of vectors in shared memory, 16 bytes of every thread side by side
+// A thread's own rows of vectors in shared memory, 16 bytes of every thread side by side.  By addresses of the shared window: through
+// pointers that lambdas carry the accesses are generic ones
 template <typename T>
 struct Kept {
   static constexpr int kThreads = threads_of(KEPT);
-  uint8_t* base;
+  uint32_t base;                                            // of this thread
   static constexpr int kPieces = (int)sizeof(T) / 2;        // of 16 bytes
   static constexpr int kBytes = kThreads * 16 * kPieces;    // of a row
   __device__ __forceinline__ void fetch(int k, const T* src) const {
-    const uint32_t at = tc05::smem_u32(base) + k * kBytes + threadIdx.x * 16;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) copy_async(at + i * kThreads * 16, (const uint8_t*)src + 16 * i);
+    for (int i = 0; i < kPieces; ++i) copy_async(base + k * kBytes + i * kThreads * 16, (const uint8_t*)src + 16 * i);
   }
   __device__ __forceinline__ Vec<T, 8> get(int k) const {
     Vec<T, 8> v;
-    uint4* w = (uint4*)&v;
+    uint32_t* w = (uint32_t*)&v;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) w[i] = *(const uint4*)(base + k * kBytes + i * kThreads * 16 + threadIdx.x * 16);
+    for (int i = 0; i < kPieces; ++i)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w[4 * i]), "=r"(w[4 * i + 1]), "=r"(w[4 * i + 2]), "=r"(w[4 * i + 3]) : "r"(base + k * kBytes + i * kThreads * 16));
     return v;
   }
   __device__ __forceinline__ void put(int k, const Vec<T, 8>& v) const {
-    const uint4* w = (const uint4*)&v;
+    const uint32_t* w = (const uint32_t*)&v;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) *(uint4*)(base + k * kBytes + i * kThreads * 16 + threadIdx.x * 16) = w[i];
+    for (int i = 0; i < kPieces; ++i)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                   ::"r"(base + k * kBytes + i * kThreads * 16), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]), "r"(w[4 * i + 3]) : "memory");
   }
 };
 // Rows of a column as a thread reads them: from its own shared memory or where they lie
@@ -300,7 +306,7 @@ group_forward_kernel(const __grid_constant__ Dev d) {
   float2* entry = (float2*)(base_of + (narrow ? (d.slice + 3) & ~3 : 0));          // [W][R][V]: sums of the threads about a column's base
   const int mine = p.mine();
   const long long at = (p.pixel + p.r) * d.ldx + p.c0 + p.v * W;
-  Rows<XT, W, KEEP> x = {(const XT*)d.x + at, (long long)d.R * d.ldx, {(uint8_t*)entry + d.entries}};
+  Rows<XT, W, KEEP> x = {(const XT*)d.x + at, (long long)d.R * d.ldx, {tc05::smem_u32(entry) + (uint32_t)d.entries + threadIdx.x * 16}};
   geeps_pdl_enter();
 
   if (PHASE != APPLY) {
@@ -514,8 +520,8 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
   float2* entry = (float2*)(((uintptr_t)(whole + gs) + 15) & ~(uintptr_t)15);      // [W][R][V], unless there is one thread a column
   const int mine = p.mine();
   const long long x_at = (p.pixel + p.r) * d.ldx + p.c0 + p.v * W, dy_at = (p.pixel + p.r) * d.lddy + p.c0 + p.v * W;
-  Rows<XT, W, KEEP> x = {(const XT*)d.x + x_at, (long long)d.R * d.ldx, {(uint8_t*)entry + d.entries}};
-  Rows<YT, W, KEEP> dy = {(const YT*)d.dy + dy_at, (long long)d.R * d.lddy, {x.kept.base + (size_t)d.keep * Kept<XT>::kBytes}};
+  Rows<XT, W, KEEP> x = {(const XT*)d.x + x_at, (long long)d.R * d.ldx, {tc05::smem_u32(entry) + (uint32_t)d.entries + threadIdx.x * 16}};
+  Rows<YT, W, KEEP> dy = {(const YT*)d.dy + dy_at, (long long)d.R * d.lddy, {x.kept.base + (uint32_t)(d.keep * Kept<XT>::kBytes)}};
   geeps_pdl_enter();
   if constexpr (KEEP) {
     const XT* xs = x.at;
@@ -762,8 +768,11 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
   s.vec = vec;
   s.threads = threads_of(KEPT);
   const int row_bytes = s.threads * 16 * (vec ? (xsize / 2 + (backward ? ysize / 2 : 0)) : 0);      // of all threads' kept rows
-  // One launch: slices of 32 channels (whole sectors of a pixel) and more, and up to eight CTAs for an item.  The cost is how often the
-  // machine is filled by three CTAs an SM x what one takes, some 6 us and 1 us for 10 KB.
+  // One launch: slices of 32 channels (whole sectors of a pixel) and more, and up to eight CTAs for an item.  The cost in us: 6 for each
+  // time that the SMs' room is filled (a CTA's steps follow one another, and CTAs that began together rarely overlap; narrow slices
+  // have fewer channels a thread to join), and the bytes that an SM reads (as many are written).  Measured, bf16 forward,
+  // slice / CTAs of a cluster: 32 x 784 x 256: 32/1 9.0 us, 64/1 9.1, 32/3 10.8, 64/7 (just over one filling) 13.8, 32/8 21.8;
+  // 64 x 49 x 1024: 128/1 7.4, 512/1 9.1, 128/6 25.8; backward, 256 x 196 x 576: 72/1 56.5, 72/2 65.9, 288/3 88.
   auto cut = [&](Shape& t) {             // what a thread has of a slice
     t.V = t.slice / W;
     t.R = t.V < t.threads ? t.threads / t.V : 1;
@@ -792,31 +801,34 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
       const size_t smem = fixed_bytes(t, cg, backward) + t.entries + (size_t)((rows + t.R - 1) / t.R) * row_bytes;
       if (smem > kSmem || (k > 1 && rows < t.R)) continue;
       const int fit = (int)(228 * 1024 / (smem + 1024)), most = !vec ? 4 : !backward ? 6 : xsize == 2 ? 5 : 4, resident = fit < most ? fit : most;
-      const double filled = (double)images * t.slices * k / ((double)sms * resident);
-      const double kb = (double)rows * t.slice * (xsize + (backward ? ysize : 0)) / 1024;
-      const double cost = (filled > 1.0 ? filled : 1.0) * (6.0 + kb / (vec ? 10.0 : 1.7) + (k > 1 ? 2.0 : 0.0));
+      const double ctas = (double)images * t.slices * k, filled = ctas / ((double)sms * resident);
+      const double kb = (double)rows * t.slice * (xsize + (backward ? ysize : 0)) / 1024, join = k > 1 ? 0.5 : 0.0;
+      const double cost = vec ? ceil(filled) * (6.0 + 0.4 * t.slice / t.threads) + ceil(ctas / sms) * (0.15 + kb / (xsize == 2 ? 21.0 : 18.0)) + join
+                              : (filled > 1.0 ? filled : 1.0) * (6.0 + kb / 2.7 + join);
       if (cost < best) { best = cost; s = t; chunks = k; }
     }
   }
-  s.fused = chunks > 0;
-  // Two launches: what each SM reads twice from memory or L2, and their beginnings and ends
-  const double twice = 14.0 + (double)images * pixels * C * (xsize + (backward ? ysize : 0)) / 1024 / sms / (vec ? 14.0 : 2.0);
-  if (!s.fused || twice < best) {
-    s.fused = 0;
-    int n = 1;
-    while (unit * n < C && (unit * n < 64 || C / unit % n)) ++n;
-    s.threads = threads_of(SUMS);
-    for (;; --n) {                             // down to a width that fits (one group does)
-      if (C / unit % n) continue;
-      s.slice = unit * n;
-      s.slices = C / s.slice;
-      cut(s);
-      if (fixed_bytes(s, cg, backward) + s.entries <= kSmem) break;
-    }
-    const long long items = (long long)images * s.slices;
-    const long long want = (2LL * sms + items - 1) / items, most = (pixels + s.R - 1) / s.R;
-    chunks = (int)(want < most ? want : most);
-    if (chunks > kMostParts) chunks = kMostParts;
+  // Two launches, at best of one filling of two blocks an SM.  32 x 784 x 256: 9 x 32 = 288 blocks 13.1 us, 12 x 32 = 384 20.5.  Against one
+  // launch (two / one): bf16 32 x 784 x 256 forward 13.1 / 9.0, 32 x 3136 x 192 forward 31.5 / 25.9, backward 44.1 / 45.5, in fp32 75 / 122.
+  Shape u = s;
+  int n = 1;
+  while (unit * n < C && (unit * n < 64 || C / unit % n)) ++n;
+  u.threads = threads_of(SUMS);
+  for (;; --n) {                             // down to a width that fits (one group does)
+    if (C / unit % n) continue;
+    u.slice = unit * n;
+    u.slices = C / u.slice;
+    cut(u);
+    if (fixed_bytes(u, cg, backward) + u.entries <= kSmem) break;
+  }
+  const long long parts = (long long)images * u.slices, most = (pixels + u.R - 1) / u.R;
+  const int cuts = (int)std::max(1LL, std::min({2LL * sms / parts, most, (long long)kMostParts}));
+  const double kb = (double)images * pixels * C * (xsize + (backward ? ysize : 0)) / 1024 / sms;
+  const double twice = (backward ? 4.5 : 2.0) + 6.0 * ceil(parts * cuts / (2.0 * sms)) + kb / (!vec ? 2.0 : backward ? 16.0 : 11.6);
+  s.fused = chunks > 0 && best <= twice;
+  if (!s.fused) {
+    s = u;
+    chunks = cuts;
   }
   const long long items = (long long)images * s.slices;
   s.rows = (pixels + chunks - 1) / chunks;
@@ -900,7 +912,7 @@ int check(const GeepsGroupNorm* k, bool backward) {
   if (!k || k->images < 0 || k->pixels < 0 || (k->y_fp32 && !k->x_fp32) || !(k->eps >= 0.f) || k->act < 0 || k->act > 2) return (int)cudaErrorInvalidValue;
   if (k->C < 1 || k->C > 16384) return GEEPS_ERR_NORM_CHANNELS;
   if (k->groups < 1 || k->C % k->groups) return GEEPS_ERR_GROUPS;
-  if (k->images * k->pixels > (1LL << 30)) return (int)cudaErrorInvalidValue;
+  if (k->images > (1LL << 30) || k->pixels > (1LL << 30) || k->images * k->pixels > (1LL << 30)) return (int)cudaErrorInvalidValue;
   const long long rows = k->images * k->pixels;
   const int xs = k->x_fp32 ? 4 : 2, ys = k->y_fp32 ? 4 : 2;
   struct Range { const void* at; long long bytes; bool written; long long pitch; int align; };      // pitch: of rows, in bytes; 0: none
@@ -959,7 +971,7 @@ int call(const GeepsGroupNorm* k, bool backward, void* stream) {
 extern "C" {
 
 long long geeps_group_norm_work(long long images, long long pixels, int C, int groups, int backward) {
-  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || images * pixels > (1LL << 30)) return 0;
+  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30)) return 0;
   // of two launches for vectors or single values, whichever the addresses will allow, of any type: the chunks' group sums; backward
   // also the channels' sums of the chunks or images
   long long most = 0;
@@ -977,7 +989,8 @@ int geeps_group_norm_forward(const GeepsGroupNorm* p, void* stream) { return cal
 int geeps_group_norm_backward(const GeepsGroupNorm* p, void* stream) { return call(p, true, stream); }
 
 int geeps_group_norm_shape(long long images, long long pixels, int C, int groups, int backward, int vec, int x_fp32, int y_fp32, int* out) {
-  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || (vec && C % 8)) return (int)cudaErrorInvalidValue;
+  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || (vec && C % 8) || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30))
+    return (int)cudaErrorInvalidValue;
   const Shape s = choose((int)images, (int)pixels, C, groups, backward, vec, x_fp32 ? 4 : 2, y_fp32 ? 4 : 2);
   out[0] = s.fused; out[1] = s.slice; out[2] = s.chunks; out[3] = s.rows; out[4] = s.keep; out[5] = s.blocks; out[6] = (int)s.smem; out[7] = s.threads;
   return 0;
