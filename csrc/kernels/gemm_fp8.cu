@@ -17,7 +17,9 @@
 #include <mutex>
 
 #include "kernels.h"
+#include "nn_ops.h"
 #include "tc05.cuh"
+#include "tensor_list.h"
 
 namespace {
 
@@ -605,8 +607,14 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
   if (p->M == 0 || p->N == 0) return 0;
   if (p->K == 0) return (int)cudaErrorInvalidValue;
   if ((((uintptr_t)p->A | (uintptr_t)p->B | (uintptr_t)p->scale_a | (uintptr_t)p->scale_b) & 15) || (p->lda & 15) || (p->ldb & 15) ||
-      p->lda < p->K || p->ldb < p->K || p->ldc < p->N)
+      p->lda < p->K || p->ldb < p->K || p->ldc < p->N || !p->A || !p->B || !p->scale_a || !p->scale_b || !p->C ||
+      ((uintptr_t)p->C & (p->out_fp32 ? 3 : 1)) || (((uintptr_t)p->bias | (uintptr_t)p->status) & 3))
     return (int)cudaErrorInvalidValue;
+  const long long quads = (p->K + 511) / 512;
+  const MemoryRange ranges[] = {{p->C, ((p->M - 1) * p->ldc + p->N) * (p->out_fp32 ? 4 : 2)}, {p->A, (p->M - 1) * p->lda + p->K}, {p->B, (p->N - 1) * p->ldb + p->K},
+                                {p->scale_a, (p->M + 127) / 128 * quads * 512}, {p->scale_b, (p->N + 127) / 128 * quads * 512},
+                                {p->bias, p->bias ? p->N * 4 : 0}, {p->status, p->status ? 16 : 0}};
+  if (ranges_overlap(ranges, 1, 7)) return GEEPS_ERR_NORM_OVERLAP;
   const int sms = geeps_sm_count();
   Plan plan = p->bn ? Plan{p->swap, p->bn, p->cluster < 0 ? 1 : p->cluster, p->cluster < 0} : choose(p, sms);
   Dev d = {};

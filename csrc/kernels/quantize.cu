@@ -8,6 +8,8 @@
 // x transposed (through shared memory) or both, so that a training step reads its gradient once for its two products.
 #include "common.cuh"
 #include "kernels.h"
+#include "nn_ops.h"
+#include "tensor_list.h"
 
 namespace {
 
@@ -145,6 +147,7 @@ quantize_tile_kernel(const GeepsQuantizeFp8 p, unsigned tiles_c, long long quads
     __syncthreads();
   }
   if (p.q != nullptr) {
+    const long long pitch = (p.cols + 15) & ~15LL;         // what a row has, with its padding: others may lie behind it
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t b = byte;
@@ -160,7 +163,7 @@ quantize_tile_kernel(const GeepsQuantizeFp8 p, unsigned tiles_c, long long quads
       const float inv = inverse(b);
       const uint32_t lo = e4m3x2(f[i][0] * inv, f[i][1] * inv) | e4m3x2(f[i][2] * inv, f[i][3] * inv) << 16;
       const uint32_t hi = e4m3x2(f[i][4] * inv, f[i][5] * inv) | e4m3x2(f[i][6] * inv, f[i][7] * inv) << 16;
-      if (r0 + i < p.rows && c0 < p.ldq) *reinterpret_cast<uint2*>((uint8_t*)p.q + (r0 + i) * p.ldq + c0) = make_uint2(lo, hi);
+      if (r0 + i < p.rows && c0 < pitch) *reinterpret_cast<uint2*>((uint8_t*)p.q + (r0 + i) * p.ldq + c0) = make_uint2(lo, hi);
     }
   }
   if (p.qt != nullptr) {
@@ -178,7 +181,7 @@ quantize_tile_kernel(const GeepsQuantizeFp8 p, unsigned tiles_c, long long quads
       const int c = s * 32 + (tid >> 3), piece = (tid & 7) * 2, x = c >> 3;
       const uint2 a = turned[c * 16 + (piece ^ x)], b = turned[c * 16 + ((piece + 1) ^ x)];
       const long long row = bc * 128 + c, at = br * 128 + piece * 8;
-      if (row < p.cols && at < p.ldqt) *reinterpret_cast<uint4*>((uint8_t*)p.qt + row * p.ldqt + at) = make_uint4(a.x, a.y, b.x, b.y);
+      if (row < p.cols && at < ((p.rows + 15) & ~15LL)) *reinterpret_cast<uint4*>((uint8_t*)p.qt + row * p.ldqt + at) = make_uint4(a.x, a.y, b.x, b.y);
     }
   }
 }
@@ -189,11 +192,16 @@ extern "C" int geeps_quantize_fp8(const GeepsQuantizeFp8* p, void* stream) {
   const int size = p->fp32 ? 4 : 2;
   if (p->rows < 0 || p->cols < 0 || p->rows > 0x3fffffffLL || p->cols > 0x3fffffffLL) return (int)cudaErrorInvalidValue;
   if (p->rows == 0 || p->cols == 0 || (p->q == nullptr && p->qt == nullptr)) return 0;
-  if (((uintptr_t)p->x & (size - 1)) || p->ldx < p->cols) return (int)cudaErrorInvalidValue;
+  if (p->x == nullptr || ((uintptr_t)p->x & (size - 1)) || p->ldx < p->cols) return (int)cudaErrorInvalidValue;
   if (p->q != nullptr && (((uintptr_t)p->q & 15) || (p->ldq & 15) || p->ldq < p->cols || p->scale == nullptr)) return (int)cudaErrorInvalidValue;
   if (p->qt != nullptr && (((uintptr_t)p->qt & 15) || (p->ldqt & 15) || p->ldqt < p->rows || p->scale_t == nullptr)) return (int)cudaErrorInvalidValue;
-  const bool vec = ((uintptr_t)p->x & 15) == 0 && p->ldx * size % 16 == 0;
   const long long quads = (p->cols + 511) / 512, quads_t = (p->rows + 511) / 512;
+  auto bytes = [](long long rows, long long ld, long long cols) { return (rows - 1) * ld + cols; };
+  const MemoryRange ranges[] = {{p->q, p->q ? bytes(p->rows, p->ldq, (p->cols + 15) & ~15LL) : 0}, {p->scale, p->q ? (p->rows + 127) / 128 * quads * 512 : 0},
+                                {p->qt, p->qt ? bytes(p->cols, p->ldqt, (p->rows + 15) & ~15LL) : 0}, {p->scale_t, p->qt ? (p->cols + 127) / 128 * quads_t * 512 : 0},
+                                {p->x, bytes(p->rows, p->ldx, p->cols) * size}};
+  if (ranges_overlap(ranges, 4, 5)) return GEEPS_ERR_NORM_OVERLAP;
+  const bool vec = ((uintptr_t)p->x & 15) == 0 && p->ldx * size % 16 == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (p->qt == nullptr && !p->tile) {
     const long long units = p->rows * quads, most = (long long)geeps_sm_count() * 8, want = (units + 7) / 8;

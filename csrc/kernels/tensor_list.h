@@ -1,8 +1,17 @@
-// Lists of tensors as clip.cu and adamw.cu take them: addresses and overlaps (host arithmetic only).
+// Operands' memory: ranges, and lists of tensors as clip.cu and adamw.cu take them (host arithmetic only).
 #pragma once
 #include <stdint.h>
 
 #include "nn_ops.h"
+
+struct MemoryRange { const void* at; long long bytes; };
+// Does one of the first `written` ranges share memory with another of all?  Absent ones have no bytes.
+inline bool ranges_overlap(const MemoryRange* r, int written, int all) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < all; ++j)
+      if (r[i].bytes > 0 && r[j].bytes > 0 && (uintptr_t)r[i].at < (uintptr_t)r[j].at + r[j].bytes && (uintptr_t)r[j].at < (uintptr_t)r[i].at + r[i].bytes) return true;
+  return false;
+}
 
 struct TensorRange { uintptr_t from, to; };
 inline TensorRange tensor_range(const GeepsTensors& t, long long i) {

@@ -878,15 +878,31 @@ def adamw_moments(state: AdamWState, m: torch.Tensor, v: torch.Tensor):
 class Fp8Matrix:
     """A matrix [rows, cols] in e4m3 with a scale 2^e for every 128 columns of a row: `q` (float8_e4m3fn, rows on a pitch of a
     multiple of 16) and `scale` (E8M0 bytes, 512 for 128 rows x 4 blocks, in the order in which the tensor cores take them).
-    quantize_fp8() fills it, matmul_fp8() multiplies it."""
-    __slots__ = ("rows", "cols", "q", "scale", "pitch", "device", "_at")
+    quantize_fp8() fills it, matmul_fp8() multiplies it.  Values from elsewhere are copied into q and scale, which stay where they are."""
+    __slots__ = ("rows", "cols", "_q", "_scale", "pitch", "device", "_at")
 
     def __init__(self, rows: int, cols: int, device):
         _need(0 <= rows < 1 << 30 and 0 < cols < 1 << 30, f"Fp8Matrix: need 0 to 2^30 rows and 1 to 2^30 columns, got {rows} x {cols}")
-        self.rows, self.cols, self.pitch = rows, cols, (cols + 15) // 16 * 16
-        self.q = torch.zeros(rows, self.pitch, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)[:, :cols]
-        self.scale = torch.zeros((rows + 127) // 128, (cols + 511) // 512, 512, dtype=torch.uint8, device=device)
-        self.device, self._at = self.q.get_device(), (self.q.data_ptr(), self.scale.data_ptr())
+        pitch = (cols + 15) // 16 * 16
+        self.__setstate__((rows, cols, torch.zeros(rows, pitch, dtype=torch.uint8, device=device),
+                           torch.zeros((rows + 127) // 128, (cols + 511) // 512, 512, dtype=torch.uint8, device=device)))
+
+    def __getstate__(self):
+        return self.rows, self.cols, self._q.as_strided((self.rows, self.pitch), (self.pitch, 1)).view(torch.uint8), self._scale
+
+    def __setstate__(self, state):
+        """Addresses are those of this object's tensors: a copy has its own."""
+        self.rows, self.cols, q, self._scale = state
+        self._q, self.pitch = q.view(torch.float8_e4m3fn)[:, :self.cols], q.shape[1]
+        self.device, self._at = q.get_device(), (q.data_ptr(), self._scale.data_ptr())
+
+    @property
+    def q(self) -> torch.Tensor:
+        return self._q
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._scale
 
     def exponents(self) -> torch.Tensor:
         """e + 127 of every block, uint8 [rows, ceil(cols / 128)]; 255 where the block stands for NaN."""

@@ -129,6 +129,12 @@ def main(argv=None) -> None:
     ap.add_argument("--no-graph", action="store_true")
     ap.add_argument("--seed", type=int, default=1)
     args = ap.parse_args(argv)
+    if args.fp8_linear and args.model != "alexnet":
+        ap.error("--fp8-linear is for alexnet")
+    if args.norm == "group" and args.model == "alexnet":
+        ap.error("--norm group is for the Inception models")
+    if args.adam_bits == 8 and args.optimizer != "adamw":
+        ap.error("--adam-bits is for --optimizer adamw")
 
     import numpy as np
     import torch

@@ -1,4 +1,5 @@
 """Casts to e4m3 with a scale for each block of 128, and products of such matrices, against 64-bit arithmetic."""
+import copy
 import math
 
 import pytest
@@ -197,6 +198,32 @@ def test_products_repeat_on_other_streams_and_in_graphs():
                 g.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_a_copied_matrix_multiplies_its_own_values():
+    from geeps_b200.ops import functional as F
+    a, b = F.quantize_fp8(torch.randn(130, 700, device=DEV)), F.quantize_fp8(torch.randn(40, 700, device=DEV))
+    want, got = torch.empty(130, 40, device=DEV), torch.empty(130, 40, device=DEV)
+    F.matmul_fp8(a, b, want)
+    c = copy.deepcopy(a)
+    a.q.zero_()
+    F.matmul_fp8(c, b, got)
+    assert torch.equal(want, got)
+
+
+def test_shared_memory_is_refused():
+    from geeps_b200.ops import functional as F
+    x = torch.zeros(40, 40, device=DEV)
+    q = F.quantize_fp8(x)
+    with pytest.raises(ValueError, match="overlaps"):
+        F.quantize_fp8(x, q, transposed=q)
+    out = torch.zeros(1600, dtype=torch.bfloat16, device=DEV)                    # a product into one of its operands, and a cast of itself
+    a = F.Fp8Matrix(30, 48, DEV)
+    a.__setstate__((30, 48, out.view(torch.uint8)[1600:1600 + 30 * 48].view(30, 48), a.scale))
+    with pytest.raises(ValueError, match="overlaps"):
+        F.matmul_fp8(a, F.Fp8Matrix(20, 48, DEV), out[600:1200].view(30, 20))
+    with pytest.raises(ValueError, match="overlaps"):
+        F.quantize_fp8(out[:1440].view(30, 48), a)
 
 
 def test_refusals():

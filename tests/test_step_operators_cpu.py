@@ -1,11 +1,15 @@
 """Host side of group norm, AdamW steps and 8-bit products: launch shapes, workspaces and refusals, which need no GPU."""
+import copy
 import ctypes as C
+import pickle
 
 import pytest
 import torch
 
+from geeps_b200 import train
 from geeps_b200.models.inception_bn import inception_bn_22k, inception_bn_small, norm_groups
 from geeps_b200.ops import _lib as L
+from geeps_b200.ops import functional as F
 from geeps_b200.ops.layers import BatchNorm, GroupNorm
 
 A, B, D = 1 << 32, 1 << 36, 1 << 40          # addresses that are never touched: every call here is refused
@@ -137,7 +141,11 @@ def test_fp8_refusals():
     for kw in (dict(x=A + 1), dict(x=A + 2, fp32=1), dict(ldx=19), dict(q=B + 8), dict(ldq=24), dict(ldq=16), dict(scale=0), dict(rows=-1), dict(cols=1 << 30),
                dict(qt=B + 16, scale_t=0, ldqt=16), dict(qt=B + 4, scale_t=D, ldqt=16), dict(qt=B, scale_t=D, ldqt=8)):
         assert quantize(**kw) == 1, kw
-    assert quantize(rows=0) == 0 and quantize(q=0) == 0
+    assert quantize(rows=0) == 0 and quantize(q=0) == 0 and quantize(x=0) == 1
+    both = dict(qt=B + 4096, scale_t=D + 4096, ldqt=16)
+    for kw in (dict(q=A), dict(q=A + 384), dict(scale=A + 399), dict(scale=B + 304), dict(both, qt=B), dict(both, qt=B + 304), dict(both, scale_t=D), dict(both, scale_t=D + 511),
+               dict(both, scale_t=A), dict(both, qt=D + 496)):
+        assert quantize(**kw) == -12, kw
 
     def gemm(**kw):
         p = L.GemmFp8()
@@ -150,6 +158,30 @@ def test_fp8_refusals():
                dict(bn=64, cluster=-2, C=D + 4098), dict(bn=64, cluster=-2, ldc=201), dict(bn=96, cluster=-2), dict(bn=64, cluster=-2, swap=1)):
         assert gemm(**kw) == 1, kw
     assert gemm(M=0) == 0 and gemm(N=0) == 0
+    for kw in (dict(A=0), dict(B=0), dict(scale_a=0), dict(scale_b=0), dict(C=0), dict(C=D + 4097), dict(C=D + 4098, out_fp32=1), dict(bias=D + 2), dict(status=D + 3)):
+        assert gemm(**kw) == 1, kw
+    for kw in (dict(C=A), dict(C=A + 304 * 99 + 298), dict(C=B - 2), dict(C=D - 39998), dict(C=D + 512 + 1022), dict(bias=D + 4096), dict(status=D + 4096 + 39996)):
+        assert gemm(**kw) == -12, kw
+
+
+def test_a_copied_matrix_has_its_own_memory():
+    a = F.Fp8Matrix(5, 20, "cpu")
+    a.q.copy_(torch.arange(100.0).view(5, 20))
+    a.scale.fill_(127)
+    for b in (copy.deepcopy(a), pickle.loads(pickle.dumps(a))):
+        assert b._at == (b.q.data_ptr(), b.scale.data_ptr()) and b._at[0] != a._at[0] and b._at[1] != a._at[1] and b.q.stride() == (32, 1)
+        assert torch.equal(b.dequantize(), a.dequantize()) and (b.rows, b.cols, b.pitch, b.device) == (5, 20, 32, -1)
+    with pytest.raises(AttributeError):
+        a.q = a.q.clone()
+    with pytest.raises(AttributeError):
+        a.scale = a.scale.clone()
+
+
+@pytest.mark.parametrize("options", [["--model", "inception_bn_small", "--fp8-linear"], ["--model", "alexnet", "--norm", "group"], ["--adam-bits", "8"]])
+def test_the_trainer_refuses_options_without_effect(options, capsys):
+    with pytest.raises(SystemExit):
+        train.main(options)
+    assert "is for" in capsys.readouterr().err
 
 
 def test_the_inception_models_with_group_norms():
