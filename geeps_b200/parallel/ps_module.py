@@ -13,6 +13,8 @@ Stands in for the solver glue of the reference's (absent) Caffe application.
 """
 from __future__ import annotations
 
+import os
+
 import torch
 
 from ..ops import _lib as L
@@ -48,11 +50,26 @@ class _Table:
 
 class _AdamW:
     """The AdamW step of a module's tables: gradients in the update buffers become the updates."""
+    _KEPT = ("m", "v", "exponents", "steps")
 
     def __init__(self, device, world, learning_rate, weight_decay, betas=(0.9, 0.999), eps: float = 1e-8, bits: int = 32, seed: int | None = None):
         self.betas, self.eps, self.bits, self.seed, self.weight_decay, self.world = betas, eps, bits, seed, weight_decay, world
         self.lr = torch.tensor([learning_rate / world], device=device)
-        self.state, self._lists = None, {}
+        self.state, self._lists, self._resumed = None, {}, None
+
+    def save(self, directory: str, rank: int) -> None:
+        if self.state is not None:
+            os.makedirs(directory, exist_ok=True)
+            torch.save({k: getattr(self.state, k) for k in self._KEPT}, os.path.join(directory, f"adamw.{rank}"))
+
+    def resume(self, directory: str, rank: int) -> None:
+        """A rank that the saved job did not have goes on with rank 0's states; a snapshot without any begins anew."""
+        with open(os.path.join(directory, "LATEST")) as f:
+            at = os.path.join(directory, f"snapshot.{int(f.read())}")
+        for r in (rank, 0):
+            if os.path.exists(os.path.join(at, f"adamw.{r}")):
+                self._resumed = torch.load(os.path.join(at, f"adamw.{r}"), map_location=self.lr.device)
+                return
 
     def set(self, learning_rate=None, weight_decay=None) -> bool:
         """Whether a recorded step carries an old value."""
@@ -74,6 +91,10 @@ class _AdamW:
         _, params, grads = lists
         if self.state is None:
             self.state = F.AdamWState(params, self.bits, [sp.decay for _, sp in names])
+            if self._resumed is not None:
+                for k in self._KEPT:
+                    setattr(self.state, k, self._resumed[k])
+                self._resumed = None
         clip = None
         if mod.clip_gradients is not None:
             if mod._clip_work is None:
@@ -120,8 +141,8 @@ class PSModule:
         stochastic rounding; None: to the nearest), each optional.  The rate is ps_config.learning_rate (set_hyper_params changes it
         without a new capture), the decay ps_config.weight_decay, for the parameters that decay.  Of several workers each takes 1 /
         world of its own step.  With clip_gradients the gradients are scaled on their way into the step and `clip_result` holds {norm, 1}.
-        Parameters are given back when the step has read them.  The states (`adamw.state`) are the worker's own and not part of a
-        table snapshot."""
+        Parameters are given back when the step has read them.  The states (`adamw.state`) are the worker's own; save_snapshot writes
+        and resume_from reads them."""
         self.net, self.rank, self.world, self.slack = net, rank, world, slack
         self.device = torch.device(device)
         self.trace = trace or NullTrace()
@@ -223,6 +244,8 @@ class PSModule:
         if resume_from is not None:
             if not self.ps.load_snapshot(resume_from):
                 raise RuntimeError(f"resume from {resume_from}: {self.ps.last_error_string()}")
+            if self.adamw is not None:
+                self.adamw.resume(resume_from, rank)
         else:
             self._bootstrap(seed)
         self.ps.start_iterations()
@@ -478,7 +501,9 @@ class PSModule:
 
     def save_snapshot(self, directory: str) -> None:
         """Write every table (master rows, momentum, clocks) under directory/snapshot.<clock>; every rank calls it
-        before the same step."""
+        before the same step.  AdamW's states go beside them, a file for each rank."""
+        if self.adamw is not None:          # first: what LATEST names is complete
+            self.adamw.save(os.path.join(directory, f"snapshot.{self.ps.clock_value}"), self.rank)
         if not self.ps.save_snapshot(directory):
             raise RuntimeError(f"snapshot to {directory}: {self.ps.last_error_string()}")
 

@@ -164,6 +164,36 @@ def test_an_inception_net_with_group_norms_trains_in_graphs_and_with_managed_act
         assert abs(other[0] - losses[0][0]) <= 64 * 2.0 ** -24 * abs(losses[0][0])
 
 
+@pytest.mark.parametrize("bits,seed", [(32, None), (8, 3)])
+def test_a_resumed_module_goes_on_with_its_states(bits, seed, tmp_path):
+    x, y = batch()
+    kw = dict(adamw=dict(bits=bits, seed=seed))
+    mod = module(**kw)
+    for _ in range(3):
+        mod.step(x, y)
+    mod.save_snapshot(str(tmp_path))
+    kept = {k: None if getattr(mod.adamw.state, k) is None else getattr(mod.adamw.state, k).clone() for k in ("m", "v", "exponents", "steps")}
+    mod.step(x, y)
+    went = mod.adamw.state.m.float()
+    mod.close()
+    other = module(resume_from=str(tmp_path), **kw)
+    assert other.steps == 3 and all(k is None or torch.equal(k, other.adamw._resumed[n]) for n, k in kept.items())
+    other.step(x, y)
+    state = other.adamw.state
+    assert state.steps.tolist() == [4, 0]
+    if bits == 32:            # the gradients of equal parameters: sums in any order, at worst another rounding (2^-8) of a layer's bf16 gradient
+        for o, n in zip(state.offsets, state.params.numel):
+            a, b = went[o:o + n], state.m[o:o + n]
+            assert (a - b).abs().max() <= 2.0 ** -8 * a.abs().max()
+    other.close()
+    with pytest.raises(ValueError, match="AdamWState"):
+        wrong = module(resume_from=str(tmp_path), adamw=dict(bits=40 - bits))
+        try:
+            wrong.step(x, y)
+        finally:
+            wrong.close()
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="additive"):
         PSModule(net(), (16, 3, 8, 8), cfg(TRANSPORT_NVLINK), device="cuda:0", adamw={})
