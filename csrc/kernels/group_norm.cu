@@ -854,8 +854,11 @@ Shape choose(int images, int pixels, int C, int groups, bool backward, bool vec,
   return m.s;
 }
 
+// Dependent launches (us in a captured chain of 12, ordinary / dependent): 1 x 196 x 576 6.0 / 5.6, 8 x 196 x 512 5.8 / 5.4, backward of
+// 4 x 784 x 256 8.1 / 7.8 and of 16 x 1024 x 640 in fp32 (two launches) 46.4 / 45.3.  Forward with several blocks an SM in one launch
+// they come up where the predecessor leaves room, and SMs run dry: 64 x 49 x 1024 7.4 / 7.9, 37 x 113 x 1003 14.3 / 15.2.
 template <auto kernel, typename... A>
-int launch(const Shape& s, bool cluster, cudaStream_t st, A&&... args) {
+int launch(const Shape& s, bool cluster, bool dependent, cudaStream_t st, A&&... args) {
   static std::atomic<unsigned long long> ready{0};           // devices on which the kernel may have all shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -869,12 +872,14 @@ int launch(const Shape& s, bool cluster, cudaStream_t st, A&&... args) {
   cfg.blockDim = dim3(s.threads);
   cfg.dynamicSmemBytes = s.smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)s.chunks;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = cluster && s.chunks > 1 ? 1 : 0;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)s.chunks;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = dependent ? at : at + 1;
+  cfg.numAttrs = (dependent ? 1 : 0) + (cluster && s.chunks > 1 ? 1 : 0);
   return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...);
 }
 
@@ -883,19 +888,19 @@ int run(const GeepsGroupNorm& k, const Shape& s, const Dev& d, bool backward, cu
   constexpr int ONE = VEC ? KEPT : TWICE;
   int e;
   if (!backward) {
-    if (s.fused) return launch<group_forward_kernel<XT, YT, VEC, ONE>>(s, true, st, d);
-    e = launch<group_forward_kernel<XT, YT, VEC, SUMS>>(s, false, st, d);
-    return e ? e : launch<group_forward_kernel<XT, YT, VEC, APPLY>>(s, false, st, d);
+    if (s.fused) return launch<group_forward_kernel<XT, YT, VEC, ONE>>(s, true, s.blocks <= geeps_sm_count(), st, d);
+    e = launch<group_forward_kernel<XT, YT, VEC, SUMS>>(s, false, true, st, d);
+    return e ? e : launch<group_forward_kernel<XT, YT, VEC, APPLY>>(s, false, true, st, d);
   }
   const bool want = k.dweight != nullptr || k.dbias != nullptr;
   // group sums of the chunks (two launches only), then the channels' sums of the images or chunks
   const long long parts = (long long)k.images * (s.fused ? 1 : s.chunks);
   float* channel = want ? k.work + (s.fused ? 0 : parts * k.groups * 2) : nullptr;
   if (s.fused) {
-    e = launch<group_backward_kernel<XT, YT, VEC, ONE>>(s, true, st, d, channel);
+    e = launch<group_backward_kernel<XT, YT, VEC, ONE>>(s, true, true, st, d, channel);
   } else {
-    e = launch<group_backward_kernel<XT, YT, VEC, SUMS>>(s, false, st, d, channel);
-    if (!e) e = launch<group_backward_kernel<XT, YT, VEC, APPLY>>(s, false, st, d, channel);
+    e = launch<group_backward_kernel<XT, YT, VEC, SUMS>>(s, false, true, st, d, channel);
+    if (!e) e = launch<group_backward_kernel<XT, YT, VEC, APPLY>>(s, false, true, st, d, channel);
   }
   if (e || !want) return e;
   geeps_launch(group_parameters_kernel, dim3((unsigned)((k.C + 7) / 8)), dim3(256), 0, st, (const float2*)channel, parts, k.C, k.dweight, k.dbias);
