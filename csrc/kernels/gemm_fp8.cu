@@ -13,6 +13,7 @@
 // Every mbarrier wait is bounded; on expiry the CTA records TIMEOUT in `status`, stops issuing work, frees its TMEM and returns.
 #include <cuda.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -124,6 +125,34 @@ __device__ __forceinline__ void store_slabs(const Dev& d, const CUtensorMap& tmC
       tc05::bulk_commit();
     }
     ++slab_i;
+  }
+}
+
+// The same for rows of any pitch and alignment: a warp turns its 32 rows from row0 on through 4 KB of shared memory, 32 columns at a
+// time, so that its lanes store neighbours.  (A row a lane: 4068 x 647, K = 74 32.6 us, so 8.7.)
+template <int G>
+__device__ __forceinline__ void store_rows(const Dev& d, uint8_t* turned, uint32_t tacc, int row0, int n0, int grp, int lane) {
+  const int rows = (int)min((long long)32, d.M - row0);
+#pragma unroll 1
+  for (int c = grp * 32; c < d.bn; c += G * 32) {
+    if ((long long)n0 + c >= d.N) break;
+    uint32_t w[32];
+    tc05::tmem_ld_32x32(tacc + (uint32_t)c, w);
+    tc05::tmem_ld_wait();
+    __syncwarp();              // the last 32 columns have been read
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      *reinterpret_cast<uint4*>(turned + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+    const long long col = (long long)n0 + c + lane;
+    if (col >= d.N) continue;
+    const float bias = d.bias != nullptr ? __ldg(d.bias + col) : 0.f;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      float v = *reinterpret_cast<const float*>(turned + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) + bias;
+      if (d.relu) v = v < 0.f ? 0.f : v;
+      store1(d, (row0 + r) * d.ldc + col, v);
+    }
   }
 }
 
@@ -313,10 +342,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         leave_part(tiles, tacc, r, BN);
       } else if (d.tma_store) {
         store_slabs<G, true>(d, tmC, slabs, tacc, m0, n0, grp, r, slab_i);
+      } else if (!d.swap) {
+        store_rows<G>(d, slabs + grp * SLAB_BYTES + q * 32 * 128, tacc, m0 + q * 32, n0, grp, lane);
       } else {
-        // any pitch and alignment; with the operands swapped the lanes of a warp are neighbours in C
-        const long long ri = d.swap ? 1 : d.ldc, ci = d.swap ? d.ldc : 1;
-        const float bias_row = d.swap && d.bias != nullptr && row < d.M ? d.bias[row] : 0.f;
+        // the lanes of a warp are neighbours in C
+        const float bias_row = d.bias != nullptr && row < d.M ? d.bias[row] : 0.f;
 #pragma unroll 1
         for (int c = grp * 32; c < BN; c += G * 32) {
           uint32_t w[32];
@@ -328,9 +358,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             for (int j = 0; j < 32; ++j) {
               if (col0 + j < d.N) {
                 float v = __uint_as_float(w[j]) + bias_row;
-                if (!d.swap && d.bias != nullptr) v += __ldg(d.bias + col0 + j);
                 if (d.relu) v = v < 0.f ? 0.f : v;
-                store1(d, row * ri + (col0 + j) * ci, v);
+                store1(d, row + (col0 + j) * d.ldc, v);
               }
             }
           }
@@ -523,14 +552,16 @@ bool width_ok(int bn, long long N) { return bn == 64 || bn == 128 || bn == 192 |
 // Whether an atom's worth of every slice is there
 bool slices_ok(int quads, int cluster) { return (long long)((quads + cluster - 1) / cluster) * (cluster - 1) < quads; }
 
-// The cut with the shortest expected time.  A k tile takes a round trip through the ring of stages (0.25 us, pairs 0.33) or what L2
-// needs for its operands (130 KB/us an SM, 15.5 MB/us in all): seldom the tensor pipe's time (0.2 us for 128 x 192), so wide tiles and
+// The cut with the shortest expected time.  A k tile takes a round trip through the ring of stages (0.18 us, pairs 0.30) or what L2
+// needs for its operands (128 KB/us an SM, 14 MB/us in all): seldom the tensor pipe's time (0.2 us for 128 x 192), so wide tiles and
 // pairs win where there are enough of them, and slices of K where there are not.  In a captured chain, us (width / CTAs that share K,
 // p: pairs): 8192 x 16384, K = 4096 407 (192p), 482 (192/1), 588 (128/1); 1024 x 9216, K = 4096 32.2 (192p), 39.1, 39.2; 2048 x 4096,
 // K = 4096 31.8 (192p), 34.9, 36.6; 512 x 4096, K = 4096 11.8 (128/1), 13.9 (192p), 14.0; 256 x 4096, K = 9216 17.8 (128/2), 19.6
 // (64/1), 20.0 (128/1); with B's rows on the tall side 7 x 4096, K = 4096 7 (32/4), 8.3 (32/2), 10.3 (32/1).
+// With few k tiles what is around them counts: 449 x 6912, K = 256 5.0 (192/1), 6.8 (192p); 3913 x 1408 in fp32 7.6, 11.6; 6313 x 4352,
+// K = 512 in fp32 29.0, 37.3.  Over 110 sizes of 1 to 9216 the chosen cut takes 1.5 % longer than the best one.
 Plan choose(const GeepsGemmFp8* p, int sms) {
-  const int quads = (int)((p->K + 511) / 512);
+  const int quads = (int)((p->K + 511) / 512), tiles_k = (int)((p->K + BK - 1) / BK);
   const bool rows16 = ((uintptr_t)p->C & 15) == 0 && p->ldc * (p->out_fp32 ? 4 : 2) % 16 == 0;
   Plan best = {0, 64, 1, 0};
   double least = 1e300;
@@ -549,13 +580,11 @@ Plan choose(const GeepsGemmFp8* p, int sms) {
           const int slots = size <= 2 ? sms : size <= 4 ? sms * 9 / 10 / size * size : sms * 5 / 6 / size * size;
           const long long rounds = (tiles * size + slots - 1) / slots;
           if (cs > 1 && rounds > 1) continue;
-          const double active = (double)(tiles * size < slots ? tiles * size : slots), kt = 4.0 * ((quads + cs - 1) / cs);
+          const double active = (double)(tiles * size < slots ? tiles * size : slots), kt = std::min<double>(tiles_k, 4.0 * ((quads + cs - 1) / cs));
           const double kb = 16.0 + (pair ? 0.5 : 1.0) * bn / 8;
-          double each = pair ? 0.33 : 0.25;
-          if (kb / 130.0 > each) each = kb / 130.0;
-          if (active * kb / 15500.0 > each) each = active * kb / 15500.0;
-          // an epilogue of single columns or of rows that TMA does not store is seen behind the products
-          const double over = cs > 1 ? 5.0 + bn / 64.0 : swap || !rows16 ? 2.5 + 0.03 * bn * rounds : 2.5;
+          const double each = std::max({pair ? 0.30 : 0.18, kb / 128.0, active * kb / 14000.0});
+          // what is seen before and behind the products; pairs begin and end together
+          const double over = cs > 1 ? 4.8 + 0.03 * bn : 3.3 + (pair ? 3.4 : 0.0) + (swap ? 0.015 : !rows16 ? 0.006 : pair && p->out_fp32 ? 0.005 : 0.001) * bn * rounds;
           const double time = rounds * kt * each + over;
           if (time < least * 0.99) { least = time; best = {swap, bn, cs, pair}; }
         }
@@ -649,7 +678,7 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
     d.tma_store = 0;
   if (pair && !d.tma_store) return (int)cudaErrorInvalidValue;
   if (!d.tma_store) tc = ta;   // unused by the kernel
-  d.slabs = d.tma_store ? (pair ? 2 : d.bn > (p->out_fp32 ? 32 : 64) ? 4 : 2) : 0;
+  d.slabs = d.tma_store ? (pair ? 2 : d.bn > (p->out_fp32 ? 32 : 64) ? 4 : 2) : plan.cluster == 1 && !plan.swap ? 2 : 0;
   const int stage = A_BYTES + (pair ? d.bn / 2 : d.bn) * BK + SCALE_BYTES;
   d.stages = (224 * 1024 - d.slabs * SLAB_BYTES) / stage;
   if (d.stages > MAX_STAGES) d.stages = MAX_STAGES;
