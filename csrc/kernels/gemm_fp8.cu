@@ -552,14 +552,15 @@ bool width_ok(int bn, long long N) { return bn == 64 || bn == 128 || bn == 192 |
 // Whether an atom's worth of every slice is there
 bool slices_ok(int quads, int cluster) { return (long long)((quads + cluster - 1) / cluster) * (cluster - 1) < quads; }
 
-// The cut with the shortest expected time.  A k tile takes a round trip through the ring of stages (0.18 us, pairs 0.30) or what L2
-// needs for its operands (128 KB/us an SM, 14 MB/us in all): seldom the tensor pipe's time (0.2 us for 128 x 192), so wide tiles and
-// pairs win where there are enough of them, and slices of K where there are not.  In a captured chain, us (width / CTAs that share K,
-// p: pairs): 8192 x 16384, K = 4096 407 (192p), 482 (192/1), 588 (128/1); 1024 x 9216, K = 4096 32.2 (192p), 39.1, 39.2; 2048 x 4096,
-// K = 4096 31.8 (192p), 34.9, 36.6; 512 x 4096, K = 4096 11.8 (128/1), 13.9 (192p), 14.0; 256 x 4096, K = 9216 17.8 (128/2), 19.6
-// (64/1), 20.0 (128/1); with B's rows on the tall side 7 x 4096, K = 4096 7 (32/4), 8.3 (32/2), 10.3 (32/1).
-// With few k tiles what is around them counts: 449 x 6912, K = 256 5.0 (192/1), 6.8 (192p); 3913 x 1408 in fp32 7.6, 11.6; 6313 x 4352,
-// K = 512 in fp32 29.0, 37.3.  Over 110 sizes of 1 to 9216 the chosen cut takes 1.5 % longer than the best one.
+// The cut with the shortest expected time.  A k tile takes a round trip through the ring of stages (0.22 us, pairs 0.29) or what L2
+// needs for its operands (128 KB/us an SM, 14.5 MB/us in all, the same line for 300 readers a us): seldom the tensor pipe's time (0.2 us
+// for 128 x 192), so wide tiles and pairs win where there are enough of them, and slices of K where there are not.  A tile's stores run
+// beside the next one's products.  The constants are fitted to 550 sizes of 1 to 9216; over others the chosen cut takes 0.8 % longer
+// than the best one.  In a captured chain, us (width / CTAs that share K, p: pairs, t: B's rows on the tall side): 8192 x 16384, K =
+// 4096 407 (192p), 482 (192/1), 588 (128/1); 1024 x 9216, K = 4096 32.2 (192p), 39.1, 39.2; 2048 x 4096, K = 4096 31.8 (192p), 34.9,
+// 36.6; 512 x 4096, K = 4096 11.8 (128/1), 13.9 (192p), 14.0; 256 x 4096, K = 9216 17.8 (128/2), 19.6 (64/1), 20.0 (128/1); 7 x 4096,
+// K = 4096 7 (32/4t), 8.3 (32/2t), 10.3 (32/1t); 4 x 6400, K = 2688 8.3 (128/1), 12.0 (64/1: 100 CTAs read the same lines of A); 449 x
+// 6912, K = 256 5.0 (192/1), 6.8 (192p); 3913 x 1408, K = 256 in fp32 7.6, 11.6; 7451 x 8960, K = 256 30.2, 55.6 (its stores).
 Plan choose(const GeepsGemmFp8* p, int sms) {
   const int quads = (int)((p->K + 511) / 512), tiles_k = (int)((p->K + BK - 1) / BK);
   const bool rows16 = ((uintptr_t)p->C & 15) == 0 && p->ldc * (p->out_fp32 ? 4 : 2) % 16 == 0;
@@ -582,10 +583,12 @@ Plan choose(const GeepsGemmFp8* p, int sms) {
           if (cs > 1 && rounds > 1) continue;
           const double active = (double)(tiles * size < slots ? tiles * size : slots), kt = std::min<double>(tiles_k, 4.0 * ((quads + cs - 1) / cs));
           const double kb = 16.0 + (pair ? 0.5 : 1.0) * bn / 8;
-          const double each = std::max({pair ? 0.30 : 0.18, kb / 128.0, active * kb / 14000.0});
-          // what is seen before and behind the products; pairs begin and end together
-          const double over = cs > 1 ? 4.8 + 0.03 * bn : 3.3 + (pair ? 3.4 : 0.0) + (swap ? 0.015 : !rows16 ? 0.006 : pair && p->out_fp32 ? 0.005 : 0.001) * bn * rounds;
-          const double time = rounds * kt * each + over;
+          const double m_tiles = (double)((M + tall - 1) / tall), at_once = active / size, readers = std::max(std::min(m_tiles, at_once), at_once / m_tiles);
+          const double products = kt * std::max({pair ? 0.29 : 0.22, kb / 128.0, active * kb / 14500.0, 0.0033 * readers});
+          // the stores of a tile, beside the next one's products
+          const double store = (0.53 + 0.005 * bn) * (p->out_fp32 ? 1.25 : 1.0) * (pair ? 1.8 : 1.0) * (swap ? 2.1 : rows16 ? 1.0 : 1.6);
+          const double time = cs > 1 ? products + 5.0 + 0.0275 * bn + (swap ? 0.6 : 0.0)
+                                     : 2.3 + (pair ? 1.1 : 0.0) + products + store + (rounds - 1) * std::max(products, store);
           if (time < least * 0.99) { least = time; best = {swap, bn, cs, pair}; }
         }
       }
