@@ -53,6 +53,33 @@ def test_casts_are_the_definition_bit_for_bit(rows, cols, dtype, tile):
     assert torch.equal(t2.q.view(torch.uint8), t.q.view(torch.uint8)) and torch.equal(t2.exponents(), t.exponents())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("pitch", [300, 304])
+def test_scales_change_where_the_definition_says(dtype, tile, pitch):
+    """Largest magnitudes at and around 1.75 x 2^k (448 = 1.75 x 2^8), powers of two, the largest finite number, and rows whose other
+    values end in every bit."""
+    from geeps_b200.ops import functional as F
+    edge = torch.tensor([1.75, 1.0, 2.0, 1.75 * 2.0 ** 100, 1.75 * 2.0 ** -118, 448.0, 2.0 ** -126, 1.5 * 2.0 ** 127], device=DEV)
+    tops = torch.cat([edge, torch.nextafter(edge, edge * 2), torch.nextafter(edge, edge * 0), torch.tensor([torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal], device=DEV)])
+    for shift in range(tops.numel()):
+        n = 256 if not tile else 128
+        top = (tops[shift:shift + 1] if tile else tops.roll(shift)[torch.arange(n, device=DEV) % tops.numel()]).view(-1, 1)
+        x = (top * (2 * torch.rand(n, pitch, device=DEV) - 1)).to(dtype)[:, :300]
+        x[:, 7::128] = top.to(dtype)
+        a, t = F.Fp8Matrix(n, 300, DEV), F.Fp8Matrix(300, n, DEV)
+        F.quantize_fp8(x, a, transposed=t, tile=tile)
+        same(a, x, tile)
+        same(t, x.T, tile)
+        same(F.quantize_fp8(x, tile=tile), x, tile)
+        if not tile:
+            y = x.T.contiguous()                # the tops by columns
+            F.quantize_fp8(y, t, transposed=a)
+            same(a, x)
+            same(t, y)
+            break
+
+
 def plain(a, b):
     return values(a.q.double(), a.exponents().int() - 127) @ values(b.q.double(), b.exponents().int() - 127).T
 
