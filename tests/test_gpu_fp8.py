@@ -180,6 +180,36 @@ def test_small_and_odd_sizes(M, N, K):
     F.matmul_fp8(F.quantize_fp8(torch.empty(0, K, device=DEV)), b, empty)
 
 
+def test_offsets_that_pass_32_bits():
+    """A matrix of more than 2^31 values, cast both ways, and a product of as many: what lies last is that of the last rows alone."""
+    from geeps_b200.ops import functional as F
+    rows, cols, last = 65664, 32832, 128
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(rows, cols, dtype=torch.bfloat16, device=DEV, generator=gen)
+    q, t = F.Fp8Matrix(rows, cols, DEV), F.Fp8Matrix(cols, rows, DEV)
+    end = x[-last:].clone()
+    want, want_t = F.Fp8Matrix(last, cols, DEV), F.Fp8Matrix(cols, last, DEV)
+    F.quantize_fp8(end, want, transposed=want_t)
+    for both in (False, True):
+        q.q.view(torch.uint8).zero_()
+        F.quantize_fp8(x, q, transposed=t if both else None)
+        assert torch.equal(q.q[-last:].view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(q.exponents()[-last:], want.exponents())
+    assert torch.equal(t.q[:, -last:].view(torch.uint8), want_t.q.view(torch.uint8)) and torch.equal(t.exponents()[:, -1:], want_t.exponents())
+    del x, q, t, end, want, want_t
+    a, b = F.quantize_fp8(torch.randn(rows, 200, device=DEV, generator=gen)), F.quantize_fp8(torch.randn(cols, 200, device=DEV, generator=gen))
+    for n in (cols, cols - 1):                  # rows that TMA stores, and rows that it does not
+        if n < cols:
+            b = F.quantize_fp8(b.dequantize()[:n])
+        out = torch.empty(rows, n, dtype=torch.bfloat16, device=DEV)
+        F.matmul_fp8(a, b, out)
+        e = F.Fp8Matrix(last, 200, DEV)
+        F.quantize_fp8(a.dequantize()[-last:], e)
+        ref = plain(e, b)
+        mags, half = tolerance(e, b, out, 200)
+        assert ((out[-last:].double() - ref).abs() <= mags + half * (ref.abs() + mags)).all()
+        del out
+
+
 def test_gradients_of_a_layer():
     """Forward and both gradients as a layer forms them, each operand cast once: against the products of what the casts stand for."""
     from geeps_b200.ops import functional as F

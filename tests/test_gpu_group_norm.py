@@ -239,6 +239,26 @@ def test_repeats_bit_for_bit_on_other_streams_and_in_two_graphs_at_once():
         assert all(torch.equal(o[k], first[k]) for k in first)
 
 
+def test_offsets_that_pass_32_bits():
+    """More than 2^31 values: the last image is normalised as by itself."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = 33, 1 << 20, 64, 8
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x = torch.randn(images * pixels, c, dtype=BF, device=DEV, generator=gen)
+    w, b = 1 + 0.3 * torch.randn(c, device=DEV, generator=gen), 0.3 * torch.randn(c, device=DEV, generator=gen)
+    y, stats = torch.empty_like(x), torch.empty(images, groups, 2, device=DEV)
+    F.group_norm_forward(x, y, images, F.GroupNorm(groups, w, b, stats, EPS, "relu"))
+    last = x[-pixels:]
+    check_forward(last, y[-pixels:], stats[-1:], statistics(last, 1, groups), w, b, 1, groups, "relu")
+    del y
+    dx, alone = torch.empty_like(x), torch.empty_like(last)
+    F.group_norm_backward(x, x, dx, images, F.GroupNorm(groups, w, b, stats, EPS, "relu"))
+    F.group_norm_backward(last, last, alone, 1, F.GroupNorm(groups, w, b, stats[-1:].clone(), EPS, "relu"))
+    # two cuts of the same sums: 2^20 terms of random signs in parts of 2^12 at the most, whose means are off by 2^-12 of a term's size at
+    # the worst; then a rounding on either side
+    assert ((dx[-pixels:].double() - alone.double()).abs() <= 2.0 ** -7 * alone.double().abs() + 2.0 ** -10).all()
+
+
 def test_gradients_match_differences():
     """Of the sum of dy y, in fp32: a central difference with step h is off by h^2 of a third derivative and 2^-22 / h of the sum."""
     from geeps_b200.ops import functional as F
