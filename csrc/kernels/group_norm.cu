@@ -330,12 +330,14 @@ group_forward_kernel(const __grid_constant__ Dev d) {
       for (int k = 0; k < mine;) {
         const int end = min(mine, k + kPart), count = end - k;
         float2 s[H], q[H], base[H];
-        x.get(k).get(base);
+        auto begin = [&](const Vec<XT, W>& in) {
+          in.get(base);
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-          s[i] = q[i] = both(0.f);
-          base[i] = make_float2(-base[i].x, -base[i].y);
-        }
+          for (int i = 0; i < H; ++i) {
+            s[i] = q[i] = both(0.f);
+            base[i] = make_float2(-base[i].x, -base[i].y);
+          }
+        };
         auto add = [&](const Vec<XT, W>& in) {
           float2 f[H];
           in.get(f);
@@ -346,16 +348,29 @@ group_forward_kernel(const __grid_constant__ Dev d) {
             q[i] = fma2(e, e, q[i]);
           }
         };
-        int j = k + 1;
-        for (; j + FLIGHT <= end; j += FLIGHT) {
-          Vec<XT, W> in[FLIGHT];
+        if constexpr (KEEP) {
+          begin(x.get(k));
+          int j = k + 1;
+          for (; j + FLIGHT <= end; j += FLIGHT) {
+            Vec<XT, W> in[FLIGHT];
 #pragma unroll
-          for (int u = 0; u < FLIGHT; ++u) in[u] = x.get(j + u);
+            for (int u = 0; u < FLIGHT; ++u) in[u] = x.get(j + u);
 #pragma unroll
-          for (int u = 0; u < FLIGHT; ++u) add(in[u]);
-        }
+            for (int u = 0; u < FLIGHT; ++u) add(in[u]);
+          }
 #pragma unroll 1
-        for (; j < end; ++j) add(x.get(j));
+          for (; j < end; ++j) add(x.get(j));
+        } else {             // no load waits by itself: the first row, which adds nothing about itself, and the last ones come with others
+          for (int j = k; j < end; j += FLIGHT) {
+            Vec<XT, W> in[FLIGHT];
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u) in[u] = x.get(min(j + u, end - 1));
+            if (j == k) begin(in[0]);
+#pragma unroll
+            for (int u = 0; u < FLIGHT; ++u)
+              if (j + u < end) add(in[u]);
+          }
+        }
         const float inv = __frcp_rn((float)count), share = n ? (float)count / (n + count) : 1.f, weight = n * share;
 #pragma unroll
         for (int i = 0; i < H; ++i) {
@@ -491,8 +506,17 @@ group_forward_kernel(const __grid_constant__ Dev d) {
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) finish(in[u]);
     }
+    if constexpr (KEEP) {
 #pragma unroll 1
-    for (; k < mine; ++k) finish(x.get(k));
+      for (; k < mine; ++k) finish(x.get(k));
+    } else if (k < mine) {
+      Vec<XT, W> in[FLIGHT];
+#pragma unroll
+      for (int u = 0; u < FLIGHT - 1; ++u) in[u] = x.get(min(k + u, mine - 1));
+#pragma unroll
+      for (int u = 0; u < FLIGHT - 1; ++u)
+        if (k + u < mine) finish(in[u]);
+    }
   };
   auto by_act = [&](int v) __attribute__((always_inline)) {
     if (d.act == 0) pass(v, std::integral_constant<int, 0>());
@@ -561,8 +585,20 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) f(k + u, xi[u], di[u]);
     }
+    if constexpr (KEEP) {
 #pragma unroll 1
-    for (; k < mine; ++k) f(k, x.get(k), dy.get(k));
+      for (; k < mine; ++k) f(k, x.get(k), dy.get(k));
+    } else if (k + 1 == mine) {
+      f(k, x.get(k), dy.get(k));
+    } else if (k < mine) {
+      Vec<XT, W> xi[FLIGHT];
+      Vec<YT, W> di[FLIGHT];
+#pragma unroll
+      for (int u = 0; u < FLIGHT - 1; ++u) { xi[u] = x.get(min(k + u, mine - 1)); di[u] = dy.get(min(k + u, mine - 1)); }
+#pragma unroll
+      for (int u = 0; u < FLIGHT - 1; ++u)
+        if (k + u < mine) f(k + u, xi[u], di[u]);
+    }
   };
   // z, rounded after each operation: not in pairs, which are contracted to fused multiply-adds
   auto border = [&](const float2& n, const float2& w, const float2& b) {
