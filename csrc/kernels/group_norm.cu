@@ -12,8 +12,8 @@
 // for the machine as items are cut over many CTAs in two launches (sums, then the rest), which meet in a workspace.
 // Forward reads x and writes y, backward reads x and dy and writes dx.  A block's life is a chain of waits (its pixels, the column sums,
 // the group sums, the stores: some 6 us), of which as many run side by side as shared memory holds slices: 0.45 to 0.55 of the copy
-// rate (32 x 3136 x 192 forward 26 us, 256 x 196 x 576 backward 56).  Neither taking turns at the start (55 to 57), nor four groups of
-// copies with sums between them, nor reading again from L2 instead of keeping (121) does better.
+// rate (32 x 3136 x 192 forward 26 us, 256 x 196 x 576 backward 52.6).  Neither taking turns at the start (55 to 57 of 56 at the time), nor
+// four groups of copies with sums between them, nor reading again from L2 instead of keeping (121) does better.
 //
 // Variance: values less the first of every 32 of a thread's pixels are added and squared, and such parts meet as count, mean and
 // sum of squared differences, so a mean far from zero costs nothing (a part's error is at most 32 x 2^-24 of its variance).
@@ -36,12 +36,15 @@ namespace {
 
 constexpr int kMostParts = 256;            // chunks of an image in two launches
 constexpr int kPart = 32;                  // pixels of a part of the variance
-// One launch with the pixels kept in shared memory, or read again; or two launches
-enum Phase { KEPT = 0, TWICE = 1, SUMS = 2, APPLY = 3 };
+// One launch with the pixels kept in shared memory, or read again; or two launches; or kept, the first of a thread in registers
+enum Phase { KEPT = 0, TWICE = 1, SUMS = 2, APPLY = 3, MIXED = 4 };
+// Backward, bf16: pixels of a thread in registers, where that lets another block onto an SM (256 x 196 x 576 56.4 -> 52.6 us, 64 x 196 x 1024
+// 29.1 -> 24.9).  Four spill (112 bytes, three 64).
+constexpr int kInRegisters = 3;
 // Threads of a block.  Where a slice's pixels stay in the block, 128: more blocks then share an SM, each in another step.  With 256, us,
 // bf16: 512 x 64 x 96 forward 7.1 -> 11.4, 256 x 196 x 576 backward 56.5 -> 75.8, 8 x 12544 x 128 18.2 -> 31.1; only some forward passes of
 // many channels gain (256 x 196 x 576 35.2 -> 31.2).
-constexpr int threads_of(int phase) { return phase == KEPT || phase == TWICE ? 128 : 256; }
+constexpr int threads_of(int phase) { return phase == SUMS || phase == APPLY ? 256 : 128; }
 
 // n / d for n below 2^31 by a multiplication (Granlund and Montgomery)
 struct Divide {
@@ -532,11 +535,11 @@ group_forward_kernel(const __grid_constant__ Dev d) {
 }
 
 template <typename XT, typename YT, bool VEC, int PHASE>
-__global__ void __launch_bounds__(threads_of(PHASE), PHASE == KEPT && sizeof(XT) == 2 ? 5 : PHASE == KEPT || PHASE == TWICE ? 4 : 2)
+__global__ void __launch_bounds__(threads_of(PHASE), PHASE == KEPT && sizeof(XT) == 2 ? 5 : threads_of(PHASE) == 128 ? 4 : 2)
 group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
-  constexpr int W = VEC ? 8 : 1, H = (W + 1) / 2, FLIGHT = PHASE == KEPT ? 2 : W == 1 ? 8 : sizeof(XT) > 2 ? 2 : 4;
-  constexpr int kThreads = threads_of(PHASE);
-  constexpr bool KEEP = PHASE == KEPT, ONE = PHASE == KEPT || PHASE == TWICE;
+  constexpr bool KEEP = PHASE == KEPT || PHASE == MIXED, ONE = KEEP || PHASE == TWICE;
+  constexpr int W = VEC ? 8 : 1, H = (W + 1) / 2, FLIGHT = KEEP ? 2 : W == 1 ? 8 : sizeof(XT) > 2 ? 2 : 4;
+  constexpr int kThreads = threads_of(PHASE), REG = PHASE == MIXED ? kInRegisters : 0;
   extern __shared__ __align__(16) uint8_t smem[];
   const Place<W> p(d);
   const int cg = d.by_cg.d, gs = d.slice / cg, chunks = d.by_chunks.d;
@@ -553,11 +556,16 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
   Rows<XT, W, KEEP> x = {(const XT*)d.x + x_at, (long long)d.R * d.ldx, {tc05::smem_u32(entry) + (uint32_t)d.entries + threadIdx.x * 16}};
   Rows<YT, W, KEEP> dy = {(const YT*)d.dy + dy_at, (long long)d.R * d.lddy, {x.kept.base + (uint32_t)(d.keep * Kept<XT>::kBytes)}};
   geeps_pdl_enter();
+  Vec<XT, W> xr[REG + 1];                // (an array has one element at least)
+  Vec<YT, W> dr[REG + 1];
   if constexpr (KEEP) {
     const XT* xs = x.at;
     const YT* ds = dy.at;
+#pragma unroll
+    for (int k = 0; k < REG; ++k, xs += x.step, ds += dy.step)
+      if (k < mine) { xr[k].load(xs); dr[k].load(ds); }
 #pragma unroll 4
-    for (int k = 0; k < mine; ++k, xs += x.step, ds += dy.step) {
+    for (int k = 0; k < mine - REG; ++k, xs += x.step, ds += dy.step) {
       x.kept.fetch(k, xs);
       dy.kept.fetch(k, ds);
     }
@@ -574,30 +582,43 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
     for (int c = threadIdx.x; c < d.slice; c += kThreads) constant(c, mean_of[c], rstd_of[c], w_of[c], b_of[c]);
     __syncthreads();
   }
-  // f(k, x, dy) for all rows of a column, FLIGHT of them in flight
-  auto rows = [&](auto f) {
+  // f(x, dy) for all rows of a column, FLIGHT of them in flight.  keep: dy as f leaves it is kept for the next time
+  auto rows = [&](auto f, auto keep) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < REG; ++k)
+      if (k < mine) {
+        Vec<YT, W> d = dr[k];
+        f(xr[k], d);
+        if (decltype(keep)::value) dr[k] = d;
+      }
+    const int end = mine - REG;
     int k = 0;
-    for (; k + FLIGHT <= mine; k += FLIGHT) {
+    auto one = [&](int k, const Vec<XT, W>& xi, Vec<YT, W>& di) {
+      f(xi, di);
+      if constexpr (KEEP) { if (decltype(keep)::value) dy.kept.put(k, di); }
+    };
+    for (; k + FLIGHT <= end; k += FLIGHT) {
       Vec<XT, W> xi[FLIGHT];
       Vec<YT, W> di[FLIGHT];
 #pragma unroll
       for (int u = 0; u < FLIGHT; ++u) { xi[u] = x.get(k + u); di[u] = dy.get(k + u); }
 #pragma unroll
-      for (int u = 0; u < FLIGHT; ++u) f(k + u, xi[u], di[u]);
+      for (int u = 0; u < FLIGHT; ++u) one(k + u, xi[u], di[u]);
     }
-    if constexpr (KEEP) {
+    if (KEEP || k + 1 == end) {
 #pragma unroll 1
-      for (; k < mine; ++k) f(k, x.get(k), dy.get(k));
-    } else if (k + 1 == mine) {
-      f(k, x.get(k), dy.get(k));
-    } else if (k < mine) {
+      for (; k < end; ++k) {
+        Vec<YT, W> d = dy.get(k);
+        one(k, x.get(k), d);
+      }
+    } else if (k < end) {
       Vec<XT, W> xi[FLIGHT];
       Vec<YT, W> di[FLIGHT];
 #pragma unroll
-      for (int u = 0; u < FLIGHT - 1; ++u) { xi[u] = x.get(min(k + u, mine - 1)); di[u] = dy.get(min(k + u, mine - 1)); }
+      for (int u = 0; u < FLIGHT - 1; ++u) { xi[u] = x.get(min(k + u, end - 1)); di[u] = dy.get(min(k + u, end - 1)); }
 #pragma unroll
       for (int u = 0; u < FLIGHT - 1; ++u)
-        if (k + u < mine) f(k + u, xi[u], di[u]);
+        if (k + u < end) one(k + u, xi[u], di[u]);
     }
   };
   // z, rounded after each operation: not in pairs, which are contracted to fused multiply-adds
@@ -619,7 +640,7 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
       }
 #pragma unroll
       for (int i = 0; i < H; ++i) sa[i] = sb[i] = both(0.f);
-      rows([&](int k, const Vec<XT, W>& xi, Vec<YT, W> di) {
+      rows([&](const Vec<XT, W>& xi, Vec<YT, W>& di) {
         float2 dz[H], n[H], z[H];
         xi.get(n);
 #pragma unroll
@@ -627,10 +648,7 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
           n[i] = mul2(add2(n[i], mean[i]), rstd[i]);
           if (ACT) z[i] = border(n[i], w[i], b[i]);
         }
-        if (ACT == 1) {
-          di.mask(z);
-          if constexpr (KEEP) dy.kept.put(k, di);       // for the second pass, which needs no z then
-        }
+        if (ACT == 1) di.mask(z);                        // kept for the second pass, which needs no z then
         di.get(dz);
 #pragma unroll
         for (int i = 0; i < H; ++i) {
@@ -638,7 +656,7 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
           sa[i] = add2(sa[i], dz[i]);
           sb[i] = fma2(dz[i], n[i], sb[i]);
         }
-      });
+      }, std::integral_constant<bool, ACT == 1>());
       float2* to = d.R == 1 ? column + v * W : entry + p.r * d.V + v;
       const int next = d.R == 1 ? 1 : d.R * d.V;
 #pragma unroll
@@ -733,7 +751,7 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
       }
     }
     XT* to = dx;
-    rows([&](int, const Vec<XT, W>& xi, Vec<YT, W> di) {
+    rows([&](const Vec<XT, W>& xi, Vec<YT, W>& di) {
       float2 dz[H], e[H], z[H];
       xi.get(e);
 #pragma unroll
@@ -752,7 +770,7 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
       o.set(dz);
       o.store(to);
       to += ostep;
-    });
+    }, std::false_type());
   };
   auto by_act = [&](int v) __attribute__((always_inline)) {
     if (d.act == 0) pass(v, std::integral_constant<int, 0>());
@@ -789,7 +807,7 @@ group_parameters_kernel(const float2* __restrict__ sums, long long parts, int C,
 }
 
 // ---------------- host side ----------------
-struct Shape { int vec, threads, fused, slice, slices, chunks, rows, keep, blocks, V, R, entries; size_t smem; };
+struct Shape { int vec, threads, in_registers, fused, slice, slices, chunks, rows, keep, blocks, V, R, entries; size_t smem; };
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
@@ -814,7 +832,8 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
   // time that the SMs' room is filled (a CTA's steps follow one another, and CTAs that began together rarely overlap; narrow slices
   // have fewer channels a thread to join), and the bytes that an SM reads (as many are written).  Measured, bf16 forward,
   // slice / CTAs of a cluster: 32 x 784 x 256: 32/1 9.0 us, 64/1 9.1, 32/3 10.8, 64/7 (just over one filling) 13.8, 32/8 21.8;
-  // 64 x 49 x 1024: 128/1 7.4, 512/1 9.1, 128/6 25.8; backward, 256 x 196 x 576: 72/1 56.5, 72/2 65.9, 288/3 88.
+  // 64 x 49 x 1024: 128/1 7.4, 512/1 9.1, 128/6 25.8; backward, 256 x 196 x 576, all pixels in shared memory:
+  // 72/1 56.5, 72/2 65.9, 288/3 88.
   auto cut = [&](Shape& t) {             // what a thread has of a slice
     t.V = t.slice / W;
     t.R = t.V < t.threads ? t.threads / t.V : 1;
@@ -839,15 +858,21 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
     cut(t);
     if (vec && t.V > t.threads) continue;
     for (int k = 1; k <= kMostChunks; ++k) {
-      const int rows = (pixels + k - 1) / k;
-      const size_t smem = fixed_bytes(t, cg, backward) + t.entries + (size_t)((rows + t.R - 1) / t.R) * row_bytes;
-      if (smem > kSmem || (k > 1 && rows < t.R)) continue;
-      const int fit = (int)(228 * 1024 / (smem + 1024)), most = !vec ? 4 : !backward ? 6 : xsize == 2 ? 5 : 4, resident = fit < most ? fit : most;
-      const double ctas = (double)images * t.slices * k, filled = ctas / ((double)sms * resident);
-      const double kb = (double)rows * t.slice * (xsize + (backward ? ysize : 0)) / 1024, join = k > 1 ? 0.5 : 0.0;
-      const double cost = vec ? ceil(filled) * (6.0 + 0.4 * t.slice / t.threads) + ceil(ctas / sms) * (0.15 + kb / (xsize == 2 ? 21.0 : 18.0)) + join
-                              : (filled > 1.0 ? filled : 1.0) * (6.0 + kb / 2.7 + join);
-      if (cost < best) { best = cost; s = t; chunks = k; }
+      const int rows = (pixels + k - 1) / k, keep = (rows + t.R - 1) / t.R;
+      if (k > 1 && rows < t.R) continue;
+      int fewer = 0;                       // blocks an SM without pixels in registers
+      for (int held = 0; held <= (vec && backward && xsize == 2 ? kInRegisters : 0); held += kInRegisters) {
+        const size_t smem = fixed_bytes(t, cg, backward) + t.entries + (size_t)(keep > held ? keep - held : 0) * row_bytes;
+        if (smem > kSmem) continue;
+        const int fit = (int)(228 * 1024 / (smem + 1024)), most = !vec || held ? 4 : !backward ? 6 : xsize == 2 ? 5 : 4, resident = fit < most ? fit : most;
+        if (held && (resident < 3 || resident <= fewer)) continue;
+        fewer = resident;
+        const double ctas = (double)images * t.slices * k, filled = ctas / ((double)sms * resident);
+        const double kb = (double)rows * t.slice * (xsize + (backward ? ysize : 0)) / 1024, join = k > 1 ? 0.5 : 0.0;
+        const double cost = vec ? ceil(filled) * (6.0 + 0.4 * t.slice / t.threads) + ceil(ctas / sms) * (0.15 + kb / (xsize == 2 ? 21.0 : 18.0)) + join
+                                : (filled > 1.0 ? filled : 1.0) * (6.0 + kb / 2.7 + join);
+        if (cost < best) { best = cost; s = t; s.in_registers = held; chunks = k; }
+      }
     }
   }
   // Two launches, at best of one filling of two blocks an SM.  32 x 784 x 256: 9 x 32 = 288 blocks 13.1 us, 12 x 32 = 384 20.5.  Against one
@@ -870,12 +895,13 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
   s.fused = chunks > 0 && best <= twice;
   if (!s.fused) {
     s = u;
+    s.in_registers = 0;
     chunks = cuts;
   }
   const long long items = (long long)images * s.slices;
   s.rows = (pixels + chunks - 1) / chunks;
   s.chunks = s.fused ? chunks : (pixels + s.rows - 1) / s.rows;
-  s.keep = vec && s.fused ? (s.rows + s.R - 1) / s.R : 0;
+  s.keep = vec && s.fused ? std::max(0, (s.rows + s.R - 1) / s.R - s.in_registers) : 0;
   s.smem = fixed_bytes(s, cg, backward) + s.entries + (size_t)s.keep * row_bytes;
   s.blocks = items * s.chunks > 0x7fffffffLL ? 0 : (int)(items * s.chunks);
   return s;
@@ -938,7 +964,10 @@ int run(const GeepsGroupNorm& k, const Shape& s, const Dev& d, bool backward, cu
   // group sums of the chunks (two launches only), then the channels' sums of the images or chunks
   const long long parts = (long long)k.images * (s.fused ? 1 : s.chunks);
   float* channel = want ? k.work + (s.fused ? 0 : parts * k.groups * 2) : nullptr;
-  if (s.fused) {
+  if (s.fused && s.in_registers) {
+    if constexpr (VEC && sizeof(XT) == 2) e = launch<group_backward_kernel<XT, YT, VEC, MIXED>>(s, true, true, st, d, channel);
+    else e = (int)cudaErrorInvalidValue;
+  } else if (s.fused) {
     e = launch<group_backward_kernel<XT, YT, VEC, ONE>>(s, true, true, st, d, channel);
   } else {
     e = launch<group_backward_kernel<XT, YT, VEC, SUMS>>(s, false, true, st, d, channel);
@@ -1039,7 +1068,7 @@ int geeps_group_norm_shape(long long images, long long pixels, int C, int groups
   if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || (vec && C % 8) || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30))
     return (int)cudaErrorInvalidValue;
   const Shape s = choose((int)images, (int)pixels, C, groups, backward, vec, x_fp32 ? 4 : 2, y_fp32 ? 4 : 2);
-  out[0] = s.fused; out[1] = s.slice; out[2] = s.chunks; out[3] = s.rows; out[4] = s.keep; out[5] = s.blocks; out[6] = (int)s.smem; out[7] = s.threads;
+  out[0] = s.fused; out[1] = s.slice; out[2] = s.chunks; out[3] = s.rows; out[4] = s.keep; out[5] = s.blocks; out[6] = (int)s.smem; out[7] = s.threads; out[8] = s.in_registers;
   return 0;
 }
 

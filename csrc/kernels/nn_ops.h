@@ -212,8 +212,8 @@ typedef struct GeepsGroupNorm {
 long long geeps_group_norm_work(long long images, long long pixels, int C, int groups, int backward);
 int geeps_group_norm_forward(const GeepsGroupNorm* p, void* stream);
 int geeps_group_norm_backward(const GeepsGroupNorm* p, void* stream);
-// launch shape (host arithmetic only), eight values: one launch of clusters or two launches, channels of a slice, chunks of an image,
-// pixels of a chunk, pixels that a thread keeps, blocks, bytes of shared memory, threads
+// launch shape (host arithmetic only), nine values: one launch of clusters or two launches, channels of a slice, chunks of an image,
+// pixels of a chunk, pixels that a thread keeps in shared memory, blocks, bytes of shared memory, threads, pixels that a thread keeps in registers
 int geeps_group_norm_shape(long long images, long long pixels, int C, int groups, int backward, int vec, int x_fp32, int y_fp32, int* out);
 
 // ---- clipping of gradients by their global norm (the reference's solver had it in its absent Caffe application) ----

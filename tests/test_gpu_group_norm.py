@@ -10,10 +10,10 @@ BF, F32 = torch.bfloat16, torch.float32
 TYPES = {"bf16": (BF, BF), "mixed": (F32, BF), "fp32": (F32, F32)}
 
 # images, pixels, channels, groups: single values, odd widths, groups across vectors, wide groups, many small images, images cut over
-# many blocks in two launches
+# many blocks in two launches, many images with some pixels in registers (bf16, backward)
 SIZES = [(1, 1, 1, 1), (3, 1, 8, 2), (2, 5, 7, 7), (2, 3, 24, 8), (1, 196, 576, 32), (5, 49, 1003, 17), (4, 64, 96, 32), (3, 100, 256, 1),
          (700, 2, 16, 4), (1, 20000, 32, 4), (2, 3000, 136, 17), (1, 33, 4096, 1), (1, 9, 16384, 1), (2, 7, 16383, 3), (9, 3136, 64, 32),
-         (1, 1, 16384, 16384), (1, 5000, 9, 3)]
+         (1, 1, 16384, 16384), (1, 5000, 9, 3), (460, 196, 72, 4), (500, 190, 72, 4)]
 
 
 def made(images, pixels, c, groups, types, seed, offset=0.0, wider=0):

@@ -16,7 +16,7 @@ A, B, D = 1 << 32, 1 << 36, 1 << 40          # addresses that are never touched:
 
 
 def shape(images, pixels, c, groups, backward, vec, types):
-    out = (C.c_int * 8)()
+    out = (C.c_int * 9)()
     assert L.lib().geeps_group_norm_shape(C.c_longlong(images), C.c_longlong(pixels), c, groups, int(backward), int(vec), *types, out) == 0
     return list(out)
 
@@ -32,17 +32,18 @@ def test_group_norm_shapes_cover_the_pixels_within_the_launch_limits(images, pix
     for backward in (False, True):
         for types in ((0, 0), (1, 0), (1, 1)):
             for vec in ((True, False) if c % 8 == 0 else (False,)):
-                fused, width, chunks, rows, keep, blocks, smem, threads = shape(images, pixels, c, groups, backward, vec, types)
+                fused, width, chunks, rows, keep, blocks, smem, threads, held = shape(images, pixels, c, groups, backward, vec, types)
                 assert c % width == 0 and width % (c // groups) == 0 and (not vec or width % 8 == 0)
                 assert chunks * rows >= pixels and blocks == images * (c // width) * chunks < 1 << 31
                 assert 1 <= chunks <= (8 if fused else 256) and smem <= 227 * 1024
                 columns = width // (8 if vec else 1)
                 if fused and vec:
-                    assert columns <= threads and keep == -(-rows // max(1, threads // columns))
+                    assert columns <= threads and keep == max(0, -(-rows // max(1, threads // columns)) - held) and held in (0, 3)
+                    assert not held or (backward and not types[0] and 3 * (smem + 1024) <= 228 * 1024)
                     # everything kept lies in shared memory
                     assert keep * threads * 16 * ((2 if types[0] else 1) + ((2 if types[1] else 1) if backward else 0)) < smem
                 else:
-                    assert keep == 0
+                    assert keep == 0 and held == 0
                 parts = images * (1 if fused else chunks)
                 assert work(images, pixels, c, groups, backward) >= (0 if fused else parts * groups * 2) + (parts * c * 2 if backward else 0)
 
