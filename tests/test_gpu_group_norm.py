@@ -209,9 +209,10 @@ def test_values_that_are_not_finite_stay_in_their_group():
         assert not dx[pixels:, 8:16].isfinite().any() and dx[~hit].isfinite().all()
 
 
-def test_repeats_bit_for_bit_on_other_streams_and_in_two_graphs_at_once():
+@pytest.mark.parametrize("size", [(5, 400, 96, 32), (460, 196, 72, 4), (2, 20000, 64, 8), (3, 300, 51, 3)], ids=str)
+def test_repeats_bit_for_bit_on_other_streams_and_in_two_graphs_at_once(size):
     from geeps_b200.ops import functional as F
-    images, pixels, c, groups = 5, 400, 96, 32
+    images, pixels, c, groups = size
     x, dy, w, b = made(images, pixels, c, groups, "bf16", 7)
 
     def buffers():
