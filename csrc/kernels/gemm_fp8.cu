@@ -30,13 +30,16 @@ constexpr int A_BYTES = BM * BK;
 constexpr int ATOM = 512;                   // scales of 128 rows x 4 k tiles
 constexpr int SCALE_BYTES = 2048;           // of a stage: one atom of A, up to three of B
 constexpr int MAX_STAGES = 8;
-constexpr int SCALE_SETS = 3;               // sets of scales in TMEM, 16 columns each.  The set that k tiles 4q to 4q + 3 use was
-                                            // read last by k tile 4q - 9; tile 4q is loaded when MAX_STAGES tiles before it are done
+constexpr int SCALE_SETS = 4;               // sets of scales in TMEM, 16 columns each, for four k tiles (the last of a tile: one to four) in turn.
+                                            // A set is written anew when the MMAs that read it have been waited for, in whatever order copies
+                                            // and MMAs run: with three quads or more a tile, any three that follow one another have 4 + 4 + 1 k tiles at
+                                            // least, so the set was read last 10 k tiles ago, and a k tile is loaded when the one MAX_STAGES before it is done;
+                                            // with one or two it was read by a tile before the last, whose accumulator has been handed back
 constexpr int SLAB_BYTES = BM * 128;
 constexpr uint64_t WAIT_BUDGET_NS = 2000000000ull;
 constexpr int groups(bool cl) { return cl ? 1 : 2; }
 constexpr int threads(bool cl) { return 64 + 128 * groups(cl); }
-static_assert(MAX_STAGES <= 4 * SCALE_SETS - 3, "scales in TMEM are overwritten while MMAs may read them");
+static_assert(SCALE_SETS == 4 && MAX_STAGES <= 10, "scales in TMEM are overwritten while MMAs may read them");
 
 struct Dev {
   void* C; const float* bias; int* status;
@@ -596,6 +599,46 @@ Plan choose(const GeepsGemmFp8* p, int sms) {
   return best;
 }
 
+// Bytes of a stage of the ring
+int stage_bytes(const Dev& d, const Plan& plan) { return A_BYTES + (plan.pair ? d.bn / 2 : d.bn) * BK + SCALE_BYTES; }
+// Slabs of the epilogue, and as many stages as fit beside them
+void give_memory(Dev& d, const Plan& plan) {
+  d.slabs = d.tma_store ? (plan.pair ? 2 : d.bn > (d.out_fp32 ? 32 : 64) ? 4 : 2) : plan.cluster == 1 && !plan.swap ? 2 : 0;
+  d.stages = std::min((224 * 1024 - d.slabs * SLAB_BYTES) / stage_bytes(d, plan), MAX_STAGES);
+}
+int ctas(const Dev& d, const Plan& plan, int sms) {
+  const long long tiles = (long long)d.m_tiles * d.n_tiles;
+  return (int)(plan.pair ? std::min(tiles, (long long)sms / 2) * 2 : d.cluster > 1 ? tiles * d.cluster : std::min(tiles, (long long)sms));
+}
+// The cut and all that follows from it without a look at the GPU
+int lay_out(const GeepsGemmFp8* p, Plan& plan, Dev& d) {
+  plan = p->bn ? Plan{p->swap, p->bn, p->cluster < 0 ? 1 : p->cluster, p->cluster < 0} : choose(p, geeps_sm_count());
+  d = Dev{};
+  d.kt = (int)((p->K + BK - 1) / BK);
+  d.quads = (d.kt + 3) / 4;
+  const bool pair = plan.pair != 0;
+  const int size = p->out_fp32 ? 4 : 2;
+  const bool rows16 = ((uintptr_t)p->C & 15) == 0 && p->ldc * size % 16 == 0;       // what TMA stores
+  if (plan.cluster < 1 || plan.cluster > 8 || (plan.cluster & (plan.cluster - 1)) || !slices_ok(d.quads, plan.cluster) ||
+      (pair ? plan.swap || !rows16 || (plan.bn != 64 && plan.bn != 128 && plan.bn != 192) : !width_ok(plan.bn, plan.swap ? p->M : p->N)))
+    return (int)cudaErrorInvalidValue;
+  d.C = p->C; d.bias = p->bias; d.status = p->status;
+  d.swap = plan.swap; d.relu = p->relu; d.out_fp32 = p->out_fp32;
+  d.M = plan.swap ? p->N : p->M; d.N = plan.swap ? p->M : p->N; d.ldc = p->ldc;
+  d.scale_a = plan.swap ? p->scale_b : p->scale_a; d.scale_b = plan.swap ? p->scale_a : p->scale_b;
+  d.tma_store = plan.cluster == 1 && !plan.swap && rows16;
+  d.bn = plan.bn;
+  d.cluster = plan.cluster;
+  d.m_tiles = (int)((d.M + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM));
+  const long long n_tiles = (d.N + d.bn - 1) / d.bn;
+  if (n_tiles * d.m_tiles > 0x3fffffffLL) return (int)cudaErrorInvalidValue;
+  d.n_tiles = (int)n_tiles;
+  d.tmem_cols = 32;
+  while (d.tmem_cols < 2 * d.bn + 16 * SCALE_SETS) d.tmem_cols <<= 1;
+  give_memory(d, plan);
+  return 0;
+}
+
 // Lets a kernel have all shared memory of the current device, once
 template <auto kernel>
 int all_shared() {
@@ -647,45 +690,24 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
                                 {p->scale_a, (p->M + 127) / 128 * quads * 512}, {p->scale_b, (p->N + 127) / 128 * quads * 512},
                                 {p->bias, p->bias ? p->N * 4 : 0}, {p->status, p->status ? 16 : 0}};
   if (ranges_overlap(ranges, 1, 7)) return GEEPS_ERR_NORM_OVERLAP;
-  const int sms = geeps_sm_count();
-  Plan plan = p->bn ? Plan{p->swap, p->bn, p->cluster < 0 ? 1 : p->cluster, p->cluster < 0} : choose(p, sms);
-  Dev d = {};
-  d.kt = (int)((p->K + BK - 1) / BK);
-  d.quads = (d.kt + 3) / 4;
+  Plan plan;
+  Dev d;
+  const int bad = lay_out(p, plan, d);
+  if (bad) return bad;
   const bool pair = plan.pair != 0;
-  const int size = p->out_fp32 ? 4 : 2;
-  const bool rows16 = ((uintptr_t)p->C & 15) == 0 && p->ldc * size % 16 == 0;       // what TMA stores
-  if (plan.cluster < 1 || plan.cluster > 8 || (plan.cluster & (plan.cluster - 1)) || !slices_ok(d.quads, plan.cluster) ||
-      (pair ? plan.swap || !rows16 || (plan.bn != 64 && plan.bn != 128 && plan.bn != 192) : !width_ok(plan.bn, plan.swap ? p->M : p->N)))
-    return (int)cudaErrorInvalidValue;
-  d.C = p->C; d.bias = p->bias; d.status = p->status;
-  d.swap = plan.swap; d.relu = p->relu; d.out_fp32 = p->out_fp32;
-  d.M = plan.swap ? p->N : p->M; d.N = plan.swap ? p->M : p->N; d.ldc = p->ldc;
-  d.scale_a = plan.swap ? p->scale_b : p->scale_a; d.scale_b = plan.swap ? p->scale_a : p->scale_b;
+  const int size = p->out_fp32 ? 4 : 2, sms = geeps_sm_count();
   const void *A = plan.swap ? p->B : p->A, *B = plan.swap ? p->A : p->B;
   const long long lda = plan.swap ? p->ldb : p->lda, ldb = plan.swap ? p->lda : p->ldb;
-  d.tma_store = plan.cluster == 1 && !plan.swap && rows16;
-  d.bn = plan.bn;
-  d.cluster = plan.cluster;
-  d.m_tiles = (int)((d.M + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM));
-  const long long n_tiles = (d.N + d.bn - 1) / d.bn;
-  if (n_tiles * d.m_tiles > 0x3fffffffLL) return (int)cudaErrorInvalidValue;
-  d.n_tiles = (int)n_tiles;
-  d.tmem_cols = 32;
-  while (d.tmem_cols < 2 * d.bn + 16 * SCALE_SETS) d.tmem_cols <<= 1;
   CUtensorMap ta, tb, tc;
   if (!make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, p->K, d.M, lda, BK, BM) || !make_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, p->K, d.N, ldb, BK, pair ? d.bn / 2 : d.bn))
     return (int)cudaErrorInvalidValue;
   if (d.tma_store && !make_map(&tc, p->out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p->C, p->N, p->M,
-                               p->ldc * size, p->out_fp32 ? 32 : 64, BM))
+                               p->ldc * size, p->out_fp32 ? 32 : 64, BM)) {
+    if (pair) return (int)cudaErrorInvalidValue;
     d.tma_store = 0;
-  if (pair && !d.tma_store) return (int)cudaErrorInvalidValue;
+    give_memory(d, plan);
+  }
   if (!d.tma_store) tc = ta;   // unused by the kernel
-  d.slabs = d.tma_store ? (pair ? 2 : d.bn > (p->out_fp32 ? 32 : 64) ? 4 : 2) : plan.cluster == 1 && !plan.swap ? 2 : 0;
-  const int stage = A_BYTES + (pair ? d.bn / 2 : d.bn) * BK + SCALE_BYTES;
-  d.stages = (224 * 1024 - d.slabs * SLAB_BYTES) / stage;
-  if (d.stages > MAX_STAGES) d.stages = MAX_STAGES;
-  const long long tiles = (long long)d.m_tiles * d.n_tiles;
   cudaStream_t st = (cudaStream_t)stream;
   if (pair) {
     const long long rows_a = (d.M + 127) / 128 * d.quads, rows_b = (d.N + 127) / 128 * d.quads;
@@ -695,12 +717,22 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
       return (int)cudaErrorInvalidValue;
     const int e = all_shared<gemm_fp8_pair_kernel>();
     if (e) return e;
-    const size_t smem = (size_t)d.stages * stage + d.slabs * SLAB_BYTES + sizeof(Ctl) + 1024;
-    geeps_launch(gemm_fp8_pair_kernel, (int)(tiles < sms / 2 ? tiles : sms / 2) * 2, threads(false), smem, st, ta, tb, tc, sa, sb, d);
+    const size_t smem = (size_t)d.stages * stage_bytes(d, plan) + d.slabs * SLAB_BYTES + sizeof(Ctl) + 1024;
+    geeps_launch(gemm_fp8_pair_kernel, ctas(d, plan, sms), threads(false), smem, st, ta, tb, tc, sa, sb, d);
     return (int)cudaGetLastError();
   }
-  if (d.cluster > 1) return launch<true>(ta, tb, tc, d, (int)(tiles * d.cluster), st);
-  return launch<false>(ta, tb, tc, d, (int)(tiles < sms ? tiles : sms), st);
+  return d.cluster > 1 ? launch<true>(ta, tb, tc, d, ctas(d, plan, sms), st) : launch<false>(ta, tb, tc, d, ctas(d, plan, sms), st);
+}
+
+int geeps_gemm_fp8_shape(const GeepsGemmFp8* p, int* out) {
+  if (p->M < 1 || p->N < 1 || p->K < 1 || p->M > 0x3fffffffLL || p->N > 0x3fffffffLL || p->K > 0x3fffffffLL) return (int)cudaErrorInvalidValue;
+  Plan plan;
+  Dev d;
+  const int bad = lay_out(p, plan, d);
+  if (bad) return bad;
+  out[0] = d.bn; out[1] = plan.pair ? -2 : d.cluster; out[2] = d.swap; out[3] = ctas(d, plan, geeps_sm_count());
+  out[4] = d.m_tiles * d.n_tiles; out[5] = d.kt; out[6] = d.stages; out[7] = SCALE_SETS; out[8] = d.tmem_cols;
+  return 0;
 }
 
 }  // extern "C"

@@ -176,6 +176,9 @@ typedef struct GeepsGemmFp8 {
   int bn, cluster, swap;       // bn 0: chosen.  Tile width (64, 128, 192, or 32 where one tile is enough); CTAs that share K, or -2 for CTA pairs; B's rows on the 128-row side
 } GeepsGemmFp8;
 int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream);
+// launch shape (host arithmetic only), nine values: tile width, CTAs that share K (-2: CTA pairs), operands swapped, CTAs, tiles, k tiles, stages
+// of the ring, sets of scales in TMEM, columns of TMEM
+int geeps_gemm_fp8_shape(const GeepsGemmFp8* p, int* out);
 int geeps_clear_f32(float* c, long long n, void* stream);           // n zeros
 // C[m][n] = beta * C[m][n] (exactly 0 when beta == 0) over an M x N view with pitch ldc
 int geeps_scale_matrix_f32(float* c, long long M, long long N, long long ldc, float beta, void* stream);

@@ -299,3 +299,22 @@ def test_refusals():
             ("bias", lambda: F.matmul_fp8(a, b, out, bias=torch.zeros(20, device=DEV).bfloat16()))):
         with pytest.raises(ValueError, match=match):
             call()
+
+
+@pytest.mark.parametrize("K", [640, 768, 1100])
+@pytest.mark.parametrize("plan,M,N", [((64, -2, 0), 16384, 256), ((128, -2, 0), 16384, 512), ((64, 1, 0), 16384, 256), ((64, 1, 1), 250, 16384), ((32, 1, 0), 75776, 32)])
+def test_several_tiles_a_cta_with_other_scales_in_every_block(plan, M, N, K):
+    """Three tiles of K and more for a CTA, whose k tiles are no whole quads, so that the sets of scales in TMEM come round inside a tile."""
+    from geeps_b200.ops import functional as F
+    gen = torch.Generator(device=DEV).manual_seed(K + N)
+    blocks = (K + 127) // 128
+
+    def spread(rows):          # a block's size is a power of two of its own
+        e = torch.randint(-6, 7, (rows, blocks), generator=gen, device=DEV).float()
+        return torch.randn(rows, K, generator=gen, device=DEV) * torch.exp2(e).repeat_interleave(128, 1)[:, :K]
+    a, b = F.quantize_fp8(spread(M)), F.quantize_fp8(spread(N))
+    out = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device=DEV)
+    F.matmul_fp8(a, b, out, plan=plan)
+    exact = plain(a, b)
+    sums, half = tolerance(a, b, out, K)
+    assert ((out.double() - exact).abs() <= sums + half * (exact.abs() + sums)).all()

@@ -198,3 +198,52 @@ def test_the_inception_models_with_group_norms():
     assert [norm_groups(c) for c in (1, 3, 24, 80, 96, 160, 576)] == [1, 1, 8, 16, 32, 32, 32]
     with pytest.raises(ValueError, match="norm"):
         inception_bn_small(norm="layer")
+
+
+def fp8_shape(m, n, k, fp32, plan=(0, 0, 0), odd=False):
+    """Tile width, CTAs that share K, operands swapped, CTAs, tiles, k tiles, stages, sets of scales, columns of TMEM."""
+    p, out = L.GemmFp8(), (C.c_int * 9)()
+    p.C, p.M, p.N, p.K, p.out_fp32 = D, m, n, k, int(fp32)
+    p.ldc = n + 1 if odd else (n + 7) // 8 * 8
+    p.bn, p.cluster, p.swap = plan
+    assert L.lib().geeps_gemm_fp8_shape(C.byref(p), out) == 0, (m, n, k, plan)
+    return list(out)
+
+
+def read_while_overwritten(m, n, k, fp32, plan=(0, 0, 0), odd=False):
+    """Follows the products of a CTA in the order in which they are issued.  The k tile at place i of that order is issued when its stage
+    has arrived, so the one at i - stages has been waited for; a tile's first when the tile before the last has left its accumulator.
+    Places at which a set of scales is written that a k tile not yet waited for reads."""
+    bn, cluster, swap, ctas, tiles, kt, stages, sets, columns = fp8_shape(m, n, k, fp32, plan, odd)
+    assert 2 * bn + 16 * sets <= columns <= 512 and 2 <= stages
+    if cluster > 1:                      # a slice of one tile, whole quads in all but the last one
+        kt, count = min(kt, -(-((kt + 3) // 4) // cluster) * 4), 1
+    else:
+        count = -(-tiles // (ctas // 2 if cluster < 0 else ctas))
+    reader, ends, bad, i, at = [-1] * sets, [], [], 0, 0
+    for t in range(min(count, 12)):      # by then the pattern has come round
+        for j in range(kt):
+            if j % 4 == 0:
+                done = max(i - stages, ends[t - 2] if t >= 2 else -1)
+                if reader[at] > done:
+                    bad.append((t, j, i - reader[at]))
+                now, at = at, (at + 1) % sets
+            reader[now] = i
+            i += 1
+        ends.append(i - 1)
+    return bad
+
+
+@pytest.mark.parametrize("kt", list(range(1, 20)) + [37, 38, 72])
+def test_fp8_scales_are_not_overwritten_before_the_products_that_read_them_are_done(kt):
+    k = kt * 128 - 5
+    assert fp8_shape(128 * 148 * 6, 32, k, False, (32, 1, 0))[4:6] == [888, kt]          # six tiles a CTA
+    for fp32 in (False, True):
+        for bn in (64, 128, 192):
+            for plan, odd in (((bn, 1, 0), False), ((bn, 1, 0), True), ((bn, 1, 1), False), ((bn, -2, 0), False)):
+                assert not read_while_overwritten(128 * 120, 64 * 150, k, fp32, plan, odd), (plan, fp32, odd)
+        assert not read_while_overwritten(128 * 1500, 32, k, fp32, (32, 1, 0)) and not read_while_overwritten(32, 128 * 1500, k, fp32, (32, 1, 1))
+        for m, n in ((16384, 256), (32768, 32), (32768, 64), (4096, 1000), (200, 60000)):      # as the sizes choose
+            assert not read_while_overwritten(m, n, k, fp32) and not read_while_overwritten(m, n, k, fp32, odd=True)
+    if kt in (16, 37, 38, 72):           # where four slices of whole quads are there
+        assert not read_while_overwritten(100, 300, k, False, (64, 4, 0))
