@@ -35,6 +35,7 @@ typedef __nv_bfloat16 bf16;
 namespace {
 
 constexpr int kMostParts = 256;            // chunks of an image in two launches
+constexpr int kMostChannels = 16384;       // for which a slice of a single group fits in shared memory, both ways
 constexpr int kPart = 32;                  // pixels of a part of the variance
 // One launch with the pixels kept in shared memory, or read again; or two launches; or kept, the first of a thread in registers
 enum Phase { KEPT = 0, TWICE = 1, SUMS = 2, APPLY = 3, MIXED = 4 };
@@ -881,12 +882,12 @@ Shape plan(int images, int pixels, int C, int groups, bool backward, bool vec, i
   int n = 1;
   while (unit * n < C && (unit * n < 64 || C / unit % n)) ++n;
   u.threads = threads_of(SUMS);
-  for (;; --n) {                             // down to a width that fits (one group does)
+  for (;; --n) {                             // down to a width that fits (one group does, of kMostChannels channels too)
     if (C / unit % n) continue;
     u.slice = unit * n;
     u.slices = C / u.slice;
     cut(u);
-    if (fixed_bytes(u, cg, backward) + u.entries <= kSmem) break;
+    if (n == 1 || fixed_bytes(u, cg, backward) + u.entries <= kSmem) break;
   }
   const long long parts = (long long)images * u.slices, most = (pixels + u.R - 1) / u.R;
   const int cuts = (int)std::max(1LL, std::min({2LL * sms / parts, most, (long long)kMostParts}));
@@ -986,7 +987,7 @@ bool vectors(const GeepsGroupNorm& k, bool backward) {
 
 int check(const GeepsGroupNorm* k, bool backward) {
   if (!k || k->images < 0 || k->pixels < 0 || (k->y_fp32 && !k->x_fp32) || !(k->eps >= 0.f) || k->act < 0 || k->act > 2) return (int)cudaErrorInvalidValue;
-  if (k->C < 1 || k->C > 16384) return GEEPS_ERR_NORM_CHANNELS;
+  if (k->C < 1 || k->C > kMostChannels) return GEEPS_ERR_NORM_CHANNELS;
   if (k->groups < 1 || k->C % k->groups) return GEEPS_ERR_GROUPS;
   if (k->images > (1LL << 30) || k->pixels > (1LL << 30) || k->images * k->pixels > (1LL << 30)) return (int)cudaErrorInvalidValue;
   const long long rows = k->images * k->pixels;
@@ -1047,7 +1048,8 @@ int call(const GeepsGroupNorm* k, bool backward, void* stream) {
 extern "C" {
 
 long long geeps_group_norm_work(long long images, long long pixels, int C, int groups, int backward) {
-  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30)) return 0;
+  if (images < 1 || pixels < 1 || C < 1 || C > kMostChannels || groups < 1 || C % groups || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30))
+    return 0;                              // the call itself says why
   // of two launches for vectors or single values, whichever the addresses will allow, of any type: the chunks' group sums; backward
   // also the channels' sums of the chunks or images
   long long most = 0;
@@ -1065,7 +1067,8 @@ int geeps_group_norm_forward(const GeepsGroupNorm* p, void* stream) { return cal
 int geeps_group_norm_backward(const GeepsGroupNorm* p, void* stream) { return call(p, true, stream); }
 
 int geeps_group_norm_shape(long long images, long long pixels, int C, int groups, int backward, int vec, int x_fp32, int y_fp32, int* out) {
-  if (images < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || (vec && C % 8) || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30))
+  if (C < 1 || C > kMostChannels) return GEEPS_ERR_NORM_CHANNELS;
+  if (images < 1 || pixels < 1 || groups < 1 || C % groups || (vec && C % 8) || images > (1LL << 30) || pixels > (1LL << 30) || images * pixels > (1LL << 30))
     return (int)cudaErrorInvalidValue;
   const Shape s = choose((int)images, (int)pixels, C, groups, backward, vec, x_fp32 ? 4 : 2, y_fp32 ? 4 : 2);
   out[0] = s.fused; out[1] = s.slice; out[2] = s.chunks; out[3] = s.rows; out[4] = s.keep; out[5] = s.blocks; out[6] = (int)s.smem; out[7] = s.threads; out[8] = s.in_registers;

@@ -346,3 +346,14 @@ def test_refusals():
             ("on cpu", lambda: F.group_norm_forward(x, x.cpu(), 3, ok))):
         with pytest.raises((ValueError, RuntimeError), match=match):
             call()
+
+
+@pytest.mark.parametrize("c", [16385, 25600, 40000])
+def test_too_many_channels_are_refused(c):
+    from geeps_b200.ops import functional as F
+    x = torch.zeros(4, c, dtype=BF, device=DEV)
+    stats = torch.zeros(2, 1, 2, device=DEV)
+    for call in (lambda: F.group_norm_forward(x, torch.empty_like(x), 2, F.GroupNorm(1)),
+                 lambda: F.group_norm_backward(x, x.clone(), torch.empty_like(x), 2, F.GroupNorm(1, stats=stats))):
+        with pytest.raises(ValueError, match="16384"):
+            call()

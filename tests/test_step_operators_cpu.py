@@ -1,7 +1,10 @@
 """Host side of group norm, AdamW steps and 8-bit products: launch shapes, workspaces and refusals, which need no GPU."""
 import copy
 import ctypes as C
+import os
 import pickle
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -247,3 +250,23 @@ def test_fp8_scales_are_not_overwritten_before_the_products_that_read_them_are_d
             assert not read_while_overwritten(m, n, k, fp32) and not read_while_overwritten(m, n, k, fp32, odd=True)
     if kt in (16, 37, 38, 72):           # where four slices of whole quads are there
         assert not read_while_overwritten(100, 300, k, False, (64, 4, 0))
+
+
+def test_group_norms_of_too_many_channels_are_refused_before_a_launch_shape_is_sought():
+    """In a process of its own: what went wrong here was a division by zero, which ends the process."""
+    code = """
+import ctypes as C
+from geeps_b200.ops import _lib as L
+from geeps_b200.ops import functional as F
+out = (C.c_int * 9)()
+for c in (16385, 16392, 25600, 32768, 40000, 1 << 30):
+    for groups in (1, c):
+        for backward in (0, 1):
+            assert F.group_norm_work(4, 50, c, groups, bool(backward)) == 0, (c, groups, backward)
+            for vec in ((0, 1) if c % 8 == 0 else (0,)):
+                assert L.lib().geeps_group_norm_shape(C.c_longlong(4), C.c_longlong(50), c, groups, backward, vec, 0, 0, out) == -10, (c, groups, backward, vec)
+assert L.lib().geeps_group_norm_shape(C.c_longlong(4), C.c_longlong(50), 16384, 1, 1, 1, 0, 0, out) == 0 and F.group_norm_work(4, 50, 16384, 1, True) > 0
+print("through")
+"""
+    got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=300)
+    assert got.returncode == 0 and got.stdout.strip() == "through", (got.returncode, got.stderr[-500:])
