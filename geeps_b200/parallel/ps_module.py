@@ -58,9 +58,11 @@ class _AdamW:
         self.state, self._lists, self._resumed = None, {}, None
 
     def save(self, directory: str, rank: int) -> None:
-        if self.state is not None:
+        """Nothing before the first step; after a resume what it brought back."""
+        kept = self._resumed if self.state is None else {k: getattr(self.state, k) for k in self._KEPT}
+        if kept is not None:
             os.makedirs(directory, exist_ok=True)
-            torch.save({k: getattr(self.state, k) for k in self._KEPT}, os.path.join(directory, f"adamw.{rank}"))
+            torch.save(kept, os.path.join(directory, f"adamw.{rank}"))
 
     def resume(self, directory: str, rank: int) -> None:
         """A rank that the saved job did not have goes on with rank 0's states; a snapshot without any begins anew."""

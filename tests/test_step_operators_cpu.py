@@ -270,3 +270,21 @@ print("through")
 """
     got = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=300)
     assert got.returncode == 0 and got.stdout.strip() == "through", (got.returncode, got.stderr[-500:])
+
+
+@pytest.mark.parametrize("rank", [0, 2])
+def test_states_that_were_resumed_are_saved_before_the_first_step_too(rank, tmp_path):
+    """A rank that the saved job did not have takes rank 0's."""
+    from geeps_b200.parallel.ps_module import _AdamW
+    kept = dict(m=torch.arange(256, dtype=torch.uint8), v=torch.arange(256, dtype=torch.uint8).flip(0), exponents=torch.full((2, 2), 40, dtype=torch.uint8),
+                steps=torch.tensor([7, 0]))
+    for d, clock in (("old", 8), ("new", 9)):
+        (tmp_path / d / f"snapshot.{clock}").mkdir(parents=True)
+        (tmp_path / d / "LATEST").write_text(str(clock))
+    torch.save(kept, tmp_path / "old" / "snapshot.8" / "adamw.0")
+    first = _AdamW(torch.device("cpu"), 1, 0.1, 0.0, bits=8)
+    first.resume(str(tmp_path / "old"), rank)
+    first.save(str(tmp_path / "new" / "snapshot.9"), rank)
+    again = _AdamW(torch.device("cpu"), 1, 0.1, 0.0, bits=8)
+    again.resume(str(tmp_path / "new"), rank)
+    assert again._resumed is not None and all(torch.equal(again._resumed[k], kept[k]) for k in kept)
