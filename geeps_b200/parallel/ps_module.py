@@ -14,6 +14,7 @@ Stands in for the solver glue of the reference's (absent) Caffe application.
 from __future__ import annotations
 
 import os
+from dataclasses import replace
 
 import torch
 
@@ -143,8 +144,8 @@ class PSModule:
         stochastic rounding; None: to the nearest), each optional.  The rate is ps_config.learning_rate (set_hyper_params changes it
         without a new capture), the decay ps_config.weight_decay, for the parameters that decay.  Of several workers each takes 1 /
         world of its own step.  With clip_gradients the gradients are scaled on their way into the step and `clip_result` holds {norm, 1}.
-        Parameters are given back when the step has read them.  The states (`adamw.state`) are the worker's own; save_snapshot writes
-        and resume_from reads them."""
+        Parameters are given back when the step has read them.  The states (`adamw.state`) are the worker's own; save_snapshot and
+        the snapshots of ps_config.snapshot_interval write and resume_from reads them."""
         self.net, self.rank, self.world, self.slack = net, rank, world, slack
         self.device = torch.device(device)
         self.trace = trace or NullTrace()
@@ -216,7 +217,10 @@ class PSModule:
             for t in self.tables:
                 if t.specs and t.specs[0].name == "weight" and not t.pull:
                     ps_config.table_fp32_from_row[t.table_id] = (t.offsets[1] // ROW_FLOATS) if len(t.specs) > 1 else t.rows
-        self.ps = GeePs(rank, ps_config)
+        # the runtime's periodic snapshots are taken inside a clock and know nothing of AdamW's states: the module takes them instead
+        self._snapshot_every = ps_config.snapshot_interval if adamw is not None and ps_config.snapshot_dir else 0
+        self._snapshot_dir = ps_config.snapshot_dir
+        self.ps = GeePs(rank, replace(ps_config, snapshot_interval=0) if self._snapshot_every else ps_config)
         # tape replay: record two consecutive steps; if they issued identical native calls (static pointers),
         # later steps walk the tape instead of re-running the Python layer code
         self.use_graph = (use_graph and not manage_activations and ps_config.transport == TRANSPORT_NVLINK
@@ -333,6 +337,7 @@ class PSModule:
                     self.initial_params[f"{t.layer.name}.{sp.name}"] = init.clone()
             self.ps.update(t.h_upd)
         self.ps.clock()
+        self._periodic_snapshot()
 
     def _bind_read_pull(self, t):
         """Fully-connected layer on an uncached table: no copy of the weights is made here - the layer's forward
@@ -382,6 +387,11 @@ class PSModule:
     def step(self, x: torch.Tensor, labels: torch.Tensor, capture: bool = False) -> torch.Tensor:
         """One clock: forward, backward, push.  Returns the mean loss as a 1-element device tensor.
         capture=True keeps clones of the parameters this clock read in `self.captured`."""
+        loss = self._step(x, labels, capture)
+        self._periodic_snapshot()
+        return loss
+
+    def _step(self, x, labels, capture):
         net, tr = self.net, self.trace
         key = self._step_key(x, labels)
         graph = self._graphs.get(key) if self.use_graph and not capture else None
@@ -492,6 +502,10 @@ class PSModule:
             self._finish_recording(L.stop_recording(), key)
         self.steps += 1
         return loss
+
+    def _periodic_snapshot(self) -> None:
+        if self._snapshot_every and self.ps.clock_value % self._snapshot_every == 0:
+            self.save_snapshot(self._snapshot_dir)
 
     def is_steady(self, x: torch.Tensor, labels: torch.Tensor) -> bool:
         """True when the next step with these buffers replays a captured graph (or, without graphs, a recorded

@@ -207,3 +207,40 @@ def test_refusals():
         PSModule(net(), (16, 3, 8, 8), cfg(TRANSPORT_NVLINK), device="cuda:0", adamw={})
     with pytest.raises(ValueError, match="fp32"):
         module(bf16_weights_only=True)
+
+
+def exact_net():
+    """A network whose gradients are sums in one order: the same steps end in the same bits."""
+    return Net("n", Input(cpad=8), [GroupNorm("g0", 4, act="relu"), Linear("f1", 64, relu=True, std=0.2, fp8=True), GroupNorm("g1", 8, act="silu"),
+                                    Linear("fc", 10, std=0.3, fp32_out=True, fp8=True)])
+
+
+@pytest.mark.parametrize("how", ["plain", "tape", "graph"])
+def test_periodic_snapshots_hold_the_states(how, tmp_path):
+    kw = {"plain": {}, "tape": dict(use_tape=True), "graph": dict(use_graph=True)}[how]
+    x, y = batch()
+
+    def run(steps, every=0, **more):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            c = cfg(TRANSPORT_NVLINK, table_mode=TABLE_ADDITIVE, learning_rate=0.01, weight_decay=0.1, snapshot_interval=every, snapshot_dir=str(tmp_path))
+            mod = PSModule(exact_net(), (16, 3, 8, 8), c, device="cuda:0", seed=4, adamw=dict(bits=8, seed=3), **kw, **more)
+            for _ in range(steps):
+                mod.step(x, y)
+            st.synchronize()
+            state = {k: getattr(mod.adamw.state, k).clone() for k in ("m", "v", "exponents", "steps")}
+            mod.step(x, y, capture=True)
+            end = {k: v.clone() for k, v in mod.captured.items()}
+            assert mod.ps.clock_value == mod.steps + 1
+            mod.close()
+            return state, end
+    want, end = run(12)
+    for every in (5, 3):
+        run(7 if every == 5 else 11, every)          # the initial values are clock 0, so step 12 ends clock 12
+        clocks = [5] if every == 5 else [3, 5, 6, 9, 12]
+        assert sorted(int(p.name.split(".")[1]) for p in tmp_path.glob("snapshot.*")) == clocks and (tmp_path / "LATEST").read_text() == str(clocks[-1])
+        for c in clocks:
+            kept = torch.load(tmp_path / f"snapshot.{c}" / "adamw.0")
+            assert kept["steps"].tolist() == [c - 1, 0] and (kept["v"] != 0).any()
+        state, other = run(12 - (clocks[-1] - 1), resume_from=str(tmp_path))
+        assert all(torch.equal(state[k], want[k]) for k in want) and all(torch.equal(other[k], end[k]) for k in end)
