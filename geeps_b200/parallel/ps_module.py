@@ -62,6 +62,8 @@ class _AdamW:
         """Nothing before the first step; after a resume what it brought back."""
         kept = self._resumed if self.state is None else {k: getattr(self.state, k) for k in self._KEPT}
         if kept is not None:
+            if self.lr.is_cuda:
+                torch.cuda.synchronize(self.lr.device)      # the last step may be on its way on another stream than this call's
             os.makedirs(directory, exist_ok=True)
             torch.save(kept, os.path.join(directory, f"adamw.{rank}"))
 

@@ -244,3 +244,21 @@ def test_periodic_snapshots_hold_the_states(how, tmp_path):
             assert kept["steps"].tolist() == [c - 1, 0] and (kept["v"] != 0).any()
         state, other = run(12 - (clocks[-1] - 1), resume_from=str(tmp_path))
         assert all(torch.equal(state[k], want[k]) for k in want) and all(torch.equal(other[k], end[k]) for k in end)
+
+
+def test_a_snapshot_taken_from_another_stream_has_the_last_step(tmp_path):
+    """The step is still on its way on the stream that it was called on."""
+    x, y = batch()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        mod = module(make=exact_net, adamw=dict(bits=32))
+        for _ in range(3):
+            mod.step(x, y)
+        st.synchronize()
+        torch.cuda._sleep(400_000_000)           # some 0.2 s
+        mod.step(x, y)
+    mod.save_snapshot(str(tmp_path))
+    kept = torch.load(tmp_path / "snapshot.5" / "adamw.0")
+    st.synchronize()
+    assert kept["steps"].tolist() == [4, 0] and torch.equal(kept["m"], mod.adamw.state.m) and torch.equal(kept["v"], mod.adamw.state.v)
+    mod.close()
