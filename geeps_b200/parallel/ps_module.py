@@ -56,7 +56,7 @@ class _AdamW:
     def __init__(self, device, world, learning_rate, weight_decay, betas=(0.9, 0.999), eps: float = 1e-8, bits: int = 32, seed: int | None = None):
         self.betas, self.eps, self.bits, self.seed, self.weight_decay, self.world = betas, eps, bits, seed, weight_decay, world
         self.lr = torch.tensor([learning_rate / world], device=device)
-        self.state, self._lists, self._resumed = None, {}, None
+        self.state, self._lists, self._resumed, self._rate = None, {}, None, None
 
     def save(self, directory: str, rank: int) -> None:
         """Nothing before the first step; after a resume what it brought back."""
@@ -79,11 +79,17 @@ class _AdamW:
     def set(self, learning_rate=None, weight_decay=None) -> bool:
         """Whether a recorded step carries an old value."""
         if learning_rate is not None:
-            self.lr.fill_(learning_rate / self.world)
+            self._rate = learning_rate / self.world
         changed = weight_decay is not None and weight_decay != self.weight_decay
         if changed:
             self.weight_decay = weight_decay
         return changed
+
+    def begin(self) -> None:
+        """In front of a step and on its stream: steps that are still on their way there keep the rate that they were called with."""
+        if self._rate is not None:
+            self.lr.fill_(self._rate)
+            self._rate = None
 
     def step(self, mod) -> None:
         names = [(t.layer, sp) for t in mod.tables for sp in t.specs]
@@ -389,6 +395,8 @@ class PSModule:
     def step(self, x: torch.Tensor, labels: torch.Tensor, capture: bool = False) -> torch.Tensor:
         """One clock: forward, backward, push.  Returns the mean loss as a 1-element device tensor.
         capture=True keeps clones of the parameters this clock read in `self.captured`."""
+        if self.adamw is not None:
+            self.adamw.begin()
         loss = self._step(x, labels, capture)
         self._periodic_snapshot()
         return loss

@@ -262,3 +262,30 @@ def test_a_snapshot_taken_from_another_stream_has_the_last_step(tmp_path):
     st.synchronize()
     assert kept["steps"].tolist() == [4, 0] and torch.equal(kept["m"], mod.adamw.state.m) and torch.equal(kept["v"], mod.adamw.state.v)
     mod.close()
+
+
+def test_a_rate_set_from_another_stream_is_for_the_next_step():
+    """A step that is still on its way keeps the rate that it was called with, the one called next has the new one."""
+    x, y = batch()
+    ends = []
+    for apart in (False, True):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            mod = module(make=exact_net, adamw=dict(bits=32))
+            for _ in range(3):
+                mod.step(x, y)
+            st.synchronize()
+            if apart:
+                torch.cuda._sleep(400_000_000)           # some 0.2 s
+            mod.step(x, y)
+            if not apart:
+                mod.set_hyper_params(learning_rate=0.5)
+        if apart:
+            mod.set_hyper_params(learning_rate=0.5)
+        with torch.cuda.stream(st):
+            mod.step(x, y)
+            mod.step(x, y, capture=True)
+            st.synchronize()
+            ends.append({k: v.clone() for k, v in mod.captured.items()})
+            mod.close()
+    assert all(torch.equal(ends[0][k], ends[1][k]) for k in ends[0])
