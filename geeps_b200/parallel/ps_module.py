@@ -53,8 +53,11 @@ class _AdamW:
     """The AdamW step of a module's tables: gradients in the update buffers become the updates."""
     _KEPT = ("m", "v", "exponents", "steps")
 
-    def __init__(self, device, world, learning_rate, weight_decay, betas=(0.9, 0.999), eps: float = 1e-8, bits: int = 32, seed: int | None = None):
-        self.betas, self.eps, self.bits, self.seed, self.weight_decay, self.world = betas, eps, bits, seed, weight_decay, world
+    def __init__(self, device, world, learning_rate, weight_decay, betas=(0.9, 0.999), eps: float = 1e-8, bits: int = 32, seed: int | None = None,
+                 rank: int = 0):
+        self.betas, self.eps, self.bits, self.weight_decay, self.world = betas, eps, bits, weight_decay, world
+        # each worker rounds with bits of its own, so that what their roundings add to the sum of their steps averages out
+        self.seed = None if seed is None else seed + (rank << 32)
         self.lr = torch.tensor([learning_rate / world], device=device)
         self.state, self._lists, self._resumed, self._rate = None, {}, None, None
 
@@ -149,7 +152,7 @@ class PSModule:
         inf only measures.
         adamw: the worker computes the updates of all tables with one AdamW step (F.adamw_step) at the end of the backward pass and the
         shards add them (tables must be TABLE_ADDITIVE): a dict of betas, eps, bits (32, or 8 for states in 8 bits) and seed (of
-        stochastic rounding; None: to the nearest), each optional.  The rate is ps_config.learning_rate (set_hyper_params changes it
+        stochastic rounding, to which the rank is added; None: to the nearest), each optional.  The rate is ps_config.learning_rate (set_hyper_params changes it
         without a new capture), the decay ps_config.weight_decay, for the parameters that decay.  Of several workers each takes 1 /
         world of its own step.  With clip_gradients the gradients are scaled on their way into the step and `clip_result` holds {norm, 1}.
         Parameters are given back when the step has read them.  The states (`adamw.state`) are the worker's own; save_snapshot and
@@ -253,7 +256,7 @@ class PSModule:
         if adamw is not None:
             if self.device.type != "cuda" or ps_config.table_mode != TABLE_ADDITIVE or pull_fc or bf16_weights_only:
                 raise ValueError("adamw needs a GPU, additive tables and fp32 parameters of the worker (neither pull_fc nor bf16_weights_only)")
-            self.adamw = _AdamW(self.device, world, ps_config.learning_rate, ps_config.weight_decay, **adamw)
+            self.adamw = _AdamW(self.device, world, ps_config.learning_rate, ps_config.weight_decay, rank=rank, **adamw)
         self._declare()
         if resume_from is not None:
             if not self.ps.load_snapshot(resume_from):

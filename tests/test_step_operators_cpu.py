@@ -288,3 +288,14 @@ def test_states_that_were_resumed_are_saved_before_the_first_step_too(rank, tmp_
     again = _AdamW(torch.device("cpu"), 1, 0.1, 0.0, bits=8)
     again.resume(str(tmp_path / "new"), rank)
     assert again._resumed is not None and all(torch.equal(again._resumed[k], kept[k]) for k in kept)
+
+
+def test_workers_round_with_bits_of_their_own():
+    """A step's random bits are a hash of seed x 0x100000001B3 + step: no worker meets another's in 2^32 steps."""
+    from geeps_b200.parallel.ps_module import _AdamW
+    for seed in (0, 7, -1, (1 << 64) - 1):
+        at = [_AdamW(torch.device("cpu"), 8, 0.1, 0.0, rank=r, seed=seed).seed for r in range(8)]
+        assert at[0] == seed
+        keys = sorted((s & 0xFFFFFFFFFFFFFFFF) * 0x100000001B3 % (1 << 64) for s in at)
+        assert all(b - a > 1 << 32 for a, b in zip(keys, keys[1:])) and keys[0] + (1 << 64) - keys[-1] > 1 << 32
+    assert _AdamW(torch.device("cpu"), 8, 0.1, 0.0, rank=3).seed is None
