@@ -246,3 +246,27 @@ def test_refusals():
     state.m = state.m[:64]
     with pytest.raises(ValueError, match="AdamWState"):
         step()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-30, 1e-20, 1e-15])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [1024, 1001])
+def test_small_gradients_beside_a_small_eps(eps, bits, n):
+    """Second moments below the smallest normal number (1.2e-38) count, and a gradient of zero beside an eps above zero changes nothing.
+    The change: 2^-19 of it as elsewhere, and what v's two roundings and eps' own leave, each half of 2^-149 at the most: of the root half
+    of what v is off by, relative to v."""
+    from geeps_b200.ops import functional as F
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    g = torch.where(torch.rand(n, generator=gen, device=DEV) < 0.5, -1.0, 1.0) * 10.0 ** (-19.0 + 4 * torch.rand(n, generator=gen, device=DEV))
+    g[3::5] = 1.0                                   # beside large ones
+    if eps:
+        g[4::5] = 0.0
+    p, out = torch.zeros(n, device=DEV), torch.empty(n, device=DEV)
+    state = F.AdamWState([p], bits=bits)
+    F.adamw_step([p], [g], state, LR, betas=(B1, B2), eps=eps, out=[out])
+    d = g.double()
+    m, v, e = (1 - B1) * d, (1 - B2) * d * d, torch.tensor(eps).float().double().item()
+    change = -LR * (m / (1 - B1)) / (torch.sqrt(v / (1 - B2)) + e)
+    change[d == 0] = 0.0
+    off = 2.0 ** -19 + torch.where(v > 0, 2.1 * 2.0 ** -150 / v, 0.0)
+    assert ((out.double() - change).abs() <= off * change.abs()).all()
