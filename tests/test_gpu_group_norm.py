@@ -357,3 +357,27 @@ def test_too_many_channels_are_refused(c):
                  lambda: F.group_norm_backward(x, x.clone(), torch.empty_like(x), 2, F.GroupNorm(1, stats=stats))):
         with pytest.raises(ValueError, match="16384"):
             call()
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("size", [(1, 64, 64, 8), (1, 30000, 64, 8), (1, 9, 16384, 1), (1, 50, 21, 3), (1, 20000, 21, 3)], ids=str)
+def test_the_border_of_the_relu_is_the_same_forward_and_backward(size, types):
+    """A bias that is minus the product to the last bit, as above: what the forward pass lets through is what the backward pass lets
+    through, and z of rounded operations says what that is."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = size
+    x, _, w, _ = made(*size, types, 9)
+    x[::2] = x[:1]                                                       # half of the pixels of a channel have one value, and z
+    stats, y = torch.empty(1, groups, 2, device=DEV), torch.empty(x.shape, dtype=TYPES[types][1], device=DEV)
+    F.group_norm_forward(x, y, 1, F.GroupNorm(groups, w, None, stats, EPS))
+    mean, rstd = (spread(stats[:, :, i], 1, groups, c)[0] for i in range(2))
+    b = -(((x[:1].float() - mean) * rstd) * w)[0]
+    norm = F.GroupNorm(groups, w, b, stats, EPS, "relu", torch.empty(c, device=DEV), torch.empty(c, device=DEV))
+    F.group_norm_forward(x, y, 1, norm)
+    z = ((x.float() - mean) * rstd) * w + b
+    assert (z[::2] == 0).all() and torch.equal(y > 0, z > 0)
+    for r in (0, 1, pixels // 2, pixels - 1):                            # the gradient of the bias, from a row at a time
+        dy = torch.zeros_like(y)
+        dy[r] = 1.0
+        F.group_norm_backward(x, dy, torch.empty_like(x), 1, norm)
+        assert torch.equal(norm.dbias, (y[r] > 0).float())
