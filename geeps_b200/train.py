@@ -114,7 +114,7 @@ def main(argv=None) -> None:
     ap.add_argument("--stepvalue", type=int, action="append", default=[])
     ap.add_argument("--power", type=float, default=1.0)
     ap.add_argument("--lr-hold", type=int, default=200)
-    ap.add_argument("--momentum", type=float, default=0.9)
+    ap.add_argument("--momentum", type=float, default=None, help="of --optimizer sgd (0.9)")
     ap.add_argument("--weight-decay", type=float, default=5e-4)
     ap.add_argument("--clip-gradients", type=float, default=0.0, help="bound of the gradients' norm (Caffe's clip_gradients; 0: none)")
     ap.add_argument("--optimizer", default="sgd", choices=["sgd", "adamw"], help="momentum SGD in the shards, or AdamW in the worker")
@@ -135,6 +135,10 @@ def main(argv=None) -> None:
         ap.error("--norm group is for the Inception models")
     if args.adam_bits == 8 and args.optimizer != "adamw":
         ap.error("--adam-bits is for --optimizer adamw")
+    if args.momentum is not None and args.optimizer != "sgd":
+        ap.error("--momentum is for --optimizer sgd")
+    if args.momentum is None and args.optimizer == "sgd":
+        args.momentum = 0.9
 
     import numpy as np
     import torch
@@ -175,7 +179,7 @@ def main(argv=None) -> None:
     base_port = 10000 + (int(os.environ.get("MASTER_PORT", "29500")) % 500) * 40
     cfg = GeePsConfig(host_list=["127.0.0.1"] * world, port_list=[base_port + 10 * r for r in range(world)],
                       device=DEVICE_CUDA, cuda_device=local_rank, transport=TRANSPORT_NVLINK,
-                      table_mode=TABLE_ADDITIVE if adamw else TABLE_SGD_MOMENTUM, learning_rate=args.base_lr, momentum=args.momentum,
+                      table_mode=TABLE_ADDITIVE if adamw else TABLE_SGD_MOMENTUM, learning_rate=args.base_lr, momentum=args.momentum or 0.0,
                       weight_decay=args.weight_decay, grad_scale=1.0 / world, bf16_compute_cache=1)
     resume = args.snapshot_dir if args.resume else None
     if args.resume and not (args.snapshot_dir and os.path.exists(os.path.join(args.snapshot_dir, "LATEST"))):

@@ -299,3 +299,10 @@ def test_workers_round_with_bits_of_their_own():
         keys = sorted((s & 0xFFFFFFFFFFFFFFFF) * 0x100000001B3 % (1 << 64) for s in at)
         assert all(b - a > 1 << 32 for a, b in zip(keys, keys[1:])) and keys[0] + (1 << 64) - keys[-1] > 1 << 32
     assert _AdamW(torch.device("cpu"), 8, 0.1, 0.0, rank=3).seed is None
+
+
+@pytest.mark.parametrize("momentum", ["0.5", "0.9"])
+def test_the_trainer_refuses_a_momentum_beside_adamw(momentum, capsys):
+    with pytest.raises(SystemExit):
+        train.main(["--optimizer", "adamw", "--momentum", momentum, "--max-iter", "0", "--synthetic-images", "0"])
+    assert "--momentum is for --optimizer sgd" in capsys.readouterr().err
