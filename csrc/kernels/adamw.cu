@@ -428,8 +428,7 @@ int run(const GeepsAdamW& k, cudaStream_t st) {
 }  // namespace
 
 extern "C" int geeps_adamw(const GeepsAdamW* k, void* stream) {
-  if (!k || !k->params || !k->grads || !k->m || !k->v || !k->steps || !k->decay || (k->bits != 8 && k->bits != 32) || (k->bits == 8 && !k->exponents))
-    return (int)cudaErrorInvalidValue;
+  if (!k || !k->params || !k->grads || !k->steps || !k->decay || (k->bits != 8 && k->bits != 32)) return (int)cudaErrorInvalidValue;
   const GeepsTensors &p = *k->params, &g = *k->grads;
   if (p.n < 0 || g.n != p.n || (k->out && k->out->n != p.n)) return (int)cudaErrorInvalidValue;
   if (!(k->beta1 >= 0 && k->beta1 < 1 && k->beta2 >= 0 && k->beta2 < 1 && k->eps >= 0)) return (int)cudaErrorInvalidValue;
@@ -439,7 +438,7 @@ extern "C" int geeps_adamw(const GeepsAdamW* k, void* stream) {
     if (p.count[i] && (!p.ptr[i] || !g.ptr[i] || (k->out && !k->out->ptr[i]))) return (int)cudaErrorInvalidValue;
     blocks += (p.count[i] + 127) >> 7;
   }
-  if (blocks > k->blocks) return (int)cudaErrorInvalidValue;
+  if (blocks > k->blocks || (blocks && (!k->m || !k->v || (k->bits == 8 && !k->exponents)))) return (int)cudaErrorInvalidValue;
   const int size = k->bits / 8;
   if ((((uintptr_t)k->m | (uintptr_t)k->v) & (size == 4 ? 15 : 3)) || ((uintptr_t)k->exponents & 1) || ((uintptr_t)k->steps & 7) ||
       ((uintptr_t)k->lr_ref & 3) || ((uintptr_t)k->norm & 3) || tensors_between(p) || tensors_between(g) || (k->out && tensors_between(*k->out)))
@@ -467,8 +466,8 @@ extern "C" int geeps_adamw(const GeepsAdamW* k, void* stream) {
 }
 
 extern "C" int geeps_adamw_moments(const unsigned char* codes, const unsigned char* exponents, void* out, int second, int fp32, long long blocks, void* stream) {
-  if (blocks < 0 || !codes || !exponents || !out || ((uintptr_t)codes & 15) || ((uintptr_t)out & 31)) return (int)cudaErrorInvalidValue;
   if (blocks == 0) return 0;
+  if (blocks < 0 || !codes || !exponents || !out || ((uintptr_t)codes & 15) || ((uintptr_t)out & 31)) return (int)cudaErrorInvalidValue;
   const long long n16 = blocks * 8, want = (n16 + 255) / 256, most = (long long)geeps_sm_count() * 8;
   auto kernel = second ? (fp32 ? moments_kernel<true, 255> : moments_kernel<false, 255>) : (fp32 ? moments_kernel<true, 127> : moments_kernel<false, 127>);
   geeps_launch(kernel, dim3((unsigned)(want < most ? want : most)), dim3(256), 0, (cudaStream_t)stream, codes, exponents, out, n16);

@@ -270,3 +270,17 @@ def test_small_gradients_beside_a_small_eps(eps, bits, n):
     change[d == 0] = 0.0
     off = 2.0 ** -19 + torch.where(v > 0, 2.1 * 2.0 ** -150 / v, 0.0)
     assert ((out.double() - change).abs() <= off * change.abs()).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameters_without_values_take_their_steps(bits):
+    """A worker whose share is empty: the steps count, and what is asked of no values gives none."""
+    from geeps_b200.ops import functional as F
+    p, g = [torch.empty(0, device=DEV), torch.empty(0, dtype=torch.bfloat16, device=DEV)], [torch.empty(0, device=DEV)] * 2
+    state = F.AdamWState(p, bits=bits)
+    for _ in range(2):
+        F.adamw_step(p, g, state, LR, seed=1)
+    F.adamw_step(p, g, state, LR, out=[torch.empty(0, device=DEV)] * 2)
+    assert state.steps.tolist() == [3, 0]
+    if bits == 8:
+        F.adamw_moments(state, torch.empty(0, device=DEV), torch.empty(0, device=DEV))
