@@ -289,3 +289,29 @@ def test_a_rate_set_from_another_stream_is_for_the_next_step():
             ends.append({k: v.clone() for k, v in mod.captured.items()})
             mod.close()
     assert all(torch.equal(ends[0][k], ends[1][k]) for k in ends[0])
+
+
+def test_group_norms_whose_inputs_are_evicted_and_in_graphs_train_alike():
+    """Parameters after ten steps to the last bit, of which the last ones are replays, or have their activations fetched back."""
+    make = lambda: Net("n", Input(cpad=8), [GroupNorm("g0", 4, act="relu"), GroupNorm("g1", 2, act="silu"), GroupNorm("g2", 8), GroupNorm("g3", 4, act="relu"),
+                                            Linear("f1", 32, relu=True, std=0.01, fp8=True), Linear("fc", 10, std=0.3, fp32_out=True, fp8=True)])
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x, y = torch.randn(16, 3, 64, 64, generator=gen, device=DEV), torch.randint(0, 10, (16,), generator=gen, device=DEV)
+    ends = []
+    for kw in (dict(), dict(use_graph=True), dict(manage_activations=True, cache_fraction=0.0)):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            mod = module(make=make, shape=(16, 3, 64, 64), adamw=dict(bits=8, seed=2), **kw)
+            if "cache_fraction" in kw:
+                assert len(mod.managed) == 4 and mod.budget_rows < mod.working_set_rows            # not all of them fit
+            for _ in range(10):
+                mod.step(x, y)
+            assert "use_graph" not in kw or mod.is_steady(x, y), mod.tape_mismatch
+            mod.step(x, y, capture=True)
+            st.synchronize()
+            ends.append({k: v.clone() for k, v in mod.captured.items()})
+            mod.close()
+    first = ends[0]
+    assert all(v.isfinite().all() for v in first.values()) and (first["g0.gamma"] != 1).any() and (first["g3.beta"] != 0).any()
+    for other in ends[1:]:
+        assert other.keys() == first.keys() and all(torch.equal(other[k], first[k]) for k in first), [k for k in first if not torch.equal(other[k], first[k])]
