@@ -315,3 +315,41 @@ def test_group_norms_whose_inputs_are_evicted_and_in_graphs_train_alike():
     assert all(v.isfinite().all() for v in first.values()) and (first["g0.gamma"] != 1).any() and (first["g3.beta"] != 0).any()
     for other in ends[1:]:
         assert other.keys() == first.keys() and all(torch.equal(other[k], first[k]) for k in first), [k for k in first if not torch.equal(other[k], first[k])]
+
+
+def test_two_workers_give_half_of_their_own_steps_each():
+    """The updates that an additive table gets from two workers with gradients of their own: the mean of their steps, each clipped by
+    its own norm.  Each change is within 2^-18 of itself, and an fp32 rounding of the quantities that it is the sum of."""
+    from types import SimpleNamespace as Space
+
+    from geeps_b200.parallel.ps_module import _AdamW
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    sizes, world = {"weight": 3000, "bias": 70}, 2
+    p = {k: torch.randn(n, generator=gen, device=DEV) for k, n in sizes.items()}
+    workers = [_AdamW(DEV, world, 0.02, 0.1, rank=r) for r in range(world)]
+    state = [{k: (torch.zeros(n, device=DEV, dtype=F64), torch.zeros(n, device=DEV, dtype=F64)) for k, n in sizes.items()} for _ in workers]
+    mods = [Space(steps=0, _period=2, clip_gradients=1.5, _clip_work=None, clip_result=torch.zeros(2, device=DEV), device=DEV) for _ in workers]
+    for step in range(1, 4):
+        total, want, size = ({k: torch.zeros(n, device=DEV, dtype=F64) for k, n in sizes.items()} for _ in range(3))
+        for w, mod, s in zip(workers, mods, state):
+            g = {k: 0.1 * torch.randn(n, generator=gen, device=DEV) for k, n in sizes.items()}
+            norm = sum(v.to(F64).square().sum() for v in g.values()).sqrt()
+            c = min(1.0, 1.5 / norm.item())
+            assert c < 1.0
+            for k in sizes:
+                m, v = s[k]
+                m.mul_(0.9).add_(0.1 * c * g[k].to(F64))
+                v.mul_(0.999).add_(0.001 * (c * g[k].to(F64)).square())
+                own = -0.02 * (m / (1 - 0.9 ** step) / ((v / (1 - 0.999 ** step)).sqrt() + 1e-8) + (0.1 * p[k].to(F64) if k == "weight" else 0.0))
+                want[k] += own / world
+                # m is a sum of signed terms: its roundings go by their sizes, of which a step's 0.1 g is the largest part
+                size[k] += 0.02 / world * (0.9 * m.abs() + c * g[k].to(F64).abs()) / (v / (1 - 0.999 ** step)).sqrt() + own.abs() / world
+            layer = Space(p32=p, g32=g)
+            mod.tables, mod.steps = [Space(layer=layer, specs=[Space(name="weight", decay=True), Space(name="bias", decay=False)])], step - 1
+            w.begin()
+            w.step(mod)
+            for k in sizes:
+                total[k] += g[k].to(F64)
+        for k in sizes:
+            assert ((total[k] - want[k]).abs() <= 2.0 ** -18 * size[k]).all()
+            p[k] += want[k].float()
