@@ -12,9 +12,12 @@
 // subnormals every code costs an addition and a shift each way, and infinities and NaN go through as they are (with them in a block,
 // E is 255 and its finite values vanish or become v's least).
 // An exponential mean moves by (1 - b) of its value a step, less than half of the distance between two codes, so nearest rounding
-// leaves it where it is.  Stochastic rounding adds 16 random bits below the last one that is kept: the mean of the rounded values
-// is the value.  The bits come from a hash of seed, step and place (the finaliser of the splittable generator of Steele, Lea and
-// Flood, as in the dropout kernel), 64 for two neighbours.
+// leaves it where it is.  Stochastic rounding adds 16 random bits below the last one that is kept: from code 1 on the mean of the
+// rounded values is the value.  Below, m has less: from 2^-15 (of the power of two at or below the block's largest) to code 1, 9/8 of that,
+// it becomes 0 or code 1 by the distance from the two, and under 2^-15 always 0, where v becomes code 1.  A parameter whose
+// gradients are that much smaller than those of its 128 neighbours so moves by its decay alone.
+// The bits come from a hash of seed, step and place (the finaliser of the splittable generator of Steele, Lea and Flood, as in the
+// dropout kernel), 64 for two neighbours.
 // m and v are rounded after every operation (no fused multiply-add), so that their codes do not depend on how they are compiled.
 //
 // Bound by memory with states in 32 bits (28 bytes a value with fp32 parameters and gradients), by instructions with 8.

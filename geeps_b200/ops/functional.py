@@ -827,8 +827,9 @@ def adamw_step(params, grads, state: AdamWState, lr, *, betas=(0.9, 0.999), eps:
     on the device, which a captured step then reads.  clip: (norm, max_norm) with the result of clip_gradients(grads, inf, norm): c =
     max_norm / norm where the norm exceeds max_norm.  eps (fp32): from 0 up; 0 leaves 0 / 0 to a parameter whose gradients were all
     zero.  seed: round 8-bit states and bf16 parameters up or down at random, by bits that are a function of seed, step and place, so
-    that small changes are not lost; None: to the nearest.  A gradient that is not finite makes its parameter's states so, with states
-    in 8 bits those of its neighbours (128 values) useless."""
+    that changes of less than half a code are not lost; None: to the nearest.  With states in 8 bits a first moment below some 2^-15 of
+    the largest of its block of 128 is zero all the same, and its parameter moves by the decay alone.  A gradient that is not finite
+    makes its parameter's states so, with states in 8 bits those of its neighbours (128 values) useless."""
     params = params if isinstance(params, GradList) else GradList(params)
     grads = grads if isinstance(grads, GradList) else GradList(grads)
     out = out if out is None or isinstance(out, GradList) else GradList(out)

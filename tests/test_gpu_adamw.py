@@ -284,3 +284,24 @@ def test_parameters_without_values_take_their_steps(bits):
     assert state.steps.tolist() == [3, 0]
     if bits == 8:
         F.adamw_moments(state, torch.empty(0, device=DEV), torch.empty(0, device=DEV))
+
+
+def test_the_mean_of_first_moments_at_the_end_of_their_codes():
+    """Beside a 1, whose code is 120: code 1 is 2^-15 x 9/8.  From there on the mean of what random rounding leaves is the value; from
+    2^-15 to code 1 it is code 1 by the odds of the distance from 2^-15; below it is 0.  n values that are one of two, d apart: 5
+    standard deviations of their mean, d / (2 sqrt(n)) each, and the 2^-16 that 16 random bits leave of d."""
+    from geeps_b200.ops import functional as F
+    blocks, least, step = 4096, 2.0 ** -15, 2.0 ** -18
+    for x in (3.0e-5, 3.1e-5, 3.2e-5, 3.4e-5, 3.5e-5, 5.0e-5, 6.0e-5, 1.0e-3):
+        g = torch.full((blocks, 128), 2 * x, device=DEV)
+        g[:, 0] = 2.0                                       # m = g / 2
+        p, out = torch.zeros(blocks * 128, device=DEV), torch.empty(blocks * 128, device=DEV)
+        state = F.AdamWState([p], bits=8)
+        F.adamw_step([p], [g.view(-1)], state, LR, betas=(0.5, B2), out=[out], seed=9)
+        m, _ = F.adamw_moments(state, torch.empty_like(p), torch.empty_like(p))
+        m = m.view(blocks, 128)
+        assert (m[:, 0] == 1).all()
+        mean = m[:, 1:].double().mean().item()
+        want = x if x >= least + step else 0.0 if x < least else (x - least) / step * (least + step)
+        d = least + step if x < least + step else 2.0 ** math.floor(math.log2(x)) / 8
+        assert abs(mean - want) <= 5 * d / (2 * math.sqrt(blocks * 127)) + 2.0 ** -16 * d + 2.0 ** -23 * x
