@@ -14,6 +14,7 @@ Stands in for the solver glue of the reference's (absent) Caffe application.
 from __future__ import annotations
 
 import os
+import warnings
 from dataclasses import replace
 
 import torch
@@ -78,6 +79,7 @@ class _AdamW:
             if os.path.exists(os.path.join(at, f"adamw.{r}")):
                 self._resumed = torch.load(os.path.join(at, f"adamw.{r}"), map_location=self.lr.device)
                 return
+        warnings.warn(f"{at} has no AdamW states: moments and steps begin anew")
 
     def set(self, learning_rate=None, weight_decay=None) -> bool:
         """Whether a recorded step carries an old value."""

@@ -306,3 +306,13 @@ def test_the_trainer_refuses_a_momentum_beside_adamw(momentum, capsys):
     with pytest.raises(SystemExit):
         train.main(["--optimizer", "adamw", "--momentum", momentum, "--max-iter", "0", "--synthetic-images", "0"])
     assert "--momentum is for --optimizer sgd" in capsys.readouterr().err
+
+
+def test_a_snapshot_without_states_is_not_resumed_in_silence(tmp_path):
+    from geeps_b200.parallel.ps_module import _AdamW
+    (tmp_path / "snapshot.4").mkdir()
+    (tmp_path / "LATEST").write_text("4")
+    a = _AdamW(torch.device("cpu"), 1, 0.1, 0.0)
+    with pytest.warns(UserWarning, match="snapshot.4 has no AdamW states"):
+        a.resume(str(tmp_path), 0)
+    assert a._resumed is None
