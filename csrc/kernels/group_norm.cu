@@ -11,7 +11,7 @@
 // read from memory once.  The CTAs' sums meet over distributed shared memory in the order of their ranks.  Images that are too few
 // for the machine as items are cut over many CTAs in two launches (sums, then the rest), which meet in a workspace.
 // Forward reads x and writes y, backward reads x and dy and writes dx.  A block's life is a chain of waits (its pixels, the column sums,
-// the group sums, the stores: some 6 us), of which as many run side by side as shared memory holds slices: 0.45 to 0.55 of the copy
+// the group sums, the stores: some 6 us; nothing is loaded while it sums), of which as many run side by side as shared memory holds slices: 0.45 to 0.55 of the copy
 // rate (32 x 3136 x 192 forward 26 us, 256 x 196 x 576 backward 52.6).  Neither taking turns at the start (55 to 57 of 56 at the time), nor
 // four groups of copies with sums between them, nor reading again from L2 instead of keeping (121) does better.
 //
@@ -291,6 +291,8 @@ __device__ __forceinline__ void column_sums(const Dev& d, float2* entry, F finis
   }
 }
 
+// The exponential is off by up to 2 + 1.2 |z| units in the last place, the quotient by 2, where results are fp32 too: far below zero, where that is
+// much, the result itself is some z e^z
 __device__ __forceinline__ float silu(float z) { return __fdividef(z, 1.f + __expf(-z)); }
 __device__ __forceinline__ float silu_slope(float z, float dy) {
   const float g = __fdividef(1.f, 1.f + __expf(-z));
