@@ -45,6 +45,7 @@ struct Dev {
   void* C; const float* bias; int* status;
   const uint8_t *scale_a, *scale_b;
   long long M, N, ldc;                      // rows of the operand with 128-row tiles, of the other one, pitch of C
+  long long whole;                          // columns of C in whole pieces of 16 bytes
   int out_fp32, swap, relu;                 // swap: C is [N, M]
   int kt, quads;                            // k tiles, and atoms along K
   int bn, m_tiles, n_tiles, cluster, stages, slabs, tma_store, tmem_cols;
@@ -74,7 +75,7 @@ __device__ __forceinline__ void store1(const Dev& d, long long i, float v) {
 }
 
 // The epilogue of a group of four warps (group grp of G) for its share of a tile's columns: slabs 128 bytes wide (64 bf16 or 32 fp32
-// columns) leave with one TMA store each, clipped at the matrix edge.  r: the thread's row of the tile
+// columns) leave with one TMA store each, clipped at the matrix edge, which for TMA is d.whole (store_tail).  r: the thread's row of the tile
 // TWO: two slabs a group, used in turn
 template <int G, bool TWO>
 __device__ __forceinline__ void store_slabs(const Dev& d, const CUtensorMap& tmC, uint8_t* slabs, uint32_t tacc, int m0, int n0, int grp, int r,
@@ -84,7 +85,7 @@ __device__ __forceinline__ void store_slabs(const Dev& d, const CUtensorMap& tmC
   const uint32_t row_off = (uint32_t)r * 128u, rsw = (uint32_t)(r & 7);
 #pragma unroll 1
   for (int c = grp * cols; c < d.bn; c += G * cols) {
-    if ((long long)n0 + c >= d.N) break;
+    if ((long long)n0 + c >= d.whole) break;
     uint8_t* slab = slabs + (size_t)(TWO ? 2 * grp + (slab_i & 1u) : grp) * SLAB_BYTES;
     if (issuer) { if (TWO) tc05::bulk_wait_read<1>(); else tc05::bulk_wait_read<0>(); }      // the slab this group stored there has been read out
     tc05::named_bar_sync(1 + grp, 128);
@@ -128,6 +129,28 @@ __device__ __forceinline__ void store_slabs(const Dev& d, const CUtensorMap& tmC
       tc05::bulk_commit();
     }
     ++slab_i;
+  }
+}
+
+// The last columns of a row where it does not end in a whole piece of 16 bytes: a TMA store writes such a piece whole, zeros behind the last
+// column, where something else may lie.  By the group that does not have to store the slab before them, each row by its thread.  (As a part of
+// store_slabs 7452 x 8960, K = 256 30.0 us -> 31.3, without a tail.)
+template <int G>
+__device__ __forceinline__ void store_tail(const Dev& d, uint32_t tacc, int m0, int n0, int grp, int r) {
+  if (d.whole == d.N || d.whole < n0 || d.whole >= n0 + d.bn) return;
+  const int c = (int)(d.whole - n0) & ~31;
+  if (G > 1 && grp != ((int)(d.whole - n0) / (d.out_fp32 ? 32 : 64) + 1) % G) return;
+  uint32_t w[32];
+  tc05::tmem_ld_32x32(tacc + (uint32_t)c, w);
+  tc05::tmem_ld_wait();
+  if (m0 + r >= d.M) return;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const long long col = (long long)n0 + c + j;
+    if (col < d.whole || col >= d.N) continue;
+    float v = __uint_as_float(w[j]) + (d.bias != nullptr ? __ldg(d.bias + col) : 0.f);
+    if (d.relu) v = v < 0.f ? 0.f : v;
+    store1(d, (m0 + r) * d.ldc + col, v);
   }
 }
 
@@ -345,6 +368,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         leave_part(tiles, tacc, r, BN);
       } else if (d.tma_store) {
         store_slabs<G, true>(d, tmC, slabs, tacc, m0, n0, grp, r, slab_i);
+        store_tail<G>(d, tacc, m0, n0, grp, r);
       } else if (!d.swap) {
         store_rows<G>(d, slabs + grp * SLAB_BYTES + q * 32 * 128, tacc, m0 + q * 32, n0, grp, lane);
       } else {
@@ -501,7 +525,10 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       if (!tc05::mbar_wait(&ctl->tmem_full[acc], acc_ph, abort_flag, WAIT_BUDGET_NS)) break;
       tc05::fence_after_sync();
       const uint32_t tacc = tmem + acc * (uint32_t)BN + ((uint32_t)(q * 32) << 16);
-      if (m0 < d.M) store_slabs<2, false>(d, tmC, slabs, tacc, m0, n0, grp, q * 32 + lane, slab_i);
+      if (m0 < d.M) {
+        store_slabs<2, false>(d, tmC, slabs, tacc, m0, n0, grp, q * 32 + lane, slab_i);
+        store_tail<2>(d, tacc, m0, n0, grp, q * 32 + lane);
+      }
       tc05::fence_before_sync();
       __syncwarp();
       if (lane == 0) tc05::mbar_arrive_cluster(tc05::map_to_cta(tc05::smem_u32(&ctl->tmem_empty[acc]), 0));      // the warps of both report
@@ -627,6 +654,7 @@ int lay_out(const GeepsGemmFp8* p, Plan& plan, Dev& d) {
   d.M = plan.swap ? p->N : p->M; d.N = plan.swap ? p->M : p->N; d.ldc = p->ldc;
   d.scale_a = plan.swap ? p->scale_b : p->scale_a; d.scale_b = plan.swap ? p->scale_a : p->scale_b;
   d.tma_store = plan.cluster == 1 && !plan.swap && rows16;
+  d.whole = p->N & -(16LL / size);
   d.bn = plan.bn;
   d.cluster = plan.cluster;
   d.m_tiles = (int)((d.M + (pair ? 2 : 1) * BM - 1) / ((pair ? 2 : 1) * BM));
@@ -701,8 +729,8 @@ int geeps_gemm_fp8(const GeepsGemmFp8* p, void* stream) {
   CUtensorMap ta, tb, tc;
   if (!make_map(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, A, p->K, d.M, lda, BK, BM) || !make_map(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, B, p->K, d.N, ldb, BK, pair ? d.bn / 2 : d.bn))
     return (int)cudaErrorInvalidValue;
-  if (d.tma_store && !make_map(&tc, p->out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p->C, p->N, p->M,
-                               p->ldc * size, p->out_fp32 ? 32 : 64, BM)) {
+  if (d.tma_store && !make_map(&tc, p->out_fp32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p->C,
+                               d.whole ? d.whole : 16 / size, p->M, p->ldc * size, p->out_fp32 ? 32 : 64, BM)) {
     if (pair) return (int)cudaErrorInvalidValue;
     d.tma_store = 0;
     give_memory(d, plan);

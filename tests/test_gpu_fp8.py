@@ -318,3 +318,24 @@ def test_several_tiles_a_cta_with_other_scales_in_every_block(plan, M, N, K):
     exact = plain(a, b)
     sums, half = tolerance(a, b, out, K)
     assert ((out.double() - exact).abs() <= sums + half * (exact.abs() + sums)).all()
+
+
+@pytest.mark.parametrize("plan", [(0, 0, 0), (64, 1, 0), (32, 1, 0), (192, 1, 0), (64, -2, 0), (128, -2, 0)])
+@pytest.mark.parametrize("N", [1, 5, 8, 33, 90, 100, 250, 257])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_what_lies_behind_the_last_column_stays(N, dtype, plan):
+    """Rows on a pitch that TMA stores, whose last column is inside a piece of 16 bytes."""
+    from geeps_b200.ops import functional as F
+    if plan[0] == 32 and N > 32:
+        plan = (128, 1, 0)
+    gen = torch.Generator(device=DEV).manual_seed(N)
+    for M in (40, 300):
+        a, b = F.quantize_fp8(torch.randn(M, 200, generator=gen, device=DEV)), F.quantize_fp8(torch.randn(N, 200, generator=gen, device=DEV))
+        bias = torch.randn(N, generator=gen, device=DEV)
+        wide = torch.full((M + 2, (N + 47) // 16 * 16), 9.0, dtype=dtype, device=DEV)
+        F.matmul_fp8(a, b, wide[:M, :N], bias=bias, relu=True, plan=plan)
+        exact = (plain(a, b) + bias.double()).relu()
+        sums, half = tolerance(a, b, wide, 200)
+        sums = sums + 2.0 ** -23 * bias.double().abs()
+        assert ((wide[:M, :N].double() - exact).abs() <= sums + half * (exact.abs() + sums)).all()
+        assert (wide[:, N:] == 9.0).all() and (wide[M:] == 9.0).all()
