@@ -45,6 +45,7 @@ constexpr int gemm_threads(bool cl) { return 64 + 128 * epi_groups(cl); }
 struct GemmDev {
   void* C; const float* bias; int* status;
   long long M, N, K, ldc;
+  long long whole;  // columns that TMA stores: N in whole pieces of 16 bytes (sums: N, what is added behind it is zero)
   float alpha, beta;
   int out_fp32, bias_mode, relu, split_k, kt_total, stages;
   int bn;           // tile width: multiple of 32 (64 for an MN-major B), <= 256
@@ -248,7 +249,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         const int n_lim = (int)d.N;
 #pragma unroll 1
         for (int c = grp * cols_per_slab; c < BN; c += G * cols_per_slab) {
-          if ((long long)n0 + c >= d.N) break;
+          if ((long long)n0 + c >= d.whole) break;
           uint8_t* slab = cslab + (size_t)(2 * grp + (slab_i & 1u)) * C_SLAB_BYTES;
           if (issuer) tc05::bulk_wait_read<1>();   // the slab this group stored two slabs ago has been read out
           tc05::named_bar_sync(1 + grp, 128);
@@ -300,6 +301,25 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             tc05::bulk_commit();
           }
           ++slab_i;
+        }
+        // a TMA store writes a piece of 16 bytes whole, zeros behind the last column, where something else may lie: the last columns of a
+        // row leave by its thread, in the group that does not have to store the slab before them
+        if (d.whole < d.N && d.whole >= n0 && d.whole < n0 + BN && (G == 1 || grp == ((int)(d.whole - n0) / cols_per_slab + 1) % G)) {
+          const int c = (int)(d.whole - n0) & ~31;
+          uint32_t r[32];
+          tc05::tmem_ld_32x32(tacc + (uint32_t)c, r);
+          tc05::tmem_ld_wait();
+          if (row < d.M) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const long long col = (long long)n0 + c + j;
+              if (col < d.whole || col >= d.N) continue;
+              float v = fmaf(alpha, __uint_as_float(r[j]), bmode == 1 ? __ldg(d.bias + col) : bias_row);
+              if (relu) v = fmaxf(v, 0.f);
+              if (d.out_fp32) ((float*)d.C)[row * d.ldc + col] = v;
+              else ((__nv_bfloat16*)d.C)[row * d.ldc + col] = __float2bfloat16(v);
+            }
+          }
         }
       } else {
   #pragma unroll 1
@@ -698,9 +718,11 @@ int geeps_gemm_bf16(const GeepsGemmParams* p, void* stream) {
     d.beta = 0.f;
   }
   d.tma_store = tma_c && cluster == 1 ? 1 : 0;
+  const int size = p->out_fp32 ? 4 : 2;
+  d.whole = d.split_k > 1 ? p->N : p->N & -(16LL / size);
   CUtensorMap tc;
   if (d.tma_store) {
-    if (!make_map(&tc, p->C, p->N, p->M, p->ldc, p->out_fp32 ? 32 : 64, BM, p->out_fp32 != 0)) d.tma_store = 0;
+    if (!make_map(&tc, p->C, d.whole ? d.whole : 16 / size, p->M, p->ldc, p->out_fp32 ? 32 : 64, BM, p->out_fp32 != 0)) d.tma_store = 0;
   }
   if (!d.tma_store) tc = ta;   // unused by the kernel
   const int stage_bytes = A_STAGE_BYTES + bn * BK * 2;

@@ -40,6 +40,9 @@ struct PairDev {
   float alpha;
   int out_fp32, bias_mode, relu, kt_total, stages;
   int bn, tmem_cols, m_tiles, n_tiles;   // m_tiles counts 256-row tiles
+  int whole;                             // columns that TMA stores: N in whole pieces of 16 bytes
+  void* C;
+  long long ldc;
 };
 
 struct SmemCtl {
@@ -162,7 +165,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const float bias_row = (d.bias_mode == 2 && row < d.M) ? d.bias[row] : 0.f;
 #pragma unroll 1
       for (int c = 0; c < BN; c += cols_per_slab) {
-        if (n0 + c >= n_lim) break;
+        if (n0 + c >= d.whole) break;
         uint8_t* slab = cslab + (size_t)(slab_i & 1u) * C_SLAB_BYTES;
         if (issuer) tc05::bulk_wait_read<1>();
         tc05::named_bar_sync(1, 128);
@@ -207,6 +210,25 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           tc05::bulk_commit();
         }
         ++slab_i;
+      }
+      // a TMA store writes a piece of 16 bytes whole, zeros behind the last column, where something else may lie: the last columns of a row
+      // leave by its thread
+      if (d.whole < n_lim && d.whole >= n0 && d.whole < n0 + BN) {
+        const int c = (d.whole - n0) & ~31;
+        uint32_t r[32];
+        tc05::tmem_ld_32x32(tacc + (uint32_t)c, r);
+        tc05::tmem_ld_wait();
+        if (row < d.M) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int col = n0 + c + j;
+            if (col < d.whole || col >= n_lim) continue;
+            float v = fmaf(d.alpha, __uint_as_float(r[j]), d.bias_mode == 1 ? __ldg(d.bias + col) : bias_row);
+            if (relu) v = fmaxf(v, 0.f);
+            if (d.out_fp32) ((float*)d.C)[row * d.ldc + col] = v;
+            else ((__nv_bfloat16*)d.C)[row * d.ldc + col] = __float2bfloat16(v);
+          }
+        }
       }
       // this warp has drained the accumulator: tell the leader's MMA thread (8 warps report per tile)
       tc05::fence_before_sync();
@@ -285,6 +307,8 @@ int geeps_gemm_bf16_pair(const GeepsGemmParams* p, void* stream) {
   d.alpha = p->alpha;
   d.out_fp32 = p->out_fp32; d.bias_mode = p->bias ? p->bias_mode : 0; d.relu = p->relu;
   d.kt_total = (int)((p->K + BK - 1) / BK);
+  const int size = p->out_fp32 ? 4 : 2;
+  d.whole = (int)(p->N & -(16LL / size)); d.C = p->C; d.ldc = p->ldc;
   d.bn = bn;
   d.m_tiles = (int)((p->M + 2 * BM - 1) / (2 * BM));
   d.n_tiles = (int)((p->N + bn - 1) / bn);
@@ -297,7 +321,7 @@ int geeps_gemm_bf16_pair(const GeepsGemmParams* p, void* stream) {
   if (d.stages < 2) d.stages = 2;
   CUtensorMap ta, tb, tc;
   if (!make_map(&ta, p->A, p->K, p->M, p->lda, BK, BM) || !make_map(&tb, p->B, p->K, p->N, p->ldb, BK, bn / 2) ||
-      !make_map(&tc, p->C, p->N, p->M, p->ldc, p->out_fp32 ? 32 : 64, BM, p->out_fp32 != 0))
+      !make_map(&tc, p->C, d.whole, p->M, p->ldc, p->out_fp32 ? 32 : 64, BM, p->out_fp32 != 0))
     return (int)cudaErrorInvalidValue;
   const long long num_tiles = (long long)d.m_tiles * d.n_tiles;
   const int pairs = (int)(num_tiles < kPairs ? num_tiles : kPairs);

@@ -216,3 +216,28 @@ def test_dependent_launches_keep_reads_and_writes_in_order(captured):
     for r, g in zip(ref[:5], got[:5]):
         assert torch.equal(r, g)
     assert torch.allclose(ref[5], got[5], atol=1e-4)   # block sums meet in atomics
+
+
+@pytest.mark.parametrize("impl,bn", [("tc", 0), ("tc", 32), ("tc", 64), ("tc", 192), ("pair", 64), ("pair", 0), ("auto", 0)])
+@pytest.mark.parametrize("N", [1, 5, 8, 33, 90, 100, 250, 257])
+@pytest.mark.parametrize("fp32", [False, True])
+def test_gemm_leaves_what_lies_behind_the_last_column(N, fp32, impl, bn):
+    """Rows on a pitch that TMA stores, whose last column is inside a piece of 16 bytes.  Products of two bf16 values are exact; a sum of
+    K of them is off by K steps of 2^-23 of the magnitudes at most, the bias and the output by their roundings."""
+    if impl == "pair" and N < 64:
+        N += 64
+    dev = torch.device("cuda:0")
+    torch.manual_seed(N)
+    K = 200
+    for M in (40, 300) if impl != "pair" else (300, 1000):
+        a, b = _mk(M, K, False, dev, pad=8), _mk(N, K, False, dev, pad=8)
+        for mode, bias in ((1, torch.randn(N, device=dev)), (2, torch.randn(M, device=dev)), (0, None)):
+            wide = torch.full((M + 2, (N + 47) // 16 * 16), 9.0, dtype=torch.float32 if fp32 else torch.bfloat16, device=dev)
+            F.gemm(a, b, wide[:M, :N], bias=bias, bias_mode=mode or 1, relu=mode == 1, alpha=0.5, block_n=bn, impl=impl)
+            torch.cuda.synchronize()
+            assert (wide[:, N:] == 9.0).all() and (wide[M:] == 9.0).all()
+            add = 0.0 if bias is None else bias.double() if mode == 1 else bias.double()[:, None]
+            exact = 0.5 * a.double() @ b.double().t() + add
+            sums = K * 2.0 ** -23 * 0.5 * a.double().abs() @ b.double().abs().t() + 2.0 ** -23 * (exact.abs() + (0.0 if bias is None else add.abs()))
+            want = exact.relu() if mode == 1 else exact
+            assert ((wide[:M, :N].double() - want).abs() <= sums + (2.0 ** -24 if fp32 else 2.0 ** -8) * (exact.abs() + sums)).all()
