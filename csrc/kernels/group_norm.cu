@@ -16,7 +16,8 @@
 // four groups of copies with sums between them, nor reading again from L2 instead of keeping (121) does better.
 //
 // Variance: values less the first of every 32 of a thread's pixels are added and squared, and such parts meet as count, mean and
-// sum of squared differences, so a mean far from zero costs nothing (a part's error is at most 32 x 2^-24 of its variance).
+// sum of squared differences, so a mean far from zero costs nothing.  A first value far from the others does: squares about it are at most
+// 32 times those about a part's mean, which leaves 1/std up to 1e-5 off (of 64-bit arithmetic; 2e-7 otherwise).
 // The backward pass, and with a ReLU the forward pass, form z in the four rounded operations above, so that the border of the ReLU is one and
 // does not depend on how it is compiled (forward by a subtraction and a fused operation 32 x 3136 x 192 26.0 us, so 26.2; 37 x 113 x 1003 15.4, 15.8).
 #include <math.h>
@@ -274,7 +275,7 @@ __device__ __forceinline__ void each_group(int gs, int lanes, F f) {
   }
 }
 
-// finish(c, sum over the R threads of channel c of entry[i][r][v]), c = W v + i, by one thread a channel; entry is overwritten.
+// finish(c, sum over the R threads of channel c of entry[i][r][v], the first of those), c = W v + i, by one thread a channel.
 // Every thread of the block calls it; no barrier behind it.
 template <int kThreads, int W, typename F>
 __device__ __forceinline__ void column_sums(const Dev& d, float2* entry, F finish) {
@@ -287,7 +288,7 @@ __device__ __forceinline__ void column_sums(const Dev& d, float2* entry, F finis
     float2 s = at[0];
 #pragma unroll 4
     for (int r = 1; r < d.R; ++r) s = add2(s, at[r * d.V]);
-    finish(v * W + e, s);
+    finish(v * W + e, s, at);
   }
 }
 
@@ -408,8 +409,22 @@ group_forward_kernel(const __grid_constant__ Dev d) {
         }
       }
       const float inv = p.rows ? __frcp_rn((float)p.rows) : 0.f;
-      column_sums<kThreads, W>(d, entry, [&](int c, float2 t) {
-        column[c] = make_float2(fmaf(t.x, inv, base_of[c]), fmaxf(t.y - t.x * t.x * inv, 0.f));
+      column_sums<kThreads, W>(d, entry, [&](int c, float2 t, const float2* at) {
+        const float away = t.x * inv;
+        float sq = fmaxf(t.y - t.x * away, 0.f);
+        // A base far from the mean, as of a first pixel far from the others, leaves a small difference of large sums (1/std 8e-5 off for 119 pixels):
+        // beyond five standard deviations, which a few pixels' mean seldom is by chance, the squares are formed again about the mean.  (Beyond
+        // two 1 x 196 x 576 5.45 us -> 6.0; for every channel 256 x 196 x 576 35.0 -> 36.4.)
+        if (t.x * away > 25.f * sq) {
+          sq = 0.f;
+#pragma unroll 1
+          for (int r = 0; r < d.R; ++r) {
+            const float2 u = at[r * d.V];
+            const float n = (float)(p.most + (r < p.extra)), e = n > 0.f ? __fdividef(u.x, n) : 0.f;
+            sq += fmaxf(u.y - u.x * e, 0.f) + n * (e - away) * (e - away);
+          }
+        }
+        column[c] = make_float2(base_of[c] + away, sq);
       });
     } else {
       for (int v = threadIdx.x; v < d.V; v += kThreads, x.at += kThreads * W) {
@@ -688,7 +703,7 @@ group_backward_kernel(const __grid_constant__ Dev d, float* channel_sums) {
       x.at = (const XT*)d.x + x_at;
       dy.at = (const YT*)d.dy + dy_at;
     }
-    if (d.R > 1) column_sums<kThreads, W>(d, entry, [&](int c, float2 t) { column[c] = t; });
+    if (d.R > 1) column_sums<kThreads, W>(d, entry, [&](int c, float2 t, const float2*) { column[c] = t; });
     __syncthreads();
     const int lanes = lanes_for(cg);
     each_group<kThreads>(gs, lanes, [&](int g, int l, bool mine_g) {

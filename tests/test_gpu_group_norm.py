@@ -381,3 +381,23 @@ def test_the_border_of_the_relu_is_the_same_forward_and_backward(size, types):
         dy[r] = 1.0
         F.group_norm_backward(x, dy, torch.empty_like(x), 1, norm)
         assert torch.equal(norm.dbias, (y[r] > 0).float())
+
+
+@pytest.mark.parametrize("types", ["bf16", "fp32"])
+@pytest.mark.parametrize("size", [(64, 119, 2, 2), (64, 119, 8, 8), (64, 64, 64, 64), (20, 100, 21, 7)], ids=str)
+def test_a_first_pixel_far_from_the_others(size, types):
+    """As the corner of an image may be.  A thread has one or two of these pixels, and the first one is what the threads' means are taken
+    from: the squares about it, at most 128 times those about the mean, are rounded four times each (2^-24) before the latter come of them, and
+    these are added, 128 of them at most: 640 roundings in all, half of that of 1/std.  The mean: 160 of differences, at most the outlier's."""
+    from geeps_b200.ops import functional as F
+    images, pixels, c, groups = size
+    for far in (30.0, 1000.0):
+        x, _, _, _ = made(*size, types, 11)
+        first = x.view(images, pixels, c)[:, 0]
+        first.copy_(far * torch.where(first > 0, 1.0, -1.0))
+        stats = torch.empty(images, groups, 2, device=DEV)
+        F.group_norm_forward(x, torch.empty_like(x), images, F.GroupNorm(groups, stats=stats, eps=EPS))
+        want = statistics(x, images, groups)
+        print("largest error of 1/std", (stats[..., 1].double() / want[..., 1] - 1).abs().max().item() * 2 ** 24)
+        assert ((stats[..., 1].double() / want[..., 1] - 1).abs() <= 320 * 2.0 ** -24).all()
+        assert ((stats[..., 0].double() - want[..., 0]).abs() <= 160 * 2.0 ** -24 * far).all()
